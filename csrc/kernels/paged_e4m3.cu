@@ -1,0 +1,182 @@
+// Paged KV cache in e4m3: storing the keys and values of new tokens, and reading whole sequences back.
+//
+// Why a power of two for a tile: an e4m3 number has three bits behind its first whatever its size, so a scale only has to bring the tile's largest
+// number under 448 and keep the small ones out of the subnormals; which of the scales within a factor of two does not matter for the others.  With a
+// power of two the product with a code is exact in every type that has its range, and a tile whose exponent grows under a later token keeps its
+// numbers as they were, but for those that become subnormal.  A scale that is not a power of two would round every code of the page again with every
+// token that raises it.
+#include "pdl.cuh"
+#include "paged_e4m3.cuh"
+
+namespace rb {
+
+constexpr int kE4AppendThreads = 64;                 // a warp for the keys of a tile and one for its values
+
+// A CTA takes the pages that begin, for this call, within `per_cta` rows, for one KV head: those whose first new token is one of these rows.  A page's
+// tokens may lie in the next CTA's rows too.
+template <typename T, int D>
+__global__ void __launch_bounds__(kE4AppendThreads)
+e4_append_kernel(const RbE4m3AppendArgs a, int per_cta RB_BOUNDS_PARAM) {
+  pdl_wait();
+  pdl_launch();
+  const int lane = threadIdx.x & 31, values = threadIdx.x >> 5;        // warp 0: keys, warp 1: values
+  const int G = a.pages.kv_heads, bs = a.pages.block_size, h = blockIdx.y;
+  const T* rows = reinterpret_cast<const T*>(values ? a.v_new : a.k_new);
+  const long long ld = values ? a.ld_v : a.ld_k;
+  uint8_t* codes = reinterpret_cast<uint8_t*>(values ? a.pages.v : a.pages.k);
+  signed char* exps = values ? a.pages.v_exp : a.pages.k_exp;
+  constexpr int LPR = D / 8, RPW = 32 / LPR;                           // lanes for a row, rows for a warp
+  const int r_lane = lane / LPR, c_lane = (lane % LPR) * 8;
+  const long long end_all = a.row_starts ? min(a.row_starts[a.batch], a.rows) : a.rows;
+  const long long stop = min(end_all, (static_cast<long long>(blockIdx.x) + 1) * per_cta);
+  for (long long r = max(static_cast<long long>(blockIdx.x) * per_cta, a.row_starts ? static_cast<long long>(a.row_starts[0]) : 0ll); r < stop;) {
+    const int b = a.row_starts ? e4_sequence_of(a.row_starts, a.batch, static_cast<int>(r)) : static_cast<int>(r);
+    const int first = a.row_starts ? a.row_starts[b] : b, last = a.row_starts ? min(a.row_starts[b + 1], a.rows) : b + 1;
+    const long long pos = static_cast<long long>(a.context_lens[b]) - (a.row_starts ? a.row_starts[b + 1] : b + 1) + r;
+    if (pos < 0) {                                                     // more rows than the sequence has tokens
+      r = min(r - pos, static_cast<long long>(last));
+      continue;
+    }
+    const int off = static_cast<int>(pos % bs);
+    const int n = static_cast<int>(min(static_cast<long long>(bs - off), last - r));
+    const long long r0 = r;
+    r += n;
+    if (off != 0 && r0 != first) continue;                             // the page's first new token is an earlier row
+    const int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, static_cast<int>(pos / bs));
+    if (page < 0) {
+      RB_BOUNDS_HIT(104);
+      continue;
+    }
+    const T* src = rows + r0 * ld + static_cast<long long>(h) * D + c_lane;
+    float most = 0.f;
+    for (int i = r_lane; i < n; i += RPW) {
+      float x[8];
+      E4Row<T>::load(src + i * ld, x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = fmaxf(most, e4_finite_abs(x[j]));
+    }
+    const long long tile = static_cast<long long>(page) * G + h;
+    int e = e4_exponent(warp_max(most));
+    uint8_t* dst = codes + tile * bs * D;
+    if (off > 0) {
+      const int had = exps[tile];
+      if (had >= e) e = had;
+      else
+        for (int i = lane * 16; i < off * D; i += 512) {               // the codes in front of the new ones
+          uint4 u = *reinterpret_cast<const uint4*>(dst + i);
+          u = make_uint4(e4_lower4(u.x, e - had), e4_lower4(u.y, e - had), e4_lower4(u.z, e - had), e4_lower4(u.w, e - had));
+          *reinterpret_cast<uint4*>(dst + i) = u;
+        }
+    }
+    const float down = e4_two(-e);
+    for (int i = r_lane; i < n; i += RPW) {
+      float x[8];
+      E4Row<T>::load(src + i * ld, x);
+      uint2 u;
+      u.x = e4_pack2(x[0] * down, x[1] * down) | e4_pack2(x[2] * down, x[3] * down) << 16;
+      u.y = e4_pack2(x[4] * down, x[5] * down) | e4_pack2(x[6] * down, x[7] * down) << 16;
+      *reinterpret_cast<uint2*>(dst + (off + i) * D + c_lane) = u;
+    }
+    __syncwarp();                                                      // every lane has the old exponent
+    if (lane == 0) exps[tile] = static_cast<signed char>(e);
+    if (!values && a.pages.weight)
+      for (int i = lane; i < n; i += 32) a.pages.weight[tile * bs + off + i] = 0.f;
+  }
+}
+
+constexpr int kE4ReadRows = 16;
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+e4_read_kernel(const RbE4m3ReadArgs a RB_BOUNDS_PARAM) {
+  pdl_wait();
+  pdl_launch();
+  __shared__ long long slot[kE4ReadRows];            // page * block_size + offset, -1: no position
+  const int G = a.pages.kv_heads, bs = a.pages.block_size, D = a.pages.head_dim;
+  const long long r0 = static_cast<long long>(blockIdx.x) * kE4ReadRows;
+  if (threadIdx.x < kE4ReadRows) {
+    const long long r = r0 + threadIdx.x;
+    long long at = -1;
+    if (r < a.rows && r < a.row_starts[a.batch] && r >= a.row_starts[0]) {
+      const int b = e4_sequence_of(a.row_starts, a.batch, static_cast<int>(r));
+      const int i = static_cast<int>(r) - a.row_starts[b];
+      if (i < a.context_lens[b]) {
+        const int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, i / bs);
+        if (page < 0) RB_BOUNDS_HIT(104);
+        else at = static_cast<long long>(page) * bs + i % bs;
+      }
+    }
+    slot[threadIdx.x] = at;
+  }
+  __syncthreads();
+  const int pieces = G * D / 8;                      // of eight numbers
+  for (int i = threadIdx.x; i < 2 * kE4ReadRows * pieces; i += blockDim.x) {
+    const int row = i / (2 * pieces), rest = i - row * 2 * pieces, values = rest >= pieces, c = (rest - values * pieces) * 8;
+    const long long at = slot[row];
+    if (at < 0) continue;
+    const long long page = at / bs, off = at - page * bs;
+    const long long tile = page * G + c / D;
+    const uint8_t* codes = reinterpret_cast<const uint8_t*>(values ? a.pages.v : a.pages.k) + (tile * bs + off) * D + c % D;
+    const float up = e4_two((values ? a.pages.v_exp : a.pages.k_exp)[tile]);
+    const uint2 u = *reinterpret_cast<const uint2*>(codes);
+    float x[8];
+    const uint32_t w[2] = {u.x, u.y};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = e4_float2(w[j >> 1] >> (16 * (j & 1)));
+      x[2 * j] = f.x * up;
+      x[2 * j + 1] = f.y * up;
+    }
+    T* out = reinterpret_cast<T*>(values ? a.v_out : a.k_out) + (r0 + row) * (values ? a.ld_v : a.ld_k) + c;
+    E4Row<T>::store(out, x);
+  }
+}
+
+}  // namespace rb
+
+namespace {
+template <typename T>
+int append_by_dim(const RbE4m3AppendArgs& a, cudaStream_t s) {
+  const int per_cta = a.row_starts ? a.pages.block_size : 1;
+  const dim3 grid((a.rows + per_cta - 1) / per_cta, a.pages.kv_heads);
+  auto kern = a.pages.head_dim == 64 ? rb::e4_append_kernel<T, 64> : rb::e4_append_kernel<T, 128>;
+  return static_cast<int>(rbhost::launch_pdl(kern, grid, dim3(rb::kE4AppendThreads), 0, s, 1, a, per_cta RB_BOUNDS_ARG));
+}
+template <typename A>
+bool rows_fit(const A& a, const void* k, const void* v) {
+  const int per16 = a.type == RB_E4M3_F32 ? 4 : 8;
+  return !((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) && a.ld_k % per16 == 0 && a.ld_v % per16 == 0;
+}
+}  // namespace
+
+RB_API int rb_e4m3_append(const RbE4m3AppendArgs* args, void* stream_v) {
+  const RbE4m3AppendArgs& a = *args;
+  if (a.rows <= 0 || a.batch <= 0) return 0;
+  if (const int bad = rbhost::e4_check(a.pages)) return bad;
+  if (!a.k_new || !a.v_new || !a.block_tables || !a.context_lens || a.max_blocks <= 0 || a.pages.kv_heads > 65535 || (!a.row_starts && a.rows != a.batch))
+    return -1;
+  if (!rows_fit(a, a.k_new, a.v_new)) return -2;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_v);
+  switch (a.type) {
+    case RB_E4M3_BF16: return append_by_dim<__nv_bfloat16>(a, s);
+    case RB_E4M3_F16: return append_by_dim<__half>(a, s);
+    case RB_E4M3_F32: return append_by_dim<float>(a, s);
+  }
+  return -1;
+}
+
+RB_API int rb_e4m3_read(const RbE4m3ReadArgs* args, void* stream_v) {
+  const RbE4m3ReadArgs& a = *args;
+  if (a.rows <= 0 || a.batch <= 0) return 0;
+  if (const int bad = rbhost::e4_check(a.pages)) return bad;
+  if (!a.k_out || !a.v_out || !a.block_tables || !a.context_lens || !a.row_starts || a.max_blocks <= 0) return -1;
+  if (!rows_fit(a, a.k_out, a.v_out)) return -2;
+  const dim3 grid((a.rows + rb::kE4ReadRows - 1) / rb::kE4ReadRows);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_v);
+  switch (a.type) {
+    case RB_E4M3_BF16: return static_cast<int>(rbhost::launch_pdl(rb::e4_read_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, 1, a RB_BOUNDS_ARG));
+    case RB_E4M3_F16: return static_cast<int>(rbhost::launch_pdl(rb::e4_read_kernel<__half>, grid, dim3(256), 0, s, 1, a RB_BOUNDS_ARG));
+    case RB_E4M3_F32: return static_cast<int>(rbhost::launch_pdl(rb::e4_read_kernel<float>, grid, dim3(256), 0, s, 1, a RB_BOUNDS_ARG));
+  }
+  return -1;
+}

@@ -15,6 +15,7 @@ from .embed import embedding, embedding_forward, embedding_backward, embedding_r
 from .elementwise import (binary, unary, scalar_op, unary_bwd, add_row_vector, sum_dim0, sum_all, transpose2d,
                           gather_rows, scatter_rows, broadcast_to, strided_copy, apply_mask, dropout, argmax_rows,
                           gelu, relu, silu, scale_softcap_)
+from .paged_e4m3 import PagesE4M3, kv_append_e4m3, kv_evict_e4m3, kv_read_e4m3, paged_attention_decode_e4m3
 from .rotary import rope, rope_, rotary_table, rotate_halves, rotate_pairs_, swiglu, swiglu_forward, swiglu_backward
 from .optim import adam_step, sgd_step, sumsq, cast_f32_to_bf16
 
