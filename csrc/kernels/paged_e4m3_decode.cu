@@ -11,7 +11,6 @@
 namespace rb {
 
 constexpr int kE4Slice = 256;                        // tokens whose sums one CTA forms; the merge goes over them in order
-constexpr int kE4Heads = 8;                          // query heads at a time
 
 __device__ __forceinline__ float e4_ex2(float x) {
   float y;
@@ -34,94 +33,384 @@ __device__ __forceinline__ float* e4_norm(float* scratch, int batch, int heads, 
   return scratch + rows * slices * (D + 2 + kE4Slice) + (static_cast<long long>(b) * heads + h) * 2;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(128)
-e4_decode_kernel(const RbE4m3DecodeArgs a, int slices RB_BOUNDS_PARAM) {
+// The tokens of a sequence that its tables have room for.
+__device__ __forceinline__ int e4_len(const RbE4m3DecodeArgs& a, int b) {
+  const long long room = static_cast<long long>(a.max_blocks) * a.pages.block_size;
+  return static_cast<int>(max(0ll, min(static_cast<long long>(a.context_lens[b]), room)));
+}
+__device__ __forceinline__ uint4 e4_lds128(uint32_t addr) {
+  uint4 u;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(addr));
+  return u;
+}
+__device__ __forceinline__ uint2 e4_lds64(uint32_t addr) {
+  uint2 u;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(u.x), "=r"(u.y) : "r"(addr));
+  return u;
+}
+__device__ __forceinline__ void e4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t e4_half2_of(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A slice that a CTA works on, and how many follow in its run.
+struct E4Place {
+  int b, hk, s, left;
+};
+
+constexpr int kE4Warps = 4, kE4Stages = 4;           // a warp has the four tiles of a slice that are its own in flight
+
+template <int D, int NH>
+struct E4Layout {
+  static constexpr int kTile = 16 * D;                                   // bytes of a tile's keys; its values follow
+  static constexpr int kRing = kE4Warps * kE4Stages * 2 * kTile;
+  static constexpr int kMerge = kE4Warps * NH * 8 * D * 4;               // the warps' sums
+  static constexpr int kBytes = kRing + kMerge + 1024;
+};
+
+// Warp w of a CTA takes tiles w, w + 4, w + 8, w + 12 of 16 tokens of a slice; its sums and those of the other warps are added in the order of the
+// warps, and a sequence's slices in order by the merge, so that a sequence has the same bits alone and beside others.
+//
+// S = Q K^T has the heads as the 16 rows of m16n8k16 (NH: 8 or 16 of them there), O^T = V^T P^T the head dimensions as rows and the heads as the 8
+// columns: the accumulators of S then are, rounded to f16, the second operand of the other product as they lie.  Codes become f16 exactly.  The
+// contraction over head dimensions may take them in any order, so a lane reads 16 codes of a row at a time and these are its operands of four
+// products; a swizzled tile gives every lane its 16 bytes without bank conflicts.  A query row is scaled to [1, 2) by a power of two first.
+// LIST: the slices of all sequences and KV heads, numbered one sequence after the other, are dealt in equal runs to CTAs that stay, and the next slice's
+// tiles are copied while this one's are worked on.  Otherwise the grid is (slices, KV heads, sequences).
+template <typename T, int D, int NH, bool LIST>
+__global__ void __launch_bounds__(kE4Warps * 32)
+e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const RbE4m3DecodeArgs a, int h0, int slices,
+                 unsigned int* status RB_BOUNDS_PARAM) {
   pdl_wait();
   pdl_launch();
-  __shared__ float q_sh[kE4Heads][D];
-  __shared__ float s_sh[kE4Heads][kE4Slice];
-  __shared__ long long tile_sh[kE4Slice / 16];
-  __shared__ float red[4];
-  const int s = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  using L = E4Layout<D, NH>;
+  constexpr int KS = D / 16;                         // products of 16 in a score
+  constexpr int MT = D / 16;                         // tiles of 16 output dimensions
+  constexpr int BR = D / 8;                          // rows of 128 bytes in a tile
+  extern __shared__ uint8_t e4_raw[];
+  __shared__ __align__(8) uint64_t bars[kE4Warps][kE4Stages];
+  __shared__ float m_sh[kE4Warps][NH * 8], l_sh[kE4Warps][NH * 8];
+  __shared__ int abort_sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
+  const uint32_t base = (smem_u32(e4_raw) + 1023u) & ~1023u;             // the swizzle goes by addresses
+  const uint32_t ring = base + warp * (kE4Stages * 2 * L::kTile);
+  float* merge = reinterpret_cast<float*>(e4_raw + (base - smem_u32(e4_raw)) + L::kRing);
   const int bs = a.pages.block_size, G = a.pages.kv_heads, group = a.heads / G;
-  const int n = min(static_cast<long long>(a.context_lens[b]), static_cast<long long>(a.max_blocks) * bs) - static_cast<long long>(s) * kE4Slice;
-  if (n <= 0) return;
-  const int here = min(n, kE4Slice);
-  if (tid < kE4Slice / 16) {
-    const int t = s * kE4Slice + tid * 16;
-    int page = tid * 16 < here ? e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, t / bs) : 0;
+  const int heads = min(NH * 8, group - h0);
+
+  // ---- this CTA's run of slices
+  E4Place at = {0, 0, 0, 1};
+  if (!LIST) {
+    at.b = blockIdx.z;
+    at.hk = blockIdx.y;
+    at.s = blockIdx.x;
+    if (at.s * kE4Slice >= e4_len(a, at.b)) return;
+  } else {
+    int n = lane < a.batch ? (e4_len(a, lane) + kE4Slice - 1) / kE4Slice : 0, total = n;
+    for (int i = lane + 32; i < a.batch; i += 32) total += (e4_len(a, i) + kE4Slice - 1) / kE4Slice;
+    total = __reduce_add_sync(0xffffffffu, total);
+    const long long all = static_cast<long long>(total) * G;
+    const long long first = all * blockIdx.x / gridDim.x, end = all * (blockIdx.x + 1) / gridDim.x;
+    if (end == first) return;
+    at.left = static_cast<int>(end - first);
+    long long skip = first;
+    for (int b0 = 0;;) {
+      long long upto = static_cast<long long>(n) * G;
+      const long long own = upto;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const unsigned int behind = __ballot_sync(0xffffffffu, upto > skip);
+      if (behind != 0u) {
+        const int which = __ffs(behind) - 1;
+        at.b = b0 + which;
+        const int in = static_cast<int>(skip - __shfl_sync(0xffffffffu, upto - own, which)), ns = __shfl_sync(0xffffffffu, n, which);
+        at.hk = in / ns;
+        at.s = in - at.hk * ns;
+        break;
+      }
+      skip -= __shfl_sync(0xffffffffu, upto, 31);
+      b0 += 32;
+      n = b0 + lane < a.batch ? (e4_len(a, b0 + lane) + kE4Slice - 1) / kE4Slice : 0;
+    }
+  }
+
+  if (threadIdx.x == 0) abort_sh = 0;
+  if (lane == 0)
+    for (int i = 0; i < kE4Stages; ++i) mbar_init(smem_u32(&bars[warp][i]), 1);
+  fence_mbar_init();
+  __syncthreads();
+
+  // the tile (of 16 tokens, over both arrays) of this warp's tile `lane & 3` of a slice, -1 where the slice ends before it
+  auto locate = [&](const E4Place& p, int n) {
+    const int t = p.s * kE4Slice + ((lane & 3) * kE4Warps + warp) * 16;
+    if (t >= n) return -1ll;
+    int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, p.b, t / bs);
     if (page < 0) {                                  // corrupt tables read block 0 instead of faulting
       RB_BOUNDS_HIT(104);
       page = 0;
     }
-    tile_sh[tid] = (static_cast<long long>(page) * G + hk) * bs + t % bs;          // token in the cache
+    return (static_cast<long long>(page) * G + p.hk) * (bs / 16) + t % bs / 16;
+  };
+  auto request = [&](int stage, long long tile) {    // lane 0
+    const uint32_t bar = smem_u32(&bars[warp][stage]), dst = ring + stage * 2 * L::kTile;
+    mbar_arrive_expect_tx(bar, 2 * L::kTile);
+    tma_load_2d(dst, &k_map, 0, static_cast<int>(tile) * BR, bar);
+    tma_load_2d(dst + L::kTile, &v_map, 0, static_cast<int>(tile) * BR, bar);
+  };
+  auto advance = [&](E4Place& p, int& n) {           // the next slice of the run
+    if (--p.left <= 0) {
+      n = 0;
+      return;
+    }
+    if (++p.s * kE4Slice < n) return;
+    p.s = 0;
+    if (++p.hk < G) return;
+    p.hk = 0;
+    do n = e4_len(a, ++p.b);
+    while (n == 0);
+  };
+
+  int n_at = e4_len(a, at.b);
+  long long tile_at = locate(at, n_at);
+#pragma unroll
+  for (int i = 0; i < kE4Stages; ++i) {
+    const long long t = __shfl_sync(0xffffffffu, tile_at, i);
+    if (lane == 0 && t >= 0) request(i, t);
   }
-  __syncthreads();
-  const uint8_t* K = reinterpret_cast<const uint8_t*>(a.pages.k);
-  const uint8_t* V = reinterpret_cast<const uint8_t*>(a.pages.v);
-  const float scale = a.scale * 1.4426950408889634f;
-  for (int h0 = 0; h0 < group; h0 += kE4Heads) {
-    const int heads = min(kE4Heads, group - h0), head = hk * group + h0;
-    for (int i = tid; i < heads * D; i += 128)
-      q_sh[i / D][i % D] = e4_get(reinterpret_cast<const T*>(a.q) + b * a.ld_q + static_cast<long long>(head) * D + i);
-    __syncthreads();
-    for (int t = tid; t < here; t += 128) {
-      const long long at = tile_sh[t >> 4] + (t & 15);
-      float acc[kE4Heads];
+  int exps = 0;                                      // lanes 0 .. 3: exponents of the four tiles' keys, 4 .. 7 of their values
+  auto exps_of = [&](long long tile) { return tile < 0 || lane >= 8 ? 0 : static_cast<int>((lane < 4 ? a.pages.k_exp : a.pages.v_exp)[tile / (bs / 16)]); };
+  exps = exps_of(tile_at);
+  E4Place next = at;
+  int n_next = n_at;
+  long long tile_next = -1;
+  if (LIST) {
+    advance(next, n_next);
+    tile_next = locate(next, n_next);
+  }
+
+  uint32_t qf[KS][NH * 2];
+  float q_up[NH];
+  bool fresh = true;
+  uint32_t parity = 0;
+  for (;;) {
+    if (fresh) {                                     // ---- query rows gq and gq + 8 of the group's heads, this lane's dimensions of them
 #pragma unroll
-      for (int h = 0; h < kE4Heads; ++h) acc[h] = 0.f;
-      for (int c = 0; c < D; c += 4) {
-        const uint32_t u = *reinterpret_cast<const uint32_t*>(K + at * D + c);
-        const float2 x = e4_float2(u), y = e4_float2(u >> 16);
+      for (int r = 0; r < NH; ++r) {
+        const bool there = r * 8 + gq < heads;
+        const T* src = reinterpret_cast<const T*>(a.q) + at.b * a.ld_q + (static_cast<long long>(at.hk) * group + h0 + r * 8 + gq) * D + tq * (D / 4);
+        float x[D / 4], most = 0.f;
 #pragma unroll
-        for (int h = 0; h < kE4Heads; ++h)
-          acc[h] += q_sh[h][c] * x.x + q_sh[h][c + 1] * x.y + q_sh[h][c + 2] * y.x + q_sh[h][c + 3] * y.y;
-      }
-      const float up = e4_two(a.pages.k_exp[at / bs]) * scale;
-#pragma unroll
-      for (int h = 0; h < kE4Heads; ++h) s_sh[h][t] = acc[h] * up;
-    }
-    __syncthreads();
-    for (int h = 0; h < heads; ++h) {
-      float m = -INFINITY;
-      for (int t = tid; t < here; t += 128) m = fmaxf(m, ceilf(s_sh[h][t]) + a.pages.v_exp[(tile_sh[t >> 4]) / bs]);
-      m = warp_max(m);
-      if ((tid & 31) == 0) red[tid >> 5] = m;
-      __syncthreads();
-      m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-      __syncthreads();
-      if (a.accumulate) {
-        float* scores = a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (D + 2) +
-                        (static_cast<long long>(b) * a.heads + head + h) * slices * kE4Slice + s * kE4Slice;
-        for (int t = tid; t < here; t += 128) scores[t] = s_sh[h][t];
-      }
-      float l = 0.f;
-      for (int t = tid; t < here; t += 128) {
-        const int e = a.pages.v_exp[(tile_sh[t >> 4]) / bs];
-        const float p = e4_ex2(s_sh[h][t] - (m - e));
-        l = fmaf(p, e4_two(-e), l);
-        s_sh[h][t] = p;
-      }
-      l = warp_sum(l);
-      if ((tid & 31) == 0) red[tid >> 5] = l;
-      __syncthreads();
-      float* out = e4_partial(a.scratch, a.heads, slices, D, b, head + h, s);
-      if (tid == 0) {
-        out[0] = m;
-        out[1] = (red[0] + red[1]) + (red[2] + red[3]);
-      }
-      if (tid < D) {
-        float o = 0.f;
-        for (int t = 0; t < here; ++t) {
-          const uint8_t* v = V + (tile_sh[t >> 4] + (t & 15)) * D + (tid & ~1);
-          const float2 x = e4_float2(*reinterpret_cast<const uint16_t*>(v));
-          o = fmaf(s_sh[h][t], tid & 1 ? x.y : x.x, o);
+        for (int i = 0; i < D / 4; ++i) {
+          x[i] = there ? e4_get(src + i) : 0.f;
+          most = fmaxf(most, fabsf(x[i]));
         }
-        out[2 + tid] = o;
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -126), 126);
+        const float down = e4_two(-e);
+        q_up[r] = e4_two(e) * a.scale * 1.4426950408889634f;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          qf[j][2 * r] = e4_half2_of(x[4 * j] * down, x[4 * j + 1] * down);
+          qf[j][2 * r + 1] = e4_half2_of(x[4 * j + 2] * down, x[4 * j + 3] * down);
+        }
       }
-      __syncthreads();
     }
+    float m[NH], l[NH], o[MT][NH][4];
+#pragma unroll
+    for (int r = 0; r < NH; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) o[i][r][0] = o[i][r][1] = o[i][r][2] = o[i][r][3] = 0.f;
+    }
+#pragma unroll 1
+    for (int i = 0; i < kE4Stages; ++i) {
+      const int n_tok = n_at - (at.s * kE4Slice + (i * kE4Warps + warp) * 16);         // tokens of the tile and behind it
+      const long long coming = __shfl_sync(0xffffffffu, tile_next, i);
+      if (n_tok > 0) {
+        mbar_wait(smem_u32(&bars[warp][i]), (parity >> i) & 1, &abort_sh, status, 130);
+        parity ^= 1u << i;
+        const uint32_t kt = ring + i * 2 * L::kTile, vt = kt + L::kTile;
+        uint32_t kw[2][D / 16];                      // codes of tokens gq and gq + 8, dimensions tq * D / 4 ..
+        uint32_t vw[4][D / 32];                      // codes of tokens 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9, dimensions gq * D / 8 ..
+        if (D == 128) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              const uint4 u = e4_lds128(kt + (t * 8 + gq) * 128 + (((tq * 2 + p) ^ gq) << 4));
+              kw[t][p * 4] = u.x; kw[t][p * 4 + 1] = u.y; kw[t][p * 4 + 2] = u.z; kw[t][p * 4 + 3] = u.w;
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const int row = tq * 2 + (t & 1) + (t >> 1) * 8;
+            const uint4 u = e4_lds128(vt + row * 128 + ((gq ^ (row & 7)) << 4));
+            vw[t][0] = u.x; vw[t][1] = u.y; vw[t][D / 32 - 2] = u.z; vw[t][D / 32 - 1] = u.w;
+          }
+        } else {                                     // two tokens in a row of 128 bytes
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int tok = t * 8 + gq, row = tok >> 1;
+            const uint4 u = e4_lds128(kt + row * 128 + ((((tok & 1) * 4 + tq) ^ row) << 4));
+            kw[t][0] = u.x; kw[t][1] = u.y; kw[t][2] = u.z; kw[t][3] = u.w;
+          }
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const int tok = tq * 2 + (t & 1) + (t >> 1) * 8, row = tok >> 1;
+            const uint2 u = e4_lds64(vt + row * 128 + ((((tok & 1) * 4 + (gq >> 1)) ^ row) << 4) + (gq & 1) * 8);
+            vw[t][0] = u.x; vw[t][1] = u.y;
+          }
+        }
+        __syncwarp();                                // the stage is free
+        if (lane == 0 && coming >= 0 && !abort_sh) request(i, coming);
+        // ---- scores of tokens 2 tq, 2 tq + 1 (c 0) and + 8 (c 1) under heads gq and gq + 8
+        float s[2][4];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          s[c][0] = s[c][1] = s[c][2] = s[c][3] = 0.f;
+#pragma unroll
+          for (int j = 0; j < KS; ++j)
+            e4_mma(s[c], qf[j][0], NH > 1 ? qf[j][NH * 2 - 2] : 0u, qf[j][1], NH > 1 ? qf[j][NH * 2 - 1] : 0u, e4_half2(kw[c][j]), e4_half2(kw[c][j] >> 16));
+        }
+        const int ev = __shfl_sync(0xffffffffu, exps, 4 + i);
+        const float up = e4_two(__shfl_sync(0xffffffffu, exps, i)), ev_down = e4_two(-ev);
+        uint32_t pf[NH][2];
+        float grow[NH];
+        bool moved = false;
+#pragma unroll
+        for (int r = 0; r < NH; ++r) {
+          const float f = up * q_up[r];
+          float most = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float x = s[c][2 * r + j] * f;
+              s[c][2 * r + j] = c * 8 + tq * 2 + j < n_tok ? x : -INFINITY;
+              most = fmaxf(most, s[c][2 * r + j]);
+            }
+          }
+          if (a.accumulate && r * 8 + gq < heads) {
+            float* scores = a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (D + 2) +
+                            (static_cast<long long>(at.b) * a.heads + at.hk * group + h0 + r * 8 + gq) * slices * kE4Slice + at.s * kE4Slice +
+                            (i * kE4Warps + warp) * 16 + tq * 2;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              scores[c * 8] = s[c][2 * r];
+              scores[c * 8 + 1] = s[c][2 * r + 1];
+            }
+          }
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+          const float to = fmaxf(m[r], ceilf(most) + static_cast<float>(ev));
+          grow[r] = to == m[r] ? 1.f : e4_ex2(m[r] - to);
+          moved |= to != m[r];
+          m[r] = to;
+          float sum = 0.f;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float p0 = e4_ex2(s[c][2 * r] - (to - static_cast<float>(ev))), p1 = e4_ex2(s[c][2 * r + 1] - (to - static_cast<float>(ev)));
+            sum += p0 + p1;
+            pf[r][c] = e4_half2_of(p0, p1);
+          }
+          l[r] = fmaf(sum, ev_down, l[r] * grow[r]);
+        }
+        if (__any_sync(0xffffffffu, moved)) {        // sums of heads 2 tq and 2 tq + 1
+#pragma unroll
+          for (int r = 0; r < NH; ++r) {
+            const float g0 = __shfl_sync(0xffffffffu, grow[r], tq * 8), g1 = __shfl_sync(0xffffffffu, grow[r], tq * 8 + 4);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+              o[t][r][0] *= g0; o[t][r][1] *= g1; o[t][r][2] *= g0; o[t][r][3] *= g1;
+            }
+          }
+        }
+        if (n_tok < 16) {                            // what lies behind the last token may be anything, NaN too
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (tq * 2 + (t & 1) + (t >> 1) * 8 >= n_tok) {
+#pragma unroll
+              for (int w = 0; w < D / 32; ++w) vw[t][w] = 0u;
+            }
+        }
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) {
+          const uint32_t lo0 = __byte_perm(vw[0][w], vw[1][w], 0x5140), lo1 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
+          const uint32_t hi0 = __byte_perm(vw[2][w], vw[3][w], 0x5140), hi1 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
+          const uint32_t a00 = e4_half2(lo0), a01 = e4_half2(lo0 >> 16), a02 = e4_half2(hi0), a03 = e4_half2(hi0 >> 16);
+          const uint32_t a10 = e4_half2(lo1), a11 = e4_half2(lo1 >> 16), a12 = e4_half2(hi1), a13 = e4_half2(hi1 >> 16);
+#pragma unroll
+          for (int r = 0; r < NH; ++r) {
+            e4_mma(o[2 * w][r], a00, a01, a02, a03, pf[r][0], pf[r][1]);
+            e4_mma(o[2 * w + 1][r], a10, a11, a12, a13, pf[r][0], pf[r][1]);
+          }
+        }
+      } else if (lane == 0 && coming >= 0 && !abort_sh) {
+        request(i, coming);
+      }
+    }
+    // ---- the slice's sums: all warps' together
+#pragma unroll
+    for (int r = 0; r < NH; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if (tq == 0) {
+        m_sh[warp][r * 8 + gq] = m[r];
+        l_sh[warp][r * 8 + gq] = l[r];
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {                  // head 2 tq + c, dimensions gq * D / 8 .., 16 bytes at a time, swizzled by the head
+        const int head = r * 8 + tq * 2 + c;
+        float* row = merge + (warp * NH * 8 + head) * D;
+#pragma unroll
+        for (int t = 0; t < MT; t += 2)
+          *reinterpret_cast<float4*>(row + (((gq * (D / 32) + t / 2) ^ tq) << 2)) = make_float4(o[t][r][c], o[t][r][2 + c], o[t + 1][r][c], o[t + 1][r][2 + c]);
+      }
+    }
+    __syncthreads();
+    const bool whole = n_at <= kE4Slice;             // the sequence has no other slice
+    for (int i = threadIdx.x; i < heads * D; i += kE4Warps * 32) {
+      const int head = i / D, d = i - head * D;
+      float top = m_sh[0][head];
+#pragma unroll
+      for (int w = 1; w < kE4Warps; ++w) top = fmaxf(top, m_sh[w][head]);
+      float sum = 0.f, den = 0.f;
+#pragma unroll
+      for (int w = 0; w < kE4Warps; ++w) {
+        const float mw = m_sh[w][head], f = mw == -INFINITY ? 0.f : e4_ex2(mw - top);
+        sum = fmaf(merge[(w * NH * 8 + head) * D + (((d >> 2) ^ (head >> 1 & 3)) << 2) + (d & 3)], f, sum);
+        den = fmaf(l_sh[w][head], f, den);
+      }
+      const int h = at.hk * group + h0 + head;
+      if (whole) e4_put(reinterpret_cast<T*>(a.out) + at.b * a.ld_o + static_cast<long long>(h) * D + d, sum / den);
+      if (!whole || a.accumulate) {
+        float* out = e4_partial(a.scratch, a.heads, slices, D, at.b, h, at.s);
+        if (d == 0) {
+          out[0] = top;
+          out[1] = den;
+        }
+        out[2 + d] = sum;
+      }
+    }
+    if (!LIST || at.left <= 1) break;
+    __syncthreads();
+    fresh = next.b != at.b || next.hk != at.hk;
+    at = next;
+    n_at = n_next;
+    exps = exps_of(tile_next);
+    advance(next, n_next);
+    tile_next = locate(next, n_next);
   }
 }
 
@@ -130,20 +419,43 @@ __global__ void __launch_bounds__(128)
 e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
   pdl_wait();
   pdl_launch();
+  __shared__ float f_sh[128], l_sh[128], red[4];
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, D = a.pages.head_dim;
-  const long long len = min(static_cast<long long>(a.context_lens[b]), static_cast<long long>(a.max_blocks) * a.pages.block_size);
-  const int here = len <= 0 ? 0 : static_cast<int>((len + kE4Slice - 1) / kE4Slice);
-  float m = -INFINITY;
-  for (int s = 0; s < here; ++s) m = fmaxf(m, e4_partial(a.scratch, a.heads, slices, D, b, h, s)[0]);
-  float l = 0.f, o = 0.f;
-  for (int s = 0; s < here; ++s) {
-    const float* p = e4_partial(a.scratch, a.heads, slices, D, b, h, s);
-    const float f = e4_ex2(p[0] - m);
-    l = fmaf(p[1], f, l);
-    if (tid < D) o = fmaf(p[2 + tid], f, o);
+  T* out = reinterpret_cast<T*>(a.out) + b * a.ld_o + static_cast<long long>(h) * D;
+  const int here = (e4_len(a, b) + kE4Slice - 1) / kE4Slice;
+  if (here == 0) {
+    if (tid < D) e4_put(out + tid, 0.f);
+    return;
   }
-  if (tid < D) e4_put(reinterpret_cast<T*>(a.out) + b * a.ld_o + static_cast<long long>(h) * D + tid, here ? o / l : 0.f);
-  if (a.accumulate && tid == 0 && here) {
+  if (here == 1 && !a.accumulate) return;            // already written
+  const float* first = e4_partial(a.scratch, a.heads, slices, D, b, h, 0);
+  float m = -INFINITY;
+  for (int s = tid; s < here; s += 128) m = fmaxf(m, first[static_cast<long long>(s) * (D + 2)]);
+  m = warp_max(m);
+  if ((tid & 31) == 0) red[tid >> 5] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float l = 0.f, o = 0.f;
+  for (int s0 = 0; s0 < here; s0 += 128) {
+    const int n = min(128, here - s0);
+    __syncthreads();
+    if (tid < n) {
+      const float* p = first + static_cast<long long>(s0 + tid) * (D + 2);
+      f_sh[tid] = e4_ex2(p[0] - m);
+      l_sh[tid] = p[1];
+    }
+    __syncthreads();
+    const float* p = first + static_cast<long long>(s0) * (D + 2) + 2 + tid;
+    if (tid < D) {
+#pragma unroll 8
+      for (int s = 0; s < n; ++s) {
+        o = fmaf(p[static_cast<long long>(s) * (D + 2)], f_sh[s], o);
+        l = fmaf(l_sh[s], f_sh[s], l);
+      }
+    }
+  }
+  if (here > 1 && tid < D) e4_put(out + tid, o / l);
+  if (a.accumulate && tid == 0) {
     // a weight is 2^(s - m) / l = 2^(s - (m + x)) / (l / 2^x), with the x that brings l / 2^x into [1, 2)
     const int x = static_cast<int>(__float_as_uint(l) >> 23) - 127;
     float* norm = e4_norm(a.scratch, a.batch, a.heads, slices, D, b, h);
@@ -158,8 +470,8 @@ e4_weight_kernel(const RbE4m3DecodeArgs a, int slices) {
   pdl_launch();
   const int s = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, D = a.pages.head_dim;
   const int bs = a.pages.block_size, G = a.pages.kv_heads, group = a.heads / G;
-  const long long t = static_cast<long long>(s) * kE4Slice + threadIdx.x;
-  if (t >= min(static_cast<long long>(a.context_lens[b]), static_cast<long long>(a.max_blocks) * bs)) return;
+  const int t = s * kE4Slice + threadIdx.x;
+  if (t >= e4_len(a, b)) return;
   const float* scores = a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (D + 2);
   float w = 0.f;
   for (int h = 0; h < group; ++h) {
@@ -167,7 +479,7 @@ e4_weight_kernel(const RbE4m3DecodeArgs a, int slices) {
     const float* norm = e4_norm(a.scratch, a.batch, a.heads, slices, D, b, hk * group + h);
     w = fmaf(e4_ex2(scores[row * slices * kE4Slice + t] - norm[0]), norm[1], w);
   }
-  const int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, static_cast<int>(t / bs));
+  const int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, t / bs);
   if (page >= 0) a.pages.weight[(static_cast<long long>(page) * G + hk) * bs + t % bs] += w;
 }
 
@@ -177,15 +489,47 @@ namespace {
 long long e4_slices(int max_blocks, int block_size) {
   return (static_cast<long long>(max_blocks) * block_size + rb::kE4Slice - 1) / rb::kE4Slice;
 }
+template <typename T, int D, int NH>
+int decode_launch(const RbE4m3DecodeArgs& a, cudaStream_t stream) {
+  using L = rb::E4Layout<D, NH>;
+  const RbPagesE4m3& p = a.pages;
+  const int slices = static_cast<int>(e4_slices(a.max_blocks, p.block_size));
+  const uint64_t rows = static_cast<uint64_t>(p.num_blocks) * p.kv_heads * p.block_size * D / 128;
+  if (rows > 0x7fffffffull) return -1;               // a copy's row is a 32-bit number
+  int err = 0;
+  const CUtensorMap* km = rbhost::get_tmap_2d(p.k, 1, 128, rows, 128, 128, D / 8, 1, &err);
+  const CUtensorMap* vm = km ? rbhost::get_tmap_2d(p.v, 1, 128, rows, 128, 128, D / 8, 1, &err) : nullptr;
+  unsigned int* status = rbhost::status_ptr();
+  if (!vm || !status) return err ? err : -3;
+  static int per_sm[2][64] = {};                     // CTAs of a list that fit on an SM
+  const int dev = rbhost::device_slot();
+  for (int list = 0; list < 2; ++list)
+    if (!per_sm[list][dev]) {
+      auto kern = list ? rb::e4_decode_kernel<T, D, NH, true> : rb::e4_decode_kernel<T, D, NH, false>;
+      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+      int n = 0;
+      if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, rb::kE4Warps * 32, L::kBytes);
+      if (e != cudaSuccess) return static_cast<int>(e);
+      per_sm[list][dev] = n > 0 ? n : 1;
+    }
+  const int some = per_sm[1][dev] * rbhost::device_sm_count();
+  const bool list = static_cast<long long>(a.batch) * p.kv_heads * slices > some;
+  auto kern = list ? rb::e4_decode_kernel<T, D, NH, true> : rb::e4_decode_kernel<T, D, NH, false>;
+  const dim3 grid = list ? dim3(some) : dim3(slices, p.kv_heads, a.batch);
+  const int group = a.heads / p.kv_heads;
+  cudaError_t e = cudaSuccess;
+  for (int h0 = 0; h0 < group && e == cudaSuccess; h0 += NH * 8)        // wider groups take several passes
+    e = rbhost::launch_pdl(kern, grid, dim3(rb::kE4Warps * 32), L::kBytes, stream, 1, *km, *vm, a, h0, slices, status RB_BOUNDS_ARG);
+  if (e == cudaSuccess) e = rbhost::launch_pdl(rb::e4_merge_kernel<T>, dim3(a.heads, a.batch), dim3(128), 0, stream, 1, a, slices);
+  if (e == cudaSuccess && a.accumulate)
+    e = rbhost::launch_pdl(rb::e4_weight_kernel, dim3(slices, p.kv_heads, a.batch), dim3(256), 0, stream, 1, a, slices);
+  return static_cast<int>(e);
+}
 template <typename T>
 int decode_by_dim(const RbE4m3DecodeArgs& a, cudaStream_t s) {
-  const int slices = static_cast<int>(e4_slices(a.max_blocks, a.pages.block_size));
-  auto kern = a.pages.head_dim == 64 ? rb::e4_decode_kernel<T, 64> : rb::e4_decode_kernel<T, 128>;
-  const dim3 grid(slices, a.pages.kv_heads, a.batch);
-  cudaError_t e = rbhost::launch_pdl(kern, grid, dim3(128), 0, s, 1, a, slices RB_BOUNDS_ARG);
-  if (e == cudaSuccess) e = rbhost::launch_pdl(rb::e4_merge_kernel<T>, dim3(a.heads, a.batch), dim3(128), 0, s, 1, a, slices);
-  if (e == cudaSuccess && a.accumulate) e = rbhost::launch_pdl(rb::e4_weight_kernel, grid, dim3(256), 0, s, 1, a, slices);
-  return static_cast<int>(e);
+  const bool narrow = a.heads / a.pages.kv_heads <= 8;
+  if (a.pages.head_dim == 64) return narrow ? decode_launch<T, 64, 1>(a, s) : decode_launch<T, 64, 2>(a, s);
+  return narrow ? decode_launch<T, 128, 1>(a, s) : decode_launch<T, 128, 2>(a, s);
 }
 }  // namespace
 
