@@ -22,15 +22,15 @@ __device__ __forceinline__ float e4_get(const __half* p) { return __half2float(*
 __device__ __forceinline__ void e4_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
 __device__ __forceinline__ void e4_put(__half* p, float v) { *p = __float2half(v); }
 
-// Scratch: [batch, heads, slices, D + 2] fp32: maximum, denominator, sums of a slice; then, where weights are summed, the scores
+// Scratch: [batch, heads, slices, D + 4] fp32: maximum, denominator, two unused, sums of a slice; then, where weights are summed, the scores
 // [batch, heads, slices * 256] and the denominators as whole powers of two and factors [batch, heads, 2].
 __device__ __forceinline__ float* e4_partial(float* scratch, int heads, int slices, int D, int b, int h, int s) {
-  return scratch + ((static_cast<long long>(b) * heads + h) * slices + s) * (D + 2);
+  return scratch + ((static_cast<long long>(b) * heads + h) * slices + s) * (D + 4);
 }
 
 __device__ __forceinline__ float* e4_norm(float* scratch, int batch, int heads, int slices, int D, int b, int h) {
   const long long rows = static_cast<long long>(batch) * heads;
-  return scratch + rows * slices * (D + 2 + kE4Slice) + (static_cast<long long>(b) * heads + h) * 2;
+  return scratch + rows * slices * (D + 4 + kE4Slice) + (static_cast<long long>(b) * heads + h) * 2;
 }
 
 // The tokens of a sequence that its tables have room for.
@@ -69,8 +69,7 @@ template <int D, int NH>
 struct E4Layout {
   static constexpr int kTile = 16 * D;                                   // bytes of a tile's keys; its values follow
   static constexpr int kRing = kE4Warps * kE4Stages * 2 * kTile;
-  static constexpr int kMerge = kE4Warps * NH * 8 * D * 4;               // the warps' sums
-  static constexpr int kBytes = kRing + kMerge + 1024;
+  static int bytes(int heads) { return kRing + kE4Warps * heads * D * 4 + 1024; }      // the warps' sums behind the ring
 };
 
 // Warp w of a CTA takes tiles w, w + 4, w + 8, w + 12 of 16 tokens of a slice; its sums and those of the other warps are added in the order of the
@@ -148,22 +147,27 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
   fence_mbar_init();
   __syncthreads();
 
-  // the tile (of 16 tokens, over both arrays) of this warp's tile `lane & 3` of a slice, -1 where the slice ends before it
-  auto locate = [&](const E4Place& p, int n) {
-    const int t = p.s * kE4Slice + ((lane & 3) * kE4Warps + warp) * 16;
-    if (t >= n) return -1ll;
-    int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, p.b, t / bs);
+  // this warp's tile `lane & 3` of a slice, counted over a whole array (-1 where the sequence ends before it), and its page and head as the exponents
+  // are counted
+  const int per_page = bs >> 4;
+  auto locate = [&](const E4Place& p, int n, int& tile, int& where) {
+    const int t = p.s * (kE4Slice / 16) + (lane & 3) * kE4Warps + warp;
+    tile = -1;
+    if (t * 16 >= n) return;
+    const int i = per_page == 1 ? t : t / per_page;
+    int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, p.b, i);
     if (page < 0) {                                  // corrupt tables read block 0 instead of faulting
       RB_BOUNDS_HIT(104);
       page = 0;
     }
-    return (static_cast<long long>(page) * G + p.hk) * (bs / 16) + t % bs / 16;
+    where = page * G + p.hk;
+    tile = where * per_page + t - i * per_page;
   };
-  auto request = [&](int stage, long long tile) {    // lane 0
+  auto request = [&](int stage, int tile) {          // lane 0
     const uint32_t bar = smem_u32(&bars[warp][stage]), dst = ring + stage * 2 * L::kTile;
     mbar_arrive_expect_tx(bar, 2 * L::kTile);
-    tma_load_2d(dst, &k_map, 0, static_cast<int>(tile) * BR, bar);
-    tma_load_2d(dst + L::kTile, &v_map, 0, static_cast<int>(tile) * BR, bar);
+    tma_load_2d(dst, &k_map, 0, tile * BR, bar);
+    tma_load_2d(dst + L::kTile, &v_map, 0, tile * BR, bar);
   };
   auto advance = [&](E4Place& p, int& n) {           // the next slice of the run
     if (--p.left <= 0) {
@@ -178,22 +182,21 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
     while (n == 0);
   };
 
-  int n_at = e4_len(a, at.b);
-  long long tile_at = locate(at, n_at);
+  int n_at = e4_len(a, at.b), tile_at, where = 0;
+  locate(at, n_at, tile_at, where);
 #pragma unroll
   for (int i = 0; i < kE4Stages; ++i) {
-    const long long t = __shfl_sync(0xffffffffu, tile_at, i);
+    const int t = __shfl_sync(0xffffffffu, tile_at, i);
     if (lane == 0 && t >= 0) request(i, t);
   }
-  int exps = 0;                                      // lanes 0 .. 3: exponents of the four tiles' keys, 4 .. 7 of their values
-  auto exps_of = [&](long long tile) { return tile < 0 || lane >= 8 ? 0 : static_cast<int>((lane < 4 ? a.pages.k_exp : a.pages.v_exp)[tile / (bs / 16)]); };
-  exps = exps_of(tile_at);
+  // lanes 0 .. 3: exponents of the four tiles' keys, 4 .. 7 of their values
+  auto exps_of = [&](int tile, int w) { return tile < 0 || lane >= 8 ? 0 : static_cast<int>((lane < 4 ? a.pages.k_exp : a.pages.v_exp)[w]); };
+  int exps = exps_of(tile_at, where);
   E4Place next = at;
-  int n_next = n_at;
-  long long tile_next = -1;
+  int n_next = n_at, tile_next = -1;
   if (LIST) {
     advance(next, n_next);
-    tile_next = locate(next, n_next);
+    locate(next, n_next, tile_next, where);
   }
 
   uint32_t qf[KS][NH * 2];
@@ -235,7 +238,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
 #pragma unroll 1
     for (int i = 0; i < kE4Stages; ++i) {
       const int n_tok = n_at - (at.s * kE4Slice + (i * kE4Warps + warp) * 16);         // tokens of the tile and behind it
-      const long long coming = __shfl_sync(0xffffffffu, tile_next, i);
+      const int coming = __shfl_sync(0xffffffffu, tile_next, i);
       if (n_tok > 0) {
         mbar_wait(smem_u32(&bars[warp][i]), (parity >> i) & 1, &abort_sh, status, 130);
         parity ^= 1u << i;
@@ -301,7 +304,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
             }
           }
           if (a.accumulate && r * 8 + gq < heads) {
-            float* scores = a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (D + 2) +
+            float* scores = a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (D + 4) +
                             (static_cast<long long>(at.b) * a.heads + at.hk * group + h0 + r * 8 + gq) * slices * kE4Slice + at.s * kE4Slice +
                             (i * kE4Warps + warp) * 16 + tq * 2;
 #pragma unroll
@@ -372,7 +375,8 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
 #pragma unroll
       for (int c = 0; c < 2; ++c) {                  // head 2 tq + c, dimensions gq * D / 8 .., 16 bytes at a time, swizzled by the head
         const int head = r * 8 + tq * 2 + c;
-        float* row = merge + (warp * NH * 8 + head) * D;
+        if (head >= heads) continue;
+        float* row = merge + (warp * heads + head) * D;
 #pragma unroll
         for (int t = 0; t < MT; t += 2)
           *reinterpret_cast<float4*>(row + (((gq * (D / 32) + t / 2) ^ tq) << 2)) = make_float4(o[t][r][c], o[t][r][2 + c], o[t + 1][r][c], o[t + 1][r][2 + c]);
@@ -380,27 +384,37 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
     }
     __syncthreads();
     const bool whole = n_at <= kE4Slice;             // the sequence has no other slice
-    for (int i = threadIdx.x; i < heads * D; i += kE4Warps * 32) {
-      const int head = i / D, d = i - head * D;
-      float top = m_sh[0][head];
+    for (int i = threadIdx.x; i < heads * (D / 4); i += kE4Warps * 32) {
+      const int head = i / (D / 4), d = i % (D / 4);
+      float f[kE4Warps], top = m_sh[0][head];
 #pragma unroll
       for (int w = 1; w < kE4Warps; ++w) top = fmaxf(top, m_sh[w][head]);
-      float sum = 0.f, den = 0.f;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      float den = 0.f;
 #pragma unroll
       for (int w = 0; w < kE4Warps; ++w) {
-        const float mw = m_sh[w][head], f = mw == -INFINITY ? 0.f : e4_ex2(mw - top);
-        sum = fmaf(merge[(w * NH * 8 + head) * D + (((d >> 2) ^ (head >> 1 & 3)) << 2) + (d & 3)], f, sum);
-        den = fmaf(l_sh[w][head], f, den);
+        const float mw = m_sh[w][head];
+        f[w] = mw == -INFINITY ? 0.f : e4_ex2(mw - top);
+        den = fmaf(l_sh[w][head], f[w], den);
+        const float4 x = *reinterpret_cast<const float4*>(merge + (w * heads + head) * D + ((d ^ (head >> 1 & 3)) << 2));
+        sum.x = fmaf(x.x, f[w], sum.x);
+        sum.y = fmaf(x.y, f[w], sum.y);
+        sum.z = fmaf(x.z, f[w], sum.z);
+        sum.w = fmaf(x.w, f[w], sum.w);
       }
       const int h = at.hk * group + h0 + head;
-      if (whole) e4_put(reinterpret_cast<T*>(a.out) + at.b * a.ld_o + static_cast<long long>(h) * D + d, sum / den);
+      if (whole) {
+        const float inv = 1.f / den;
+        T* out = reinterpret_cast<T*>(a.out) + at.b * a.ld_o + static_cast<long long>(h) * D + d * 4;
+        e4_put(out, sum.x * inv);
+        e4_put(out + 1, sum.y * inv);
+        e4_put(out + 2, sum.z * inv);
+        e4_put(out + 3, sum.w * inv);
+      }
       if (!whole || a.accumulate) {
         float* out = e4_partial(a.scratch, a.heads, slices, D, at.b, h, at.s);
-        if (d == 0) {
-          out[0] = top;
-          out[1] = den;
-        }
-        out[2 + d] = sum;
+        if (d == 0) *reinterpret_cast<float2*>(out) = make_float2(top, den);
+        *reinterpret_cast<float4*>(out + 4 + d * 4) = sum;
       }
     }
     if (!LIST || at.left <= 1) break;
@@ -408,59 +422,90 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
     fresh = next.b != at.b || next.hk != at.hk;
     at = next;
     n_at = n_next;
-    exps = exps_of(tile_next);
+    exps = exps_of(tile_next, where);
     advance(next, n_next);
-    tile_next = locate(next, n_next);
+    locate(next, n_next, tile_next, where);
   }
 }
 
-template <typename T>
+// Adds the slices of a sequence for one head: 16 chains of every 16th slice, in order, then the chains in order.  COLS: 16-byte columns that a CTA of
+// 128 threads takes, D / 4 or, where a sequence may have many slices, 8, so that more of them read at the same time; the sums are the same.
+template <typename T, int COLS>
 __global__ void __launch_bounds__(128)
 e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
   pdl_wait();
   pdl_launch();
-  __shared__ float f_sh[128], l_sh[128], red[4];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, D = a.pages.head_dim;
-  T* out = reinterpret_cast<T*>(a.out) + b * a.ld_o + static_cast<long long>(h) * D;
+  constexpr int kChains = 16, R = 128 / COLS, PER = kChains / R;
+  __shared__ float4 sum_sh[kChains][COLS];
+  __shared__ float l_sh[kChains], red[4];
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, D = a.pages.head_dim, c = tid % COLS, r = tid / COLS;
+  T* out = reinterpret_cast<T*>(a.out) + b * a.ld_o + static_cast<long long>(h) * D + blockIdx.z * (COLS * 4);
   const int here = (e4_len(a, b) + kE4Slice - 1) / kE4Slice;
   if (here == 0) {
-    if (tid < D) e4_put(out + tid, 0.f);
+    if (tid < COLS * 4) e4_put(out + tid, 0.f);
     return;
   }
   if (here == 1 && !a.accumulate) return;            // already written
   const float* first = e4_partial(a.scratch, a.heads, slices, D, b, h, 0);
+  const long long pitch = D + 4;
   float m = -INFINITY;
-  for (int s = tid; s < here; s += 128) m = fmaxf(m, first[static_cast<long long>(s) * (D + 2)]);
+  for (int s = tid; s < here; s += 128) m = fmaxf(m, first[s * pitch]);
   m = warp_max(m);
   if ((tid & 31) == 0) red[tid >> 5] = m;
   __syncthreads();
   m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  float l = 0.f, o = 0.f;
-  for (int s0 = 0; s0 < here; s0 += 128) {
-    const int n = min(128, here - s0);
-    __syncthreads();
-    if (tid < n) {
-      const float* p = first + static_cast<long long>(s0 + tid) * (D + 2);
-      f_sh[tid] = e4_ex2(p[0] - m);
-      l_sh[tid] = p[1];
-    }
-    __syncthreads();
-    const float* p = first + static_cast<long long>(s0) * (D + 2) + 2 + tid;
-    if (tid < D) {
-#pragma unroll 8
-      for (int s = 0; s < n; ++s) {
-        o = fmaf(p[static_cast<long long>(s) * (D + 2)], f_sh[s], o);
-        l = fmaf(l_sh[s], f_sh[s], l);
-      }
+  float4 sum[PER];
+  float l[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    sum[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    l[k] = 0.f;
+  }
+#pragma unroll 4
+  for (int s0 = r; s0 < here; s0 += kChains) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int s = s0 + k * R;
+      if (s >= here) break;
+      const float* p = first + s * pitch;
+      const float2 ml = *reinterpret_cast<const float2*>(p);
+      const float4 x = *reinterpret_cast<const float4*>(p + 4 + (blockIdx.z * COLS + c) * 4);
+      const float f = e4_ex2(ml.x - m);
+      l[k] = fmaf(ml.y, f, l[k]);
+      sum[k].x = fmaf(x.x, f, sum[k].x);
+      sum[k].y = fmaf(x.y, f, sum[k].y);
+      sum[k].z = fmaf(x.z, f, sum[k].z);
+      sum[k].w = fmaf(x.w, f, sum[k].w);
     }
   }
-  if (here > 1 && tid < D) e4_put(out + tid, o / l);
-  if (a.accumulate && tid == 0) {
-    // a weight is 2^(s - m) / l = 2^(s - (m + x)) / (l / 2^x), with the x that brings l / 2^x into [1, 2)
-    const int x = static_cast<int>(__float_as_uint(l) >> 23) - 127;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    sum_sh[r + k * R][c] = sum[k];
+    if (c == 0) l_sh[r + k * R] = l[k];
+  }
+  __syncthreads();
+  if (tid >= COLS) return;
+  float4 o = sum_sh[0][c];
+  float den = l_sh[0];
+#pragma unroll
+  for (int k = 1; k < kChains; ++k) {
+    const float4 x = sum_sh[k][c];
+    o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+    den += l_sh[k];
+  }
+  if (here > 1) {
+    const float inv = 1.f / den;
+    e4_put(out + c * 4, o.x * inv);
+    e4_put(out + c * 4 + 1, o.y * inv);
+    e4_put(out + c * 4 + 2, o.z * inv);
+    e4_put(out + c * 4 + 3, o.w * inv);
+  }
+  if (a.accumulate && tid == 0 && blockIdx.z == 0) {
+    // a weight is 2^(s - m) / den = 2^(s - (m + x)) / (den / 2^x), with the x that brings den / 2^x into [1, 2)
+    const int x = static_cast<int>(__float_as_uint(den) >> 23) - 127;
     float* norm = e4_norm(a.scratch, a.batch, a.heads, slices, D, b, h);
     norm[0] = m + static_cast<float>(x);
-    norm[1] = e4_two(x) / l;
+    norm[1] = e4_two(x) / den;
   }
 }
 
@@ -472,7 +517,7 @@ e4_weight_kernel(const RbE4m3DecodeArgs a, int slices) {
   const int bs = a.pages.block_size, G = a.pages.kv_heads, group = a.heads / G;
   const int t = s * kE4Slice + threadIdx.x;
   if (t >= e4_len(a, b)) return;
-  const float* scores = a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (D + 2);
+  const float* scores = a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (D + 4);
   float w = 0.f;
   for (int h = 0; h < group; ++h) {
     const long long row = static_cast<long long>(b) * a.heads + hk * group + h;
@@ -501,26 +546,30 @@ int decode_launch(const RbE4m3DecodeArgs& a, cudaStream_t stream) {
   const CUtensorMap* vm = km ? rbhost::get_tmap_2d(p.v, 1, 128, rows, 128, 128, D / 8, 1, &err) : nullptr;
   unsigned int* status = rbhost::status_ptr();
   if (!vm || !status) return err ? err : -3;
-  static int per_sm[2][64] = {};                     // CTAs of a list that fit on an SM
+  const int group = a.heads / p.kv_heads, most = group < NH * 8 ? group : NH * 8, smem = L::bytes(most);
+  static int per_sm[NH * 8 + 1][64] = {};            // CTAs of a list that fit on an SM, by the heads that a pass has
   const int dev = rbhost::device_slot();
-  for (int list = 0; list < 2; ++list)
-    if (!per_sm[list][dev]) {
-      auto kern = list ? rb::e4_decode_kernel<T, D, NH, true> : rb::e4_decode_kernel<T, D, NH, false>;
-      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
-      int n = 0;
-      if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, rb::kE4Warps * 32, L::kBytes);
-      if (e != cudaSuccess) return static_cast<int>(e);
-      per_sm[list][dev] = n > 0 ? n : 1;
-    }
-  const int some = per_sm[1][dev] * rbhost::device_sm_count();
+  if (!per_sm[most][dev]) {
+    cudaError_t e = cudaFuncSetAttribute(rb::e4_decode_kernel<T, D, NH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::bytes(NH * 8));
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(rb::e4_decode_kernel<T, D, NH, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::bytes(NH * 8));
+    int n = 0;
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rb::e4_decode_kernel<T, D, NH, true>, rb::kE4Warps * 32, smem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    per_sm[most][dev] = n > 0 ? n : 1;
+  }
+  const int some = per_sm[most][dev] * rbhost::device_sm_count();
   const bool list = static_cast<long long>(a.batch) * p.kv_heads * slices > some;
   auto kern = list ? rb::e4_decode_kernel<T, D, NH, true> : rb::e4_decode_kernel<T, D, NH, false>;
   const dim3 grid = list ? dim3(some) : dim3(slices, p.kv_heads, a.batch);
-  const int group = a.heads / p.kv_heads;
   cudaError_t e = cudaSuccess;
   for (int h0 = 0; h0 < group && e == cudaSuccess; h0 += NH * 8)        // wider groups take several passes
-    e = rbhost::launch_pdl(kern, grid, dim3(rb::kE4Warps * 32), L::kBytes, stream, 1, *km, *vm, a, h0, slices, status RB_BOUNDS_ARG);
-  if (e == cudaSuccess) e = rbhost::launch_pdl(rb::e4_merge_kernel<T>, dim3(a.heads, a.batch), dim3(128), 0, stream, 1, a, slices);
+    e = rbhost::launch_pdl(kern, grid, dim3(rb::kE4Warps * 32), smem, stream, 1, *km, *vm, a, h0, slices, status RB_BOUNDS_ARG);
+  if (e == cudaSuccess) {
+    const bool many = slices > 64;
+    e = rbhost::launch_pdl(many ? rb::e4_merge_kernel<T, 8> : rb::e4_merge_kernel<T, D / 4>, dim3(a.heads, a.batch, many ? D / 32 : 1), dim3(128), 0, stream, 1,
+                           a, slices);
+  }
   if (e == cudaSuccess && a.accumulate)
     e = rbhost::launch_pdl(rb::e4_weight_kernel, dim3(slices, p.kv_heads, a.batch), dim3(256), 0, stream, 1, a, slices);
   return static_cast<int>(e);
@@ -535,7 +584,7 @@ int decode_by_dim(const RbE4m3DecodeArgs& a, cudaStream_t s) {
 
 RB_API long long rb_e4m3_decode_scratch_floats(int batch, int heads, int head_dim, int max_blocks, int block_size, int accumulate) {
   const long long slices = e4_slices(max_blocks, block_size), rows = static_cast<long long>(batch) * heads;
-  return rows * slices * (head_dim + 2) + (accumulate ? rows * (slices * rb::kE4Slice + 2) : 0);
+  return rows * slices * (head_dim + 4) + (accumulate ? rows * (slices * rb::kE4Slice + 2) : 0);
 }
 
 RB_API int rb_e4m3_decode(const RbE4m3DecodeArgs* args, void* stream_v) {
