@@ -35,6 +35,10 @@ __device__ __forceinline__ uint32_t e4_half2(uint32_t codes) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(codes)));
   return r;
 }
+// four codes to two pairs of halves
+__device__ __forceinline__ void e4_half4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(codes));
+}
 __device__ __forceinline__ float2 e4_float2(uint32_t codes) {
   const uint32_t h = e4_half2(codes);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));

@@ -23,7 +23,7 @@ __device__ __forceinline__ void e4_put(__nv_bfloat16* p, float v) { *p = __float
 __device__ __forceinline__ void e4_put(__half* p, float v) { *p = __float2half(v); }
 
 // Scratch: [batch, heads, slices, D + 4] fp32: maximum, denominator, two unused, sums of a slice; then, where weights are summed, the scores
-// [batch, heads, slices * 256] and the denominators as whole powers of two and factors [batch, heads, 2].
+// [batch, KV heads, slices * 256, heads of a group] and the denominators as whole powers of two and factors [batch, heads, 2].
 __device__ __forceinline__ float* e4_partial(float* scratch, int heads, int slices, int D, int b, int h, int s) {
   return scratch + ((static_cast<long long>(b) * heads + h) * slices + s) * (D + 4);
 }
@@ -75,14 +75,15 @@ struct E4Layout {
 // Warp w of a CTA takes tiles w, w + 4, w + 8, w + 12 of 16 tokens of a slice; its sums and those of the other warps are added in the order of the
 // warps, and a sequence's slices in order by the merge, so that a sequence has the same bits alone and beside others.
 //
-// S = Q K^T has the heads as the 16 rows of m16n8k16 (NH: 8 or 16 of them there), O^T = V^T P^T the head dimensions as rows and the heads as the 8
-// columns: the accumulators of S then are, rounded to f16, the second operand of the other product as they lie.  Codes become f16 exactly.  The
-// contraction over head dimensions may take them in any order, so a lane reads 16 codes of a row at a time and these are its operands of four
-// products; a swizzled tile gives every lane its 16 bytes without bank conflicts.  A query row is scaled to [1, 2) by a power of two first.
+// S^T = K Q^T has the tokens as the 16 rows of m16n8k16 and the heads as its 8 columns (NH: 8 or 16 heads), O^T = V^T P^T the head dimensions as
+// rows and the heads as columns, so that no row is left empty and a lane's factors are those of its own columns; P^T, rounded to f16, takes its place as
+// the second operand by a transposition of 8 x 8 (movmatrix).  Codes become f16 exactly.  The contraction over head dimensions may take them in any
+// order, so a lane reads 16 codes of a row at a time and these are its operands of four products; a swizzled tile gives every lane its 16 bytes without
+// bank conflicts.  A query row is scaled to [1, 2) by a power of two first.
 // LIST: the slices of all sequences and KV heads, numbered one sequence after the other, are dealt in equal runs to CTAs that stay, and the next slice's
 // tiles are copied while this one's are worked on.  Otherwise the grid is (slices, KV heads, sequences).
 template <typename T, int D, int NH, bool LIST>
-__global__ void __launch_bounds__(kE4Warps * 32)
+__global__ void __launch_bounds__(kE4Warps * 32, NH == 1 ? 3 : 2)
 e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const RbE4m3DecodeArgs a, int h0, int slices,
                  unsigned int* status RB_BOUNDS_PARAM) {
   pdl_wait();
@@ -91,6 +92,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
   constexpr int KS = D / 16;                         // products of 16 in a score
   constexpr int MT = D / 16;                         // tiles of 16 output dimensions
   constexpr int BR = D / 8;                          // rows of 128 bytes in a tile
+  constexpr int kNone = static_cast<int>(0x80000000);
   extern __shared__ uint8_t e4_raw[];
   __shared__ __align__(8) uint64_t bars[kE4Warps][kE4Stages];
   __shared__ float m_sh[kE4Warps][NH * 8], l_sh[kE4Warps][NH * 8];
@@ -112,25 +114,23 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
   } else {
     int n = lane < a.batch ? (e4_len(a, lane) + kE4Slice - 1) / kE4Slice : 0, total = n;
     for (int i = lane + 32; i < a.batch; i += 32) total += (e4_len(a, i) + kE4Slice - 1) / kE4Slice;
-    total = __reduce_add_sync(0xffffffffu, total);
-    const long long all = static_cast<long long>(total) * G;
-    const long long first = all * blockIdx.x / gridDim.x, end = all * (blockIdx.x + 1) / gridDim.x;
-    if (end == first) return;
-    at.left = static_cast<int>(end - first);
-    long long skip = first;
+    const unsigned int all = __reduce_add_sync(0xffffffffu, total) * static_cast<unsigned int>(G);      // the host bounds it
+    const unsigned int share = all / gridDim.x, over = all - share * gridDim.x;
+    at.left = share + (blockIdx.x < over ? 1 : 0);
+    if (at.left == 0) return;
+    unsigned int skip = blockIdx.x * share + min(blockIdx.x, over);
     for (int b0 = 0;;) {
-      long long upto = static_cast<long long>(n) * G;
-      const long long own = upto;
+      unsigned int upto = n * G;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        const unsigned int v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
       }
       const unsigned int behind = __ballot_sync(0xffffffffu, upto > skip);
       if (behind != 0u) {
         const int which = __ffs(behind) - 1;
         at.b = b0 + which;
-        const int in = static_cast<int>(skip - __shfl_sync(0xffffffffu, upto - own, which)), ns = __shfl_sync(0xffffffffu, n, which);
+        const int in = skip - __shfl_sync(0xffffffffu, upto - n * G, which), ns = __shfl_sync(0xffffffffu, n, which);
         at.hk = in / ns;
         at.s = in - at.hk * ns;
         break;
@@ -147,21 +147,24 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
   fence_mbar_init();
   __syncthreads();
 
-  // this warp's tile `lane & 3` of a slice, counted over a whole array (-1 where the sequence ends before it), and its page and head as the exponents
-  // are counted
-  const int per_page = bs >> 4;
-  auto locate = [&](const E4Place& p, int n, int& tile, int& where) {
-    const int t = p.s * (kE4Slice / 16) + (lane & 3) * kE4Warps + warp;
-    tile = -1;
-    if (t * 16 >= n) return;
+  // The page of this warp's tile `lane & 3` of a slice as the table says it, kNone where the sequence ends before the tile
+  const int per_page = bs >> 4, tile_in = (lane & 3) * kE4Warps + warp;
+  auto look_up = [&](const E4Place& p, int n) {
+    const int t = p.s * (kE4Slice / 16) + tile_in;
+    if (t * 16 >= n) return kNone;
     const int i = per_page == 1 ? t : t / per_page;
-    int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, p.b, i);
-    if (page < 0) {                                  // corrupt tables read block 0 instead of faulting
+    return a.block_tables[static_cast<long long>(p.b) * a.max_blocks + i];             // n is no more than the table has room for
+  };
+  // the tile counted over a whole array (-1: none), and its page and head as the exponents are counted
+  auto locate = [&](const E4Place& p, int page, int& tile, int& where) {
+    tile = -1;
+    if (page == kNone) return;
+    if (page < 0 || page >= a.pages.num_blocks) {    // corrupt tables read block 0 instead of faulting
       RB_BOUNDS_HIT(104);
       page = 0;
     }
     where = page * G + p.hk;
-    tile = where * per_page + t - i * per_page;
+    tile = per_page == 1 ? where : where * per_page + (p.s * (kE4Slice / 16) + tile_in) % per_page;
   };
   auto request = [&](int stage, int tile) {          // lane 0
     const uint32_t bar = smem_u32(&bars[warp][stage]), dst = ring + stage * 2 * L::kTile;
@@ -181,226 +184,282 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
     do n = e4_len(a, ++p.b);
     while (n == 0);
   };
+  // lanes 0 .. 3: exponents of the four tiles' keys, 4 .. 7 of their values
+  auto exps_of = [&](int tile, int w) { return tile < 0 || lane >= 8 ? 0 : static_cast<int>((lane < 4 ? a.pages.k_exp : a.pages.v_exp)[w]); };
 
   int n_at = e4_len(a, at.b), tile_at, where = 0;
-  locate(at, n_at, tile_at, where);
+  locate(at, look_up(at, n_at), tile_at, where);
 #pragma unroll
   for (int i = 0; i < kE4Stages; ++i) {
     const int t = __shfl_sync(0xffffffffu, tile_at, i);
     if (lane == 0 && t >= 0) request(i, t);
   }
-  // lanes 0 .. 3: exponents of the four tiles' keys, 4 .. 7 of their values
-  auto exps_of = [&](int tile, int w) { return tile < 0 || lane >= 8 ? 0 : static_cast<int>((lane < 4 ? a.pages.k_exp : a.pages.v_exp)[w]); };
   int exps = exps_of(tile_at, where);
-  E4Place next = at;
-  int n_next = n_at, tile_next = -1;
+  // Of a list, the next slice's tiles are known and their exponents on their way, and so are the pages of the one behind it: every load has a slice's
+  // time to arrive.
+  E4Place next = at, then = at;
+  int n_next = n_at, n_then = n_at, tile_next = -1, exps_next = 0, page_then = 0;
   if (LIST) {
     advance(next, n_next);
-    locate(next, n_next, tile_next, where);
+    locate(next, look_up(next, n_next), tile_next, where);
+    exps_next = exps_of(tile_next, where);
+    then = next;
+    n_then = n_next;
+    advance(then, n_then);
+    page_then = look_up(then, n_then);
   }
 
-  uint32_t qf[KS][NH * 2];
-  float q_up[NH];
-  bool fresh = true;
+  const bool q_whole = !((reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.ld_q * 2)) & 15);
+  uint32_t qf[KS][NH][2];                            // head r * 8 + gq, this lane's dimensions of it
+  float q_up[NH][2];                                 // heads r * 8 + 2 tq and + 1: what a product with their rows is to be multiplied with
   uint32_t parity = 0;
-  for (;;) {
-    if (fresh) {                                     // ---- query rows gq and gq + 8 of the group's heads, this lane's dimensions of them
+  for (bool fresh = true;;) {
+    if (fresh) {
 #pragma unroll
       for (int r = 0; r < NH; ++r) {
         const bool there = r * 8 + gq < heads;
         const T* src = reinterpret_cast<const T*>(a.q) + at.b * a.ld_q + (static_cast<long long>(at.hk) * group + h0 + r * 8 + gq) * D + tq * (D / 4);
         float x[D / 4], most = 0.f;
+        if (there && q_whole) {
 #pragma unroll
-        for (int i = 0; i < D / 4; ++i) {
-          x[i] = there ? e4_get(src + i) : 0.f;
-          most = fmaxf(most, fabsf(x[i]));
+          for (int i = 0; i < D / 4; i += 8) {
+            float y[8];
+            E4Row<T>::load(src + i, y);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[i + j] = y[j];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 4; ++i) x[i] = there ? e4_get(src + i) : 0.f;
         }
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) most = fmaxf(most, fabsf(x[i]));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -126), 126);
-        const float down = e4_two(-e);
-        q_up[r] = e4_two(e) * a.scale * 1.4426950408889634f;
+        const float down = e4_two(-e), up = e4_two(e) * a.scale * 1.4426950408889634f;
+        q_up[r][0] = __shfl_sync(0xffffffffu, up, tq * 8);
+        q_up[r][1] = __shfl_sync(0xffffffffu, up, tq * 8 + 4);
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
-          qf[j][2 * r] = e4_half2_of(x[4 * j] * down, x[4 * j + 1] * down);
-          qf[j][2 * r + 1] = e4_half2_of(x[4 * j + 2] * down, x[4 * j + 3] * down);
+          qf[j][r][0] = e4_half2_of(x[4 * j] * down, x[4 * j + 1] * down);
+          qf[j][r][1] = e4_half2_of(x[4 * j + 2] * down, x[4 * j + 3] * down);
         }
       }
     }
-    float m[NH], l[NH], o[MT][NH][4];
+    float m[NH][2], l[NH][2], o[MT][NH][4];          // of heads r * 8 + 2 tq and + 1; l: this lane's tokens
 #pragma unroll
     for (int r = 0; r < NH; ++r) {
-      m[r] = -INFINITY;
-      l[r] = 0.f;
+      m[r][0] = m[r][1] = -INFINITY;
+      l[r][0] = l[r][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[i][r][0] = o[i][r][1] = o[i][r][2] = o[i][r][3] = 0.f;
     }
 #pragma unroll 1
-    for (int i = 0; i < kE4Stages; ++i) {
-      const int n_tok = n_at - (at.s * kE4Slice + (i * kE4Warps + warp) * 16);         // tokens of the tile and behind it
-      const int coming = __shfl_sync(0xffffffffu, tile_next, i);
-      if (n_tok > 0) {
-        mbar_wait(smem_u32(&bars[warp][i]), (parity >> i) & 1, &abort_sh, status, 130);
-        parity ^= 1u << i;
-        const uint32_t kt = ring + i * 2 * L::kTile, vt = kt + L::kTile;
+    for (int i = 0; i < kE4Stages; i += 2) {         // two tiles at a time, each in two chains of products
+      int n_tok[2], coming[2], ev[2];                // tokens of a tile and behind it
+      float up[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        n_tok[u] = n_at - (at.s * kE4Slice + ((i + u) * kE4Warps + warp) * 16);
+        coming[u] = __shfl_sync(0xffffffffu, tile_next, i + u);
+        ev[u] = __shfl_sync(0xffffffffu, exps, 4 + i + u);
+        up[u] = e4_two(__shfl_sync(0xffffffffu, exps, i + u));
+      }
+      if (n_tok[0] <= 0) {
+        if (lane == 0) {
+          if (coming[0] >= 0) request(i, coming[0]);
+          if (coming[1] >= 0) request(i + 1, coming[1]);
+        }
+        continue;
+      }
+      float s[2][NH][4];                             // (token gq, heads 2 tq and + 1), (token gq + 8, the same)
+      uint32_t vw[2][4][D / 32];                     // codes of tokens 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9, dimensions gq * D / 8 ..
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (n_tok[u] > 0) {
+          mbar_wait(smem_u32(&bars[warp][i + u]), (parity >> (i + u)) & 1, &abort_sh, status, 130);
+          parity ^= 1u << (i + u);
+        }
+        const uint32_t kt = ring + (i + u) * 2 * L::kTile, vt = kt + L::kTile;
         uint32_t kw[2][D / 16];                      // codes of tokens gq and gq + 8, dimensions tq * D / 4 ..
-        uint32_t vw[4][D / 32];                      // codes of tokens 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9, dimensions gq * D / 8 ..
         if (D == 128) {
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-              const uint4 u = e4_lds128(kt + (t * 8 + gq) * 128 + (((tq * 2 + p) ^ gq) << 4));
-              kw[t][p * 4] = u.x; kw[t][p * 4 + 1] = u.y; kw[t][p * 4 + 2] = u.z; kw[t][p * 4 + 3] = u.w;
+              const uint4 x = e4_lds128(kt + (t * 8 + gq) * 128 + (((tq * 2 + p) ^ gq) << 4));
+              kw[t][p * 4] = x.x; kw[t][p * 4 + 1] = x.y; kw[t][p * 4 + 2] = x.z; kw[t][p * 4 + 3] = x.w;
             }
           }
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
             const int row = tq * 2 + (t & 1) + (t >> 1) * 8;
-            const uint4 u = e4_lds128(vt + row * 128 + ((gq ^ (row & 7)) << 4));
-            vw[t][0] = u.x; vw[t][1] = u.y; vw[t][D / 32 - 2] = u.z; vw[t][D / 32 - 1] = u.w;
+            const uint4 x = e4_lds128(vt + row * 128 + ((gq ^ (row & 7)) << 4));
+            vw[u][t][0] = x.x; vw[u][t][1] = x.y; vw[u][t][D / 32 - 2] = x.z; vw[u][t][D / 32 - 1] = x.w;
           }
         } else {                                     // two tokens in a row of 128 bytes
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             const int tok = t * 8 + gq, row = tok >> 1;
-            const uint4 u = e4_lds128(kt + row * 128 + ((((tok & 1) * 4 + tq) ^ row) << 4));
-            kw[t][0] = u.x; kw[t][1] = u.y; kw[t][2] = u.z; kw[t][3] = u.w;
+            const uint4 x = e4_lds128(kt + row * 128 + ((((tok & 1) * 4 + tq) ^ row) << 4));
+            kw[t][0] = x.x; kw[t][1] = x.y; kw[t][2] = x.z; kw[t][3] = x.w;
           }
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
             const int tok = tq * 2 + (t & 1) + (t >> 1) * 8, row = tok >> 1;
-            const uint2 u = e4_lds64(vt + row * 128 + ((((tok & 1) * 4 + (gq >> 1)) ^ row) << 4) + (gq & 1) * 8);
-            vw[t][0] = u.x; vw[t][1] = u.y;
+            const uint2 x = e4_lds64(vt + row * 128 + ((((tok & 1) * 4 + (gq >> 1)) ^ row) << 4) + (gq & 1) * 8);
+            vw[u][t][0] = x.x; vw[u][t][1] = x.y;
           }
         }
-        __syncwarp();                                // the stage is free
-        if (lane == 0 && coming >= 0 && !abort_sh) request(i, coming);
-        // ---- scores of tokens 2 tq, 2 tq + 1 (c 0) and + 8 (c 1) under heads gq and gq + 8
-        float s[2][4];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          s[c][0] = s[c][1] = s[c][2] = s[c][3] = 0.f;
-#pragma unroll
-          for (int j = 0; j < KS; ++j)
-            e4_mma(s[c], qf[j][0], NH > 1 ? qf[j][NH * 2 - 2] : 0u, qf[j][1], NH > 1 ? qf[j][NH * 2 - 1] : 0u, e4_half2(kw[c][j]), e4_half2(kw[c][j] >> 16));
-        }
-        const int ev = __shfl_sync(0xffffffffu, exps, 4 + i);
-        const float up = e4_two(__shfl_sync(0xffffffffu, exps, i)), ev_down = e4_two(-ev);
-        uint32_t pf[NH][2];
-        float grow[NH];
-        bool moved = false;
+        float odd[NH][4];
 #pragma unroll
         for (int r = 0; r < NH; ++r) {
-          const float f = up * q_up[r];
-          float most = -INFINITY;
+          s[u][r][0] = s[u][r][1] = s[u][r][2] = s[u][r][3] = 0.f;
+          odd[r][0] = odd[r][1] = odd[r][2] = odd[r][3] = 0.f;
+        }
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+        for (int j = 0; j < KS; ++j) {
+          uint32_t a0, a1, a2, a3;
+          e4_half4(kw[0][j], a0, a2);
+          e4_half4(kw[1][j], a1, a3);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const float x = s[c][2 * r + j] * f;
-              s[c][2 * r + j] = c * 8 + tq * 2 + j < n_tok ? x : -INFINITY;
-              most = fmaxf(most, s[c][2 * r + j]);
-            }
+          for (int r = 0; r < NH; ++r) e4_mma(j & 1 ? odd[r] : s[u][r], a0, a1, a2, a3, qf[j][r][0], qf[j][r][1]);
+        }
+#pragma unroll
+        for (int r = 0; r < NH; ++r) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[u][r][j] += odd[r][j];
+        }
+      }
+      __syncwarp();                                  // the stages are free
+      if (lane == 0) {
+        if (coming[0] >= 0) request(i, coming[0]);
+        if (coming[1] >= 0) request(i + 1, coming[1]);
+      }
+      uint32_t pf[2][NH][2];
+      float grow[NH][2];
+      bool moved = false;
+#pragma unroll
+      for (int r = 0; r < NH; ++r) {
+        float to[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[u][r][j] *= up[u] * q_up[r][j & 1];
+            if (n_tok[u] < 16 && gq + (j >> 1) * 8 >= n_tok[u]) s[u][r][j] = -INFINITY;
           }
-          if (a.accumulate && r * 8 + gq < heads) {
+          if (a.accumulate) {                        // [batch, KV heads, tokens, heads of a group]
             float* scores = a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (D + 4) +
-                            (static_cast<long long>(at.b) * a.heads + at.hk * group + h0 + r * 8 + gq) * slices * kE4Slice + at.s * kE4Slice +
-                            (i * kE4Warps + warp) * 16 + tq * 2;
+                            ((static_cast<long long>(at.b) * G + at.hk) * slices * kE4Slice + at.s * kE4Slice + ((i + u) * kE4Warps + warp) * 16 + gq) * group + h0;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              scores[c * 8] = s[c][2 * r];
-              scores[c * 8 + 1] = s[c][2 * r + 1];
+            for (int j = 0; j < 4; ++j) {
+              const int h = r * 8 + tq * 2 + (j & 1);
+              if (h < heads) scores[(j >> 1) * 8 * group + h] = s[u][r][j];
             }
           }
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-          const float to = fmaxf(m[r], ceilf(most) + static_cast<float>(ev));
-          grow[r] = to == m[r] ? 1.f : e4_ex2(m[r] - to);
-          moved |= to != m[r];
-          m[r] = to;
-          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) to[j] = fmaxf(to[j], ceilf(fmaxf(s[u][r][j], s[u][r][2 + j])) + static_cast<float>(ev[u]));
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) to[j] = fmaxf(to[j], __shfl_xor_sync(0xffffffffu, to[j], x));
+          to[j] = fmaxf(to[j], m[r][j]);
+          grow[r][j] = to[j] == m[r][j] ? 1.f : e4_ex2(m[r][j] - to[j]);
+          moved |= to[j] != m[r][j];
+          m[r][j] = to[j];
+          l[r][j] *= grow[r][j];
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float e = static_cast<float>(ev[u]), down = e4_two(-ev[u]);
+          float p[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p[j] = e4_ex2(s[u][r][j] - (to[j & 1] - e));
+          l[r][0] = fmaf(p[0] + p[2], down, l[r][0]);
+          l[r][1] = fmaf(p[1] + p[3], down, l[r][1]);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float p0 = e4_ex2(s[c][2 * r] - (to - static_cast<float>(ev))), p1 = e4_ex2(s[c][2 * r + 1] - (to - static_cast<float>(ev)));
-            sum += p0 + p1;
-            pf[r][c] = e4_half2_of(p0, p1);
-          }
-          l[r] = fmaf(sum, ev_down, l[r] * grow[r]);
-        }
-        if (__any_sync(0xffffffffu, moved)) {        // sums of heads 2 tq and 2 tq + 1
-#pragma unroll
-          for (int r = 0; r < NH; ++r) {
-            const float g0 = __shfl_sync(0xffffffffu, grow[r], tq * 8), g1 = __shfl_sync(0xffffffffu, grow[r], tq * 8 + 4);
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-              o[t][r][0] *= g0; o[t][r][1] *= g1; o[t][r][2] *= g0; o[t][r][3] *= g1;
-            }
+            const uint32_t h2 = e4_half2_of(p[2 * c], p[2 * c + 1]);
+            asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pf[u][r][c]) : "r"(h2));
           }
         }
-        if (n_tok < 16) {                            // what lies behind the last token may be anything, NaN too
+      }
+      if (i > 0 && __any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int r = 0; r < NH; ++r) {
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[t][r][j] *= grow[r][j & 1];
+          }
+        }
+      }
+      // ---- O^T += V^T P^T
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (n_tok[u] < 16) {                         // what lies behind the last token may be anything, NaN too
 #pragma unroll
           for (int t = 0; t < 4; ++t)
-            if (tq * 2 + (t & 1) + (t >> 1) * 8 >= n_tok) {
+            if (tq * 2 + (t & 1) + (t >> 1) * 8 >= n_tok[u]) {
 #pragma unroll
-              for (int w = 0; w < D / 32; ++w) vw[t][w] = 0u;
+              for (int w = 0; w < D / 32; ++w) vw[u][t][w] = 0u;
             }
         }
-        // ---- O^T += V^T P^T
 #pragma unroll
         for (int w = 0; w < D / 32; ++w) {
-          const uint32_t lo0 = __byte_perm(vw[0][w], vw[1][w], 0x5140), lo1 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
-          const uint32_t hi0 = __byte_perm(vw[2][w], vw[3][w], 0x5140), hi1 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
-          const uint32_t a00 = e4_half2(lo0), a01 = e4_half2(lo0 >> 16), a02 = e4_half2(hi0), a03 = e4_half2(hi0 >> 16);
-          const uint32_t a10 = e4_half2(lo1), a11 = e4_half2(lo1 >> 16), a12 = e4_half2(hi1), a13 = e4_half2(hi1 >> 16);
+          uint32_t a00, a01, a02, a03, a10, a11, a12, a13;
+          e4_half4(__byte_perm(vw[u][0][w], vw[u][1][w], 0x5140), a00, a01);
+          e4_half4(__byte_perm(vw[u][2][w], vw[u][3][w], 0x5140), a02, a03);
+          e4_half4(__byte_perm(vw[u][0][w], vw[u][1][w], 0x7362), a10, a11);
+          e4_half4(__byte_perm(vw[u][2][w], vw[u][3][w], 0x7362), a12, a13);
 #pragma unroll
           for (int r = 0; r < NH; ++r) {
-            e4_mma(o[2 * w][r], a00, a01, a02, a03, pf[r][0], pf[r][1]);
-            e4_mma(o[2 * w + 1][r], a10, a11, a12, a13, pf[r][0], pf[r][1]);
+            e4_mma(o[2 * w][r], a00, a01, a02, a03, pf[u][r][0], pf[u][r][1]);
+            e4_mma(o[2 * w + 1][r], a10, a11, a12, a13, pf[u][r][0], pf[u][r][1]);
           }
         }
-      } else if (lane == 0 && coming >= 0 && !abort_sh) {
-        request(i, coming);
       }
     }
     // ---- the slice's sums: all warps' together
 #pragma unroll
     for (int r = 0; r < NH; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (tq == 0) {
-        m_sh[warp][r * 8 + gq] = m[r];
-        l_sh[warp][r * 8 + gq] = l[r];
-      }
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {                  // head 2 tq + c, dimensions gq * D / 8 .., 16 bytes at a time, swizzled by the head
-        const int head = r * 8 + tq * 2 + c;
+      for (int j = 0; j < 2; ++j) {                  // head r * 8 + 2 tq + j, dimensions gq * D / 8 .., 16 bytes at a time, swizzled by the head
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[r][j] += __shfl_xor_sync(0xffffffffu, l[r][j], x);
+        const int head = r * 8 + tq * 2 + j;
         if (head >= heads) continue;
+        if (gq == 0) {
+          m_sh[warp][head] = m[r][j];
+          l_sh[warp][head] = l[r][j];
+        }
         float* row = merge + (warp * heads + head) * D;
 #pragma unroll
         for (int t = 0; t < MT; t += 2)
-          *reinterpret_cast<float4*>(row + (((gq * (D / 32) + t / 2) ^ tq) << 2)) = make_float4(o[t][r][c], o[t][r][2 + c], o[t + 1][r][c], o[t + 1][r][2 + c]);
+          *reinterpret_cast<float4*>(row + (((gq * (D / 32) + t / 2) ^ tq) << 2)) = make_float4(o[t][r][j], o[t][r][2 + j], o[t + 1][r][j], o[t + 1][r][2 + j]);
       }
     }
     __syncthreads();
     const bool whole = n_at <= kE4Slice;             // the sequence has no other slice
     for (int i = threadIdx.x; i < heads * (D / 4); i += kE4Warps * 32) {
       const int head = i / (D / 4), d = i % (D / 4);
-      float f[kE4Warps], top = m_sh[0][head];
+      float top = m_sh[0][head];
 #pragma unroll
       for (int w = 1; w < kE4Warps; ++w) top = fmaxf(top, m_sh[w][head]);
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
       float den = 0.f;
 #pragma unroll
       for (int w = 0; w < kE4Warps; ++w) {
-        const float mw = m_sh[w][head];
-        f[w] = mw == -INFINITY ? 0.f : e4_ex2(mw - top);
-        den = fmaf(l_sh[w][head], f[w], den);
+        const float mw = m_sh[w][head], f = mw == -INFINITY ? 0.f : e4_ex2(mw - top);
+        den = fmaf(l_sh[w][head], f, den);
         const float4 x = *reinterpret_cast<const float4*>(merge + (w * heads + head) * D + ((d ^ (head >> 1 & 3)) << 2));
-        sum.x = fmaf(x.x, f[w], sum.x);
-        sum.y = fmaf(x.y, f[w], sum.y);
-        sum.z = fmaf(x.z, f[w], sum.z);
-        sum.w = fmaf(x.w, f[w], sum.w);
+        sum.x = fmaf(x.x, f, sum.x);
+        sum.y = fmaf(x.y, f, sum.y);
+        sum.z = fmaf(x.z, f, sum.z);
+        sum.w = fmaf(x.w, f, sum.w);
       }
       const int h = at.hk * group + h0 + head;
       if (whole) {
@@ -422,9 +481,18 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
     fresh = next.b != at.b || next.hk != at.hk;
     at = next;
     n_at = n_next;
-    exps = exps_of(tile_next, where);
-    advance(next, n_next);
-    locate(next, n_next, tile_next, where);
+    exps = exps_next;
+    next = then;
+    n_next = n_then;
+    if (abort_sh) {                                  // a copy did not arrive: no new ones
+      next.left = then.left = 0;
+      n_next = 0;
+      page_then = kNone;
+    }
+    locate(next, page_then, tile_next, where);
+    exps_next = exps_of(tile_next, where);
+    advance(then, n_then);
+    page_then = look_up(then, n_then);
   }
 }
 
@@ -520,9 +588,8 @@ e4_weight_kernel(const RbE4m3DecodeArgs a, int slices) {
   const float* scores = a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (D + 4);
   float w = 0.f;
   for (int h = 0; h < group; ++h) {
-    const long long row = static_cast<long long>(b) * a.heads + hk * group + h;
     const float* norm = e4_norm(a.scratch, a.batch, a.heads, slices, D, b, hk * group + h);
-    w = fmaf(e4_ex2(scores[row * slices * kE4Slice + t] - norm[0]), norm[1], w);
+    w = fmaf(e4_ex2(scores[((static_cast<long long>(b) * G + hk) * slices * kE4Slice + t) * group + h] - norm[0]), norm[1], w);
   }
   const int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, t / bs);
   if (page >= 0) a.pages.weight[(static_cast<long long>(page) * G + hk) * bs + t % bs] += w;
@@ -592,7 +659,8 @@ RB_API int rb_e4m3_decode(const RbE4m3DecodeArgs* args, void* stream_v) {
   if (a.batch <= 0) return 0;
   if (const int bad = rbhost::e4_check(a.pages)) return bad;
   if (!a.q || !a.out || !a.block_tables || !a.context_lens || !a.scratch || a.max_blocks <= 0 || a.heads <= 0 || a.heads % a.pages.kv_heads ||
-      a.batch > 65535 || a.pages.kv_heads > 65535 || (a.accumulate && !a.pages.weight) || e4_slices(a.max_blocks, a.pages.block_size) > 0x7fffff)
+      a.batch > 65535 || a.pages.kv_heads > 65535 || (a.accumulate && !a.pages.weight) ||
+      static_cast<long long>(a.batch) * a.pages.kv_heads * e4_slices(a.max_blocks, a.pages.block_size) > 0x3fffffff)
     return -1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_v);
   switch (a.type) {
