@@ -83,11 +83,11 @@ struct E4Layout {
 // LIST: the slices of all sequences and KV heads, numbered one sequence after the other, are dealt in equal runs to CTAs that stay, and the next slice's
 // tiles are copied while this one's are worked on.  Otherwise the grid is (slices, KV heads, sequences).
 template <typename T, int D, int NH, bool LIST>
-__global__ void __launch_bounds__(kE4Warps * 32, NH == 1 ? 3 : 2)
+__global__ void __launch_bounds__(kE4Warps * 32, NH > 1 ? 2 : D == 64 ? 4 : 3)
 e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const RbE4m3DecodeArgs a, int h0, int slices,
                  unsigned int* status RB_BOUNDS_PARAM) {
   pdl_wait();
-  pdl_launch();
+  if (!LIST) pdl_launch();                           // CTAs that stay let the merge in at the end of their runs: 177 us at once, 159 then (64 of 4096 to 8192)
   using L = E4Layout<D, NH>;
   constexpr int KS = D / 16;                         // products of 16 in a score
   constexpr int MT = D / 16;                         // tiles of 16 output dimensions
@@ -117,7 +117,10 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
     const unsigned int all = __reduce_add_sync(0xffffffffu, total) * static_cast<unsigned int>(G);      // the host bounds it
     const unsigned int share = all / gridDim.x, over = all - share * gridDim.x;
     at.left = share + (blockIdx.x < over ? 1 : 0);
-    if (at.left == 0) return;
+    if (at.left == 0) {
+      pdl_launch();
+      return;
+    }
     unsigned int skip = blockIdx.x * share + min(blockIdx.x, over);
     for (int b0 = 0;;) {
       unsigned int upto = n * G;
@@ -442,6 +445,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
           *reinterpret_cast<float4*>(row + (((gq * (D / 32) + t / 2) ^ tq) << 2)) = make_float4(o[t][r][j], o[t][r][2 + j], o[t + 1][r][j], o[t + 1][r][2 + j]);
       }
     }
+    if (LIST && at.left <= 1) pdl_launch();
     __syncthreads();
     const bool whole = n_at <= kE4Slice;             // the sequence has no other slice
     for (int i = threadIdx.x; i < heads * (D / 4); i += kE4Warps * 32) {
@@ -505,7 +509,7 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
   pdl_launch();
   constexpr int kChains = 16, R = 128 / COLS, PER = kChains / R;
   __shared__ float4 sum_sh[kChains][COLS];
-  __shared__ float l_sh[kChains], red[4];
+  __shared__ float2 ml_sh[kChains];
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, D = a.pages.head_dim, c = tid % COLS, r = tid / COLS;
   T* out = reinterpret_cast<T*>(a.out) + b * a.ld_o + static_cast<long long>(h) * D + blockIdx.z * (COLS * 4);
   const int here = (e4_len(a, b) + kE4Slice - 1) / kE4Slice;
@@ -516,51 +520,76 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
   if (here == 1 && !a.accumulate) return;            // already written
   const float* first = e4_partial(a.scratch, a.heads, slices, D, b, h, 0);
   const long long pitch = D + 4;
-  float m = -INFINITY;
-  for (int s = tid; s < here; s += 128) m = fmaxf(m, first[s * pitch]);
-  m = warp_max(m);
-  if ((tid & 31) == 0) red[tid >> 5] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  // every sum beside its own maximum; a new maximum's factor is a power of two, so that the sums are those under the largest of all
   float4 sum[PER];
-  float l[PER];
+  float m[PER], l[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     sum[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    m[k] = -INFINITY;
     l[k] = 0.f;
   }
-#pragma unroll 4
-  for (int s0 = r; s0 < here; s0 += kChains) {
+  auto add = [](float4& x, float& mx, float& lx, const float4& y, float my, float ly) {
+    const float to = fmaxf(mx, my);
+    const float f = mx == to ? 1.f : e4_ex2(mx - to), g = my == to ? 1.f : e4_ex2(my - to);
+    x.x = fmaf(y.x, g, x.x * f);
+    x.y = fmaf(y.y, g, x.y * f);
+    x.z = fmaf(y.z, g, x.z * f);
+    x.w = fmaf(y.w, g, x.w * f);
+    lx = fmaf(ly, g, lx * f);
+    mx = to;
+  };
+  constexpr int kAhead = PER == 1 ? 8 : 1;           // slices of a chain that are loaded together
+  for (int s0 = r; s0 < here; s0 += kChains * kAhead) {
+    float4 x[PER][kAhead];
+    float2 ml[PER][kAhead];
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int s = s0 + k * R;
-      if (s >= here) break;
-      const float* p = first + s * pitch;
-      const float2 ml = *reinterpret_cast<const float2*>(p);
-      const float4 x = *reinterpret_cast<const float4*>(p + 4 + (blockIdx.z * COLS + c) * 4);
-      const float f = e4_ex2(ml.x - m);
-      l[k] = fmaf(ml.y, f, l[k]);
-      sum[k].x = fmaf(x.x, f, sum[k].x);
-      sum[k].y = fmaf(x.y, f, sum[k].y);
-      sum[k].z = fmaf(x.z, f, sum[k].z);
-      sum[k].w = fmaf(x.w, f, sum[k].w);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int s = s0 + k * R + i * kChains;
+        ml[k][i] = make_float2(-INFINITY, 0.f);
+        x[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s < here) {
+          const float* p = first + s * pitch;
+          ml[k][i] = *reinterpret_cast<const float2*>(p);
+          x[k][i] = *reinterpret_cast<const float4*>(p + 4 + (blockIdx.z * COLS + c) * 4);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      float to = m[k];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) to = fmaxf(to, ml[k][i].x);
+      const float f = m[k] == to ? 1.f : e4_ex2(m[k] - to);
+      sum[k].x *= f; sum[k].y *= f; sum[k].z *= f; sum[k].w *= f;
+      l[k] *= f;
+      m[k] = to;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (s0 + k * R + i * kChains >= here) break;
+        const float g = ml[k][i].x == to ? 1.f : e4_ex2(ml[k][i].x - to);
+        sum[k].x = fmaf(x[k][i].x, g, sum[k].x);
+        sum[k].y = fmaf(x[k][i].y, g, sum[k].y);
+        sum[k].z = fmaf(x[k][i].z, g, sum[k].z);
+        sum[k].w = fmaf(x[k][i].w, g, sum[k].w);
+        l[k] = fmaf(ml[k][i].y, g, l[k]);
+      }
     }
   }
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     sum_sh[r + k * R][c] = sum[k];
-    if (c == 0) l_sh[r + k * R] = l[k];
+    if (c == 0) ml_sh[r + k * R] = make_float2(m[k], l[k]);
   }
   __syncthreads();
   if (tid >= COLS) return;
   float4 o = sum_sh[0][c];
-  float den = l_sh[0];
+  float top = ml_sh[0].x, den = ml_sh[0].y;
 #pragma unroll
-  for (int k = 1; k < kChains; ++k) {
-    const float4 x = sum_sh[k][c];
-    o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
-    den += l_sh[k];
-  }
+  for (int k = 1; k < kChains; ++k)
+    if (k < here) add(o, top, den, sum_sh[k][c], ml_sh[k].x, ml_sh[k].y);
   if (here > 1) {
     const float inv = 1.f / den;
     e4_put(out + c * 4, o.x * inv);
@@ -572,7 +601,7 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
     // a weight is 2^(s - m) / den = 2^(s - (m + x)) / (den / 2^x), with the x that brings den / 2^x into [1, 2)
     const int x = static_cast<int>(__float_as_uint(den) >> 23) - 127;
     float* norm = e4_norm(a.scratch, a.batch, a.heads, slices, D, b, h);
-    norm[0] = m + static_cast<float>(x);
+    norm[0] = top + static_cast<float>(x);
     norm[1] = e4_two(x) / den;
   }
 }
