@@ -48,16 +48,29 @@ e4_append_kernel(const RbE4m3AppendArgs a, int per_cta RB_BOUNDS_PARAM) {
       continue;
     }
     const T* src = rows + r0 * ld + static_cast<long long>(h) * D + c_lane;
-    float most = 0.f;
-    for (int i = r_lane; i < n; i += RPW) {
-      float x[8];
-      E4Row<T>::load(src + i * ld, x);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) most = fmaxf(most, e4_finite_abs(x[j]));
-    }
     const long long tile = static_cast<long long>(page) * G + h;
-    int e = e4_exponent(warp_max(most));
     uint8_t* dst = codes + tile * bs * D;
+    // up to 16 rows stay in registers between the search for their largest number and their rounding; of pages with more the rows are read again
+    constexpr int kHeld = 16 / RPW;
+    uint4 raw[kHeld][sizeof(T) / 2];
+    float most = 0.f;
+    for (int i0 = 0; i0 < n; i0 += 16) {
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k)
+        if (i0 + k * RPW + r_lane < n) {
+#pragma unroll
+          for (int x = 0; x < static_cast<int>(sizeof(T) / 2); ++x) raw[k][x] = reinterpret_cast<const uint4*>(src + (i0 + k * RPW + r_lane) * ld)[x];
+        }
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k)
+        if (i0 + k * RPW + r_lane < n) {
+          float x[8];
+          E4Row<T>::load(reinterpret_cast<const T*>(raw[k]), x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) most = fmaxf(most, e4_finite_abs(x[j]));
+        }
+    }
+    int e = e4_exponent(warp_max(most));
     if (off > 0) {
       const int had = exps[tile];
       if (had >= e) e = had;
@@ -69,13 +82,18 @@ e4_append_kernel(const RbE4m3AppendArgs a, int per_cta RB_BOUNDS_PARAM) {
         }
     }
     const float down = e4_two(-e);
-    for (int i = r_lane; i < n; i += RPW) {
-      float x[8];
-      E4Row<T>::load(src + i * ld, x);
-      uint2 u;
-      u.x = e4_pack2(x[0] * down, x[1] * down) | e4_pack2(x[2] * down, x[3] * down) << 16;
-      u.y = e4_pack2(x[4] * down, x[5] * down) | e4_pack2(x[6] * down, x[7] * down) << 16;
-      *reinterpret_cast<uint2*>(dst + (off + i) * D + c_lane) = u;
+    for (int i0 = 0; i0 < n; i0 += 16) {
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) {
+        const int i = i0 + k * RPW + r_lane;
+        if (i >= n) continue;
+        float x[8];
+        E4Row<T>::load(n > 16 ? src + i * ld : reinterpret_cast<const T*>(raw[k]), x);
+        uint2 u;
+        u.x = e4_pack2(x[0] * down, x[1] * down) | e4_pack2(x[2] * down, x[3] * down) << 16;
+        u.y = e4_pack2(x[4] * down, x[5] * down) | e4_pack2(x[6] * down, x[7] * down) << 16;
+        *reinterpret_cast<uint2*>(dst + (off + i) * D + c_lane) = u;
+      }
     }
     __syncwarp();                                                      // every lane has the old exponent
     if (lane == 0) exps[tile] = static_cast<signed char>(e);
@@ -84,51 +102,70 @@ e4_append_kernel(const RbE4m3AppendArgs a, int per_cta RB_BOUNDS_PARAM) {
   }
 }
 
-constexpr int kE4ReadRows = 16;
+constexpr int kE4ReadRows = 32;
 
-template <typename T>
+// A CTA takes 32 rows; a warp reads 512 bytes of codes at a time, neighbouring rows of one head, 16 bytes a lane, four such reads in flight.
+template <typename T, int D>
 __global__ void __launch_bounds__(256)
 e4_read_kernel(const RbE4m3ReadArgs a RB_BOUNDS_PARAM) {
   pdl_wait();
   pdl_launch();
-  __shared__ long long slot[kE4ReadRows];            // page * block_size + offset, -1: no position
-  const int G = a.pages.kv_heads, bs = a.pages.block_size, D = a.pages.head_dim;
+  constexpr int LPR = D / 16, RPW = 32 / LPR;        // lanes for a row, rows for a warp
+  constexpr int kSteps = kE4ReadRows / RPW;          // reads for the rows' part of one head
+  __shared__ int page_sh[kE4ReadRows], off_sh[kE4ReadRows];              // page -1: the row has no position
+  const int G = a.pages.kv_heads, bs = a.pages.block_size, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long r0 = static_cast<long long>(blockIdx.x) * kE4ReadRows;
   if (threadIdx.x < kE4ReadRows) {
     const long long r = r0 + threadIdx.x;
-    long long at = -1;
+    int page = -1, off = 0;
     if (r < a.rows && r < a.row_starts[a.batch] && r >= a.row_starts[0]) {
       const int b = e4_sequence_of(a.row_starts, a.batch, static_cast<int>(r));
       const int i = static_cast<int>(r) - a.row_starts[b];
       if (i < a.context_lens[b]) {
-        const int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, i / bs);
+        page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, i / bs);
         if (page < 0) RB_BOUNDS_HIT(104);
-        else at = static_cast<long long>(page) * bs + i % bs;
+        off = i % bs;
       }
     }
-    slot[threadIdx.x] = at;
+    page_sh[threadIdx.x] = page;
+    off_sh[threadIdx.x] = off;
   }
   __syncthreads();
-  const int pieces = G * D / 8;                      // of eight numbers
-  for (int i = threadIdx.x; i < 2 * kE4ReadRows * pieces; i += blockDim.x) {
-    const int row = i / (2 * pieces), rest = i - row * 2 * pieces, values = rest >= pieces, c = (rest - values * pieces) * 8;
-    const long long at = slot[row];
-    if (at < 0) continue;
-    const long long page = at / bs, off = at - page * bs;
-    const long long tile = page * G + c / D;
-    const uint8_t* codes = reinterpret_cast<const uint8_t*>(values ? a.pages.v : a.pages.k) + (tile * bs + off) * D + c % D;
-    const float up = e4_two((values ? a.pages.v_exp : a.pages.k_exp)[tile]);
-    const uint2 u = *reinterpret_cast<const uint2*>(codes);
-    float x[8];
-    const uint32_t w[2] = {u.x, u.y};
+  const int r_lane = lane / LPR, c_lane = lane % LPR * 16;
+  for (int unit = warp; unit < 2 * G * (kSteps / 4); unit += 8) {        // four reads each: keys' heads, then values'
+    const int values = unit >= G * (kSteps / 4), in = values ? unit - G * (kSteps / 4) : unit, h = in / (kSteps / 4), step = in % (kSteps / 4) * 4;
+    const uint8_t* codes = reinterpret_cast<const uint8_t*>(values ? a.pages.v : a.pages.k);
+    const signed char* exps = values ? a.pages.v_exp : a.pages.k_exp;
+    uint4 u[4];
+    int e[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = e4_float2(w[j >> 1] >> (16 * (j & 1)));
-      x[2 * j] = f.x * up;
-      x[2 * j + 1] = f.y * up;
+    for (int k = 0; k < 4; ++k) {
+      const int r = (step + k) * RPW + r_lane, page = page_sh[r];
+      if (page < 0) continue;
+      const long long tile = static_cast<long long>(page) * G + h;
+      e[k] = exps[tile];
+      u[k] = *reinterpret_cast<const uint4*>(codes + (tile * bs + off_sh[r]) * D + c_lane);
     }
-    T* out = reinterpret_cast<T*>(values ? a.v_out : a.k_out) + (r0 + row) * (values ? a.ld_v : a.ld_k) + c;
-    E4Row<T>::store(out, x);
+    T* out = reinterpret_cast<T*>(values ? a.v_out : a.k_out) + static_cast<long long>(h) * D + c_lane;
+    const long long ld = values ? a.ld_v : a.ld_k;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = (step + k) * RPW + r_lane;
+      if (page_sh[r] < 0) continue;
+      const float up = e4_two(e[k]);
+      const uint32_t w[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = e4_float2(w[p * 2 + (j >> 1)] >> (16 * (j & 1)));
+          x[2 * j] = f.x * up;
+          x[2 * j + 1] = f.y * up;
+        }
+        E4Row<T>::store(out + (r0 + r) * ld + p * 8, x);
+      }
+    }
   }
 }
 
@@ -141,6 +178,12 @@ int append_by_dim(const RbE4m3AppendArgs& a, cudaStream_t s) {
   const dim3 grid((a.rows + per_cta - 1) / per_cta, a.pages.kv_heads);
   auto kern = a.pages.head_dim == 64 ? rb::e4_append_kernel<T, 64> : rb::e4_append_kernel<T, 128>;
   return static_cast<int>(rbhost::launch_pdl(kern, grid, dim3(rb::kE4AppendThreads), 0, s, 1, a, per_cta RB_BOUNDS_ARG));
+}
+template <typename T>
+int read_by_dim(const RbE4m3ReadArgs& a, cudaStream_t s) {
+  auto kern = a.pages.head_dim == 64 ? rb::e4_read_kernel<T, 64> : rb::e4_read_kernel<T, 128>;
+  const dim3 grid((a.rows + rb::kE4ReadRows - 1) / rb::kE4ReadRows);
+  return static_cast<int>(rbhost::launch_pdl(kern, grid, dim3(256), 0, s, 1, a RB_BOUNDS_ARG));
 }
 template <typename A>
 bool rows_fit(const A& a, const void* k, const void* v) {
@@ -171,12 +214,11 @@ RB_API int rb_e4m3_read(const RbE4m3ReadArgs* args, void* stream_v) {
   if (const int bad = rbhost::e4_check(a.pages)) return bad;
   if (!a.k_out || !a.v_out || !a.block_tables || !a.context_lens || !a.row_starts || a.max_blocks <= 0) return -1;
   if (!rows_fit(a, a.k_out, a.v_out)) return -2;
-  const dim3 grid((a.rows + rb::kE4ReadRows - 1) / rb::kE4ReadRows);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_v);
   switch (a.type) {
-    case RB_E4M3_BF16: return static_cast<int>(rbhost::launch_pdl(rb::e4_read_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, 1, a RB_BOUNDS_ARG));
-    case RB_E4M3_F16: return static_cast<int>(rbhost::launch_pdl(rb::e4_read_kernel<__half>, grid, dim3(256), 0, s, 1, a RB_BOUNDS_ARG));
-    case RB_E4M3_F32: return static_cast<int>(rbhost::launch_pdl(rb::e4_read_kernel<float>, grid, dim3(256), 0, s, 1, a RB_BOUNDS_ARG));
+    case RB_E4M3_BF16: return read_by_dim<__nv_bfloat16>(a, s);
+    case RB_E4M3_F16: return read_by_dim<__half>(a, s);
+    case RB_E4M3_F32: return read_by_dim<float>(a, s);
   }
   return -1;
 }

@@ -1,10 +1,16 @@
 // Eviction from a paged cache in e4m3: which tokens of a sequence stay, by their attention weight, and their move to the front.
+#include <cooperative_groups.h>
+
 #include "pdl.cuh"
 #include "paged_e4m3.cuh"
 
 namespace rb {
 
-constexpr int kE4SelectThreads = 1024;
+namespace cg = cooperative_groups;
+
+constexpr int kE4SelectThreads = 1024, kE4SelectWarps = 32;
+constexpr int kE4SelectShare = 16384;                // tokens that a CTA of a cluster is meant for
+constexpr int kE4SelectKeys = 49152;                 // and those that its shared memory has room for
 
 // order-preserving: larger weights have larger keys, -0 is 0, a NaN is largest
 __device__ __forceinline__ uint32_t e4_key(float w) {
@@ -13,177 +19,301 @@ __device__ __forceinline__ uint32_t e4_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// A CTA for a sequence and KV head: the `take`-th largest key of the tokens that may go, by radix selection in four passes of eight bits, then
-// the places that stay, in order.
+// The places that stay, for a sequence and KV head.  The `take`-th largest key of the tokens that may go is found by radix selection, four passes of
+// eight bits over keys in shared memory; every pass counts the next digit of the keys that still may be it.  Then each warp counts what stays of its tokens,
+// and writes it where the counts in front of it end.  Sequences of many tokens are shared by the CTAs of a cluster (x: rank in the cluster), which
+// add their counts through distributed shared memory.
+// One B200, 24 sequences of 1500 to 8192 tokens, 8 KV heads: 94 us with one thread that looks for the digit and keys read from the pages in every pass.
+template <bool CLUSTER>
 __global__ void __launch_bounds__(kE4SelectThreads)
-e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
+e4_select_kernel(const RbE4m3EvictArgs a, int room RB_BOUNDS_PARAM) {
   pdl_wait();
   pdl_launch();
-  __shared__ uint32_t hist[256], warp_n[2][32];
-  __shared__ uint32_t s_digit, s_need;
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int bs = a.pages.block_size, G = a.pages.kv_heads;
+  extern __shared__ uint32_t e4_keys[];              // [room]
+  __shared__ uint32_t hist[256], part[2], digit[2];
+  __shared__ uint32_t warp_n[2][kE4SelectWarps];
+  const int ranks = CLUSTER ? gridDim.x : 1, rank = CLUSTER ? blockIdx.x : 0;
+  const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int bs = a.pages.block_size, G = a.pages.kv_heads, per_page = bs >> 4;
   const int n = static_cast<int>(max(0ll, min(static_cast<long long>(a.context_lens[b]), static_cast<long long>(a.max_blocks) * bs)));
   int* kept = a.kept + (static_cast<long long>(b) * G + h) * a.keep;
-  if (h == 0 && tid == 0) a.lens_out[b] = min(n, a.keep);
-  if (n <= a.keep) {
-    for (int j = tid; j < a.keep; j += kE4SelectThreads) kept[j] = j < n ? j : -1;
+  if (h == 0 && rank == 0 && tid == 0) a.lens_out[b] = min(n, a.keep);
+  if (n <= a.keep) {                                 // all CTAs of a cluster alike
+    for (int j = rank * kE4SelectThreads + tid; j < a.keep; j += ranks * kE4SelectThreads) kept[j] = j < n ? j : -1;
     return;
   }
-  const int lo = a.keep_first, hi = n - a.recent;    // tokens that may go
   const uint32_t take = a.keep - a.keep_first - a.recent;
-  auto key = [&](int t) {
-    const int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, t / bs);
-    if (page < 0) {
+  for (int j = rank * kE4SelectThreads + tid; j < a.keep_first; j += ranks * kE4SelectThreads) kept[j] = j;
+  for (int j = rank * kE4SelectThreads + tid; j < a.recent; j += ranks * kE4SelectThreads) kept[a.keep - a.recent + j] = n - a.recent + j;
+  if (take == 0) return;
+  // this CTA's tokens among those that may go: [lo, hi), of which a warp has `span` at a time
+  const int first = a.keep_first, count = n - a.recent - first, share = ((count + ranks - 1) / ranks + 31) & ~31;
+  const int lo = first + min(count, rank * share), hi = first + min(count, (rank + 1) * share), mine = hi - lo;
+  const int* table = a.block_tables + static_cast<long long>(b) * a.max_blocks;
+  auto from_page = [&](int t) {
+    const int i = per_page == 1 ? t >> 4 : t / bs, off = per_page == 1 ? t & 15 : t - i * bs;
+    const int page = table[i];
+    if (page < 0 || page >= a.pages.num_blocks) {
       RB_BOUNDS_HIT(104);
       return 0u;
     }
-    return e4_key(a.pages.weight[(static_cast<long long>(page) * G + h) * bs + t % bs]);
+    return e4_key(a.pages.weight[(static_cast<long long>(page) * G + h) * bs + off]);
   };
+  const bool here = mine <= room;
+  if (here) {
+#pragma unroll 4
+    for (int i = tid; i < mine; i += kE4SelectThreads) e4_keys[i] = from_page(lo + i);
+  }
+  auto key = [&](int i) { return here ? e4_keys[i] : from_page(lo + i); };
   uint32_t prefix = 0, mask = 0, need = take;        // keys that begin with `prefix`; how many of them stay
-  for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
+#pragma unroll 1
+  for (int shift = 24; shift >= 0; shift -= 8) {
     if (tid < 256) hist[tid] = 0;
     __syncthreads();
-    for (int t = lo + tid; t < hi; t += kE4SelectThreads) {
-      const uint32_t k = key(t);
+    for (int i = tid; i < mine; i += kE4SelectThreads) {
+      const uint32_t k = key(i);
       if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
     }
-    __syncthreads();
-    if (tid == 0) {
-      uint32_t above = 0;
-      int d = 255;
-      for (; d > 0 && above + hist[d] < need; --d) above += hist[d];
-      s_digit = d;
-      s_need = need - above;
+    if (CLUSTER) cg::this_cluster().sync();
+    else __syncthreads();
+    if (warp == 0) {                                 // lane i: digits 255 - 8 i downwards
+      uint32_t c[8], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        c[j] = hist[255 - lane * 8 - j];
+        if (CLUSTER) {
+          for (int r = 1; r < ranks; ++r) c[j] += *cg::this_cluster().map_shared_rank(&hist[255 - lane * 8 - j], (rank + r) % ranks);
+        }
+        sum += c[j];
+      }
+      uint32_t upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      uint32_t above = upto - sum;
+      if (above < need && need <= upto) {            // one lane
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (above < need && need <= above + c[j]) {
+            digit[0] = 255 - lane * 8 - j;
+            digit[1] = need - above;
+          }
+          above += c[j];
+        }
+      }
     }
-    __syncthreads();
-    prefix |= s_digit << shift;
+    if (CLUSTER) cg::this_cluster().sync();          // and nobody reads another's counts any more
+    else __syncthreads();
+    prefix |= digit[0] << shift;
     mask |= 255u << shift;
-    need = s_need;
+    need = digit[1];
   }
-  // keys above `prefix` stay, and the first `need` of those equal to it
-  uint32_t placed = a.keep_first, equal = 0;
-  for (int j = tid; j < a.keep_first; j += kE4SelectThreads) kept[j] = j;
-  for (int j = tid; j < a.recent; j += kE4SelectThreads) kept[a.keep - a.recent + j] = hi + j;
-  if (take > 0)
-    for (int t0 = lo; t0 < hi; t0 += kE4SelectThreads) {
-      const int t = t0 + tid;
-      const uint32_t k = t < hi ? key(t) : 0u;
-      const bool is_equal = t < hi && k == prefix;
-      const uint32_t eq = __ballot_sync(0xffffffffu, is_equal);
-      if (lane == 0) warp_n[0][warp] = __popc(eq);
-      __syncthreads();
-      uint32_t before = equal + __popc(eq & ((1u << lane) - 1));
-      for (int w = 0; w < 32; ++w) {
-        if (w < warp) before += warp_n[0][w];
-        equal += warp_n[0][w];
-      }
-      const bool stays = t < hi && (k > prefix || (is_equal && before < need));
-      const uint32_t st = __ballot_sync(0xffffffffu, stays);
-      if (lane == 0) warp_n[1][warp] = __popc(st);
-      __syncthreads();
-      uint32_t at = placed + __popc(st & ((1u << lane) - 1));
-      for (int w = 0; w < 32; ++w) {
-        if (w < warp) at += warp_n[1][w];
-        placed += warp_n[1][w];
-      }
-      if (stays && at < static_cast<uint32_t>(a.keep)) kept[at] = t;
+  // keys above `prefix` stay, and of those equal to it the first `need`
+  const int span = ((mine + kE4SelectThreads - 1) / kE4SelectThreads) * 32, w0 = warp * span, w1 = min(mine, w0 + span);
+  uint32_t above = 0, equal = 0;                     // of this warp
+  for (int i0 = w0; i0 < w1; i0 += 32) {
+    const uint32_t k = i0 + lane < w1 ? key(i0 + lane) : 0u;
+    above += __popc(__ballot_sync(0xffffffffu, i0 + lane < w1 && k > prefix));
+    equal += __popc(__ballot_sync(0xffffffffu, i0 + lane < w1 && k == prefix));
+  }
+  if (lane == 0) {
+    warp_n[0][warp] = above;
+    warp_n[1][warp] = equal;
+  }
+  __syncthreads();
+  uint32_t before[2];                                // keys above and equal in the warps in front
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const uint32_t v = warp_n[x][lane], all = __reduce_add_sync(0xffffffffu, v);
+    before[x] = __reduce_add_sync(0xffffffffu, lane < warp ? v : 0u);
+    if (CLUSTER && tid == 0) part[x] = all;
+  }
+  if (CLUSTER) {
+    cg::this_cluster().sync();
+    for (int r = 0; r < rank; ++r) {
+      before[0] += *cg::this_cluster().map_shared_rank(&part[0], r);
+      before[1] += *cg::this_cluster().map_shared_rank(&part[1], r);
     }
+  }
+  for (int i0 = w0; i0 < w1; i0 += 32) {
+    const uint32_t k = i0 + lane < w1 ? key(i0 + lane) : 0u;
+    const uint32_t gt = __ballot_sync(0xffffffffu, i0 + lane < w1 && k > prefix), eq = __ballot_sync(0xffffffffu, i0 + lane < w1 && k == prefix);
+    const uint32_t in_front = (1u << lane) - 1;
+    const uint32_t equals = before[1] + __popc(eq & in_front);           // equal ones in front of this token
+    const uint32_t at = first + before[0] + __popc(gt & in_front) + min(equals, need);
+    if (((gt >> lane) & 1 || ((eq >> lane) & 1 && equals < need)) && at < static_cast<uint32_t>(a.keep)) kept[at] = lo + i0 + lane;
+    before[0] += __popc(gt);
+    before[1] += __popc(eq);
+  }
+  if (CLUSTER) cg::this_cluster().sync();            // others may still read this CTA's counts
 }
 
-// A CTA for a sequence and KV head, page after page: a token moves to a place in front of its own or to its own, so that what later pages take has not
-// been written yet.
-__global__ void __launch_bounds__(256)
+constexpr int kE4MoveThreads = 256, kE4MoveTokens = 128;
+
+// Moves the kept tokens of a sequence and KV head.  A CTA takes whole pages, as many as have at most 128 tokens (or one that has more, in parts).
+// INPLACE: the CTAs of a cluster take neighbouring runs of pages and go on together.  A token moves to a place in front of its own, or stays, so what
+// one round writes lies in front of all that later rounds read; within a round all tokens are in registers before the first is written.  Pages of more
+// than 128 tokens are taken by one CTA, where the same holds from part to part.  Otherwise the pages are of no other use and the grid has a CTA for
+// each run of pages.
+template <int D, bool INPLACE>
+__global__ void __launch_bounds__(kE4MoveThreads)
 e4_move_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
   pdl_wait();
   pdl_launch();
-  __shared__ int src_sh[256];                        // page of each token of a run of a page, and slot in it
-  __shared__ short off_sh[256];
-  __shared__ int exp_sh[2][256];
-  __shared__ int top_sh[2];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const int bs = a.pages.block_size, G = a.pages.kv_heads, D = a.pages.head_dim;
+  constexpr int kPieces = D / 16, kRows = kE4MoveThreads / kPieces, kPer = kE4MoveTokens / kRows;     // a thread has kPer pieces of keys and of values
+  __shared__ long long row_sh[kE4MoveTokens];        // where a token comes from, in rows of D codes
+  __shared__ int exp_sh[2][kE4MoveTokens], top_sh[2][kE4MoveTokens / 16], still_sh;
+  const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int bs = a.pages.block_size, G = a.pages.kv_heads;
   const int n = a.lens_out[b];
+  if (INPLACE && static_cast<long long>(a.context_lens[b]) <= a.keep) return;           // a whole cluster
   const int* kept = a.kept + (static_cast<long long>(b) * G + h) * a.keep;
-  if (!a.out_tables && static_cast<long long>(a.context_lens[b]) <= a.keep) return;
-  const int* to_tables = a.out_tables ? a.out_tables : a.block_tables;
-  const int to_blocks = a.out_tables ? a.out_blocks : a.max_blocks;
-  for (int j0 = 0; j0 < n; j0 += bs) {
-    const int m = min(bs, n - j0);
-    const int to = e4_page(to_tables, to_blocks, a.pages.num_blocks, b, j0 / bs);
-    __syncthreads();
-    if (tid < 2) top_sh[tid] = -128;
-    __syncthreads();
-    for (int i = tid; i < m; i += 256) {
-      const int t = kept[j0 + i];
-      int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, t / bs);
-      if (page < 0) {
-        RB_BOUNDS_HIT(104);
-        page = 0;
-      }
-      const long long tile = static_cast<long long>(page) * G + h;
-      atomicMax(&top_sh[0], static_cast<int>(a.pages.k_exp[tile]));
-      atomicMax(&top_sh[1], static_cast<int>(a.pages.v_exp[tile]));
-    }
-    __syncthreads();
-    const int top_k = top_sh[0], top_v = top_sh[1];
-    const long long tile_to = static_cast<long long>(to < 0 ? 0 : to) * G + h;
-    for (int i0 = 0; i0 < m; i0 += 16) {
-      const int rows = min(16, m - i0);
+  const int* from = a.block_tables + static_cast<long long>(b) * a.max_blocks;
+  const int* to_tables = INPLACE ? a.block_tables : a.out_tables;
+  const int to_blocks = INPLACE ? a.max_blocks : a.out_blocks;
+  const int run = bs >= kE4MoveTokens ? bs : kE4MoveTokens / bs * bs;  // tokens of a CTA's run of pages
+  for (int j0 = blockIdx.x * run; INPLACE ? j0 - static_cast<int>(blockIdx.x) * run < n : j0 < n; j0 += gridDim.x * run) {
+    // exponents of the run's pages: the largest of their tokens'
+    const int m = min(run, n - j0);                  // not positive: this CTA only keeps its cluster company
+    int top_k = -128, top_v = -128;                  // of a page that is taken in parts
+    for (int part = 0; part < run; part += kE4MoveTokens) {
+      const int here = min(kE4MoveTokens, m - part);
+      __syncthreads();
+      if (tid < 2 * (kE4MoveTokens / 16)) (&top_sh[0][0])[tid] = -128;
+      if (tid == 0) still_sh = 1;
       __syncthreads();
       float w = 0.f;
-      if (tid < rows) {
-        const int t = kept[j0 + i0 + tid];
-        const int page = max(0, e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, t / bs));
-        const long long tile = static_cast<long long>(page) * G + h;
-        src_sh[tid] = page;
-        off_sh[tid] = static_cast<short>(t % bs);
-        exp_sh[0][tid] = a.pages.k_exp[tile];
-        exp_sh[1][tid] = a.pages.v_exp[tile];
-        if (a.pages.weight) w = a.pages.weight[tile * bs + t % bs];
-      }
-      __syncthreads();
-      const int per = D / 16;                        // pieces of a row
-      const int piece = tid % per, row = tid / per % 16, values = tid / (16 * per);
-      uint4 u = make_uint4(0, 0, 0, 0);
-      const bool mine = values < 2 && row < rows;
-      if (mine) {
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(values ? a.pages.v : a.pages.k);
-        u = *reinterpret_cast<const uint4*>(src + ((static_cast<long long>(src_sh[row]) * G + h) * bs + off_sh[row]) * D + piece * 16);
-        const int up = (values ? top_v : top_k) - exp_sh[values][row];
-        if (up > 0) u = make_uint4(e4_lower4(u.x, up), e4_lower4(u.y, up), e4_lower4(u.z, up), e4_lower4(u.w, up));
-      }
-      __syncthreads();
-      if (to >= 0) {
-        if (mine) {
-          uint8_t* dst = reinterpret_cast<uint8_t*>(values ? a.pages.v : a.pages.k);
-          *reinterpret_cast<uint4*>(dst + (tile_to * bs + i0 + row) * D + piece * 16) = u;
+      if (tid < here) {
+        const int j = j0 + part + tid, t = kept[j];
+        int page = from[t / bs];
+        if (page < 0 || page >= a.pages.num_blocks) {
+          RB_BOUNDS_HIT(104);
+          page = 0;
         }
-        if (tid < rows && a.pages.weight) a.pages.weight[tile_to * bs + i0 + tid] = w;
-      } else if (tid == 0) {
-        RB_BOUNDS_HIT(104);
+        const long long tile = static_cast<long long>(page) * G + h;
+        const int ek = a.pages.k_exp[tile], ev = a.pages.v_exp[tile];
+        row_sh[tid] = tile * bs + t % bs;
+        exp_sh[0][tid] = ek;
+        exp_sh[1][tid] = ev;
+        w = a.pages.weight[tile * bs + t % bs];
+        if (run <= kE4MoveTokens) {
+          atomicMax(&top_sh[0][tid / bs], ek);
+          atomicMax(&top_sh[1][tid / bs], ev);
+        }
+        if (t != j) still_sh = 0;
       }
-    }
-    __syncthreads();
-    if (tid == 0 && to >= 0) {
-      a.pages.k_exp[tile_to] = static_cast<signed char>(top_k);
-      a.pages.v_exp[tile_to] = static_cast<signed char>(top_v);
+      if (run > kE4MoveTokens && part == 0) {        // a page of many tokens: its exponents first
+        for (int i = tid; i < m; i += kE4MoveThreads) {
+          const int page = from[kept[j0 + i] / bs];
+          const long long tile = static_cast<long long>(page < 0 || page >= a.pages.num_blocks ? 0 : page) * G + h;
+          top_k = max(top_k, static_cast<int>(a.pages.k_exp[tile]));
+          top_v = max(top_v, static_cast<int>(a.pages.v_exp[tile]));
+        }
+        top_k = __reduce_max_sync(0xffffffffu, top_k);
+        top_v = __reduce_max_sync(0xffffffffu, top_v);
+        if ((tid & 31) == 0) {
+          atomicMax(&top_sh[0][0], top_k);
+          atomicMax(&top_sh[1][0], top_v);
+        }
+        __syncthreads();
+        top_k = top_sh[0][0];
+        top_v = top_sh[1][0];
+      }
+      __syncthreads();
+      const bool moves = here > 0 && !(INPLACE && still_sh && run <= kE4MoveTokens);    // tokens that all keep their places stay as they are
+      const int piece = tid % kPieces, r0 = tid / kPieces;
+      uint4 u[2][kPer];
+      if (moves) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint8_t* src = reinterpret_cast<const uint8_t*>(x ? a.pages.v : a.pages.k);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const int r = r0 + i * kRows;
+            if (r < here) u[x][i] = *reinterpret_cast<const uint4*>(src + row_sh[r] * D + piece * 16);
+          }
+        }
+      }
+      // everything of this round is in registers
+      if (INPLACE && gridDim.x > 1) cg::this_cluster().sync();
+      else if (INPLACE) __syncthreads();
+      if (!moves) continue;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint8_t* dst = reinterpret_cast<uint8_t*>(x ? a.pages.v : a.pages.k);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int r = r0 + i * kRows;
+          if (r >= here) continue;
+          const int j = j0 + part + r, pi = j / bs;
+          const int page = pi < to_blocks ? to_tables[static_cast<long long>(b) * to_blocks + pi] : -1;
+          if (page < 0 || page >= a.pages.num_blocks) {
+            RB_BOUNDS_HIT(104);
+            continue;
+          }
+          const int top = run > kE4MoveTokens ? (x ? top_v : top_k) : top_sh[x][r / bs];
+          const int up = top - exp_sh[x][r];
+          uint4 c = u[x][i];
+          if (up > 0) c = make_uint4(e4_lower4(c.x, up), e4_lower4(c.y, up), e4_lower4(c.z, up), e4_lower4(c.w, up));
+          const long long tile = static_cast<long long>(page) * G + h;
+          *reinterpret_cast<uint4*>(dst + (tile * bs + j - pi * bs) * D + piece * 16) = c;
+          // the page's exponent with its last token: tokens of a page that is taken in parts are read under the old one until then
+          if (piece == 0 && (j - pi * bs == bs - 1 || j == n - 1)) (x ? a.pages.v_exp : a.pages.k_exp)[tile] = static_cast<signed char>(top);
+        }
+      }
+      if (tid < here) {
+        const int j = j0 + part + tid, pi = j / bs;
+        const int page = pi < to_blocks ? to_tables[static_cast<long long>(b) * to_blocks + pi] : -1;
+        if (page >= 0 && page < a.pages.num_blocks) a.pages.weight[(static_cast<long long>(page) * G + h) * bs + j - pi * bs] = w;
+      }
     }
   }
 }
 
 }  // namespace rb
 
+namespace {
+template <int D>
+cudaError_t move_tokens(const RbE4m3EvictArgs& a, cudaStream_t s) {
+  const int bs = a.pages.block_size, run = bs >= rb::kE4MoveTokens ? bs : rb::kE4MoveTokens / bs * bs;
+  if (a.out_tables)
+    return rbhost::launch_pdl(rb::e4_move_kernel<D, false>, dim3((a.keep + run - 1) / run, a.pages.kv_heads, a.batch), dim3(rb::kE4MoveThreads), 0, s, 1,
+                              a RB_BOUNDS_ARG);
+  // as many CTAs for a sequence and head as the GPU has room for, four on an SM
+  int cluster = 1;
+  while (cluster < 8 && run <= rb::kE4MoveTokens && cluster * run < a.keep &&
+         2ll * cluster * a.pages.kv_heads * a.batch <= 4ll * rbhost::device_sm_count())
+    cluster *= 2;
+  return rbhost::launch_pdl(rb::e4_move_kernel<D, true>, dim3(cluster, a.pages.kv_heads, a.batch), dim3(rb::kE4MoveThreads), 0, s, cluster, a RB_BOUNDS_ARG);
+}
+}  // namespace
+
 RB_API int rb_e4m3_evict(const RbE4m3EvictArgs* args, void* stream_v) {
   const RbE4m3EvictArgs& a = *args;
   if (a.batch <= 0) return 0;
   if (const int bad = rbhost::e4_check(a.pages)) return bad;
+  const long long tokens = static_cast<long long>(a.max_blocks) * a.pages.block_size;   // that a sequence can have
   if (!a.pages.weight || !a.block_tables || !a.context_lens || !a.kept || !a.lens_out || a.max_blocks <= 0 || (a.out_tables && a.out_blocks <= 0) || a.keep <= 0 ||
-      a.recent < 0 || a.keep_first < 0 || static_cast<long long>(a.recent) + a.keep_first > a.keep || a.batch > 65535 || a.pages.block_size > 32768)
+      a.recent < 0 || a.keep_first < 0 || static_cast<long long>(a.recent) + a.keep_first > a.keep || a.batch > 65535 || a.pages.kv_heads > 65535 ||
+      tokens > 0x3fffffff || a.keep > 0x3fffffff)
     return -1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_v);
-  const dim3 grid(a.pages.kv_heads, a.batch);
-  cudaError_t e = rbhost::launch_pdl(rb::e4_select_kernel, grid, dim3(rb::kE4SelectThreads), 0, s, 1, a RB_BOUNDS_ARG);
-  if (e == cudaSuccess) e = rbhost::launch_pdl(rb::e4_move_kernel, grid, dim3(256), 0, s, 1, a RB_BOUNDS_ARG);
+  int cluster = 1;
+  while (cluster < 8 && static_cast<long long>(cluster) * rb::kE4SelectShare < tokens) cluster *= 2;
+  long long room = (tokens + cluster - 1) / cluster + 32;
+  if (room > rb::kE4SelectKeys) room = rb::kE4SelectKeys;
+  static bool set[64] = {};
+  const int dev = rbhost::device_slot();
+  if (!set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(rb::e4_select_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, rb::kE4SelectKeys * 4);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(rb::e4_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, rb::kE4SelectKeys * 4);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    set[dev] = true;
+  }
+  cudaError_t e = rbhost::launch_pdl(cluster > 1 ? rb::e4_select_kernel<true> : rb::e4_select_kernel<false>, dim3(cluster, a.pages.kv_heads, a.batch),
+                                     dim3(rb::kE4SelectThreads), static_cast<size_t>(room) * 4, s, cluster, a, static_cast<int>(room) RB_BOUNDS_ARG);
+  if (e == cudaSuccess) e = a.pages.head_dim == 64 ? move_tokens<64>(a, s) : move_tokens<128>(a, s);
   return static_cast<int>(e);
 }
