@@ -10,17 +10,18 @@
 
 namespace rb {
 
-constexpr int kE4AppendThreads = 64;                 // a warp for the keys of a tile and one for its values
+constexpr int kE4AppendHeads = 4;                    // of a CTA: a warp for the keys of each and one for its values
 
-// A CTA takes the pages that begin, for this call, within `per_cta` rows, for one KV head: those whose first new token is one of these rows.  A page's
+// A CTA takes the pages that begin, for this call, within `per_cta` rows, for four KV heads: those whose first new token is one of these rows.  A page's
 // tokens may lie in the next CTA's rows too.
 template <typename T, int D>
-__global__ void __launch_bounds__(kE4AppendThreads)
+__global__ void __launch_bounds__(kE4AppendHeads * 64)
 e4_append_kernel(const RbE4m3AppendArgs a, int per_cta RB_BOUNDS_PARAM) {
   pdl_wait();
   pdl_launch();
-  const int lane = threadIdx.x & 31, values = threadIdx.x >> 5;        // warp 0: keys, warp 1: values
-  const int G = a.pages.kv_heads, bs = a.pages.block_size, h = blockIdx.y;
+  const int lane = threadIdx.x & 31, values = threadIdx.x >> 5 & 1;    // even warps: keys, odd ones: values
+  const int G = a.pages.kv_heads, bs = a.pages.block_size, h = blockIdx.y * kE4AppendHeads + (threadIdx.x >> 6);
+  if (h >= G) return;
   const T* rows = reinterpret_cast<const T*>(values ? a.v_new : a.k_new);
   const long long ld = values ? a.ld_v : a.ld_k;
   uint8_t* codes = reinterpret_cast<uint8_t*>(values ? a.pages.v : a.pages.k);
@@ -34,13 +35,14 @@ e4_append_kernel(const RbE4m3AppendArgs a, int per_cta RB_BOUNDS_PARAM) {
     const int first = a.row_starts ? a.row_starts[b] : b, last = a.row_starts ? min(a.row_starts[b + 1], a.rows) : b + 1;
     const long long pos = static_cast<long long>(a.context_lens[b]) - (a.row_starts ? a.row_starts[b + 1] : b + 1) + r;
     if (pos < 0) {                                                     // more rows than the sequence has tokens
-      r = min(r - pos, static_cast<long long>(last));
+      r = max(r + 1, min(r - pos, static_cast<long long>(last)));
       continue;
     }
     const int off = static_cast<int>(pos % bs);
     const int n = static_cast<int>(min(static_cast<long long>(bs - off), last - r));
     const long long r0 = r;
-    r += n;
+    r += max(n, 1);                                  // starts that do not ascend end the loop too
+    if (n <= 0) continue;
     if (off != 0 && r0 != first) continue;                             // the page's first new token is an earlier row
     const int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, static_cast<int>(pos / bs));
     if (page < 0) {
@@ -102,24 +104,26 @@ e4_append_kernel(const RbE4m3AppendArgs a, int per_cta RB_BOUNDS_PARAM) {
   }
 }
 
-constexpr int kE4ReadRows = 32;
+constexpr int kE4ReadRows = 16;
 
-// A CTA takes 32 rows; a warp reads 512 bytes of codes at a time, neighbouring rows of one head, 16 bytes a lane, four such reads in flight.
+// A CTA takes 16 rows; a warp reads 512 bytes of codes at a time, neighbouring rows of one head, 16 bytes a lane, four such reads in flight.
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
 e4_read_kernel(const RbE4m3ReadArgs a RB_BOUNDS_PARAM) {
   pdl_wait();
   pdl_launch();
   constexpr int LPR = D / 16, RPW = 32 / LPR;        // lanes for a row, rows for a warp
-  constexpr int kSteps = kE4ReadRows / RPW;          // reads for the rows' part of one head
+  constexpr int kSteps = kE4ReadRows / RPW;          // reads for the rows' part of one head: 4, or 2 of two heads
   __shared__ int page_sh[kE4ReadRows], off_sh[kE4ReadRows];              // page -1: the row has no position
   const int G = a.pages.kv_heads, bs = a.pages.block_size, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long r0 = static_cast<long long>(blockIdx.x) * kE4ReadRows;
-  if (threadIdx.x < kE4ReadRows) {
-    const long long r = r0 + threadIdx.x;
+  if (warp == 0) {
+    const int end = min(a.rows, a.row_starts[a.batch]), b0 = e4_sequence_of(a.row_starts, a.batch, static_cast<int>(r0));
+    const long long r = r0 + lane;
     int page = -1, off = 0;
-    if (r < a.rows && r < a.row_starts[a.batch] && r >= a.row_starts[0]) {
-      const int b = e4_sequence_of(a.row_starts, a.batch, static_cast<int>(r));
+    if (lane < kE4ReadRows && r < end && r >= a.row_starts[0]) {
+      int b = b0;
+      while (a.row_starts[b + 1] <= r) ++b;          // ends: r is in front of the last one
       const int i = static_cast<int>(r) - a.row_starts[b];
       if (i < a.context_lens[b]) {
         page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, i / bs);
@@ -127,31 +131,35 @@ e4_read_kernel(const RbE4m3ReadArgs a RB_BOUNDS_PARAM) {
         off = i % bs;
       }
     }
-    page_sh[threadIdx.x] = page;
-    off_sh[threadIdx.x] = off;
+    if (lane < kE4ReadRows) {
+      page_sh[lane] = page;
+      off_sh[lane] = off;
+    }
   }
   __syncthreads();
   const int r_lane = lane / LPR, c_lane = lane % LPR * 16;
-  for (int unit = warp; unit < 2 * G * (kSteps / 4); unit += 8) {        // four reads each: keys' heads, then values'
-    const int values = unit >= G * (kSteps / 4), in = values ? unit - G * (kSteps / 4) : unit, h = in / (kSteps / 4), step = in % (kSteps / 4) * 4;
+  constexpr int kHeads = 4 / kSteps;                 // of a unit of four reads
+  const int units = (G + kHeads - 1) / kHeads;
+  for (int unit = warp; unit < 2 * units; unit += 8) {
+    const int values = unit >= units, h0 = (values ? unit - units : unit) * kHeads;
     const uint8_t* codes = reinterpret_cast<const uint8_t*>(values ? a.pages.v : a.pages.k);
     const signed char* exps = values ? a.pages.v_exp : a.pages.k_exp;
     uint4 u[4];
     int e[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int r = (step + k) * RPW + r_lane, page = page_sh[r];
-      if (page < 0) continue;
+      const int r = k % kSteps * RPW + r_lane, page = page_sh[r], h = h0 + k / kSteps;
+      if (page < 0 || h >= G) continue;
       const long long tile = static_cast<long long>(page) * G + h;
       e[k] = exps[tile];
       u[k] = *reinterpret_cast<const uint4*>(codes + (tile * bs + off_sh[r]) * D + c_lane);
     }
-    T* out = reinterpret_cast<T*>(values ? a.v_out : a.k_out) + static_cast<long long>(h) * D + c_lane;
+    T* out = reinterpret_cast<T*>(values ? a.v_out : a.k_out) + c_lane;
     const long long ld = values ? a.ld_v : a.ld_k;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int r = (step + k) * RPW + r_lane;
-      if (page_sh[r] < 0) continue;
+      const int r = k % kSteps * RPW + r_lane, h = h0 + k / kSteps;
+      if (page_sh[r] < 0 || h >= G) continue;
       const float up = e4_two(e[k]);
       const uint32_t w[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
 #pragma unroll
@@ -163,7 +171,7 @@ e4_read_kernel(const RbE4m3ReadArgs a RB_BOUNDS_PARAM) {
           x[2 * j] = f.x * up;
           x[2 * j + 1] = f.y * up;
         }
-        E4Row<T>::store(out + (r0 + r) * ld + p * 8, x);
+        E4Row<T>::store(out + (r0 + r) * ld + h * D + p * 8, x);
       }
     }
   }
@@ -175,9 +183,9 @@ namespace {
 template <typename T>
 int append_by_dim(const RbE4m3AppendArgs& a, cudaStream_t s) {
   const int per_cta = a.row_starts ? a.pages.block_size : 1;
-  const dim3 grid((a.rows + per_cta - 1) / per_cta, a.pages.kv_heads);
+  const dim3 grid((a.rows + per_cta - 1) / per_cta, (a.pages.kv_heads + rb::kE4AppendHeads - 1) / rb::kE4AppendHeads);
   auto kern = a.pages.head_dim == 64 ? rb::e4_append_kernel<T, 64> : rb::e4_append_kernel<T, 128>;
-  return static_cast<int>(rbhost::launch_pdl(kern, grid, dim3(rb::kE4AppendThreads), 0, s, 1, a, per_cta RB_BOUNDS_ARG));
+  return static_cast<int>(rbhost::launch_pdl(kern, grid, dim3(rb::kE4AppendHeads * 64), 0, s, 1, a, per_cta RB_BOUNDS_ARG));
 }
 template <typename T>
 int read_by_dim(const RbE4m3ReadArgs& a, cudaStream_t s) {

@@ -60,15 +60,11 @@ __device__ __forceinline__ uint32_t e4_lower4(uint32_t codes, int up) {
 }
 
 // The sequence that row r of rows packed one sequence behind the other belongs to: the last b with starts[b] <= r (sequences without rows are
-// passed over).  r < starts[batch].
+// passed over), found by a whole warp by counting: loads that do not wait for one another.
 __device__ __forceinline__ int e4_sequence_of(const int* __restrict__ starts, int batch, int r) {
-  int lo = 0, hi = batch;                            // starts[lo] <= r < starts[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (starts[mid] <= r) lo = mid;
-    else hi = mid;
-  }
-  return lo;
+  int upto = 0;
+  for (int i = 1 + (threadIdx.x & 31); i < batch; i += 32) upto += starts[i] <= r ? 1 : 0;
+  return __reduce_add_sync(0xffffffffu, upto);
 }
 
 // Page `i` of sequence b, -1 where the table has none or names one that is not there.

@@ -9,8 +9,7 @@ namespace rb {
 namespace cg = cooperative_groups;
 
 constexpr int kE4SelectThreads = 1024, kE4SelectWarps = 32;
-constexpr int kE4SelectShare = 16384;                // tokens that a CTA of a cluster is meant for
-constexpr int kE4SelectKeys = 49152;                 // and those that its shared memory has room for
+constexpr int kE4SelectKeys = 16;                    // keys that a thread holds
 
 // order-preserving: larger weights have larger keys, -0 is 0, a NaN is largest
 __device__ __forceinline__ uint32_t e4_key(float w) {
@@ -20,16 +19,16 @@ __device__ __forceinline__ uint32_t e4_key(float w) {
 }
 
 // The places that stay, for a sequence and KV head.  The `take`-th largest key of the tokens that may go is found by radix selection, four passes of
-// eight bits over keys in shared memory; every pass counts the next digit of the keys that still may be it.  Then each warp counts what stays of its tokens,
-// and writes it where the counts in front of it end.  Sequences of many tokens are shared by the CTAs of a cluster (x: rank in the cluster), which
-// add their counts through distributed shared memory.
-// One B200, 24 sequences of 1500 to 8192 tokens, 8 KV heads: 94 us with one thread that looks for the digit and keys read from the pages in every pass.
+// eight bits over keys in registers; every pass counts the next digit of the keys that still may be it.  Then each warp counts what stays of its tokens,
+// and writes it where the counts in front of it end.  Sequences of more than 16384 tokens are shared by the CTAs of a cluster (x: rank in the cluster),
+// which add their counts through distributed shared memory; behind 131072 the keys are read from the pages again in every pass.
+// Bound by its instructions, not by the weights' bytes.  One B200, 24 sequences of 1500 to 8192 tokens, 8 KV heads: 94 us with one thread that looks
+// for the digit and keys read from the pages in every pass, 25 with keys in shared memory.
 template <bool CLUSTER>
 __global__ void __launch_bounds__(kE4SelectThreads)
-e4_select_kernel(const RbE4m3EvictArgs a, int room RB_BOUNDS_PARAM) {
+e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
   pdl_wait();
   pdl_launch();
-  extern __shared__ uint32_t e4_keys[];              // [room]
   __shared__ uint32_t hist[256], part[2], digit[2];
   __shared__ uint32_t warp_n[2][kE4SelectWarps];
   const int ranks = CLUSTER ? gridDim.x : 1, rank = CLUSTER ? blockIdx.x : 0;
@@ -46,9 +45,10 @@ e4_select_kernel(const RbE4m3EvictArgs a, int room RB_BOUNDS_PARAM) {
   for (int j = rank * kE4SelectThreads + tid; j < a.keep_first; j += ranks * kE4SelectThreads) kept[j] = j;
   for (int j = rank * kE4SelectThreads + tid; j < a.recent; j += ranks * kE4SelectThreads) kept[a.keep - a.recent + j] = n - a.recent + j;
   if (take == 0) return;
-  // this CTA's tokens among those that may go: [lo, hi), of which a warp has `span` at a time
-  const int first = a.keep_first, count = n - a.recent - first, share = ((count + ranks - 1) / ranks + 31) & ~31;
-  const int lo = first + min(count, rank * share), hi = first + min(count, (rank + 1) * share), mine = hi - lo;
+  // this CTA's tokens among those that may go, `mine` from `lo` on, of which a warp has `span` one behind the other
+  const int first = a.keep_first, count = n - a.recent - first, share = (count + ranks - 1) / ranks;
+  const int lo = first + min(count, rank * share), mine = first + min(count, (rank + 1) * share) - lo;
+  const int span = (mine + kE4SelectThreads - 1) / kE4SelectThreads * 32, w0 = warp * span, w1 = min(mine, w0 + span);
   const int* table = a.block_tables + static_cast<long long>(b) * a.max_blocks;
   auto from_page = [&](int t) {
     const int i = per_page == 1 ? t >> 4 : t / bs, off = per_page == 1 ? t & 15 : t - i * bs;
@@ -59,21 +59,34 @@ e4_select_kernel(const RbE4m3EvictArgs a, int room RB_BOUNDS_PARAM) {
     }
     return e4_key(a.pages.weight[(static_cast<long long>(page) * G + h) * bs + off]);
   };
-  const bool here = mine <= room;
-  if (here) {
-#pragma unroll 4
-    for (int i = tid; i < mine; i += kE4SelectThreads) e4_keys[i] = from_page(lo + i);
+  const bool held = span <= kE4SelectKeys * 32;
+  uint32_t keys[kE4SelectKeys];
+#pragma unroll
+  for (int x = 0; x < kE4SelectKeys; ++x) {
+    keys[x] = 0u;
+    if (held && w0 + x * 32 + lane < w1) keys[x] = from_page(lo + w0 + x * 32 + lane);
   }
-  auto key = [&](int i) { return here ? e4_keys[i] : from_page(lo + i); };
+  // f(place, key) for this warp's tokens, 32 at a time; a lane without a token has place -1
+  auto each = [&](auto f) {
+    if (held) {
+#pragma unroll
+      for (int x = 0; x < kE4SelectKeys; ++x) {
+        if (w0 + x * 32 >= w1) break;
+        f(w0 + x * 32 + lane < w1 ? lo + w0 + x * 32 + lane : -1, keys[x]);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = w0 + lane; i - lane < w1; i += 32) f(i < w1 ? lo + i : -1, i < w1 ? from_page(lo + i) : 0u);
+    }
+  };
   uint32_t prefix = 0, mask = 0, need = take;        // keys that begin with `prefix`; how many of them stay
 #pragma unroll 1
   for (int shift = 24; shift >= 0; shift -= 8) {
     if (tid < 256) hist[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < mine; i += kE4SelectThreads) {
-      const uint32_t k = key(i);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
-    }
+    each([&](int t, uint32_t k) {
+      if (t >= 0 && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
+    });
     if (CLUSTER) cg::this_cluster().sync();
     else __syncthreads();
     if (warp == 0) {                                 // lane i: digits 255 - 8 i downwards
@@ -111,13 +124,11 @@ e4_select_kernel(const RbE4m3EvictArgs a, int room RB_BOUNDS_PARAM) {
     need = digit[1];
   }
   // keys above `prefix` stay, and of those equal to it the first `need`
-  const int span = ((mine + kE4SelectThreads - 1) / kE4SelectThreads) * 32, w0 = warp * span, w1 = min(mine, w0 + span);
   uint32_t above = 0, equal = 0;                     // of this warp
-  for (int i0 = w0; i0 < w1; i0 += 32) {
-    const uint32_t k = i0 + lane < w1 ? key(i0 + lane) : 0u;
-    above += __popc(__ballot_sync(0xffffffffu, i0 + lane < w1 && k > prefix));
-    equal += __popc(__ballot_sync(0xffffffffu, i0 + lane < w1 && k == prefix));
-  }
+  each([&](int t, uint32_t k) {
+    above += __popc(__ballot_sync(0xffffffffu, t >= 0 && k > prefix));
+    equal += __popc(__ballot_sync(0xffffffffu, t >= 0 && k == prefix));
+  });
   if (lane == 0) {
     warp_n[0][warp] = above;
     warp_n[1][warp] = equal;
@@ -137,16 +148,15 @@ e4_select_kernel(const RbE4m3EvictArgs a, int room RB_BOUNDS_PARAM) {
       before[1] += *cg::this_cluster().map_shared_rank(&part[1], r);
     }
   }
-  for (int i0 = w0; i0 < w1; i0 += 32) {
-    const uint32_t k = i0 + lane < w1 ? key(i0 + lane) : 0u;
-    const uint32_t gt = __ballot_sync(0xffffffffu, i0 + lane < w1 && k > prefix), eq = __ballot_sync(0xffffffffu, i0 + lane < w1 && k == prefix);
+  each([&](int t, uint32_t k) {
+    const uint32_t gt = __ballot_sync(0xffffffffu, t >= 0 && k > prefix), eq = __ballot_sync(0xffffffffu, t >= 0 && k == prefix);
     const uint32_t in_front = (1u << lane) - 1;
     const uint32_t equals = before[1] + __popc(eq & in_front);           // equal ones in front of this token
     const uint32_t at = first + before[0] + __popc(gt & in_front) + min(equals, need);
-    if (((gt >> lane) & 1 || ((eq >> lane) & 1 && equals < need)) && at < static_cast<uint32_t>(a.keep)) kept[at] = lo + i0 + lane;
+    if (((gt >> lane) & 1 || ((eq >> lane) & 1 && equals < need)) && at < static_cast<uint32_t>(a.keep)) kept[at] = t;
     before[0] += __popc(gt);
     before[1] += __popc(eq);
-  }
+  });
   if (CLUSTER) cg::this_cluster().sync();            // others may still read this CTA's counts
 }
 
@@ -300,20 +310,10 @@ RB_API int rb_e4m3_evict(const RbE4m3EvictArgs* args, void* stream_v) {
       tokens > 0x3fffffff || a.keep > 0x3fffffff)
     return -1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_v);
-  int cluster = 1;
-  while (cluster < 8 && static_cast<long long>(cluster) * rb::kE4SelectShare < tokens) cluster *= 2;
-  long long room = (tokens + cluster - 1) / cluster + 32;
-  if (room > rb::kE4SelectKeys) room = rb::kE4SelectKeys;
-  static bool set[64] = {};
-  const int dev = rbhost::device_slot();
-  if (!set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(rb::e4_select_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, rb::kE4SelectKeys * 4);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(rb::e4_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, rb::kE4SelectKeys * 4);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    set[dev] = true;
-  }
+  int cluster = 1;                                   // as many CTAs for a sequence and head as hold its keys
+  while (cluster < 8 && static_cast<long long>(cluster) * rb::kE4SelectKeys * rb::kE4SelectThreads < tokens) cluster *= 2;
   cudaError_t e = rbhost::launch_pdl(cluster > 1 ? rb::e4_select_kernel<true> : rb::e4_select_kernel<false>, dim3(cluster, a.pages.kv_heads, a.batch),
-                                     dim3(rb::kE4SelectThreads), static_cast<size_t>(room) * 4, s, cluster, a, static_cast<int>(room) RB_BOUNDS_ARG);
+                                     dim3(rb::kE4SelectThreads), 0, s, cluster, a RB_BOUNDS_ARG);
   if (e == cudaSuccess) e = a.pages.head_dim == 64 ? move_tokens<64>(a, s) : move_tokens<128>(a, s);
   return static_cast<int>(e);
 }
