@@ -15,7 +15,7 @@ constexpr int kE4AppendHeads = 4;                    // of a CTA: a warp for the
 // A CTA takes the pages that begin, for this call, within `per_cta` rows, for four KV heads: those whose first new token is one of these rows.  A page's
 // tokens may lie in the next CTA's rows too.
 template <typename T, int D>
-__global__ void __launch_bounds__(kE4AppendHeads * 64)
+__global__ void __launch_bounds__(kE4AppendHeads * 64, sizeof(T) == 4 ? 2 : 3)
 e4_append_kernel(const RbE4m3AppendArgs a, int per_cta RB_BOUNDS_PARAM) {
   pdl_wait();
   pdl_launch();
@@ -44,18 +44,12 @@ e4_append_kernel(const RbE4m3AppendArgs a, int per_cta RB_BOUNDS_PARAM) {
     r += max(n, 1);                                  // starts that do not ascend end the loop too
     if (n <= 0) continue;
     if (off != 0 && r0 != first) continue;                             // the page's first new token is an earlier row
-    const int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, static_cast<int>(pos / bs));
-    if (page < 0) {
-      RB_BOUNDS_HIT(104);
-      continue;
-    }
     const T* src = rows + r0 * ld + static_cast<long long>(h) * D + c_lane;
-    const long long tile = static_cast<long long>(page) * G + h;
-    uint8_t* dst = codes + tile * bs * D;
     // up to 16 rows stay in registers between the search for their largest number and their rounding; of pages with more the rows are read again
     constexpr int kHeld = 16 / RPW;
     uint4 raw[kHeld][sizeof(T) / 2];
     float most = 0.f;
+    int page = -1;
     for (int i0 = 0; i0 < n; i0 += 16) {
 #pragma unroll
       for (int k = 0; k < kHeld; ++k)
@@ -63,6 +57,13 @@ e4_append_kernel(const RbE4m3AppendArgs a, int per_cta RB_BOUNDS_PARAM) {
 #pragma unroll
           for (int x = 0; x < static_cast<int>(sizeof(T) / 2); ++x) raw[k][x] = reinterpret_cast<const uint4*>(src + (i0 + k * RPW + r_lane) * ld)[x];
         }
+      if (i0 == 0) {                                                   // looked up while the rows arrive
+        page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, static_cast<int>(pos / bs));
+        if (page < 0) {
+          RB_BOUNDS_HIT(104);
+          break;
+        }
+      }
 #pragma unroll
       for (int k = 0; k < kHeld; ++k)
         if (i0 + k * RPW + r_lane < n) {
@@ -72,6 +73,9 @@ e4_append_kernel(const RbE4m3AppendArgs a, int per_cta RB_BOUNDS_PARAM) {
           for (int j = 0; j < 8; ++j) most = fmaxf(most, e4_finite_abs(x[j]));
         }
     }
+    if (page < 0) continue;
+    const long long tile = static_cast<long long>(page) * G + h;
+    uint8_t* dst = codes + tile * bs * D;
     int e = e4_exponent(warp_max(most));
     if (off > 0) {
       const int had = exps[tile];
