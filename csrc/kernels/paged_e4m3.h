@@ -52,7 +52,7 @@ int rb_e4m3_read(const RbE4m3ReadArgs* args, void* stream);
 
 // Attention of one token per sequence: q [batch, heads * head_dim], pitch ld_q, out the same with ld_o (bf16 or f16).  accumulate: every cached
 // token's weight grows by its softmax weights, summed over the query heads of its KV head.  A sequence without tokens gets zeros.
-// scratch: fp32 [rb_e4m3_decode_scratch_floats(...)].
+// scratch: fp32 [rb_e4m3_decode_scratch_floats(...)], NULL where that is 0 (few and short sequences).
 typedef struct RbE4m3DecodeArgs {
   RbPagesE4m3 pages;
   const void* q;
@@ -64,7 +64,7 @@ typedef struct RbE4m3DecodeArgs {
   int batch, max_blocks, heads, type, accumulate;
   float scale;
 } RbE4m3DecodeArgs;
-long long rb_e4m3_decode_scratch_floats(int batch, int heads, int head_dim, int max_blocks, int block_size, int accumulate);
+long long rb_e4m3_decode_scratch_floats(int batch, int heads, int kv_heads, int head_dim, int max_blocks, int block_size, int accumulate);
 int rb_e4m3_decode(const RbE4m3DecodeArgs* args, void* stream);
 
 // Sequences of more than `keep` tokens keep the first keep_first, the last `recent` and, of the others, those with the largest weights (of equal

@@ -5,10 +5,14 @@
 // of the codes are then at most 1 whatever the tiles' exponents, and the denominator is summed in fp32 from p_j 2^(-e_j).  M is rounded up to a whole
 // number, so that M - e_j and the factors that bring sums from one M to another are exact; with exponents of -100 a fractional M would cost the
 // scores seven bits.
+#include <cooperative_groups.h>
+
 #include "pdl.cuh"
 #include "paged_e4m3.cuh"
 
 namespace rb {
+
+namespace cg = cooperative_groups;
 
 constexpr int kE4Slice = 256;                        // tokens whose sums one CTA forms; the merge goes over them in order
 
@@ -80,14 +84,35 @@ struct E4Layout {
 // the second operand by a transposition of 8 x 8 (movmatrix).  Codes become f16 exactly.  The contraction over head dimensions may take them in any
 // order, so a lane reads 16 codes of a row at a time and these are its operands of four products; a swizzled tile gives every lane its 16 bytes without
 // bank conflicts.  A query row is scaled to [1, 2) by a power of two first.
-// LIST: the slices of all sequences and KV heads, numbered one sequence after the other, are dealt in equal runs to CTAs that stay, and the next slice's
-// tiles are copied while this one's are worked on.  Otherwise the grid is (slices, KV heads, sequences).
-template <typename T, int D, int NH, bool LIST>
+// HOW: kE4List: the slices of all sequences and KV heads, numbered one sequence after the other, are dealt in equal runs to CTAs that stay, and the next
+// slice's tiles are copied while this one's are worked on.  Otherwise the grid is (slices, KV heads, sequences); kE4Cluster: the CTAs of a sequence and KV
+// head are a cluster and merge their sums, and add the weights, through distributed shared memory.
+enum { kE4Grid, kE4List, kE4Cluster };
+
+// Sums y under the maximum my, added to x under mx.  Maxima are whole, so the factors are exact and the sum does not depend on which maximum it is under.
+__device__ __forceinline__ void e4_add(float4& x, float& mx, float& lx, const float4& y, float my, float ly) {
+  const float to = fmaxf(mx, my);
+  const float f = mx == to ? 1.f : e4_ex2(mx - to), g = my == to ? 1.f : e4_ex2(my - to);
+  x.x = fmaf(y.x, g, x.x * f);
+  x.y = fmaf(y.y, g, x.y * f);
+  x.z = fmaf(y.z, g, x.z * f);
+  x.w = fmaf(y.w, g, x.w * f);
+  lx = fmaf(ly, g, lx * f);
+  mx = to;
+}
+// A weight is 2^(s - m) / den = 2^(s - (m + x)) / (den / 2^x), with the x that brings den / 2^x into [1, 2): (m + x, 2^x / den).
+__device__ __forceinline__ float2 e4_norm_of(float m, float den) {
+  const int x = static_cast<int>(__float_as_uint(den) >> 23) - 127;
+  return make_float2(m + static_cast<float>(x), e4_two(x) / den);
+}
+
+template <typename T, int D, int NH, int HOW>
 __global__ void __launch_bounds__(kE4Warps * 32, NH > 1 ? 2 : D == 64 ? 4 : 3)
 e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const RbE4m3DecodeArgs a, int h0, int slices,
                  unsigned int* status RB_BOUNDS_PARAM) {
   pdl_wait();
-  if (!LIST) pdl_launch();                           // CTAs that stay let the merge in at the end of their runs: 177 us at once, 159 then (64 of 4096 to 8192)
+  if (HOW != kE4List) pdl_launch();                  // CTAs that stay let the merge in at the end of their runs: 177 us at once, 159 then (64 of 4096 to 8192)
+  constexpr bool LIST = HOW == kE4List, CLUSTER = HOW == kE4Cluster;
   using L = E4Layout<D, NH>;
   constexpr int KS = D / 16;                         // products of 16 in a score
   constexpr int MT = D / 16;                         // tiles of 16 output dimensions
@@ -96,13 +121,16 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
   extern __shared__ uint8_t e4_raw[];
   __shared__ __align__(8) uint64_t bars[kE4Warps][kE4Stages];
   __shared__ float m_sh[kE4Warps][NH * 8], l_sh[kE4Warps][NH * 8];
+  __shared__ float2 ml_sh[NH * 8], norm_sh[NH * 8];
   __shared__ int abort_sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
   const uint32_t base = (smem_u32(e4_raw) + 1023u) & ~1023u;             // the swizzle goes by addresses
   const uint32_t ring = base + warp * (kE4Stages * 2 * L::kTile);
-  float* merge = reinterpret_cast<float*>(e4_raw + (base - smem_u32(e4_raw)) + L::kRing);
+  float* merge = reinterpret_cast<float*>(e4_raw + (base - smem_u32(e4_raw)) + L::kRing);           // [warps][heads][D]
+  float* scores_sh = nullptr;                        // CLUSTER, where weights are summed: [256][heads] behind it
   const int bs = a.pages.block_size, G = a.pages.kv_heads, group = a.heads / G;
   const int heads = min(NH * 8, group - h0);
+  if (CLUSTER) scores_sh = merge + kE4Warps * heads * D;
 
   // ---- this CTA's run of slices
   E4Place at = {0, 0, 0, 1};
@@ -110,7 +138,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
     at.b = blockIdx.z;
     at.hk = blockIdx.y;
     at.s = blockIdx.x;
-    if (at.s * kE4Slice >= e4_len(a, at.b)) return;
+    if (!CLUSTER && at.s * kE4Slice >= e4_len(a, at.b)) return;
   } else {
     int n = lane < a.batch ? (e4_len(a, lane) + kE4Slice - 1) / kE4Slice : 0, total = n;
     for (int i = lane + 32; i < a.batch; i += 32) total += (e4_len(a, i) + kE4Slice - 1) / kE4Slice;
@@ -354,12 +382,14 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
             if (n_tok[u] < 16 && gq + (j >> 1) * 8 >= n_tok[u]) s[u][r][j] = -INFINITY;
           }
           if (a.accumulate) {                        // [batch, KV heads, tokens, heads of a group]
-            float* scores = a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (D + 4) +
-                            ((static_cast<long long>(at.b) * G + at.hk) * slices * kE4Slice + at.s * kE4Slice + ((i + u) * kE4Warps + warp) * 16 + gq) * group + h0;
+            const int t = ((i + u) * kE4Warps + warp) * 16 + gq;
+            float* scores = CLUSTER ? scores_sh + t * heads
+                                    : a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (D + 4) +
+                                          ((static_cast<long long>(at.b) * G + at.hk) * slices * kE4Slice + at.s * kE4Slice + t) * group + h0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int h = r * 8 + tq * 2 + (j & 1);
-              if (h < heads) scores[(j >> 1) * 8 * group + h] = s[u][r][j];
+              if (h < heads) scores[(j >> 1) * 8 * (CLUSTER ? heads : group) + h] = s[u][r][j];
             }
           }
 #pragma unroll
@@ -447,7 +477,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
     }
     if (LIST && at.left <= 1) pdl_launch();
     __syncthreads();
-    const bool whole = n_at <= kE4Slice;             // the sequence has no other slice
+    const bool whole = !CLUSTER && n_at <= kE4Slice; // the sequence has no other slice
     for (int i = threadIdx.x; i < heads * (D / 4); i += kE4Warps * 32) {
       const int head = i / (D / 4), d = i % (D / 4);
       float top = m_sh[0][head];
@@ -465,6 +495,11 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
         sum.z = fmaf(x.z, f, sum.z);
         sum.w = fmaf(x.w, f, sum.w);
       }
+      if (CLUSTER) {                                 // where this thread read the first warp's
+        *reinterpret_cast<float4*>(merge + head * D + ((d ^ (head >> 1 & 3)) << 2)) = sum;
+        if (d == 0) ml_sh[head] = make_float2(top, den);
+        continue;
+      }
       const int h = at.hk * group + h0 + head;
       if (whole) {
         const float inv = 1.f / den;
@@ -479,6 +514,47 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
         if (d == 0) *reinterpret_cast<float2*>(out) = make_float2(top, den);
         *reinterpret_cast<float4*>(out + 4 + d * 4) = sum;
       }
+    }
+    if (CLUSTER) {
+      auto all = cg::this_cluster();
+      const int ranks = gridDim.x, here = (n_at + kE4Slice - 1) / kE4Slice;              // slices that are there
+      if (ranks > 1) all.sync();
+      else __syncthreads();
+      for (int i = threadIdx.x + blockIdx.x * (kE4Warps * 32); i < heads * (D / 4); i += ranks * (kE4Warps * 32)) {
+        const int head = i / (D / 4), d = i % (D / 4), at_sh = head * D + ((d ^ (head >> 1 & 3)) << 2);
+        float4 sum = *reinterpret_cast<const float4*>(all.map_shared_rank(merge + at_sh, 0));
+        float2 ml = *all.map_shared_rank(&ml_sh[head], 0);
+        for (int k = 1; k < here; ++k) {
+          const float2 other = *all.map_shared_rank(&ml_sh[head], k);
+          e4_add(sum, ml.x, ml.y, *reinterpret_cast<const float4*>(all.map_shared_rank(merge + at_sh, k)), other.x, other.y);
+        }
+        const float inv = here > 0 ? 1.f / ml.y : 0.f;                   // without tokens the sums are zero
+        T* out = reinterpret_cast<T*>(a.out) + at.b * a.ld_o + (static_cast<long long>(at.hk) * group + h0 + head) * D + d * 4;
+        e4_put(out, sum.x * inv);
+        e4_put(out + 1, sum.y * inv);
+        e4_put(out + 2, sum.z * inv);
+        e4_put(out + 3, sum.w * inv);
+      }
+      if (a.accumulate) {
+        if (static_cast<int>(threadIdx.x) < heads) {
+          float2 ml = *all.map_shared_rank(&ml_sh[threadIdx.x], 0);
+          float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int k = 1; k < here; ++k) {
+            const float2 other = *all.map_shared_rank(&ml_sh[threadIdx.x], k);
+            e4_add(none, ml.x, ml.y, none, other.x, other.y);
+          }
+          norm_sh[threadIdx.x] = e4_norm_of(ml.x, ml.y);
+        }
+        __syncthreads();
+        for (int t = threadIdx.x; t < min(kE4Slice, n_at - at.s * kE4Slice); t += kE4Warps * 32) {
+          float w = 0.f;
+          for (int h = 0; h < heads; ++h) w = fmaf(e4_ex2(scores_sh[t * heads + h] - norm_sh[h].x), norm_sh[h].y, w);
+          const int token = at.s * kE4Slice + t;
+          const int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, at.b, token / bs);
+          if (page >= 0) a.pages.weight[(static_cast<long long>(page) * G + at.hk) * bs + token % bs] += w;
+        }
+      }
+      if (ranks > 1) all.sync();                     // others may still read this CTA's sums
     }
     if (!LIST || at.left <= 1) break;
     __syncthreads();
@@ -529,16 +605,6 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
     m[k] = -INFINITY;
     l[k] = 0.f;
   }
-  auto add = [](float4& x, float& mx, float& lx, const float4& y, float my, float ly) {
-    const float to = fmaxf(mx, my);
-    const float f = mx == to ? 1.f : e4_ex2(mx - to), g = my == to ? 1.f : e4_ex2(my - to);
-    x.x = fmaf(y.x, g, x.x * f);
-    x.y = fmaf(y.y, g, x.y * f);
-    x.z = fmaf(y.z, g, x.z * f);
-    x.w = fmaf(y.w, g, x.w * f);
-    lx = fmaf(ly, g, lx * f);
-    mx = to;
-  };
   constexpr int kAhead = PER == 1 ? 8 : 1;           // slices of a chain that are loaded together
   for (int s0 = r; s0 < here; s0 += kChains * kAhead) {
     float4 x[PER][kAhead];
@@ -589,7 +655,7 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
   float top = ml_sh[0].x, den = ml_sh[0].y;
 #pragma unroll
   for (int k = 1; k < kChains; ++k)
-    if (k < here) add(o, top, den, sum_sh[k][c], ml_sh[k].x, ml_sh[k].y);
+    if (k < here) e4_add(o, top, den, sum_sh[k][c], ml_sh[k].x, ml_sh[k].y);
   if (here > 1) {
     const float inv = 1.f / den;
     e4_put(out + c * 4, o.x * inv);
@@ -598,11 +664,10 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
     e4_put(out + c * 4 + 3, o.w * inv);
   }
   if (a.accumulate && tid == 0 && blockIdx.z == 0) {
-    // a weight is 2^(s - m) / den = 2^(s - (m + x)) / (den / 2^x), with the x that brings den / 2^x into [1, 2)
-    const int x = static_cast<int>(__float_as_uint(den) >> 23) - 127;
     float* norm = e4_norm(a.scratch, a.batch, a.heads, slices, D, b, h);
-    norm[0] = top + static_cast<float>(x);
-    norm[1] = e4_two(x) / den;
+    const float2 x = e4_norm_of(top, den);
+    norm[0] = x.x;
+    norm[1] = x.y;
   }
 }
 
@@ -630,6 +695,12 @@ namespace {
 long long e4_slices(int max_blocks, int block_size) {
   return (static_cast<long long>(max_blocks) * block_size + rb::kE4Slice - 1) / rb::kE4Slice;
 }
+// Whether the CTAs of a sequence and KV head merge as a cluster: few slices, heads for one pass, and no more CTAs than fit on the GPU at a time (three on an
+// SM).  One B200, us: one sequence of 300, 12 KV heads of 64 13.0, with a list or grid and its merge 20.6; of 2047, 4 KV heads of 128, with weights 13.1 / 21.7;
+// 48 of 16 to 1024, 8 KV heads of 64, 1536 CTAs, many without a token, 23.1 on the GPU / 19.2.
+bool in_clusters(int batch, int kv_heads, long long slices, int group) {
+  return slices <= 8 && group <= 16 && batch * kv_heads * slices <= 3ll * rbhost::device_sm_count();
+}
 template <typename T, int D, int NH>
 int decode_launch(const RbE4m3DecodeArgs& a, cudaStream_t stream) {
   using L = rb::E4Layout<D, NH>;
@@ -646,21 +717,25 @@ int decode_launch(const RbE4m3DecodeArgs& a, cudaStream_t stream) {
   static int per_sm[NH * 8 + 1][64] = {};            // CTAs of a list that fit on an SM, by the heads that a pass has
   const int dev = rbhost::device_slot();
   if (!per_sm[most][dev]) {
-    cudaError_t e = cudaFuncSetAttribute(rb::e4_decode_kernel<T, D, NH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::bytes(NH * 8));
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(rb::e4_decode_kernel<T, D, NH, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::bytes(NH * 8));
+    const int bytes = L::bytes(NH * 8) + rb::kE4Slice * NH * 8 * 4;
+    cudaError_t e = cudaFuncSetAttribute(rb::e4_decode_kernel<T, D, NH, rb::kE4List>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(rb::e4_decode_kernel<T, D, NH, rb::kE4Grid>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(rb::e4_decode_kernel<T, D, NH, rb::kE4Cluster>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     int n = 0;
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rb::e4_decode_kernel<T, D, NH, true>, rb::kE4Warps * 32, smem);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rb::e4_decode_kernel<T, D, NH, rb::kE4List>, rb::kE4Warps * 32, smem);
     if (e != cudaSuccess) return static_cast<int>(e);
     per_sm[most][dev] = n > 0 ? n : 1;
   }
+  const dim3 threads(rb::kE4Warps * 32), whole(slices, p.kv_heads, a.batch);
+  if (in_clusters(a.batch, p.kv_heads, slices, group))
+    return static_cast<int>(rbhost::launch_pdl(rb::e4_decode_kernel<T, D, NH, rb::kE4Cluster>, whole, threads, smem + (a.accumulate ? rb::kE4Slice * most * 4 : 0),
+                                               stream, slices, *km, *vm, a, 0, slices, status RB_BOUNDS_ARG));
   const int some = per_sm[most][dev] * rbhost::device_sm_count();
   const bool list = static_cast<long long>(a.batch) * p.kv_heads * slices > some;
-  auto kern = list ? rb::e4_decode_kernel<T, D, NH, true> : rb::e4_decode_kernel<T, D, NH, false>;
-  const dim3 grid = list ? dim3(some) : dim3(slices, p.kv_heads, a.batch);
+  auto kern = list ? rb::e4_decode_kernel<T, D, NH, rb::kE4List> : rb::e4_decode_kernel<T, D, NH, rb::kE4Grid>;
   cudaError_t e = cudaSuccess;
   for (int h0 = 0; h0 < group && e == cudaSuccess; h0 += NH * 8)        // wider groups take several passes
-    e = rbhost::launch_pdl(kern, grid, dim3(rb::kE4Warps * 32), smem, stream, 1, *km, *vm, a, h0, slices, status RB_BOUNDS_ARG);
+    e = rbhost::launch_pdl(kern, list ? dim3(some) : whole, threads, smem, stream, 1, *km, *vm, a, h0, slices, status RB_BOUNDS_ARG);
   if (e == cudaSuccess) {
     const bool many = slices > 64;
     e = rbhost::launch_pdl(many ? rb::e4_merge_kernel<T, 8> : rb::e4_merge_kernel<T, D / 4>, dim3(a.heads, a.batch, many ? D / 32 : 1), dim3(128), 0, stream, 1,
@@ -678,8 +753,9 @@ int decode_by_dim(const RbE4m3DecodeArgs& a, cudaStream_t s) {
 }
 }  // namespace
 
-RB_API long long rb_e4m3_decode_scratch_floats(int batch, int heads, int head_dim, int max_blocks, int block_size, int accumulate) {
+RB_API long long rb_e4m3_decode_scratch_floats(int batch, int heads, int kv_heads, int head_dim, int max_blocks, int block_size, int accumulate) {
   const long long slices = e4_slices(max_blocks, block_size), rows = static_cast<long long>(batch) * heads;
+  if (in_clusters(batch, kv_heads, slices, heads / kv_heads)) return 0;
   return rows * slices * (head_dim + 4) + (accumulate ? rows * (slices * rb::kE4Slice + 2) : 0);
 }
 
@@ -687,7 +763,8 @@ RB_API int rb_e4m3_decode(const RbE4m3DecodeArgs* args, void* stream_v) {
   const RbE4m3DecodeArgs& a = *args;
   if (a.batch <= 0) return 0;
   if (const int bad = rbhost::e4_check(a.pages)) return bad;
-  if (!a.q || !a.out || !a.block_tables || !a.context_lens || !a.scratch || a.max_blocks <= 0 || a.heads <= 0 || a.heads % a.pages.kv_heads ||
+  if (!a.q || !a.out || !a.block_tables || !a.context_lens || a.max_blocks <= 0 || a.heads <= 0 || a.heads % a.pages.kv_heads ||
+      (!a.scratch && !in_clusters(a.batch, a.pages.kv_heads, e4_slices(a.max_blocks, a.pages.block_size), a.heads / a.pages.kv_heads)) ||
       a.batch > 65535 || a.pages.kv_heads > 65535 || (a.accumulate && !a.pages.weight) ||
       static_cast<long long>(a.batch) * a.pages.kv_heads * e4_slices(a.max_blocks, a.pages.block_size) > 0x3fffffff)
     return -1;

@@ -10,7 +10,9 @@ bf16 cache: int32 [batch, width] and int32 [batch], tokens in the cache with the
 """
 from __future__ import annotations
 
+import functools
 import math
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -22,40 +24,16 @@ LEAST_EXPONENT, MOST_EXPONENT, LARGEST_CODE = -100, 119, 448.0
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-class _Pages(C.Structure):
-    _fields_ = [("k", N.c_void_p), ("v", N.c_void_p), ("k_exp", N.c_void_p), ("v_exp", N.c_void_p), ("weight", N.c_void_p), ("num_blocks", N.c_ll),
-                ("block_size", N.c_int), ("kv_heads", N.c_int), ("head_dim", N.c_int)]
+# The argument blocks of csrc/kernels/paged_e4m3.h, packed: a ctypes structure of 25 fields takes 2 us to fill, a fifth of a small call.
+_PAGES = "6P3i0q"                                                     # k, v, exponents, weights, blocks; block size, KV heads, head size
+_APPEND = struct.Struct("@" + _PAGES + "5P2q4i")                      # k, v, tables, lengths, starts; pitches; rows, batch, width, type
+_READ = struct.Struct("@" + _PAGES + "5P2q4i")                        # the same
+_DECODE = struct.Struct("@" + _PAGES + "5P2q5if")                     # q, out, tables, lengths, scratch; pitches; batch, width, heads, type, accumulate; scale
+_EVICT = struct.Struct("@" + _PAGES + "5P6i")                         # tables, lengths, out tables, kept, lengths out; batch, widths, keep, recent, first
 
-
-class _AppendArgs(C.Structure):
-    _fields_ = [("pages", _Pages), ("k_new", N.c_void_p), ("v_new", N.c_void_p), ("block_tables", N.c_void_p), ("context_lens", N.c_void_p),
-                ("row_starts", N.c_void_p), ("ld_k", N.c_ll), ("ld_v", N.c_ll), ("rows", N.c_int), ("batch", N.c_int), ("max_blocks", N.c_int),
-                ("type", N.c_int)]
-
-
-class _ReadArgs(C.Structure):
-    _fields_ = [("pages", _Pages), ("k_out", N.c_void_p), ("v_out", N.c_void_p), ("block_tables", N.c_void_p), ("context_lens", N.c_void_p),
-                ("row_starts", N.c_void_p), ("ld_k", N.c_ll), ("ld_v", N.c_ll), ("rows", N.c_int), ("batch", N.c_int), ("max_blocks", N.c_int),
-                ("type", N.c_int)]
-
-
-class _DecodeArgs(C.Structure):
-    _fields_ = [("pages", _Pages), ("q", N.c_void_p), ("out", N.c_void_p), ("block_tables", N.c_void_p), ("context_lens", N.c_void_p),
-                ("scratch", N.c_void_p), ("ld_q", N.c_ll), ("ld_o", N.c_ll), ("batch", N.c_int), ("max_blocks", N.c_int), ("heads", N.c_int),
-                ("type", N.c_int), ("accumulate", N.c_int), ("scale", N.c_float)]
-
-
-class _EvictArgs(C.Structure):
-    _fields_ = [("pages", _Pages), ("block_tables", N.c_void_p), ("context_lens", N.c_void_p), ("out_tables", N.c_void_p), ("kept", N.c_void_p),
-                ("lens_out", N.c_void_p), ("batch", N.c_int), ("max_blocks", N.c_int), ("out_blocks", N.c_int), ("keep", N.c_int),
-                ("recent", N.c_int), ("keep_first", N.c_int)]
-
-
-N.optional_sig("rb_e4m3_append", [C.POINTER(_AppendArgs), N.c_void_p])
-N.optional_sig("rb_e4m3_read", [C.POINTER(_ReadArgs), N.c_void_p])
-N.optional_sig("rb_e4m3_decode", [C.POINTER(_DecodeArgs), N.c_void_p])
-N.optional_sig("rb_e4m3_decode_scratch_floats", [N.c_int] * 6, N.c_ll)
-N.optional_sig("rb_e4m3_evict", [C.POINTER(_EvictArgs), N.c_void_p])
+for _name in ("append", "read", "decode", "evict"):
+    N.optional_sig("rb_e4m3_" + _name, [C.c_char_p, N.c_void_p])
+N.optional_sig("rb_e4m3_decode_scratch_floats", [N.c_int] * 7, N.c_ll)
 N._LAUNCHES["rb_e4m3_decode"] = 2
 N._LAUNCHES["rb_e4m3_evict"] = 2
 
@@ -88,37 +66,51 @@ class PagesE4M3:
 
 def _check(what: str, pages: PagesE4M3, block_tables, context_lens, *others) -> tuple:
     """(blocks, KV heads, block size, head size) of pages that a kernel can take with these tables; `others`: further tensors of the call."""
-    k, w = pages.k, pages.weight
-    nb, G, bs, D = k.shape
-    if not (k.dtype is pages.v.dtype is torch.float8_e4m3fn and pages.k_exp.dtype is pages.v_exp.dtype is torch.int8 and pages.v.shape == k.shape and
-            pages.k_exp.shape == pages.v_exp.shape == (nb, G) and k.is_contiguous() and pages.v.is_contiguous() and pages.k_exp.is_contiguous() and
-            pages.v_exp.is_contiguous()):
+    k, v, ke, ve, w = pages.k, pages.v, pages.k_exp, pages.v_exp, pages.weight
+    shape = k.shape
+    nb, G, bs, D = shape
+    if not (k.dtype is v.dtype is torch.float8_e4m3fn and ke.dtype is ve.dtype is torch.int8 and v.shape == shape and ke.shape == ve.shape == (nb, G) and
+            k.is_contiguous() and v.is_contiguous() and ke.is_contiguous() and ve.is_contiguous()):
         raise TypeError(f"{what}: pages are contiguous e4m3 codes [blocks, kv_heads, block_size, head_dim] with int8 exponents [blocks, kv_heads]")
-    if w is not None and not (w.dtype is torch.float32 and w.shape == (nb, G, bs) and w.is_contiguous()):
-        raise TypeError(f"{what}: weights are contiguous fp32 [blocks, kv_heads, block_size]")
+    dev = k.get_device()
+    if w is not None:
+        if not (w.dtype is torch.float32 and w.shape == (nb, G, bs) and w.is_contiguous()):
+            raise TypeError(f"{what}: weights are contiguous fp32 [blocks, kv_heads, block_size]")
+        others += (w,)
     if not (block_tables.dtype is context_lens.dtype is torch.int32 and block_tables.dim() == 2 and block_tables.is_contiguous() and
-            context_lens.is_contiguous() and context_lens.shape == (block_tables.shape[0],)):
+            context_lens.is_contiguous() and context_lens.shape == block_tables.shape[:1]):
         raise TypeError(f"{what}: a contiguous int32 table row and an int32 length per sequence are required")
-    dev = k.device
-    for t in (pages.v, pages.k_exp, pages.v_exp, w, block_tables, context_lens, *others):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
-    if k.is_cuda:
-        if bs % 16 or D not in (64, 128):
+    for t in (v, ke, ve, block_tables, context_lens, *others):
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{what}: tensors on {k.device} and {t.device}")
+    if dev >= 0:
+        if bs & 15 or (D != 64 and D != 128):
             raise ValueError(f"{what}: pages of a multiple of 16 tokens and heads of 64 or 128 are required, not {bs} and {D}")
-        if dev.index != torch.cuda.current_device():
-            raise ValueError(f"{what}: the pages are on {dev}, which is not the current device")
-    return nb, G, bs, D
+        if dev != torch._C._cuda_getDevice():
+            raise ValueError(f"{what}: the pages are on {k.device}, which is not the current device")
+    return shape
 
 
-def _native(p: PagesE4M3, shape) -> _Pages:
-    return _Pages(p.k.data_ptr(), p.v.data_ptr(), p.k_exp.data_ptr(), p.v_exp.data_ptr(), N.ptr(p.weight), shape[0], shape[2], shape[1], shape[3])
+def _native(p: PagesE4M3, shape) -> tuple:
+    return (p.k.data_ptr(), p.v.data_ptr(), p.k_exp.data_ptr(), p.v_exp.data_ptr(), _ptr(p.weight), shape[0], shape[2], shape[1], shape[3])
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+@functools.lru_cache(4096)
+def _scratch_floats(*sizes) -> int:
+    return N.kernels().rb_e4m3_decode_scratch_floats(*sizes)
+
+
+_scratch: dict = {}
 
 
 def _aligned(t: torch.Tensor) -> bool:
     """Whether the kernels can read or write the rows of `t` 16 bytes at a time."""
-    size = t.element_size()
-    return t.stride(1) == 1 and not (t.data_ptr() | t.stride(0) * size) & 15
+    pitch, step = t.stride()
+    return step == 1 and not (t.data_ptr() | pitch * t.element_size()) & 15
 
 
 def _starts(what: str, row_starts, batch: int):
@@ -193,9 +185,9 @@ def kv_append_e4m3(pages: PagesE4M3, k_new, v_new, block_tables, context_lens, r
     A page whose first slot gets a token forgets what it held and takes its exponents from this call; in any other page an exponent grows if a
     new token asks for it, and the codes in front are rounded to it (exactly, but for those that become subnormal).  Rows whose position has no
     page are not stored.  The new tokens' weights become 0."""
-    nb, G, bs, D = _check("kv_append_e4m3", pages, block_tables, context_lens, k_new, v_new, row_starts)
-    rows, batch = k_new.shape[0], block_tables.shape[0]
-    if k_new.dtype not in _TYPES or v_new.dtype is not k_new.dtype or k_new.shape != (rows, G * D) or v_new.shape != (rows, G * D):
+    shape = _check("kv_append_e4m3", pages, block_tables, context_lens, k_new, v_new, row_starts)
+    rows, batch, row = k_new.shape[0], context_lens.shape[0], (k_new.shape[0], shape[1] * shape[3])
+    if k_new.dtype not in _TYPES or v_new.dtype is not k_new.dtype or k_new.shape != row or v_new.shape != row:
         raise TypeError("kv_append_e4m3: keys and values are [rows, kv_heads * head_dim] in bf16, fp16 or fp32")
     if row_starts is not None:
         _starts("kv_append_e4m3", row_starts, batch)
@@ -209,8 +201,8 @@ def kv_append_e4m3(pages: PagesE4M3, k_new, v_new, block_tables, context_lens, r
         k_new = k_new.clone(memory_format=torch.contiguous_format)
     if not _aligned(v_new):
         v_new = v_new.clone(memory_format=torch.contiguous_format)
-    a = _AppendArgs(_native(pages, (nb, G, bs, D)), k_new.data_ptr(), v_new.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(),
-                    N.ptr(row_starts), k_new.stride(0), v_new.stride(0), rows, batch, block_tables.shape[1], _TYPES[k_new.dtype])
+    a = _APPEND.pack(*_native(pages, shape), k_new.data_ptr(), v_new.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), _ptr(row_starts),
+                     k_new.stride(0), v_new.stride(0), rows, batch, block_tables.shape[1], _TYPES[k_new.dtype])
     N.check(N.kernels().rb_e4m3_append(a, N.stream_ptr()), "rb_e4m3_append")
 
 
@@ -218,13 +210,14 @@ def kv_read_e4m3(pages: PagesE4M3, block_tables, context_lens, row_starts, rows:
     """Keys and values of whole sequences, (k, v) of [rows, kv_heads * head_dim] each: position i of sequence b in row row_starts[b] + i.
     bf16 and fp32 hold every number of a page exactly (fp16: those in its range).  `out`: a pair that receives them; rows that no position has
     stay as they are (in a pair made here: undefined)."""
-    nb, G, bs, D = _check("kv_read_e4m3", pages, block_tables, context_lens, row_starts, *(out or ()))
+    shape = _check("kv_read_e4m3", pages, block_tables, context_lens, row_starts, *(out or ()))
+    nb, G, bs, D = shape
     _starts("kv_read_e4m3", row_starts, block_tables.shape[0])
     if out is None:
         if dtype not in _TYPES:
             raise TypeError("kv_read_e4m3: rows in bf16, fp16 or fp32")
-        both = torch.empty((2, rows, G * D), dtype=dtype, device=pages.k.device)
-        out = (both[0], both[1])
+        k = torch.empty((rows, G * D), dtype=dtype, device=pages.k.device)
+        out = (k, torch.empty_like(k))
     k, v = out
     if k.dtype not in _TYPES or v.dtype is not k.dtype or k.shape != (rows, G * D) or v.shape != (rows, G * D):
         raise TypeError("kv_read_e4m3: out is a pair of [rows, kv_heads * head_dim] in bf16, fp16 or fp32")
@@ -241,8 +234,8 @@ def kv_read_e4m3(pages: PagesE4M3, block_tables, context_lens, row_starts, rows:
         return k, v
     if not (_aligned(k) and _aligned(v)):
         raise ValueError("kv_read_e4m3: rows of out start at multiples of 16 bytes")
-    a = _ReadArgs(_native(pages, (nb, G, bs, D)), k.data_ptr(), v.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), row_starts.data_ptr(),
-                  k.stride(0), v.stride(0), rows, block_tables.shape[0], block_tables.shape[1], _TYPES[k.dtype])
+    a = _READ.pack(*_native(pages, shape), k.data_ptr(), v.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), row_starts.data_ptr(),
+                   k.stride(0), v.stride(0), rows, *block_tables.shape, _TYPES[k.dtype])
     N.check(N.kernels().rb_e4m3_read(a, N.stream_ptr()), "rb_e4m3_read")
     return k, v
 
@@ -252,16 +245,17 @@ def paged_attention_decode_e4m3(q, pages: PagesE4M3, block_tables, context_lens,
     views allowed; on a GPU bf16 or fp16), the same out.  A sequence of length 0 gets zeros.  With `accumulate` the weight of every cached token
     (`pages.weight`) grows by its softmax weights, summed over the query heads of its KV head; sequences that share a page must then not be in
     one call."""
-    nb, G, bs, D = _check("paged_attention_decode_e4m3", pages, block_tables, context_lens, q, out)
-    B = block_tables.shape[0]
-    if q.dim() != 2 or q.shape[0] != B or q.shape[1] == 0 or q.shape[1] % (G * D):
+    shape = _check("paged_attention_decode_e4m3", pages, block_tables, context_lens, q, out)
+    nb, G, bs, D = shape
+    B, row = block_tables.shape[0], q.shape[-1]
+    if q.dim() != 2 or q.shape[0] != B or row == 0 or row % (G * D):
         raise TypeError("paged_attention_decode_e4m3: q is [batch, heads * head_dim], a multiple of the KV heads")
     if accumulate and pages.weight is None:
         raise ValueError("paged_attention_decode_e4m3: these pages keep no weights")
-    heads = q.shape[1] // D
+    heads = row // D
     scale = 1.0 / math.sqrt(D) if scale is None else scale
     if out is None:
-        out = torch.empty((B, heads * D), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty((B, row), dtype=q.dtype, device=q.device)
     elif out.dtype is not q.dtype or out.shape != q.shape or out.stride(1) != 1:
         raise TypeError("paged_attention_decode_e4m3: out is like q, with contiguous rows")
     if not q.is_cuda:
@@ -284,14 +278,16 @@ def paged_attention_decode_e4m3(q, pages: PagesE4M3, block_tables, context_lens,
         return out
     if q.stride(1) != 1:
         q = q.contiguous()
-    lib = N.kernels()
     width = block_tables.shape[1]
     if width == 0:
         return out.zero_()
-    scratch = torch.empty(lib.rb_e4m3_decode_scratch_floats(B, heads, D, width, bs, int(accumulate)), dtype=torch.float32, device=q.device)
-    a = _DecodeArgs(_native(pages, (nb, G, bs, D)), q.data_ptr(), out.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), scratch.data_ptr(),
-                    q.stride(0), out.stride(0), B, width, heads, _TYPES[q.dtype], int(accumulate), scale)
-    N.check(lib.rb_e4m3_decode(a, N.stream_ptr()), "rb_e4m3_decode")
+    floats = _scratch_floats(B, heads, G, D, width, bs, accumulate)
+    # small scratch is kept for the stream's next call, large scratch (many or long sequences) is not
+    scratch = None if floats == 0 else N.scratch(_scratch, q.device, floats, torch.float32) if floats <= 1 << 24 else \
+        torch.empty(floats, dtype=torch.float32, device=q.device)
+    a = _DECODE.pack(*_native(pages, shape), q.data_ptr(), out.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), _ptr(scratch),
+                     q.stride(0), out.stride(0), B, width, heads, _TYPES[q.dtype], accumulate, scale)
+    N.check(N.kernels().rb_e4m3_decode(a, N.stream_ptr()), "rb_e4m3_decode")
     return out
 
 
@@ -305,15 +301,15 @@ def kv_evict_e4m3(pages: PagesE4M3, block_tables, context_lens, keep: int, recen
 
     A page's exponent becomes the largest of those that its tokens had; codes from smaller ones are rounded to it.  Attention does not ask for
     positions (keys are stored rotated), but a sequence's next position is no longer its length."""
-    nb, G, bs, D = _check("kv_evict_e4m3", pages, block_tables, context_lens, out_tables)
-    B = block_tables.shape[0]
+    shape = _check("kv_evict_e4m3", pages, block_tables, context_lens, out_tables)
+    B, G = block_tables.shape[0], shape[1]
     if pages.weight is None:
         raise ValueError("kv_evict_e4m3: these pages keep no weights")
     if keep < 1 or recent < 0 or keep_first < 0 or recent + keep_first > keep:
         raise ValueError("kv_evict_e4m3: keep must be at least 1 and at least recent + keep_first")
     if out_tables is not None and not (out_tables.dtype is torch.int32 and out_tables.dim() == 2 and out_tables.shape[0] == B and out_tables.is_contiguous()):
         raise TypeError("kv_evict_e4m3: out_tables is a contiguous int32 table row per sequence")
-    lens = torch.empty(B, dtype=torch.int32, device=pages.k.device)
+    lens = torch.empty_like(context_lens)
     kept = torch.empty((B, G, keep), dtype=torch.int32, device=pages.k.device)
     if not pages.k.is_cuda:
         _evict_cpu(pages, block_tables, context_lens, keep, recent, keep_first, out_tables, lens, kept)
@@ -322,8 +318,8 @@ def kv_evict_e4m3(pages: PagesE4M3, block_tables, context_lens, keep: int, recen
         return lens, kept
     if block_tables.shape[1] == 0:
         return lens.zero_(), kept.fill_(-1)
-    a = _EvictArgs(_native(pages, (nb, G, bs, D)), block_tables.data_ptr(), context_lens.data_ptr(), N.ptr(out_tables), kept.data_ptr(), lens.data_ptr(),
-                   B, block_tables.shape[1], 0 if out_tables is None else out_tables.shape[1], keep, recent, keep_first)
+    a = _EVICT.pack(*_native(pages, shape), block_tables.data_ptr(), context_lens.data_ptr(), _ptr(out_tables), kept.data_ptr(), lens.data_ptr(),
+                    B, block_tables.shape[1], 0 if out_tables is None else out_tables.shape[1], keep, recent, keep_first)
     N.check(N.kernels().rb_e4m3_evict(a, N.stream_ptr()), "rb_e4m3_evict")
     return lens, kept
 
