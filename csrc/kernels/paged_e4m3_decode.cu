@@ -7,6 +7,8 @@
 // scores seven bits.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "pdl.cuh"
 #include "paged_e4m3.cuh"
 
@@ -27,14 +29,9 @@ __device__ __forceinline__ void e4_put(__nv_bfloat16* p, float v) { *p = __float
 __device__ __forceinline__ void e4_put(__half* p, float v) { *p = __float2half(v); }
 
 // Scratch: [batch, heads, slices, D + 4] fp32: maximum, denominator, two unused, sums of a slice; then, where weights are summed, the scores
-// [batch, KV heads, slices * 256, heads of a group] and the denominators as whole powers of two and factors [batch, heads, 2].
+// [batch, KV heads, slices * 256, heads of a group].
 __device__ __forceinline__ float* e4_partial(float* scratch, int heads, int slices, int D, int b, int h, int s) {
   return scratch + ((static_cast<long long>(b) * heads + h) * slices + s) * (D + 4);
-}
-
-__device__ __forceinline__ float* e4_norm(float* scratch, int batch, int heads, int slices, int D, int b, int h) {
-  const long long rows = static_cast<long long>(batch) * heads;
-  return scratch + rows * slices * (D + 4 + kE4Slice) + (static_cast<long long>(b) * heads + h) * 2;
 }
 
 // The tokens of a sequence that its tables have room for.
@@ -83,23 +80,17 @@ struct E4Layout {
 // rows and the heads as columns, so that no row is left empty and a lane's factors are those of its own columns; P^T, rounded to f16, takes its place as
 // the second operand by a transposition of 8 x 8 (movmatrix).  Codes become f16 exactly.  The contraction over head dimensions may take them in any
 // order, so a lane reads 16 codes of a row at a time and these are its operands of four products; a swizzled tile gives every lane its 16 bytes without
-// bank conflicts.  A query row is scaled to [1, 2) by a power of two first.
+// bank conflicts.  A query row is scaled to [1, 2) by a power of two first.  Rounding a factor p_j to f16 is off by 2^-12 of it, which the output's
+// rounding to bf16 (2^-9) hides; an output in f16 would show it, and there what the rounding left is a second operand.
 // HOW: kE4List: the slices of all sequences and KV heads, numbered one sequence after the other, are dealt in equal runs to CTAs that stay, and the next
 // slice's tiles are copied while this one's are worked on.  Otherwise the grid is (slices, KV heads, sequences); kE4Cluster: the CTAs of a sequence and KV
 // head are a cluster and merge their sums, and add the weights, through distributed shared memory.
 enum { kE4Grid, kE4List, kE4Cluster };
 
-// Sums y under the maximum my, added to x under mx.  Maxima are whole, so the factors are exact and the sum does not depend on which maximum it is under.
-__device__ __forceinline__ void e4_add(float4& x, float& mx, float& lx, const float4& y, float my, float ly) {
-  const float to = fmaxf(mx, my);
-  const float f = mx == to ? 1.f : e4_ex2(mx - to), g = my == to ? 1.f : e4_ex2(my - to);
-  x.x = fmaf(y.x, g, x.x * f);
-  x.y = fmaf(y.y, g, x.y * f);
-  x.z = fmaf(y.z, g, x.z * f);
-  x.w = fmaf(y.w, g, x.w * f);
-  lx = fmaf(ly, g, lx * f);
-  mx = to;
-}
+// The factor that brings sums under the maximum m to the maximum `to`.  Maxima are whole, so it is exact, and a sum of such sums does not depend on which
+// maximum they are brought to on the way.
+__device__ __forceinline__ float e4_factor(float m, float to) { return m == to ? 1.f : e4_ex2(m - to); }
+
 // A weight is 2^(s - m) / den = 2^(s - (m + x)) / (den / 2^x), with the x that brings den / 2^x into [1, 2): (m + x, 2^x / den).
 __device__ __forceinline__ float2 e4_norm_of(float m, float den) {
   const int x = static_cast<int>(__float_as_uint(den) >> 23) - 127;
@@ -118,6 +109,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
   constexpr int MT = D / 16;                         // tiles of 16 output dimensions
   constexpr int BR = D / 8;                          // rows of 128 bytes in a tile
   constexpr int kNone = static_cast<int>(0x80000000);
+  constexpr int PF = std::is_same<T, __half>::value ? 2 : 1;             // operands that a factor makes
   extern __shared__ uint8_t e4_raw[];
   __shared__ __align__(8) uint64_t bars[kE4Warps][kE4Stages];
   __shared__ float m_sh[kE4Warps][NH * 8], l_sh[kE4Warps][NH * 8];
@@ -368,7 +360,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
         if (coming[0] >= 0) request(i, coming[0]);
         if (coming[1] >= 0) request(i + 1, coming[1]);
       }
-      uint32_t pf[2][NH][2];
+      uint32_t pf[2][NH][2][PF];
       float grow[NH][2];
       bool moved = false;
 #pragma unroll
@@ -416,7 +408,12 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const uint32_t h2 = e4_half2_of(p[2 * c], p[2 * c + 1]);
-            asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pf[u][r][c]) : "r"(h2));
+            asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pf[u][r][c][0]) : "r"(h2));
+            if (PF > 1) {
+              const float2 got = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+              const uint32_t rest = e4_half2_of(p[2 * c] - got.x, p[2 * c + 1] - got.y);
+              asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pf[u][r][c][PF - 1]) : "r"(rest));
+            }
           }
         }
       }
@@ -450,8 +447,11 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
           e4_half4(__byte_perm(vw[u][2][w], vw[u][3][w], 0x7362), a12, a13);
 #pragma unroll
           for (int r = 0; r < NH; ++r) {
-            e4_mma(o[2 * w][r], a00, a01, a02, a03, pf[u][r][0], pf[u][r][1]);
-            e4_mma(o[2 * w + 1][r], a10, a11, a12, a13, pf[u][r][0], pf[u][r][1]);
+#pragma unroll
+            for (int x = 0; x < PF; ++x) {
+              e4_mma(o[2 * w][r], a00, a01, a02, a03, pf[u][r][0][x], pf[u][r][1][x]);
+              e4_mma(o[2 * w + 1][r], a10, a11, a12, a13, pf[u][r][0][x], pf[u][r][1][x]);
+            }
           }
         }
       }
@@ -509,7 +509,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
         e4_put(out + 2, sum.z * inv);
         e4_put(out + 3, sum.w * inv);
       }
-      if (!whole || a.accumulate) {
+      if (!whole || a.accumulate) {                  // the weights' denominators come from here too
         float* out = e4_partial(a.scratch, a.heads, slices, D, at.b, h, at.s);
         if (d == 0) *reinterpret_cast<float2*>(out) = make_float2(top, den);
         *reinterpret_cast<float4*>(out + 4 + d * 4) = sum;
@@ -522,13 +522,27 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
       else __syncthreads();
       for (int i = threadIdx.x + blockIdx.x * (kE4Warps * 32); i < heads * (D / 4); i += ranks * (kE4Warps * 32)) {
         const int head = i / (D / 4), d = i % (D / 4), at_sh = head * D + ((d ^ (head >> 1 & 3)) << 2);
-        float4 sum = *reinterpret_cast<const float4*>(all.map_shared_rank(merge + at_sh, 0));
-        float2 ml = *all.map_shared_rank(&ml_sh[head], 0);
-        for (int k = 1; k < here; ++k) {
-          const float2 other = *all.map_shared_rank(&ml_sh[head], k);
-          e4_add(sum, ml.x, ml.y, *reinterpret_cast<const float4*>(all.map_shared_rank(merge + at_sh, k)), other.x, other.y);
-        }
-        const float inv = here > 0 ? 1.f / ml.y : 0.f;                   // without tokens the sums are zero
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f), x[8];
+        float2 ml[8];
+        float top = -INFINITY, den = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < here) {
+            ml[k] = *all.map_shared_rank(&ml_sh[head], k);
+            x[k] = *reinterpret_cast<const float4*>(all.map_shared_rank(merge + at_sh, k));
+            top = fmaxf(top, ml[k].x);
+          }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < here) {
+            const float f = e4_factor(ml[k].x, top);
+            sum.x = fmaf(x[k].x, f, sum.x);
+            sum.y = fmaf(x[k].y, f, sum.y);
+            sum.z = fmaf(x[k].z, f, sum.z);
+            sum.w = fmaf(x[k].w, f, sum.w);
+            den = fmaf(ml[k].y, f, den);
+          }
+        const float inv = here > 0 ? 1.f / den : 0.f;                    // without tokens the sums are zero
         T* out = reinterpret_cast<T*>(a.out) + at.b * a.ld_o + (static_cast<long long>(at.hk) * group + h0 + head) * D + d * 4;
         e4_put(out, sum.x * inv);
         e4_put(out + 1, sum.y * inv);
@@ -537,13 +551,18 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
       }
       if (a.accumulate) {
         if (static_cast<int>(threadIdx.x) < heads) {
-          float2 ml = *all.map_shared_rank(&ml_sh[threadIdx.x], 0);
-          float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int k = 1; k < here; ++k) {
-            const float2 other = *all.map_shared_rank(&ml_sh[threadIdx.x], k);
-            e4_add(none, ml.x, ml.y, none, other.x, other.y);
-          }
-          norm_sh[threadIdx.x] = e4_norm_of(ml.x, ml.y);
+          float2 ml[8];
+          float top = -INFINITY, den = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < here) {
+              ml[k] = *all.map_shared_rank(&ml_sh[threadIdx.x], k);
+              top = fmaxf(top, ml[k].x);
+            }
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < here) den = fmaf(ml[k].y, e4_factor(ml[k].x, top), den);
+          norm_sh[threadIdx.x] = e4_norm_of(top, den);
         }
         __syncthreads();
         for (int t = threadIdx.x; t < min(kE4Slice, n_at - at.s * kE4Slice); t += kE4Warps * 32) {
@@ -576,24 +595,97 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
   }
 }
 
+constexpr int kE4Chains = 16;
+
+// Adds the attention weights of a run of slices to the tokens' sums, for the finishing kernel.
+__device__ __forceinline__ void e4_weights(const RbE4m3DecodeArgs& a, int slices, int b, int hk, int s0, int count) {
+  extern __shared__ float2 e4_ml[];                  // [heads of a group][chains], then their norms
+  const int tid = threadIdx.x, D = a.pages.head_dim, bs = a.pages.block_size, G = a.pages.kv_heads, group = a.heads / G;
+  const int n = e4_len(a, b), here = (n + kE4Slice - 1) / kE4Slice;
+  if (s0 >= here) return;
+  float2* norms = e4_ml + group * kE4Chains;
+  const int end = min(n, (s0 + count) * kE4Slice);
+  auto page_of = [&](int t) { return t < end ? e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, t / bs) : -1; };
+  int t = s0 * kE4Slice + tid, page[2] = {page_of(t), page_of(t + 128)};                 // on their way while the denominators are formed
+  for (int i = tid; i < group * kE4Chains; i += 128) {
+    const float* first = e4_partial(a.scratch, a.heads, slices, D, b, hk * group + i / kE4Chains, 0);
+    float2 sum = make_float2(-INFINITY, 0.f);
+#pragma unroll 4
+    for (int s = i % kE4Chains; s < here; s += kE4Chains) {
+      const float2 ml = *reinterpret_cast<const float2*>(first + static_cast<long long>(s) * (D + 4));
+      const float to = fmaxf(sum.x, ml.x);
+      sum = make_float2(to, fmaf(ml.y, e4_factor(ml.x, to), sum.y * e4_factor(sum.x, to)));
+    }
+    e4_ml[i] = sum;
+  }
+  __syncthreads();
+  for (int h = tid; h < group; h += 128) {
+    float top = -INFINITY, den = 0.f;
+#pragma unroll
+    for (int k = 0; k < kE4Chains; ++k) top = fmaxf(top, e4_ml[h * kE4Chains + k].x);
+#pragma unroll
+    for (int k = 0; k < kE4Chains; ++k)
+      if (k < here) den = fmaf(e4_ml[h * kE4Chains + k].y, e4_factor(e4_ml[h * kE4Chains + k].x, top), den);
+    norms[h] = e4_norm_of(top, den);
+  }
+  __syncthreads();
+  const float* scores = a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (D + 4) +
+                        (static_cast<long long>(b) * G + hk) * slices * kE4Slice * group;
+  for (; t < end; t += 256) {
+    float w[2] = {0.f, 0.f};
+    float* to[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      to[x] = page[x] < 0 ? nullptr : a.pages.weight + (static_cast<long long>(page[x]) * G + hk) * bs + (t + x * 128) % bs;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      if (!to[x]) continue;
+      const float* of = scores + static_cast<long long>(t + x * 128) * group;
+      if (group % 4 == 0) {
+        for (int h = 0; h < group; h += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(of + h);
+          w[x] = fmaf(e4_ex2(v.x - norms[h].x), norms[h].y, w[x]);
+          w[x] = fmaf(e4_ex2(v.y - norms[h + 1].x), norms[h + 1].y, w[x]);
+          w[x] = fmaf(e4_ex2(v.z - norms[h + 2].x), norms[h + 2].y, w[x]);
+          w[x] = fmaf(e4_ex2(v.w - norms[h + 3].x), norms[h + 3].y, w[x]);
+        }
+      } else {
+        for (int h = 0; h < group; ++h) w[x] = fmaf(e4_ex2(of[h] - norms[h].x), norms[h].y, w[x]);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      if (to[x]) *to[x] += w[x];
+      page[x] = page_of(t + 256 + x * 128);
+    }
+  }
+}
+
 // Adds the slices of a sequence for one head: 16 chains of every 16th slice, in order, then the chains in order.  COLS: 16-byte columns that a CTA of
 // 128 threads takes, D / 4 or, where a sequence may have many slices, 8, so that more of them read at the same time; the sums are the same.
+// Grid: (heads * D / 4 / COLS CTAs, then those that add attention weights, sequences).  The latter take `run` slices each, so that a long sequence's
+// denominators, which each of them forms from the slices' again, are not formed too often.
 template <typename T, int COLS>
 __global__ void __launch_bounds__(128)
-e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
+e4_merge_kernel(const RbE4m3DecodeArgs a, int slices, int run) {
   pdl_wait();
   pdl_launch();
-  constexpr int kChains = 16, R = 128 / COLS, PER = kChains / R;
+  constexpr int kChains = kE4Chains, R = 128 / COLS, PER = kChains / R;
   __shared__ float4 sum_sh[kChains][COLS];
   __shared__ float2 ml_sh[kChains];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, D = a.pages.head_dim, c = tid % COLS, r = tid / COLS;
-  T* out = reinterpret_cast<T*>(a.out) + b * a.ld_o + static_cast<long long>(h) * D + blockIdx.z * (COLS * 4);
+  const int b = blockIdx.y, tid = threadIdx.x, D = a.pages.head_dim, c = tid % COLS, r = tid / COLS, parts = D / 4 / COLS;
+  if (static_cast<int>(blockIdx.x) >= a.heads * parts) {
+    const int i = blockIdx.x - a.heads * parts, runs = (slices + run - 1) / run;
+    return e4_weights(a, slices, b, i / runs, i % runs * run, run);
+  }
+  const int h = blockIdx.x / parts, z = blockIdx.x % parts;
+  T* out = reinterpret_cast<T*>(a.out) + b * a.ld_o + static_cast<long long>(h) * D + z * (COLS * 4);
   const int here = (e4_len(a, b) + kE4Slice - 1) / kE4Slice;
   if (here == 0) {
     if (tid < COLS * 4) e4_put(out + tid, 0.f);
     return;
   }
-  if (here == 1 && !a.accumulate) return;            // already written
+  if (here == 1) return;                             // already written
   const float* first = e4_partial(a.scratch, a.heads, slices, D, b, h, 0);
   const long long pitch = D + 4;
   // every sum beside its own maximum; a new maximum's factor is a power of two, so that the sums are those under the largest of all
@@ -619,7 +711,7 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
         if (s < here) {
           const float* p = first + s * pitch;
           ml[k][i] = *reinterpret_cast<const float2*>(p);
-          x[k][i] = *reinterpret_cast<const float4*>(p + 4 + (blockIdx.z * COLS + c) * 4);
+          x[k][i] = *reinterpret_cast<const float4*>(p + 4 + (z * COLS + c) * 4);
         }
       }
     }
@@ -628,14 +720,14 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
       float to = m[k];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) to = fmaxf(to, ml[k][i].x);
-      const float f = m[k] == to ? 1.f : e4_ex2(m[k] - to);
+      const float f = e4_factor(m[k], to);
       sum[k].x *= f; sum[k].y *= f; sum[k].z *= f; sum[k].w *= f;
       l[k] *= f;
       m[k] = to;
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         if (s0 + k * R + i * kChains >= here) break;
-        const float g = ml[k][i].x == to ? 1.f : e4_ex2(ml[k][i].x - to);
+        const float g = e4_factor(ml[k][i].x, to);
         sum[k].x = fmaf(x[k][i].x, g, sum[k].x);
         sum[k].y = fmaf(x[k][i].y, g, sum[k].y);
         sum[k].z = fmaf(x[k][i].z, g, sum[k].z);
@@ -651,42 +743,26 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
   }
   __syncthreads();
   if (tid >= COLS) return;
-  float4 o = sum_sh[0][c];
-  float top = ml_sh[0].x, den = ml_sh[0].y;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float top = -INFINITY, den = 0.f;
 #pragma unroll
-  for (int k = 1; k < kChains; ++k)
-    if (k < here) e4_add(o, top, den, sum_sh[k][c], ml_sh[k].x, ml_sh[k].y);
-  if (here > 1) {
-    const float inv = 1.f / den;
-    e4_put(out + c * 4, o.x * inv);
-    e4_put(out + c * 4 + 1, o.y * inv);
-    e4_put(out + c * 4 + 2, o.z * inv);
-    e4_put(out + c * 4 + 3, o.w * inv);
-  }
-  if (a.accumulate && tid == 0 && blockIdx.z == 0) {
-    float* norm = e4_norm(a.scratch, a.batch, a.heads, slices, D, b, h);
-    const float2 x = e4_norm_of(top, den);
-    norm[0] = x.x;
-    norm[1] = x.y;
-  }
-}
-
-__global__ void __launch_bounds__(256)
-e4_weight_kernel(const RbE4m3DecodeArgs a, int slices) {
-  pdl_wait();
-  pdl_launch();
-  const int s = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, D = a.pages.head_dim;
-  const int bs = a.pages.block_size, G = a.pages.kv_heads, group = a.heads / G;
-  const int t = s * kE4Slice + threadIdx.x;
-  if (t >= e4_len(a, b)) return;
-  const float* scores = a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (D + 4);
-  float w = 0.f;
-  for (int h = 0; h < group; ++h) {
-    const float* norm = e4_norm(a.scratch, a.batch, a.heads, slices, D, b, hk * group + h);
-    w = fmaf(e4_ex2(scores[((static_cast<long long>(b) * G + hk) * slices * kE4Slice + t) * group + h] - norm[0]), norm[1], w);
-  }
-  const int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, t / bs);
-  if (page >= 0) a.pages.weight[(static_cast<long long>(page) * G + hk) * bs + t % bs] += w;
+  for (int k = 0; k < kChains; ++k) top = fmaxf(top, ml_sh[k].x);      // -infinity where there is no such slice
+#pragma unroll
+  for (int k = 0; k < kChains; ++k)
+    if (k < here) {
+      const float f = e4_factor(ml_sh[k].x, top);
+      const float4 x = sum_sh[k][c];
+      o.x = fmaf(x.x, f, o.x);
+      o.y = fmaf(x.y, f, o.y);
+      o.z = fmaf(x.z, f, o.z);
+      o.w = fmaf(x.w, f, o.w);
+      den = fmaf(ml_sh[k].y, f, den);
+    }
+  const float inv = 1.f / den;
+  e4_put(out + c * 4, o.x * inv);
+  e4_put(out + c * 4 + 1, o.y * inv);
+  e4_put(out + c * 4 + 2, o.z * inv);
+  e4_put(out + c * 4 + 3, o.w * inv);
 }
 
 }  // namespace rb
@@ -738,11 +814,10 @@ int decode_launch(const RbE4m3DecodeArgs& a, cudaStream_t stream) {
     e = rbhost::launch_pdl(kern, list ? dim3(some) : whole, threads, smem, stream, 1, *km, *vm, a, h0, slices, status RB_BOUNDS_ARG);
   if (e == cudaSuccess) {
     const bool many = slices > 64;
-    e = rbhost::launch_pdl(many ? rb::e4_merge_kernel<T, 8> : rb::e4_merge_kernel<T, D / 4>, dim3(a.heads, a.batch, many ? D / 32 : 1), dim3(128), 0, stream, 1,
-                           a, slices);
+    const int run = (slices + 31) / 32, adds = a.accumulate ? (slices + run - 1) / run * p.kv_heads : 0;
+    e = rbhost::launch_pdl(many ? rb::e4_merge_kernel<T, 8> : rb::e4_merge_kernel<T, D / 4>, dim3(a.heads * (many ? D / 32 : 1) + adds, a.batch), dim3(128),
+                           a.accumulate ? group * (rb::kE4Chains + 1) * sizeof(float2) : 0, stream, 1, a, slices, run);
   }
-  if (e == cudaSuccess && a.accumulate)
-    e = rbhost::launch_pdl(rb::e4_weight_kernel, dim3(slices, p.kv_heads, a.batch), dim3(256), 0, stream, 1, a, slices);
   return static_cast<int>(e);
 }
 template <typename T>
@@ -756,7 +831,7 @@ int decode_by_dim(const RbE4m3DecodeArgs& a, cudaStream_t s) {
 RB_API long long rb_e4m3_decode_scratch_floats(int batch, int heads, int kv_heads, int head_dim, int max_blocks, int block_size, int accumulate) {
   const long long slices = e4_slices(max_blocks, block_size), rows = static_cast<long long>(batch) * heads;
   if (in_clusters(batch, kv_heads, slices, heads / kv_heads)) return 0;
-  return rows * slices * (head_dim + 4) + (accumulate ? rows * (slices * rb::kE4Slice + 2) : 0);
+  return rows * slices * (head_dim + 4) + (accumulate ? rows * slices * rb::kE4Slice : 0);
 }
 
 RB_API int rb_e4m3_decode(const RbE4m3DecodeArgs* args, void* stream_v) {
@@ -765,7 +840,7 @@ RB_API int rb_e4m3_decode(const RbE4m3DecodeArgs* args, void* stream_v) {
   if (const int bad = rbhost::e4_check(a.pages)) return bad;
   if (!a.q || !a.out || !a.block_tables || !a.context_lens || a.max_blocks <= 0 || a.heads <= 0 || a.heads % a.pages.kv_heads ||
       (!a.scratch && !in_clusters(a.batch, a.pages.kv_heads, e4_slices(a.max_blocks, a.pages.block_size), a.heads / a.pages.kv_heads)) ||
-      a.batch > 65535 || a.pages.kv_heads > 65535 || (a.accumulate && !a.pages.weight) ||
+      a.batch > 65535 || a.pages.kv_heads > 65535 || (a.accumulate && (!a.pages.weight || a.heads / a.pages.kv_heads > 256)) ||
       static_cast<long long>(a.batch) * a.pages.kv_heads * e4_slices(a.max_blocks, a.pages.block_size) > 0x3fffffff)
     return -1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_v);
