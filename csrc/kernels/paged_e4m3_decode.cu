@@ -29,11 +29,15 @@ __device__ __forceinline__ void e4_put(__nv_bfloat16* p, float v) { *p = __float
 __device__ __forceinline__ void e4_put(__half* p, float v) { *p = __float2half(v); }
 
 // Scratch: [batch, heads, slices, D + 4] fp32: maximum, denominator, two unused, sums of a slice; then, where weights are summed, the scores
-// [batch, KV heads, slices * 256, heads of a group].
+// [batch, KV heads, slices * 256, heads of a group] and what makes weights of them [batch, heads, 2].
 __device__ __forceinline__ float* e4_partial(float* scratch, int heads, int slices, int D, int b, int h, int s) {
   return scratch + ((static_cast<long long>(b) * heads + h) * slices + s) * (D + 4);
 }
 
+__device__ __forceinline__ float2* e4_norm(const RbE4m3DecodeArgs& a, int slices, int b, int h) {
+  const long long rows = static_cast<long long>(a.batch) * a.heads;
+  return reinterpret_cast<float2*>(a.scratch + rows * slices * (a.pages.head_dim + 4 + kE4Slice)) + static_cast<long long>(b) * a.heads + h;
+}
 // The tokens of a sequence that its tables have room for.
 __device__ __forceinline__ int e4_len(const RbE4m3DecodeArgs& a, int b) {
   const long long room = static_cast<long long>(a.max_blocks) * a.pages.block_size;
@@ -597,95 +601,25 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
 
 constexpr int kE4Chains = 16;
 
-// Adds the attention weights of a run of slices to the tokens' sums, for the finishing kernel.
-__device__ __forceinline__ void e4_weights(const RbE4m3DecodeArgs& a, int slices, int b, int hk, int s0, int count) {
-  extern __shared__ float2 e4_ml[];                  // [heads of a group][chains], then their norms
-  const int tid = threadIdx.x, D = a.pages.head_dim, bs = a.pages.block_size, G = a.pages.kv_heads, group = a.heads / G;
-  const int n = e4_len(a, b), here = (n + kE4Slice - 1) / kE4Slice;
-  if (s0 >= here) return;
-  float2* norms = e4_ml + group * kE4Chains;
-  const int end = min(n, (s0 + count) * kE4Slice);
-  auto page_of = [&](int t) { return t < end ? e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, t / bs) : -1; };
-  int t = s0 * kE4Slice + tid, page[2] = {page_of(t), page_of(t + 128)};                 // on their way while the denominators are formed
-  for (int i = tid; i < group * kE4Chains; i += 128) {
-    const float* first = e4_partial(a.scratch, a.heads, slices, D, b, hk * group + i / kE4Chains, 0);
-    float2 sum = make_float2(-INFINITY, 0.f);
-#pragma unroll 4
-    for (int s = i % kE4Chains; s < here; s += kE4Chains) {
-      const float2 ml = *reinterpret_cast<const float2*>(first + static_cast<long long>(s) * (D + 4));
-      const float to = fmaxf(sum.x, ml.x);
-      sum = make_float2(to, fmaf(ml.y, e4_factor(ml.x, to), sum.y * e4_factor(sum.x, to)));
-    }
-    e4_ml[i] = sum;
-  }
-  __syncthreads();
-  for (int h = tid; h < group; h += 128) {
-    float top = -INFINITY, den = 0.f;
-#pragma unroll
-    for (int k = 0; k < kE4Chains; ++k) top = fmaxf(top, e4_ml[h * kE4Chains + k].x);
-#pragma unroll
-    for (int k = 0; k < kE4Chains; ++k)
-      if (k < here) den = fmaf(e4_ml[h * kE4Chains + k].y, e4_factor(e4_ml[h * kE4Chains + k].x, top), den);
-    norms[h] = e4_norm_of(top, den);
-  }
-  __syncthreads();
-  const float* scores = a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (D + 4) +
-                        (static_cast<long long>(b) * G + hk) * slices * kE4Slice * group;
-  for (; t < end; t += 256) {
-    float w[2] = {0.f, 0.f};
-    float* to[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-      to[x] = page[x] < 0 ? nullptr : a.pages.weight + (static_cast<long long>(page[x]) * G + hk) * bs + (t + x * 128) % bs;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if (!to[x]) continue;
-      const float* of = scores + static_cast<long long>(t + x * 128) * group;
-      if (group % 4 == 0) {
-        for (int h = 0; h < group; h += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(of + h);
-          w[x] = fmaf(e4_ex2(v.x - norms[h].x), norms[h].y, w[x]);
-          w[x] = fmaf(e4_ex2(v.y - norms[h + 1].x), norms[h + 1].y, w[x]);
-          w[x] = fmaf(e4_ex2(v.z - norms[h + 2].x), norms[h + 2].y, w[x]);
-          w[x] = fmaf(e4_ex2(v.w - norms[h + 3].x), norms[h + 3].y, w[x]);
-        }
-      } else {
-        for (int h = 0; h < group; ++h) w[x] = fmaf(e4_ex2(of[h] - norms[h].x), norms[h].y, w[x]);
-      }
-    }
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if (to[x]) *to[x] += w[x];
-      page[x] = page_of(t + 256 + x * 128);
-    }
-  }
-}
-
 // Adds the slices of a sequence for one head: 16 chains of every 16th slice, in order, then the chains in order.  COLS: 16-byte columns that a CTA of
 // 128 threads takes, D / 4 or, where a sequence may have many slices, 8, so that more of them read at the same time; the sums are the same.
-// Grid: (heads * D / 4 / COLS CTAs, then those that add attention weights, sequences).  The latter take `run` slices each, so that a long sequence's
-// denominators, which each of them forms from the slices' again, are not formed too often.
+// Grid: (heads, sequences, D / 4 / COLS).
 template <typename T, int COLS>
 __global__ void __launch_bounds__(128)
-e4_merge_kernel(const RbE4m3DecodeArgs a, int slices, int run) {
+e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
   pdl_wait();
   pdl_launch();
   constexpr int kChains = kE4Chains, R = 128 / COLS, PER = kChains / R;
   __shared__ float4 sum_sh[kChains][COLS];
   __shared__ float2 ml_sh[kChains];
-  const int b = blockIdx.y, tid = threadIdx.x, D = a.pages.head_dim, c = tid % COLS, r = tid / COLS, parts = D / 4 / COLS;
-  if (static_cast<int>(blockIdx.x) >= a.heads * parts) {
-    const int i = blockIdx.x - a.heads * parts, runs = (slices + run - 1) / run;
-    return e4_weights(a, slices, b, i / runs, i % runs * run, run);
-  }
-  const int h = blockIdx.x / parts, z = blockIdx.x % parts;
+  const int h = blockIdx.x, b = blockIdx.y, z = blockIdx.z, tid = threadIdx.x, D = a.pages.head_dim, c = tid % COLS, r = tid / COLS;
   T* out = reinterpret_cast<T*>(a.out) + b * a.ld_o + static_cast<long long>(h) * D + z * (COLS * 4);
   const int here = (e4_len(a, b) + kE4Slice - 1) / kE4Slice;
   if (here == 0) {
     if (tid < COLS * 4) e4_put(out + tid, 0.f);
     return;
   }
-  if (here == 1) return;                             // already written
+  if (here == 1 && !a.accumulate) return;            // already written
   const float* first = e4_partial(a.scratch, a.heads, slices, D, b, h, 0);
   const long long pitch = D + 4;
   // every sum beside its own maximum; a new maximum's factor is a power of two, so that the sums are those under the largest of all
@@ -758,11 +692,44 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices, int run) {
       o.w = fmaf(x.w, f, o.w);
       den = fmaf(ml_sh[k].y, f, den);
     }
-  const float inv = 1.f / den;
-  e4_put(out + c * 4, o.x * inv);
-  e4_put(out + c * 4 + 1, o.y * inv);
-  e4_put(out + c * 4 + 2, o.z * inv);
-  e4_put(out + c * 4 + 3, o.w * inv);
+  if (here > 1) {
+    const float inv = 1.f / den;
+    e4_put(out + c * 4, o.x * inv);
+    e4_put(out + c * 4 + 1, o.y * inv);
+    e4_put(out + c * 4 + 2, o.z * inv);
+    e4_put(out + c * 4 + 3, o.w * inv);
+  }
+  if (a.accumulate && tid == 0 && z == 0) *e4_norm(a, slices, b, h) = e4_norm_of(top, den);
+}
+
+// Adds the attention weights of a slice to its tokens' sums, a thread a token.  (As a part of the merge, with denominators formed in every CTA, it was
+// slower, 33 against 31 us for 24 sequences of 128 to 2560: the merge's registers leave room for fewer of its threads, and it waits for memory.)
+__global__ void __launch_bounds__(kE4Slice)
+e4_weight_kernel(const RbE4m3DecodeArgs a, int slices) {
+  pdl_wait();
+  pdl_launch();
+  const int hk = blockIdx.y, b = blockIdx.z, bs = a.pages.block_size, G = a.pages.kv_heads, group = a.heads / G;
+  const int t = blockIdx.x * kE4Slice + threadIdx.x;
+  if (t >= e4_len(a, b)) return;
+  const int page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, t / bs);
+  if (page < 0) return;
+  float* to = a.pages.weight + (static_cast<long long>(page) * G + hk) * bs + t % bs;
+  const float* scores = a.scratch + static_cast<long long>(a.batch) * a.heads * slices * (a.pages.head_dim + 4) +
+                        ((static_cast<long long>(b) * G + hk) * slices * kE4Slice + t) * group;
+  const float2* norms = e4_norm(a, slices, b, hk * group);
+  float w = 0.f;
+  if (group % 4 == 0) {
+    for (int h = 0; h < group; h += 4) {
+      const float4 s = *reinterpret_cast<const float4*>(scores + h);
+      w = fmaf(e4_ex2(s.x - norms[h].x), norms[h].y, w);
+      w = fmaf(e4_ex2(s.y - norms[h + 1].x), norms[h + 1].y, w);
+      w = fmaf(e4_ex2(s.z - norms[h + 2].x), norms[h + 2].y, w);
+      w = fmaf(e4_ex2(s.w - norms[h + 3].x), norms[h + 3].y, w);
+    }
+  } else {
+    for (int h = 0; h < group; ++h) w = fmaf(e4_ex2(scores[h] - norms[h].x), norms[h].y, w);
+  }
+  *to += w;
 }
 
 }  // namespace rb
@@ -814,10 +781,10 @@ int decode_launch(const RbE4m3DecodeArgs& a, cudaStream_t stream) {
     e = rbhost::launch_pdl(kern, list ? dim3(some) : whole, threads, smem, stream, 1, *km, *vm, a, h0, slices, status RB_BOUNDS_ARG);
   if (e == cudaSuccess) {
     const bool many = slices > 64;
-    const int run = (slices + 31) / 32, adds = a.accumulate ? (slices + run - 1) / run * p.kv_heads : 0;
-    e = rbhost::launch_pdl(many ? rb::e4_merge_kernel<T, 8> : rb::e4_merge_kernel<T, D / 4>, dim3(a.heads * (many ? D / 32 : 1) + adds, a.batch), dim3(128),
-                           a.accumulate ? group * (rb::kE4Chains + 1) * sizeof(float2) : 0, stream, 1, a, slices, run);
+    e = rbhost::launch_pdl(many ? rb::e4_merge_kernel<T, 8> : rb::e4_merge_kernel<T, D / 4>, dim3(a.heads, a.batch, many ? D / 32 : 1), dim3(128), 0, stream, 1,
+                           a, slices);
   }
+  if (e == cudaSuccess && a.accumulate) e = rbhost::launch_pdl(rb::e4_weight_kernel, whole, dim3(rb::kE4Slice), 0, stream, 1, a, slices);
   return static_cast<int>(e);
 }
 template <typename T>
@@ -831,7 +798,7 @@ int decode_by_dim(const RbE4m3DecodeArgs& a, cudaStream_t s) {
 RB_API long long rb_e4m3_decode_scratch_floats(int batch, int heads, int kv_heads, int head_dim, int max_blocks, int block_size, int accumulate) {
   const long long slices = e4_slices(max_blocks, block_size), rows = static_cast<long long>(batch) * heads;
   if (in_clusters(batch, kv_heads, slices, heads / kv_heads)) return 0;
-  return rows * slices * (head_dim + 4) + (accumulate ? rows * slices * rb::kE4Slice : 0);
+  return rows * slices * (head_dim + 4) + (accumulate ? rows * (slices * rb::kE4Slice + 2) : 0);
 }
 
 RB_API int rb_e4m3_decode(const RbE4m3DecodeArgs* args, void* stream_v) {
@@ -840,7 +807,7 @@ RB_API int rb_e4m3_decode(const RbE4m3DecodeArgs* args, void* stream_v) {
   if (const int bad = rbhost::e4_check(a.pages)) return bad;
   if (!a.q || !a.out || !a.block_tables || !a.context_lens || a.max_blocks <= 0 || a.heads <= 0 || a.heads % a.pages.kv_heads ||
       (!a.scratch && !in_clusters(a.batch, a.pages.kv_heads, e4_slices(a.max_blocks, a.pages.block_size), a.heads / a.pages.kv_heads)) ||
-      a.batch > 65535 || a.pages.kv_heads > 65535 || (a.accumulate && (!a.pages.weight || a.heads / a.pages.kv_heads > 256)) ||
+      a.batch > 65535 || a.pages.kv_heads > 65535 || (a.accumulate && !a.pages.weight) ||
       static_cast<long long>(a.batch) * a.pages.kv_heads * e4_slices(a.max_blocks, a.pages.block_size) > 0x3fffffff)
     return -1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_v);

@@ -274,8 +274,6 @@ def paged_attention_decode_e4m3(q, pages: PagesE4M3, block_tables, context_lens,
         return out
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError("paged_attention_decode_e4m3: CUDA queries are bf16 or fp16")
-    if accumulate and heads > 256 * G:
-        raise ValueError("paged_attention_decode_e4m3: weights of more than 256 query heads a KV head")
     if B == 0:
         return out
     if q.stride(1) != 1:
