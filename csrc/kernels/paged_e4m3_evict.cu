@@ -8,8 +8,8 @@ namespace rb {
 
 namespace cg = cooperative_groups;
 
-constexpr int kE4SelectThreads = 1024, kE4SelectWarps = 32;
-constexpr int kE4SelectKeys = 16;                    // keys that a thread holds
+constexpr int kE4SelectThreads = 1024, kE4SelectWarps = kE4SelectThreads / 32;
+constexpr int kE4SelectKeys = 16384;                 // keys that a CTA holds
 
 // order-preserving: larger weights have larger keys, -0 is 0, a NaN is largest
 __device__ __forceinline__ uint32_t e4_key(float w) {
@@ -18,18 +18,19 @@ __device__ __forceinline__ uint32_t e4_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// The places that stay, for a sequence and KV head.  The `take`-th largest key of the tokens that may go is found by radix selection, four passes of
-// eight bits over keys in registers; every pass counts the next digit of the keys that still may be it.  Then each warp counts what stays of its tokens,
-// and writes it where the counts in front of it end.  Sequences of more than 16384 tokens are shared by the CTAs of a cluster (x: rank in the cluster),
-// which add their counts through distributed shared memory; behind 131072 the keys are read from the pages again in every pass.
-// Bound by its instructions, not by the weights' bytes.  One B200, 24 sequences of 1500 to 8192 tokens, 8 KV heads: 94 us with one thread that looks
-// for the digit and keys read from the pages in every pass, 25 with keys in shared memory.
+// The places that stay, for a sequence and KV head.  The `take`-th largest key of the tokens that may go is found by radix selection, passes of
+// 11, 11 and 10 bits over keys in shared memory; every pass counts the next digit of the keys that still may be it (weights have few exponents, and
+// threads that count the same digit wait for one another, so digits are long).  Then each warp counts what stays of its tokens, and writes it where the
+// counts in front of it end.  Sequences of more than 16384 tokens are shared by the CTAs of a cluster (x: rank in the cluster), which add their counts
+// through distributed shared memory; of more than 131072, the keys are read from the pages again in every pass.
+// Bound by latencies: table, weight and the passes' barriers follow one another.
 template <bool CLUSTER>
-__global__ void __launch_bounds__(kE4SelectThreads)
+__global__ void __launch_bounds__(kE4SelectThreads, 2)
 e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
   pdl_wait();
   pdl_launch();
-  __shared__ uint32_t hist[256], part[2], digit[2];
+  extern __shared__ uint32_t e4_keys[];
+  __shared__ uint32_t hist[2048], part[2], digit[2];
   __shared__ uint32_t warp_n[2][kE4SelectWarps];
   const int ranks = CLUSTER ? gridDim.x : 1, rank = CLUSTER ? blockIdx.x : 0;
   const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -50,85 +51,91 @@ e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
   const int lo = first + min(count, rank * share), mine = first + min(count, (rank + 1) * share) - lo;
   const int span = (mine + kE4SelectThreads - 1) / kE4SelectThreads * 32, w0 = warp * span, w1 = min(mine, w0 + span);
   const int* table = a.block_tables + static_cast<long long>(b) * a.max_blocks;
-  auto from_page = [&](int t) {
-    const int i = per_page == 1 ? t >> 4 : t / bs, off = per_page == 1 ? t & 15 : t - i * bs;
-    const int page = table[i];
-    if (page < 0 || page >= a.pages.num_blocks) {
-      RB_BOUNDS_HIT(104);
-      return 0u;
-    }
-    return e4_key(a.pages.weight[(static_cast<long long>(page) * G + h) * bs + off]);
+  auto page_of = [&](int t) { return table[per_page == 1 ? t >> 4 : t / bs]; };
+  const float* weights = a.pages.weight + static_cast<long long>(h) * bs;
+  const unsigned int blocks = static_cast<unsigned int>(a.pages.num_blocks);
+  const long long per_block = static_cast<long long>(G) * bs;
+  auto key_of = [&](int t, int page) {
+    const bool there = static_cast<unsigned int>(page) < blocks;
+    if (!there) RB_BOUNDS_HIT(104);
+    const float w = weights[(there ? page : 0) * per_block + (per_page == 1 ? t & 15 : t % bs)];
+    return there ? e4_key(w) : 0u;
   };
-  const bool held = span <= kE4SelectKeys * 32;
-  uint32_t keys[kE4SelectKeys];
+  const bool held = mine <= kE4SelectKeys;
+  if (held)
+    for (int i0 = tid; i0 < mine; i0 += 4 * kE4SelectThreads) {         // four pages, then four weights: loads that do not wait for one another
+      int page[4];
+      uint32_t k[4];
 #pragma unroll
-  for (int x = 0; x < kE4SelectKeys; ++x) {
-    keys[x] = 0u;
-    if (held && w0 + x * 32 + lane < w1) keys[x] = from_page(lo + w0 + x * 32 + lane);
-  }
+      for (int x = 0; x < 4; ++x) page[x] = page_of(lo + min(i0 + x * kE4SelectThreads, mine - 1));
+#pragma unroll
+      for (int x = 0; x < 4; ++x) k[x] = key_of(lo + min(i0 + x * kE4SelectThreads, mine - 1), page[x]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (i0 + x * kE4SelectThreads < mine) e4_keys[i0 + x * kE4SelectThreads] = k[x];
+    }
+  __syncthreads();
   // f(place, key) for this warp's tokens, 32 at a time; a lane without a token has place -1
   auto each = [&](auto f) {
-    if (held) {
-#pragma unroll
-      for (int x = 0; x < kE4SelectKeys; ++x) {
-        if (w0 + x * 32 >= w1) break;
-        f(w0 + x * 32 + lane < w1 ? lo + w0 + x * 32 + lane : -1, keys[x]);
-      }
-    } else {
-#pragma unroll 1
-      for (int i = w0 + lane; i - lane < w1; i += 32) f(i < w1 ? lo + i : -1, i < w1 ? from_page(lo + i) : 0u);
-    }
+#pragma unroll 4
+    for (int i = w0 + lane; i - lane < w1; i += 32) f(i < w1 ? lo + i : -1, i >= w1 ? 0u : held ? e4_keys[i] : key_of(lo + i, page_of(lo + i)));
   };
   uint32_t prefix = 0, mask = 0, need = take;        // keys that begin with `prefix`; how many of them stay
 #pragma unroll 1
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t digits = pass < 2 ? 2047u : 1023u;
+    constexpr int kBins = 2048 / kE4SelectThreads;   // of a thread
+#pragma unroll
+    for (int j = 0; j < kBins; ++j) hist[tid + j * kE4SelectThreads] = 0;
     __syncthreads();
     each([&](int t, uint32_t k) {
-      if (t >= 0 && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
+      if (t >= 0 && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digits], 1u);
     });
     if (CLUSTER) cg::this_cluster().sync();
     else __syncthreads();
-    if (warp == 0) {                                 // lane i: digits 255 - 8 i downwards
-      uint32_t c[8], sum = 0;
+    uint32_t c[kBins], sum = 0;                      // digits 2047 - kBins * tid downwards
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        c[j] = hist[255 - lane * 8 - j];
-        if (CLUSTER) {
-          for (int r = 1; r < ranks; ++r) c[j] += *cg::this_cluster().map_shared_rank(&hist[255 - lane * 8 - j], (rank + r) % ranks);
+    for (int j = 0; j < kBins; ++j) {
+      uint32_t* bin = &hist[2047 - tid * kBins - j];
+      c[j] = *bin;
+      if (CLUSTER)
+        for (int r = 1; r < ranks; ++r) c[j] += *cg::this_cluster().map_shared_rank(bin, (rank + r) % ranks);
+      sum += c[j];
+    }
+    uint32_t upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) warp_n[0][warp] = upto;
+    __syncthreads();
+    uint32_t above = upto - sum + __reduce_add_sync(0xffffffffu, lane < warp ? warp_n[0][lane] : 0u);
+    if (above < need && need <= above + sum) {       // one thread
+#pragma unroll
+      for (int j = 0; j < kBins; ++j) {
+        if (above < need && need <= above + c[j]) {
+          digit[0] = 2047 - tid * kBins - j;
+          digit[1] = need - above;
         }
-        sum += c[j];
-      }
-      uint32_t upto = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-      }
-      uint32_t above = upto - sum;
-      if (above < need && need <= upto) {            // one lane
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (above < need && need <= above + c[j]) {
-            digit[0] = 255 - lane * 8 - j;
-            digit[1] = need - above;
-          }
-          above += c[j];
-        }
+        above += c[j];
       }
     }
     if (CLUSTER) cg::this_cluster().sync();          // and nobody reads another's counts any more
     else __syncthreads();
     prefix |= digit[0] << shift;
-    mask |= 255u << shift;
+    mask |= digits << shift;
     need = digit[1];
   }
   // keys above `prefix` stay, and of those equal to it the first `need`
   uint32_t above = 0, equal = 0;                     // of this warp
   each([&](int t, uint32_t k) {
-    above += __popc(__ballot_sync(0xffffffffu, t >= 0 && k > prefix));
-    equal += __popc(__ballot_sync(0xffffffffu, t >= 0 && k == prefix));
+    above += t >= 0 && k > prefix ? 1 : 0;
+    equal += t >= 0 && k == prefix ? 1 : 0;
   });
+  above = __reduce_add_sync(0xffffffffu, above);
+  equal = __reduce_add_sync(0xffffffffu, equal);
   if (lane == 0) {
     warp_n[0][warp] = above;
     warp_n[1][warp] = equal;
@@ -137,7 +144,7 @@ e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
   uint32_t before[2];                                // keys above and equal in the warps in front
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    const uint32_t v = warp_n[x][lane], all = __reduce_add_sync(0xffffffffu, v);
+    const uint32_t v = lane < kE4SelectWarps ? warp_n[x][lane] : 0u, all = __reduce_add_sync(0xffffffffu, v);
     before[x] = __reduce_add_sync(0xffffffffu, lane < warp ? v : 0u);
     if (CLUSTER && tid == 0) part[x] = all;
   }
@@ -160,12 +167,12 @@ e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
   if (CLUSTER) cg::this_cluster().sync();            // others may still read this CTA's counts
 }
 
-constexpr int kE4MoveThreads = 256, kE4MoveTokens = 128;
+constexpr int kE4MoveThreads = 256, kE4MoveTokens = 64;
 
-// Moves the kept tokens of a sequence and KV head.  A CTA takes whole pages, as many as have at most 128 tokens (or one that has more, in parts).
+// Moves the kept tokens of a sequence and KV head.  A CTA takes whole pages, as many as have at most 64 tokens (or one that has more, in parts).
 // INPLACE: the CTAs of a cluster take neighbouring runs of pages and go on together.  A token moves to a place in front of its own, or stays, so what
 // one round writes lies in front of all that later rounds read; within a round all tokens are in registers before the first is written.  Pages of more
-// than 128 tokens are taken by one CTA, where the same holds from part to part.  Otherwise the pages are of no other use and the grid has a CTA for
+// than 64 tokens are taken by one CTA, where the same holds from part to part.  Otherwise the pages are of no other use and the grid has a CTA for
 // each run of pages.
 template <int D, bool INPLACE>
 __global__ void __launch_bounds__(kE4MoveThreads)
@@ -311,9 +318,19 @@ RB_API int rb_e4m3_evict(const RbE4m3EvictArgs* args, void* stream_v) {
     return -1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_v);
   int cluster = 1;                                   // as many CTAs for a sequence and head as hold its keys
-  while (cluster < 8 && static_cast<long long>(cluster) * rb::kE4SelectKeys * rb::kE4SelectThreads < tokens) cluster *= 2;
+  while (cluster < 8 && static_cast<long long>(cluster) * rb::kE4SelectKeys < tokens) cluster *= 2;
+  const long long share = (tokens + cluster - 1) / cluster;
+  const size_t smem = static_cast<size_t>(share < rb::kE4SelectKeys ? share : rb::kE4SelectKeys) * 4;
+  static bool set[64] = {};
+  const int dev = rbhost::device_slot();
+  if (!set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(rb::e4_select_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, rb::kE4SelectKeys * 4);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(rb::e4_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, rb::kE4SelectKeys * 4);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    set[dev] = true;
+  }
   cudaError_t e = rbhost::launch_pdl(cluster > 1 ? rb::e4_select_kernel<true> : rb::e4_select_kernel<false>, dim3(cluster, a.pages.kv_heads, a.batch),
-                                     dim3(rb::kE4SelectThreads), 0, s, cluster, a RB_BOUNDS_ARG);
+                                     dim3(rb::kE4SelectThreads), smem, s, cluster, a RB_BOUNDS_ARG);
   if (e == cudaSuccess) e = a.pages.head_dim == 64 ? move_tokens<64>(a, s) : move_tokens<128>(a, s);
   return static_cast<int>(e);
 }
