@@ -8,7 +8,7 @@ namespace rb {
 
 namespace cg = cooperative_groups;
 
-constexpr int kE4SelectThreads = 1024, kE4SelectWarps = kE4SelectThreads / 32;
+constexpr int kE4SelectThreads = 512, kE4SelectWarps = kE4SelectThreads / 32;
 constexpr int kE4SelectKeys = 16384;                 // keys that a CTA holds
 
 // order-preserving: larger weights have larger keys, -0 is 0, a NaN is largest
@@ -25,7 +25,7 @@ __device__ __forceinline__ uint32_t e4_key(float w) {
 // through distributed shared memory; of more than 131072, the keys are read from the pages again in every pass.
 // Bound by latencies: table, weight and the passes' barriers follow one another.
 template <bool CLUSTER>
-__global__ void __launch_bounds__(kE4SelectThreads, 2)
+__global__ void __launch_bounds__(kE4SelectThreads, 3)
 e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
   pdl_wait();
   pdl_launch();
@@ -77,8 +77,13 @@ e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
   __syncthreads();
   // f(place, key) for this warp's tokens, 32 at a time; a lane without a token has place -1
   auto each = [&](auto f) {
+    if (held) {
+#pragma unroll 2
+      for (int i = w0 + lane; i - lane < w1; i += 32) f(i < w1 ? lo + i : -1, i < w1 ? e4_keys[i] : 0u);
+    } else {
 #pragma unroll 4
-    for (int i = w0 + lane; i - lane < w1; i += 32) f(i < w1 ? lo + i : -1, i >= w1 ? 0u : held ? e4_keys[i] : key_of(lo + i, page_of(lo + i)));
+      for (int i = w0 + lane; i - lane < w1; i += 32) f(i < w1 ? lo + i : -1, i < w1 ? key_of(lo + i, page_of(lo + i)) : 0u);
+    }
   };
   uint32_t prefix = 0, mask = 0, need = take;        // keys that begin with `prefix`; how many of them stay
 #pragma unroll 1
