@@ -103,6 +103,20 @@ int rb_ba_free(RbBlockAllocator* a, int64_t seq_id) {
   return n;
 }
 
+// Gives back the blocks behind the first num_tokens tokens of a sequence, which keeps its other blocks and its state slot.  Returns their
+// number, -1 for an unknown sequence.
+int rb_ba_trim(RbBlockAllocator* a, int64_t seq_id, int num_tokens) {
+  std::lock_guard<std::mutex> l(a->mu);
+  auto it = a->tables.find(seq_id);
+  if (it == a->tables.end() || num_tokens < 0) return -1;
+  int n = 0;
+  for (const size_t keep = blocks_for(a, num_tokens); it->second.size() > keep; ++n) {
+    a->free_list.push_back(it->second.back());
+    it->second.pop_back();
+  }
+  return n;
+}
+
 int rb_ba_table_len(const RbBlockAllocator* a, int64_t seq_id) {
   std::lock_guard<std::mutex> l(a->mu);
   auto it = a->tables.find(seq_id);

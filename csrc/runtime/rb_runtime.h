@@ -19,6 +19,7 @@ int rb_ba_reserve(RbBlockAllocator* a, int64_t seq_id, int num_tokens);
 // Can `num_tokens` more tokens be held for this sequence (existing or new) without running out of blocks?
 int rb_ba_can_reserve(const RbBlockAllocator* a, int64_t seq_id, int num_tokens);
 int rb_ba_free(RbBlockAllocator* a, int64_t seq_id);           // returns the number of blocks released
+int rb_ba_trim(RbBlockAllocator* a, int64_t seq_id, int num_tokens);               // blocks behind num_tokens tokens; returns their number
 int rb_ba_table_len(const RbBlockAllocator* a, int64_t seq_id);
 int rb_ba_table(const RbBlockAllocator* a, int64_t seq_id, int32_t* out, int max_out);   // copies the table; returns its length
 int64_t rb_ba_slot(const RbBlockAllocator* a, int64_t seq_id, int token_index);          // block * block_size + offset, -1 if unmapped

@@ -36,6 +36,7 @@ def declare_runtime(lib) -> None:
     _sig(lib, "rb_ba_reserve", [P, LL, I], I)
     _sig(lib, "rb_ba_can_reserve", [P, LL, I], I)
     _sig(lib, "rb_ba_free", [P, LL], I)
+    _sig(lib, "rb_ba_trim", [P, LL, I], I)
     _sig(lib, "rb_ba_table_len", [P, LL], I)
     _sig(lib, "rb_ba_table", [P, LL, P, I], I)
     _sig(lib, "rb_ba_tables", [P, P, I, I, P], I)

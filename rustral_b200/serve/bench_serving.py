@@ -25,6 +25,7 @@ import torch.distributed as dist
 
 from ..models.registry import build_weights, load_tensors, resolve_config
 from .engine import ServingEngine, run_poisson_workload
+from .kv_cache import CacheQuantization
 from .model_runner import ModelRunner
 
 
@@ -39,6 +40,7 @@ def main(argv=None):
     ap.add_argument("--max-batch", type=int, default=64)
     ap.add_argument("--blocks", type=int, default=16384)
     ap.add_argument("--page", type=int, default=16)
+    ap.add_argument("--kv-cache", default="model", choices=["model", "e4m3"], help="keys and values in the model's type or in e4m3")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--tp", type=int, default=1)
     ap.add_argument("--time-limit", type=float, default=3600.0)
@@ -68,13 +70,13 @@ def main(argv=None):
     # bf16 inference weights where the architecture has them: the trainer's flat buffers would not fit
     params = build_weights(cfg, dev, None, load_tensors(a.model), a.seed) if tp is None else None
     runner = ModelRunner(cfg, params=params, device=dev, num_blocks=a.blocks, block_size=a.page, seed=a.seed, tp=tp,
-                         num_slots=a.max_batch)
+                         num_slots=a.max_batch, kv_quantization=CacheQuantization.FP8 if a.kv_cache == "e4m3" else None)
     eng = ServingEngine(runner, max_batch_size=a.max_batch, prefill_chunk=a.prefill_chunk)
     # warm-up: one short request end to end
     eng.generate(list(range(1, 33)), 4)
     eng.scheduler.completed.clear()
     out = {"metric": "serving", "model": a.model, "layers": cfg.n_layer, "requests": a.requests, "rate_per_s": a.rate,
-           "page_size": a.page, "decoding": "greedy", "tp": a.tp, "tp_allreduce": (tp.transport if tp is not None else None), "prefill_chunk": a.prefill_chunk, "max_batch": a.max_batch,
+           "page_size": a.page, "kv_cache": a.kv_cache, "decoding": "greedy", "tp": a.tp, "tp_allreduce": (tp.transport if tp is not None else None), "prefill_chunk": a.prefill_chunk, "max_batch": a.max_batch,
            "data": "synthetic uniform random prompt tokens; random-init weights"}
     if a.rates:
         sweep, saturated = [], None

@@ -65,7 +65,7 @@ class GPTBody:
 
     def embed(self, sb):
         P, cfg = self.r.params, self.cfg
-        if cfg.arch == "gpt2" and not sb.spans and sb.ids.is_cuda:
+        if cfg.arch == "gpt2" and not sb.spans and not sb.moved and sb.ids.is_cuda:
             return ops.embedding_forward(sb.ids, P.w("tok_embed.embed"), P.w("pos_embed.embed"), lengths=sb.ctx)
         x = ops.embedding_forward(sb.ids, P.w("tok_embed.embed"))
         if cfg.arch == "gpt2":
@@ -76,13 +76,17 @@ class GPTBody:
         P, r, rms = self.r.params, self.r, self.rms
         H, Hk, D = r.n_head, r.n_kv_head, self.cfg.head_dim
         p = f"layers.{l}."
-        kc, vc = r.cache.k[l], r.cache.v[l]
+        kc, vc = (None, None) if r.cache.pages is not None else (r.cache.k[l], r.cache.v[l])
         qkv = self._norm_product(x, p + "ln1", P.w(p + "attn.wqkv.weight"), bias=None if rms else P.w(p + "attn.wqkv.bias"))
-        if sb.arrived is not None and paged_ops.step_supported(qkv, H, Hk, D, kc, vc, sb.bt):
+        k2, v2 = qkv[:, H * D:(H + Hk) * D], qkv[:, (H + Hk) * D:]
+        if r.cache.pages is not None:
+            if rms:
+                rope_ops.rope_(qkv, H + Hk, D, positions=sb.pos, theta=self.cfg.rope_theta)
+            a = r.store_and_attend(l, qkv[:, :H * D], k2, v2, sb, self.scale)
+        elif sb.arrived is not None and paged_ops.step_supported(qkv, H, Hk, D, kc, vc, sb.bt):
             # the kernel in front is the projection: tables, lengths and cached tokens are older
             a = paged_ops.attention_step(qkv, H, Hk, D, self.cfg.rope_theta if rms else 0.0, kc, vc, sb.bt, sb.ctx, sb.arrived, self.scale)
         else:
-            k2, v2 = qkv[:, H * D:(H + Hk) * D], qkv[:, (H + Hk) * D:]
             if rms:
                 rope_ops.rope_append_(qkv, H, Hk, D, sb.pos, self.cfg.rope_theta, kc, vc, sb.slots)
             else:

@@ -271,10 +271,12 @@ def build_state(a) -> ServerState:
     from ..core import B200Backend, CpuBackend
     if a.model:
         from .engine import ServingEngine
+        from .kv_cache import CacheQuantization
         from .model_runner import load_runner
         dtype = getattr(torch, a.dtype) if a.dtype else None
         runner = load_runner(a.model, device=a.device, dtype=dtype, num_blocks=a.blocks, block_size=a.page, weights=a.weights,
-                             seed=a.seed, num_slots=a.max_batch, **({"n_layer": a.layers} if a.layers else {}))   # weights are loaded strictly
+                             seed=a.seed, num_slots=a.max_batch, kv_quantization=CacheQuantization.FP8 if a.kv_cache == "e4m3" else None,
+                             **({"n_layer": a.layers} if a.layers else {}))                                       # weights are loaded strictly
         cfg = runner.cfg
         engine = ServingEngine(runner, max_batch_size=a.max_batch, eos_id=a.eos_id)
         engine.generate([1, 2, 3], 2)                       # warm-up: compiles nothing, but touches every kernel once
@@ -313,6 +315,8 @@ def parse_args(argv=None):
     e.add_argument("--weights", help="safetensors state dict of the model; random-init when absent")
     e.add_argument("--blocks", type=int, default=4096, help="KV-cache pages")
     e.add_argument("--page", type=int, default=16, help="tokens per KV-cache page")
+    e.add_argument("--kv-cache", default="model", choices=["model", "e4m3"], help="keys and values in the model's type, or in e4m3 (GPT-2 and "
+                   "Llama style models): half the bytes, a power of two for each page and head")
     e.add_argument("--max-batch", type=int, default=64, help="requests in one step; also the state slots of models with "
                    "recurrent layers")
     e.add_argument("--eos-id", type=int, default=None)

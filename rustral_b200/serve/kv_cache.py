@@ -14,6 +14,7 @@ import torch
 
 from .. import _native as N
 from ..core.errors import InvalidArgument
+from ..ops.paged_e4m3 import PagesE4M3, kv_evict_e4m3
 
 
 class CacheQuantization(enum.Enum):
@@ -186,11 +187,21 @@ class PagedCache:
 
     Layers with recurrent state add one tensor [num_slots, ...] per state name (`state[layer][name]`); a sequence holds the
     same slot in all of them from its first `allocate` to `free`.  A slot is not cleared when it changes hands: the layers
-    take a sequence's state as zero at position 0, whatever the slot holds."""
+    take a sequence's state as zero at position 0, whatever the slot holds.
+
+    `quantization` FP8 (not with `layers`): keys and values are e4m3 codes with a power of two for each page and head, one
+    `ops.PagesE4M3` per layer in `pages` (`k` and `v` stay None); with `attention_weights` they keep the attention weight of every
+    token, by which `evict` thins out sequences."""
 
     def __init__(self, num_blocks: int, block_size: int = 16, num_layers: int = 1, num_kv_heads: int = 1, head_dim: int = 64,
                  dtype=torch.bfloat16, device="cpu", allocate_storage: bool = True, layers: list | None = None,
-                 num_slots: int = 64):
+                 num_slots: int = 64, quantization: CacheQuantization | None = None, attention_weights: bool = False):
+        if quantization not in (None, CacheQuantization.FP8):
+            raise InvalidArgument("PagedCache: pages are kept in their dtype or, with CacheQuantization.FP8, in e4m3")
+        if layers is not None and quantization is not None:
+            raise InvalidArgument("PagedCache: layers of their own sizes are kept in their dtype")
+        if attention_weights and quantization is None:
+            raise InvalidArgument("PagedCache: attention weights are kept beside pages in e4m3")
         if layers is not None:
             num_layers = len(layers)
         self.block_size, self.num_blocks = block_size, num_blocks
@@ -199,7 +210,7 @@ class PagedCache:
         self._h = self._lib.rb_ba_create(num_blocks, block_size)
         if not self._h:
             raise InvalidArgument("PagedCache: num_blocks and block_size must be positive")
-        self.k = self.v = None
+        self.k = self.v = self.pages = None
         self.state = [{} for _ in range(num_layers)]
         recurrent = layers is not None and any(c.state for c in layers)
         self.num_slots = num_slots if recurrent else 0
@@ -216,6 +227,8 @@ class PagedCache:
             self._own = [(c.kv_of is None, c.kv_of is None and not c.joint) for c in layers]       # keys, values take room
             self.state = [{n: torch.zeros((num_slots, *shape), dtype=dt or dtype, device=device) for n, shape, dt in c.state}
                           for c in layers]
+        elif allocate_storage and quantization is not None:
+            self.pages = [PagesE4M3.zeros(num_blocks, block_size, num_kv_heads, head_dim, device, attention_weights) for _ in range(num_layers)]
         elif allocate_storage:
             shape = (num_layers, num_blocks, block_size, num_kv_heads, head_dim)
             self.k = torch.zeros(shape, dtype=dtype, device=device)
@@ -242,6 +255,37 @@ class PagedCache:
 
     def free(self, seq_id: int) -> int:
         return self._lib.rb_ba_free(self._h, seq_id)
+
+    def trim(self, seq_id: int, num_tokens: int) -> int:
+        """Gives back the blocks behind the sequence's first `num_tokens` tokens; returns their number."""
+        n = self._lib.rb_ba_trim(self._h, seq_id, num_tokens)
+        if n < 0:
+            raise InvalidArgument(f"PagedCache.trim: no sequence {seq_id}")
+        return n
+
+    def evict(self, seq_ids: list, lens: list, keep: int, recent: int = 0, keep_first: int = 0) -> list:
+        """Brings sequences of `lens` cached tokens down to `keep` (see ops.kv_evict_e4m3), every layer by its own tokens' attention weights,
+        and gives back the blocks that this empties.  Returns the new lengths; the sequences' positions do not change with them."""
+        if self.pages is None or self.pages[0].weight is None:
+            raise InvalidArgument("PagedCache.evict: these pages keep no attention weights")
+        if len(seq_ids) != len(lens) or len(set(seq_ids)) != len(seq_ids):
+            raise InvalidArgument("PagedCache.evict: a length for every sequence, and no sequence twice")
+        tables = [self.block_table(s) for s in seq_ids]
+        for s, t, n in zip(seq_ids, tables, lens):
+            if n < 0 or n > len(t) * self.block_size:
+                raise InvalidArgument(f"PagedCache.evict: sequence {s} has no blocks for {n} tokens")
+        if not seq_ids:
+            return []
+        host = torch.empty((len(seq_ids), max(len(t) for t in tables)), dtype=torch.int32)
+        self.fill_tables(seq_ids, host)
+        device = self.pages[0].k.device
+        table, length = host.to(device), torch.tensor(lens, dtype=torch.int32, device=device)
+        for pages in self.pages:
+            kv_evict_e4m3(pages, table, length, keep, recent, keep_first)
+        new = [min(n, keep) for n in lens]
+        for s, n in zip(seq_ids, new):
+            self.trim(s, n)
+        return new
 
     def block_table(self, seq_id: int) -> list:
         n = self._lib.rb_ba_table_len(self._h, seq_id)
@@ -277,6 +321,8 @@ class PagedCache:
         return self._lib.rb_ba_num_sequences(self._h)
 
     def memory_bytes(self) -> int:
+        if self.pages is not None:
+            return sum(p.memory_bytes() for p in self.pages)
         if self.k is None:
             return 0
         own = getattr(self, "_own", [(True, True)] * len(self.v))

@@ -21,12 +21,13 @@ from ..models.registry import architecture, build_weights
 from ..ops import attention as attn_ops
 from ..ops import latent as latent_ops
 from ..ops import paged as paged_ops
+from ..ops import paged_e4m3 as e4m3_ops
 from ..ops import rotary as rope_ops
 from ..ops.matmul import gemm
 from ..ops.recurrent import Segments
 from ..runtime.fused_gpt import FlatParams
 from . import decoder_body
-from .kv_cache import PagedCache
+from .kv_cache import CacheQuantization, PagedCache
 
 
 # Keys and values gathered for later portions of prompts live until their launch, which several portions share: at most this many bytes of them (or one
@@ -39,9 +40,10 @@ class StepBatch:
     `segments`: the same sequences for layers with recurrent state (None: the model has none).  `arrived`: given for a step of decoded
     sequences only whose tables and lengths were complete before it began (see ops.paged.attention_step); positions and slots (None) then
     follow from them where a layer asks.  `cached`: cache slots of all positions of the portions that do not begin at 0 (index -> int64 tensor
-    on the device), where they came with the step's other inputs."""
+    on the device), where they came with the step's other inputs.  `moved`: the decoded rows' positions are not their lengths less one."""
 
-    def __init__(self, ids, pos, slots, spans, rd, tables, bt, ctx, block_size, segments=None, arrived=None, cached=None):
+    def __init__(self, ids, pos, slots, spans, rd, tables, bt, ctx, block_size, segments=None, arrived=None, cached=None, moved=False):
+        self.moved, self._packed = moved, None
         self.ids, self._pos, self._slots, self.arrived = ids, pos, slots, arrived      # int64 device tensors, one entry per row
         self.spans = spans                                        # (first row, end row, first position) per portion
         self.rd, self.rows = rd, ids.shape[0]
@@ -96,6 +98,18 @@ class StepBatch:
             pos = torch.cat([torch.arange(kept), torch.arange(first, start + r1 - r0)])
             self._keys[key] = (torch.tensor(self.tables[i], dtype=torch.int64)[pos // bs] * bs + pos % bs).to(self.ids.device)
         return self._keys[key]
+
+    def packed(self):
+        """(block tables, lengths, first rows) of all sequences of the step, portions and decoded rows, as ops.kv_append_e4m3 takes them."""
+        if self._packed is None:
+            if not self.spans:
+                self._packed = (self.bt, self.ctx, None)
+            else:
+                bt, dev = self.row_tables()[0], self.ids.device
+                lens = torch.tensor([start + r1 - r0 for r0, r1, start in self.spans], dtype=torch.int32, device=dev)
+                starts = torch.tensor([r0 for r0, _, _ in self.spans] + list(range(self.rd, self.rows + 1)), dtype=torch.int32, device=dev)
+                self._packed = (bt.contiguous(), lens if self.ctx is None else torch.cat([lens, self.ctx]), starts)
+        return self._packed
 
     def row_tables(self):
         """(block tables int32 [sequences, width], sequence index int32 per row) over all rows of the step."""
@@ -153,10 +167,14 @@ class ModelRunner:
     ranks run the same calls in the same order and obtain bit-identical logits.
 
     `dtype` (bf16 or fp32, where the architecture runs in both) applies when `params` is not given.  `num_slots`: sequences
-    that can hold recurrent state at a time (models without such layers have no limit of that kind)."""
+    that can hold recurrent state at a time (models without such layers have no limit of that kind).
+
+    `kv_quantization` CacheQuantization.FP8 (GPT-2 and Llama style models): keys and values are cached in e4m3, half the bytes.  Whole prompts
+    attend over their keys and values as they are, later portions and decoded tokens over the cached ones.  With `kv_weights` decoding sums
+    every cached token's attention weight, and `cache.evict` may drop tokens between steps; a decoded token's position is then given to `decode`."""
 
     def __init__(self, cfg, params=None, device=None, num_blocks: int = 1024, block_size: int = 16, seed: int = 0, tp=None,
-                 dtype=None, num_slots: int = 64):
+                 dtype=None, num_slots: int = 64, kv_quantization: CacheQuantization | None = None, kv_weights: bool = False):
         if device is None:
             device = "cuda" if torch.cuda.is_available() else "cpu"
         self.cfg = cfg
@@ -179,8 +197,14 @@ class ModelRunner:
             self.n_head, self.n_kv_head = cfg.n_head // self.tp_world, cfg.n_kv_head // self.tp_world
         self.body = getattr(decoder_body, architecture(cfg.arch).body)(self)
         layers = self.body.cache_layers()
+        self.kv_weights = kv_weights
         if layers is None:
-            self.cache = PagedCache(num_blocks, block_size, cfg.n_layer, self.n_kv_head, cfg.head_dim, self.dtype, self.device)
+            if kv_quantization is not None and self.device.type == "cuda" and (block_size % 16 or cfg.head_dim not in (64, 128)):
+                raise ValueError("a cache in e4m3 has pages of a multiple of 16 tokens and heads of 64 or 128")
+            self.cache = PagedCache(num_blocks, block_size, cfg.n_layer, self.n_kv_head, cfg.head_dim, self.dtype, self.device,
+                                    quantization=kv_quantization, attention_weights=kv_weights)
+        elif kv_quantization is not None or kv_weights:
+            raise ValueError("a cache in e4m3 serves GPT-2 and Llama style models")
         else:
             self.cache = PagedCache(num_blocks, block_size, dtype=self.dtype, device=self.device, layers=layers, num_slots=num_slots)
         self.recurrent = self.cache.num_slots > 0
@@ -235,6 +259,51 @@ class ModelRunner:
             paged_ops.paged_attention_decode(q[sb.rd:], kc, vc, sb.bt, sb.ctx, scale, out=a[sb.rd:], rule=rule,
                                              gate=None if gate is None else gate[sb.rd:],
                                              head_gate=None if head_gate is None else head_gate[sb.rd:])
+        return a
+
+    def store_and_attend(self, l: int, q, k2, v2, sb: StepBatch, scale: float) -> torch.Tensor:
+        """`attend` with a cache in e4m3: stores the rows' keys and values first.  Portions that begin at 0 attend over their own rows, later ones
+        over all their positions, read back from the pages, at most MOST_GATHERED bytes of them at a time; decoded rows go through the kernel
+        that reads the codes."""
+        pages, T, rd = self.cache.pages[l], sb.rows, sb.rd
+        H, G, dk = self.n_head, self.n_kv_head, pages.k.shape[3]
+        bt, lens, starts = sb.packed()
+        e4m3_ops.kv_append_e4m3(pages, k2, v2, bt, lens, starts)
+        a = torch.empty((T, H * dk), dtype=q.dtype, device=self.device)
+        whole = [i for i, span in enumerate(sb.spans) if span[2] == 0]
+        groups, size = [[]], 0                       # later portions that are read together
+        for i, (r0, r1, start) in enumerate(sb.spans):
+            if start == 0:
+                continue
+            more = 2 * (start + r1 - r0) * G * dk * q.element_size()
+            if groups[-1] and size + more > MOST_GATHERED:
+                groups.append([])
+                size = 0
+            groups[-1].append(i)
+            size += more
+        for later in groups:
+            parts = []
+            for i in whole:
+                r0, r1, _ = sb.spans[i]
+                parts.append((q[r0:r1].view(1, r1 - r0, H, dk), k2[r0:r1].view(1, r1 - r0, G, dk), v2[r0:r1].view(1, r1 - r0, G, dk),
+                              a[r0:r1].view(1, r1 - r0, H, dk)))
+            whole = []
+            if later:
+                ends = [0]
+                for i in later:
+                    r0, r1, start = sb.spans[i]
+                    ends.append(ends[-1] + start + r1 - r0)
+                which = torch.tensor(later, device=self.device)
+                kk, vv = e4m3_ops.kv_read_e4m3(pages, bt.index_select(0, which), lens.index_select(0, which),
+                                               torch.tensor(ends, dtype=torch.int32, device=self.device), ends[-1], dtype=q.dtype)
+                for i, lo, hi in zip(later, ends, ends[1:]):
+                    r0, r1, _ = sb.spans[i]
+                    parts.append((q[r0:r1].view(1, r1 - r0, H, dk), kk[lo:hi].view(1, hi - lo, G, dk), vv[lo:hi].view(1, hi - lo, G, dk),
+                                  a[r0:r1].view(1, r1 - r0, H, dk)))
+            if parts:
+                attn_ops.prompt_attention_many(parts, scale)
+        if rd < T:
+            e4m3_ops.paged_attention_decode_e4m3(q[rd:], pages, sb.bt, sb.ctx, scale, out=a[rd:], accumulate=self.kv_weights)
         return a
 
     def attend_latent(self, l: int, q, kv, sb: StepBatch, m, w_ukv, table, gate=None) -> torch.Tensor:
@@ -377,7 +446,7 @@ class ModelRunner:
 
     def _attends_in_one_launch(self, context_lens, width: int) -> bool:
         """Whether a decoding step's layers attend in one launch: by the slices that its lengths have."""
-        if self.device.type != "cuda" or not isinstance(self.body, decoder_body.GPTBody):
+        if self.device.type != "cuda" or not isinstance(self.body, decoder_body.GPTBody) or self.cache.pages is not None:
             return False
         key = (len(context_lens), width)
         most = self._most_slices.get(key)
@@ -391,17 +460,20 @@ class ModelRunner:
         """Zeros that the steps of one stream share (see ops.paged.attention_step)."""
         return torch.zeros(batch * self.n_kv_head, dtype=torch.int32, device=self.device)
 
-    def _decode_body(self, ids, ctx, bt, segments=None, arrived=None):
+    def _decode_body(self, ids, ctx, bt, segments=None, arrived=None, pos=None):
         """The device-side part of a decode step on static tensors (captured into a CUDA graph per batch size)."""
-        return self._run(StepBatch(ids, None, None, [], 0, [], bt, ctx, self.block_size, segments, arrived), None)
+        return self._run(StepBatch(ids, pos, None, [], 0, [], bt, ctx, self.block_size, segments, arrived, moved=pos is not None), None)
 
     @torch.no_grad()
-    def decode(self, seq_ids: list, last_tokens: list, context_lens: list) -> torch.Tensor:
-        """One new token per sequence.  context_lens[i] counts the tokens in the cache AFTER this token is appended.
+    def decode(self, seq_ids: list, last_tokens: list, context_lens: list, positions: list | None = None) -> torch.Tensor:
+        """One new token per sequence.  context_lens[i] counts the tokens in the cache AFTER this token is appended.  `positions`: the tokens'
+        positions, where tokens have left the cache (a cache in e4m3; otherwise they are the lengths less one).
         Returns logits [batch, vocab_padded] (with CUDA graphs: valid until the next decode call)."""
         dev = self.device
+        if positions is not None and self.cache.pages is None:
+            raise ValueError("positions apart from the lengths need a cache in e4m3")
         if self.use_graphs and dev.type == "cuda":
-            return self._decode_graphed(seq_ids, last_tokens, context_lens)
+            return self._decode_graphed(seq_ids, last_tokens, context_lens, positions)
         ids = torch.tensor(last_tokens, dtype=torch.int64, device=dev)
         ctx = torch.tensor(context_lens, dtype=torch.int32, device=dev)
         max_blocks = max(len(self.cache.block_table(s)) for s in seq_ids)
@@ -410,7 +482,8 @@ class ModelRunner:
         bt = bt.to(dev)
         seg = Segments.of(self._decode_segments(seq_ids, context_lens), dev) if self.recurrent else None
         one = self._attends_in_one_launch(context_lens, max_blocks)
-        return self._decode_body(ids, ctx, bt, seg, self._step_counters(len(seq_ids)) if one else None)
+        pos = None if positions is None else torch.tensor(positions, dtype=torch.int64, device=dev)
+        return self._decode_body(ids, ctx, bt, seg, self._step_counters(len(seq_ids)) if one else None, pos)
 
     def _table_width(self, context_lens) -> int:
         """Block-table columns of a graphed decode step: the model's whole context when that is at most 1024 blocks, else
@@ -422,31 +495,34 @@ class ModelRunner:
         return min(full, max(64, 1 << (need - 1).bit_length()))
 
     @staticmethod
-    def _step_views(buf: torch.Tensor, B: int, width: int) -> dict:
-        return {"ids": buf[:8 * B].view(torch.int64), "ctx": buf[8 * B:12 * B].view(torch.int32),
-                "bt": buf[12 * B:].view(torch.int32).view(B, width)}
+    def _step_views(buf: torch.Tensor, B: int, width: int, moved: bool = False) -> dict:
+        at = 16 * B if moved else 8 * B
+        return {"ids": buf[:8 * B].view(torch.int64), "pos": buf[8 * B:16 * B].view(torch.int64) if moved else None,
+                "ctx": buf[at:at + 4 * B].view(torch.int32), "bt": buf[at + 4 * B:].view(torch.int32).view(B, width)}
 
-    def _decode_graphed(self, seq_ids, last_tokens, context_lens) -> torch.Tensor:
+    def _decode_graphed(self, seq_ids, last_tokens, context_lens, positions=None) -> torch.Tensor:
         """Replays one captured CUDA graph per batch size, table width and form of the attention: the 10 to 20 launches per layer of a decode step are
         launch-bound from Python, the graph submits them in one call.  Inputs live in a static device buffer that
         one copy refreshes before each replay."""
         B = len(seq_ids)
         dev = self.device
         width = self._table_width(context_lens)
-        one = self._attends_in_one_launch(context_lens, width)
-        g = self._graphs.get((B, width, one))
+        one, moved = self._attends_in_one_launch(context_lens, width), positions is not None
+        g = self._graphs.get((B, width, one, moved))
         if g is None:
-            # ids (int64), context lengths and block tables (int32) behind one another: one copy refreshes all three
-            buf = torch.zeros(12 * B + 4 * B * width, dtype=torch.uint8, device=dev)
+            # ids and, where they are given, positions (int64), context lengths and block tables (int32) behind one another: one copy refreshes all
+            buf = torch.zeros((20 if moved else 12) * B + 4 * B * width, dtype=torch.uint8, device=dev)
             g = {"buf": buf, "seg": None, "graph": None, "out": None, "arrived": self._step_counters(B) if one else None,
-                 **self._step_views(buf, B, width)}
+                 **self._step_views(buf, B, width, moved)}
             if self.recurrent:
                 g["seg"] = Segments(torch.zeros((B, 4), dtype=torch.int32, device=dev), None)
-            self._graphs[(B, width, one)] = g
+            self._graphs[(B, width, one, moved)] = g
         memory, copied = self._memory.take(g["buf"].numel())
         host = memory[:g["buf"].numel()]
-        view = self._step_views(host, B, width)
+        view = self._step_views(host, B, width, moved)
         view["ids"].numpy()[:] = last_tokens
+        if moved:
+            view["pos"].numpy()[:] = positions
         view["ctx"].numpy()[:] = context_lens
         self.cache.fill_tables(seq_ids, view["bt"])
         g["buf"].copy_(host, non_blocking=True)
@@ -455,7 +531,7 @@ class ModelRunner:
             g["seg"].table.copy_(torch.tensor(self._decode_segments(seq_ids, context_lens), dtype=torch.int32), non_blocking=True)
         if g["graph"] is None:
             # first use of this batch size: one eager run (lazy kernel configuration, tensor-map cache), then capture
-            out = self._decode_body(g["ids"], g["ctx"], g["bt"], g["seg"], g["arrived"])
+            out = self._decode_body(g["ids"], g["ctx"], g["bt"], g["seg"], g["arrived"], g["pos"])
             torch.cuda.current_stream().synchronize()
             graph = torch.cuda.CUDAGraph()
             # A collection in the middle of a capture could destroy an earlier runner's graphs, which ends the capture with an error
@@ -463,7 +539,7 @@ class ModelRunner:
             gc.disable()
             try:
                 with torch.cuda.graph(graph):
-                    g["out"] = self._decode_body(g["ids"], g["ctx"], g["bt"], g["seg"], g["arrived"])
+                    g["out"] = self._decode_body(g["ids"], g["ctx"], g["bt"], g["seg"], g["arrived"], g["pos"])
             finally:
                 if collecting:
                     gc.enable()
@@ -474,7 +550,7 @@ class ModelRunner:
 
 
 def load_runner(model: str, device=None, dtype=None, num_blocks: int = 1024, block_size: int = 16, weights: str | None = None,
-                seed: int = 0, num_slots: int = 64, **overrides) -> ModelRunner:
+                seed: int = 0, num_slots: int = 64, kv_quantization: CacheQuantization | None = None, **overrides) -> ModelRunner:
     """Runner of a preset name or of a model folder (config.json + model.safetensors, the model class chosen by the
     configuration); `weights` names another safetensors file.  Without weights: random initialisation."""
     from ..models.registry import load_tensors, resolve_config
@@ -483,4 +559,4 @@ def load_runner(model: str, device=None, dtype=None, num_blocks: int = 1024, blo
         device = "cuda" if torch.cuda.is_available() else "cpu"
     params = build_weights(cfg, device, dtype, load_tensors(model, weights), seed)
     return ModelRunner(cfg, params=params, device=device, num_blocks=num_blocks, block_size=block_size, seed=seed,
-                       num_slots=num_slots)
+                       num_slots=num_slots, kv_quantization=kv_quantization)

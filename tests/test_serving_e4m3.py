@@ -1,0 +1,222 @@
+"""Serving over a cache in e4m3: what the runner stores, reads and attends over, against the oracle of the pages; graphs, the engine, eviction."""
+import pytest
+import torch
+
+from paged_e4m3_oracle import Cache
+from rustral_b200 import ops
+from rustral_b200.core.errors import InvalidArgument
+from rustral_b200.models.config import preset
+from rustral_b200.ops import paged_e4m3 as e4m3_ops
+from rustral_b200.serve import CacheQuantization, ModelRunner, PagedCache, ServingEngine
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+FP8 = CacheQuantization.FP8
+
+
+def runner_of(name, device, **kw):
+    # heads of 64, as the kernels have them
+    cfg = preset(name, seq_len=512, n_layer=2, d_model=256, n_head=4, ffn_dim=256, **({"n_kv_head": 2} if name == "llama-test" else {}))
+    return ModelRunner(cfg, device=device, num_blocks=64, seed=3, kv_quantization=FP8, **kw)
+
+
+def tokens(cfg, n, seed):
+    return torch.randint(0, cfg.vocab_size, (n,), generator=torch.Generator().manual_seed(seed)).tolist()
+
+
+class Watch:
+    """Follows every call of the cache's operators with an oracle of each layer's pages."""
+
+    def __init__(self, monkeypatch, runner):
+        self.oracles = {id(p): Cache(p) for p in runner.cache.pages}
+        self.calls = {"append": 0, "read": 0, "attend": 0}
+        append, read, attend = e4m3_ops.kv_append_e4m3, e4m3_ops.kv_read_e4m3, e4m3_ops.paged_attention_decode_e4m3
+
+        def watched_append(pages, k, v, tables, lens, starts=None):
+            append(pages, k, v, tables, lens, starts)
+            o = self.oracles[id(pages)]
+            o.append(k.cpu(), v.cpu(), tables.cpu(), lens.tolist(), list(range(k.shape[0] + 1)) if starts is None else starts.tolist())
+            o.same(pages)
+            self.calls["append"] += 1
+
+        def watched_read(pages, tables, lens, starts, rows, dtype=torch.bfloat16, out=None):
+            got = read(pages, tables, lens, starts, rows, dtype, out)
+            o, n = self.oracles[id(pages)], lens.tolist()
+            assert starts.tolist() == [sum(n[:i]) for i in range(len(n) + 1)] and rows == sum(n)
+            for x, name in zip(got, "kv"):
+                ref = torch.cat([o.tokens(name, tables.cpu(), b, m).reshape(m, -1) for b, m in enumerate(n)])
+                assert torch.equal(x.cpu().double(), ref)
+            self.calls["read"] += 1
+            return got
+
+        def watched_attend(q, pages, tables, lens, scale=None, out=None, accumulate=False):
+            o = self.oracles[id(pages)]
+            got = attend(q, pages, tables, lens, scale, out, accumulate)
+            ref, err, _, _ = o.attend(q.cpu(), tables.cpu(), lens.tolist(), scale)
+            assert bool(((got.cpu().double() - ref).abs() <= err + ref.abs() * torch.finfo(q.dtype).eps / 2 + 1e-30).all())
+            if accumulate:
+                o.w = pages.weight.cpu().double()
+            self.calls["attend"] += 1
+            return got
+
+        for name, f in (("kv_append_e4m3", watched_append), ("kv_read_e4m3", watched_read), ("paged_attention_decode_e4m3", watched_attend)):
+            monkeypatch.setattr(e4m3_ops, name, f)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("name", ["gpt2-test", "llama-test"])
+def test_steps_follow_the_pages(device, name, monkeypatch):
+    r = runner_of(name, device)
+    r.use_graphs = False
+    watch, cfg = Watch(monkeypatch, r), r.cfg
+    a, b, c = tokens(cfg, 60, 1), tokens(cfg, 21, 2), tokens(cfg, 37, 3)
+    for s, n in ((1, 70), (2, 30), (3, 40)):
+        assert r.cache.allocate(s, n)
+    r.step_mixed([(1, a[:25], 0, False), (2, b, 0, True)], [], [], [])
+    assert watch.calls == {"append": 2, "read": 0, "attend": 0}
+    # a later portion beside a whole prompt and a decoded sequence
+    out, dec = r.step_mixed([(1, a[25:], 25, True), (3, c[:30], 0, False)], [2], [5], [22])
+    assert watch.calls == {"append": 4, "read": 2, "attend": 2} and out[0].shape == dec[0].shape
+    r.step_mixed([(3, c[30:], 30, True)], [1, 2], [7, 8], [61, 23])
+    r.decode([1, 2, 3], [1, 2, 3], [62, 24, 38])
+    assert watch.calls == {"append": 8, "read": 4, "attend": 6}
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_portions_read_in_groups(device, monkeypatch):
+    """More gathered keys than the limit: the same logits from several reads."""
+    from rustral_b200.serve import model_runner
+    logits = []
+    for most in (model_runner.MOST_GATHERED, 1):
+        monkeypatch.setattr(model_runner, "MOST_GATHERED", most)
+        r = runner_of("llama-test", device)
+        parts = []
+        for s, n in ((1, 40), (2, 33), (3, 17)):
+            assert r.cache.allocate(s, 60)
+            r.step_mixed([(s, tokens(r.cfg, n, s), 0, False)], [], [], [])
+            parts.append((s, tokens(r.cfg, 11, s + 9), n, True))
+        assert r.cache.allocate(4, 20)
+        out, _ = r.step_mixed(parts + [(4, tokens(r.cfg, 9, 8), 0, True)], [], [], [])
+        logits.append(torch.stack(out))
+    assert torch.equal(*logits)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["gpt2-test", "llama-test"])
+def test_graphs_give_what_eager_steps_give(name, cuda_status):
+    got = []
+    for graphs in (True, False):
+        r = runner_of(name, "cuda", kv_weights=True)
+        r.use_graphs = graphs
+        for s in (1, 2):
+            assert r.cache.allocate(s, 100)
+            r.prefill(s, tokens(r.cfg, 20 + s, s))
+        lens, logits = [21, 22], []
+        for step in range(4):
+            lens = [n + 1 for n in lens]
+            logits.append(r.decode([1, 2], [step, step + 1], lens).clone())
+        lens = r.cache.evict([1, 2], lens, 16, 4, 1)
+        assert lens == [16, 16] and r.cache.allocate(1, 20) and r.cache.allocate(2, 20)
+        for step in range(4):
+            lens = [n + 1 for n in lens]
+            logits.append(r.decode([1, 2], [step, step + 1], lens, [25 + step, 26 + step]).clone())
+        got.append((torch.stack(logits), torch.stack([p.weight for p in r.cache.pages])))
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["gpt2-test", "llama-test"])
+def test_gpu_logits_match_cpu(name, cuda_status):
+    """As the runner with a bf16 cache is held to the CPU's (tests/test_gpu_serving.py), with the same cache of codes on either side: its keys differ by the
+    bf16 rounding of the projections, which moves a number by a step of its code, 2^-3 of it, where it lies beside a border."""
+    gpu, cpu = runner_of(name, "cuda"), runner_of(name, "cpu")
+    cpu.params.master.copy_(gpu.params.lowp.float().cpu())
+    cpu.params.sync_lowp()
+    prompt = tokens(gpu.cfg, 37, 0)
+    for r in (gpu, cpu):
+        assert r.cache.allocate(1, 50)
+    lg, lc = gpu.prefill(1, prompt), cpu.prefill(1, prompt)
+    assert (lg.float().cpu() - lc).abs().max() < 0.05 * lc.abs().max() + 0.02
+    tok = int(lc[:gpu.cfg.vocab_size].argmax())
+    for step in range(3):
+        dg, dc = gpu.decode([1], [tok], [38 + step]), cpu.decode([1], [tok], [38 + step])
+        assert (dg.float().cpu() - dc).abs().max() < 0.05 * dc.abs().max() + 0.02
+        tok = int(dc[0, :gpu.cfg.vocab_size].argmax())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_engine_completes_and_frees(device):
+    r = runner_of("llama-test", device, kv_weights=True)
+    eng = ServingEngine(r, max_batch_size=4, prefill_chunk=16)
+    ids = [eng.submit(tokens(r.cfg, n, n), 6) for n in (3, 30, 64, 17, 5)]
+    done = eng.run_to_completion()
+    assert sorted(x.id for x in done) == ids and all(len(x.generated) == 6 for x in done)
+    assert r.cache.free_blocks == 64
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_eviction_in_a_runner(device):
+    r = runner_of("llama-test", device, kv_weights=True)
+    r.use_graphs = False
+    assert r.cache.allocate(1, 120) and r.cache.allocate(2, 40)
+    r.prefill(1, tokens(r.cfg, 100, 1))
+    r.prefill(2, tokens(r.cfg, 20, 2))
+    lens = [100, 20]
+    for step in range(3):
+        lens = [n + 1 for n in lens]
+        logits = r.decode([1, 2], [3, 4], lens)
+    grown = torch.stack([p.weight.sum() for p in r.cache.pages]).cpu()
+    # every step adds one for each of two sequences and four heads
+    torch.testing.assert_close(grown, torch.full((2,), 3.0 * 2 * 4), rtol=1e-5, atol=0)
+    # a budget that all sequences keep changes nothing but the blocks behind their tokens
+    assert r.cache.evict([1, 2], lens, 200) == lens and len(r.cache.block_table(1)) == 7 and len(r.cache.block_table(2)) == 2
+    before = r.cache.free_blocks
+    assert r.cache.evict([1, 2], lens, 32, 8, 2) == [32, 23]
+    assert r.cache.free_blocks == before + 5 and len(r.cache.block_table(1)) == 2
+    assert r.cache.allocate(1, 33)
+    logits = r.decode([1, 2], [5, 6], [33, 24], [103, 23])
+    assert bool(torch.isfinite(logits).all())
+
+
+def test_positions_apart_from_lengths_are_those_without():
+    """Positions that are the lengths less one: the same logits as without them, from a cache in e4m3 (both architectures)."""
+    for name in ("gpt2-test", "llama-test"):
+        out = []
+        for given in (False, True):
+            r = runner_of(name, "cpu")
+            assert r.cache.allocate(1, 40)
+            r.prefill(1, tokens(r.cfg, 20, 1))
+            out.append(r.decode([1], [4], [21], [20] if given else None))
+        assert torch.equal(*out)
+
+
+def test_trim():
+    c = PagedCache(8, 16, allocate_storage=False)
+    assert c.allocate(1, 70) and c.block_table(1) == [0, 1, 2, 3, 4] and c.free_blocks == 3
+    assert c.trim(1, 33) == 2 and c.block_table(1) == [0, 1, 2] and c.free_blocks == 5
+    assert c.trim(1, 100) == 0 and c.trim(1, 0) == 3 and c.free_blocks == 8
+    assert c.allocate(1, 17) and len(c.block_table(1)) == 2
+    with pytest.raises(InvalidArgument):
+        c.trim(9, 1)
+
+
+def test_refusals():
+    with pytest.raises(InvalidArgument):
+        PagedCache(4, 16, quantization=CacheQuantization.INT8)
+    with pytest.raises(InvalidArgument):
+        PagedCache(4, 16, attention_weights=True)
+    with pytest.raises(ValueError):
+        ModelRunner(preset("dolurax-test"), device="cpu", kv_quantization=FP8)
+    c = PagedCache(4, 16, head_dim=64, quantization=FP8)
+    with pytest.raises(InvalidArgument):
+        c.evict([1], [1], 1)                                          # no weights
+    c = PagedCache(4, 16, head_dim=64, quantization=FP8, attention_weights=True)
+    assert c.allocate(1, 20) and c.evict([], [], 4) == []
+    for ids, lens in (([1], [33]), ([1], [-1]), ([1, 1], [4, 4]), ([1], []), ([2], [4])):
+        with pytest.raises(InvalidArgument):
+            c.evict(ids, lens, 4)
+    assert c.memory_bytes() == 4 * (2 * 16 * 64 + 2 + 16 * 4)
+    assert ops.PagesE4M3.zeros(4, 16, 1, 64).memory_bytes() == 4 * (2 * 16 * 64 + 2)
+    r = ModelRunner(preset("llama-test"), device="cpu", num_blocks=8)
+    with pytest.raises(ValueError):
+        r.decode([1], [1], [1], [0])                                  # positions without a cache in e4m3
