@@ -164,6 +164,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
       }
       skip -= __shfl_sync(0xffffffffu, upto, 31);
       b0 += 32;
+      if (b0 >= a.batch) return;                     // lengths that changed meanwhile
       n = b0 + lane < a.batch ? (e4_len(a, b0 + lane) + kE4Slice - 1) / kE4Slice : 0;
     }
   }
@@ -208,8 +209,9 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
     p.s = 0;
     if (++p.hk < G) return;
     p.hk = 0;
-    do n = e4_len(a, ++p.b);
-    while (n == 0);
+    do n = ++p.b < a.batch ? e4_len(a, p.b) : 0;
+    while (n == 0 && p.b < a.batch);
+    if (n == 0) p.left = 0;                          // lengths that changed meanwhile
   };
   // lanes 0 .. 3: exponents of the four tiles' keys, 4 .. 7 of their values
   auto exps_of = [&](int tile, int w) { return tile < 0 || lane >= 8 ? 0 : static_cast<int>((lane < 4 ? a.pages.k_exp : a.pages.v_exp)[w]); };

@@ -104,9 +104,6 @@ def _scratch_floats(*sizes) -> int:
     return N.kernels().rb_e4m3_decode_scratch_floats(*sizes)
 
 
-_scratch: dict = {}
-
-
 def _aligned(t: torch.Tensor) -> bool:
     """Whether the kernels can read or write the rows of `t` 16 bytes at a time."""
     pitch, step = t.stride()
@@ -184,7 +181,7 @@ def kv_append_e4m3(pages: PagesE4M3, k_new, v_new, block_tables, context_lens, r
 
     A page whose first slot gets a token forgets what it held and takes its exponents from this call; in any other page an exponent grows if a
     new token asks for it, and the codes in front are rounded to it (exactly, but for those that become subnormal).  Rows whose position has no
-    page are not stored.  The new tokens' weights become 0."""
+    page are not stored.  The new tokens' weights become 0.  No two sequences of a call store into the same page."""
     shape = _check("kv_append_e4m3", pages, block_tables, context_lens, k_new, v_new, row_starts)
     rows, batch, row = k_new.shape[0], context_lens.shape[0], (k_new.shape[0], shape[1] * shape[3])
     if k_new.dtype not in _TYPES or v_new.dtype is not k_new.dtype or k_new.shape != row or v_new.shape != row:
@@ -282,9 +279,7 @@ def paged_attention_decode_e4m3(q, pages: PagesE4M3, block_tables, context_lens,
     if width == 0:
         return out.zero_()
     floats = _scratch_floats(B, heads, G, D, width, bs, accumulate)
-    # small scratch is kept for the stream's next call, large scratch (many or long sequences) is not
-    scratch = None if floats == 0 else N.scratch(_scratch, q.device, floats, torch.float32) if floats <= 1 << 24 else \
-        torch.empty(floats, dtype=torch.float32, device=q.device)
+    scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     a = _DECODE.pack(*_native(pages, shape), q.data_ptr(), out.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), _ptr(scratch),
                      q.stride(0), out.stride(0), B, width, heads, _TYPES[q.dtype], accumulate, scale)
     N.check(N.kernels().rb_e4m3_decode(a, N.stream_ptr()), "rb_e4m3_decode")
@@ -295,7 +290,8 @@ def kv_evict_e4m3(pages: PagesE4M3, block_tables, context_lens, keep: int, recen
     """Brings every sequence down to `keep` tokens.  A longer one keeps, for each KV head, its first `keep_first` tokens, its last `recent` and,
     of the others, those with the largest weights (`pages.weight`; of equal ones the earlier, NaN counts as largest).  They move, in their order and
     with their weights, to the front of the sequence's pages; what lies behind is free.  With `out_tables` (int32 [batch, width], pages that no
-    sequence of `block_tables` has) every sequence moves there instead, also one that is short enough, and the old pages stay as they are.
+    sequence of `block_tables` has) every sequence moves there instead, also one that is short enough, and the old pages stay as they are; only
+    then may sequences share pages.
 
     Returns (lengths int32 [batch], kept int32 [batch, kv_heads, keep]): the place that each token came from, -1 behind the last.
 
@@ -309,6 +305,8 @@ def kv_evict_e4m3(pages: PagesE4M3, block_tables, context_lens, keep: int, recen
         raise ValueError("kv_evict_e4m3: keep must be at least 1 and at least recent + keep_first")
     if out_tables is not None and not (out_tables.dtype is torch.int32 and out_tables.dim() == 2 and out_tables.shape[0] == B and out_tables.is_contiguous()):
         raise TypeError("kv_evict_e4m3: out_tables is a contiguous int32 table row per sequence")
+    if out_tables is not None and out_tables.shape[1] * shape[2] < min(keep, block_tables.shape[1] * shape[2]):
+        raise ValueError("kv_evict_e4m3: out_tables has no room for the tokens that may be kept")
     lens = torch.empty_like(context_lens)
     kept = torch.empty((B, G, keep), dtype=torch.int32, device=pages.k.device)
     if not pages.k.is_cuda:

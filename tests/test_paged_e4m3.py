@@ -26,7 +26,7 @@ def tables_of(lens, bs, blocks, seed, width=0):
 
 
 def filled(blocks, bs, G, D, seed, weights=False, spread=3):
-    """Pages of random codes, infinities' and NaN's codes among the first page's: what earlier owners left."""
+    """Pages of random codes: what earlier owners left."""
     g = torch.Generator().manual_seed(seed)
     p = ops.PagesE4M3.zeros(blocks, bs, G, D, weights=weights)
     for codes, exps in ((p.k, p.k_exp), (p.v, p.v_exp)):
@@ -60,6 +60,7 @@ APPENDS = [
     ([(0, 0), (0, 129), (0, 0), (7, 1), (0, 0)], 32, 2, 64, torch.float16),
     ([(63, 65), (64, 64), (1, 200)], 64, 1, 128, torch.float32),
     ([(9, 300)], 48, 5, 64, torch.bfloat16),
+    ([(100, 300), (0, 128)], 128, 2, 64, torch.float32),
 ]
 
 
@@ -275,6 +276,15 @@ def test_attention_has_the_same_bits_alone_and_beside_others():
     assert torch.equal(p.weight, p2.weight)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,D,dtype", [(4, 128, torch.bfloat16), (1, 64, torch.float16), (12, 64, torch.bfloat16)])
+def test_attention_over_many_slices(group, D, dtype):
+    """Tables with room for more than 64 slices: long sequences, and short ones in such tables."""
+    check_attention("cuda", [17000, 40, 0, 16641], 1, group, D, 16, dtype, True, seed=5)
+    check_attention("cuda", [300, 1, 2049], 2, group, D, 16, dtype, True, seed=6, width=1200)
+    check_attention("cuda", [511] * 40 + [0, 7], 2, group, D, 64, dtype, False, seed=7, width=80)
+
+
 EVICTS = [
     # lengths, keep, recent, first, block size, KV heads, head size
     ([40], 20, 4, 2, 16, 1, 64),
@@ -284,6 +294,8 @@ EVICTS = [
     ([50, 31, 200], 32, 0, 32, 16, 2, 64),
     ([130, 129, 128, 127], 1, 0, 0, 64, 2, 128),
     ([700, 90], 600, 100, 8, 48, 2, 64),
+    ([300, 50, 200, 129], 150, 20, 3, 128, 2, 64),
+    ([300, 81, 500], 170, 0, 0, 80, 1, 128),
 ]
 
 
@@ -542,6 +554,8 @@ def test_refuses_operands(device):
         ops.kv_evict_e4m3(p, t, n, 1, out_tables=t.long())
     with pytest.raises(TypeError):
         ops.kv_evict_e4m3(p, t, n, 1, out_tables=t[:1])
+    with pytest.raises(ValueError):
+        ops.kv_evict_e4m3(p, t, n, 20, out_tables=t[:, :1].contiguous())
     q, t2, n2 = small(device, weights=False)
     with pytest.raises(ValueError):
         ops.kv_evict_e4m3(q, t, n, 1)
