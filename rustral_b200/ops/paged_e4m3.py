@@ -65,22 +65,24 @@ class PagesE4M3:
 
 
 def _check(what: str, pages: PagesE4M3, block_tables, context_lens, *others) -> tuple:
-    """(blocks, KV heads, block size, head size) of pages that a kernel can take with these tables; `others`: further tensors of the call."""
+    """(blocks, KV heads, block size, head size, sequences, table width) of pages and tables that a kernel can take; `others`: further tensors of the
+    call.  (Every look at a tensor counts here: the attributes are read once, and shapes before anything else.)"""
     k, v, ke, ve, w = pages.k, pages.v, pages.k_exp, pages.v_exp, pages.weight
-    shape = k.shape
+    shape, dev = k.shape, k.get_device()
     nb, G, bs, D = shape
     if not (k.dtype is v.dtype is torch.float8_e4m3fn and ke.dtype is ve.dtype is torch.int8 and v.shape == shape and ke.shape == ve.shape == (nb, G) and
             k.is_contiguous() and v.is_contiguous() and ke.is_contiguous() and ve.is_contiguous()):
         raise TypeError(f"{what}: pages are contiguous e4m3 codes [blocks, kv_heads, block_size, head_dim] with int8 exponents [blocks, kv_heads]")
-    dev = k.get_device()
-    if w is not None:
-        if not (w.dtype is torch.float32 and w.shape == (nb, G, bs) and w.is_contiguous()):
-            raise TypeError(f"{what}: weights are contiguous fp32 [blocks, kv_heads, block_size]")
-        others += (w,)
-    if not (block_tables.dtype is context_lens.dtype is torch.int32 and block_tables.dim() == 2 and block_tables.is_contiguous() and
-            context_lens.is_contiguous() and context_lens.shape == block_tables.shape[:1]):
+    if w is not None and not (w.dtype is torch.float32 and w.shape == (nb, G, bs) and w.is_contiguous()):
+        raise TypeError(f"{what}: weights are contiguous fp32 [blocks, kv_heads, block_size]")
+    table, batch = block_tables.shape, context_lens.shape
+    if not (block_tables.dtype is context_lens.dtype is torch.int32 and len(table) == 2 and len(batch) == 1 and table[0] == batch[0] and
+            block_tables.is_contiguous() and context_lens.is_contiguous()):
         raise TypeError(f"{what}: a contiguous int32 table row and an int32 length per sequence are required")
-    for t in (v, ke, ve, block_tables, context_lens, *others):
+    if not (v.get_device() == ke.get_device() == ve.get_device() == block_tables.get_device() == context_lens.get_device() == dev and
+            (w is None or w.get_device() == dev)):
+        raise ValueError(f"{what}: pages, tables and lengths are on one device")
+    for t in others:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"{what}: tensors on {k.device} and {t.device}")
     if dev >= 0:
@@ -88,11 +90,12 @@ def _check(what: str, pages: PagesE4M3, block_tables, context_lens, *others) -> 
             raise ValueError(f"{what}: pages of a multiple of 16 tokens and heads of 64 or 128 are required, not {bs} and {D}")
         if dev != torch._C._cuda_getDevice():
             raise ValueError(f"{what}: the pages are on {k.device}, which is not the current device")
-    return shape
+    return nb, G, bs, D, table[0], table[1]
 
 
 def _native(p: PagesE4M3, shape) -> tuple:
-    return (p.k.data_ptr(), p.v.data_ptr(), p.k_exp.data_ptr(), p.v_exp.data_ptr(), _ptr(p.weight), shape[0], shape[2], shape[1], shape[3])
+    w = p.weight
+    return (p.k.data_ptr(), p.v.data_ptr(), p.k_exp.data_ptr(), p.v_exp.data_ptr(), 0 if w is None else w.data_ptr(), shape[0], shape[2], shape[1], shape[3])
 
 
 def _ptr(t) -> int:
@@ -104,10 +107,10 @@ def _scratch_floats(*sizes) -> int:
     return N.kernels().rb_e4m3_decode_scratch_floats(*sizes)
 
 
-def _aligned(t: torch.Tensor) -> bool:
-    """Whether the kernels can read or write the rows of `t` 16 bytes at a time."""
+def _pitch(t: torch.Tensor) -> int:
+    """The pitch of the rows of `t`, 0 where the kernels cannot read or write them 16 bytes at a time."""
     pitch, step = t.stride()
-    return step == 1 and not (t.data_ptr() | pitch * t.element_size()) & 15
+    return 0 if step != 1 or (t.data_ptr() | pitch * t.element_size()) & 15 else pitch
 
 
 def _starts(what: str, row_starts, batch: int):
@@ -183,8 +186,10 @@ def kv_append_e4m3(pages: PagesE4M3, k_new, v_new, block_tables, context_lens, r
     new token asks for it, and the codes in front are rounded to it (exactly, but for those that become subnormal).  Rows whose position has no
     page are not stored.  The new tokens' weights become 0.  No two sequences of a call store into the same page."""
     shape = _check("kv_append_e4m3", pages, block_tables, context_lens, k_new, v_new, row_starts)
-    rows, batch, row = k_new.shape[0], context_lens.shape[0], (k_new.shape[0], shape[1] * shape[3])
-    if k_new.dtype not in _TYPES or v_new.dtype is not k_new.dtype or k_new.shape != row or v_new.shape != row:
+    batch, width = shape[4:]
+    given, kind = k_new.shape, k_new.dtype
+    rows = given[0]
+    if kind not in _TYPES or v_new.dtype is not kind or given != (rows, shape[1] * shape[3]) or v_new.shape != given:
         raise TypeError("kv_append_e4m3: keys and values are [rows, kv_heads * head_dim] in bf16, fp16 or fp32")
     if row_starts is not None:
         _starts("kv_append_e4m3", row_starts, batch)
@@ -194,12 +199,13 @@ def kv_append_e4m3(pages: PagesE4M3, k_new, v_new, block_tables, context_lens, r
         return _append_cpu(pages, k_new, v_new, block_tables, context_lens, row_starts)
     if rows == 0 or batch == 0:
         return
-    if not _aligned(k_new):
-        k_new = k_new.clone(memory_format=torch.contiguous_format)
-    if not _aligned(v_new):
-        v_new = v_new.clone(memory_format=torch.contiguous_format)
+    ld_k, ld_v = _pitch(k_new), _pitch(v_new)
+    if not ld_k:
+        k_new, ld_k = k_new.clone(memory_format=torch.contiguous_format), given[1]
+    if not ld_v:
+        v_new, ld_v = v_new.clone(memory_format=torch.contiguous_format), given[1]
     a = _APPEND.pack(*_native(pages, shape), k_new.data_ptr(), v_new.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), _ptr(row_starts),
-                     k_new.stride(0), v_new.stride(0), rows, batch, block_tables.shape[1], _TYPES[k_new.dtype])
+                     ld_k, ld_v, rows, batch, width, _TYPES[kind])
     N.check(N.kernels().rb_e4m3_append(a, N.stream_ptr()), "rb_e4m3_append")
 
 
@@ -208,18 +214,21 @@ def kv_read_e4m3(pages: PagesE4M3, block_tables, context_lens, row_starts, rows:
     bf16 and fp32 hold every number of a page exactly (fp16: those in its range).  `out`: a pair that receives them; rows that no position has
     stay as they are (in a pair made here: undefined)."""
     shape = _check("kv_read_e4m3", pages, block_tables, context_lens, row_starts, *(out or ()))
-    nb, G, bs, D = shape
-    _starts("kv_read_e4m3", row_starts, block_tables.shape[0])
+    nb, G, bs, D, batch, width = shape
+    _starts("kv_read_e4m3", row_starts, batch)
+    ld_k = ld_v = G * D
     if out is None:
         if dtype not in _TYPES:
             raise TypeError("kv_read_e4m3: rows in bf16, fp16 or fp32")
-        k = torch.empty((rows, G * D), dtype=dtype, device=pages.k.device)
-        out = (k, torch.empty_like(k))
-    k, v = out
-    if k.dtype not in _TYPES or v.dtype is not k.dtype or k.shape != (rows, G * D) or v.shape != (rows, G * D):
-        raise TypeError("kv_read_e4m3: out is a pair of [rows, kv_heads * head_dim] in bf16, fp16 or fp32")
+        k = pages.k.new_empty((rows, ld_k), dtype=dtype)
+        v = torch.empty_like(k)
+    else:
+        k, v = out
+        dtype = k.dtype
+        if dtype not in _TYPES or v.dtype is not dtype or k.shape != (rows, ld_k) or v.shape != (rows, ld_k):
+            raise TypeError("kv_read_e4m3: out is a pair of [rows, kv_heads * head_dim] in bf16, fp16 or fp32")
     if not k.is_cuda:
-        for b in range(block_tables.shape[0]):
+        for b in range(batch):
             first = int(row_starts[b])
             n = max(0, min(_held(pages, block_tables, context_lens, b), int(row_starts[b + 1]) - first, rows - first))
             there = [_page(block_tables, nb, b, i // bs) >= 0 for i in range(n)]
@@ -227,12 +236,14 @@ def kv_read_e4m3(pages: PagesE4M3, block_tables, context_lens, row_starts, rows:
                 x = _values_cpu(codes, exps, block_tables, b, n).reshape(n, G * D).to(to.dtype)
                 to[first:first + n][there] = x[there]
         return k, v
-    if rows == 0 or block_tables.shape[0] == 0:
+    if rows == 0 or batch == 0:
         return k, v
-    if not (_aligned(k) and _aligned(v)):
-        raise ValueError("kv_read_e4m3: rows of out start at multiples of 16 bytes")
+    if out is not None:
+        ld_k, ld_v = _pitch(k), _pitch(v)
+        if not (ld_k and ld_v):
+            raise ValueError("kv_read_e4m3: rows of out start at multiples of 16 bytes")
     a = _READ.pack(*_native(pages, shape), k.data_ptr(), v.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), row_starts.data_ptr(),
-                   k.stride(0), v.stride(0), rows, *block_tables.shape, _TYPES[k.dtype])
+                   ld_k, ld_v, rows, batch, width, _TYPES[dtype])
     N.check(N.kernels().rb_e4m3_read(a, N.stream_ptr()), "rb_e4m3_read")
     return k, v
 
@@ -243,17 +254,18 @@ def paged_attention_decode_e4m3(q, pages: PagesE4M3, block_tables, context_lens,
     (`pages.weight`) grows by its softmax weights, summed over the query heads of its KV head; sequences that share a page must then not be in
     one call."""
     shape = _check("paged_attention_decode_e4m3", pages, block_tables, context_lens, q, out)
-    nb, G, bs, D = shape
-    B, row = block_tables.shape[0], q.shape[-1]
-    if q.dim() != 2 or q.shape[0] != B or row == 0 or row % (G * D):
+    nb, G, bs, D, B, width = shape
+    given, kind = q.shape, q.dtype
+    row = given[-1] if len(given) == 2 else 0
+    if row == 0 or given[0] != B or row % (G * D):
         raise TypeError("paged_attention_decode_e4m3: q is [batch, heads * head_dim], a multiple of the KV heads")
     if accumulate and pages.weight is None:
         raise ValueError("paged_attention_decode_e4m3: these pages keep no weights")
     heads = row // D
     scale = 1.0 / math.sqrt(D) if scale is None else scale
     if out is None:
-        out = torch.empty_like(q) if q.is_contiguous() else torch.empty((B, row), dtype=q.dtype, device=q.device)
-    elif out.dtype is not q.dtype or out.shape != q.shape or out.stride(1) != 1:
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, row))
+    elif out.dtype is not kind or out.shape != given or out.stride(1) != 1:
         raise TypeError("paged_attention_decode_e4m3: out is like q, with contiguous rows")
     if not q.is_cuda:
         for b in range(B):
@@ -269,19 +281,19 @@ def paged_attention_decode_e4m3(q, pages: PagesE4M3, block_tables, context_lens,
                         w = p[:, :, i * bs:(i + 1) * bs].sum(1)
                         pages.weight[page, :, :w.shape[1]] += w
         return out
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    if kind is not torch.bfloat16 and kind is not torch.float16:
         raise TypeError("paged_attention_decode_e4m3: CUDA queries are bf16 or fp16")
     if B == 0:
         return out
-    if q.stride(1) != 1:
-        q = q.contiguous()
-    width = block_tables.shape[1]
+    ld_q, step = q.stride()
+    if step != 1:
+        q, ld_q = q.contiguous(), row
     if width == 0:
         return out.zero_()
     floats = _scratch_floats(B, heads, G, D, width, bs, accumulate)
     scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     a = _DECODE.pack(*_native(pages, shape), q.data_ptr(), out.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), _ptr(scratch),
-                     q.stride(0), out.stride(0), B, width, heads, _TYPES[q.dtype], accumulate, scale)
+                     ld_q, out.stride(0), B, width, heads, _TYPES[kind], accumulate, scale)
     N.check(N.kernels().rb_e4m3_decode(a, N.stream_ptr()), "rb_e4m3_decode")
     return out
 
@@ -298,26 +310,28 @@ def kv_evict_e4m3(pages: PagesE4M3, block_tables, context_lens, keep: int, recen
     A page's exponent becomes the largest of those that its tokens had; codes from smaller ones are rounded to it.  Attention does not ask for
     positions (keys are stored rotated), but a sequence's next position is no longer its length."""
     shape = _check("kv_evict_e4m3", pages, block_tables, context_lens, out_tables)
-    B, G = block_tables.shape[0], shape[1]
+    _, G, bs, _, B, width = shape
     if pages.weight is None:
         raise ValueError("kv_evict_e4m3: these pages keep no weights")
     if keep < 1 or recent < 0 or keep_first < 0 or recent + keep_first > keep:
         raise ValueError("kv_evict_e4m3: keep must be at least 1 and at least recent + keep_first")
-    if out_tables is not None and not (out_tables.dtype is torch.int32 and out_tables.dim() == 2 and out_tables.shape[0] == B and out_tables.is_contiguous()):
-        raise TypeError("kv_evict_e4m3: out_tables is a contiguous int32 table row per sequence")
-    if out_tables is not None and out_tables.shape[1] * shape[2] < min(keep, block_tables.shape[1] * shape[2]):
-        raise ValueError("kv_evict_e4m3: out_tables has no room for the tokens that may be kept")
-    lens = torch.empty_like(context_lens)
-    kept = torch.empty((B, G, keep), dtype=torch.int32, device=pages.k.device)
+    out_width = 0
+    if out_tables is not None:
+        if not (out_tables.dtype is torch.int32 and out_tables.dim() == 2 and out_tables.shape[0] == B and out_tables.is_contiguous()):
+            raise TypeError("kv_evict_e4m3: out_tables is a contiguous int32 table row per sequence")
+        out_width = out_tables.shape[1]
+        if out_width * bs < min(keep, width * bs):
+            raise ValueError("kv_evict_e4m3: out_tables has no room for the tokens that may be kept")
+    lens, kept = torch.empty_like(context_lens), context_lens.new_empty((B, G, keep))
     if not pages.k.is_cuda:
         _evict_cpu(pages, block_tables, context_lens, keep, recent, keep_first, out_tables, lens, kept)
         return lens, kept
     if B == 0:
         return lens, kept
-    if block_tables.shape[1] == 0:
+    if width == 0:
         return lens.zero_(), kept.fill_(-1)
     a = _EVICT.pack(*_native(pages, shape), block_tables.data_ptr(), context_lens.data_ptr(), _ptr(out_tables), kept.data_ptr(), lens.data_ptr(),
-                    B, block_tables.shape[1], 0 if out_tables is None else out_tables.shape[1], keep, recent, keep_first)
+                    B, width, out_width, keep, recent, keep_first)
     N.check(N.kernels().rb_e4m3_evict(a, N.stream_ptr()), "rb_e4m3_evict")
     return lens, kept
 
