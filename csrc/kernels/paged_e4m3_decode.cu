@@ -601,17 +601,15 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
   }
 }
 
-constexpr int kE4Chains = 16;
-
-// Adds the slices of a sequence for one head: 16 chains of every 16th slice, in order, then the chains in order.  COLS: 16-byte columns that a CTA of
-// 128 threads takes, D / 4 or, where a sequence may have many slices, 8, so that more of them read at the same time; the sums are the same.
-// Grid: (heads, sequences, D / 4 / COLS).
-template <typename T, int COLS>
-__global__ void __launch_bounds__(128)
+// Adds the slices of a sequence for one head: 16 chains of every 16th slice, in order (with more than 64 slices 64 chains), then the chains in order.
+// COLS: 16-byte columns that a CTA takes, D / 4 of 128 threads or, MANY, where sequences may have more than 64 slices, 8 of 512 threads: one of 131072
+// tokens takes 10 us with 128 threads and 16 chains.  Grid: (heads, sequences, D / 4 / COLS).
+template <typename T, int COLS, bool MANY>
+__global__ void __launch_bounds__(MANY ? 512 : 128)
 e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
   pdl_wait();
   pdl_launch();
-  constexpr int kChains = kE4Chains, R = 128 / COLS, PER = kChains / R;
+  constexpr int kChains = MANY ? 64 : 16, R = (MANY ? 512 : 128) / COLS, PER = kChains / R;
   __shared__ float4 sum_sh[kChains][COLS];
   __shared__ float2 ml_sh[kChains];
   const int h = blockIdx.x, b = blockIdx.y, z = blockIdx.z, tid = threadIdx.x, D = a.pages.head_dim, c = tid % COLS, r = tid / COLS;
@@ -622,6 +620,7 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
     return;
   }
   if (here == 1 && !a.accumulate) return;            // already written
+  const int chains = MANY && here <= 64 ? 16 : kChains;
   const float* first = e4_partial(a.scratch, a.heads, slices, D, b, h, 0);
   const long long pitch = D + 4;
   // every sum beside its own maximum; a new maximum's factor is a power of two, so that the sums are those under the largest of all
@@ -634,14 +633,14 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
     l[k] = 0.f;
   }
   constexpr int kAhead = PER == 1 ? 8 : 1;           // slices of a chain that are loaded together
-  for (int s0 = r; s0 < here; s0 += kChains * kAhead) {
+  for (int s0 = r; s0 < here && (!MANY || r < chains); s0 += chains * kAhead) {
     float4 x[PER][kAhead];
     float2 ml[PER][kAhead];
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int s = s0 + k * R + i * kChains;
+        const int s = s0 + k * R + i * chains;
         ml[k][i] = make_float2(-INFINITY, 0.f);
         x[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (s < here) {
@@ -662,7 +661,7 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
       m[k] = to;
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        if (s0 + k * R + i * kChains >= here) break;
+        if (s0 + k * R + i * chains >= here) break;
         const float g = e4_factor(ml[k][i].x, to);
         sum[k].x = fmaf(x[k][i].x, g, sum[k].x);
         sum[k].y = fmaf(x[k][i].y, g, sum[k].y);
@@ -683,9 +682,9 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
   float top = -INFINITY, den = 0.f;
 #pragma unroll
   for (int k = 0; k < kChains; ++k) top = fmaxf(top, ml_sh[k].x);      // -infinity where there is no such slice
-#pragma unroll
+#pragma unroll 16
   for (int k = 0; k < kChains; ++k)
-    if (k < here) {
+    if (k < here && k < chains) {
       const float f = e4_factor(ml_sh[k].x, top);
       const float4 x = sum_sh[k][c];
       o.x = fmaf(x.x, f, o.x);
@@ -783,8 +782,8 @@ int decode_launch(const RbE4m3DecodeArgs& a, cudaStream_t stream) {
     e = rbhost::launch_pdl(kern, list ? dim3(some) : whole, threads, smem, stream, 1, *km, *vm, a, h0, slices, status RB_BOUNDS_ARG);
   if (e == cudaSuccess) {
     const bool many = slices > 64;
-    e = rbhost::launch_pdl(many ? rb::e4_merge_kernel<T, 8> : rb::e4_merge_kernel<T, D / 4>, dim3(a.heads, a.batch, many ? D / 32 : 1), dim3(128), 0, stream, 1,
-                           a, slices);
+    e = rbhost::launch_pdl(many ? rb::e4_merge_kernel<T, 8, true> : rb::e4_merge_kernel<T, D / 4, false>, dim3(a.heads, a.batch, many ? D / 32 : 1),
+                           dim3(many ? 512 : 128), 0, stream, 1, a, slices);
   }
   if (e == cudaSuccess && a.accumulate) e = rbhost::launch_pdl(rb::e4_weight_kernel, whole, dim3(rb::kE4Slice), 0, stream, 1, a, slices);
   return static_cast<int>(e);
