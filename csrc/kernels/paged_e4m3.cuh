@@ -74,12 +74,26 @@ __device__ __forceinline__ int e4_page(const int* __restrict__ tables, int max_b
   return p < 0 || p >= num_blocks ? -1 : p;
 }
 
+// Eight numbers of a row.  `largest` takes the larger magnitudes of eight into `acc` as their bits, two 16-bit ones beside each other; `one` makes one number's
+// bits of that, `value` the number; from kNotFinite on they are an infinity's or a NaN's.
 template <typename T>
-struct E4Row;                                        // eight numbers of a row
+struct E4Row;
+__device__ __forceinline__ void e4_largest16(const uint4& u, uint32_t& acc) {
+  acc = __vmaxu2(__vmaxu2(acc, u.x & 0x7fff7fffu), u.y & 0x7fff7fffu);
+  acc = __vmaxu2(__vmaxu2(acc, u.z & 0x7fff7fffu), u.w & 0x7fff7fffu);
+}
 template <>
 struct E4Row<__nv_bfloat16> {
+  static constexpr uint32_t kNotFinite = 0x7f80u;
+  static __device__ __forceinline__ void largest(const uint4 (&raw)[1], uint32_t& acc) { e4_largest16(raw[0], acc); }
+  static __device__ __forceinline__ uint32_t one(uint32_t acc) { return max(acc & 0xffffu, acc >> 16); }
+  static __device__ __forceinline__ float value(uint32_t bits) { return __uint_as_float(bits << 16); }
   static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&x)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint4 u[1] = {*reinterpret_cast<const uint4*>(p)};
+    of(u, x);
+  }
+  static __device__ __forceinline__ void of(const uint4 (&raw)[1], float (&x)[8]) {
+    const uint4 u = raw[0];
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -94,8 +108,16 @@ struct E4Row<__nv_bfloat16> {
 };
 template <>
 struct E4Row<__half> {
+  static constexpr uint32_t kNotFinite = 0x7c00u;
+  static __device__ __forceinline__ void largest(const uint4 (&raw)[1], uint32_t& acc) { e4_largest16(raw[0], acc); }
+  static __device__ __forceinline__ uint32_t one(uint32_t acc) { return max(acc & 0xffffu, acc >> 16); }
+  static __device__ __forceinline__ float value(uint32_t bits) { return __half2float(__ushort_as_half(static_cast<unsigned short>(bits))); }
   static __device__ __forceinline__ void load(const __half* p, float (&x)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint4 u[1] = {*reinterpret_cast<const uint4*>(p)};
+    of(u, x);
+  }
+  static __device__ __forceinline__ void of(const uint4 (&raw)[1], float (&x)[8]) {
+    const uint4 u = raw[0];
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -116,10 +138,26 @@ struct E4Row<__half> {
 };
 template <>
 struct E4Row<float> {
+  static constexpr uint32_t kNotFinite = 0x7f800000u;
+  static __device__ __forceinline__ void largest(const uint4 (&raw)[2], uint32_t& acc) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      acc = max(acc, max(max(raw[i].x & 0x7fffffffu, raw[i].y & 0x7fffffffu), max(raw[i].z & 0x7fffffffu, raw[i].w & 0x7fffffffu)));
+  }
+  static __device__ __forceinline__ uint32_t one(uint32_t acc) { return acc; }
+  static __device__ __forceinline__ float value(uint32_t bits) { return __uint_as_float(bits); }
   static __device__ __forceinline__ void load(const float* p, float (&x)[8]) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    const uint4 u[2] = {reinterpret_cast<const uint4*>(p)[0], reinterpret_cast<const uint4*>(p)[1]};
+    of(u, x);
+  }
+  static __device__ __forceinline__ void of(const uint4 (&raw)[2], float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      x[4 * i] = __uint_as_float(raw[i].x);
+      x[4 * i + 1] = __uint_as_float(raw[i].y);
+      x[4 * i + 2] = __uint_as_float(raw[i].z);
+      x[4 * i + 3] = __uint_as_float(raw[i].w);
+    }
   }
   static __device__ __forceinline__ void store(float* p, const float (&x)[8]) {
     *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
