@@ -160,25 +160,36 @@ def bench_adam(a):
 
 def bench_paged(a):
     """Decode attention over a paged KV cache: `batch` sequences of `context` cached tokens, pages handed out in a
-    shuffled order so that consecutive pages of a sequence are not adjacent in memory."""
+    shuffled order so that consecutive pages of a sequence are not adjacent in memory.  `kv_cache` e4m3: the cache of
+    ops.paged_e4m3, its tokens stored by its own append; `weights`: their attention weights are summed."""
     import math
-    from ..ops import paged
+    from ..ops import paged, paged_e4m3
     B, H, Hk, D, bs = a.batch, a.heads, a.kv_heads, a.head_dim, a.block_size
     per = (a.context + bs - 1) // bs
     nb = B * per + 1
     g = torch.Generator().manual_seed(0)
-    kc = torch.randn(nb, bs, Hk, D, generator=g).bfloat16().cuda()
-    vc = torch.randn(nb, bs, Hk, D, generator=g).bfloat16().cuda()
+    if a.weights and a.kv_cache != "e4m3":
+        raise SystemExit("--weights needs --kv-cache e4m3")
+    if a.kv_cache == "bf16":
+        kc = torch.randn(nb, bs, Hk, D, generator=g).bfloat16().cuda()
+        vc = torch.randn(nb, bs, Hk, D, generator=g).bfloat16().cuda()
     bt = (torch.randperm(nb - 1, generator=g)[:B * per] + 1).to(torch.int32).view(B, per).cuda()
     ctx = torch.full((B,), a.context, dtype=torch.int32, device="cuda")
     q = torch.randn(B, H * D, generator=g).bfloat16().cuda()
     out = torch.empty_like(q)
-    fn = lambda: paged.paged_attention_decode(q, kc, vc, bt, ctx, 1.0 / math.sqrt(D), out=out)
+    if a.kv_cache == "bf16":
+        fn = lambda: paged.paged_attention_decode(q, kc, vc, bt, ctx, 1.0 / math.sqrt(D), out=out)
+    else:
+        pages = paged_e4m3.PagesE4M3.zeros(nb, bs, Hk, D, "cuda", weights=a.weights)
+        for b in range(B):
+            k, v = (torch.randn(a.context, Hk * D, device="cuda").bfloat16() for _ in range(2))
+            paged_e4m3.kv_append_e4m3(pages, k, v, bt[b:b + 1], ctx[:1], torch.tensor([0, a.context], dtype=torch.int32, device="cuda"))
+        fn = lambda: paged_e4m3.paged_attention_decode_e4m3(q, pages, bt, ctx, out=out, accumulate=a.weights)
     ms = timed(fn, a.warmup, a.iters)
-    kv_bytes = 2.0 * B * a.context * Hk * D * 2
+    kv_bytes = 2.0 * B * a.context * Hk * D * (2 if a.kv_cache == "bf16" else 1)
     return report("paged_decode_attention", ms, 0, kv_bytes,
                   {"batch": B, "context": a.context, "heads": H, "kv_heads": Hk, "head_dim": D, "block_size": bs,
-                   "kv_cache_bytes": int(kv_bytes)})
+                   "kv_cache": a.kv_cache, "weights": a.weights, "kv_cache_bytes": int(kv_bytes)})
 
 
 def bench_launch_overhead(a):
@@ -261,6 +272,8 @@ def main(argv=None):
     pg.add_argument("--kv-heads", type=int, default=8)
     pg.add_argument("--head-dim", type=int, default=128)
     pg.add_argument("--block-size", type=int, default=16)
+    pg.add_argument("--kv-cache", default="bf16", choices=["bf16", "e4m3"])
+    pg.add_argument("--weights", action="store_true", help="sum every cached token's attention weight (e4m3)")
     lo = sub.add_parser("launch-overhead")
     lo.add_argument("--calls", type=int, default=5000)
     a = ap.parse_args(argv)
