@@ -74,7 +74,10 @@ template <int D, int NH>
 struct E4Layout {
   static constexpr int kTile = 16 * D;                                   // bytes of a tile's keys; its values follow
   static constexpr int kRing = kE4Warps * kE4Stages * 2 * kTile;
-  static int bytes(int heads) { return kRing + kE4Warps * heads * D * 4 + 1024; }      // the warps' sums behind the ring
+  // The warps' sums lie behind the ring, those of `kRound` heads at a time (of a cluster those of all heads): with 4 heads of 128 three CTAs fit on an SM.
+  // 64 sequences of 4096, 4 KV heads for 32 heads of 128, one B200: 78.9 us with 8 at a time and two CTAs an SM, 74.8 so.
+  static constexpr int kRound = NH == 1 && D == 128 ? 4 : 8;
+  static int bytes(int heads) { return kRing + kE4Warps * heads * D * 4 + 1024; }
 };
 
 // Warp w of a CTA takes tiles w, w + 4, w + 8, w + 12 of 16 tokens of a slice; its sums and those of the other warps are added in the order of the
@@ -462,63 +465,75 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
         }
       }
     }
-    // ---- the slice's sums: all warps' together
+    // ---- the slice's sums: all warps' together, those of some heads after those of others
 #pragma unroll
     for (int r = 0; r < NH; ++r) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {                  // head r * 8 + 2 tq + j, dimensions gq * D / 8 .., 16 bytes at a time, swizzled by the head
+      for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[r][j] += __shfl_xor_sync(0xffffffffu, l[r][j], x);
-        const int head = r * 8 + tq * 2 + j;
-        if (head >= heads) continue;
         if (gq == 0) {
-          m_sh[warp][head] = m[r][j];
-          l_sh[warp][head] = l[r][j];
+          m_sh[warp][r * 8 + tq * 2 + j] = m[r][j];
+          l_sh[warp][r * 8 + tq * 2 + j] = l[r][j];
         }
-        float* row = merge + (warp * heads + head) * D;
-#pragma unroll
-        for (int t = 0; t < MT; t += 2)
-          *reinterpret_cast<float4*>(row + (((gq * (D / 32) + t / 2) ^ tq) << 2)) = make_float4(o[t][r][j], o[t][r][2 + j], o[t + 1][r][j], o[t + 1][r][2 + j]);
       }
     }
-    if (LIST && at.left <= 1) pdl_launch();
-    __syncthreads();
     const bool whole = !CLUSTER && n_at <= kE4Slice; // the sequence has no other slice
-    for (int i = threadIdx.x; i < heads * (D / 4); i += kE4Warps * 32) {
-      const int head = i / (D / 4), d = i % (D / 4);
-      float top = m_sh[0][head];
+    constexpr int kRound = CLUSTER ? NH * 8 : L::kRound;
+#pragma unroll 1
+    for (int hb = 0; hb < heads; hb += kRound) {
+      const int rows = min(kRound, heads - hb);        // of a warp in `merge`
+      if (hb > 0) __syncthreads();
 #pragma unroll
-      for (int w = 1; w < kE4Warps; ++w) top = fmaxf(top, m_sh[w][head]);
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      float den = 0.f;
+      for (int r = 0; r < NH; ++r) {
 #pragma unroll
-      for (int w = 0; w < kE4Warps; ++w) {
-        const float mw = m_sh[w][head], f = mw == -INFINITY ? 0.f : e4_ex2(mw - top);
-        den = fmaf(l_sh[w][head], f, den);
-        const float4 x = *reinterpret_cast<const float4*>(merge + (w * heads + head) * D + ((d ^ (head >> 1 & 3)) << 2));
-        sum.x = fmaf(x.x, f, sum.x);
-        sum.y = fmaf(x.y, f, sum.y);
-        sum.z = fmaf(x.z, f, sum.z);
-        sum.w = fmaf(x.w, f, sum.w);
+        for (int j = 0; j < 2; ++j) {                  // head r * 8 + 2 tq + j, dimensions gq * D / 8 .., 16 bytes at a time, swizzled by the head
+          const int head = r * 8 + tq * 2 + j;
+          if (head < hb || head >= hb + rows) continue;
+          float* row = merge + (warp * rows + head - hb) * D;
+#pragma unroll
+          for (int t = 0; t < MT; t += 2)
+            *reinterpret_cast<float4*>(row + (((gq * (D / 32) + t / 2) ^ tq) << 2)) = make_float4(o[t][r][j], o[t][r][2 + j], o[t + 1][r][j], o[t + 1][r][2 + j]);
+        }
       }
-      if (CLUSTER) {                                 // where this thread read the first warp's
-        *reinterpret_cast<float4*>(merge + head * D + ((d ^ (head >> 1 & 3)) << 2)) = sum;
-        if (d == 0) ml_sh[head] = make_float2(top, den);
-        continue;
-      }
-      const int h = at.hk * group + h0 + head;
-      if (whole) {
-        const float inv = 1.f / den;
-        T* out = reinterpret_cast<T*>(a.out) + at.b * a.ld_o + static_cast<long long>(h) * D + d * 4;
-        e4_put(out, sum.x * inv);
-        e4_put(out + 1, sum.y * inv);
-        e4_put(out + 2, sum.z * inv);
-        e4_put(out + 3, sum.w * inv);
-      }
-      if (!whole || a.accumulate) {                  // the weights' denominators come from here too
-        float* out = e4_partial(a.scratch, a.heads, slices, D, at.b, h, at.s);
-        if (d == 0) *reinterpret_cast<float2*>(out) = make_float2(top, den);
-        *reinterpret_cast<float4*>(out + 4 + d * 4) = sum;
+      if (LIST && at.left <= 1) pdl_launch();
+      __syncthreads();
+      for (int i = threadIdx.x; i < rows * (D / 4); i += kE4Warps * 32) {
+        const int head = hb + i / (D / 4), d = i % (D / 4);
+        float top = m_sh[0][head];
+#pragma unroll
+        for (int w = 1; w < kE4Warps; ++w) top = fmaxf(top, m_sh[w][head]);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        float den = 0.f;
+#pragma unroll
+        for (int w = 0; w < kE4Warps; ++w) {
+          const float mw = m_sh[w][head], f = mw == -INFINITY ? 0.f : e4_ex2(mw - top);
+          den = fmaf(l_sh[w][head], f, den);
+          const float4 x = *reinterpret_cast<const float4*>(merge + (w * rows + head - hb) * D + ((d ^ (head >> 1 & 3)) << 2));
+          sum.x = fmaf(x.x, f, sum.x);
+          sum.y = fmaf(x.y, f, sum.y);
+          sum.z = fmaf(x.z, f, sum.z);
+          sum.w = fmaf(x.w, f, sum.w);
+        }
+        if (CLUSTER) {                                 // where this thread read the first warp's
+          *reinterpret_cast<float4*>(merge + head * D + ((d ^ (head >> 1 & 3)) << 2)) = sum;
+          if (d == 0) ml_sh[head] = make_float2(top, den);
+          continue;
+        }
+        const int h = at.hk * group + h0 + head;
+        if (whole) {
+          const float inv = 1.f / den;
+          T* out = reinterpret_cast<T*>(a.out) + at.b * a.ld_o + static_cast<long long>(h) * D + d * 4;
+          e4_put(out, sum.x * inv);
+          e4_put(out + 1, sum.y * inv);
+          e4_put(out + 2, sum.z * inv);
+          e4_put(out + 3, sum.w * inv);
+        }
+        if (!whole || a.accumulate) {                  // the weights' denominators come from here too
+          float* out = e4_partial(a.scratch, a.heads, slices, D, at.b, h, at.s);
+          if (d == 0) *reinterpret_cast<float2*>(out) = make_float2(top, den);
+          *reinterpret_cast<float4*>(out + 4 + d * 4) = sum;
+        }
       }
     }
     if (CLUSTER) {
@@ -757,7 +772,7 @@ int decode_launch(const RbE4m3DecodeArgs& a, cudaStream_t stream) {
   const CUtensorMap* vm = km ? rbhost::get_tmap_2d(p.v, 1, 128, rows, 128, 128, D / 8, 1, &err) : nullptr;
   unsigned int* status = rbhost::status_ptr();
   if (!vm || !status) return err ? err : -3;
-  const int group = a.heads / p.kv_heads, most = group < NH * 8 ? group : NH * 8, smem = L::bytes(most);
+  const int group = a.heads / p.kv_heads, most = group < NH * 8 ? group : NH * 8, smem = L::bytes(most < L::kRound ? most : L::kRound);
   static int per_sm[NH * 8 + 1][64] = {};            // CTAs of a list that fit on an SM, by the heads that a pass has
   const int dev = rbhost::device_slot();
   if (!per_sm[most][dev]) {
@@ -772,8 +787,8 @@ int decode_launch(const RbE4m3DecodeArgs& a, cudaStream_t stream) {
   }
   const dim3 threads(rb::kE4Warps * 32), whole(slices, p.kv_heads, a.batch);
   if (in_clusters(a.batch, p.kv_heads, slices, group))
-    return static_cast<int>(rbhost::launch_pdl(rb::e4_decode_kernel<T, D, NH, rb::kE4Cluster>, whole, threads, smem + (a.accumulate ? rb::kE4Slice * most * 4 : 0),
-                                               stream, slices, *km, *vm, a, 0, slices, status RB_BOUNDS_ARG));
+    return static_cast<int>(rbhost::launch_pdl(rb::e4_decode_kernel<T, D, NH, rb::kE4Cluster>, whole, threads,
+                                               L::bytes(most) + (a.accumulate ? rb::kE4Slice * most * 4 : 0), stream, slices, *km, *vm, a, 0, slices, status RB_BOUNDS_ARG));
   const int some = per_sm[most][dev] * rbhost::device_sm_count();
   const bool list = static_cast<long long>(a.batch) * p.kv_heads * slices > some;
   auto kern = list ? rb::e4_decode_kernel<T, D, NH, rb::kE4List> : rb::e4_decode_kernel<T, D, NH, rb::kE4Grid>;
