@@ -94,9 +94,12 @@ struct E4Layout {
 // head are a cluster and merge their sums, and add the weights, through distributed shared memory.
 enum { kE4Grid, kE4List, kE4Cluster };
 
-// The factor that brings sums under the maximum m to the maximum `to`.  Maxima are whole, so it is exact, and a sum of such sums does not depend on which
-// maximum they are brought to on the way.
-__device__ __forceinline__ float e4_factor(float m, float to) { return m == to ? 1.f : e4_ex2(m - to); }
+// The factor that brings sums under the maximum m to the maximum `to` >= m.  Maxima are whole, so it is an exact power of two, and a sum of such sums does
+// not depend on which maximum they are brought to on the way.
+__device__ __forceinline__ float e4_factor(float m, float to) {
+  const float d = m == to ? 0.f : m - to;            // -infinity: no sum yet, or no maximum at all
+  return d < -126.f ? 0.f : e4_two(static_cast<int>(d));
+}
 
 // A weight is 2^(s - m) / den = 2^(s - (m + x)) / (den / 2^x), with the x that brings den / 2^x into [1, 2): (m + x, 2^x / den).
 __device__ __forceinline__ float2 e4_norm_of(float m, float den) {
@@ -401,7 +404,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) to[j] = fmaxf(to[j], __shfl_xor_sync(0xffffffffu, to[j], x));
           to[j] = fmaxf(to[j], m[r][j]);
-          grow[r][j] = to[j] == m[r][j] ? 1.f : e4_ex2(m[r][j] - to[j]);
+          grow[r][j] = e4_factor(m[r][j], to[j]);
           moved |= to[j] != m[r][j];
           m[r][j] = to[j];
           l[r][j] *= grow[r][j];
@@ -507,7 +510,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
         float den = 0.f;
 #pragma unroll
         for (int w = 0; w < kE4Warps; ++w) {
-          const float mw = m_sh[w][head], f = mw == -INFINITY ? 0.f : e4_ex2(mw - top);
+          const float mw = m_sh[w][head], f = mw == -INFINITY ? 0.f : e4_factor(mw, top);
           den = fmaf(l_sh[w][head], f, den);
           const float4 x = *reinterpret_cast<const float4*>(merge + (w * rows + head - hb) * D + ((d ^ (head >> 1 & 3)) << 2));
           sum.x = fmaf(x.x, f, sum.x);
