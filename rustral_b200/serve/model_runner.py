@@ -43,7 +43,7 @@ class StepBatch:
     on the device), where they came with the step's other inputs.  `moved`: the decoded rows' positions are not their lengths less one."""
 
     def __init__(self, ids, pos, slots, spans, rd, tables, bt, ctx, block_size, segments=None, arrived=None, cached=None, moved=False):
-        self.moved, self._packed = moved, None
+        self.moved, self._packed, self._groups = moved, None, None
         self.ids, self._pos, self._slots, self.arrived = ids, pos, slots, arrived      # int64 device tensors, one entry per row
         self.spans = spans                                        # (first row, end row, first position) per portion
         self.rd, self.rows = rd, ids.shape[0]
@@ -110,6 +110,22 @@ class StepBatch:
                 starts = torch.tensor([r0 for r0, _, _ in self.spans] + list(range(self.rd, self.rows + 1)), dtype=torch.int32, device=dev)
                 self._packed = (bt.contiguous(), lens if self.ctx is None else torch.cat([lens, self.ctx]), starts)
         return self._packed
+
+    def read_groups(self, row_bytes: int) -> list:
+        """The portions that do not begin at 0, in groups whose positions take at most MOST_GATHERED bytes (or one portion): (their indices, block
+        tables, first row of each and the end as a list and int32 on the device, lengths).  Formed once for all layers."""
+        if self._groups is None:
+            bt, lens, _ = self.packed()
+            groups = []
+            for i, (r0, r1, start) in enumerate(self.spans):
+                if start and (not groups or (groups[-1][1][-1] + start + r1 - r0) * row_bytes > MOST_GATHERED):
+                    groups.append(([], [0]))
+                if start:
+                    groups[-1][0].append(i)
+                    groups[-1][1].append(groups[-1][1][-1] + start + r1 - r0)
+            dev = self.ids.device
+            self._groups = [(later, bt[later].contiguous(), ends, torch.tensor(ends, dtype=torch.int32, device=dev), lens[later]) for later, ends in groups]
+        return self._groups
 
     def row_tables(self):
         """(block tables int32 [sequences, width], sequence index int32 per row) over all rows of the step."""
@@ -270,41 +286,23 @@ class ModelRunner:
         bt, lens, starts = sb.packed()
         e4m3_ops.kv_append_e4m3(pages, k2, v2, bt, lens, starts)
         a = torch.empty((T, H * dk), dtype=q.dtype, device=self.device)
-        whole = [i for i, span in enumerate(sb.spans) if span[2] == 0]
-        groups, size = [[]], 0                       # later portions that are read together
-        for i, (r0, r1, start) in enumerate(sb.spans):
-            if start == 0:
-                continue
-            more = 2 * (start + r1 - r0) * G * dk * q.element_size()
-            if groups[-1] and size + more > MOST_GATHERED:
-                groups.append([])
-                size = 0
-            groups[-1].append(i)
-            size += more
-        for later in groups:
+        parts = [(r0, r1, k2[r0:r1], v2[r0:r1]) for r0, r1, start in sb.spans if start == 0]
+        for later, tables, ends, starts, sizes in sb.read_groups(2 * G * dk * q.element_size()):
+            kk, vv = e4m3_ops.kv_read_e4m3(pages, tables, sizes, starts, ends[-1], dtype=q.dtype)
+            parts += [(*sb.spans[i][:2], kk[lo:hi], vv[lo:hi]) for i, lo, hi in zip(later, ends, ends[1:])]
+            self._attend_parts(q, a, parts, scale)
             parts = []
-            for i in whole:
-                r0, r1, _ = sb.spans[i]
-                parts.append((q[r0:r1].view(1, r1 - r0, H, dk), k2[r0:r1].view(1, r1 - r0, G, dk), v2[r0:r1].view(1, r1 - r0, G, dk),
-                              a[r0:r1].view(1, r1 - r0, H, dk)))
-            whole = []
-            if later:
-                ends = [0]
-                for i in later:
-                    r0, r1, start = sb.spans[i]
-                    ends.append(ends[-1] + start + r1 - r0)
-                which = torch.tensor(later, device=self.device)
-                kk, vv = e4m3_ops.kv_read_e4m3(pages, bt.index_select(0, which), lens.index_select(0, which),
-                                               torch.tensor(ends, dtype=torch.int32, device=self.device), ends[-1], dtype=q.dtype)
-                for i, lo, hi in zip(later, ends, ends[1:]):
-                    r0, r1, _ = sb.spans[i]
-                    parts.append((q[r0:r1].view(1, r1 - r0, H, dk), kk[lo:hi].view(1, hi - lo, G, dk), vv[lo:hi].view(1, hi - lo, G, dk),
-                                  a[r0:r1].view(1, r1 - r0, H, dk)))
-            if parts:
-                attn_ops.prompt_attention_many(parts, scale)
+        self._attend_parts(q, a, parts, scale)
         if rd < T:
             e4m3_ops.paged_attention_decode_e4m3(q[rd:], pages, sb.bt, sb.ctx, scale, out=a[rd:], accumulate=self.kv_weights)
         return a
+
+    def _attend_parts(self, q, a, parts, scale: float) -> None:
+        """Prompt attention of portions (first row, end row, keys, values) from q into a."""
+        H, G = self.n_head, self.n_kv_head
+        if parts:
+            attn_ops.prompt_attention_many([(q[r0:r1].view(1, r1 - r0, H, -1), k.view(1, k.shape[0], G, -1), v.view(1, v.shape[0], G, -1),
+                                             a[r0:r1].view(1, r1 - r0, H, -1)) for r0, r1, k, v in parts], scale)
 
     def attend_latent(self, l: int, q, kv, sb: StepBatch, m, w_ukv, table, gate=None) -> torch.Tensor:
         """Latent attention of layer `l` (`m`: models.layered.LatentSpec) for every row of `sb`.  q [rows, heads * qk_dim] (not rotated
