@@ -187,7 +187,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
     const int t = p.s * (kE4Slice / 16) + tile_in;
     if (t * 16 >= n) return kNone;
     const int i = per_page == 1 ? t : t / per_page;
-    return a.block_tables[static_cast<long long>(p.b) * a.max_blocks + i];             // n is no more than the table has room for
+    return max(a.block_tables[static_cast<long long>(p.b) * a.max_blocks + i], -1);    // n is no more than the table has room for; never kNone
   };
   // the tile counted over a whole array (-1: none), and its page and head as the exponents are counted
   auto locate = [&](const E4Place& p, int page, int& tile, int& where) {

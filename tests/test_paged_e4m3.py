@@ -237,6 +237,24 @@ def test_attention_where_one_key_has_all_the_weight(device):
     check_attention(device, lens, 1, 4, 128, 16, torch.bfloat16, False, seed=9, scale=0.0, pages=p0)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens", [[40, 300], [300, 2500] * 40])
+def test_attention_over_tables_with_pages_that_are_not_there(device, lens):
+    """Whatever number a table has for a page that is not there, it counts as page 0, and no weight is added for it."""
+    p0 = filled(sum((n + 15) // 16 for n in lens) + 1, 16, 2, 64, 6, weights=True)
+    t = tables_of(lens, 16, p0.k.shape[0], 6)
+    q = torch.randn(len(lens), 8 * 64, generator=torch.Generator().manual_seed(7)).bfloat16().to(device)
+    got = []
+    for gone in (-1, 1 << 30, -2 ** 31, 2 ** 31 - 1):
+        t[:, 1], p = gone, to(p0, device)
+        out = ops.paged_attention_decode_e4m3(q, p, t.to(device), ints(lens, device), accumulate=True)
+        got.append((out, p.weight))
+    for out, weight in got[1:]:
+        assert torch.equal(out, got[0][0]) and torch.equal(weight, got[0][1])
+    t[:, 1] = 0
+    assert torch.equal(ops.paged_attention_decode_e4m3(q, to(p0, device), t.to(device), ints(lens, device)), got[0][0])
+
+
 @pytest.mark.gpu
 def test_attention_of_queries_of_all_sizes():
     """Query rows far apart in size, of bf16's smallest and largest numbers too; strided rows, an output in place of columns."""
