@@ -142,7 +142,7 @@ e4_read_kernel(const RbE4m3ReadArgs a RB_BOUNDS_PARAM) {
       int b = b0;
       while (a.row_starts[b + 1] <= r) ++b;          // ends: r is in front of the last one
       const int i = static_cast<int>(r) - a.row_starts[b];
-      if (i < a.context_lens[b]) {
+      if (i >= 0 && i < a.context_lens[b]) {           // starts that do not ascend may put a row in front of its sequence
         page = e4_page(a.block_tables, a.max_blocks, a.pages.num_blocks, b, i / bs);
         if (page < 0) RB_BOUNDS_HIT(104);
         off = i % bs;

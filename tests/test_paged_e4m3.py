@@ -635,3 +635,15 @@ def test_rows_and_lengths_that_do_not_match(device):
     ops.kv_read_e4m3(p, t.to(device), ints(lens, device), ints(starts, device), 50, out=(out, out.clone()))
     for row, filled_ in ((0, True), (1, True), (2, False), (5, True), (20, True), (21, False), (29, False), (30, False), (45, False), (46, True), (49, True)):
         assert bool((out[row] == 2.0).all()) != filled_
+
+
+@pytest.mark.gpu
+def test_read_with_starts_that_do_not_ascend():
+    """A row in front of the sequence that it is counted to has no position: it stays as it was."""
+    p = to(filled(8, 16, 1, 64, 0), "cuda")
+    t = torch.arange(1, 6, dtype=I32, device="cuda").view(5, 1)
+    out = [torch.full((40, 64), 7.0, dtype=torch.bfloat16, device="cuda") for _ in "kv"]
+    ops.kv_read_e4m3(p, t, ints([16] * 5, "cuda"), ints([0, 5, 20, 21, 5, 40], "cuda"), 40, out=out)
+    # of rows 16 to 31, whose search begins with sequence 2: 16 to 19 lie in front of it, 20 is its first, 21 on are counted to sequence 4
+    for x in out:
+        assert bool((x[16:20] == 7.0).all()) and not bool((x[20] == 7.0).all())
