@@ -170,7 +170,8 @@ struct E4Row<float> {
 namespace rbhost {
 // 0 where the pages are as paged_e4m3.h says
 inline int e4_check(const RbPagesE4m3& p) {
-  if (!p.k || !p.v || !p.k_exp || !p.v_exp || p.num_blocks <= 0 || p.num_blocks > 0x7fffffffll || p.block_size <= 0 || (p.block_size & 15) || p.kv_heads <= 0 ||
+  if (!p.k || !p.v || !p.k_exp || !p.v_exp || p.num_blocks <= 0 || p.num_blocks > 0x7fffffffll || p.block_size <= 0 || (p.block_size & 15) ||
+      p.block_size > 1 << 20 || p.kv_heads <= 0 ||
       (p.head_dim != 64 && p.head_dim != 128))
     return -1;
   if ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15) return -2;

@@ -2,7 +2,7 @@
 //
 // A page holds block_size tokens of a sequence.  For every KV head it has a tile of codes [block_size, head_dim] for keys and one for
 // values, and for each tile a power of two: the number that code c stands for is c * 2^exp, exp in [-100, 119].  block_size is a multiple
-// of 16, head_dim 64 or 128.  All arrays are contiguous and 16-byte aligned.
+// of 16, at most 2^20, head_dim 64 or 128; a row of a block table has room for fewer than 2^30 tokens.  All arrays are contiguous and 16-byte aligned.
 #pragma once
 #ifdef __cplusplus
 extern "C" {

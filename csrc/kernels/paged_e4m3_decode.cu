@@ -826,7 +826,7 @@ RB_API int rb_e4m3_decode(const RbE4m3DecodeArgs* args, void* stream_v) {
   if (const int bad = rbhost::e4_check(a.pages)) return bad;
   if (!a.q || !a.out || !a.block_tables || !a.context_lens || a.max_blocks <= 0 || a.heads <= 0 || a.heads % a.pages.kv_heads ||
       (!a.scratch && !in_clusters(a.batch, a.pages.kv_heads, e4_slices(a.max_blocks, a.pages.block_size), a.heads / a.pages.kv_heads)) ||
-      a.batch > 65535 || a.pages.kv_heads > 65535 || (a.accumulate && !a.pages.weight) ||
+      a.batch > 65535 || a.pages.kv_heads > 65535 || (a.accumulate && !a.pages.weight) || static_cast<long long>(a.max_blocks) * a.pages.block_size > 0x3fffffff ||
       static_cast<long long>(a.batch) * a.pages.kv_heads * e4_slices(a.max_blocks, a.pages.block_size) > 0x3fffffff)
     return -1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_v);

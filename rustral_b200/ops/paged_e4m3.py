@@ -21,6 +21,7 @@ from .. import _native as N
 
 C = N.C
 LEAST_EXPONENT, MOST_EXPONENT, LARGEST_CODE = -100, 119, 448.0
+MOST_BLOCK, MOST_TOKENS = 1 << 20, (1 << 30) - 1        # on a GPU: of a page, of a table's row
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -42,7 +43,7 @@ N._LAUNCHES["rb_e4m3_evict"] = 2
 class PagesE4M3:
     """The pages of one layer: codes `k`, `v` (float8_e4m3fn [num_blocks, kv_heads, block_size, head_dim]), exponents `k_exp`, `v_exp` (int8
     [num_blocks, kv_heads]) and, where attention weights are kept, `weight` (fp32 [num_blocks, kv_heads, block_size]).  On a GPU block_size is a
-    multiple of 16 and head_dim 64 or 128."""
+    multiple of 16, at most 2^20, head_dim 64 or 128, and a table's row has room for fewer than 2^30 tokens."""
     k: torch.Tensor
     v: torch.Tensor
     k_exp: torch.Tensor
@@ -86,8 +87,10 @@ def _check(what: str, pages: PagesE4M3, block_tables, context_lens, *others) -> 
         if t is not None and t.get_device() != dev:
             raise ValueError(f"{what}: tensors on {k.device} and {t.device}")
     if dev >= 0:
-        if bs & 15 or (D != 64 and D != 128):
-            raise ValueError(f"{what}: pages of a multiple of 16 tokens and heads of 64 or 128 are required, not {bs} and {D}")
+        if bs & 15 or bs > MOST_BLOCK or (D != 64 and D != 128):
+            raise ValueError(f"{what}: pages of a multiple of 16 tokens, at most 2^20, and heads of 64 or 128 are required, not {bs} and {D}")
+        if table[1] * bs > MOST_TOKENS:
+            raise ValueError(f"{what}: a table's row has room for fewer than 2^30 tokens, not {table[1]} pages of {bs}")
         if dev != torch._C._cuda_getDevice():
             raise ValueError(f"{what}: the pages are on {k.device}, which is not the current device")
     return nb, G, bs, D, table[0], table[1]

@@ -597,6 +597,18 @@ def test_refuses_what_no_kernel_takes():
         ops.kv_read_e4m3(p, t, n, ints([0, 1, 2], "cuda"), 2, out=(x, x))
 
 
+@pytest.mark.gpu
+def test_refuses_more_tokens_than_the_kernels_count():
+    for bs, width in ((1 << 20, 1024), ((1 << 20) + 16, 1)):
+        p = ops.PagesE4M3.zeros(1, bs, 1, 64, "cuda", weights=True)
+        t, n = torch.zeros(1, width, dtype=I32, device="cuda"), ints([1], "cuda")
+        x = torch.zeros(1, 64, device="cuda").bfloat16()
+        for call in (lambda: ops.kv_append_e4m3(p, x, x, t, n), lambda: ops.kv_read_e4m3(p, t, n, ints([0, 1], "cuda"), 1),
+                     lambda: ops.paged_attention_decode_e4m3(x, p, t, n), lambda: ops.kv_evict_e4m3(p, t, n, 1)):
+            with pytest.raises(ValueError):
+                call()
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_empty_calls(device):
     p, t, n = small(device)
