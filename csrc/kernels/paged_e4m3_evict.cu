@@ -8,7 +8,7 @@ namespace rb {
 
 namespace cg = cooperative_groups;
 
-constexpr int kE4SelectThreads = 512, kE4SelectWarps = kE4SelectThreads / 32;
+constexpr int kE4SelectThreads = 1024, kE4SelectWarps = kE4SelectThreads / 32;
 constexpr int kE4SelectKeys = 16384;                 // keys that a CTA holds
 
 // order-preserving: larger weights have larger keys, -0 is 0, a NaN is largest
@@ -18,19 +18,20 @@ __device__ __forceinline__ uint32_t e4_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// The places that stay, for a sequence and KV head.  The `take`-th largest key of the tokens that may go is found by radix selection, passes of
-// 11, 11 and 10 bits over keys in shared memory; every pass counts the next digit of the keys that still may be it (weights have few exponents, and
-// threads that count the same digit wait for one another, so digits are long).  Then each warp counts what stays of its tokens, and writes it where the
-// counts in front of it end.  Sequences of more than 16384 tokens are shared by the CTAs of a cluster (x: rank in the cluster), which add their counts
-// through distributed shared memory; of more than 131072, the keys are read from the pages again in every pass.
-// Bound by latencies: table, weight and the passes' barriers follow one another.
+// The places that stay, for a sequence and KV head.  The `take`-th largest key of the tokens that may go is found by radix selection over keys in shared
+// memory, 11 bits a pass: every pass counts the next digit of the keys that still may be it, until all that are left stay.  The digits are those of a
+// key's distance from the least one: weights have few exponents, and threads that count the same digit wait for one another.  Then each warp counts what
+// stays of its tokens, and writes it where the counts in front of it end.  Sequences of more than 16384 tokens are shared by the CTAs of a cluster (x: rank
+// in the cluster), which add their counts through distributed shared memory; of more than 131072, the keys are read from the pages again in every pass.
+// Bound by latencies: table, weight and the passes' barriers follow one another, and a warp goes through its keys.  24 sequences of 1500 to 8192, 8 KV heads,
+// one B200: with digits of the keys themselves 25 us, of distances 23.5, with 1024 threads in place of 512 20.8.
 template <bool CLUSTER>
-__global__ void __launch_bounds__(kE4SelectThreads, 3)
+__global__ void __launch_bounds__(kE4SelectThreads, 2)
 e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
   pdl_wait();
   pdl_launch();
   extern __shared__ uint32_t e4_keys[];
-  __shared__ uint32_t hist[2048], part[2], digit[2];
+  __shared__ uint32_t hist[2048], part[2], ends[2], digit[3];
   __shared__ uint32_t warp_n[2][kE4SelectWarps];
   const int ranks = CLUSTER ? gridDim.x : 1, rank = CLUSTER ? blockIdx.x : 0;
   const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -62,6 +63,7 @@ e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
     return there ? e4_key(w) : 0u;
   };
   const bool held = mine <= kE4SelectKeys;
+  uint32_t least = 0xffffffffu, most = 0;            // keys
   if (held)
     for (int i0 = tid; i0 < mine; i0 += 4 * kE4SelectThreads) {         // four pages, then four weights: loads that do not wait for one another
       int page[4];
@@ -73,29 +75,63 @@ e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
 #pragma unroll
       for (int x = 0; x < 4; ++x)
         if (i0 + x * kE4SelectThreads < mine) e4_keys[i0 + x * kE4SelectThreads] = k[x];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        least = min(least, k[x]);
+        most = max(most, k[x]);
+      }
     }
-  __syncthreads();
   // f(place, key) for this warp's tokens, 32 at a time; a lane without a token has place -1
   auto each = [&](auto f) {
     if (held) {
-#pragma unroll 2
+#pragma unroll 4
       for (int i = w0 + lane; i - lane < w1; i += 32) f(i < w1 ? lo + i : -1, i < w1 ? e4_keys[i] : 0u);
     } else {
 #pragma unroll 4
       for (int i = w0 + lane; i - lane < w1; i += 32) f(i < w1 ? lo + i : -1, i < w1 ? key_of(lo + i, page_of(lo + i)) : 0u);
     }
   };
-  uint32_t prefix = 0, mask = 0, need = take;        // keys that begin with `prefix`; how many of them stay
+  if (!held)
+    each([&](int t, uint32_t k) {
+      if (t >= 0) {
+        least = min(least, k);
+        most = max(most, k);
+      }
+    });
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) {
+    warp_n[0][warp] = least;
+    warp_n[1][warp] = most;
+  }
+  __syncthreads();
+  least = __reduce_min_sync(0xffffffffu, warp_n[0][lane % kE4SelectWarps]);
+  most = __reduce_max_sync(0xffffffffu, warp_n[1][lane % kE4SelectWarps]);
+  if (CLUSTER) {
+    if (tid == 0) {
+      ends[0] = least;
+      ends[1] = most;
+    }
+    cg::this_cluster().sync();
+    for (int r = 1; r < ranks; ++r) {
+      least = min(least, *cg::this_cluster().map_shared_rank(&ends[0], (rank + r) % ranks));
+      most = max(most, *cg::this_cluster().map_shared_rank(&ends[1], (rank + r) % ranks));
+    }
+  }
+  // bits from `shift` on of the distances from the least key: those above `prefix` stay, and `need` of those equal to it
+  uint32_t prefix = 0, need = take;
+  int shift = most > least ? 32 - __clz(most - least) : 0;
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const uint32_t digits = pass < 2 ? 2047u : 1023u;
+  while (shift > 0) {
+    const int known = shift, width = min(shift, 11);
+    shift -= width;
     constexpr int kBins = 2048 / kE4SelectThreads;   // of a thread
 #pragma unroll
     for (int j = 0; j < kBins; ++j) hist[tid + j * kE4SelectThreads] = 0;
     __syncthreads();
     each([&](int t, uint32_t k) {
-      if (t >= 0 && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digits], 1u);
+      const uint32_t d = k - least;
+      if (t >= 0 && (d >> (known - 1) >> 1) == prefix) atomicAdd(&hist[(d >> shift) & ((1u << width) - 1)], 1u);
     });
     if (CLUSTER) cg::this_cluster().sync();
     else __syncthreads();
@@ -123,21 +159,23 @@ e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
         if (above < need && need <= above + c[j]) {
           digit[0] = 2047 - tid * kBins - j;
           digit[1] = need - above;
+          digit[2] = c[j];
         }
         above += c[j];
       }
     }
     if (CLUSTER) cg::this_cluster().sync();          // and nobody reads another's counts any more
     else __syncthreads();
-    prefix |= digit[0] << shift;
-    mask |= digits << shift;
+    prefix = prefix << width | digit[0];
     need = digit[1];
+    if (need == digit[2]) break;                     // all that are equal stay
   }
-  // keys above `prefix` stay, and of those equal to it the first `need`
+  // of the equal ones, the first `need` stay
   uint32_t above = 0, equal = 0;                     // of this warp
   each([&](int t, uint32_t k) {
-    above += t >= 0 && k > prefix ? 1 : 0;
-    equal += t >= 0 && k == prefix ? 1 : 0;
+    const uint32_t d = (k - least) >> shift;
+    above += t >= 0 && d > prefix ? 1 : 0;
+    equal += t >= 0 && d == prefix ? 1 : 0;
   });
   above = __reduce_add_sync(0xffffffffu, above);
   equal = __reduce_add_sync(0xffffffffu, equal);
@@ -161,7 +199,7 @@ e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
     }
   }
   each([&](int t, uint32_t k) {
-    const uint32_t gt = __ballot_sync(0xffffffffu, t >= 0 && k > prefix), eq = __ballot_sync(0xffffffffu, t >= 0 && k == prefix);
+    const uint32_t d = (k - least) >> shift, gt = __ballot_sync(0xffffffffu, t >= 0 && d > prefix), eq = __ballot_sync(0xffffffffu, t >= 0 && d == prefix);
     const uint32_t in_front = (1u << lane) - 1;
     const uint32_t equals = before[1] + __popc(eq & in_front);           // equal ones in front of this token
     const uint32_t at = first + before[0] + __popc(gt & in_front) + min(equals, need);

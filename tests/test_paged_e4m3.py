@@ -375,6 +375,30 @@ def test_evict_long(own_pages):
         assert torch.equal(x, y.cpu())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["plain", "odd", "equal", "narrow", "wide"])
+@pytest.mark.parametrize("lens,keep,recent,first", [([40000, 16385, 300], 9000, 100, 4), ([16300, 4000, 2048], 2000, 0, 0), ([140000, 20000], 15000, 64, 1),
+                                                    ([140000], 139998, 139990, 4)])
+def test_evict_of_weights_of_all_spreads(kind, lens, keep, recent, first):
+    """Weights that are all equal, that differ in their last bits only, or in all; against the host's path."""
+    p0 = filled(sum((n + 15) // 16 for n in lens), 16, 1, 64, 3, weights=True)
+    g = torch.Generator().manual_seed(8)
+    if kind in ("plain", "odd"):
+        weights_for(p0, 3, kind)
+    elif kind == "equal":
+        p0.weight.fill_(0.25)
+    elif kind == "narrow":
+        p0.weight.copy_(1.0 + torch.randint(0, 1500, p0.weight.shape, generator=g) * 2.0 ** -23)
+    else:                                                             # both signs, every exponent
+        p0.weight.copy_(torch.randint(-2 ** 31, 2 ** 31, p0.weight.shape, generator=g, dtype=torch.int64).to(I32).view(torch.float32))
+    t = tables_of(lens, 16, p0.k.shape[0], 3)
+    host, dev = to(p0, "cpu"), to(p0, "cuda")
+    a = ops.kv_evict_e4m3(host, t, ints(lens, "cpu"), keep, recent, first)
+    b = ops.kv_evict_e4m3(dev, t.cuda(), ints(lens, "cuda"), keep, recent, first)
+    assert all(torch.equal(x, y.cpu()) for x, y in zip(a, b))
+    assert torch.equal(host.k.view(torch.uint8), dev.k.cpu().view(torch.uint8)) and torch.equal(host.weight.view(I32), dev.weight.cpu().view(I32))
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_a_run_of_all(device):
     """A prompt in two portions, decoded tokens, eviction, more decoded tokens: state bit for bit, outputs within the bound."""
