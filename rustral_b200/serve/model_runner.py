@@ -548,7 +548,8 @@ class ModelRunner:
 
 
 def load_runner(model: str, device=None, dtype=None, num_blocks: int = 1024, block_size: int = 16, weights: str | None = None,
-                seed: int = 0, num_slots: int = 64, kv_quantization: CacheQuantization | None = None, **overrides) -> ModelRunner:
+                seed: int = 0, num_slots: int = 64, kv_quantization: CacheQuantization | None = None, kv_weights: bool = False,
+                **overrides) -> ModelRunner:
     """Runner of a preset name or of a model folder (config.json + model.safetensors, the model class chosen by the
     configuration); `weights` names another safetensors file.  Without weights: random initialisation."""
     from ..models.registry import load_tensors, resolve_config
@@ -557,4 +558,4 @@ def load_runner(model: str, device=None, dtype=None, num_blocks: int = 1024, blo
         device = "cuda" if torch.cuda.is_available() else "cpu"
     params = build_weights(cfg, device, dtype, load_tensors(model, weights), seed)
     return ModelRunner(cfg, params=params, device=device, num_blocks=num_blocks, block_size=block_size, seed=seed,
-                       num_slots=num_slots, kv_quantization=kv_quantization)
+                       num_slots=num_slots, kv_quantization=kv_quantization, kv_weights=kv_weights)

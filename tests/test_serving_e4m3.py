@@ -8,6 +8,7 @@ from rustral_b200.core.errors import InvalidArgument
 from rustral_b200.models.config import preset
 from rustral_b200.ops import paged_e4m3 as e4m3_ops
 from rustral_b200.serve import CacheQuantization, ModelRunner, PagedCache, ServingEngine
+from rustral_b200.serve.model_runner import load_runner
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 FP8 = CacheQuantization.FP8
@@ -220,3 +221,10 @@ def test_refusals():
     r = ModelRunner(preset("llama-test"), device="cpu", num_blocks=8)
     with pytest.raises(ValueError):
         r.decode([1], [1], [1], [0])                                  # positions without a cache in e4m3
+
+
+def test_a_loaded_runner_keeps_weights():
+    r = load_runner("llama-test", device="cpu", num_blocks=4, kv_quantization=FP8, kv_weights=True)
+    assert r.kv_weights and all(p.weight is not None for p in r.cache.pages)
+    with pytest.raises(InvalidArgument):
+        load_runner("llama-test", device="cpu", num_blocks=4, kv_weights=True)
