@@ -33,6 +33,7 @@ e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
   extern __shared__ uint32_t e4_keys[];
   __shared__ uint32_t hist[2048], part[2], ends[2], digit[3];
   __shared__ uint32_t warp_n[2][kE4SelectWarps];
+  __shared__ uint32_t warp_end[2][kE4SelectWarps];   // not warp_n: where all keys are equal, no barrier lies between its reads and the counts' writes
   const int ranks = CLUSTER ? gridDim.x : 1, rank = CLUSTER ? blockIdx.x : 0;
   const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int bs = a.pages.block_size, G = a.pages.kv_heads, per_page = bs >> 4;
@@ -101,12 +102,12 @@ e4_select_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
   least = __reduce_min_sync(0xffffffffu, least);
   most = __reduce_max_sync(0xffffffffu, most);
   if (lane == 0) {
-    warp_n[0][warp] = least;
-    warp_n[1][warp] = most;
+    warp_end[0][warp] = least;
+    warp_end[1][warp] = most;
   }
   __syncthreads();
-  least = __reduce_min_sync(0xffffffffu, warp_n[0][lane % kE4SelectWarps]);
-  most = __reduce_max_sync(0xffffffffu, warp_n[1][lane % kE4SelectWarps]);
+  least = __reduce_min_sync(0xffffffffu, warp_end[0][lane % kE4SelectWarps]);
+  most = __reduce_max_sync(0xffffffffu, warp_end[1][lane % kE4SelectWarps]);
   if (CLUSTER) {
     if (tid == 0) {
       ends[0] = least;
@@ -228,9 +229,21 @@ e4_move_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
   const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const int bs = a.pages.block_size, G = a.pages.kv_heads;
   const int n = a.lens_out[b];
-  if (INPLACE && static_cast<long long>(a.context_lens[b]) <= a.keep) return;           // a whole cluster
+  if (INPLACE && a.context_lens[b] <= a.keep) return;                  // a whole cluster
   const int* kept = a.kept + (static_cast<long long>(b) * G + h) * a.keep;
   const int* from = a.block_tables + static_cast<long long>(b) * a.max_blocks;
+  const int held = static_cast<int>(max(0ll, min(static_cast<long long>(a.context_lens[b]), static_cast<long long>(a.max_blocks) * bs)));
+  // The page that place t lies in.  A place that the sequence does not have counts as the first one, a page that is not there as page 0.
+  auto page_of = [&](int& t) {
+    if (t < 0 || t >= held) {
+      RB_BOUNDS_HIT(104);
+      t = 0;
+    }
+    const int page = from[t / bs];
+    if (page >= 0 && page < a.pages.num_blocks) return page;
+    RB_BOUNDS_HIT(104);
+    return 0;
+  };
   const int* to_tables = INPLACE ? a.block_tables : a.out_tables;
   const int to_blocks = INPLACE ? a.max_blocks : a.out_blocks;
   const int run = bs >= kE4MoveTokens ? bs : kE4MoveTokens / bs * bs;  // tokens of a CTA's run of pages
@@ -246,13 +259,9 @@ e4_move_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
       __syncthreads();
       float w = 0.f;
       if (tid < here) {
-        const int j = j0 + part + tid, t = kept[j];
-        int page = from[t / bs];
-        if (page < 0 || page >= a.pages.num_blocks) {
-          RB_BOUNDS_HIT(104);
-          page = 0;
-        }
-        const long long tile = static_cast<long long>(page) * G + h;
+        const int j = j0 + part + tid;
+        int t = kept[j];
+        const long long tile = static_cast<long long>(page_of(t)) * G + h;
         const int ek = a.pages.k_exp[tile], ev = a.pages.v_exp[tile];
         row_sh[tid] = tile * bs + t % bs;
         exp_sh[0][tid] = ek;
@@ -266,8 +275,8 @@ e4_move_kernel(const RbE4m3EvictArgs a RB_BOUNDS_PARAM) {
       }
       if (run > kE4MoveTokens && part == 0) {        // a page of many tokens: its exponents first
         for (int i = tid; i < m; i += kE4MoveThreads) {
-          const int page = from[kept[j0 + i] / bs];
-          const long long tile = static_cast<long long>(page < 0 || page >= a.pages.num_blocks ? 0 : page) * G + h;
+          int t = kept[j0 + i];
+          const long long tile = static_cast<long long>(page_of(t)) * G + h;
           top_k = max(top_k, static_cast<int>(a.pages.k_exp[tile]));
           top_v = max(top_v, static_cast<int>(a.pages.v_exp[tile]));
         }

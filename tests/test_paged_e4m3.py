@@ -683,3 +683,29 @@ def test_read_with_starts_that_do_not_ascend():
     # of rows 16 to 31, whose search begins with sequence 2: 16 to 19 lie in front of it, 20 is its first, 21 on are counted to sequence 4
     for x in out:
         assert bool((x[16:20] == 7.0).all()) and not bool((x[20] == 7.0).all())
+
+
+@pytest.mark.gpu
+def test_evict_right_after_a_prompt():
+    """Weights that are all zero, as appending leaves them: of short sequences most of a CTA's warps have no token and are done at once, and two CTAs
+    share an SM.  The earliest stay beside the last, call after call."""
+    G, D, bs, keep, recent = 8, 64, 16, 16, 5
+    lens = [17 + 3 * b % 190 for b in range(160)]
+    p = ops.PagesE4M3.zeros(sum((n + bs - 1) // bs for n in lens), bs, G, D, "cuda", weights=True)
+    t = tables_of(lens, bs, p.k.shape[0], 0).cuda()
+    k = torch.randn(sum(lens), G * D, generator=torch.Generator().manual_seed(0)).bfloat16().cuda()
+    ops.kv_append_e4m3(p, k, k, t, ints(lens, "cuda"), ints(starts_of(lens), "cuda"))
+    assert not bool(p.weight.any())
+    want = torch.tensor([[*range(keep - recent), *range(n - recent, n)] for n in lens], dtype=I32)[:, None].expand(-1, G, -1)
+    starts = ints([keep * b for b in range(len(lens) + 1)], "cuda")
+    rows = torch.cat([starts_of(lens)[b] + want[b, 0].long() for b in range(len(lens))])
+    host = ops.PagesE4M3.zeros(sum((n + bs - 1) // bs for n in lens), bs, G, D)
+    ops.kv_append_e4m3(host, k.cpu(), k.cpu(), t.cpu(), ints(lens, "cpu"), ints(starts_of(lens), "cpu"))
+    exact = ops.kv_read_e4m3(host, t.cpu(), ints(lens, "cpu"), ints(starts_of(lens), "cpu"), sum(lens), dtype=torch.float32)[0][rows]
+    for _ in range(50):
+        q = to(p, "cuda")
+        got, kept = ops.kv_evict_e4m3(q, t, ints(lens, "cuda"), keep, recent)
+        assert bool((got == keep).all()) and torch.equal(kept.cpu(), want)
+    # codes are rounded once to a larger exponent, that of numbers below 2^3, -5 at most: by half a step of a code, 2^-4 of it, or of a subnormal one, 2^-10 * 2^-5
+    back = ops.kv_read_e4m3(q, t, got, starts, keep * len(lens), dtype=torch.float32)[0].cpu()
+    assert bool(((back - exact).abs() <= exact.abs() * 2.0 ** -4 + 2.0 ** -15).all())
