@@ -2,9 +2,13 @@
 //
 // With key j's score s_j (base 2: scale, log2 e and the keys' exponent included) and the exponent e_j of its value's tile, the output is
 // sum_j 2^(s_j) 2^(e_j) c_j / sum_j 2^(s_j).  The maximum M that keeps the numbers in range is taken over s_j + e_j: the factors p_j = 2^(s_j + e_j - M)
-// of the codes are then at most 1 whatever the tiles' exponents, and the denominator is summed in fp32 from p_j 2^(-e_j).  M is rounded up to a whole
-// number, so that M - e_j and the factors that bring sums from one M to another are exact; with exponents of -100 a fractional M would cost the
-// scores seven bits.
+// of the codes are then at most 1 whatever the tiles' exponents.  M is rounded up to a whole number, so that M - e_j and the factors that bring sums from one M
+// to another are exact; with exponents of -100 a fractional M would cost the scores seven bits.
+//
+// The denominator has a maximum M' of its own, whole too: a factor p_j below 2^-126 is lost, which the numerator never misses, but the token behind it
+// may have the largest score of all, with values that are small or zero beside others' large ones.  The tiles of a warp in a slice seldom have exponents
+// far apart; if they are within 64 of the largest, E, the denominator is the sum of p_j 2^(E - e_j) under M' = M - E (a factor that is lost is then of a score
+// 2^-61 below the largest, or less), otherwise of 2^(s_j - M') with a second exponential, where every lane has the largest of its own scores as M'.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -27,8 +31,15 @@ __device__ __forceinline__ float e4_get(const __nv_bfloat16* p) { return __bfloa
 __device__ __forceinline__ float e4_get(const __half* p) { return __half2float(*p); }
 __device__ __forceinline__ void e4_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
 __device__ __forceinline__ void e4_put(__half* p, float v) { *p = __float2half(v); }
+template <typename T>
+__device__ __forceinline__ void e4_put4(T* p, const float4& x, float inv, const float2& size) {
+  e4_put(p, x.x * inv * size.x * size.y);
+  e4_put(p + 1, x.y * inv * size.x * size.y);
+  e4_put(p + 2, x.z * inv * size.x * size.y);
+  e4_put(p + 3, x.w * inv * size.x * size.y);
+}
 
-// Scratch: [batch, heads, slices, D + 4] fp32: maximum, denominator, two unused, sums of a slice; then, where weights are summed, the scores
+// Scratch: [batch, heads, slices, D + 4] fp32: maximum, denominator and its maximum, one unused, sums of a slice; then, where weights are summed, the scores
 // [batch, KV heads, slices * 256, heads of a group] and what makes weights of them [batch, heads, 2].
 __device__ __forceinline__ float* e4_partial(float* scratch, int heads, int slices, int D, int b, int h, int s) {
   return scratch + ((static_cast<long long>(b) * heads + h) * slices + s) * (D + 4);
@@ -95,10 +106,16 @@ struct E4Layout {
 enum { kE4Grid, kE4List, kE4Cluster };
 
 // The factor that brings sums under the maximum m to the maximum `to` >= m.  Maxima are whole, so it is an exact power of two, and a sum of such sums does
-// not depend on which maximum they are brought to on the way.
+// not depend on which maximum they are brought to on the way.  Zero where it would be below 2^-126 and where there is no maximum yet (-infinity).  A whole number that
+// 1.5 * 2^23 is added to stands in the last bits of the sum: its exponent bits come without a conversion.
 __device__ __forceinline__ float e4_factor(float m, float to) {
-  const float d = m == to ? 0.f : m - to;            // -infinity: no sum yet, or no maximum at all
-  return d < -126.f ? 0.f : e4_two(static_cast<int>(d));
+  return __int_as_float(__float_as_int(fmaxf(m - to, -127.f) + (12582912.f + 127.f)) << 23);
+}
+
+// What brings a sum under the maximum m, divided by a denominator under the maximum d, to its own size: 2^(m - d), in two steps that are in range.
+__device__ __forceinline__ float2 e4_size(float m, float d) {
+  const int e = static_cast<int>(fminf(fmaxf(m - d, -252.f), 252.f)), half = e >> 1;
+  return make_float2(e4_two(half), e4_two(e - half));
 }
 
 // A weight is 2^(s - m) / den = 2^(s - (m + x)) / (den / 2^x), with the x that brings den / 2^x into [1, 2): (m + x, 2^x / den).
@@ -122,8 +139,9 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
   constexpr int PF = std::is_same<T, __half>::value ? 2 : 1;             // operands that a factor makes
   extern __shared__ uint8_t e4_raw[];
   __shared__ __align__(8) uint64_t bars[kE4Warps][kE4Stages];
-  __shared__ float m_sh[kE4Warps][NH * 8], l_sh[kE4Warps][NH * 8];
-  __shared__ float2 ml_sh[NH * 8], norm_sh[NH * 8];
+  __shared__ float m_sh[kE4Warps][NH * 8], l_sh[kE4Warps][NH * 8], d_sh[kE4Warps][NH * 8];
+  __shared__ float4 mld_sh[NH * 8];                  // maximum, denominator, its maximum
+  __shared__ float2 norm_sh[NH * 8];
   __shared__ int abort_sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
   const uint32_t base = (smem_u32(e4_raw) + 1023u) & ~1023u;             // the swizzle goes by addresses
@@ -282,10 +300,14 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
         }
       }
     }
-    float m[NH][2], l[NH][2], o[MT][NH][4];          // of heads r * 8 + 2 tq and + 1; l: this lane's tokens
+    // the exponents of this warp's values: the largest, and whether they are far apart
+    const bool counts = lane >= 4 && lane < 8 && at.s * kE4Slice + tile_in * 16 < n_at;
+    const int e_top = __reduce_max_sync(0xffffffffu, counts ? exps : -128);
+    const bool far = e_top - __reduce_min_sync(0xffffffffu, counts ? exps : 127) > 64;
+    float m[NH][2], l[NH][2], dm[NH][2], o[MT][NH][4];   // of heads r * 8 + 2 tq and + 1; l: this lane's tokens, dm (far): the largest score of them
 #pragma unroll
     for (int r = 0; r < NH; ++r) {
-      m[r][0] = m[r][1] = -INFINITY;
+      m[r][0] = m[r][1] = dm[r][0] = dm[r][1] = -INFINITY;
       l[r][0] = l[r][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[i][r][0] = o[i][r][1] = o[i][r][2] = o[i][r][3] = 0.f;
@@ -407,11 +429,24 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
           grow[r][j] = e4_factor(m[r][j], to[j]);
           moved |= to[j] != m[r][j];
           m[r][j] = to[j];
-          l[r][j] *= grow[r][j];
+        }
+        if (far) {                                     // this lane's scores are its own
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float top = fmaxf(dm[r][j], ceilf(fmaxf(fmaxf(s[0][r][j], s[0][r][2 + j]), fmaxf(s[1][r][j], s[1][r][2 + j]))));
+            const float under = top == -INFINITY ? 0.f : top;            // no token yet
+            l[r][j] *= e4_factor(dm[r][j], top);
+            l[r][j] += e4_ex2(s[0][r][j] - under) + e4_ex2(s[0][r][2 + j] - under);
+            l[r][j] += e4_ex2(s[1][r][j] - under) + e4_ex2(s[1][r][2 + j] - under);
+            dm[r][j] = top;
+          }
+        } else {
+          l[r][0] *= grow[r][0];
+          l[r][1] *= grow[r][1];
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float e = static_cast<float>(ev[u]), down = e4_two(-ev[u]);
+          const float e = static_cast<float>(ev[u]), down = far ? 0.f : e4_two(e_top - ev[u]);
           float p[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) p[j] = e4_ex2(s[u][r][j] - (to[j & 1] - e));
@@ -473,11 +508,19 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
     for (int r = 0; r < NH; ++r) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
+        float top = m[r][j] - static_cast<float>(e_top);
+        if (far) {
+          top = dm[r][j];
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+          l[r][j] *= e4_factor(dm[r][j], top);
+        }
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[r][j] += __shfl_xor_sync(0xffffffffu, l[r][j], x);
         if (gq == 0) {
           m_sh[warp][r * 8 + tq * 2 + j] = m[r][j];
           l_sh[warp][r * 8 + tq * 2 + j] = l[r][j];
+          d_sh[warp][r * 8 + tq * 2 + j] = top;
         }
       }
     }
@@ -503,15 +546,18 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
       __syncthreads();
       for (int i = threadIdx.x; i < rows * (D / 4); i += kE4Warps * 32) {
         const int head = hb + i / (D / 4), d = i % (D / 4);
-        float top = m_sh[0][head];
+        float top = m_sh[0][head], dtop = d_sh[0][head];
 #pragma unroll
-        for (int w = 1; w < kE4Warps; ++w) top = fmaxf(top, m_sh[w][head]);
+        for (int w = 1; w < kE4Warps; ++w) {
+          top = fmaxf(top, m_sh[w][head]);
+          dtop = fmaxf(dtop, d_sh[w][head]);
+        }
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
         float den = 0.f;
 #pragma unroll
         for (int w = 0; w < kE4Warps; ++w) {
-          const float mw = m_sh[w][head], f = mw == -INFINITY ? 0.f : e4_factor(mw, top);
-          den = fmaf(l_sh[w][head], f, den);
+          const float f = e4_factor(m_sh[w][head], top);
+          den = fmaf(l_sh[w][head], e4_factor(d_sh[w][head], dtop), den);
           const float4 x = *reinterpret_cast<const float4*>(merge + (w * rows + head - hb) * D + ((d ^ (head >> 1 & 3)) << 2));
           sum.x = fmaf(x.x, f, sum.x);
           sum.y = fmaf(x.y, f, sum.y);
@@ -520,21 +566,16 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
         }
         if (CLUSTER) {                                 // where this thread read the first warp's
           *reinterpret_cast<float4*>(merge + head * D + ((d ^ (head >> 1 & 3)) << 2)) = sum;
-          if (d == 0) ml_sh[head] = make_float2(top, den);
+          if (d == 0) mld_sh[head] = make_float4(top, den, dtop, 0.f);
           continue;
         }
         const int h = at.hk * group + h0 + head;
         if (whole) {
-          const float inv = 1.f / den;
-          T* out = reinterpret_cast<T*>(a.out) + at.b * a.ld_o + static_cast<long long>(h) * D + d * 4;
-          e4_put(out, sum.x * inv);
-          e4_put(out + 1, sum.y * inv);
-          e4_put(out + 2, sum.z * inv);
-          e4_put(out + 3, sum.w * inv);
+          e4_put4(reinterpret_cast<T*>(a.out) + at.b * a.ld_o + static_cast<long long>(h) * D + d * 4, sum, 1.f / den, e4_size(top, dtop));
         }
         if (!whole || a.accumulate) {                  // the weights' denominators come from here too
           float* out = e4_partial(a.scratch, a.heads, slices, D, at.b, h, at.s);
-          if (d == 0) *reinterpret_cast<float2*>(out) = make_float2(top, den);
+          if (d == 0) *reinterpret_cast<float4*>(out) = make_float4(top, den, dtop, 0.f);
           *reinterpret_cast<float4*>(out + 4 + d * 4) = sum;
         }
       }
@@ -546,46 +587,42 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
       else __syncthreads();
       for (int i = threadIdx.x + blockIdx.x * (kE4Warps * 32); i < heads * (D / 4); i += ranks * (kE4Warps * 32)) {
         const int head = i / (D / 4), d = i % (D / 4), at_sh = head * D + ((d ^ (head >> 1 & 3)) << 2);
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f), x[8];
-        float2 ml[8];
-        float top = -INFINITY, den = 0.f;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f), x[8], mld[8];
+        float top = -INFINITY, dtop = -INFINITY, den = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           if (k < here) {
-            ml[k] = *all.map_shared_rank(&ml_sh[head], k);
+            mld[k] = *all.map_shared_rank(&mld_sh[head], k);
             x[k] = *reinterpret_cast<const float4*>(all.map_shared_rank(merge + at_sh, k));
-            top = fmaxf(top, ml[k].x);
+            top = fmaxf(top, mld[k].x);
+            dtop = fmaxf(dtop, mld[k].z);
           }
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           if (k < here) {
-            const float f = e4_factor(ml[k].x, top);
+            const float f = e4_factor(mld[k].x, top);
             sum.x = fmaf(x[k].x, f, sum.x);
             sum.y = fmaf(x[k].y, f, sum.y);
             sum.z = fmaf(x[k].z, f, sum.z);
             sum.w = fmaf(x[k].w, f, sum.w);
-            den = fmaf(ml[k].y, f, den);
+            den = fmaf(mld[k].y, e4_factor(mld[k].z, dtop), den);
           }
         const float inv = here > 0 ? 1.f / den : 0.f;                    // without tokens the sums are zero
-        T* out = reinterpret_cast<T*>(a.out) + at.b * a.ld_o + (static_cast<long long>(at.hk) * group + h0 + head) * D + d * 4;
-        e4_put(out, sum.x * inv);
-        e4_put(out + 1, sum.y * inv);
-        e4_put(out + 2, sum.z * inv);
-        e4_put(out + 3, sum.w * inv);
+        e4_put4(reinterpret_cast<T*>(a.out) + at.b * a.ld_o + (static_cast<long long>(at.hk) * group + h0 + head) * D + d * 4, sum, inv, e4_size(top, dtop));
       }
       if (a.accumulate) {
         if (static_cast<int>(threadIdx.x) < heads) {
-          float2 ml[8];
+          float4 mld[8];
           float top = -INFINITY, den = 0.f;
 #pragma unroll
           for (int k = 0; k < 8; ++k)
             if (k < here) {
-              ml[k] = *all.map_shared_rank(&ml_sh[threadIdx.x], k);
-              top = fmaxf(top, ml[k].x);
+              mld[k] = *all.map_shared_rank(&mld_sh[threadIdx.x], k);
+              top = fmaxf(top, mld[k].z);
             }
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            if (k < here) den = fmaf(ml[k].y, e4_factor(ml[k].x, top), den);
+            if (k < here) den = fmaf(mld[k].y, e4_factor(mld[k].z, top), den);
           norm_sh[threadIdx.x] = e4_norm_of(top, den);
         }
         __syncthreads();
@@ -629,7 +666,7 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
   pdl_launch();
   constexpr int kChains = MANY ? 64 : 16, R = (MANY ? 512 : 128) / COLS, PER = kChains / R;
   __shared__ float4 sum_sh[kChains][COLS];
-  __shared__ float2 ml_sh[kChains];
+  __shared__ float4 mld_sh[kChains];                 // maximum, denominator, its maximum
   const int h = blockIdx.x, b = blockIdx.y, z = blockIdx.z, tid = threadIdx.x, D = a.pages.head_dim, c = tid % COLS, r = tid / COLS;
   T* out = reinterpret_cast<T*>(a.out) + b * a.ld_o + static_cast<long long>(h) * D + z * (COLS * 4);
   const int here = (e4_len(a, b) + kE4Slice - 1) / kE4Slice;
@@ -641,84 +678,96 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
   const int chains = MANY && here <= 64 ? 16 : kChains;
   const float* first = e4_partial(a.scratch, a.heads, slices, D, b, h, 0);
   const long long pitch = D + 4;
-  // every sum beside its own maximum; a new maximum's factor is a power of two, so that the sums are those under the largest of all
-  float4 sum[PER];
-  float m[PER], l[PER];
-#pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    sum[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    m[k] = -INFINITY;
-    l[k] = 0.f;
-  }
+  // Every sum beside its own maximum; a new maximum's factor is a power of two, so that the sums are those under the largest of all.  The maxima and
+  // denominators of a chain, the same for all its columns, are looked after by one lane for each slice that is loaded together, and factors come from there.
   constexpr int kAhead = PER == 1 ? 8 : 1;           // slices of a chain that are loaded together
+  constexpr int kHeads = PER * kAhead;
+  static_assert(kHeads <= COLS, "a lane for every slice");
+  const uint32_t group = COLS == 32 ? 0xffffffffu : ((1u << COLS) - 1) << (tid & 31 & ~(COLS - 1));
+  const int ck = c / kAhead, ci = c % kAhead;
+  float4 sum[PER];
+  float m = -INFINITY, l = 0.f, dm = -INFINITY;      // of chain r + ck * R
+#pragma unroll
+  for (int k = 0; k < PER; ++k) sum[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s0 = r; s0 < here && (!MANY || r < chains); s0 += chains * kAhead) {
-    float4 x[PER][kAhead];
-    float2 ml[PER][kAhead];
+    float4 x[PER][kAhead], mld = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+    if (c < kHeads && s0 + ck * R + ci * chains < here) mld = *reinterpret_cast<const float4*>(first + (s0 + ck * R + ci * chains) * pitch);
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int s = s0 + k * R + i * chains;
-        ml[k][i] = make_float2(-INFINITY, 0.f);
         x[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (s < here) {
-          const float* p = first + s * pitch;
-          ml[k][i] = *reinterpret_cast<const float2*>(p);
-          x[k][i] = *reinterpret_cast<const float4*>(p + 4 + (z * COLS + c) * 4);
-        }
+        if (s < here) x[k][i] = *reinterpret_cast<const float4*>(first + s * pitch + 4 + (z * COLS + c) * 4);
       }
     }
+    float to = mld.x, dto = mld.z;
+#pragma unroll
+    for (int o = 1; o < kAhead; o <<= 1) {
+      to = fmaxf(to, __shfl_xor_sync(group, to, o, COLS));
+      dto = fmaxf(dto, __shfl_xor_sync(group, dto, o, COLS));
+    }
+    to = fmaxf(to, m);
+    dto = fmaxf(dto, dm);
+    const float f = e4_factor(m, to), g = e4_factor(mld.x, to), den = mld.y * e4_factor(mld.z, dto);
+    l *= e4_factor(dm, dto);
+    if (kAhead == 1) l += den;
+    else
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) l += __shfl_sync(group, den, i, COLS);
+    m = to;
+    dm = dto;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      float to = m[k];
+      const float fk = __shfl_sync(group, f, k * kAhead, COLS);
+      sum[k].x *= fk; sum[k].y *= fk; sum[k].z *= fk; sum[k].w *= fk;
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) to = fmaxf(to, ml[k][i].x);
-      const float f = e4_factor(m[k], to);
-      sum[k].x *= f; sum[k].y *= f; sum[k].z *= f; sum[k].w *= f;
-      l[k] *= f;
-      m[k] = to;
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        if (s0 + k * R + i * chains >= here) break;
-        const float g = e4_factor(ml[k][i].x, to);
-        sum[k].x = fmaf(x[k][i].x, g, sum[k].x);
-        sum[k].y = fmaf(x[k][i].y, g, sum[k].y);
-        sum[k].z = fmaf(x[k][i].z, g, sum[k].z);
-        sum[k].w = fmaf(x[k][i].w, g, sum[k].w);
-        l[k] = fmaf(ml[k][i].y, g, l[k]);
+      for (int i = 0; i < kAhead; ++i) {             // of a slice that is not there: zero
+        const float gk = __shfl_sync(group, g, k * kAhead + i, COLS);
+        sum[k].x = fmaf(x[k][i].x, gk, sum[k].x);
+        sum[k].y = fmaf(x[k][i].y, gk, sum[k].y);
+        sum[k].z = fmaf(x[k][i].z, gk, sum[k].z);
+        sum[k].w = fmaf(x[k][i].w, gk, sum[k].w);
       }
     }
   }
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    sum_sh[r + k * R][c] = sum[k];
-    if (c == 0) ml_sh[r + k * R] = make_float2(m[k], l[k]);
-  }
+  for (int k = 0; k < PER; ++k) sum_sh[r + k * R][c] = sum[k];
+  if (c < kHeads && ci == 0) mld_sh[r + ck * R] = make_float4(m, l, dm, 0.f);
   __syncthreads();
-  if (tid >= COLS) return;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  float top = -INFINITY, den = 0.f;
+  if (tid >= 32) return;
+  // a lane forms the factors of its chains, so that no thread holds those of all
+  constexpr int kMine = (kChains + 31) / 32;
+  float4 mld[kMine];
+  float f[kMine], lf[kMine], top = -INFINITY, dtop = -INFINITY, den = 0.f;
 #pragma unroll
-  for (int k = 0; k < kChains; ++k) top = fmaxf(top, ml_sh[k].x);      // -infinity where there is no such slice
-#pragma unroll 16
-  for (int k = 0; k < kChains; ++k)
-    if (k < here && k < chains) {
-      const float f = e4_factor(ml_sh[k].x, top);
-      const float4 x = sum_sh[k][c];
-      o.x = fmaf(x.x, f, o.x);
-      o.y = fmaf(x.y, f, o.y);
-      o.z = fmaf(x.z, f, o.z);
-      o.w = fmaf(x.w, f, o.w);
-      den = fmaf(ml_sh[k].y, f, den);
-    }
-  if (here > 1) {
-    const float inv = 1.f / den;
-    e4_put(out + c * 4, o.x * inv);
-    e4_put(out + c * 4 + 1, o.y * inv);
-    e4_put(out + c * 4 + 2, o.z * inv);
-    e4_put(out + c * 4 + 3, o.w * inv);
+  for (int i = 0; i < kMine; ++i) {                  // -infinity where there is no such slice
+    mld[i] = tid + 32 * i < kChains ? mld_sh[tid + 32 * i] : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+    top = fmaxf(top, mld[i].x);
+    dtop = fmaxf(dtop, mld[i].z);
   }
-  if (a.accumulate && tid == 0 && z == 0) *e4_norm(a, slices, b, h) = e4_norm_of(top, den);
+  top = warp_max(top);
+  dtop = warp_max(dtop);
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    f[i] = e4_factor(mld[i].x, top);
+    lf[i] = mld[i].y * e4_factor(mld[i].z, dtop);
+  }
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 16
+  for (int k = 0; k < kChains; ++k) {
+    const float fk = __shfl_sync(0xffffffffu, f[MANY ? k >> 5 : 0], k & 31), lk = __shfl_sync(0xffffffffu, lf[MANY ? k >> 5 : 0], k & 31);
+    if (k < here && k < chains) {
+      const float4 x = sum_sh[k][c];
+      o.x = fmaf(x.x, fk, o.x);
+      o.y = fmaf(x.y, fk, o.y);
+      o.z = fmaf(x.z, fk, o.z);
+      o.w = fmaf(x.w, fk, o.w);
+      den += lk;
+    }
+  }
+  if (here > 1 && tid < COLS) e4_put4(out + c * 4, o, 1.f / den, e4_size(top, dtop));
+  if (a.accumulate && tid == 0 && z == 0) *e4_norm(a, slices, b, h) = e4_norm_of(dtop, den);
 }
 
 // Adds the attention weights of a slice to its tokens' sums, a thread a token.  (As a part of the merge, with denominators formed in every CTA, it was

@@ -709,3 +709,39 @@ def test_evict_right_after_a_prompt():
     # codes are rounded once to a larger exponent, that of numbers below 2^3, -5 at most: by half a step of a code, 2^-4 of it, or of a subnormal one, 2^-10 * 2^-5
     back = ops.kv_read_e4m3(q, t, got, starts, keep * len(lens), dtype=torch.float32)[0].cpu()
     assert bool(((back - exact).abs() <= exact.abs() * 2.0 ** -4 + 2.0 ** -15).all())
+
+
+# one sequence in a cluster; several slices and a merge; tables with room for more than 64 slices
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens,width", [([1, 16, 40, 300], 0), ([520] * 30 + [1, 17], 0), ([1, 300, 5000], 1200)])
+@pytest.mark.parametrize("group,D", [(4, 128), (12, 64)])
+@pytest.mark.parametrize("lean", [0.0, 330.0, -330.0, 2600.0, -2600.0])
+def test_attention_over_pages_at_both_ends_of_the_exponents(device, lens, width, group, D, lean):
+    """Pages of zeros (exponent -100) beside pages of exponent 119.  `lean`: the scores of the former lie lean / 32 above those of the latter (up to 81, 117 powers
+    of two), so that they have nearly all of the denominator, half or nearly nothing, and the latter nearly all of the sums."""
+    G, bs = 2, 16
+    p0 = filled(sum((n + bs - 1) // bs for n in lens) + 2, bs, G, D, 12, weights=True)
+    zeros = torch.arange(p0.k.shape[0]) % 3 == 0
+    zeros[tables_of(lens, bs, p0.k.shape[0], 13, width)[:, 0].long()] = False           # every sequence has a page of either kind where it has two
+    p0.k_exp.fill_(-6)
+    p0.v_exp.fill_(119)
+    p0.v_exp[zeros] = -100
+    p0.v.view(torch.uint8)[zeros] = 0
+    # dimension 0: code 64 for pages of zeros and -64 for the others, under an exponent of -6, times lean / 8 in the query
+    p0.k.view(torch.uint8)[..., 0] = torch.where(zeros, 0x68, 0xe8).to(torch.uint8)[:, None, None]
+    t = tables_of(lens, bs, p0.k.shape[0], 13, width)
+    q = torch.randn(len(lens), G * group, D, generator=torch.Generator().manual_seed(3))
+    q[..., 0] = lean / 8
+    q = q.view(len(lens), -1).bfloat16()
+    want, err, ws, wrel = Cache(p0).attend(q, t, lens, 0.125)
+    p = to(p0, device)
+    out = ops.paged_attention_decode_e4m3(q.to(device), p, t.to(device), ints(lens, device), 0.125, accumulate=True).cpu().double()
+    off, most = (out - want).abs(), err + want.abs() * 2.0 ** -8
+    assert bool((off <= most).all()), f"worst {float((off / most).max())} of the bound"
+    for b, n in enumerate(lens):
+        at = torch.arange(n)
+        pages = t[b, at // bs].long()
+        was, got = p0.weight[pages, :, at % bs].double(), p.weight.cpu()[pages, :, at % bs].double()
+        most = (was + ws[b]) * 2.0 ** -23 + ws[b] * (wrel[b] + group * 2.0 ** -23)
+        assert bool(((got - was - ws[b]).abs() <= most).all())
+        assert abs(float((got - was).sum()) - G * group) <= n * G * 2.0 ** -23 * 2 + G * group * wrel[b]
