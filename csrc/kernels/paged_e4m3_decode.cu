@@ -2,8 +2,10 @@
 //
 // With key j's score s_j (base 2: scale, log2 e and the keys' exponent included) and the exponent e_j of its value's tile, the output is
 // sum_j 2^(s_j) 2^(e_j) c_j / sum_j 2^(s_j).  The maximum M that keeps the numbers in range is taken over s_j + e_j: the factors p_j = 2^(s_j + e_j - M)
-// of the codes are then at most 1 whatever the tiles' exponents.  M is rounded up to a whole number, so that M - e_j and the factors that bring sums from one M
-// to another are exact; with exponents of -100 a fractional M would cost the scores seven bits.
+// of the codes are then at most 2^15 whatever the tiles' exponents.  M lies 15 below the largest: an f16 ends at 2^16 and has all its bits down to 2^-14, so with
+// factors up to 1 those below 2^-25 would be lost, of which a long context beside a token with nearly all the weight has many.  M is rounded up to a
+// whole number, so that M - e_j and the factors that bring sums from one M to another are exact; with exponents of -100 a fractional M would cost the scores
+// seven bits.
 //
 // The denominator has a maximum M' of its own, whole too: a factor p_j below 2^-126 is lost, which the numerator never misses, but the token behind it
 // may have the largest score of all, with values that are small or zero beside others' large ones.  The tiles of a warp in a slice seldom have exponents
@@ -20,6 +22,7 @@ namespace rb {
 
 namespace cg = cooperative_groups;
 
+constexpr int kE4Room = 15;                          // factors of codes reach 2^15
 constexpr int kE4Slice = 256;                        // tokens whose sums one CTA forms; the merge goes over them in order
 
 __device__ __forceinline__ float e4_ex2(float x) {
@@ -98,8 +101,9 @@ struct E4Layout {
 // rows and the heads as columns, so that no row is left empty and a lane's factors are those of its own columns; P^T, rounded to f16, takes its place as
 // the second operand by a transposition of 8 x 8 (movmatrix).  Codes become f16 exactly.  The contraction over head dimensions may take them in any
 // order, so a lane reads 16 codes of a row at a time and these are its operands of four products; a swizzled tile gives every lane its 16 bytes without
-// bank conflicts.  A query row is scaled to [1, 2) by a power of two first.  Rounding a factor p_j to f16 is off by 2^-12 of it, which the output's
-// rounding to bf16 (2^-9) hides; an output in f16 would show it, and there what the rounding left is a second operand.
+// bank conflicts.  A query row is scaled to [1, 2) by a power of two first.  Rounding a factor p_j to f16 is off by at most 2^-11 of it, or by 2^-25 where it is
+// below 2^-14 (2^-39 of the largest, which is 2^15 or, where M was rounded up, down to half of that).  2^-11 of an output is an eighth of what rounding it to bf16
+// may take, 2^-8; an output in f16, which loses 2^-11 itself, would show it, and there what the rounding left of a factor is a second operand.
 // HOW: kE4List: the slices of all sequences and KV heads, numbered one sequence after the other, are dealt in equal runs to CTAs that stay, and the next
 // slice's tiles are copied while this one's are worked on.  Otherwise the grid is (slices, KV heads, sequences); kE4Cluster: the CTAs of a sequence and KV
 // head are a cluster and merge their sums, and add the weights, through distributed shared memory.
@@ -419,7 +423,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
             }
           }
 #pragma unroll
-          for (int j = 0; j < 2; ++j) to[j] = fmaxf(to[j], ceilf(fmaxf(s[u][r][j], s[u][r][2 + j])) + static_cast<float>(ev[u]));
+          for (int j = 0; j < 2; ++j) to[j] = fmaxf(to[j], ceilf(fmaxf(s[u][r][j], s[u][r][2 + j])) + static_cast<float>(ev[u] - kE4Room));
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {

@@ -745,3 +745,31 @@ def test_attention_over_pages_at_both_ends_of_the_exponents(device, lens, width,
         most = (was + ws[b]) * 2.0 ** -23 + ws[b] * (wrel[b] + group * 2.0 ** -23)
         assert bool(((got - was - ws[b]).abs() <= most).all())
         assert abs(float((got - was).sum()) - G * group) <= n * G * 2.0 ** -23 * 2 + G * group * wrel[b]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens", [[300], [17, 2000], [9000, 700]])
+@pytest.mark.parametrize("group,D,dtype", [(4, 128, torch.bfloat16), (1, 64, torch.float16), (12, 64, torch.bfloat16)])
+def test_attention_beside_one_token_with_nearly_all_the_weight(device, lens, group, D, dtype):
+    """The first token has nearly all the weight and a value of zero, so that the output is what the others add, each with 2^-27 of its weight."""
+    G, bs = 2, 16
+    p0 = filled(sum((n + bs - 1) // bs for n in lens), bs, G, D, 14, spread=0)
+    t = tables_of(lens, bs, p0.k.shape[0], 14)
+    p0.k_exp.fill_(-6)
+    p0.k.view(torch.uint8)[..., 0] = 0xe8                             # -64: -1 with the exponent
+    p0.v.view(torch.uint8).bitwise_and_(0x7f)                         # values without signs: no sum is smaller than its terms
+    for b in range(len(lens)):
+        p0.k.view(torch.uint8)[int(t[b, 0]), :, 0, 0] = 0x68
+        p0.v.view(torch.uint8)[int(t[b, 0]), :, 0] = 0
+    q = torch.zeros(len(lens), G * group, D)
+    q[..., 0] = 75.0                                                  # scores 150 / 8 apart, 27.05 powers of two
+    q = q.view(len(lens), -1).to(dtype)
+    want, _, _, _ = Cache(p0).attend(q, t, lens, 0.125)
+    out = ops.paged_attention_decode_e4m3(q.to(device), to(p0, device), t.to(device), ints(lens, device), 0.125).cpu().double()
+    # factors: half a step of an f16, 2^-11, or 2^-39 of the largest; scores of 9.4 in 32 bits (twice, 2^-24 each) and two exponentials, below 2^-17 together;
+    # the output's own rounding, half a step
+    largest = float(p0.v.float().max()) * 2.0 ** int(p0.v_exp.max())
+    f = torch.finfo(dtype)
+    most = want * (2.0 ** -11 + 2.0 ** -17 + f.eps / 2) + max(lens) * 2.0 ** -39 * largest + f.smallest_normal * f.eps / 2
+    off = (out - want).abs()
+    assert bool((off <= most).all()), f"worst {float((off / most).max())} of the bound"
