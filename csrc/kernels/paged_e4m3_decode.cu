@@ -116,6 +116,14 @@ __device__ __forceinline__ float e4_factor(float m, float to) {
   return __int_as_float(__float_as_int(fmaxf(m - to, -127.f) + (12582912.f + 127.f)) << 23);
 }
 
+// A score from a sum of products of keys' codes and a scaled query, where it may leave the range of 32 bits.  The factor stays finite, so that a sum of zero is
+// a score of zero; a score below the range is the least number, so that a tile of such scores has a maximum.
+__device__ __forceinline__ float e4_far_score(float sum, float factor) {
+  factor = factor > 3.4028235e38f ? 3.4028235e38f : factor < -3.4028235e38f ? -3.4028235e38f : factor;
+  const float s = sum * factor;
+  return s == -INFINITY ? -3.4028235e38f : s;
+}
+
 // What brings a sum under the maximum m, divided by a denominator under the maximum d, to its own size: 2^(m - d), in two steps that are in range.
 __device__ __forceinline__ float2 e4_size(float m, float d) {
   const int e = static_cast<int>(fminf(fmaxf(m - d, -252.f), 252.f)), half = e >> 1;
@@ -269,9 +277,11 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
   const bool q_whole = !((reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.ld_q * 2)) & 15);
   uint32_t qf[KS][NH][2];                            // head r * 8 + gq, this lane's dimensions of it
   float q_up[NH][2];                                 // heads r * 8 + 2 tq and + 1: what a product with their rows is to be multiplied with
+  int q_top = 0;                                     // the largest one's exponent
   uint32_t parity = 0;
   for (bool fresh = true;;) {
     if (fresh) {
+      q_top = -127;
 #pragma unroll
       for (int r = 0; r < NH; ++r) {
         const bool there = r * 8 + gq < heads;
@@ -295,6 +305,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -126), 126);
         const float down = e4_two(-e), up = e4_two(e) * a.scale * 1.4426950408889634f;
+        q_top = max(q_top, static_cast<int>(__float_as_uint(up) >> 23 & 255) - 127);
         q_up[r][0] = __shfl_sync(0xffffffffu, up, tq * 8);
         q_up[r][1] = __shfl_sync(0xffffffffu, up, tq * 8 + 4);
 #pragma unroll
@@ -303,11 +314,14 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
           qf[j][r][1] = e4_half2_of(x[4 * j + 2] * down, x[4 * j + 3] * down);
         }
       }
+      q_top = __reduce_max_sync(0xffffffffu, q_top);
     }
     // the exponents of this warp's values: the largest, and whether they are far apart
-    const bool counts = lane >= 4 && lane < 8 && at.s * kE4Slice + tile_in * 16 < n_at;
-    const int e_top = __reduce_max_sync(0xffffffffu, counts ? exps : -128);
-    const bool far = e_top - __reduce_min_sync(0xffffffffu, counts ? exps : 127) > 64;
+    const bool there = lane < 8 && at.s * kE4Slice + tile_in * 16 < n_at, values = there && lane >= 4;
+    const int e_top = __reduce_max_sync(0xffffffffu, values ? exps : -128);
+    const bool far = e_top - __reduce_min_sync(0xffffffffu, values ? exps : 127) > 64;
+    // whether a score may leave the range: a sum is below 2 * 448 * 128 < 2^17, the query's factor below 2^(q_top + 1)
+    const bool wide = __reduce_max_sync(0xffffffffu, there && lane < 4 ? exps : -128) + q_top + 18 > 127;
     float m[NH][2], l[NH][2], dm[NH][2], o[MT][NH][4];   // of heads r * 8 + 2 tq and + 1; l: this lane's tokens, dm (far): the largest score of them
 #pragma unroll
     for (int r = 0; r < NH; ++r) {
@@ -403,12 +417,18 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
       bool moved = false;
 #pragma unroll
       for (int r = 0; r < NH; ++r) {
+        if (wide) {
+#pragma unroll
+          for (int x = 0; x < 8; ++x) s[x >> 2][r][x & 3] = e4_far_score(s[x >> 2][r][x & 3], up[x >> 2] * q_up[r][x & 1]);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 8; ++x) s[x >> 2][r][x & 3] *= up[x >> 2] * q_up[r][x & 1];
+        }
         float to[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            s[u][r][j] *= up[u] * q_up[r][j & 1];
             if (n_tok[u] < 16 && gq + (j >> 1) * 8 >= n_tok[u]) s[u][r][j] = -INFINITY;
           }
           if (a.accumulate) {                        // [batch, KV heads, tokens, heads of a group]

@@ -773,3 +773,45 @@ def test_attention_beside_one_token_with_nearly_all_the_weight(device, lens, gro
     most = want * (2.0 ** -11 + 2.0 ** -17 + f.eps / 2) + max(lens) * 2.0 ** -39 * largest + f.smallest_normal * f.eps / 2
     off = (out - want).abs()
     assert bool((off <= most).all()), f"worst {float((off / most).max())} of the bound"
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens,width", [([40, 300], 0), ([520] * 30 + [1, 17], 0)])
+@pytest.mark.parametrize("group,D,dtype", [(4, 128, torch.bfloat16), (12, 64, torch.float16)])
+@pytest.mark.parametrize("first", [0.0, -64.0])
+def test_attention_of_scores_past_the_range(device, lens, width, group, D, dtype, first):
+    """Keys of 2^125 in dimension 0 of some tokens, alone in their pages.  A query without that dimension has scores of zero with them, one with -64 there scores of
+    -2^131 / 8, below what 32 bits have: no weight."""
+    G, bs = 2, 16
+    p0 = filled(sum((n + bs - 1) // bs for n in lens), bs, G, D, 15, weights=True, spread=2)
+    t = tables_of(lens, bs, p0.k.shape[0], 15, width)
+    g = torch.Generator().manual_seed(4)
+    for b, n in enumerate(lens):
+        for i in range(1, (n + bs - 1) // bs, 2):                     # two of a warp's tiles in a row too
+            page = int(t[b, i])
+            p0.k.view(torch.uint8)[page] = 0
+            p0.k.view(torch.uint8)[page, ..., 0] = 0x68               # 64 under 2^119
+            p0.k_exp[page] = 119
+    q = torch.randn(len(lens), G * group, D, generator=g)
+    q[..., 0] = first
+    q[..., 1] = 2.0 ** 13                                             # 2^119 times the query's power of two is past the range; keys are zero there
+    p0.k.view(torch.uint8)[..., 1] = 0
+    q = q.view(len(lens), -1).to(dtype)
+    want, err, ws, wrel = Cache(p0).attend(q, t, lens, 0.125)
+    p = to(p0, device)
+    out = ops.paged_attention_decode_e4m3(q.to(device), p, t.to(device), ints(lens, device), 0.125, accumulate=True).cpu().double()
+    assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(p.weight).all())
+    # The oracle's bound goes by the largest key and says nothing here.  A query's numbers lie 2^-13 below its largest, in f16 off by 2^-25 of that at most; D products are
+    # summed in 32 bits; a weight is off by twice what its score is (its own and the largest's); factors by 2^-11 or 2^-39 of the largest, exponentials by 2^-17.
+    most = torch.zeros(len(lens))
+    for b, n in enumerate(lens):
+        k, v = (Cache(p0).tokens(x, t, b, n).abs() for x in "kv")
+        k = torch.where(k > 1e30, 0.0, k)
+        scores = 0.125 * (k.sum(-1).max() * 2.0 ** -12 + (q[b].double().view(G, group, 1, D).abs() * k.transpose(0, 1)[:, None]).sum(-1).max() * (D + 4) * 2.0 ** -24)
+        most[b] = (torch.expm1(2 * scores) + 2.0 ** -11 + 2.0 ** -17 + n * 2.0 ** -39) * v.max()
+    assert bool(((out - want).abs() <= want.abs() * torch.finfo(dtype).eps / 2 + most[:, None] + 2.0 ** -24).all())
+    grown = (p.weight.cpu() - p0.weight).double()
+    assert abs(float(grown.sum()) - len(lens) * G * group) < 1e-2
+    if first:
+        gone = torch.cat([t[b, 1:(n + bs - 1) // bs:2] for b, n in enumerate(lens)]).long()
+        assert not bool(grown[gone].any())
