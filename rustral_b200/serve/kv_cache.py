@@ -211,6 +211,7 @@ class PagedCache:
         if not self._h:
             raise InvalidArgument("PagedCache: num_blocks and block_size must be positive")
         self.k = self.v = self.pages = None
+        self.thinned: set = set()       # sequences that tokens have left (`evict`): their positions go on, their lengths do not
         self.state = [{} for _ in range(num_layers)]
         recurrent = layers is not None and any(c.state for c in layers)
         self.num_slots = num_slots if recurrent else 0
@@ -254,6 +255,7 @@ class PagedCache:
         return self._lib.rb_ba_reserve(self._h, seq_id, num_tokens) >= 0
 
     def free(self, seq_id: int) -> int:
+        self.thinned.discard(seq_id)
         return self._lib.rb_ba_free(self._h, seq_id)
 
     def trim(self, seq_id: int, num_tokens: int) -> int:
@@ -261,11 +263,14 @@ class PagedCache:
         n = self._lib.rb_ba_trim(self._h, seq_id, num_tokens)
         if n < 0:
             raise InvalidArgument(f"PagedCache.trim: no sequence {seq_id}")
+        if num_tokens == 0:
+            self.thinned.discard(seq_id)
         return n
 
     def evict(self, seq_ids: list, lens: list, keep: int, recent: int = 0, keep_first: int = 0) -> list:
         """Brings sequences of `lens` cached tokens down to `keep` (see ops.kv_evict_e4m3), every layer by its own tokens' attention weights,
-        and gives back the blocks that this empties.  Returns the new lengths; the sequences' positions do not change with them."""
+        and gives back the blocks behind their tokens, those that hold none yet among them.  Returns the new lengths; the sequences' positions do not
+        change with them, so that the steps of a sequence that tokens have left ask for its positions from here on (`thinned`)."""
         if self.pages is None or self.pages[0].weight is None:
             raise InvalidArgument("PagedCache.evict: these pages keep no attention weights")
         if len(seq_ids) != len(lens) or len(set(seq_ids)) != len(seq_ids):
@@ -283,8 +288,10 @@ class PagedCache:
         for pages in self.pages:
             kv_evict_e4m3(pages, table, length, keep, recent, keep_first)
         new = [min(n, keep) for n in lens]
-        for s, n in zip(seq_ids, new):
-            self.trim(s, n)
+        for s, n, m in zip(seq_ids, lens, new):
+            self.trim(s, m)
+            if n > m:
+                self.thinned.add(s)
         return new
 
     def block_table(self, seq_id: int) -> list:

@@ -187,7 +187,9 @@ class ModelRunner:
 
     `kv_quantization` CacheQuantization.FP8 (GPT-2 and Llama style models): keys and values are cached in e4m3, half the bytes.  Whole prompts
     attend over their keys and values as they are, later portions and decoded tokens over the cached ones.  With `kv_weights` decoding sums
-    every cached token's attention weight, and `cache.evict` may drop tokens between steps; a decoded token's position is then given to `decode`."""
+    every cached token's attention weight, and `cache.evict` may drop tokens between steps; the positions of such a sequence's tokens are then given
+    to `decode`, `step` and `step_mixed`, which refuse it without them.  A prompt's own rows add no weight: right after it all weights are zero, and of equal
+    ones the earliest tokens stay."""
 
     def __init__(self, cfg, params=None, device=None, num_blocks: int = 1024, block_size: int = 16, seed: int = 0, tp=None,
                  dtype=None, num_slots: int = 64, kv_quantization: CacheQuantization | None = None, kv_weights: bool = False):
@@ -353,18 +355,36 @@ class ModelRunner:
         logits of the last position, [vocab_padded]."""
         return self.step_mixed([(seq_id, tokens, 0, True)], [], [], [])[0][0]
 
+    def _check_positions(self, seq_ids, first: dict | None, tokens) -> None:
+        """`first`: positions of the first of `tokens[i]` tokens of sequence seq_ids[i], where they are not their places in the cache."""
+        if first and self.cache.pages is None:
+            raise ValueError("positions apart from the lengths need a cache in e4m3")
+        for s, n in zip(seq_ids, tokens):
+            p = first.get(s) if first else None
+            if p is None and s in self.cache.thinned:
+                raise ValueError(f"tokens of sequence {s} have left the cache: its positions are needed")
+            if p is not None and (p < 0 or (self.cfg.arch == "gpt2" and p + n > self.cfg.seq_len)):
+                raise ValueError(f"sequence {s}: no position {p if p < 0 else p + n - 1}")
+
     @torch.no_grad()
-    def step_mixed(self, chunks: list, dec_ids: list, dec_tok: list, dec_len: list):
+    def step_mixed(self, chunks: list, dec_ids: list, dec_tok: list, dec_len: list, positions: dict | None = None):
         """One model pass over several prompt chunks and the decode batch.
 
         `chunks`: list of (seq_id, tokens, start, want): `tokens` are positions [start, start + len) of the sequence's
         prefix; everything before `start` is already in the cache.  `want`: True for the logits of the last position,
         False for none, or a list of places among `tokens`.  `dec_*`: as for `decode`.  All rows go through the
         projections, the MLP and the collectives together (the weights are read once per step); attention runs per part.
+        `positions`: for a sequence that tokens have left (`cache.evict`) the position of its first token in this step; `start` and `dec_len` count what
+        is cached.  A portion that begins at 0 begins the sequence anew.
         Returns (per chunk: logits [vocab_padded], None, or [len(want), vocab_padded]; decode logits
         [len(dec_ids), vocab_padded] or None).
         (Batched and chunked prefill of the reference's scheduler: crates/nn/src/continuous_batching.rs:248-295.)"""
         dev, bs = self.device, self.block_size
+        if positions or self.cache.thinned:
+            for seq_id, _, start, _ in chunks:
+                if start == 0 and not (positions and seq_id in positions):
+                    self.cache.thinned.discard(seq_id)
+            self._check_positions([c[0] for c in chunks] + list(dec_ids), positions, [len(c[1]) for c in chunks] + [1] * len(dec_ids))
         rd = sum(len(c[1]) for c in chunks)
         nd = len(dec_ids)
         T = rd + nd
@@ -395,9 +415,13 @@ class ModelRunner:
             tables.append(self.cache.block_table(seq_id))
             numbers[r0:r1] = tokens
             self.cache.fill_slots(seq_id, start, r1 - r0, at + 8 * (T + r0), at + 8 * (2 * T + r0))
+            if positions and seq_id in positions:
+                numbers[T + r0:T + r1] = range(positions[seq_id], positions[seq_id] + r1 - r0)
         for r, (seq_id, tok, n) in enumerate(zip(dec_ids, dec_tok, dec_len), rd):
             numbers[r] = tok
             self.cache.fill_slots(seq_id, n - 1, 1, at + 8 * (T + r), at + 8 * (2 * T + r))
+            if positions and seq_id in positions:
+                numbers[T + r] = positions[seq_id]
         numbers[3 * T:3 * T + n_sel] = rows[:n_sel]
         end, places = 3 * T + n_sel, {}
         for i, n in later:
@@ -422,7 +446,7 @@ class ModelRunner:
             table += [(rd + i, 1, self.cache.state_slot(s_), n - 1) for i, (s_, n) in enumerate(zip(dec_ids, dec_len))]
             segments = Segments.of(table, dev)
         sb = StepBatch(ids, pos, slots, spans, rd, tables, bt, ctx, bs, segments,
-                       cached={i: sent_longs[lo:hi] for i, (lo, hi) in places.items()})
+                       cached={i: sent_longs[lo:hi] for i, (lo, hi) in places.items()}, moved=bool(positions))
         sel = sent_longs[3 * T:3 * T + n_sel] if n_sel else None if rows else []
         logits = self._run(sb, sel)
         out, at = [], 0
@@ -432,11 +456,14 @@ class ModelRunner:
             at += len(w)
         return out, (logits[at:] if dec_ids else None)
 
-    def step(self, chunks: list, dec_ids: list, dec_tok: list, dec_len: list):
+    def step(self, chunks: list, dec_ids: list, dec_tok: list, dec_len: list, positions: dict | None = None):
         """One engine iteration: `step_mixed` when there is prompt work, else the graphed `decode`."""
         if chunks:
-            return self.step_mixed(chunks, dec_ids, dec_tok, dec_len)
-        return [], (self.decode(dec_ids, dec_tok, dec_len) if dec_ids else None)
+            return self.step_mixed(chunks, dec_ids, dec_tok, dec_len, positions)
+        at = [positions.get(s, n - 1) for s, n in zip(dec_ids, dec_len)] if positions else None
+        if at is not None and self.cache.thinned:
+            self._check_positions(dec_ids, positions, [1] * len(dec_ids))          # which sequences were given one
+        return [], (self.decode(dec_ids, dec_tok, dec_len, at) if dec_ids else None)
 
     # ---- decode ------------------------------------------------------------------------------------------------------
     def _decode_segments(self, seq_ids, context_lens) -> list:
@@ -468,8 +495,10 @@ class ModelRunner:
         positions, where tokens have left the cache (a cache in e4m3; otherwise they are the lengths less one).
         Returns logits [batch, vocab_padded] (with CUDA graphs: valid until the next decode call)."""
         dev = self.device
-        if positions is not None and self.cache.pages is None:
-            raise ValueError("positions apart from the lengths need a cache in e4m3")
+        if positions is not None or self.cache.thinned:
+            if positions is not None and len(positions) != len(seq_ids):
+                raise ValueError(f"{len(positions)} positions for {len(seq_ids)} sequences")
+            self._check_positions(seq_ids, None if positions is None else dict(zip(seq_ids, positions)), [1] * len(seq_ids))
         if self.use_graphs and dev.type == "cuda":
             return self._decode_graphed(seq_ids, last_tokens, context_lens, positions)
         ids = torch.tensor(last_tokens, dtype=torch.int64, device=dev)

@@ -228,3 +228,126 @@ def test_a_loaded_runner_keeps_weights():
     assert r.kv_weights and all(p.weight is not None for p in r.cache.pages)
     with pytest.raises(InvalidArgument):
         load_runner("llama-test", device="cpu", num_blocks=4, kv_weights=True)
+
+
+def thinned(name, device, graphs=False):
+    """A runner with 41 tokens of sequence 1 brought down to 16."""
+    r = runner_of(name, device, kv_weights=True)
+    r.use_graphs = graphs
+    assert r.cache.allocate(1, 60)
+    r.prefill(1, tokens(r.cfg, 40, 1))
+    r.decode([1], [3], [41])
+    assert r.cache.evict([1], [41], 16, 4, 1) == [16] and r.cache.thinned == {1}
+    assert r.cache.allocate(1, 60) and r.cache.allocate(2, 40)
+    return r
+
+
+def keys_of(r, toks, positions):
+    """Keys of layer 0 in 64 bits from the weights, and how far 16-bit activations may take them: the embedding and the norm's output are rounded (2^-8 each, the
+    first also through the norm's statistics), and so are the product and the rotation."""
+    P, cfg = r.params, r.cfg
+    w = lambda n: P.w(n).double().cpu()  # noqa: E731
+    pos, H, G, D = torch.tensor(positions), cfg.n_head, cfg.n_kv_head, cfg.head_dim
+    x = w("tok_embed.embed")[torch.tensor(toks)]
+    if cfg.arch == "gpt2":
+        x = x + w("pos_embed.embed")[pos]
+        x = x - x.mean(-1, keepdim=True)
+    x = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + cfg.norm_eps) * w("layers.0.ln1.weight")
+    x = x + (w("layers.0.ln1.bias") if cfg.arch == "gpt2" else 0.0)
+    W = w("layers.0.attn.wqkv.weight")[H * D:(H + G) * D]
+    k = x @ W.t() + (w("layers.0.attn.wqkv.bias")[H * D:(H + G) * D] if cfg.arch == "gpt2" else 0.0)
+    off = 3 * 2.0 ** -8 * (x.abs() @ W.abs().t()) + 2.0 ** -8 * k.abs()
+    if cfg.arch == "llama":
+        a, b = k.view(-1, G, 2, D // 2).unbind(2)
+        angle = pos.double()[:, None, None] * cfg.rope_theta ** (-torch.arange(D // 2, dtype=torch.float64) * 2 / D)
+        k = torch.stack([a * angle.cos() - b * angle.sin(), a * angle.sin() + b * angle.cos()], 2).view(-1, G * D)
+        off = off.view(-1, G, 2, D // 2).sum(2, keepdim=True).expand(-1, -1, 2, -1).reshape(-1, G * D)
+        # the rotation's own rounding, and of a 32-bit angle 2^-24 of it and of its cosine's argument
+        off = off + k.abs() * 2.0 ** -8 + pos.double()[:, None] * 2.0 ** -22 * k.abs().amax()
+    return k, off
+
+
+def holds_keys(r, seq, place, toks, positions):
+    """The pages' keys of tokens at places `place` on are those of tokens `toks` at `positions`, and not those at their places."""
+    pages, n = r.cache.pages[0], place + len(toks)
+    t = torch.tensor([r.cache.block_table(seq)], dtype=torch.int32, device=r.device)
+    lens, starts = (torch.tensor(x, dtype=torch.int32, device=r.device) for x in ([n], [0, n]))
+    got = ops.kv_read_e4m3(pages, t, lens, starts, n, dtype=torch.float32)[0][place:].double().cpu()
+    e = pages.k_exp[t[0].long()][torch.arange(place, n) // 16].double().cpu().repeat_interleave(r.cfg.head_dim, 1)
+    rounded = lambda k: k.abs() * 2.0 ** -3 + torch.exp2(e - 9)  # noqa: E731  half a step of a code, twice where its page's exponent grew
+    want, off = keys_of(r, toks, positions)
+    assert bool(((got - want).abs() <= off + rounded(want)).all())
+    for i, p in enumerate(positions):
+        if p != place + i:
+            other, off2 = keys_of(r, toks[i:i + 1], [place + i])
+            assert bool(((got[i] - other[0]).abs() > off2[0] + rounded(other)[i]).any())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("name", ["gpt2-test", "llama-test"])
+def test_positions_decide_the_keys(name, graphs, device):
+    """Steps of all kinds after an eviction: the stored keys are those of the positions that were given, formed apart from the runner."""
+    r = thinned(name, device, graphs)
+    for i, (tok, pos) in enumerate(((7, 41), (9, 42), (11, 90))):     # with graphs: captured, then replayed
+        r.decode([1], [tok], [17 + i], [pos])
+        holds_keys(r, 1, 16 + i, [tok], [pos])
+    r.step([], [1], [5], [20], {1: 91})
+    holds_keys(r, 1, 19, [5], [91])
+    more = tokens(r.cfg, 23, 9)
+    logits, decoded = r.step([(2, more, 0, True)], [1], [6], [21], {1: 92})
+    assert bool(torch.isfinite(logits[0]).all()) and bool(torch.isfinite(decoded).all())
+    holds_keys(r, 1, 20, [6], [92])
+    holds_keys(r, 2, 0, more, list(range(23)))
+    r.step_mixed([(1, more[:5], 21, True)], [2], [8], [24], {1: 93})
+    holds_keys(r, 1, 21, more[:5], [93, 94, 95, 96, 97])
+    holds_keys(r, 2, 23, [8], [23])
+    r.step_mixed([], [1, 2], [4, 4], [27, 25], {1: 98})
+    holds_keys(r, 1, 26, [4], [98])
+    holds_keys(r, 2, 24, [4], [24])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_mixed_step_gives_what_decoding_gives(device):
+    """A decoded row beside a portion of another sequence, after an eviction: the logits of a decoding step at the same position."""
+    out = []
+    for mixed in (False, True):
+        r = thinned("llama-test", device)
+        if mixed:
+            out.append(r.step([(2, tokens(r.cfg, 9, 2), 0, True)], [1], [6], [17], {1: 41})[1][0])
+        else:
+            out.append(r.decode([1], [6], [17], [41])[0])
+    off = (out[0] - out[1]).abs().max()                               # products of other numbers of rows may add up in another order
+    assert float(off) <= float(out[0].abs().max()) * (2.0 ** -5 if device == "cuda" else 1e-5)
+
+
+def test_sequences_that_tokens_have_left_ask_for_positions():
+    r = thinned("llama-test", "cpu")
+    more = tokens(r.cfg, 5, 2)
+    for call in (lambda: r.decode([1], [4], [17]), lambda: r.step([], [1], [4], [17]), lambda: r.step([], [1], [4], [17], {2: 0}),
+                 lambda: r.step([(2, more, 0, True)], [1], [4], [17]), lambda: r.step_mixed([(1, more, 16, True)], [], [], []),
+                 lambda: r.decode([1], [4], [17], []), lambda: r.decode([1], [4], [17], [-1])):
+        before = r.cache.pages[0].k.view(torch.uint8).clone()
+        with pytest.raises(ValueError):
+            call()
+        assert torch.equal(before, r.cache.pages[0].k.view(torch.uint8))
+    r.cache.free(1)
+    assert not r.cache.thinned and r.cache.allocate(1, 60)
+    r.prefill(1, tokens(r.cfg, 40, 1))
+    r.decode([1], [4], [41])
+    assert r.cache.evict([1], [41], 50) == [41] and not r.cache.thinned                  # nothing left
+    assert r.cache.evict([1], [41], 20) == [20] and r.cache.trim(1, 0) == 2 and not r.cache.thinned
+    assert r.cache.allocate(1, 60)
+    r.prefill(1, more)
+    r.decode([1], [4], [6])
+    assert r.cache.evict([1], [6], 3) == [3] and r.cache.allocate(1, 60)
+    r.prefill(1, more)                                                # a portion that begins at 0
+    r.decode([1], [4], [6])
+    g = thinned("gpt2-test", "cpu")
+    with pytest.raises(ValueError):
+        g.decode([1], [4], [17], [g.cfg.seq_len])                     # no such learned position
+    plain = ModelRunner(preset("llama-test"), device="cpu", num_blocks=8)
+    assert plain.cache.allocate(1, 4)
+    for call in (lambda: plain.step([], [1], [1], [1], {1: 3}), lambda: plain.step_mixed([], [1], [1], [1], {1: 3})):
+        with pytest.raises(ValueError):
+            call()
