@@ -277,6 +277,8 @@ class PagedCache:
             raise InvalidArgument("PagedCache.evict: a length for every sequence, and no sequence twice")
         tables = [self.block_table(s) for s in seq_ids]
         for s, t, n in zip(seq_ids, tables, lens):
+            if self._lib.rb_ba_table_len(self._h, s) < 0:
+                raise InvalidArgument(f"PagedCache.evict: no sequence {s}")
             if n < 0 or n > len(t) * self.block_size:
                 raise InvalidArgument(f"PagedCache.evict: sequence {s} has no blocks for {n} tokens")
         if not seq_ids:

@@ -351,3 +351,40 @@ def test_sequences_that_tokens_have_left_ask_for_positions():
     for call in (lambda: plain.step([], [1], [1], [1], {1: 3}), lambda: plain.step_mixed([], [1], [1], [1], {1: 3})):
         with pytest.raises(ValueError):
             call()
+
+
+def test_evict_refuses_before_it_drops():
+    """A sequence that is not there, or a budget that is none: nothing has been dropped or given back."""
+    c = PagedCache(8, 16, num_layers=2, head_dim=64, quantization=FP8, attention_weights=True)
+    assert c.allocate(1, 60)
+    for p in c.pages:
+        p.weight.uniform_()
+    before = [p.weight.clone() for p in c.pages]
+    for ids, lens, keep, recent in (([1, 9], [60, 0], 16, 0), ([1], [60], 0, 0), ([1], [60], 4, 5)):
+        with pytest.raises((InvalidArgument, ValueError)):
+            c.evict(ids, lens, keep, recent)
+        assert all(torch.equal(p.weight, w) for p, w in zip(c.pages, before)) and len(c.block_table(1)) == 4 and not c.thinned
+    assert c.allocate(2, 0) and c.evict([1, 2], [60, 0], 16) == [16, 0]             # a sequence without tokens is one
+    assert not any(torch.equal(p.weight, w) for p, w in zip(c.pages, before))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_evict_all_sequences_right_after_their_prompts(device):
+    """Weights of zero in every layer: the earliest tokens stay beside the last."""
+    lens, keep, recent, G = [20 + 7 * b % 90 for b in range(40)], 18, 6, 8
+    c = PagedCache(sum((n + 15) // 16 for n in lens), 16, 2, G, 64, device=device, quantization=FP8, attention_weights=True)
+    g, want = torch.Generator().manual_seed(1), []
+    ids = list(range(len(lens)))
+    assert all(c.allocate(s, n) for s, n in zip(ids, lens))
+    table = torch.empty((len(lens), max((n + 15) // 16 for n in lens)), dtype=torch.int32)
+    c.fill_tables(ids, table)
+    starts = torch.tensor([0, *lens], dtype=torch.int32).cumsum(0, dtype=torch.int32)
+    for p in c.pages:
+        k = torch.randn(sum(lens), G * 64, generator=g).bfloat16().to(device)
+        ops.kv_append_e4m3(p, k, -k, table.to(device), torch.tensor(lens, dtype=torch.int32, device=device), starts.to(device))
+        want.append(Cache(p))
+    assert c.evict(ids, lens, keep, recent) == [keep] * len(lens) and c.thinned == set(ids)
+    for p, o in zip(c.pages, want):
+        o.evict(table, lens, keep, recent, 0)
+        o.same(p)
+    assert all(len(c.block_table(s)) == 2 for s in ids)
