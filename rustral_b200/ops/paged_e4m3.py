@@ -200,7 +200,7 @@ def kv_append_e4m3(pages: PagesE4M3, k_new, v_new, block_tables, context_lens, r
         raise ValueError(f"kv_append_e4m3: {rows} rows for {batch} sequences need row_starts")
     if not k_new.is_cuda:
         return _append_cpu(pages, k_new, v_new, block_tables, context_lens, row_starts)
-    if rows == 0 or batch == 0:
+    if rows == 0 or batch == 0 or width == 0:
         return
     ld_k, ld_v = _pitch(k_new), _pitch(v_new)
     if not ld_k:
@@ -239,7 +239,7 @@ def kv_read_e4m3(pages: PagesE4M3, block_tables, context_lens, row_starts, rows:
                 x = _values_cpu(codes, exps, block_tables, b, n).reshape(n, G * D).to(to.dtype)
                 to[first:first + n][there] = x[there]
         return k, v
-    if rows == 0 or batch == 0:
+    if rows == 0 or batch == 0 or width == 0:
         return k, v
     if out is not None:
         ld_k, ld_v = _pitch(k), _pitch(v)

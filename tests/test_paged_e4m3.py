@@ -815,3 +815,19 @@ def test_attention_of_scores_past_the_range(device, lens, width, group, D, dtype
     if first:
         gone = torch.cat([t[b, 1:(n + bs - 1) // bs:2] for b, n in enumerate(lens)]).long()
         assert not bool(grown[gone].any())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_tables_without_pages(device):
+    """No position has a page: nothing is stored, no row is written."""
+    p, _, n = small(device)
+    before = to(p, device)
+    t, s = torch.zeros(2, 0, dtype=I32, device=device), ints([0, 1, 2], device)
+    x = torch.ones(2, 128, device=device).bfloat16()
+    ops.kv_append_e4m3(p, x, x, t, n)
+    ops.kv_append_e4m3(p, x, x, t, n, s)
+    for a, b in ((p.k, before.k), (p.v, before.v), (p.k_exp, before.k_exp), (p.weight, before.weight)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    out = (x.clone(), x.clone())
+    assert ops.kv_read_e4m3(p, t, n, s, 2, out=out) is not None and all(bool((y == 1).all()) for y in out)
+    assert ops.kv_read_e4m3(p, t, n, s, 2)[0].shape == (2, 128)
