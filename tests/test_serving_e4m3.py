@@ -388,3 +388,79 @@ def test_evict_all_sequences_right_after_their_prompts(device):
         o.evict(table, lens, keep, recent, 0)
         o.same(p)
     assert all(len(c.block_table(s)) == 2 for s in ids)
+
+
+class Ranks:
+    """Ranks of one process, a thread each, with the calls that a step makes of parallel.tp_inference.TPInferenceComm."""
+
+    def __init__(self, world):
+        import threading
+        self.world, self.meet, self.staged = world, threading.Barrier(world, timeout=60), [None] * world
+
+    def of(self, rank):
+        ranks = self
+
+        class Comm:
+            world = ranks.world
+            transport = "threads"
+
+            def __init__(self):
+                self.rank = rank
+
+            def staging(self, rows, cols):
+                ranks.staged[rank] = torch.empty(rows, cols)
+                return ranks.staged[rank]
+
+            def _all(self):
+                ranks.meet.wait()
+                got = [t.clone() for t in ranks.staged]
+                ranks.meet.wait()
+                return got
+
+            def all_reduce(self, rows, cols, residual=None):
+                total = sum(self._all())
+                return total if residual is None else total + residual
+
+            def all_gather_cols(self, rows, cols):
+                return torch.cat(self._all(), 1)
+
+            def end_step(self):
+                pass
+        return Comm()
+
+
+def test_ranks_cache_their_heads_in_e4m3():
+    """Two tensor-parallel ranks: a page's exponents are a head's own, so that every rank holds the codes that the whole model has for its heads, also after an
+    eviction, and all have its logits."""
+    from concurrent.futures import ThreadPoolExecutor
+    from rustral_b200.serve.weights import InferenceWeights
+    cfg = preset("llama-test", seq_len=512, n_layer=2, d_model=256, n_head=4, ffn_dim=256, n_kv_head=2)
+    whole = ModelRunner(cfg, device="cpu", num_blocks=32, seed=3, kv_quantization=FP8, kv_weights=True)
+    ranks = Ranks(2)
+    shards = [ModelRunner(cfg, params=InferenceWeights.shard_of(whole.params, cfg, i, 2), device="cpu", num_blocks=32, tp=ranks.of(i),
+                          kv_quantization=FP8, kv_weights=True) for i in range(2)]
+    a, b = tokens(cfg, 50, 1), tokens(cfg, 20, 2)
+
+    @torch.no_grad()
+    def steps(r):
+        assert r.cache.allocate(1, 80) and r.cache.allocate(2, 40)
+        out = [r.step([(1, a[:30], 0, False), (2, b, 0, True)], [], [], [])[0][1][None]]
+        logits, decoded = r.step([(1, a[30:], 30, True)], [2], [5], [21])
+        out += [logits[0][None], decoded]
+        out.append(r.decode([1, 2], [6, 7], [51, 22]))
+        before = [p.k.float() * torch.exp2(p.k_exp.float())[..., None, None] for p in r.cache.pages]
+        lens = r.cache.evict([1, 2], [51, 22], 30, 8, 2)
+        out.append(r.decode([1, 2], [8, 9], [lens[0] + 1, lens[1] + 1], [51, 22]))
+        return torch.cat(out), before
+
+    want, keys = steps(whole)
+    with ThreadPoolExecutor(2) as pool:
+        got = list(pool.map(steps, shards))
+    assert torch.equal(got[0][0], got[1][0])
+    for i, (logits, k) in enumerate(got):
+        assert k[0].shape[1] == 1
+        # sums of two ranks add up in another order: a number beside a border of its code may take the other code, a step of 2^-3 of it
+        for x, y in zip(keys, k):
+            assert bool(((x[:, i] - y[:, 0]).abs() <= x[:, i].abs() * 2.0 ** -3 + 1e-4).all())
+            assert float((x[:, i] != y[:, 0]).float().mean()) < 0.01
+        torch.testing.assert_close(logits[:, :cfg.vocab_size], want[:, :cfg.vocab_size], rtol=0, atol=0.05 * float(want.abs().max()) + 0.02)
