@@ -78,15 +78,15 @@ class GPTBody:
         p = f"layers.{l}."
         kc, vc = (None, None) if r.cache.pages is not None else (r.cache.k[l], r.cache.v[l])
         qkv = self._norm_product(x, p + "ln1", P.w(p + "attn.wqkv.weight"), bias=None if rms else P.w(p + "attn.wqkv.bias"))
-        k2, v2 = qkv[:, H * D:(H + Hk) * D], qkv[:, (H + Hk) * D:]
         if r.cache.pages is not None:
             if rms:
                 rope_ops.rope_(qkv, H + Hk, D, positions=sb.pos, theta=self.cfg.rope_theta)
-            a = r.store_and_attend(l, qkv[:, :H * D], k2, v2, sb, self.scale)
+            a = r.store_and_attend(l, qkv[:, :H * D], qkv[:, H * D:(H + Hk) * D], qkv[:, (H + Hk) * D:], sb, self.scale)
         elif sb.arrived is not None and paged_ops.step_supported(qkv, H, Hk, D, kc, vc, sb.bt):
             # the kernel in front is the projection: tables, lengths and cached tokens are older
             a = paged_ops.attention_step(qkv, H, Hk, D, self.cfg.rope_theta if rms else 0.0, kc, vc, sb.bt, sb.ctx, sb.arrived, self.scale)
         else:
+            k2, v2 = qkv[:, H * D:(H + Hk) * D], qkv[:, (H + Hk) * D:]
             if rms:
                 rope_ops.rope_append_(qkv, H, Hk, D, sb.pos, self.cfg.rope_theta, kc, vc, sb.slots)
             else:
