@@ -89,7 +89,7 @@ struct E4Layout {
   static constexpr int kTile = 16 * D;                                   // bytes of a tile's keys; its values follow
   static constexpr int kRing = kE4Warps * kE4Stages * 2 * kTile;
   // The warps' sums lie behind the ring, those of `kRound` heads at a time (of a cluster those of all heads): with 4 heads of 128 three CTAs fit on an SM.
-  // 64 sequences of 4096, 4 KV heads for 32 heads of 128, one B200: 78.9 us with 8 at a time and two CTAs an SM, 74.8 so.
+  // 64 sequences of 4096, 4 KV heads for 32 heads of 128, one B200: 80.9 us with 8 at a time and two CTAs an SM, 74.9 so.
   static constexpr int kRound = NH == 1 && D == 128 ? 4 : 8;
   static int bytes(int heads) { return kRing + kE4Warps * heads * D * 4 + 1024; }
 };
@@ -682,7 +682,7 @@ e4_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
 
 // Adds the slices of a sequence for one head: 16 chains of every 16th slice, in order (with more than 64 slices 64 chains), then the chains in order.
 // COLS: 16-byte columns that a CTA takes, D / 4 of 128 threads or, MANY, where sequences may have more than 64 slices, 8 of 512 threads: one of 131072
-// tokens takes 10 us with 128 threads and 16 chains.  Grid: (heads, sequences, D / 4 / COLS).
+// tokens takes 24 us with 128 threads and 16 chains, 6.4 so.  Grid: (heads, sequences, D / 4 / COLS).
 template <typename T, int COLS, bool MANY>
 __global__ void __launch_bounds__(MANY ? 512 : 128)
 e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
@@ -795,7 +795,7 @@ e4_merge_kernel(const RbE4m3DecodeArgs a, int slices) {
 }
 
 // Adds the attention weights of a slice to its tokens' sums, a thread a token.  (As a part of the merge, with denominators formed in every CTA, it was
-// slower, 33 against 31 us for 24 sequences of 128 to 2560: the merge's registers leave room for fewer of its threads, and it waits for memory.)
+// slower, 33 against 30 us for 24 sequences of 128 to 2560: the merge's registers leave room for fewer of its threads, and it waits for memory.)
 __global__ void __launch_bounds__(kE4Slice)
 e4_weight_kernel(const RbE4m3DecodeArgs a, int slices) {
   pdl_wait();
@@ -831,8 +831,9 @@ long long e4_slices(int max_blocks, int block_size) {
   return (static_cast<long long>(max_blocks) * block_size + rb::kE4Slice - 1) / rb::kE4Slice;
 }
 // Whether the CTAs of a sequence and KV head merge as a cluster: few slices, heads for one pass, and no more CTAs than fit on the GPU at a time (three on an
-// SM).  One B200, us: one sequence of 300, 12 KV heads of 64 13.0, with a list or grid and its merge 20.6; of 2047, 4 KV heads of 128, with weights 13.1 / 21.7;
-// 48 of 16 to 1024, 8 KV heads of 64, 1536 CTAs, many without a token, 23.1 on the GPU / 19.2.
+// SM).  It goes by what the tables have room for, which the host knows, not by the lengths: a captured step whose tables are as wide as the context plans for that.
+// One B200, us from a captured graph, as a cluster / with a list or grid and its merge: one sequence of 300, 12 KV heads of 64 5.5 / 6.8; of 2047, 4 KV heads of
+// 128, with weights 8.7 / 9.9 (as calls 11.1 / 17.1: two launches less); 48 of 16 to 1024, 8 KV heads of 64, 1536 CTAs, many without a token, 20.7 / 16.2.
 bool in_clusters(int batch, int kv_heads, long long slices, int group) {
   return slices <= 8 && group <= 16 && batch * kv_heads * slices <= 3ll * rbhost::device_sm_count();
 }

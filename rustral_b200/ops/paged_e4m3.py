@@ -6,7 +6,8 @@ portions of prompts attend over them, and `kv_evict_e4m3` drops the tokens with 
 
 A number of a page is code * 2^exponent.  The exponent of a page's keys (values) for a head is the least in -100 .. 119 under which their largest
 finite number is at most 448, the largest code; infinities are held as that code, NaN stays NaN.  Block tables and lengths are those of the
-bf16 cache: int32 [batch, width] and int32 [batch], tokens in the cache with the new ones.
+bf16 cache: int32 [batch, width] and int32 [batch], tokens in the cache with the new ones.  On a GPU attention and eviction take up to 65535
+sequences a call.
 """
 from __future__ import annotations
 
