@@ -380,11 +380,11 @@ class ModelRunner:
         [len(dec_ids), vocab_padded] or None).
         (Batched and chunked prefill of the reference's scheduler: crates/nn/src/continuous_batching.rs:248-295.)"""
         dev, bs = self.device, self.block_size
+        anew = set()
         if positions or self.cache.thinned:
-            for seq_id, _, start, _ in chunks:
-                if start == 0 and not (positions and seq_id in positions):
-                    self.cache.thinned.discard(seq_id)
-            self._check_positions([c[0] for c in chunks] + list(dec_ids), positions, [len(c[1]) for c in chunks] + [1] * len(dec_ids))
+            anew = {c[0] for c in chunks if c[2] == 0 and c[1] and not (positions and c[0] in positions)}
+            self._check_positions([c[0] for c in chunks if c[0] not in anew] + list(dec_ids), positions,
+                                  [len(c[1]) for c in chunks if c[0] not in anew] + [1] * len(dec_ids))
         rd = sum(len(c[1]) for c in chunks)
         nd = len(dec_ids)
         T = rd + nd
@@ -449,6 +449,7 @@ class ModelRunner:
                        cached={i: sent_longs[lo:hi] for i, (lo, hi) in places.items()}, moved=bool(positions))
         sel = sent_longs[3 * T:3 * T + n_sel] if n_sel else None if rows else []
         logits = self._run(sb, sel)
+        self.cache.thinned -= anew
         out, at = [], 0
         for w, c in zip(want, chunks):
             part = logits[at:at + len(w)] if w else None

@@ -331,6 +331,14 @@ def test_sequences_that_tokens_have_left_ask_for_positions():
         with pytest.raises(ValueError):
             call()
         assert torch.equal(before, r.cache.pages[0].k.view(torch.uint8))
+    assert r.cache.evict([1], [16], 12) == [12] and r.cache.allocate(2, 40)
+    r.prefill(2, more)
+    r.decode([2], [4], [6])
+    assert r.cache.evict([2], [6], 3) == [3]
+    with pytest.raises(ValueError):
+        r.step([(2, more, 0, True)], [1], [4], [13])                  # 2 would begin anew, but nothing is done without a position of 1
+    assert r.cache.thinned == {1, 2}
+    r.cache.free(2)
     r.cache.free(1)
     assert not r.cache.thinned and r.cache.allocate(1, 60)
     r.prefill(1, tokens(r.cfg, 40, 1))
