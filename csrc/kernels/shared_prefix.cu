@@ -1,0 +1,529 @@
+// Decode attention for sequences that share their first tokens (beams and samples of one prompt, requests behind one system prompt).
+//
+// Alone, every sequence of a group reads the shared keys and values again: n sequences, n times the bytes.  Here the queries of all of a group's
+// sequences for one KV head are the rows of one product over the shared tokens, which are read once; each sequence's own tokens follow as in any decode
+// attention, and a last launch joins the parts of a row by their maxima and sums:
+//     out = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i,   M = max_i m_i.
+//
+// Work is a list of entries (a tile of a group's rows over its shared tokens, a sequence's rows over its own), cut into units of 128 tokens; the units of all entries,
+// one behind the other, are dealt in equal runs to CTAs that stay.  An entry's rows are accumulated over all units of a run, so there are at most (entries +
+// CTAs) partial results, whose places follow from the entry's number and the CTA's: entry k and CTA c use place k + c, which is unique, because
+// from one (entry, CTA) of the list to the next one of the two grows.  Every CTA forms the list of running totals itself from the lengths.
+//
+// This file's split kernel is for few rows (up to 32): the rows are one or two m16n8k16 tiles, a warp takes 32 of a unit's tokens, keys and values come
+// by 16-byte asynchronous copies into tiles of its own.  It is bound by these reads.
+#include "shared_prefix.h"
+
+#include <cuda_fp16.h>
+#include <limits.h>
+
+#include "pdl.cuh"
+#include "warp_mma.cuh"
+
+namespace rb {
+
+constexpr int kSpWarps = 4;
+constexpr int kSpUnit = 128;                     // tokens
+constexpr float kSpLog2e = 1.4426950408889634f;
+
+struct SpParams {
+  const void* q;
+  void* out;
+  const void* k;
+  const void* v;
+  const int* tables;
+  const int* lens;
+  const int* shared;
+  const int* starts;
+  const int* group_of;
+  int* totals;                                   // [2 batch + 1] running totals of units, for the join
+  float* partial;
+  long long ld_q, ld_o, num_blocks;
+  int batch, groups, width, block_size, heads, kv_heads, per, parts, seqs, cap;
+  // per: query heads of a virtual KV head (a KV head's group in `parts` equal parts, so that a sequence's rows fit a tile); seqs: sequences of a tile; cap: tokens of a table's row
+  int rows;                                      // of a tile
+  int own_first;                                 // place of the first own entry among the entries
+  int ctas;                                      // along x
+  float scale2;                                  // scale * log2(e)
+};
+
+template <typename T>
+__device__ __forceinline__ void sp_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void sp_mma<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { wm_mma(c, a, b0, b1); }
+template <>
+__device__ __forceinline__ void sp_mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t sp_pack(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t sp_pack<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+template <>
+__device__ __forceinline__ uint32_t sp_pack<__half>(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <typename T>
+__device__ __forceinline__ T sp_round(float v);
+template <>
+__device__ __forceinline__ __nv_bfloat16 sp_round<__nv_bfloat16>(float v) { return __float2bfloat16(v); }
+template <>
+__device__ __forceinline__ __half sp_round<__half>(float v) { return __float2half(v); }
+
+__device__ __forceinline__ int sp_length(const SpParams& p, int b) { return min(max(p.lens[b], 0), p.cap); }
+// What each group's sequences read together: no more tokens than the shortest of them has, those without tokens aside, so that all rows of a tile see all of its
+// tokens.  `shared`: [groups] of the CTA's shared memory.
+__device__ __forceinline__ void sp_shared(const SpParams& p, int* shared) {
+  for (int g = threadIdx.x; g < p.groups; g += blockDim.x) shared[g] = INT_MAX;
+  __syncthreads();
+  for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
+    const int n = sp_length(p, b);
+    if (n > 0) atomicMin(&shared[p.group_of[b]], n);
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g < p.groups; g += blockDim.x) {
+    const int n = shared[g];
+    shared[g] = n == INT_MAX ? 0 : min(n, max(p.shared[g], 0));
+  }
+  __syncthreads();
+}
+// Units of entry e: tiles of rows begin at every `seqs`-th sequence of a group.
+__device__ __forceinline__ int sp_units(const SpParams& p, const int* shared_of, int e) {
+  const int b = e < p.batch ? e : e - p.batch, g = p.group_of[b], shared = shared_of[g];
+  if (e < p.batch) return (b - p.starts[g]) % p.seqs == 0 ? (shared + kSpUnit - 1) / kSpUnit : 0;
+  return max(0, sp_length(p, b) - shared + kSpUnit - 1) / kSpUnit;
+}
+// Running totals of the units of all entries, [2 batch + 1], formed by all threads of a CTA.
+__device__ __forceinline__ void sp_totals(const SpParams& p, const int* shared_of, int* totals, int* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int before = 0;
+  if (threadIdx.x == 0) totals[0] = 0;
+  for (int first = 0; first < 2 * p.batch; first += blockDim.x) {
+    const int e = first + threadIdx.x;
+    int upto = e < 2 * p.batch ? sp_units(p, shared_of, e) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) warp_sums[warp] = upto;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < warps; ++w) {
+      const int s = warp_sums[w];
+      if (w < warp) upto += s;
+      all += s;
+    }
+    if (e < 2 * p.batch) totals[e + 1] = before + upto;
+    before += all;
+    __syncthreads();
+  }
+}
+// First unit of CTA c's run, and the CTA that has unit u.
+__device__ __forceinline__ int sp_run(int total, int ctas, int c) {
+  const int share = total / ctas, over = total - share * ctas;
+  return c * share + min(c, over);
+}
+__device__ __forceinline__ int sp_cta_of(int total, int ctas, int u) {
+  const int share = total / ctas, over = total - share * ctas, wide = over * (share + 1);
+  return u < wide ? u / (share + 1) : over + (u - wide) / share;
+}
+// Place of an entry among those that have partial results; grows with e.
+__device__ __forceinline__ int sp_place(const SpParams& p, int e) {
+  return e < p.batch ? e / p.seqs + p.group_of[e] : p.own_first + e - p.batch;
+}
+
+template <int D, int MT>
+struct SpSmem {
+  static constexpr int kRow = D + 8;             // padded rows (elements): ldmatrix rows hit distinct banks
+  static constexpr int kTile = 32 * kRow;        // a warp's tile of K or V
+  static constexpr int kQ = kSpWarps * 2 * kTile * 2;                    // byte offsets
+  static constexpr int kMl = kQ + 16 * MT * kRow * 2;
+  static constexpr int kTotals = kMl + kSpWarps * 16 * MT * 8;
+};
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kSpWarps * 32, MT == 1 ? 3 : 2)
+shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
+  pdl_wait();
+  pdl_launch();
+  using L = SpSmem<D, MT>;
+  constexpr int kRow = L::kRow, NT = D / 8, LP = D / 8, kRows = 16 * MT;
+  extern __shared__ __align__(16) uint8_t sp_mem[];
+  __shared__ int warp_sums[kSpWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
+  T* q_sh = reinterpret_cast<T*>(sp_mem + L::kQ);
+  float2* ml_sh = reinterpret_cast<float2*>(sp_mem + L::kMl);           // [warp][row]: maximum, sum
+  int* totals = reinterpret_cast<int*>(sp_mem + L::kTotals);
+  const uint32_t q_u32 = smem_u32(q_sh), k_u32 = smem_u32(sp_mem) + warp * 2 * L::kTile * 2, v_u32 = k_u32 + L::kTile * 2;
+  int* shared_of = totals + 2 * p.batch + 1;
+  sp_shared(p, shared_of);
+  sp_totals(p, shared_of, totals, warp_sums);
+  const int entries = 2 * p.batch, total = totals[entries];
+  const int vh = blockIdx.y, hk = vh / p.parts, head0 = (vh - hk * p.parts) * p.per;
+  const int group = p.heads / p.kv_heads, per = min(p.per, group - head0);
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = threadIdx.x; i <= entries; i += blockDim.x) p.totals[i] = totals[i];
+  int u = sp_run(total, gridDim.x, blockIdx.x);
+  const int u_end = sp_run(total, gridDim.x, blockIdx.x + 1);
+  if (u >= u_end) return;
+  // the entry that has unit u: the last one that begins at or in front of it
+  int e = 0;
+  for (int hi = entries; hi - e > 1;) {
+    const int mid = (e + hi) >> 1;
+    if (totals[mid] <= u) e = mid;
+    else hi = mid;
+  }
+  const T* K = static_cast<const T*>(p.k);
+  const T* V = static_cast<const T*>(p.v);
+
+  while (u < u_end) {
+    while (totals[e + 1] <= u) ++e;
+    // ---- this entry's rows and tokens
+    const bool own = e >= p.batch;
+    const int b = own ? e - p.batch : e, g = p.group_of[b], shared = shared_of[g];
+    const int rows = own ? per : min(p.seqs, p.starts[g + 1] - b) * per;
+    const int first = own ? shared : 0, count = own ? sp_length(p, b) - shared : shared;
+    const int* table = p.tables + static_cast<long long>(own ? b : p.starts[g]) * p.width;
+    const int u0 = u - totals[e], u1 = min(u_end, totals[e + 1]) - totals[e];
+    __syncthreads();                             // the last entry's queries and results have been read
+    for (int i = threadIdx.x; i < kRows * LP; i += blockDim.x) {
+      const int r = i / LP, c = (i - r * LP) * 8;
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (r < rows) {
+        const int s = r / per;
+        x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (b + s) * p.ld_q + static_cast<long long>(hk * group + head0 + r - s * per) * D + c);
+      }
+      *reinterpret_cast<uint4*>(q_sh + r * kRow + c) = x;
+    }
+    __syncthreads();
+
+    int slot = 0, n_next = 0;
+    auto locate = [&](int unit) {
+      const int at = unit * kSpUnit + warp * 32;
+      n_next = unit < u1 ? min(32, count - at) : 0;
+      slot = -1;
+      if (lane < n_next) {
+        const int token = first + at + lane, page = token / p.block_size;
+        int blk = table[page];
+        if (blk < 0 || blk >= p.num_blocks) {                          // corrupt tables read block 0 instead of faulting
+          RB_BOUNDS_HIT(104);
+          blk = 0;
+        }
+        slot = blk * p.block_size + (token - page * p.block_size);     // the host bounds num_blocks * block_size below 2^31
+      }
+    };
+    auto request = [&](const T* cache, uint32_t tile) {
+      if (n_next > 0) {
+#pragma unroll
+        for (int i = 0; i < LP; ++i) {
+          const int idx = i * 32 + lane, r = idx / LP, c = (idx - r * LP) * 8;
+          const int s = __shfl_sync(0xffffffffu, slot, r);
+          wm_cp16(tile + (r * kRow + c) * 2, s >= 0 ? cache + (static_cast<long long>(s) * p.kv_heads + hk) * D + c : cache, s >= 0);
+        }
+      }
+      wm_cp_commit();
+    };
+    float m[MT][2], l[MT][2], acc[MT][NT][4];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      m[t][0] = m[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) acc[t][n][0] = acc[t][n][1] = acc[t][n][2] = acc[t][n][3] = 0.f;
+    }
+    locate(u0);
+    request(K, k_u32);
+    request(V, v_u32);
+    for (int unit = u0; unit < u1; ++unit) {
+      const int n_tok = n_next;
+      wm_cp_wait<1>();                           // this unit's K tile has landed (V may be on its way)
+      __syncwarp();
+      float s[MT][4][4];
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) s[t][n][0] = s[t][n][1] = s[t][n][2] = s[t][n][3] = 0.f;
+      if (n_tok > 0) {
+#pragma unroll
+        for (int k0 = 0; k0 < D; k0 += 16) {
+          uint32_t bk[2][4];
+#pragma unroll
+          for (int np = 0; np < 2; ++np) wm_ldsm_x4(wm_b(k_u32, kRow, np * 16, k0, lane), bk[np]);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            if (t > 0 && rows <= t * 16) continue;
+            uint32_t a[4];
+            wm_ldsm_x4(wm_a(q_u32, kRow, t * 16, k0, lane), a);
+#pragma unroll
+            for (int np = 0; np < 2; ++np) {
+              sp_mma<T>(s[t][2 * np], a, bk[np][0], bk[np][1]);
+              sp_mma<T>(s[t][2 * np + 1], a, bk[np][2], bk[np][3]);
+            }
+          }
+        }
+      }
+      __syncwarp();                              // every lane has read its K fragments
+      locate(unit + 1);
+      request(K, k_u32);
+      if (n_tok > 0) {
+        uint32_t pf[MT][2][4];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          if (t > 0 && rows <= t * 16) continue;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {          // rows gq and gq + 8
+            float mx = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                float& x = s[t][n][2 * i + j];
+                x = n * 8 + 2 * tq + j < n_tok ? x * p.scale2 : -INFINITY;
+                mx = fmaxf(mx, x);
+              }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float mn = fmaxf(m[t][i], mx), from = mn == -INFINITY ? 0.f : mn;       // a row that has seen nothing yet
+            const float al = wm_ex2(m[t][i] - from);
+            float sum = 0.f;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const float p0 = wm_ex2(s[t][n][2 * i] - from), p1 = wm_ex2(s[t][n][2 * i + 1] - from);
+              sum += p0 + p1;
+              pf[t][n >> 1][(n & 1) * 2 + i] = sp_pack<T>(p0, p1);
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            l[t][i] = fmaf(l[t][i], al, sum);
+            m[t][i] = mn;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              acc[t][n][2 * i] *= al;
+              acc[t][n][2 * i + 1] *= al;
+            }
+          }
+        }
+        wm_cp_wait<1>();                         // this unit's V tile has landed
+        __syncwarp();
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int n2 = 0; n2 < NT / 2; ++n2) {
+            uint32_t bv[4];
+            wm_ldsm_x4_t(wm_b_t(v_u32, kRow, n2 * 16, ks * 16, lane), bv);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+              if (t > 0 && rows <= t * 16) continue;
+              sp_mma<T>(acc[t][2 * n2], pf[t][ks], bv[0], bv[1]);
+              sp_mma<T>(acc[t][2 * n2 + 1], pf[t][ks], bv[2], bv[3]);
+            }
+          }
+        __syncwarp();                            // every lane has read its V fragments
+      }
+      request(V, v_u32);
+    }
+
+    // ---- the warps' sums are joined in the memory of their tiles: fp32 [rows][D + 8]
+    wm_cp_wait<0>();
+    __syncwarp();
+    float* mine = reinterpret_cast<float*>(sp_mem + warp * 2 * L::kTile * 2);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      if (t > 0 && rows <= t * 16) continue;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = t * 16 + gq + i * 8;
+        if (tq == 0) ml_sh[warp * kRows + r] = make_float2(m[t][i], l[t][i]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(mine + r * kRow + n * 8 + 2 * tq) = make_float2(acc[t][n][2 * i], acc[t][n][2 * i + 1]);
+      }
+    }
+    __syncthreads();
+    const long long place = static_cast<long long>(sp_place(p, e) + blockIdx.x) * gridDim.y + vh;
+    float* part = p.partial + place * kRows * (D + 2);
+    for (int i = threadIdx.x; i < rows * (D / 4); i += blockDim.x) {
+      const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kSpWarps; ++w) mx = fmaxf(mx, ml_sh[w * kRows + r].x);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      float den = 0.f;
+#pragma unroll
+      for (int w = 0; w < kSpWarps; ++w) {
+        const float2 ml = ml_sh[w * kRows + r];
+        const float f = ml.x == -INFINITY ? 0.f : wm_ex2(ml.x - mx);
+        const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sp_mem + w * 2 * L::kTile * 2) + r * kRow + c);
+        sum.x = fmaf(x.x, f, sum.x); sum.y = fmaf(x.y, f, sum.y); sum.z = fmaf(x.z, f, sum.z); sum.w = fmaf(x.w, f, sum.w);
+        den = fmaf(ml.y, f, den);
+      }
+      *reinterpret_cast<float4*>(part + 2 * kRows + r * D + c) = sum;
+      if (c == 0) *reinterpret_cast<float2*>(part + 2 * r) = make_float2(mx, den);
+    }
+    u = totals[e] + u1;
+  }
+}
+
+// out[b, head] from the partial results of its rows: a warp per head, lanes own D / 32 neighbouring columns.  Grid (batch, virtual KV heads).
+template <typename T, int D>
+__global__ void __launch_bounds__(kSpWarps * 32)
+shared_join_kernel(const SpParams p) {
+  pdl_wait();
+  pdl_launch();
+  constexpr int C = D / 32;
+  const int b = blockIdx.x, vh = blockIdx.y, hk = vh / p.parts, head0 = (vh - hk * p.parts) * p.per;
+  const int group = p.heads / p.kv_heads, per = min(p.per, group - head0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = p.group_of[b], tile = b - (b - p.starts[g]) % p.seqs, total = p.totals[2 * p.batch];
+  // places of the parts: those of the shared tokens, then the sequence's own
+  int at[2], n[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = i == 0 ? tile : p.batch + b, t0 = p.totals[e], t1 = p.totals[e + 1];
+    const int c0 = t1 > t0 ? sp_cta_of(total, p.ctas, t0) : 0;
+    n[i] = t1 > t0 ? sp_cta_of(total, p.ctas, t1 - 1) - c0 + 1 : 0;
+    at[i] = sp_place(p, e) + c0;
+  }
+  const int parts = sp_length(p, b) > 0 ? n[0] + n[1] : 0;              // a sequence without tokens gets zeros
+  for (int h = warp; h < per; h += kSpWarps) {
+    const int r0 = (b - tile) * per + h;
+    auto part_of = [&](int s) {
+      const int i = s >= n[0] ? 1 : 0;
+      return p.partial + (static_cast<long long>(at[i] + s - (i ? n[0] : 0)) * gridDim.y + vh) * p.rows * (D + 2);
+    };
+    auto row_of = [&](int s) { return s >= n[0] ? h : r0; };
+    float mx = -INFINITY;
+    for (int s = lane; s < parts; s += 32) mx = fmaxf(mx, part_of(s)[2 * row_of(s)]);
+    mx = warp_max(mx);
+    float acc[C], den = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[c] = 0.f;
+    for (int s0 = 0; s0 < parts; s0 += 32) {
+      float f = 0.f;
+      if (s0 + lane < parts) {
+        const float2 ml = *reinterpret_cast<const float2*>(part_of(s0 + lane) + 2 * row_of(s0 + lane));
+        f = ml.x == -INFINITY ? 0.f : wm_ex2(ml.x - mx);
+        den = fmaf(ml.y, f, den);
+      }
+      const int m = min(32, parts - s0);
+#pragma unroll 4
+      for (int s = 0; s < m; ++s) {
+        const float fs = __shfl_sync(0xffffffffu, f, s);
+        const float* x = part_of(s0 + s) + 2 * p.rows + row_of(s0 + s) * D + lane * C;
+        float v[C];
+        if (C == 4) {
+          const float4 w = *reinterpret_cast<const float4*>(x);
+          v[0] = w.x; v[1] = w.y; v[2 % C] = w.z; v[3 % C] = w.w;
+        } else {
+          const float2 w = *reinterpret_cast<const float2*>(x);
+          v[0] = w.x; v[1] = w.y;
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] = fmaf(v[c], fs, acc[c]);
+      }
+    }
+    den = warp_sum(den);
+    const float inv = parts > 0 ? 1.f / den : 0.f;
+    T* o = static_cast<T*>(p.out) + b * p.ld_o + static_cast<long long>(hk * group + head0 + h) * D + lane * C;
+    uint32_t w[C / 2];
+#pragma unroll
+    for (int c = 0; c < C / 2; ++c) w[c] = sp_pack<T>(acc[2 * c] * inv, acc[2 * c + 1] * inv);
+    if (C == 4) *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1 % (C / 2)]);
+    else *reinterpret_cast<uint32_t*>(o) = w[0];
+  }
+}
+
+}  // namespace rb
+
+namespace {
+
+struct Plan {
+  int tiles, rows, parts, per, seqs, ctas, virtual_heads, own_first;
+  long long places;
+  size_t smem;
+};
+// Two m-tiles where a group has more rows than one takes.
+Plan plan_of(int batch, int heads, int kv_heads, int head_dim, int most_rows) {
+  Plan p;
+  const int group = heads / kv_heads;
+  p.tiles = static_cast<long long>(most_rows) * group > 16 ? 2 : 1;
+  p.rows = 16 * p.tiles;
+  p.parts = (group + p.rows - 1) / p.rows;
+  p.per = (group + p.parts - 1) / p.parts;
+  p.parts = (group + p.per - 1) / p.per;
+  p.seqs = p.rows / p.per;
+  p.virtual_heads = kv_heads * p.parts;
+  const size_t tiles = head_dim == 64 ? (p.tiles == 1 ? rb::SpSmem<64, 1>::kTotals : rb::SpSmem<64, 2>::kTotals)
+                                      : (p.tiles == 1 ? rb::SpSmem<128, 1>::kTotals : rb::SpSmem<128, 2>::kTotals);
+  p.smem = tiles + (3 * static_cast<size_t>(batch) + 1) * 4;
+  const int resident = static_cast<int>((228 * 1024) / (p.smem + 1024 + 64)), most = p.tiles == 1 ? 3 : 2;
+  const int waves = resident < 1 ? 1 : resident < most ? resident : most;
+  const int ctas = rbhost::device_sm_count() * waves / p.virtual_heads;
+  p.ctas = ctas < 1 ? 1 : ctas;
+  // the groups' tiles: entry e of group g has place e / seqs + g
+  p.own_first = batch / p.seqs + batch;
+  p.places = static_cast<long long>(p.own_first) + batch + p.ctas;
+  return p;
+}
+long long totals_bytes(int batch) { return ((2ll * batch + 1) * 4 + 15) / 16 * 16; }
+bool sound(int batch, int heads, int kv_heads, int head_dim, int block_size) {
+  return batch >= 0 && batch <= 8192 && kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && (head_dim == 64 || head_dim == 128) && block_size >= 1;
+}
+
+template <typename T, int D, int MT>
+cudaError_t split(const rb::SpParams& p, const Plan& l, cudaStream_t s) {
+  static size_t configured[64] = {0};
+  const int dev = rbhost::device_slot();
+  if (configured[dev] < l.smem) {
+    const cudaError_t e = cudaFuncSetAttribute(rb::shared_split_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(l.smem));
+    if (e != cudaSuccess) return e;
+    configured[dev] = l.smem;
+  }
+  return rbhost::launch_pdl(rb::shared_split_kernel<T, D, MT>, dim3(l.ctas, l.virtual_heads), dim3(rb::kSpWarps * 32), l.smem, s, 1, p RB_BOUNDS_ARG);
+}
+template <typename T, int D>
+cudaError_t both(const rb::SpParams& p, const Plan& l, cudaStream_t s) {
+  const cudaError_t e = l.tiles == 1 ? split<T, D, 1>(p, l, s) : split<T, D, 2>(p, l, s);
+  if (e != cudaSuccess) return e;
+  return rbhost::launch_pdl(rb::shared_join_kernel<T, D>, dim3(p.batch, l.virtual_heads), dim3(rb::kSpWarps * 32), 0, s, 1, p);
+}
+
+}  // namespace
+
+RB_API long long rb_shared_prefix_scratch_bytes(int batch, int heads, int kv_heads, int head_dim, int block_size, int most_rows) {
+  if (!sound(batch, heads, kv_heads, head_dim, block_size) || batch == 0) return 16;
+  const Plan l = plan_of(batch, heads, kv_heads, head_dim, most_rows);
+  return totals_bytes(batch) + l.places * l.virtual_heads * l.rows * (head_dim + 2) * 4;
+}
+
+RB_API int rb_shared_prefix(const RbSharedPrefixArgs* a, void* stream) {
+  if (!a || !sound(a->batch, a->heads, a->kv_heads, a->head_dim, a->block_size)) return -1;
+  if (a->batch == 0) return 0;
+  if (!a->q || !a->out || !a->k_cache || !a->v_cache || !a->block_tables || !a->context_lens || !a->shared_lens || !a->starts || !a->group_of || !a->scratch ||
+      a->groups < 1 || a->groups > a->batch || a->max_blocks < 1 || a->num_blocks < 1 || a->type < 0 || a->type > 1 || a->most_rows < 1 || a->most_rows > a->batch)
+    return -1;
+  if ((reinterpret_cast<unsigned long long>(a->q) | reinterpret_cast<unsigned long long>(a->out) | reinterpret_cast<unsigned long long>(a->k_cache) |
+       reinterpret_cast<unsigned long long>(a->v_cache)) & 15 || a->ld_q % 8 || a->ld_o % 8)
+    return -2;
+  const long long cap = static_cast<long long>(a->max_blocks) * a->block_size;
+  if (a->num_blocks * a->block_size > 0x7fffffffll || cap > (1ll << 30) || 2 * a->batch * ((cap + rb::kSpUnit - 1) / rb::kSpUnit) > 0x7fffffffll) return -3;
+  const Plan l = plan_of(a->batch, a->heads, a->kv_heads, a->head_dim, a->most_rows);
+  if (l.smem > 227 * 1024 || l.virtual_heads > 65535) return -3;
+  rb::SpParams p;
+  p.q = a->q; p.out = a->out; p.k = a->k_cache; p.v = a->v_cache;
+  p.tables = a->block_tables; p.lens = a->context_lens; p.shared = a->shared_lens; p.starts = a->starts; p.group_of = a->group_of;
+  p.totals = static_cast<int*>(a->scratch);
+  p.partial = reinterpret_cast<float*>(static_cast<char*>(a->scratch) + totals_bytes(a->batch));
+  p.ld_q = a->ld_q; p.ld_o = a->ld_o; p.num_blocks = a->num_blocks;
+  p.batch = a->batch; p.groups = a->groups; p.width = a->max_blocks; p.block_size = a->block_size; p.heads = a->heads; p.kv_heads = a->kv_heads;
+  p.per = l.per; p.parts = l.parts; p.seqs = l.seqs; p.cap = static_cast<int>(cap); p.rows = l.rows; p.own_first = l.own_first; p.ctas = l.ctas;
+  p.scale2 = a->scale * rb::kSpLog2e;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (a->type == 0) e = a->head_dim == 64 ? both<__nv_bfloat16, 64>(p, l, s) : both<__nv_bfloat16, 128>(p, l, s);
+  else e = a->head_dim == 64 ? both<__half, 64>(p, l, s) : both<__half, 128>(p, l, s);
+  return static_cast<int>(e);
+}

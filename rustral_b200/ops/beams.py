@@ -1,0 +1,338 @@
+"""Several continuations of one prompt: selection of beams, states in the order of the selected, copied blocks of a cache, attention over what they share.
+
+`beam_select` chooses the best continuations over beams and vocabulary.  What the chosen beams inherit moves in one of two ways: dense states (caches
+[batch, ...], recurrent cells) take the selection's order in place with `reorder_rows_`; sequences of a paged cache share their full pages
+(`serve.kv_cache.PagedCache.fork`) and only the page that is still filling is copied, in all layers by one `copy_blocks_`.  `paged_attention_shared` is
+decode attention for sequences that share their first tokens, whose keys and values are then read once for all of them.
+"""
+from __future__ import annotations
+
+import functools
+import math
+import struct
+from array import array
+
+import torch
+
+from .. import _native as N
+
+C = N.C
+MOST_COUNT, MOST_BEAMS, MOST_GROUP, MOST_SEQUENCES = 128, 256, 256, 8192
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+# The argument blocks of csrc/kernels/beam.h, move_rows.h and shared_prefix.h, packed
+_SELECT = struct.Struct("@7Pq6i")                # logits, scores, ended, out scores, rows, tokens, scratch; pitch; groups, beams, vocab, count, type, end token
+_MOVE = struct.Struct("@P4q2i")                  # base; outer, row and segment stride, segment bytes; outer, segments
+_SHARED = struct.Struct("@10P3q9if")             # q, out, caches, tables, lengths, shared, starts, group of, scratch; pitches, blocks; sizes; scale
+
+N.optional_sig("rb_beam_select", [C.c_char_p, N.c_void_p])
+N.optional_sig("rb_beam_select_scratch_bytes", [N.c_int] * 5, N.c_ll)
+N.optional_sig("rb_move_blocks", [C.c_char_p, N.c_int, N.c_void_p, N.c_void_p, N.c_int, N.c_int, N.c_void_p])
+N.optional_sig("rb_move_reorder", [C.c_char_p, N.c_int, N.c_void_p, N.c_int, N.c_int, N.c_void_p])
+N.optional_sig("rb_shared_prefix", [C.c_char_p, N.c_void_p])
+N.optional_sig("rb_shared_prefix_scratch_bytes", [N.c_int] * 6, N.c_ll)
+N._LAUNCHES["rb_beam_select"] = N._LAUNCHES["rb_shared_prefix"] = 2
+
+
+def _here(what: str, dev: int, *tensors) -> None:
+    """All tensors are on the device `dev`, which on a GPU is the current one."""
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{what}: tensors on different devices")
+    if dev >= 0 and dev != torch._C._cuda_getDevice():
+        raise ValueError(f"{what}: the tensors are not on the current device")
+
+
+# ---- selection ---------------------------------------------------------------------------------------------------------------------------
+@functools.lru_cache(4096)
+def _select_bytes(*sizes) -> int:
+    return N.kernels().rb_beam_select_scratch_bytes(*sizes)
+
+
+def beam_select(logits, scores, count: int, ended=None, end_token: int = 0):
+    """The `count` best continuations of every group of beams.  logits [groups * beams, vocab] (bf16, fp16 or fp32; row-strided views allowed, such as the
+    real columns of a padded vocabulary), scores fp32 [groups, beams]: the sums of the beams' logarithmic probabilities.  Continuing row r by token t gives
+    scores[r] + log_softmax(logits[r])[t].  Where `ended` (bool [groups, beams]) is true a beam has one continuation, `end_token` at its own score.
+
+    Returns (scores fp32, rows int64, tokens int64), each [groups, count] in descending order of the scores; rows index `logits`.  Equal scores go to the lowest row,
+    then the lowest token.  Sums are compared in 64 bits and rounded once.  Minus infinity is a token that is not allowed (or a beam that is not there), and NaN
+    counts as that; plus infinity counts as the largest fp32 number.  Fewer continuations than `count`: the remaining places have minus infinity and the group's first
+    (row, token) pairs that are not among the continuations.  On a GPU: up to 256 beams and a count of up to 128."""
+    if logits.dim() != 2 or scores.dim() != 2 or logits.dtype not in _TYPES or scores.dtype is not torch.float32 or not scores.is_contiguous():
+        raise TypeError("beam_select: logits [groups * beams, vocab] in bf16, fp16 or fp32 and contiguous fp32 scores [groups, beams] are required")
+    (rows, vocab), (groups, beams) = logits.shape, scores.shape
+    if rows != groups * beams or beams < 1 or vocab < 1:
+        raise ValueError(f"beam_select: {rows} rows of {vocab} logits for {groups} groups of {beams} beams")
+    if not 1 <= count <= beams * vocab:
+        raise ValueError(f"beam_select: {count} of {beams} x {vocab} continuations")
+    if ended is not None:
+        if ended.dtype is not torch.bool or ended.shape != scores.shape or not ended.is_contiguous():
+            raise TypeError("beam_select: ended is a contiguous bool tensor of the scores' shape")
+        if not 0 <= end_token < vocab:
+            raise ValueError(f"beam_select: no token {end_token} in a vocabulary of {vocab}")
+    dev = logits.get_device()
+    _here("beam_select", dev, scores, ended)
+    if dev < 0:
+        return _select_cpu(logits, scores, count, ended, end_token)
+    if beams > MOST_BEAMS or count > MOST_COUNT or vocab > 1 << 26:
+        raise ValueError(f"beam_select: up to {MOST_BEAMS} beams, a count of up to {MOST_COUNT} and 2^26 tokens are served")
+    if logits.stride(1) != 1 or logits.stride(0) < vocab:
+        logits = logits.contiguous()
+    out_scores = torch.empty((groups, count), dtype=torch.float32, device=logits.device)
+    out = torch.empty((2, groups, count), dtype=torch.int64, device=logits.device)
+    kind = _TYPES[logits.dtype]
+    scratch = torch.empty(_select_bytes(groups, beams, vocab, count, kind), dtype=torch.uint8, device=logits.device)
+    at = out.data_ptr()
+    N.check(N.kernels().rb_beam_select(
+        _SELECT.pack(logits.data_ptr(), scores.data_ptr(), 0 if ended is None else ended.data_ptr(), out_scores.data_ptr(), at, at + 8 * groups * count,
+                     scratch.data_ptr(), logits.stride(0), groups, beams, vocab, count, kind, end_token), N.stream_ptr()), "rb_beam_select")
+    return out_scores, out[0], out[1]
+
+
+def _clean(x):
+    x = x.double()
+    return torch.where(x.isnan(), -math.inf, x.clamp(max=torch.finfo(torch.float32).max))
+
+
+def _select_cpu(logits, scores, count, ended, end_token):
+    groups, beams = scores.shape
+    x, s = _clean(logits), _clean(scores)
+    most = x.amax(1, keepdim=True)
+    x = x - torch.where(most == -math.inf, 0.0, most)
+    total = s[..., None] + (x - x.exp().sum(1, keepdim=True).log()).view(groups, beams, logits.shape[1])
+    total = torch.where(total.isnan(), -math.inf, total)               # rows without a token that is allowed
+    if ended is not None:
+        total = total.masked_fill(ended[..., None], -math.inf)
+        total[:, :, end_token] = torch.where(ended, s, total[:, :, end_token])
+    best = torch.sort(total.view(groups, beams * logits.shape[1]), dim=1, descending=True, stable=True)
+    at, vocab = best.indices[:, :count], logits.shape[1]
+    return best.values[:, :count].float(), torch.arange(groups)[:, None] * beams + at // vocab, at % vocab
+
+
+# ---- moves -----------------------------------------------------------------------------------------------------------------------------------
+def _row(what: str, t, dim: int) -> tuple:
+    """(rows, and how they lie in memory: outer stride, row stride, segment stride, segment bytes, outer, segments) of the rows of `t` along `dim`."""
+    shape, size = t.shape, t.element_size()
+    if not 0 <= dim < len(shape):
+        raise ValueError(f"{what}: a tensor of shape {tuple(shape)} has no rows along dimension {dim}")
+    rows = shape[dim]
+    if t.is_contiguous():
+        row = math.prod(shape[dim + 1:]) * size
+        return rows, rows * row, row, 0, row, math.prod(shape[:dim]), 1
+    stride = t.stride()
+
+    def merged(dims):
+        """(length, stride) of these dimensions, neighbours that lie behind one another made one."""
+        out = []
+        for d in dims:
+            if shape[d] == 1:
+                continue
+            if out and out[-1][1] == stride[d] * shape[d]:
+                out[-1] = (out[-1][0] * shape[d], stride[d])
+            else:
+                out.append((shape[d], stride[d]))
+        return out
+
+    outer, inner = merged(range(dim)), merged(range(dim + 1, len(shape)))
+    if inner and inner[-1][1] == 1:
+        piece, inner = inner[-1][0], inner[:-1]
+    else:
+        piece = 1
+    if len(outer) > 1 or len(inner) > 1 or any(s <= 0 for _, s in outer + inner) or (rows > 1 and stride[dim] <= 0):
+        raise ValueError(f"{what}: the rows of a tensor of shape {tuple(shape)} and strides {tuple(stride)} are not pieces at equal distances")
+    n, far = outer[0] if outer else (1, 0)
+    segs, apart = inner[0] if inner else (1, 0)
+    return rows, far * size, (stride[dim] if rows > 1 else 0) * size, apart * size, piece * size, n, segs
+
+
+def _rows(what: str, tensors, dim: int) -> tuple:
+    """(device, rows, packed descriptions, how many) of the tensors of a call; those without elements are left out."""
+    dev, rows, packed, seen = None, None, [], set()
+    for t in tensors:
+        d, at = t.get_device(), t.data_ptr()
+        if dev is None:
+            dev = d
+        elif dev != d:
+            raise ValueError(f"{what}: tensors on different devices")
+        n, *lies = _row(what, t, dim)
+        if rows is None:
+            rows = n
+        elif rows != n:
+            raise ValueError(f"{what}: tensors of {rows} and of {n} rows")
+        if t.numel():
+            if at in seen:
+                raise ValueError(f"{what}: tensors that share memory")
+            seen.add(at)
+            packed.append(_MOVE.pack(at, *lies))
+    if dev is not None and dev >= 0 and dev != torch._C._cuda_getDevice():
+        raise ValueError(f"{what}: the tensors are not on the current device")
+    return dev, rows, b"".join(packed), len(packed)
+
+
+def copy_blocks_(tensors, src, dst, dim: int = 0) -> None:
+    """Copies blocks in place: t[dst[i]] <- t[src[i]] along dimension `dim` of every tensor (one number of blocks for all of them; other sizes, types and strides may
+    differ).  src and dst are numbers on the host (lists or the like); the call refuses blocks that are not there, a destination twice, and a destination that is a source
+    too, before it copies anything.  The tensors share no memory.  A CUDA graph keeps the numbers that it was captured with."""
+    try:
+        src, dst = array("i", src), array("i", dst)
+    except (TypeError, OverflowError) as e:
+        raise ValueError("copy_blocks_: src and dst are lists of block numbers") from e
+    if len(src) != len(dst):
+        raise ValueError(f"copy_blocks_: {len(src)} sources and {len(dst)} destinations")
+    dev, rows, packed, count = _rows("copy_blocks_", tensors, dim)
+    if rows is None:
+        return
+    if dev >= 0:
+        code = N.kernels().rb_move_blocks(packed, count, src.buffer_info()[0], dst.buffer_info()[0], len(src), rows, N.stream_ptr())
+    else:
+        code = -2 if src and not (0 <= min(src) and max(src) < rows and 0 <= min(dst) and max(dst) < rows) else \
+            -3 if len(set(dst)) != len(dst) else 0 if set(dst).isdisjoint(src) else -4
+    if code in _BLOCKS_REFUSED:
+        raise ValueError("copy_blocks_: " + _BLOCKS_REFUSED[code])
+    if dev >= 0:
+        N.check(code, "rb_move_blocks")
+    elif src:
+        of, to = torch.tensor(src, dtype=torch.int64), torch.tensor(dst, dtype=torch.int64)
+        for t in tensors:
+            bits = _bits(t)
+            bits.index_copy_(dim, to, bits.index_select(dim, of))
+
+
+_BLOCKS_REFUSED = {-2: "a block that is not there", -3: "a destination twice", -4: "a destination that is a source too"}
+
+
+def _bits(t):
+    return t.view(torch.uint8) if t.element_size() == 1 and t.dtype is not torch.bool else t
+
+
+def reorder_rows_(tensors, index, dim: int = 0, group: int | None = None) -> None:
+    """Rows in a new order, in place: t[i] <- what t[index[i]] was, along dimension `dim` of every tensor (one number of rows for all; other sizes, types and strides
+    may differ).  index: int64 [rows] on the tensors' device, any map.  `group`: rows come in groups of that many, as the beams of several prompts do, and indices stay
+    in their row's group (None: all rows are one); an index that does not leaves its row as it is.  On a GPU a group has up to 256 rows.  The tensors share no
+    memory."""
+    dev, rows, packed, count = _rows("reorder_rows_", tensors, dim)
+    if rows is None:
+        return
+    if index.dtype is not torch.int64 or index.dim() != 1 or not index.is_contiguous():
+        raise TypeError("reorder_rows_: index is a contiguous int64 vector")
+    if index.shape[0] != rows:
+        raise ValueError(f"reorder_rows_: {index.shape[0]} indices for {rows} rows")
+    group = max(rows, 1) if group is None else group
+    if group < 1 or rows % group:
+        raise ValueError(f"reorder_rows_: {rows} rows in groups of {group}")
+    if index.get_device() != dev:
+        raise ValueError("reorder_rows_: tensors on different devices")
+    if dev < 0:
+        first = torch.arange(rows) // group * group
+        safe = torch.where((index >= first) & (index < first + group), index, torch.arange(rows))
+        for t in tensors:
+            bits = _bits(t)
+            bits.copy_(bits.index_select(dim, safe))
+        return
+    if group > MOST_GROUP:
+        raise ValueError(f"reorder_rows_: groups of up to {MOST_GROUP} rows are served")
+    if rows and count:
+        N.check(N.kernels().rb_move_reorder(packed, count, index.data_ptr(), rows, group, N.stream_ptr()), "rb_move_reorder")
+
+
+# ---- attention over a shared prefix ------------------------------------------------------------------------------------------------------------
+class PrefixGroups:
+    """Which sequences of a batch share their first tokens: group i is the next `sizes[i]` sequences.  A program keeps one for as long as the batch is made up
+    like this; the lengths are tensors of the calls."""
+
+    def __init__(self, sizes, device="cpu"):
+        self.sizes = tuple(int(n) for n in sizes)
+        if any(n < 1 for n in self.sizes):
+            raise ValueError("PrefixGroups: every group has a sequence")
+        self.batch, self.most = sum(self.sizes), max(self.sizes, default=0)
+        starts = [0]
+        for n in self.sizes:
+            starts.append(starts[-1] + n)
+        both = torch.tensor(starts + [g for g, n in enumerate(self.sizes) for _ in range(n)], dtype=torch.int32).to(device)
+        self.starts, self.group_of = both[:len(starts)], both[len(starts):]
+
+    def __len__(self) -> int:
+        return len(self.sizes)
+
+
+@functools.lru_cache(4096)
+def _shared_bytes(*sizes) -> int:
+    return N.kernels().rb_shared_prefix_scratch_bytes(*sizes)
+
+
+def shared_supported(q, k_cache, v_cache) -> bool:
+    """Whether `paged_attention_shared` takes these operands (q [batch, heads * head_dim])."""
+    if not q.is_cuda:
+        return True
+    return q.dtype in (torch.bfloat16, torch.float16) and q.dtype is k_cache.dtype is v_cache.dtype and k_cache.shape == v_cache.shape and \
+        k_cache.shape[3] in (64, 128) and k_cache.is_contiguous() and v_cache.is_contiguous() and q.shape[0] <= MOST_SEQUENCES
+
+
+def paged_attention_shared(q, k_cache, v_cache, groups: PrefixGroups, shared_lens, block_tables, context_lens, scale=None, out=None):
+    """Decode attention for sequences that share their first tokens.  q [batch, heads * head_dim] (row-strided views allowed); caches
+    [blocks, block_size, kv_heads, head_dim]; block_tables int32 [batch, width], context_lens int32 [batch] as for decode attention; shared_lens int32
+    [groups]: the first tokens of a group's sequences that are the same.  Those are read once for the whole group, through the table of its first sequence, what follows through
+    each sequence's own.  Where the shortest sequence of a group has fewer tokens (those without any aside) only that many count as shared.  A sequence without tokens
+    gets zeros.  Returns [batch, heads * head_dim].
+
+    On a GPU: bf16 or fp16, heads of 64 or 128, up to 8192 sequences.  A sequence's result depends, within rounding, on the batch it is in; the same call gives the
+    same bits."""
+    if q.dim() != 2 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or not q.dtype is k_cache.dtype is v_cache.dtype or \
+            not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise TypeError("paged_attention_shared: q [batch, heads * head_dim] and contiguous caches [blocks, block_size, kv_heads, head_dim] of its type are required")
+    nb, bs, hk, d = k_cache.shape
+    batch, width = q.shape
+    heads = width // d
+    if batch != groups.batch or width != heads * d or heads % hk or heads == 0:
+        raise ValueError(f"paged_attention_shared: q of {tuple(q.shape)} for {groups.batch} sequences and {hk} KV heads of {d}")
+    if not (block_tables.dtype is context_lens.dtype is shared_lens.dtype is torch.int32 and block_tables.dim() == 2 and block_tables.is_contiguous() and
+            context_lens.is_contiguous() and shared_lens.is_contiguous()) or \
+            not (block_tables.shape[0] == batch and context_lens.shape == (batch,) and shared_lens.shape == (len(groups),)):
+        raise TypeError("paged_attention_shared: contiguous int32 tables and lengths of every sequence and shared lengths of every group are required")
+    if out is not None and (out.dtype is not q.dtype or out.shape != q.shape):
+        raise TypeError("paged_attention_shared: out has the shape and type of q")
+    dev = q.get_device()
+    _here("paged_attention_shared", dev, k_cache, v_cache, groups.starts, shared_lens, block_tables, context_lens, out)
+    scale = 1.0 / math.sqrt(d) if scale is None else scale
+    if dev < 0:
+        r = _shared_cpu(q, k_cache, v_cache, groups, shared_lens, block_tables, context_lens, scale)
+        return r if out is None else out.copy_(r)
+    kind = _TYPES[q.dtype]
+    if kind > 1 or d not in (64, 128) or batch > MOST_SEQUENCES:
+        raise ValueError(f"paged_attention_shared: bf16 or fp16, heads of 64 or 128 and up to {MOST_SEQUENCES} sequences are served, not {q.dtype}, {d} and {batch}")
+    if batch == 0 or block_tables.shape[1] == 0 or nb == 0 or bs == 0:
+        return torch.zeros_like(q) if out is None else out.zero_()
+    if nb * bs > 2 ** 31 - 1 or block_tables.shape[1] * bs > 1 << 30:
+        raise ValueError("paged_attention_shared: caches of fewer than 2^31 tokens and tables of up to 2^30 are served")
+    if q.stride(1) != 1 or q.stride(0) & 7 or q.data_ptr() & 15:
+        q = q.clone(memory_format=torch.contiguous_format)
+    res = out
+    if out is None or out.stride(1) != 1 or out.stride(0) & 7 or out.data_ptr() & 15:
+        res = torch.empty((batch, width), dtype=q.dtype, device=q.device)
+    scratch = torch.empty(_shared_bytes(batch, heads, hk, d, bs, groups.most), dtype=torch.uint8, device=q.device)
+    N.check(N.kernels().rb_shared_prefix(
+        _SHARED.pack(q.data_ptr(), res.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), shared_lens.data_ptr(),
+                     groups.starts.data_ptr(), groups.group_of.data_ptr(), scratch.data_ptr(), q.stride(0), res.stride(0), nb,
+                     batch, len(groups), block_tables.shape[1], bs, heads, hk, d, kind, groups.most, scale), N.stream_ptr()), "rb_shared_prefix")
+    return res if out is None or res is out else out.copy_(res)
+
+
+def _shared_cpu(q, k_cache, v_cache, groups, shared_lens, block_tables, context_lens, scale):
+    nb, bs, hk, d = k_cache.shape
+    batch, heads = q.shape[0], q.shape[1] // d
+    out = torch.zeros(batch, heads * d)
+    cap, first = block_tables.shape[1] * bs, 0
+    for g, size in enumerate(groups.sizes):
+        lens = [min(max(int(n), 0), cap) for n in context_lens[first:first + size]]
+        shared = min([max(int(shared_lens[g]), 0)] + [n for n in lens if n])
+        for b, n in enumerate(lens, first):
+            if n == 0:
+                continue
+            at = torch.arange(n)
+            pages = torch.where(at < shared, block_tables[first, at // bs], block_tables[b, at // bs]).long()
+            pages = torch.where((pages >= 0) & (pages < nb), pages, 0)
+            k, v = (t[pages, at % bs].float() for t in (k_cache, v_cache))          # [n, kv heads, d]
+            s = torch.einsum("hgd,nhd->hgn", q[b].float().view(hk, -1, d), k) * scale
+            out[b] = torch.einsum("hgn,nhd->hgd", torch.softmax(s, -1), v).reshape(-1)
+        first += size
+    return out.to(q.dtype)
