@@ -7,45 +7,20 @@
 //
 // Work is a list of entries (a tile of a group's rows over its shared tokens, a sequence's rows over its own), cut into units of 128 tokens; the units of all entries,
 // one behind the other, are dealt in equal runs to CTAs that stay.  An entry's rows are accumulated over all units of a run, so there are at most (entries +
-// CTAs) partial results, whose places follow from the entry's number and the CTA's: entry k and CTA c use place k + c, which is unique, because
-// from one (entry, CTA) of the list to the next one of the two grows.  Every CTA forms the list of running totals itself from the lengths.
+// CTAs) parts: the one that begins an entry has a place of the entry's own, one that goes on with it is the first of its CTA's run and has the CTA's.  Every CTA forms the
+// list of running totals itself from the lengths.
 //
 // This file's split kernel is for few rows (up to 32): the rows are one or two m16n8k16 tiles, a warp takes 32 of a unit's tokens, keys and values come
 // by 16-byte asynchronous copies into tiles of its own.  It is bound by these reads.
 #include "shared_prefix.h"
 
-#include <cuda_fp16.h>
-#include <limits.h>
+#include <string.h>
 
-#include "pdl.cuh"
-#include "warp_mma.cuh"
+#include "shared_prefix.cuh"
 
 namespace rb {
 
 constexpr int kSpWarps = 4;
-constexpr int kSpUnit = 128;                     // tokens
-constexpr float kSpLog2e = 1.4426950408889634f;
-
-struct SpParams {
-  const void* q;
-  void* out;
-  const void* k;
-  const void* v;
-  const int* tables;
-  const int* lens;
-  const int* shared;
-  const int* starts;
-  const int* group_of;
-  int* totals;                                   // [2 batch + 1] running totals of units, for the join
-  float* partial;
-  long long ld_q, ld_o, num_blocks;
-  int batch, groups, width, block_size, heads, kv_heads, per, parts, seqs, cap;
-  // per: query heads of a virtual KV head (a KV head's group in `parts` equal parts, so that a sequence's rows fit a tile); seqs: sequences of a tile; cap: tokens of a table's row
-  int rows;                                      // of a tile
-  int own_first;                                 // place of the first own entry among the entries
-  int ctas;                                      // along x
-  float scale2;                                  // scale * log2(e)
-};
 
 template <typename T>
 __device__ __forceinline__ void sp_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -57,85 +32,6 @@ __device__ __forceinline__ void sp_mma<__half>(float (&c)[4], const uint32_t (&a
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename T>
-__device__ __forceinline__ uint32_t sp_pack(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t sp_pack<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
-template <>
-__device__ __forceinline__ uint32_t sp_pack<__half>(float lo, float hi) {
-  __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-template <typename T>
-__device__ __forceinline__ T sp_round(float v);
-template <>
-__device__ __forceinline__ __nv_bfloat16 sp_round<__nv_bfloat16>(float v) { return __float2bfloat16(v); }
-template <>
-__device__ __forceinline__ __half sp_round<__half>(float v) { return __float2half(v); }
-
-__device__ __forceinline__ int sp_length(const SpParams& p, int b) { return min(max(p.lens[b], 0), p.cap); }
-// What each group's sequences read together: no more tokens than the shortest of them has, those without tokens aside, so that all rows of a tile see all of its
-// tokens.  `shared`: [groups] of the CTA's shared memory.
-__device__ __forceinline__ void sp_shared(const SpParams& p, int* shared) {
-  for (int g = threadIdx.x; g < p.groups; g += blockDim.x) shared[g] = INT_MAX;
-  __syncthreads();
-  for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
-    const int n = sp_length(p, b);
-    if (n > 0) atomicMin(&shared[p.group_of[b]], n);
-  }
-  __syncthreads();
-  for (int g = threadIdx.x; g < p.groups; g += blockDim.x) {
-    const int n = shared[g];
-    shared[g] = n == INT_MAX ? 0 : min(n, max(p.shared[g], 0));
-  }
-  __syncthreads();
-}
-// Units of entry e: tiles of rows begin at every `seqs`-th sequence of a group.
-__device__ __forceinline__ int sp_units(const SpParams& p, const int* shared_of, int e) {
-  const int b = e < p.batch ? e : e - p.batch, g = p.group_of[b], shared = shared_of[g];
-  if (e < p.batch) return (b - p.starts[g]) % p.seqs == 0 ? (shared + kSpUnit - 1) / kSpUnit : 0;
-  return max(0, sp_length(p, b) - shared + kSpUnit - 1) / kSpUnit;
-}
-// Running totals of the units of all entries, [2 batch + 1], formed by all threads of a CTA.
-__device__ __forceinline__ void sp_totals(const SpParams& p, const int* shared_of, int* totals, int* warp_sums) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  int before = 0;
-  if (threadIdx.x == 0) totals[0] = 0;
-  for (int first = 0; first < 2 * p.batch; first += blockDim.x) {
-    const int e = first + threadIdx.x;
-    int upto = e < 2 * p.batch ? sp_units(p, shared_of, e) : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    if (lane == 31) warp_sums[warp] = upto;
-    __syncthreads();
-    int all = 0;
-    for (int w = 0; w < warps; ++w) {
-      const int s = warp_sums[w];
-      if (w < warp) upto += s;
-      all += s;
-    }
-    if (e < 2 * p.batch) totals[e + 1] = before + upto;
-    before += all;
-    __syncthreads();
-  }
-}
-// First unit of CTA c's run, and the CTA that has unit u.
-__device__ __forceinline__ int sp_run(int total, int ctas, int c) {
-  const int share = total / ctas, over = total - share * ctas;
-  return c * share + min(c, over);
-}
-__device__ __forceinline__ int sp_cta_of(int total, int ctas, int u) {
-  const int share = total / ctas, over = total - share * ctas, wide = over * (share + 1);
-  return u < wide ? u / (share + 1) : over + (u - wide) / share;
-}
-// Place of an entry among those that have partial results; grows with e.
-__device__ __forceinline__ int sp_place(const SpParams& p, int e) {
-  return e < p.batch ? e / p.seqs + p.group_of[e] : p.own_first + e - p.batch;
-}
-
 template <int D, int MT>
 struct SpSmem {
   static constexpr int kRow = D + 8;             // padded rows (elements): ldmatrix rows hit distinct banks
@@ -159,44 +55,30 @@ shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
   float2* ml_sh = reinterpret_cast<float2*>(sp_mem + L::kMl);           // [warp][row]: maximum, sum
   int* totals = reinterpret_cast<int*>(sp_mem + L::kTotals);
   const uint32_t q_u32 = smem_u32(q_sh), k_u32 = smem_u32(sp_mem) + warp * 2 * L::kTile * 2, v_u32 = k_u32 + L::kTile * 2;
-  int* shared_of = totals + 2 * p.batch + 1;
+  const SpList& list = p.list;
+  int* shared_of = totals + list.entries + 1;
   sp_shared(p, shared_of);
-  sp_totals(p, shared_of, totals, warp_sums);
-  const int entries = 2 * p.batch, total = totals[entries];
-  const int vh = blockIdx.y, hk = vh / p.parts, head0 = (vh - hk * p.parts) * p.per;
-  const int group = p.heads / p.kv_heads, per = min(p.per, group - head0);
-  if (blockIdx.x == 0 && blockIdx.y == 0)
-    for (int i = threadIdx.x; i <= entries; i += blockDim.x) p.totals[i] = totals[i];
-  int u = sp_run(total, gridDim.x, blockIdx.x);
-  const int u_end = sp_run(total, gridDim.x, blockIdx.x + 1);
-  if (u >= u_end) return;
-  // the entry that has unit u: the last one that begins at or in front of it
-  int e = 0;
-  for (int hi = entries; hi - e > 1;) {
-    const int mid = (e + hi) >> 1;
-    if (totals[mid] <= u) e = mid;
-    else hi = mid;
-  }
+  sp_totals(p, list, shared_of, totals, warp_sums);
+  const int total = totals[list.entries] * list.virtual_heads, group = p.heads / p.kv_heads;
+  int u = sp_run(total, list.ctas, blockIdx.x);
+  const int u_end = sp_run(total, list.ctas, blockIdx.x + 1);
   const T* K = static_cast<const T*>(p.k);
   const T* V = static_cast<const T*>(p.v);
 
   while (u < u_end) {
-    while (totals[e + 1] <= u) ++e;
-    // ---- this entry's rows and tokens
-    const bool own = e >= p.batch;
-    const int b = own ? e - p.batch : e, g = p.group_of[b], shared = shared_of[g];
-    const int rows = own ? per : min(p.seqs, p.starts[g + 1] - b) * per;
-    const int first = own ? shared : 0, count = own ? sp_length(p, b) - shared : shared;
-    const int* table = p.tables + static_cast<long long>(own ? b : p.starts[g]) * p.width;
-    const int u0 = u - totals[e], u1 = min(u_end, totals[e + 1]) - totals[e];
+    // ---- this part's rows and tokens
+    const SpPart s_ = sp_next(p, list, totals, u, u_end);
+    const int hk = s_.vh / list.parts, head0 = (s_.vh - hk * list.parts) * list.per, per = list.per, real = min(per, group - head0);
+    const int b = s_.b, rows = s_.n * per, shared = shared_of[s_.g], u0 = s_.u0, u1 = s_.u1;
+    const int first = s_.own ? shared : 0, count = s_.own ? sp_length(p, b) - shared : shared;
+    const int* table = p.tables + static_cast<long long>(s_.own ? b : p.starts[s_.g]) * p.width;
     __syncthreads();                             // the last entry's queries and results have been read
     for (int i = threadIdx.x; i < kRows * LP; i += blockDim.x) {
       const int r = i / LP, c = (i - r * LP) * 8;
       uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (r < rows) {
-        const int s = r / per;
-        x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (b + s) * p.ld_q + static_cast<long long>(hk * group + head0 + r - s * per) * D + c);
-      }
+      const int s = r / per, h = r - s * per;
+      if (r < rows && h < real)
+        x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (b + s) * p.ld_q + static_cast<long long>(hk * group + head0 + h) * D + c);
       *reinterpret_cast<uint4*>(q_sh + r * kRow + c) = x;
     }
     __syncthreads();
@@ -227,6 +109,7 @@ shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
       }
       wm_cp_commit();
     };
+    const float scale2 = p.scale * kSpLog2e;
     float m[MT][2], l[MT][2], acc[MT][NT][4];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
@@ -282,7 +165,7 @@ shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
                 float& x = s[t][n][2 * i + j];
-                x = n * 8 + 2 * tq + j < n_tok ? x * p.scale2 : -INFINITY;
+                x = n * 8 + 2 * tq + j < n_tok ? x * scale2 : -INFINITY;
                 mx = fmaxf(mx, x);
               }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -343,8 +226,7 @@ shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
       }
     }
     __syncthreads();
-    const long long place = static_cast<long long>(sp_place(p, e) + blockIdx.x) * gridDim.y + vh;
-    float* part = p.partial + place * kRows * (D + 2);
+    const long long row0 = sp_row(list, s_.vh, s_.e, blockIdx.x, u0 == 0);
     for (int i = threadIdx.x; i < rows * (D / 4); i += blockDim.x) {
       const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
       float mx = -INFINITY;
@@ -360,43 +242,46 @@ shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
         sum.x = fmaf(x.x, f, sum.x); sum.y = fmaf(x.y, f, sum.y); sum.z = fmaf(x.z, f, sum.z); sum.w = fmaf(x.w, f, sum.w);
         den = fmaf(ml.y, f, den);
       }
-      *reinterpret_cast<float4*>(part + 2 * kRows + r * D + c) = sum;
-      if (c == 0) *reinterpret_cast<float2*>(part + 2 * r) = make_float2(mx, den);
+      *reinterpret_cast<float4*>(list.acc + (row0 + r) * D + c) = sum;
+      if (c == 0) list.ml[row0 + r] = make_float2(mx, den);
     }
-    u = totals[e] + u1;
   }
 }
 
-// out[b, head] from the partial results of its rows: a warp per head, lanes own D / 32 neighbouring columns.  Grid (batch, virtual KV heads).
+// out[b, head] from the parts of its row: a warp per head, lanes own D / 32 neighbouring columns.  Grid (batch, KV heads).
 template <typename T, int D>
 __global__ void __launch_bounds__(kSpWarps * 32)
 shared_join_kernel(const SpParams p) {
   pdl_wait();
   pdl_launch();
   constexpr int C = D / 32;
-  const int b = blockIdx.x, vh = blockIdx.y, hk = vh / p.parts, head0 = (vh - hk * p.parts) * p.per;
-  const int group = p.heads / p.kv_heads, per = min(p.per, group - head0);
+  const int b = blockIdx.x, hk = blockIdx.y, group = p.heads / p.kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = p.group_of[b], tile = b - (b - p.starts[g]) % p.seqs, total = p.totals[2 * p.batch];
-  // places of the parts: those of the shared tokens, then the sequence's own
-  int at[2], n[2];
+  const int g = p.group_of[b], tile = b - (b - p.starts[g]) % p.prefix.seqs;
+  const bool any = sp_length(p, b) > 0;          // a sequence without tokens gets zeros
+  for (int h = warp; h < group; h += kSpWarps) {
+    // parts over shared tokens, then the sequence's own: how many, the CTA of the first, and the rows where the first and those of CTA 0 are
+    int n[2], c0[2];
+    long long row[2], later[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int e = i == 0 ? tile : p.batch + b, t0 = p.totals[e], t1 = p.totals[e + 1];
-    const int c0 = t1 > t0 ? sp_cta_of(total, p.ctas, t0) : 0;
-    n[i] = t1 > t0 ? sp_cta_of(total, p.ctas, t1 - 1) - c0 + 1 : 0;
-    at[i] = sp_place(p, e) + c0;
-  }
-  const int parts = sp_length(p, b) > 0 ? n[0] + n[1] : 0;              // a sequence without tokens gets zeros
-  for (int h = warp; h < per; h += kSpWarps) {
-    const int r0 = (b - tile) * per + h;
-    auto part_of = [&](int s) {
-      const int i = s >= n[0] ? 1 : 0;
-      return p.partial + (static_cast<long long>(at[i] + s - (i ? n[0] : 0)) * gridDim.y + vh) * p.rows * (D + 2);
+    for (int i = 0; i < 2; ++i) {
+      const SpList& l = i == 0 ? p.prefix : p.list;
+      const int e = i == 0 ? tile : p.batch + b, all = l.totals[l.entries], t0 = l.totals[e], t1 = l.totals[e + 1];
+      const int k = h / l.per, vh = hk * l.parts + k, r = (i == 0 ? b - tile : 0) * l.per + h - k * l.per;
+      c0[i] = t1 > t0 ? sp_cta_of(all * l.virtual_heads, l.ctas, vh * all + t0) : 0;
+      n[i] = any && t1 > t0 ? sp_cta_of(all * l.virtual_heads, l.ctas, vh * all + t1 - 1) - c0[i] + 1 : 0;
+      row[i] = sp_row(l, vh, e, 0, true) + r;
+      later[i] = sp_row(l, vh, e, 0, false) + r;
+    }
+    const int parts = n[0] + n[1];
+    auto row_of = [&](int s) -> long long {
+      const int i = s >= n[0] ? 1 : 0, k = s - (i ? n[0] : 0);
+      const SpList& l = i ? p.list : p.prefix;
+      return k == 0 ? row[i] : later[i] + static_cast<long long>(c0[i] + k) * l.seqs * l.per;
     };
-    auto row_of = [&](int s) { return s >= n[0] ? h : r0; };
+    auto ml_of = [&](int s) { return (s >= n[0] ? p.list.ml : p.prefix.ml)[row_of(s)]; };
     float mx = -INFINITY;
-    for (int s = lane; s < parts; s += 32) mx = fmaxf(mx, part_of(s)[2 * row_of(s)]);
+    for (int s = lane; s < parts; s += 32) mx = fmaxf(mx, ml_of(s).x);
     mx = warp_max(mx);
     float acc[C], den = 0.f;
 #pragma unroll
@@ -404,7 +289,7 @@ shared_join_kernel(const SpParams p) {
     for (int s0 = 0; s0 < parts; s0 += 32) {
       float f = 0.f;
       if (s0 + lane < parts) {
-        const float2 ml = *reinterpret_cast<const float2*>(part_of(s0 + lane) + 2 * row_of(s0 + lane));
+        const float2 ml = ml_of(s0 + lane);
         f = ml.x == -INFINITY ? 0.f : wm_ex2(ml.x - mx);
         den = fmaf(ml.y, f, den);
       }
@@ -412,7 +297,7 @@ shared_join_kernel(const SpParams p) {
 #pragma unroll 4
       for (int s = 0; s < m; ++s) {
         const float fs = __shfl_sync(0xffffffffu, f, s);
-        const float* x = part_of(s0 + s) + 2 * p.rows + row_of(s0 + s) * D + lane * C;
+        const float* x = (s0 + s >= n[0] ? p.list.acc : p.prefix.acc) + row_of(s0 + s) * D + lane * C;
         float v[C];
         if (C == 4) {
           const float4 w = *reinterpret_cast<const float4*>(x);
@@ -427,7 +312,7 @@ shared_join_kernel(const SpParams p) {
     }
     den = warp_sum(den);
     const float inv = parts > 0 ? 1.f / den : 0.f;
-    T* o = static_cast<T*>(p.out) + b * p.ld_o + static_cast<long long>(hk * group + head0 + h) * D + lane * C;
+    T* o = static_cast<T*>(p.out) + b * p.ld_o + static_cast<long long>(hk * group + h) * D + lane * C;
     uint32_t w[C / 2];
 #pragma unroll
     for (int c = 0; c < C / 2; ++c) w[c] = sp_pack<T>(acc[2 * c] * inv, acc[2 * c + 1] * inv);
@@ -441,36 +326,48 @@ shared_join_kernel(const SpParams p) {
 namespace {
 
 struct Plan {
-  int tiles, rows, parts, per, seqs, ctas, virtual_heads, own_first;
-  long long places;
+  rb::SpList list, prefix;
   size_t smem;
+  int tiles;                                     // m-tiles of the split kernel
+  bool tc;
 };
-// Two m-tiles where a group has more rows than one takes.
-Plan plan_of(int batch, int heads, int kv_heads, int head_dim, int most_rows) {
+// Shared tokens of groups with more than 32 rows go to the tcgen05 kernel, which takes 256 at a time; the split kernel has one m-tile, or two where rows need them.
+Plan plan_of(int batch, int heads, int kv_heads, int head_dim, int block_size, int most, bool positive) {
   Plan p;
+  memset(&p, 0, sizeof(p));
   const int group = heads / kv_heads;
-  p.tiles = static_cast<long long>(most_rows) * group > 16 ? 2 : 1;
-  p.rows = 16 * p.tiles;
-  p.parts = (group + p.rows - 1) / p.rows;
-  p.per = (group + p.parts - 1) / p.parts;
-  p.parts = (group + p.per - 1) / p.per;
-  p.seqs = p.rows / p.per;
-  p.virtual_heads = kv_heads * p.parts;
+  p.tc = static_cast<long long>(most) * group > 32 && positive && rbhost::shared_tc_takes(batch, heads, kv_heads, block_size, most);
+  p.tiles = static_cast<long long>(p.tc ? 1 : most) * group > 16 ? 2 : 1;
+  const int rows = 16 * p.tiles;
+  rb::SpList& l = p.list;
+  l.parts = (group + rows - 1) / rows;
+  l.per = (group + l.parts - 1) / l.parts;
+  l.parts = (group + l.per - 1) / l.per;
+  l.seqs = rows / l.per;
+  l.virtual_heads = kv_heads * l.parts;
+  l.entries = 2 * batch;
+  l.skip = p.tc ? batch : 0;
   const size_t tiles = head_dim == 64 ? (p.tiles == 1 ? rb::SpSmem<64, 1>::kTotals : rb::SpSmem<64, 2>::kTotals)
                                       : (p.tiles == 1 ? rb::SpSmem<128, 1>::kTotals : rb::SpSmem<128, 2>::kTotals);
   p.smem = tiles + (3 * static_cast<size_t>(batch) + 1) * 4;
-  const int resident = static_cast<int>((228 * 1024) / (p.smem + 1024 + 64)), most = p.tiles == 1 ? 3 : 2;
-  const int waves = resident < 1 ? 1 : resident < most ? resident : most;
-  const int ctas = rbhost::device_sm_count() * waves / p.virtual_heads;
-  p.ctas = ctas < 1 ? 1 : ctas;
-  // the groups' tiles: entry e of group g has place e / seqs + g
-  p.own_first = batch / p.seqs + batch;
-  p.places = static_cast<long long>(p.own_first) + batch + p.ctas;
+  const int resident = static_cast<int>((228 * 1024) / (p.smem + 1024 + 64)), most_resident = p.tiles == 1 ? 3 : 2;
+  l.ctas = rbhost::device_sm_count() * (resident < 1 ? 1 : resident < most_resident ? resident : most_resident);
+  p.prefix = p.tc ? rbhost::shared_tc_list(batch, heads, kv_heads) : l;
   return p;
 }
-long long totals_bytes(int batch) { return ((2ll * batch + 1) * 4 + 15) / 16 * 16; }
+// Puts a list's arrays at `at` (NULL: only counts) and returns their size.
+long long place(rb::SpList& l, char* at, int head_dim) {
+  const long long totals = ((l.entries + 1) * 4ll + 15) / 16 * 16, rows = rbhost::sp_list_rows(l), ml = (rows * 8 + 15) / 16 * 16;
+  if (at) {
+    l.totals = reinterpret_cast<int*>(at);
+    l.ml = reinterpret_cast<float2*>(at + totals);
+    l.acc = reinterpret_cast<float*>(at + totals + ml);
+  }
+  return totals + ml + rows * head_dim * 4;
+}
 bool sound(int batch, int heads, int kv_heads, int head_dim, int block_size) {
-  return batch >= 0 && batch <= 8192 && kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && (head_dim == 64 || head_dim == 128) && block_size >= 1;
+  return batch >= 0 && batch <= 8192 && kv_heads >= 1 && kv_heads <= 65535 && heads >= kv_heads && heads % kv_heads == 0 && (head_dim == 64 || head_dim == 128) &&
+         block_size >= 1;
 }
 
 template <typename T, int D, int MT>
@@ -482,21 +379,26 @@ cudaError_t split(const rb::SpParams& p, const Plan& l, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     configured[dev] = l.smem;
   }
-  return rbhost::launch_pdl(rb::shared_split_kernel<T, D, MT>, dim3(l.ctas, l.virtual_heads), dim3(rb::kSpWarps * 32), l.smem, s, 1, p RB_BOUNDS_ARG);
+  return rbhost::launch_pdl(rb::shared_split_kernel<T, D, MT>, dim3(l.list.ctas), dim3(rb::kSpWarps * 32), l.smem, s, 1, p RB_BOUNDS_ARG);
 }
 template <typename T, int D>
 cudaError_t both(const rb::SpParams& p, const Plan& l, cudaStream_t s) {
   const cudaError_t e = l.tiles == 1 ? split<T, D, 1>(p, l, s) : split<T, D, 2>(p, l, s);
   if (e != cudaSuccess) return e;
-  return rbhost::launch_pdl(rb::shared_join_kernel<T, D>, dim3(p.batch, l.virtual_heads), dim3(rb::kSpWarps * 32), 0, s, 1, p);
+  return rbhost::launch_pdl(rb::shared_join_kernel<T, D>, dim3(p.batch, p.kv_heads), dim3(rb::kSpWarps * 32), 0, s, 1, p);
 }
 
 }  // namespace
 
 RB_API long long rb_shared_prefix_scratch_bytes(int batch, int heads, int kv_heads, int head_dim, int block_size, int most_rows) {
   if (!sound(batch, heads, kv_heads, head_dim, block_size) || batch == 0) return 16;
-  const Plan l = plan_of(batch, heads, kv_heads, head_dim, most_rows);
-  return totals_bytes(batch) + l.places * l.virtual_heads * l.rows * (head_dim + 2) * 4;
+  long long most = 0;
+  for (int positive = 0; positive < 2; ++positive) {
+    Plan l = plan_of(batch, heads, kv_heads, head_dim, block_size, most_rows, positive != 0);
+    const long long n = place(l.list, nullptr, head_dim) + (l.tc ? place(l.prefix, nullptr, head_dim) : 0);
+    if (n > most) most = n;
+  }
+  return most;
 }
 
 RB_API int rb_shared_prefix(const RbSharedPrefixArgs* a, void* stream) {
@@ -508,20 +410,29 @@ RB_API int rb_shared_prefix(const RbSharedPrefixArgs* a, void* stream) {
   if ((reinterpret_cast<unsigned long long>(a->q) | reinterpret_cast<unsigned long long>(a->out) | reinterpret_cast<unsigned long long>(a->k_cache) |
        reinterpret_cast<unsigned long long>(a->v_cache)) & 15 || a->ld_q % 8 || a->ld_o % 8)
     return -2;
+  Plan l = plan_of(a->batch, a->heads, a->kv_heads, a->head_dim, a->block_size, a->most_rows, a->scale > 0.f);
   const long long cap = static_cast<long long>(a->max_blocks) * a->block_size;
-  if (a->num_blocks * a->block_size > 0x7fffffffll || cap > (1ll << 30) || 2 * a->batch * ((cap + rb::kSpUnit - 1) / rb::kSpUnit) > 0x7fffffffll) return -3;
-  const Plan l = plan_of(a->batch, a->heads, a->kv_heads, a->head_dim, a->most_rows);
-  if (l.smem > 227 * 1024 || l.virtual_heads > 65535) return -3;
+  if (a->num_blocks * a->block_size > 0x7fffffffll || cap > (1ll << 30) ||
+      2ll * a->batch * ((cap + rb::kSpUnit - 1) / rb::kSpUnit) * l.list.virtual_heads > 0x7fffffffll || l.smem > 227 * 1024)
+    return -3;
   rb::SpParams p;
+  memset(&p, 0, sizeof(p));
   p.q = a->q; p.out = a->out; p.k = a->k_cache; p.v = a->v_cache;
   p.tables = a->block_tables; p.lens = a->context_lens; p.shared = a->shared_lens; p.starts = a->starts; p.group_of = a->group_of;
-  p.totals = static_cast<int*>(a->scratch);
-  p.partial = reinterpret_cast<float*>(static_cast<char*>(a->scratch) + totals_bytes(a->batch));
   p.ld_q = a->ld_q; p.ld_o = a->ld_o; p.num_blocks = a->num_blocks;
   p.batch = a->batch; p.groups = a->groups; p.width = a->max_blocks; p.block_size = a->block_size; p.heads = a->heads; p.kv_heads = a->kv_heads;
-  p.per = l.per; p.parts = l.parts; p.seqs = l.seqs; p.cap = static_cast<int>(cap); p.rows = l.rows; p.own_first = l.own_first; p.ctas = l.ctas;
-  p.scale2 = a->scale * rb::kSpLog2e;
+  p.cap = static_cast<int>(cap); p.scale = a->scale;
+  char* at = static_cast<char*>(a->scratch);
+  at += place(l.list, at, a->head_dim);
+  if (l.tc) place(l.prefix, at, a->head_dim);
+  else l.prefix = l.list;
+  p.list = l.list;
+  p.prefix = l.prefix;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (l.tc) {
+    const int e = rbhost::shared_tc(p, a->type, a->head_dim, s);
+    if (e) return e;
+  }
   cudaError_t e;
   if (a->type == 0) e = a->head_dim == 64 ? both<__nv_bfloat16, 64>(p, l, s) : both<__nv_bfloat16, 128>(p, l, s);
   else e = a->head_dim == 64 ? both<__half, 64>(p, l, s) : both<__half, 128>(p, l, s);

@@ -1,0 +1,159 @@
+// What the kernels of decode attention over a shared prefix have in common: the list of units, its division among CTAs, and the places of partial
+// results (shared_prefix.cu, shared_prefix_tc.cu).
+#pragma once
+#include <cuda_fp16.h>
+#include <limits.h>
+
+#include "pdl.cuh"
+#include "warp_mma.cuh"
+
+namespace rb {
+
+constexpr int kSpUnit = 128;                     // tokens
+constexpr float kSpLog2e = 1.4426950408889634f;
+
+// The units of `first` .. entries, for each of the virtual KV heads one after the other, dealt in equal runs to `ctas` CTAs.  Entry e < batch is the tile of
+// rows that begins with sequence e (if one does) over the group's shared tokens, entry batch + b are sequence b's rows over its own.
+struct SpList {
+  int* totals;                                   // [entries + 1] running totals of units
+  float2* ml;                                    // maximum (base 2) and sum of every row's part
+  float* acc;                                    // [part][head_dim]
+  int entries, skip;                             // skip: entries in front that have no units here
+  int per, parts, virtual_heads;                 // a KV head's query heads in `parts` equal parts of `per`, so that a sequence's rows fit a tile
+  int ctas, seqs;                                // seqs: sequences of a tile
+};
+struct SpParams {
+  const void* q;
+  void* out;
+  const void* k;
+  const void* v;
+  const int* tables;
+  const int* lens;
+  const int* shared;
+  const int* starts;
+  const int* group_of;
+  long long ld_q, ld_o, num_blocks;
+  int batch, groups, width, block_size, heads, kv_heads;
+  int cap;                                       // tokens of a table's row
+  float scale;
+  SpList list, prefix;                           // prefix: where the parts over shared tokens are; the same list, or that of the launch in front
+};
+
+__device__ __forceinline__ int sp_length(const SpParams& p, int b) { return min(max(p.lens[b], 0), p.cap); }
+// What each group's sequences read together: no more tokens than the shortest of them has, those without tokens aside, so that all rows of a tile see all of its
+// tokens.  `shared`: [groups] of the CTA's shared memory.
+__device__ __forceinline__ void sp_shared(const SpParams& p, int* shared) {
+  for (int g = threadIdx.x; g < p.groups; g += blockDim.x) shared[g] = INT_MAX;
+  __syncthreads();
+  for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
+    const int n = sp_length(p, b);
+    if (n > 0) atomicMin(&shared[p.group_of[b]], n);
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g < p.groups; g += blockDim.x) {
+    const int n = shared[g];
+    shared[g] = n == INT_MAX ? 0 : min(n, max(p.shared[g], 0));
+  }
+  __syncthreads();
+}
+// Units of entry e: tiles of rows begin at every `seqs`-th sequence of a group.
+__device__ __forceinline__ int sp_units(const SpParams& p, const SpList& l, const int* shared_of, int e) {
+  if (e < l.skip) return 0;
+  const int b = e < p.batch ? e : e - p.batch, g = p.group_of[b], shared = shared_of[g];
+  if (e < p.batch) return (b - p.starts[g]) % l.seqs == 0 ? (shared + kSpUnit - 1) / kSpUnit : 0;
+  return max(0, sp_length(p, b) - shared + kSpUnit - 1) / kSpUnit;
+}
+// Running totals of the units of all entries, [entries + 1], formed by all threads of a CTA.
+__device__ __forceinline__ void sp_totals(const SpParams& p, const SpList& l, const int* shared_of, int* totals, int* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int before = 0;
+  if (threadIdx.x == 0) totals[0] = 0;
+  for (int first = 0; first < l.entries; first += blockDim.x) {
+    const int e = first + threadIdx.x;
+    int upto = e < l.entries ? sp_units(p, l, shared_of, e) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) warp_sums[warp] = upto;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < warps; ++w) {
+      const int s = warp_sums[w];
+      if (w < warp) upto += s;
+      all += s;
+    }
+    if (e < l.entries) totals[e + 1] = before + upto;
+    before += all;
+    __syncthreads();
+  }
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i <= l.entries; i += blockDim.x) l.totals[i] = totals[i];
+}
+// First unit of CTA c's run, and the CTA that has unit u.
+__device__ __forceinline__ int sp_run(int total, int ctas, int c) {
+  const int share = total / ctas, over = total - share * ctas;
+  return c * share + min(c, over);
+}
+__device__ __forceinline__ int sp_cta_of(int total, int ctas, int u) {
+  const int share = total / ctas, over = total - share * ctas, wide = over * (share + 1);
+  return u < wide ? u / (share + 1) : over + (u - wide) / share;
+}
+// A part of an entry: units u0 .. u1 - 1 of it, for one virtual KV head.
+struct SpPart {
+  int vh, e, u0, u1;
+  int b, g, n;                                   // first sequence, group, sequences of the tile
+  bool own;
+};
+// The part that a run u .. u_end begins with; u goes behind it.  Every thread that calls it gets the same.
+__device__ __forceinline__ SpPart sp_next(const SpParams& p, const SpList& l, const int* totals, int& u, int u_end) {
+  SpPart s;
+  const int all = totals[l.entries];
+  s.vh = u / all;
+  const int at = u - s.vh * all;
+  int e = 0;
+  for (int hi = l.entries; hi - e > 1;) {        // the last entry that begins at or in front of the unit
+    const int mid = (e + hi) >> 1;
+    if (totals[mid] <= at) e = mid;
+    else hi = mid;
+  }
+  s.e = e;
+  s.u0 = at - totals[e];
+  s.u1 = min(totals[e + 1], at + u_end - u) - totals[e];
+  s.own = e >= p.batch;
+  s.b = s.own ? e - p.batch : e;
+  s.g = p.group_of[s.b];
+  s.n = s.own ? 1 : min(l.seqs, p.starts[s.g + 1] - s.b);
+  u += s.u1 - s.u0;
+  return s;
+}
+// Where a part's row 0 goes, rows (sequence, head) one behind the other.  A part that begins its entry has places of the entry's own; one that goes on with it is the
+// first of its CTA's run and has the CTA's.
+__device__ __forceinline__ long long sp_row(const SpList& l, int vh, int e, int cta, bool begins) {
+  const long long heads = static_cast<long long>(l.entries - l.skip) * l.per;
+  return begins ? vh * heads + static_cast<long long>(e - l.skip) * l.per : l.virtual_heads * heads + static_cast<long long>(cta) * l.seqs * l.per;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t sp_pack(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t sp_pack<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+template <>
+__device__ __forceinline__ uint32_t sp_pack<__half>(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+}  // namespace rb
+
+namespace rbhost {
+// Rows of partial results of a list.
+inline long long sp_list_rows(const rb::SpList& l) {
+  return static_cast<long long>(l.virtual_heads) * (l.entries - l.skip) * l.per + static_cast<long long>(l.ctas) * l.seqs * l.per;
+}
+// shared_prefix_tc.cu: the parts over shared tokens with tcgen05
+bool shared_tc_takes(int batch, int heads, int kv_heads, int block_size, int most);
+rb::SpList shared_tc_list(int batch, int heads, int kv_heads);
+int shared_tc(const rb::SpParams& p, int type, int head_dim, cudaStream_t stream);
+}  // namespace rbhost

@@ -1,0 +1,411 @@
+// Attention of many rows over shared tokens: the queries of all sequences of a group for one KV head, 256 rows a CTA, on the 5th-generation tensor cores.
+//
+// A CTA goes through its run of units (128 tokens each; see shared_prefix.cuh) with two tiles of 128 rows, A and B, that share every tile of keys and values.  TMEM holds
+// S_A, S_B (128 fp32 columns each) and the accumulators O_A, O_B (a head's columns each).  For unit j one thread issues
+//     PV(j, A)  O_A += P_A V_j   (P from TMEM, V_j row by row from shared memory),   QK(j + 1, A)  S_A = Q_A K_j+1^T,   PV(j, B),   QK(j + 1, B),
+// so that the tensor cores work for one tile while the other tile's softmax runs, one row per thread.  A row keeps its maximum until a new one is more than 2^8 larger, O
+// stays in TMEM meanwhile.  Pages come by TMA, a copy per page and 64 columns, into rings of stages that go on from one part of the run to the next; the next part's
+// queries are loaded as soon as the last product that reads the old ones is done.  A part's sums leave as they are, fp32 with the row's maximum and
+// sum, for the join (shared_prefix.cu).
+//
+// Tokens behind a group's shared ones lie in the same pages, or in none: the last unit's scores are masked, and the rows of its V tile behind the last
+// token are set to zero, since a weight of zero times what they hold need not be zero.
+//
+// Bound by the softmax's exponentials and the products where there are 256 rows, by the keys' and values' bytes where there are few.
+#define RB_INLINE_WAITS                 // registers are reallocated between warp groups
+#include <string.h>
+
+#include <type_traits>
+
+#include "shared_prefix.cuh"
+
+namespace rb {
+
+constexpr int kStThreads = 384;          // warps 0-7 softmax, 8 TMA, 9 MMA, 10-11 only give their registers away
+constexpr int kStTile = 128;
+constexpr float kStRescale = 8.f;        // log2 units
+constexpr int kStMostBatch = 2048;       // running totals beside 192 KB of tiles
+
+__device__ __forceinline__ void st_ld32(uint32_t taddr, uint32_t* r) { tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r)); }
+__device__ __forceinline__ void st_st32(uint32_t taddr, const uint32_t* r) {
+  tmem_st_32x16(taddr, *reinterpret_cast<const uint32_t(*)[16]>(r));
+  tmem_st_32x16(taddr + 16, *reinterpret_cast<const uint32_t(*)[16]>(r + 16));
+}
+
+template <int D>
+struct StSmem {
+  static constexpr int kStages = D == 64 ? 4 : 2;                // of K, and of V
+  static constexpr int kHalf = kStTile * 128;                    // one 64-column swizzle atom: 128 rows x 128 B
+  static constexpr int kTileBytes = (D / 64) * kHalf;
+  static constexpr int kQ = 0;                                   // two tiles
+  static constexpr int kK = kQ + 2 * kTileBytes;
+  static constexpr int kV = kK + kStages * kTileBytes;
+  static constexpr int kBar = kV + kStages * kTileBytes;
+  static constexpr int kNumBars = 3 + 4 * kStages + 6;           // q, q free, tail; full and empty per K and V stage; s_full[2], p_full[2], o_ready[2]
+  static constexpr int kInts = kBar + kNumBars * 8;              // TMEM address, abort flag, then running totals and shared tokens
+  static constexpr int kTotal = kInts + 16;
+};
+
+struct StMaps {
+  CUtensorMap q, k, v;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kStThreads, 1)
+shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned int* status RB_BOUNDS_PARAM) {
+  pdl_wait();
+  pdl_launch();
+  using L = StSmem<D>;
+  constexpr int kStages = L::kStages;
+  extern __shared__ __align__(1024) uint8_t st_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(st_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ int warp_sums[kStThreads / 32];
+  const uint32_t sbase = smem_u32(smem), sQ = sbase + L::kQ, sK = sbase + L::kK, sV = sbase + L::kV;
+  const uint32_t b0 = sbase + L::kBar;
+  const uint32_t bar_q = b0, bar_qfree = b0 + 8, bar_tail = b0 + 16;
+  const uint32_t bar_kfull = b0 + 24, bar_kempty = bar_kfull + 8 * kStages, bar_vfull = bar_kempty + 8 * kStages, bar_vempty = bar_vfull + 8 * kStages;
+  const uint32_t bar_sfull = bar_vempty + 8 * kStages, bar_pfull = bar_sfull + 16, bar_oready = bar_pfull + 16;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + L::kInts);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  int* totals = reinterpret_cast<int*>(smem + L::kTotal);
+  const SpList& list = p.prefix;
+  int* shared_of = totals + list.entries + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr uint32_t kTmemCols = 512;
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar_q, 1);
+    mbar_init(bar_qfree, 1);
+    mbar_init(bar_tail, 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar_kfull + 8 * s, 1);
+      mbar_init(bar_kempty + 8 * s, 1);
+      mbar_init(bar_vfull + 8 * s, 1);
+      mbar_init(bar_vempty + 8 * s, 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(bar_sfull + 8 * t, 1);
+      mbar_init(bar_pfull + 8 * t, 4);
+      mbar_init(bar_oready + 8 * t, 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&maps.q);
+    tma_prefetch_desc(&maps.k);
+    tma_prefetch_desc(&maps.v);
+  }
+  sp_shared(p, shared_of);
+  sp_totals(p, list, shared_of, totals, warp_sums);
+  if (warp == 9) {
+    tmem_alloc(smem_u32(tmem_ptr), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_ptr;
+  const int total = totals[list.entries] * list.virtual_heads, group = p.heads / p.kv_heads;
+  const int u_begin = sp_run(total, list.ctas, blockIdx.x), u_end = sp_run(total, list.ctas, blockIdx.x + 1);
+  const int half = kStTile / list.per;                         // sequences of one of the two tiles
+  const int tile_rows = half * list.per;
+
+  if (warp >= 8) {
+    setmaxnreg_dec<56>();
+    if (warp == 8) {
+      // ---------------------------------------------------------------- TMA producer, all lanes
+      bool ok = true;
+      int it = 0, part = 0, tails = 0;
+      for (int u = u_begin; u < u_end && ok; ++part) {
+        const SpPart s = sp_next(p, list, totals, u, u_end);
+        const int shared = shared_of[s.g], head0 = s.vh * list.per;
+        const int* table = p.tables + static_cast<long long>(p.starts[s.g]) * p.width;
+        if (part > 0) ok = mbar_wait(bar_qfree, (part - 1) & 1, abort_flag, status, 51);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (lane == 0) {
+          const int tiles = s.n > half ? 2 : 1;
+          mbar_arrive_expect_tx(bar_q, tiles * tile_rows * 128 * (D / 64));
+          for (int t = 0; t < tiles; ++t)
+#pragma unroll
+            for (int hf = 0; hf < D / 64; ++hf)
+              tma_load_4d(sQ + t * L::kTileBytes + hf * L::kHalf, &maps.q, hf * 64, head0, s.b + t * half, 0, bar_q);
+        }
+        for (int unit = s.u0; unit < s.u1 && ok; ++unit, ++it) {
+          const int st = it % kStages, use = it / kStages, first = unit * kSpUnit, valid = min(kSpUnit, shared - first);
+          // pages of the unit: lane i has the i-th (one of 128 rows, from `row` on, where pages are larger)
+          const int bs = p.block_size, size = min(bs, kSpUnit), pages = (valid + size - 1) / size;
+          int blk = 0, row = 0;
+          if (lane < pages) {
+            const int page = (first + lane * size) / bs;
+            row = first + lane * size - page * bs;
+            blk = table[page];
+            if (blk < 0 || blk >= p.num_blocks) {              // corrupt tables read block 0 instead of faulting
+              RB_BOUNDS_HIT(104);
+              blk = 0;
+            }
+          }
+          const uint32_t bytes = pages * size * 128 * (D / 64);
+          auto load = [&](const CUtensorMap* m, uint32_t tile, uint32_t bar) {
+            if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+            __syncwarp();
+            if (lane < pages) {
+#pragma unroll
+              for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(tile + hf * L::kHalf + lane * size * 128, m, hf * 64, s.vh, row, blk, bar);
+            }
+          };
+          if (!mbar_wait(bar_kempty + 8 * st, (use & 1) ^ 1, abort_flag, status, 52)) ok = false;
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          load(&maps.k, sK + st * L::kTileBytes, bar_kfull + 8 * st);
+          if (!mbar_wait(bar_vempty + 8 * st, (use & 1) ^ 1, abort_flag, status, 53)) ok = false;
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          const uint32_t v_tile = sV + st * L::kTileBytes;
+          if (valid == kSpUnit) {
+            load(&maps.v, v_tile, bar_vfull + 8 * st);
+          } else {
+            // the copies land, then the rows behind the last token become zero, then the tile is full
+            load(&maps.v, v_tile, bar_tail);
+            if (!mbar_wait(bar_tail, tails & 1, abort_flag, status, 54)) ok = false;
+            ++tails;
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            uint8_t* tile = smem + L::kV + st * L::kTileBytes;
+            for (int i = lane; i < (kSpUnit - valid) * 8; i += 32)
+#pragma unroll
+              for (int hf = 0; hf < D / 64; ++hf) *reinterpret_cast<uint4*>(tile + hf * L::kHalf + valid * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_vfull + 8 * st);
+          }
+        }
+      }
+    } else if (warp == 9) {
+      if (elect_one()) {
+        // ---------------------------------------------------------------- MMA issuer
+        const uint64_t dQ = umma_smem_desc_sw128(sQ, 16, 1024), dK = umma_smem_desc_sw128(sK, 16, 1024), dV = umma_smem_desc_sw128(sV, L::kHalf, 1024);
+        constexpr bool kBf16 = sizeof(T) == sizeof(__nv_bfloat16) && !std::is_same<T, __half>::value;
+        constexpr uint32_t drop = kBf16 ? 0u : (1u << 7) | (1u << 10);       // operand formats: 1 bf16, 0 f16
+        constexpr uint32_t idesc_qk = umma_idesc_bf16(128, 128, 0, 0) & ~drop;
+        constexpr uint32_t idesc_pv = umma_idesc_bf16(128, D, 0, 1) & ~drop; // A = P (TMEM), B = V, rows along the sum
+        bool ok = true;
+        int it = 0, part = 0, done[2] = {0, 0};
+        auto issue_qk = [&](int i, int t) -> bool {
+          const int st = i % kStages;
+          if (!mbar_wait(bar_kfull + 8 * st, (i / kStages) & 1, abort_flag, status, 55)) return false;
+          tc_fence_after();
+          const uint64_t q = dQ + t * (L::kTileBytes / 16), k = dK + st * (L::kTileBytes / 16);
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            const uint64_t off = (ks >> 2) * (L::kHalf / 16) + (ks & 3) * 2;
+            umma_bf16_ss(tmem_base + t * 128, q + off, k + off, idesc_qk, ks != 0 ? 1u : 0u);
+          }
+          umma_commit(bar_sfull + 8 * t);
+          return true;
+        };
+        for (int u = u_begin; u < u_end && ok; ++part) {
+          const SpPart s = sp_next(p, list, totals, u, u_end);
+          const int n = s.u1 - s.u0, tiles = s.n > half ? 2 : 1;
+          ok = mbar_wait(bar_q, part & 1, abort_flag, status, 56);
+          for (int t = 0; t < tiles && ok; ++t) ok = issue_qk(it, t);
+          if (!ok) break;
+          umma_commit(bar_kempty + 8 * (it % kStages));
+          if (n == 1) umma_commit(bar_qfree);
+          for (int j = 0; j < n && ok; ++j) {
+            const int i = it + j, st = i % kStages;
+            if (!mbar_wait(bar_vfull + 8 * st, (i / kStages) & 1, abort_flag, status, 57)) { ok = false; break; }
+            for (int t = 0; t < tiles; ++t) {
+              if (!mbar_wait(bar_pfull + 8 * t, done[t] & 1, abort_flag, status, 58)) { ok = false; break; }
+              ++done[t];
+              tc_fence_after();
+              const uint32_t tmem_p = tmem_base + t * 128, tmem_o = tmem_base + 256 + t * 128;
+              const uint64_t v = dV + st * (L::kTileBytes / 16);
+#pragma unroll
+              for (int ks = 0; ks < kSpUnit / 16; ++ks)
+                umma_bf16_ts(tmem_o, tmem_p + ks * 8, v + ks * (2048 / 16), idesc_pv, (j > 0 || ks != 0) ? 1u : 0u);
+              umma_commit(bar_oready + 8 * t);
+              if (j + 1 < n && !issue_qk(i + 1, t)) { ok = false; break; }   // overwrites S_t / P_t: ordered behind PV(j, t)
+            }
+            if (!ok) break;
+            umma_commit(bar_vempty + 8 * st);
+            if (j + 1 < n) umma_commit(bar_kempty + 8 * ((i + 1) % kStages));
+            if (j + 2 == n) umma_commit(bar_qfree);              // the last products that read the queries have been issued
+          }
+          it += n;
+        }
+      }
+    }
+  } else {
+    setmaxnreg_inc<224>();
+    // ------------------------------------------------------------------ softmax, one row per thread
+    const int t = warp >> 2, wq = warp & 3;
+    const int row = wq * 32 + lane;                            // of the tile
+    const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
+    const uint32_t tmem_s = tmem_base + t * 128 + lane_off, tmem_o = tmem_base + 256 + t * 128 + lane_off;
+    const float sl2 = p.scale * kSpLog2e;
+    bool ok = true;
+    int done = 0;
+    for (int u = u_begin; u < u_end && ok;) {
+      const SpPart s = sp_next(p, list, totals, u, u_end);
+      if (t == 1 && s.n <= half) continue;                     // no rows for tile B
+      const int shared = shared_of[s.g];
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int j = s.u0; j < s.u1; ++j, ++done) {
+        if (!mbar_wait(bar_sfull + 8 * t, done & 1, abort_flag, status, 59)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t r[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) st_ld32(tmem_s + c * 32, r + c * 32);
+        tmem_ld_wait();
+        const int valid = shared - j * kSpUnit;
+        if (valid < kSpUnit) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (i >= valid) r[i] = 0xff800000u;                // -inf
+        }
+        float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 128; i += 4) {
+          mx0 = fmaxf(mx0, __uint_as_float(r[i]));
+          mx1 = fmaxf(mx1, __uint_as_float(r[i + 1]));
+          mx2 = fmaxf(mx2, __uint_as_float(r[i + 2]));
+          mx3 = fmaxf(mx3, __uint_as_float(r[i + 3]));
+        }
+        const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+        const bool grow = mx > m_run && ((mx - m_run) * sl2 > kStRescale || m_run == -INFINITY);
+        float alpha = 1.f;
+        if (grow) {
+          alpha = m_run == -INFINITY ? 0.f : wm_ex2((m_run - mx) * sl2);
+          m_run = mx;
+          l_run *= alpha;
+        }
+        if (j > s.u0 && __any_sync(0xffffffffu, grow)) {
+          // O has the sum over the units in front once their last product is done; the next one cannot start before P below
+          if (!mbar_wait(bar_oready + 8 * t, (done - 1) & 1, abort_flag, status, 60)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            st_ld32(tmem_o + c * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            st_st32(tmem_o + c * 32, o);
+          }
+          tmem_st_wait();
+        }
+        const float msc = (m_run == -INFINITY ? 0.f : m_run) * sl2;
+        float rs0 = 0.f, rs1 = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float p0 = wm_ex2(fmaf(__uint_as_float(r[c * 32 + 2 * i]), sl2, -msc)), p1 = wm_ex2(fmaf(__uint_as_float(r[c * 32 + 2 * i + 1]), sl2, -msc));
+            rs0 += p0;
+            rs1 += p1;
+            packed[i] = sp_pack<T>(p0, p1);
+          }
+          tmem_st_32x16(tmem_s + c * 16, packed);              // every score is in registers
+        }
+        l_run += rs0 + rs1;
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_pfull + 8 * t);
+      }
+      if (!ok) break;
+      // ---- the part's sums
+      if (!mbar_wait(bar_oready + 8 * t, (done - 1) & 1, abort_flag, status, 61)) break;
+      tc_fence_after();
+      const int seq = t * half + row / list.per, h = row % list.per;
+      const bool real = row < tile_rows && seq < s.n && h < group - (s.vh % list.parts) * list.per;
+      const long long to = sp_row(list, s.vh, s.e, blockIdx.x, s.u0 == 0) + seq * list.per + h;
+      if (real) list.ml[to] = make_float2(m_run * sl2, l_run);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        st_ld32(tmem_o + c * 32, o);
+        tmem_ld_wait();
+        if (real) {
+          uint4* out = reinterpret_cast<uint4*>(list.acc + to * D + c * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) out[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+      }
+      tc_fence_before();                                       // the next part's first product overwrites O behind the next arrival
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    if (*abort_flag) {
+      // a wait gave up: let copies and products in flight land before the accumulators are released
+      const unsigned long long t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+}  // namespace rb
+
+namespace {
+
+template <typename T, int D>
+int launch(const rb::SpParams& p, cudaStream_t stream) {
+  const rb::SpList& l = p.prefix;
+  int err = 0;
+  const uint64_t q_dims[4] = {(uint64_t)D, (uint64_t)p.heads, (uint64_t)p.batch, 1}, q_str[3] = {(uint64_t)D * 2, (uint64_t)p.ld_q * 2, (uint64_t)p.ld_q * 2 * p.batch};
+  const uint32_t q_box[4] = {64, (uint32_t)l.per, (uint32_t)(rb::kStTile / l.per), 1};
+  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)p.kv_heads, (uint64_t)p.block_size, (uint64_t)p.num_blocks};
+  const uint64_t token = (uint64_t)D * p.kv_heads * 2, str[3] = {(uint64_t)D * 2, token, token * p.block_size};
+  const uint32_t box[4] = {64, 1, (uint32_t)(p.block_size < rb::kSpUnit ? p.block_size : rb::kSpUnit), 1};
+  rb::StMaps maps;
+  const CUtensorMap* m = rbhost::get_tmap_4d(p.q, 2, q_dims, q_str, q_box, 1, &err);
+  if (!m) return err ? err : -7;
+  maps.q = *m;
+  m = rbhost::get_tmap_4d(p.k, 2, dims, str, box, 1, &err);
+  if (!m) return err ? err : -7;
+  maps.k = *m;
+  m = rbhost::get_tmap_4d(p.v, 2, dims, str, box, 1, &err);
+  if (!m) return err ? err : -7;
+  maps.v = *m;
+  constexpr int kMostSmem = rb::StSmem<D>::kTotal + (2 * rb::kStMostBatch + 1) * 4 + 1024;
+  static_assert(kMostSmem + 1024 <= 227 * 1024, "shared memory");
+  static bool configured[64] = {false};
+  const int dev = rbhost::device_slot();
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(rb::shared_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    configured[dev] = true;
+  }
+  const size_t smem = rb::StSmem<D>::kTotal + (2 * static_cast<size_t>(p.batch) + 1) * 4 + 1024;
+  return static_cast<int>(rbhost::launch_pdl(rb::shared_tc_kernel<T, D>, dim3(l.ctas), dim3(rb::kStThreads), smem, stream, 1, maps, p,
+                                             rbhost::status_ptr() RB_BOUNDS_ARG));
+}
+
+}  // namespace
+
+namespace rbhost {
+
+// Pages that a unit of 128 tokens has a whole number of, or that have a whole number of units; every sequence's rows of a KV head in one tile.
+bool shared_tc_takes(int batch, int heads, int kv_heads, int block_size, int most) {
+  return batch <= rb::kStMostBatch && heads / kv_heads <= rb::kStTile && most >= 1 &&
+         (block_size % rb::kSpUnit == 0 || (block_size >= 8 && rb::kSpUnit % block_size == 0)) && block_size < (1 << 20);
+}
+rb::SpList shared_tc_list(int batch, int heads, int kv_heads) {
+  rb::SpList l;
+  memset(&l, 0, sizeof(l));
+  l.entries = batch;
+  l.per = heads / kv_heads;
+  l.parts = 1;
+  l.virtual_heads = kv_heads;
+  l.seqs = rb::kStTile / l.per * 2;
+  l.ctas = device_sm_count();
+  return l;
+}
+int shared_tc(const rb::SpParams& p, int type, int head_dim, cudaStream_t stream) {
+  if (type == 0) return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, stream) : launch<__nv_bfloat16, 128>(p, stream);
+  return head_dim == 64 ? launch<__half, 64>(p, stream) : launch<__half, 128>(p, stream);
+}
+
+}  // namespace rbhost

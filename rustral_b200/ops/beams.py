@@ -31,7 +31,8 @@ N.optional_sig("rb_move_blocks", [C.c_char_p, N.c_int, N.c_void_p, N.c_void_p, N
 N.optional_sig("rb_move_reorder", [C.c_char_p, N.c_int, N.c_void_p, N.c_int, N.c_int, N.c_void_p])
 N.optional_sig("rb_shared_prefix", [C.c_char_p, N.c_void_p])
 N.optional_sig("rb_shared_prefix_scratch_bytes", [N.c_int] * 6, N.c_ll)
-N._LAUNCHES["rb_beam_select"] = N._LAUNCHES["rb_shared_prefix"] = 2
+N._LAUNCHES["rb_beam_select"] = 2
+N._LAUNCHES["rb_shared_prefix"] = 3                 # at most: groups of few rows take two
 
 
 def _here(what: str, dev: int, *tensors) -> None:
