@@ -7,23 +7,27 @@
 // the candidates of all its rows by s_r + x - L_r in 64 bits: two continuations of different beams are often closer than 32 bits of a sum can tell,
 // and the one selected must not depend on how the sum was rounded.  Beams that have ended or have a score of minus infinity are not read.
 //
-// The best n of a set that lies in the registers of many threads: the n-th largest of the threads' own maxima is a lower bound of the n-th largest
+// The best n of a set that lies with many threads: the n-th largest of the threads' own maxima is a lower bound of the n-th largest
 // number (found by its bits, most significant first, with one count over the CTA per bit); numbers not below it, little more than n, go to a list, and a number's
-// place is the count of those before it.  Where equal numbers overflow the list the best are taken one after the other.
+// place is the count of those before it.
 #include "beam.h"
 
 #include <cuda_fp16.h>
 #include <float.h>
 
+#include <type_traits>
+
+#include "pairs.cuh"
 #include "pdl.cuh"
-#include "rb_common.cuh"
+#include "warp_mma.cuh"
 
 namespace rb {
 
 constexpr int kBsThreads = 256;
+constexpr float kBsLog2e = 1.4426950408889634f;
 constexpr int kBsMostCount = 128;
 constexpr int kBsMostBeams = 256;
-constexpr int kBsList = 1024;                    // room for the numbers that are not below the bound
+constexpr int kBsList = 1024;                    // room for the numbers that are not below a bound
 
 struct BsStat {
   float most, sum;                               // of a piece of a row: its maximum and the sum of exp(x - maximum)
@@ -43,12 +47,60 @@ struct BsParams {
   BsCandidate* found;                            // [rows, pieces, count]
   long long ld;
   int groups, beams, vocab, count, end_token, pieces, piece;
-  int vec;                                       // elements of a load: 16 bytes, or one where rows do not begin on 16 bytes
+  bool wide;                                     // rows begin on 16 bytes
 };
 
-__device__ __forceinline__ float bs_value(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float bs_value(__half v) { return __half2float(v); }
-__device__ __forceinline__ float bs_value(float v) { return v; }
+// Number i of words that hold numbers of type T one behind the other.
+template <typename T>
+__device__ __forceinline__ float bs_value(const uint32_t* w, int i);
+template <>
+__device__ __forceinline__ float bs_value<__nv_bfloat16>(const uint32_t* w, int i) { return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
+template <>
+__device__ __forceinline__ float bs_value<__half>(const uint32_t* w, int i) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? w[i / 2] >> 16 : w[i / 2])));
+}
+template <>
+__device__ __forceinline__ float bs_value<float>(const uint32_t* w, int i) { return __uint_as_float(w[i]); }
+// A word's worth of them from numbers at x that need not be aligned; minus infinity behind the last.
+template <typename T>
+__device__ __forceinline__ uint32_t bs_word(const T* x, int at, int end);
+template <>
+__device__ __forceinline__ uint32_t bs_word(const float* x, int at, int end) { return __float_as_uint(at < end ? x[at] : -INFINITY); }
+template <typename T>
+__device__ __forceinline__ uint32_t bs_word(const T* x, int at, int end) {
+  constexpr uint32_t kLeast = std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
+  const unsigned short* u = reinterpret_cast<const unsigned short*>(x);
+  const uint32_t lo = at < end ? u[at] : kLeast, hi = at + 1 < end ? u[at + 1] : kLeast;
+  return lo | hi << 16;
+}
+// The largest of W words of numbers; a NaN is none of them.
+template <typename T, int W>
+__device__ __forceinline__ float bs_most(const uint32_t* w) {
+  if (sizeof(T) == 4) {
+    float m = __uint_as_float(w[0]);
+#pragma unroll
+    for (int i = 1; i < W; ++i) m = fmaxf(m, __uint_as_float(w[i]));
+    return fmaxf(m, -INFINITY);
+  }
+  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  T2 m = *reinterpret_cast<const T2*>(w);
+#pragma unroll
+  for (int i = 1; i < W; ++i) m = __hmax2(m, *reinterpret_cast<const T2*>(w + i));
+  uint32_t u = *reinterpret_cast<const uint32_t*>(&m);
+  return fmaxf(fmaxf(bs_value<typename std::conditional<sizeof(T) == 4, __half, T>::type>(&u, 0), bs_value<typename std::conditional<sizeof(T) == 4, __half, T>::type>(&u, 1)), -INFINITY);
+}
+// 16 bytes of numbers from x[at] on.
+template <typename T>
+__device__ __forceinline__ void bs_load(const T* x, int at, int end, bool wide, uint32_t* w) {
+  constexpr int V = 16 / sizeof(T);
+  if (wide && at + V <= end) {
+    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(x + at));
+    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = bs_word(x, at + i * (V / 4), end);
+  }
+}
 // NaN is minus infinity, plus infinity the largest number
 __device__ __forceinline__ float bs_clean(float v) { return v != v ? -INFINITY : fminf(v, FLT_MAX); }
 // Order of the numbers as order of whole numbers; minus infinity is the least, and no number gives 0.
@@ -57,6 +109,7 @@ __device__ __forceinline__ uint32_t bs_key(float v) {
   const uint32_t u = __float_as_uint(v);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float bs_number(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 constexpr uint32_t kBsLeast = 0x007fffffu;       // bs_key(-infinity)
 
 __device__ __forceinline__ bool bs_live(const BsParams& p, int row) {
@@ -67,6 +120,7 @@ __device__ __forceinline__ bool bs_live(const BsParams& p, int row) {
 // The n-th largest key of the CTA's threads (one key each), 1 <= n <= blockDim.x.  Every thread gets it.
 __device__ __forceinline__ uint32_t bs_nth(uint32_t key, int n, int lowest_bit) {
   uint32_t at = 0;
+#pragma unroll 1
   for (int bit = 31; bit >= lowest_bit; --bit) {
     const uint32_t with = at | 1u << bit;
     const int c = __syncthreads_count(key >= with);
@@ -77,117 +131,300 @@ __device__ __forceinline__ uint32_t bs_nth(uint32_t key, int n, int lowest_bit) 
 }
 
 // ---- a piece of a row --------------------------------------------------------------------------------------------------------------------
-// E: elements of a thread
-template <typename T, int E>
-__global__ void __launch_bounds__(kBsThreads)
-beam_rows_kernel(const BsParams p) {
+// Numbers by their keys, each with a token, in no order.
+template <int CAP>
+struct BsList {
+  uint32_t key[CAP];
+  int token[CAP];
+  int size;
+};
+// Keeps the n best of the list's m numbers, in order.  All threads.
+template <int CAP>
+__device__ __forceinline__ void bs_keep(BsList<CAP>& l, int m, int n) {
+  constexpr int kMine = (CAP + kBsThreads - 1) / kBsThreads;
+  uint32_t k[kMine];
+  int t[kMine], at[kMine];
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) {
+    const int i = threadIdx.x + j * kBsThreads;
+    at[j] = CAP;
+    if (i < m) {
+      k[j] = l.key[i];
+      t[j] = l.token[i];
+      int before = 0;
+      for (int o = 0; o < m; ++o) before += l.key[o] > k[j] || (l.key[o] == k[j] && l.token[o] < t[j]) ? 1 : 0;
+      at[j] = before;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kMine; ++j)
+    if (at[j] < n) {
+      l.key[at[j]] = k[j];
+      l.token[at[j]] = t[j];
+    }
+  if (threadIdx.x == 0) l.size = min(m, n);
+  __syncthreads();
+}
+// Puts the n best of the numbers i = 0 .. count - 1 into an empty list, however many are equal: the n-th largest key bit by bit, counting all numbers, then of those
+// equal to it the highest token that is still taken, in the same way.  number(i, token) gives a number, -infinity for none.
+template <typename F>
+__device__ __forceinline__ void bs_search(BsList<kBsList>& l, int count, int n, F number) {
+  auto counted = [&](auto f) {
+    int c = 0;
+    for (int i = threadIdx.x; i < count; i += kBsThreads) {
+      int token;
+      const uint32_t k = bs_key(number(i, token));
+      c += f(k, token) ? 1 : 0;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) l.size = 0;
+    __syncthreads();
+    if (c) atomicAdd(&l.size, c);
+    __syncthreads();
+    return l.size;
+  };
+  uint32_t nth = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t with = nth | 1u << bit;
+    if (counted([&](uint32_t k, int) { return k >= with; }) >= n) nth = with;
+  }
+  const int room = n - counted([&](uint32_t k, int) { return k > nth; });
+  int last = 0;                                  // tokens below it are fewer than the room
+#pragma unroll 1
+  for (int bit = 30; bit >= 0; --bit) {
+    const int with = last | 1 << bit;
+    if (counted([&](uint32_t k, int t) { return k == nth && t < with; }) < room) last = with;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) l.size = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < count; i += kBsThreads) {
+    int token;
+    const uint32_t k = bs_key(number(i, token));
+    if (k > nth || (k == nth && token <= last)) {
+      const int at = atomicAdd(&l.size, 1);
+      l.key[at] = k;
+      l.token[at] = token;
+    }
+  }
+  __syncthreads();
+}
+
+// A ring of tiles in shared memory that bulk copies fill.
+constexpr int kBsStages = 2;
+constexpr int kBsApart = 4;                      // tiles between two looks at the noted chunks
+constexpr int kBsChunks = 2 * kBsMostCount + 16 + kBsApart * kBsThreads;
+__device__ __forceinline__ void bs_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  mbar_arrive_expect_tx(bar, bytes);
+  if (bytes)
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// E: numbers of a thread and tile, neighbours, so that the order of (tile, thread) is the order of tokens.  A thread that meets a number not below the bound notes its whole
+// chunk of E under the chunk's largest number: the n best numbers lie in the n chunks whose largest are the best (of equal ones the first), and which of a chunk's they are is
+// looked up once, at the end.  So the pass over the logits is a maximum and an exponential per number, a barrier per tile and few chunks noted, n (1 + 1/2 + 1/3 + ...) of
+// n, n, n, ... that would pass a bound from the first tile.
+// BULK: tiles come through the ring; else a piece is one tile, or rows do not begin on 16 bytes.
+template <typename T, int E, bool BULK>
+__global__ void __launch_bounds__(kBsThreads, 4)
+beam_rows_kernel(const BsParams p, unsigned int* status) {
   pdl_wait();
   pdl_launch();
   const int row = blockIdx.x, piece = blockIdx.y;
   if (!bs_live(p, row)) return;
-  constexpr int V = 16 / sizeof(T);              // elements of a wide load
+  constexpr int V = 16 / sizeof(T), L = E / V, W = 4 * L;       // numbers of a wide load; loads and words of a thread and tile
+  constexpr int kTile = E * kBsThreads;
+  extern __shared__ __align__(128) uint8_t bs_tiles[];
+  __shared__ BsList<kBsChunks> chunks;
+  __shared__ BsList<kBsList> best;
+  __shared__ float warp_most[kBsThreads / 32], warp_total[kBsThreads / 32];
+  __shared__ uint64_t bars[2 * kBsStages];
+  __shared__ int abort_flag;
   const T* x = static_cast<const T*>(p.logits) + static_cast<long long>(row) * p.ld;
   const int first = piece * p.piece, end = min(p.vocab, first + p.piece);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // element e of a thread is number first + (e / V) * 256 V + tid * V + e % V
-  float v[E];
-#pragma unroll
-  for (int j = 0; j < E / V; ++j) {
-    const int at = first + (j * kBsThreads + tid) * V;
-    if (p.vec > 1 && at + V <= end) {
-      const uint4 u = __ldcs(reinterpret_cast<const uint4*>(x + at));
-      const T* w = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[j * V + i] = bs_clean(bs_value(w[i]));
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[j * V + i] = at + i < end ? bs_clean(bs_value(x[at + i])) : -INFINITY;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.count;
+  const uint32_t ring = smem_u32(bs_tiles), full = smem_u32(bars), empty = full + 8 * kBsStages;
+  if (BULK && tid == 0) {
+    for (int s = 0; s < kBsStages; ++s) {
+      mbar_init(full + 8 * s, 1);
+      mbar_init(empty + 8 * s, kBsThreads / 32);
     }
+    abort_flag = 0;
+    fence_mbar_init();
   }
-  float most = -INFINITY;
+  int seen = 0;                                  // tiles of the ring so far
+  float most, sum;                               // this thread's maximum, and its sum of exp(x - maximum)
+  uint32_t bound;
+  uint32_t now[W];
+  // Two passes where there are NaN or infinities: the first one's sum is NaN then, the second replaces them.
+  auto pass = [&](auto replace) {
+    constexpr bool kClean = decltype(replace)::value;
+    auto value = [&](int e) { return kClean ? bs_clean(bs_value<T>(now, e)) : bs_value<T>(now, e); };
+    // tile i of the piece into its place of the ring: whole 16 bytes, what is behind them is loaded where it is used
+    auto request = [&](int i) {
+      const int tile = first + i * kTile, s = (seen + i) % kBsStages;
+      if (tile < end) bs_bulk(ring + s * kTile * static_cast<int>(sizeof(T)), x + tile, min(kTile, end - tile) / V * 16, full + 8 * s);
+    };
+    most = -INFINITY;
+    sum = 0.f;
+    bound = kBsLeast + 1;
+    __syncthreads();
+    if (tid == 0) {
+      chunks.size = best.size = 0;
+      if (BULK)
+        for (int i = 0; i < kBsStages; ++i) request(i);
+    }
+    int i_tile = 0;
+    for (int tile = first; tile < end; tile += kTile, ++i_tile) {
+      const int mine = tile + tid * E;
+      if (BULK) {
+        const int at = seen + i_tile, s = at % kBsStages;
+        if (tid == 0 && i_tile > 0 && tile + (kBsStages - 1) * kTile < end) {
+          // the place of the tile in front is free once every warp has its numbers
+          const int was = at - 1;
+          mbar_wait(empty + 8 * (was % kBsStages), (was / kBsStages) & 1, &abort_flag, status, 63);
+          request(i_tile - 1 + kBsStages);
+        }
+        mbar_wait(full + 8 * s, (at / kBsStages) & 1, &abort_flag, status, 62);
 #pragma unroll
-  for (int e = 0; e < E; ++e) most = fmaxf(most, v[e]);
-  __shared__ float warp_most[kBsThreads / 32], warp_total[kBsThreads / 32];
-  __shared__ int listed;
-  __shared__ uint32_t list_key[kBsList];
-  __shared__ int list_token[kBsList];
-  const float wm = warp_max(most);
-  if (lane == 0) warp_most[warp] = wm;
-  if (tid == 0) listed = 0;
-  __syncthreads();
-  float top = warp_most[0];
+        for (int j = 0; j < L; ++j) {
+          // neighbouring threads begin with different loads: no two of eight meet in a bank
+          const int to = (j + (tid >> 1)) % L * V;
+          if (mine + to + V <= end) {
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(now[4 * j]), "=r"(now[4 * j + 1]), "=r"(now[4 * j + 2]), "=r"(now[4 * j + 3])
+                         : "r"(ring + (s * kTile + tid * E + to) * static_cast<int>(sizeof(T)))
+                         : "memory");
+          } else {
 #pragma unroll
-  for (int w = 1; w < kBsThreads / 32; ++w) top = fmaxf(top, warp_most[w]);
-  float sum = 0.f;
-  if (top != -INFINITY)
+            for (int i = 0; i < 4; ++i) now[4 * j + i] = bs_word(x, mine + to + i * (V / 4), end);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + 8 * s);
+      } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) sum += __expf(v[e] - top);
-  sum = warp_sum(sum);
-  if (lane == 0) warp_total[warp] = sum;
+        for (int j = 0; j < L; ++j) bs_load(x, mine + j * V, end, p.wide, now + 4 * j);
+      }
+      float top = -INFINITY;
+      if (kClean) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) top = fmaxf(top, value(e));
+      } else {
+        top = bs_most<T, W>(now);
+      }
+      const uint32_t key = bs_key(top);
+      if (i_tile == 0) bound = max(bound, bs_nth(key, n, sizeof(T) == 4 ? 0 : 13));     // numbers of 16 bits have no lower bits in 32
+      if (key >= bound) {
+        const int at = atomicAdd(&chunks.size, 1);
+        chunks.key[at] = key;
+        chunks.token[at] = mine;
+      }
+      if (top > most) {
+        sum *= wm_ex2((most - top) * kBsLog2e);
+        most = top;
+      }
+      // exp(x - m) with the difference formed first: exact for the numbers that count
+      const float from = most == -INFINITY ? 0.f : -most;
+      const Pair from2 = pair_of(from, from), log2e = pair_of(kBsLog2e, kBsLog2e);
+      Pair add[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 y = floats(mul2(add2(pair_of(value(e), value(e + 1)), from2), log2e));
+        add[e / 2 & 1] = add2(add[e / 2 & 1], pair_of(wm_ex2(y.x), wm_ex2(y.y)));
+      }
+      const float2 added = floats(add2(add[0], add[1]));
+      sum += added.x + added.y;
+      if (i_tile % kBsApart == kBsApart - 1 && tile + kTile < end) {
+        __syncthreads();
+        const int m = chunks.size;
+        __syncthreads();
+        if (m > 2 * n + 16) {                    // no more are left in front of the next tiles than the list has room for
+          bs_keep(chunks, m, n);
+          bound = max(bound, chunks.key[n - 1] + 1);             // later chunks lose against equal ones
+        }
+      }
+    }
+    seen += i_tile;
+  };
+  pass(std::false_type());
+  const bool dirty = __syncthreads_or(sum != sum);
+  if (dirty) {
+    pass(std::true_type());
+    __syncthreads();
+  }
 
-  const long long place = static_cast<long long>(row) * p.pieces + piece;
-  BsCandidate* found = p.found + place * p.count;
-  const int n = p.count;
-  // numbers of 16 bits have no lower bits in 32
-  const uint32_t bound = max(bs_nth(bs_key(most), min(n, kBsThreads), sizeof(T) == 4 ? 0 : sizeof(T) == 2 ? 13 : 0), kBsLeast + 1);
-  if (tid == 0) {
-    float s = 0.f;
+  // ---- the n best numbers of the noted chunks
+  const bool one = !BULK && end - first <= kTile;
+  if (one) {                                     // still in registers
+    if (most != -INFINITY && bs_key(most) >= bound) {
 #pragma unroll
-    for (int w = 0; w < kBsThreads / 32; ++w) s += warp_total[w];
-    p.stats[place] = {top, s};
-  }
-  if (bs_key(most) >= bound) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const uint32_t k = bs_key(v[e]);
-      if (k >= bound) {
-        const int at = atomicAdd(&listed, 1);
-        if (at < kBsList) {
-          list_key[at] = k;
-          list_token[at] = first + ((e / V) * kBsThreads + tid) * V + e % V;
+      for (int e = 0; e < E; ++e) {
+        const float v = dirty ? bs_clean(bs_value<T>(now, e)) : bs_value<T>(now, e);
+        if (bs_key(v) >= bound) {
+          const int at = atomicAdd(&best.size, 1);
+          if (at < kBsList) {
+            best.key[at] = bs_key(v);
+            best.token[at] = first + tid * E + e;
+          }
+        }
+      }
+    }
+  } else {
+    bs_keep(chunks, chunks.size, n);
+    const int have = chunks.size;
+    if (have == n) bound = chunks.key[n - 1];
+    for (int i = tid; i < have * E; i += kBsThreads) {
+      const int t = chunks.token[i / E] + i % E;
+      if (t < end) {
+        const uint32_t w = bs_word(x, t, end);
+        const float v = bs_clean(bs_value<T>(&w, 0));
+        if (bs_key(v) >= bound && v != -INFINITY) {
+          const int at = atomicAdd(&best.size, 1);
+          if (at < kBsList) {
+            best.key[at] = bs_key(v);
+            best.token[at] = t;
+          }
         }
       }
     }
   }
   __syncthreads();
-  const int m = listed;
-  auto number = [](uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); };
-  if (m <= kBsList) {
-    for (int i = tid; i < m; i += kBsThreads) {
-      const uint32_t k = list_key[i];
-      const int t = list_token[i];
-      int before = 0;
-      for (int j = 0; j < m; ++j) before += list_key[j] > k || (list_key[j] == k && list_token[j] < t) ? 1 : 0;
-      if (before < n) found[before] = {number(k), t};
-    }
-    for (int i = m + tid; i < n; i += kBsThreads) found[i] = {0.f, -1};
-    return;
+  int m = best.size;
+  if (m > kBsList) {                             // many equal or neighbouring ones
+    bs_search(best, one ? end - first : chunks.size * E, n, [&](int i, int& token) {
+      token = one ? first + i : chunks.token[i / E] + i % E;
+      const uint32_t w = bs_word(x, token, end);
+      return bs_clean(bs_value<T>(&w, 0));
+    });
+    m = n;
   }
-  // one after the other: the largest (key, lowest token) below the last
-  __shared__ unsigned long long warp_best[kBsThreads / 32];
-  unsigned long long last = ~0ull;
-  for (int i = 0; i < n; ++i) {
-    unsigned long long best = 0;
+  bs_keep(best, m, n);
+
+  const float wm = warp_max(most);
+  const float ws = warp_sum(wm == -INFINITY ? 0.f : sum * wm_ex2((most - wm) * kBsLog2e));
+  if (lane == 0) {
+    warp_most[warp] = wm;
+    warp_total[warp] = ws;
+  }
+  __syncthreads();
+  const long long place = static_cast<long long>(row) * p.pieces + piece;
+  if (tid == 0) {
+    float top = warp_most[0], s = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int t = first + ((e / V) * kBsThreads + tid) * V + e % V;
-      const uint32_t k = bs_key(v[e]);
-      const unsigned long long c = static_cast<unsigned long long>(k) << 32 | (0xffffffffu - static_cast<uint32_t>(t));
-      if (k > kBsLeast && c < last && c > best) best = c;
-    }
+    for (int w = 1; w < kBsThreads / 32; ++w) top = fmaxf(top, warp_most[w]);
+    if (top != -INFINITY)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-      best = other > best ? other : best;
-    }
-    if (lane == 0) warp_best[warp] = best;
-    __syncthreads();
-    best = warp_best[0];
-#pragma unroll
-    for (int w = 1; w < kBsThreads / 32; ++w) best = warp_best[w] > best ? warp_best[w] : best;
-    last = best;                                 // never 0: more than kBsList >= n numbers are above minus infinity
-    if (tid == 0) found[i] = {number(static_cast<uint32_t>(best >> 32)), static_cast<int>(0xffffffffu - static_cast<uint32_t>(best))};
-    __syncthreads();
+      for (int w = 0; w < kBsThreads / 32; ++w) s += warp_total[w] * wm_ex2((warp_most[w] - top) * kBsLog2e);
+    p.stats[place] = {top, s};
+  }
+  BsCandidate* found = p.found + place * n;
+  for (int i = tid; i < n; i += kBsThreads) {
+    if (i < m) found[i] = {bs_number(best.key[i]), best.token[i]};
+    else found[i] = {0.f, -1};
   }
 }
 
@@ -197,6 +434,7 @@ __device__ __forceinline__ unsigned long long bs_key64(double v) {
   const unsigned long long u = static_cast<unsigned long long>(__double_as_longlong(v));
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
+// The pieces' candidates lie in order, so a thread has some of one list (or whole lists where there are more than threads) and knows their largest from the first.
 __global__ void __launch_bounds__(kBsThreads)
 beam_group_kernel(const BsParams p) {
   pdl_wait();
@@ -209,22 +447,30 @@ beam_group_kernel(const BsParams p) {
   __shared__ double list_total[kBsList];
   __shared__ int list_beam[kBsList], list_token[kBsList];
   __shared__ int chosen_token[kBsMostCount], chosen_beam[kBsMostCount];
-  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row0 = g * p.beams, per = p.pieces * p.count, total = p.beams * per + p.beams;
-  const BsCandidate* found = p.found + static_cast<long long>(row0) * per;
+  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.count;
+  const int row0 = g * p.beams, lists = p.beams * p.pieces;
+  const BsCandidate* found = p.found + static_cast<long long>(row0) * p.pieces * n;
+  // lists of a thread: tid / share, and every kBsThreads / share-th behind it; items `from` .. `upto` - 1 of them
+  const int share = max(1, kBsThreads / lists), step = kBsThreads / share, size = (n + share - 1) / share;
+  const int from = tid % share * size, upto = min(n, from + size), list0 = tid < share * step ? tid / share : lists;
+  BsCandidate head = {0.f, -1};                  // asked for before the rows' sums are formed
+  if (list0 < lists && from < upto) head = found[static_cast<long long>(list0) * n + from];
   if (tid == 0) listed = 0;
   for (int r = warp; r < p.beams; r += kBsThreads / 32) {
     const float score = bs_clean(p.scores[row0 + r]);
     double b = -INFINITY;
     if (bs_live(p, row0 + r)) {
       const BsStat* st = p.stats + static_cast<long long>(row0 + r) * p.pieces;
-      float most = -INFINITY;
-      for (int i = lane; i < p.pieces; i += 32) most = fmaxf(most, st[i].most);
+      const BsStat mine = lane < p.pieces ? st[lane] : BsStat{-INFINITY, 0.f};
+      float most = mine.most;
+      for (int i = lane + 32; i < p.pieces; i += 32) most = fmaxf(most, st[i].most);
       most = warp_max(most);
       double sum = 0.0;
-      if (most != -INFINITY)
-        for (int i = lane; i < p.pieces; i += 32)
+      if (most != -INFINITY) {
+        if (mine.most != -INFINITY) sum = static_cast<double>(mine.sum) * exp(static_cast<double>(mine.most) - most);
+        for (int i = lane + 32; i < p.pieces; i += 32)
           if (st[i].most != -INFINITY) sum += static_cast<double>(st[i].sum) * exp(static_cast<double>(st[i].most) - most);
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (most != -INFINITY) b = static_cast<double>(score) - log(sum);
@@ -233,42 +479,41 @@ beam_group_kernel(const BsParams p) {
     if (lane == 0) base[r] = b;
   }
   __syncthreads();
-  // Candidate i: number i % per of row i / per, and behind them one for each ended row.
-  auto candidate = [&](int i, double& t, int& token, int& beam) -> bool {
-    if (i < p.beams * per) {
-      beam = i / per;
-      if (base[beam] == -INFINITY) return false;
-      const BsCandidate c = found[i];
-      token = c.token;
-      t = base[beam] + (static_cast<double>(c.x) - row_most[beam]);
-      return token >= 0;
-    }
-    beam = i - p.beams * per;
-    token = p.end_token;
-    t = static_cast<double>(bs_clean(p.scores[row0 + beam]));
-    return p.ended && p.ended[row0 + beam] && t != -INFINITY;
-  };
-  const int n = p.count;
-  uint32_t most = 0;
-  for (int i = tid; i < total; i += kBsThreads) {
-    double t;
-    int token, beam;
-    if (candidate(i, t, token, beam)) most = max(most, bs_key(fmaxf(static_cast<float>(t), -FLT_MAX)));
-  }
-  const uint32_t bound = max(bs_nth(most, min(n, kBsThreads), 0), kBsLeast + 1);
-  if (most >= bound)
-    for (int i = tid; i < total; i += kBsThreads) {
-      double t;
-      int token, beam;
-      if (candidate(i, t, token, beam) && bs_key(fmaxf(static_cast<float>(t), -FLT_MAX)) >= bound) {
-        const int at = atomicAdd(&listed, 1);
-        if (at < kBsList) {
-          list_total[at] = t;
-          list_beam[at] = beam;
-          list_token[at] = token;
-        }
+  auto total_of = [&](int beam, float x) { return base[beam] + (static_cast<double>(x) - row_most[beam]); };
+  auto rough = [](double t) { return bs_key(fmaxf(static_cast<float>(t), -FLT_MAX)); };       // keeps the order, but for what rounds to the same
+  // a list's item, false behind the last: f(total, token, beam) until it returns false
+  auto each = [&](auto f) {
+    for (int i = list0; i < lists; i += step) {
+      const int beam = i / p.pieces;
+      if (base[beam] == -INFINITY) continue;
+      for (int j = from; j < upto; ++j) {
+        const BsCandidate c = i == list0 && j == from ? head : found[static_cast<long long>(i) * n + j];
+        if (c.token < 0 || !f(total_of(beam, c.x), c.token, beam)) break;
       }
     }
+    if (p.ended)
+      for (int r = tid; r < p.beams; r += kBsThreads) {
+        const float s = bs_clean(p.scores[row0 + r]);
+        if (p.ended[row0 + r] && s != -INFINITY) f(static_cast<double>(s), p.end_token, r);
+      }
+  };
+  uint32_t most = 0;
+  each([&](double t, int, int) {
+    most = max(most, rough(t));
+    return false;                                // the rest of a list is smaller
+  });
+  const uint32_t bound = max(bs_nth(most, n, 0), kBsLeast + 1);
+  if (most >= bound)
+    each([&](double t, int token, int beam) {
+      if (rough(t) < bound) return false;
+      const int at = atomicAdd(&listed, 1);
+      if (at < kBsList) {
+        list_total[at] = t;
+        list_beam[at] = beam;
+        list_token[at] = token;
+      }
+      return true;
+    });
   __syncthreads();
   const int m = listed;
   int have;                                      // continuations that are not minus infinity, n at most
@@ -298,14 +543,12 @@ beam_group_kernel(const BsParams p) {
     unsigned long long last_key = ~0ull, last_order = 0;
     for (int i = 0; i < n; ++i) {
       unsigned long long key = 0, order = ~0ull;
-      for (int c = tid; c < total; c += kBsThreads) {
-        double t;
-        int token, beam;
-        if (!candidate(c, t, token, beam)) continue;
+      each([&](double t, int token, int beam) {
         const unsigned long long k = bs_key64(t), o = static_cast<unsigned long long>(beam) << 32 | static_cast<unsigned int>(token);
         const bool behind = k < last_key || (k == last_key && o > last_order);
         if (behind && (k > key || (k == key && o < order))) { key = k; order = o; }
-      }
+        return true;
+      });
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const unsigned long long k = __shfl_xor_sync(0xffffffffu, key, o), w = __shfl_xor_sync(0xffffffffu, order, o);
@@ -347,20 +590,60 @@ beam_group_kernel(const BsParams p) {
 }  // namespace rb
 
 namespace {
-// Elements of a thread: 32 (8192 of a row for a CTA), fewer where that leaves SMs without a CTA: a piece is then loaded and searched in less time.
-int elements(int groups, int beams, int vocab, int type) {
-  const long long rows = static_cast<long long>(groups) * beams;
-  const int least = type == 2 ? 4 : 8;
-  int e = 32;
-  while (e > least && rows * ((vocab + e * rb::kBsThreads - 1) / (e * rb::kBsThreads)) < 148) e /= 2;
-  return e;
+struct Cut {
+  int e, pieces, piece;                          // numbers of a thread and tile; pieces of a row, numbers of one
+  bool bulk;
+};
+// Where there are at least two tiles of 8192 numbers (4096 in 32 bits) for each of an SM's four places, a CTA goes through several by bulk copies: only a piece's first
+// tile has to be searched for a bound.  Else one tile for a CTA, smaller down to one load of a thread until there is a CTA for every SM.
+Cut cut_of(int groups, int beams, int vocab, int type, bool wide) {
+  const long long rows = static_cast<long long>(groups) * beams, places = 4ll * rbhost::device_sm_count();
+  const int size = type == 2 ? 4 : 2, least = 16 / size;
+  auto tiles = [&](int e) { return (vocab + e * rb::kBsThreads - 1) / (e * rb::kBsThreads); };
+  Cut c;
+  c.e = 64 / size;
+  c.bulk = wide && rows * tiles(c.e) >= 2 * places;
+  if (!c.bulk) {
+    c.e /= 2;
+    while (c.e > least && rows * tiles(c.e) < places / 4) c.e /= 2;
+  }
+  const int all = tiles(c.e);
+  long long per = 1;                             // tiles of a piece
+  if (c.bulk || rows * all > 8 * places) {
+    const long long pieces = rows < places ? places / rows : 1;
+    per = (all + pieces - 1) / pieces;
+  }
+  c.piece = static_cast<int>(per) * c.e * rb::kBsThreads;
+  c.pieces = static_cast<int>((all + per - 1) / per);
+  return c;
 }
-int pieces_of(int vocab, int e) { return (vocab + e * rb::kBsThreads - 1) / (e * rb::kBsThreads); }
+template <typename T, int E, bool BULK>
+cudaError_t rows_kernel(const rb::BsParams& p, dim3 grid, cudaStream_t s) {
+  const size_t smem = BULK ? rb::kBsStages * E * rb::kBsThreads * sizeof(T) : 0;
+  static bool configured[64] = {false};
+  const int dev = rbhost::device_slot();
+  if (BULK && !configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(rb::beam_rows_kernel<T, E, BULK>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  return rbhost::launch_pdl(rb::beam_rows_kernel<T, E, BULK>, grid, dim3(rb::kBsThreads), smem, s, 1, p, rbhost::status_ptr());
+}
+template <typename T>
+cudaError_t rows_of(const Cut& c, const rb::BsParams& p, dim3 grid, cudaStream_t s) {
+  constexpr int kFull = 64 / sizeof(T);
+  if (c.bulk) return rows_kernel<T, kFull, true>(p, grid, s);
+  return c.e == kFull / 2 ? rows_kernel<T, kFull / 2, false>(p, grid, s) : rows_kernel<T, kFull / 4, false>(p, grid, s);
+}
 }  // namespace
 
+static long long most_pieces(int groups, int beams, int vocab, int type) {
+  const int a = cut_of(groups, beams, vocab, type, true).pieces, b = cut_of(groups, beams, vocab, type, false).pieces;
+  return a > b ? a : b;
+}
 RB_API long long rb_beam_select_scratch_bytes(int groups, int beams, int vocab, int count, int type) {
   if (groups < 0 || beams < 1 || vocab < 1 || count < 1) return 0;
-  const long long places = static_cast<long long>(groups) * beams * pieces_of(vocab, elements(groups, beams, vocab, type));
+  const long long places = static_cast<long long>(groups) * beams * most_pieces(groups, beams, vocab, type);
   return places * (sizeof(rb::BsStat) + count * sizeof(rb::BsCandidate)) + 16;
 }
 
@@ -373,29 +656,22 @@ RB_API int rb_beam_select(const RbBeamSelectArgs* a, void* stream) {
   const long long rows = static_cast<long long>(a->groups) * a->beams;
   if (rows > 0x7fffffffll) return -2;
   if (a->ended && (a->end_token < 0 || a->end_token >= a->vocab)) return -3;
-  const int size = a->type == 2 ? 4 : 2, e = elements(a->groups, a->beams, a->vocab, a->type);
+  const int size = a->type == 2 ? 4 : 2;
+  const bool wide = (reinterpret_cast<unsigned long long>(a->logits) & 15) == 0 && (a->ld * size) % 16 == 0;
+  const Cut c = cut_of(a->groups, a->beams, a->vocab, a->type, wide);
   rb::BsParams p;
   p.logits = a->logits; p.scores = a->scores; p.ended = a->ended;
   p.out_scores = a->out_scores; p.out_rows = a->out_rows; p.out_tokens = a->out_tokens;
   p.ld = a->ld; p.groups = a->groups; p.beams = a->beams; p.vocab = a->vocab; p.count = a->count; p.end_token = a->end_token;
-  p.pieces = pieces_of(a->vocab, e);
-  p.piece = e * rb::kBsThreads;
-  p.vec = (reinterpret_cast<unsigned long long>(a->logits) & 15) == 0 && (a->ld * size) % 16 == 0 ? 16 / size : 1;
+  p.pieces = c.pieces;
+  p.piece = c.piece;
+  p.wide = wide;
   if (p.pieces > 65535 || static_cast<long long>(a->beams) * p.pieces * a->count + a->beams > 0x7fffffffll) return -2;
   p.stats = static_cast<rb::BsStat*>(a->scratch);
   p.found = reinterpret_cast<rb::BsCandidate*>(p.stats + rows * p.pieces);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(rows), p.pieces), block(rb::kBsThreads);
-  auto go = [&](void (*k)(const rb::BsParams)) { return rbhost::launch_pdl(k, grid, block, 0, s, 1, p); };
-  cudaError_t err;
-  if (a->type == 2)
-    err = e == 32 ? go(rb::beam_rows_kernel<float, 32>) : e == 16 ? go(rb::beam_rows_kernel<float, 16>)
-          : e == 8 ? go(rb::beam_rows_kernel<float, 8>) : go(rb::beam_rows_kernel<float, 4>);
-  else if (a->type == 1)
-    err = e == 32 ? go(rb::beam_rows_kernel<__half, 32>) : e == 16 ? go(rb::beam_rows_kernel<__half, 16>) : go(rb::beam_rows_kernel<__half, 8>);
-  else
-    err = e == 32 ? go(rb::beam_rows_kernel<__nv_bfloat16, 32>) : e == 16 ? go(rb::beam_rows_kernel<__nv_bfloat16, 16>)
-                                                                 : go(rb::beam_rows_kernel<__nv_bfloat16, 8>);
+  const dim3 grid(static_cast<unsigned>(rows), p.pieces);
+  const cudaError_t err = a->type == 2 ? rows_of<float>(c, p, grid, s) : a->type == 1 ? rows_of<__half>(c, p, grid, s) : rows_of<__nv_bfloat16>(c, p, grid, s);
   if (err != cudaSuccess) return static_cast<int>(err);
-  return static_cast<int>(rbhost::launch_pdl(rb::beam_group_kernel, dim3(a->groups), block, 0, s, 1, p));
+  return static_cast<int>(rbhost::launch_pdl(rb::beam_group_kernel, dim3(a->groups), dim3(rb::kBsThreads), 0, s, 1, p));
 }

@@ -485,3 +485,32 @@ def test_attention_shared_captured_and_twice_the_same():
         g.replay()
         again = call()
         assert torch.equal(out, want) and torch.equal(again, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_beam_select_of_many_rows(dtype):
+    """Rows of several tiles each: random ones, rising, falling, level, with a plateau, and with infinities and NaN; a vocabulary that ends inside a tile, rows that begin on 16
+    bytes and rows that do not."""
+    beams, vocab, groups = 16, 40011, 40
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for pad in (5, 6 if dtype is torch.float32 else 4):
+        x = torch.empty(groups * beams, vocab + pad, device="cuda").normal_(0.0, 2.5, generator=g).to(dtype)[:, :vocab]
+        ramp = torch.linspace(-6, 6, vocab, device="cuda").to(dtype)
+        x[1 * beams:2 * beams] = ramp
+        x[2 * beams:3 * beams] = ramp.flip(0)
+        x[3 * beams:4 * beams] = 0.5
+        x[4 * beams:5 * beams, 7000:30000] = 9.0
+        x[5 * beams:6 * beams, 39000:] = -math.inf
+        x[6 * beams + 1, 5], x[6 * beams + 2, 33333], x[6 * beams + 3, 20000:20007] = math.nan, math.inf, math.inf
+        x[7 * beams:8 * beams] = -math.inf
+        x[7 * beams + 3, 40000:40005] = 1.0
+        scores = -5.0 - torch.rand(groups, beams, generator=g, device="cuda")
+        for count in (3, 32, 128):
+            got = ops.beam_select(x, scores, count)
+            want = ops.beam_select(x.cpu(), scores.cpu(), count)               # the definition in 64 bits, tested above
+            assert torch.equal(got[1].cpu(), want[1]) and torch.equal(got[2].cpu(), want[2])
+            finite = want[0].isfinite()
+            assert torch.equal(got[0].cpu().isfinite(), finite)
+            w = want[0][finite].double()
+            assert ((got[0].cpu()[finite].double() - w).abs() <= 2.0 ** -17 + w.abs() * 2.0 ** -23).all()     # both rounded to fp32
