@@ -71,7 +71,7 @@ shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
     const int hk = s_.vh / list.parts, head0 = (s_.vh - hk * list.parts) * list.per, per = list.per, real = min(per, group - head0);
     const int b = s_.b, rows = s_.n * per, shared = shared_of[s_.g], u0 = s_.u0, u1 = s_.u1;
     const int first = s_.own ? shared : 0, count = s_.own ? sp_length(p, b) - shared : shared;
-    const int* table = p.tables + static_cast<long long>(s_.own ? b : p.starts[s_.g]) * p.width;
+    const int* table = s_.table;
     __syncthreads();                             // the last entry's queries and results have been read
     for (int i = threadIdx.x; i < kRows * LP; i += blockDim.x) {
       const int r = i / LP, c = (i - r * LP) * 8;
@@ -248,76 +248,121 @@ shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
   }
 }
 
-// out[b, head] from the parts of its row: a warp per head, lanes own D / 32 neighbouring columns.  Grid (batch, KV heads).
+// out[b, head] from the parts of its row.  A CTA has a sequence and a KV head; a row's parts are summed by one warp or, where there are fewer heads than warps, by several, and
+// lanes own D / 32 neighbouring columns.  Grid (batch, KV heads).
+constexpr int kSpJoinWarps = 8;
 template <typename T, int D>
-__global__ void __launch_bounds__(kSpWarps * 32)
+__global__ void __launch_bounds__(kSpJoinWarps * 32)
 shared_join_kernel(const SpParams p) {
   pdl_wait();
   pdl_launch();
   constexpr int C = D / 32;
+  __shared__ float sum_sh[kSpJoinWarps][D + 2];  // a warp's columns, maximum and sum
   const int b = blockIdx.x, hk = blockIdx.y, group = p.heads / p.kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = p.group_of[b], tile = b - (b - p.starts[g]) % p.prefix.seqs;
+  const int2 span = p.span_of[b];
   const bool any = sp_length(p, b) > 0;          // a sequence without tokens gets zeros
-  for (int h = warp; h < group; h += kSpWarps) {
-    // parts over shared tokens, then the sequence's own: how many, the CTA of the first, and the rows where the first and those of CTA 0 are
-    int n[2], c0[2];
-    long long row[2], later[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const SpList& l = i == 0 ? p.prefix : p.list;
-      const int e = i == 0 ? tile : p.batch + b, all = l.totals[l.entries], t0 = l.totals[e], t1 = l.totals[e + 1];
-      const int k = h / l.per, vh = hk * l.parts + k, r = (i == 0 ? b - tile : 0) * l.per + h - k * l.per;
-      c0[i] = t1 > t0 ? sp_cta_of(all * l.virtual_heads, l.ctas, vh * all + t0) : 0;
-      n[i] = any && t1 > t0 ? sp_cta_of(all * l.virtual_heads, l.ctas, vh * all + t1 - 1) - c0[i] + 1 : 0;
-      row[i] = sp_row(l, vh, e, 0, true) + r;
-      later[i] = sp_row(l, vh, e, 0, false) + r;
-    }
-    const int parts = n[0] + n[1];
-    auto row_of = [&](int s) -> long long {
-      const int i = s >= n[0] ? 1 : 0, k = s - (i ? n[0] : 0);
-      const SpList& l = i ? p.list : p.prefix;
-      return k == 0 ? row[i] : later[i] + static_cast<long long>(c0[i] + k) * l.seqs * l.per;
-    };
-    auto ml_of = [&](int s) { return (s >= n[0] ? p.list.ml : p.prefix.ml)[row_of(s)]; };
-    float mx = -INFINITY;
-    for (int s = lane; s < parts; s += 32) mx = fmaxf(mx, ml_of(s).x);
-    mx = warp_max(mx);
-    float acc[C], den = 0.f;
+  const int tile = b - (b - span.x) % p.prefix.seqs;
+  // parts of an entry that one of two tiles of rows had alone come in twos (see shared_prefix_tc.cu)
+  const int twin = p.prefix.half > 0 && min(p.prefix.seqs, span.y - tile) <= p.prefix.half ? 2 : 1;
+  // lanes 0, 1: first and last unit over shared tokens, lanes 2, 3: the sequence's own
+  const SpList& look = lane & 2 ? p.list : p.prefix;
+  const int all = look.totals[look.entries], t0 = look.totals[lane & 2 ? look.own + b : tile], t1 = look.totals[(lane & 2 ? look.own + b : tile) + 1];
+  const int share = group < kSpJoinWarps ? kSpJoinWarps / group : 1;      // warps of a row
+  const int at_once = kSpJoinWarps / share;                             // rows
+  for (int h0 = 0; h0 < group; h0 += at_once) {
+    const int h = h0 + warp / share, which = warp % share;
+    const bool mine = warp / share < at_once && h < group;
+    float mx = -INFINITY, den = 0.f, acc[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = 0.f;
-    for (int s0 = 0; s0 < parts; s0 += 32) {
-      float f = 0.f;
-      if (s0 + lane < parts) {
-        const float2 ml = ml_of(s0 + lane);
-        f = ml.x == -INFINITY ? 0.f : wm_ex2(ml.x - mx);
-        den = fmaf(ml.y, f, den);
+    if (mine && any) {
+      // parts over shared tokens, then the sequence's own: how many CTAs, the first, and the rows where its part and those of CTA 0 are
+      const int k_look = h / look.per, u = (hk * look.parts + k_look) * all + (lane & 1 ? t1 - 1 : t0);
+      const int cta = t1 > t0 ? sp_cta_of(all * look.virtual_heads, look.ctas, u) : lane & 1 ? -1 : 0;
+      int n[2], c0[2];
+      long long row[2], later[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const SpList& l = i == 0 ? p.prefix : p.list;
+        const int e = i == 0 ? tile : l.own + b, k = h / l.per, vh = hk * l.parts + k, r = (i == 0 ? b - tile : 0) * l.per + h - k * l.per;
+        c0[i] = __shfl_sync(0xffffffffu, cta, 2 * i);
+        n[i] = __shfl_sync(0xffffffffu, cta, 2 * i + 1) - c0[i] + 1;
+        row[i] = sp_row(l, vh, e, 0, true) + r;
+        later[i] = sp_row(l, vh, e, 0, false) + r;
       }
-      const int m = min(32, parts - s0);
-#pragma unroll 4
-      for (int s = 0; s < m; ++s) {
-        const float fs = __shfl_sync(0xffffffffu, f, s);
-        const float* x = (s0 + s >= n[0] ? p.list.acc : p.prefix.acc) + row_of(s0 + s) * D + lane * C;
-        float v[C];
-        if (C == 4) {
-          const float4 w = *reinterpret_cast<const float4*>(x);
-          v[0] = w.x; v[1] = w.y; v[2 % C] = w.z; v[3 % C] = w.w;
-        } else {
-          const float2 w = *reinterpret_cast<const float2*>(x);
-          v[0] = w.x; v[1] = w.y;
+      n[0] *= twin;
+      const int parts = n[0] + n[1];
+      for (int s0 = which; s0 < parts; s0 += 32 * share) {
+        // a lane looks up one part
+        const int s = s0 + lane * share;
+        const float* columns = nullptr;
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (s < parts) {
+          const int i = s >= n[0] ? 1 : 0, j = i ? s - n[0] : twin == 2 ? s >> 1 : s;
+          const SpList& l = i ? p.list : p.prefix;
+          long long at = j == 0 ? row[i] : later[i] + static_cast<long long>(c0[i] + j) * l.seqs * l.per;
+          if (!i && twin == 2 && (s & 1)) at += l.rows;
+          ml = l.ml[at];
+          columns = l.acc + at * D;
         }
+        const float top = fmaxf(mx, warp_max(ml.x)), from = top == -INFINITY ? 0.f : top, again = wm_ex2(mx - from);
+        const float f = wm_ex2(ml.x - from);
+        den = fmaf(den, again, ml.y * f);
 #pragma unroll
-        for (int c = 0; c < C; ++c) acc[c] = fmaf(v[c], fs, acc[c]);
+        for (int c = 0; c < C; ++c) acc[c] *= again;
+        mx = top;
+        const int m = min(32, (parts - s0 + share - 1) / share);
+#pragma unroll 8
+        for (int k = 0; k < m; ++k) {
+          const float fk = __shfl_sync(0xffffffffu, f, k);
+          const float* x = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(columns), k)) + lane * C;
+          if (fk != 0.f) {                       // a part without tokens has no sums
+            if (C == 4) {
+              const float4 v = *reinterpret_cast<const float4*>(x);
+              acc[0] = fmaf(v.x, fk, acc[0]); acc[1] = fmaf(v.y, fk, acc[1]); acc[2 % C] = fmaf(v.z, fk, acc[2 % C]); acc[3 % C] = fmaf(v.w, fk, acc[3 % C]);
+            } else {
+              const float2 v = *reinterpret_cast<const float2*>(x);
+              acc[0] = fmaf(v.x, fk, acc[0]); acc[1] = fmaf(v.y, fk, acc[1]);
+            }
+          }
+        }
       }
+      den = warp_sum(den);
     }
-    den = warp_sum(den);
-    const float inv = parts > 0 ? 1.f / den : 0.f;
-    T* o = static_cast<T*>(p.out) + b * p.ld_o + static_cast<long long>(hk * group + h) * D + lane * C;
-    uint32_t w[C / 2];
+    if (share > 1) {
 #pragma unroll
-    for (int c = 0; c < C / 2; ++c) w[c] = sp_pack<T>(acc[2 * c] * inv, acc[2 * c + 1] * inv);
-    if (C == 4) *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1 % (C / 2)]);
-    else *reinterpret_cast<uint32_t*>(o) = w[0];
+      for (int c = 0; c < C; ++c) sum_sh[warp][lane * C + c] = acc[c];
+      if (lane == 0) {
+        sum_sh[warp][D] = mx;
+        sum_sh[warp][D + 1] = den;
+      }
+      __syncthreads();
+      if (mine && which == 0) {
+        float top = mx;
+        for (int w = 1; w < share; ++w) top = fmaxf(top, sum_sh[warp + w][D]);
+        const float from = top == -INFINITY ? 0.f : top, f0 = wm_ex2(mx - from);
+        den *= f0;
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] *= f0;
+        for (int w = 1; w < share; ++w) {
+          const float f = wm_ex2(sum_sh[warp + w][D] - from);
+          den = fmaf(sum_sh[warp + w][D + 1], f, den);
+#pragma unroll
+          for (int c = 0; c < C; ++c) acc[c] = fmaf(sum_sh[warp + w][lane * C + c], f, acc[c]);
+        }
+      }
+      __syncthreads();
+    }
+    if (mine && which == 0) {
+      const float inv = any ? 1.f / den : 0.f;
+      T* o = static_cast<T*>(p.out) + b * p.ld_o + static_cast<long long>(hk * group + h) * D + lane * C;
+      uint32_t w[C / 2];
+#pragma unroll
+      for (int c = 0; c < C / 2; ++c) w[c] = sp_pack<T>(acc[2 * c] * inv, acc[2 * c + 1] * inv);
+      if (C == 4) *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1 % (C / 2)]);
+      else *reinterpret_cast<uint32_t*>(o) = w[0];
+    }
   }
 }
 
@@ -331,12 +376,12 @@ struct Plan {
   int tiles;                                     // m-tiles of the split kernel
   bool tc;
 };
-// Shared tokens of groups with more than 32 rows go to the tcgen05 kernel, which takes 256 at a time; the split kernel has one m-tile, or two where rows need them.
-Plan plan_of(int batch, int heads, int kv_heads, int head_dim, int block_size, int most, bool positive) {
+// Shared tokens of groups with more than 16 rows go to the tcgen05 kernel, which takes 256 at a time; the split kernel has one m-tile, or two where rows need them.
+Plan plan_of(int batch, int groups, int heads, int kv_heads, int head_dim, int block_size, int most, bool positive) {
   Plan p;
   memset(&p, 0, sizeof(p));
   const int group = heads / kv_heads;
-  p.tc = static_cast<long long>(most) * group > 32 && positive && rbhost::shared_tc_takes(batch, heads, kv_heads, block_size, most);
+  p.tc = static_cast<long long>(most) * group > 16 && positive && rbhost::shared_tc_takes(batch, heads, kv_heads, block_size, most);
   p.tiles = static_cast<long long>(p.tc ? 1 : most) * group > 16 ? 2 : 1;
   const int rows = 16 * p.tiles;
   rb::SpList& l = p.list;
@@ -345,19 +390,20 @@ Plan plan_of(int batch, int heads, int kv_heads, int head_dim, int block_size, i
   l.parts = (group + l.per - 1) / l.per;
   l.seqs = rows / l.per;
   l.virtual_heads = kv_heads * l.parts;
-  l.entries = 2 * batch;
-  l.skip = p.tc ? batch : 0;
+  l.own = p.tc ? 0 : batch;
+  l.entries = l.own + batch;
   const size_t tiles = head_dim == 64 ? (p.tiles == 1 ? rb::SpSmem<64, 1>::kTotals : rb::SpSmem<64, 2>::kTotals)
                                       : (p.tiles == 1 ? rb::SpSmem<128, 1>::kTotals : rb::SpSmem<128, 2>::kTotals);
-  p.smem = tiles + (3 * static_cast<size_t>(batch) + 1) * 4;
+  p.smem = tiles + (static_cast<size_t>(l.entries) + 1 + groups) * 4;
   const int resident = static_cast<int>((228 * 1024) / (p.smem + 1024 + 64)), most_resident = p.tiles == 1 ? 3 : 2;
   l.ctas = rbhost::device_sm_count() * (resident < 1 ? 1 : resident < most_resident ? resident : most_resident);
+  l.rows = rbhost::sp_list_rows(l);
   p.prefix = p.tc ? rbhost::shared_tc_list(batch, heads, kv_heads) : l;
   return p;
 }
 // Puts a list's arrays at `at` (NULL: only counts) and returns their size.
 long long place(rb::SpList& l, char* at, int head_dim) {
-  const long long totals = ((l.entries + 1) * 4ll + 15) / 16 * 16, rows = rbhost::sp_list_rows(l), ml = (rows * 8 + 15) / 16 * 16;
+  const long long totals = ((l.entries + 1) * 4ll + 15) / 16 * 16, rows = l.rows * (l.half > 0 ? 2 : 1), ml = (rows * 8 + 15) / 16 * 16;
   if (at) {
     l.totals = reinterpret_cast<int*>(at);
     l.ml = reinterpret_cast<float2*>(at + totals);
@@ -385,16 +431,16 @@ template <typename T, int D>
 cudaError_t both(const rb::SpParams& p, const Plan& l, cudaStream_t s) {
   const cudaError_t e = l.tiles == 1 ? split<T, D, 1>(p, l, s) : split<T, D, 2>(p, l, s);
   if (e != cudaSuccess) return e;
-  return rbhost::launch_pdl(rb::shared_join_kernel<T, D>, dim3(p.batch, p.kv_heads), dim3(rb::kSpWarps * 32), 0, s, 1, p);
+  return rbhost::launch_pdl(rb::shared_join_kernel<T, D>, dim3(p.batch, p.kv_heads), dim3(rb::kSpJoinWarps * 32), 0, s, 1, p);
 }
 
 }  // namespace
 
-RB_API long long rb_shared_prefix_scratch_bytes(int batch, int heads, int kv_heads, int head_dim, int block_size, int most_rows) {
+RB_API long long rb_shared_prefix_scratch_bytes(int batch, int groups, int heads, int kv_heads, int head_dim, int block_size, int most_rows) {
   if (!sound(batch, heads, kv_heads, head_dim, block_size) || batch == 0) return 16;
   long long most = 0;
   for (int positive = 0; positive < 2; ++positive) {
-    Plan l = plan_of(batch, heads, kv_heads, head_dim, block_size, most_rows, positive != 0);
+    Plan l = plan_of(batch, groups, heads, kv_heads, head_dim, block_size, most_rows, positive != 0);
     const long long n = place(l.list, nullptr, head_dim) + (l.tc ? place(l.prefix, nullptr, head_dim) : 0);
     if (n > most) most = n;
   }
@@ -404,13 +450,13 @@ RB_API long long rb_shared_prefix_scratch_bytes(int batch, int heads, int kv_hea
 RB_API int rb_shared_prefix(const RbSharedPrefixArgs* a, void* stream) {
   if (!a || !sound(a->batch, a->heads, a->kv_heads, a->head_dim, a->block_size)) return -1;
   if (a->batch == 0) return 0;
-  if (!a->q || !a->out || !a->k_cache || !a->v_cache || !a->block_tables || !a->context_lens || !a->shared_lens || !a->starts || !a->group_of || !a->scratch ||
+  if (!a->q || !a->out || !a->k_cache || !a->v_cache || !a->block_tables || !a->context_lens || !a->shared_lens || !a->group_of || !a->span_of || reinterpret_cast<unsigned long long>(a->span_of) % 8 || !a->scratch ||
       a->groups < 1 || a->groups > a->batch || a->max_blocks < 1 || a->num_blocks < 1 || a->type < 0 || a->type > 1 || a->most_rows < 1 || a->most_rows > a->batch)
     return -1;
   if ((reinterpret_cast<unsigned long long>(a->q) | reinterpret_cast<unsigned long long>(a->out) | reinterpret_cast<unsigned long long>(a->k_cache) |
        reinterpret_cast<unsigned long long>(a->v_cache)) & 15 || a->ld_q % 8 || a->ld_o % 8)
     return -2;
-  Plan l = plan_of(a->batch, a->heads, a->kv_heads, a->head_dim, a->block_size, a->most_rows, a->scale > 0.f);
+  Plan l = plan_of(a->batch, a->groups, a->heads, a->kv_heads, a->head_dim, a->block_size, a->most_rows, a->scale > 0.f);
   const long long cap = static_cast<long long>(a->max_blocks) * a->block_size;
   if (a->num_blocks * a->block_size > 0x7fffffffll || cap > (1ll << 30) ||
       2ll * a->batch * ((cap + rb::kSpUnit - 1) / rb::kSpUnit) * l.list.virtual_heads > 0x7fffffffll || l.smem > 227 * 1024)
@@ -418,7 +464,8 @@ RB_API int rb_shared_prefix(const RbSharedPrefixArgs* a, void* stream) {
   rb::SpParams p;
   memset(&p, 0, sizeof(p));
   p.q = a->q; p.out = a->out; p.k = a->k_cache; p.v = a->v_cache;
-  p.tables = a->block_tables; p.lens = a->context_lens; p.shared = a->shared_lens; p.starts = a->starts; p.group_of = a->group_of;
+  p.tables = a->block_tables; p.lens = a->context_lens; p.shared = a->shared_lens; p.group_of = a->group_of;
+  p.span_of = reinterpret_cast<const int2*>(a->span_of);
   p.ld_q = a->ld_q; p.ld_o = a->ld_o; p.num_blocks = a->num_blocks;
   p.batch = a->batch; p.groups = a->groups; p.width = a->max_blocks; p.block_size = a->block_size; p.heads = a->heads; p.kv_heads = a->kv_heads;
   p.cap = static_cast<int>(cap); p.scale = a->scale;

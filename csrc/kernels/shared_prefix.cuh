@@ -12,15 +12,17 @@ namespace rb {
 constexpr int kSpUnit = 128;                     // tokens
 constexpr float kSpLog2e = 1.4426950408889634f;
 
-// The units of `first` .. entries, for each of the virtual KV heads one after the other, dealt in equal runs to `ctas` CTAs.  Entry e < batch is the tile of
-// rows that begins with sequence e (if one does) over the group's shared tokens, entry batch + b are sequence b's rows over its own.
+// Entries and their units.  A list has the tiles of rows over shared tokens (tiles: entry b is the tile that begins with sequence b, if one does), the sequences' own tokens
+// (own: one entry a sequence), or both, tiles first.  The units of all entries, for each of the virtual KV heads one after the other, are dealt in equal runs to `ctas` CTAs.
 struct SpList {
   int* totals;                                   // [entries + 1] running totals of units
   float2* ml;                                    // maximum (base 2) and sum of every row's part
   float* acc;                                    // [part][head_dim]
-  int entries, skip;                             // skip: entries in front that have no units here
+  int entries, own;                              // own: the first entry of a sequence's own tokens
   int per, parts, virtual_heads;                 // a KV head's query heads in `parts` equal parts of `per`, so that a sequence's rows fit a tile
   int ctas, seqs;                                // seqs: sequences of a tile
+  int half;                                      // > 0: parts of entries of at most so many sequences come in twos, the second `rows` behind the first
+  long long rows;                                // of parts
 };
 struct SpParams {
   const void* q;
@@ -30,8 +32,8 @@ struct SpParams {
   const int* tables;
   const int* lens;
   const int* shared;
-  const int* starts;
-  const int* group_of;
+  const int* group_of;                           // [batch]
+  const int2* span_of;                           // [batch] first sequence of the sequence's group and of the next
   long long ld_q, ld_o, num_blocks;
   int batch, groups, width, block_size, heads, kv_heads;
   int cap;                                       // tokens of a table's row
@@ -58,9 +60,8 @@ __device__ __forceinline__ void sp_shared(const SpParams& p, int* shared) {
 }
 // Units of entry e: tiles of rows begin at every `seqs`-th sequence of a group.
 __device__ __forceinline__ int sp_units(const SpParams& p, const SpList& l, const int* shared_of, int e) {
-  if (e < l.skip) return 0;
-  const int b = e < p.batch ? e : e - p.batch, g = p.group_of[b], shared = shared_of[g];
-  if (e < p.batch) return (b - p.starts[g]) % l.seqs == 0 ? (shared + kSpUnit - 1) / kSpUnit : 0;
+  const int b = e < l.own ? e : e - l.own, shared = shared_of[p.group_of[b]];
+  if (e < l.own) return (b - p.span_of[b].x) % l.seqs == 0 ? (shared + kSpUnit - 1) / kSpUnit : 0;
   return max(0, sp_length(p, b) - shared + kSpUnit - 1) / kSpUnit;
 }
 // Running totals of the units of all entries, [entries + 1], formed by all threads of a CTA.
@@ -104,6 +105,7 @@ __device__ __forceinline__ int sp_cta_of(int total, int ctas, int u) {
 struct SpPart {
   int vh, e, u0, u1;
   int b, g, n;                                   // first sequence, group, sequences of the tile
+  const int* table;
   bool own;
 };
 // The part that a run u .. u_end begins with; u goes behind it.  Every thread that calls it gets the same.
@@ -121,18 +123,20 @@ __device__ __forceinline__ SpPart sp_next(const SpParams& p, const SpList& l, co
   s.e = e;
   s.u0 = at - totals[e];
   s.u1 = min(totals[e + 1], at + u_end - u) - totals[e];
-  s.own = e >= p.batch;
-  s.b = s.own ? e - p.batch : e;
+  s.own = e >= l.own;
+  s.b = s.own ? e - l.own : e;
   s.g = p.group_of[s.b];
-  s.n = s.own ? 1 : min(l.seqs, p.starts[s.g + 1] - s.b);
+  const int2 span = p.span_of[s.b];
+  s.n = s.own ? 1 : min(l.seqs, span.y - s.b);
+  s.table = p.tables + static_cast<long long>(s.own ? s.b : span.x) * p.width;
   u += s.u1 - s.u0;
   return s;
 }
 // Where a part's row 0 goes, rows (sequence, head) one behind the other.  A part that begins its entry has places of the entry's own; one that goes on with it is the
 // first of its CTA's run and has the CTA's.
 __device__ __forceinline__ long long sp_row(const SpList& l, int vh, int e, int cta, bool begins) {
-  const long long heads = static_cast<long long>(l.entries - l.skip) * l.per;
-  return begins ? vh * heads + static_cast<long long>(e - l.skip) * l.per : l.virtual_heads * heads + static_cast<long long>(cta) * l.seqs * l.per;
+  const long long heads = static_cast<long long>(l.entries) * l.per;
+  return begins ? vh * heads + static_cast<long long>(e) * l.per : l.virtual_heads * heads + static_cast<long long>(cta) * l.seqs * l.per;
 }
 
 template <typename T>
@@ -150,7 +154,7 @@ __device__ __forceinline__ uint32_t sp_pack<__half>(float lo, float hi) {
 namespace rbhost {
 // Rows of partial results of a list.
 inline long long sp_list_rows(const rb::SpList& l) {
-  return static_cast<long long>(l.virtual_heads) * (l.entries - l.skip) * l.per + static_cast<long long>(l.ctas) * l.seqs * l.per;
+  return static_cast<long long>(l.virtual_heads) * l.entries * l.per + static_cast<long long>(l.ctas) * l.seqs * l.per;
 }
 // shared_prefix_tc.cu: the parts over shared tokens with tcgen05
 bool shared_tc_takes(int batch, int heads, int kv_heads, int block_size, int most);

@@ -1,6 +1,6 @@
 // C interface of decode attention for sequences that share their first tokens (shared_prefix.cu).
 //
-// Sequences come in groups: starts [groups + 1] are the groups' first sequences and the end, group_of [batch] every sequence's group.  The first
+// Sequences come in groups: group_of [batch] is every sequence's group, span_of [batch, 2] the first sequence of that group and of the next.  The first
 // shared_lens[g] tokens of a group's sequences are the same and are read through the block table of its first one; what follows of the context_lens[b]
 // tokens of sequence b through its own.  Of a group whose shortest sequence (those without tokens aside) has fewer tokens than shared_lens[g], only that many count
 // as shared.  A sequence without tokens gets zeros.
@@ -21,14 +21,14 @@ typedef struct RbSharedPrefixArgs {
   const int* block_tables;   // [batch, max_blocks]
   const int* context_lens;   // [batch]
   const int* shared_lens;    // [groups]
-  const int* starts;
   const int* group_of;
+  const int* span_of;        // 8-byte aligned
   void* scratch;
   long long ld_q, ld_o, num_blocks;
   int batch, groups, max_blocks, block_size, heads, kv_heads, head_dim, type, most_rows;   // most_rows: sequences of the largest group
   float scale;
 } RbSharedPrefixArgs;
-long long rb_shared_prefix_scratch_bytes(int batch, int heads, int kv_heads, int head_dim, int block_size, int most_rows);
+long long rb_shared_prefix_scratch_bytes(int batch, int groups, int heads, int kv_heads, int head_dim, int block_size, int most_rows);
 int rb_shared_prefix(const RbSharedPrefixArgs* args, void* stream);
 #ifdef __cplusplus
 }

@@ -3,7 +3,8 @@
 // A CTA goes through its run of units (128 tokens each; see shared_prefix.cuh) with two tiles of 128 rows, A and B, that share every tile of keys and values.  TMEM holds
 // S_A, S_B (128 fp32 columns each) and the accumulators O_A, O_B (a head's columns each).  For unit j one thread issues
 //     PV(j, A)  O_A += P_A V_j   (P from TMEM, V_j row by row from shared memory),   QK(j + 1, A)  S_A = Q_A K_j+1^T,   PV(j, B),   QK(j + 1, B),
-// so that the tensor cores work for one tile while the other tile's softmax runs, one row per thread.  A row keeps its maximum until a new one is more than 2^8 larger, O
+// so that the tensor cores work for one tile while the other tile's softmax runs, one row per thread.  Where all rows fit one tile, A takes the run's even units and B the
+// odd ones with the same queries, and a part has two sums.  A row keeps its maximum until a new one is more than 2^8 larger, O
 // stays in TMEM meanwhile.  Pages come by TMA, a copy per page and 64 columns, into rings of stages that go on from one part of the run to the next; the next part's
 // queries are loaded as soon as the last product that reads the old ones is done.  A part's sums leave as they are, fp32 with the row's maximum and
 // sum, for the join (shared_prefix.cu).
@@ -21,7 +22,7 @@
 
 namespace rb {
 
-constexpr int kStThreads = 384;          // warps 0-7 softmax, 8 TMA, 9 MMA, 10-11 only give their registers away
+constexpr int kStThreads = 384;          // warps 0-7 softmax, 8 and 10 TMA, 9 MMA, 11 only gives its registers away
 constexpr int kStTile = 128;
 constexpr float kStRescale = 8.f;        // log2 units
 constexpr int kStMostBatch = 2048;       // running totals beside 192 KB of tiles
@@ -106,73 +107,72 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
   const uint32_t tmem_base = *tmem_ptr;
   const int total = totals[list.entries] * list.virtual_heads, group = p.heads / p.kv_heads;
   const int u_begin = sp_run(total, list.ctas, blockIdx.x), u_end = sp_run(total, list.ctas, blockIdx.x + 1);
-  const int half = kStTile / list.per;                         // sequences of one of the two tiles
+  const int half = list.half;                                  // sequences of one of the two tiles
   const int tile_rows = half * list.per;
 
   if (warp >= 8) {
     setmaxnreg_dec<56>();
-    if (warp == 8) {
-      // ---------------------------------------------------------------- TMA producer, all lanes
+    if (warp == 8 || warp == 10) {
+      // ---------------------------------------------------------------- TMA producers, all lanes: warp 8 queries and keys, warp 10 values
+      const bool values = warp == 10;
+      const CUtensorMap* map = values ? &maps.v : &maps.k;
+      const uint32_t tiles = values ? sV : sK, full = values ? bar_vfull : bar_kfull, empty = values ? bar_vempty : bar_kempty;
+      const int bs = p.block_size, size = min(bs, kSpUnit);    // rows of a copy
       bool ok = true;
       int it = 0, part = 0, tails = 0;
       for (int u = u_begin; u < u_end && ok; ++part) {
         const SpPart s = sp_next(p, list, totals, u, u_end);
         const int shared = shared_of[s.g], head0 = s.vh * list.per;
-        const int* table = p.tables + static_cast<long long>(p.starts[s.g]) * p.width;
-        if (part > 0) ok = mbar_wait(bar_qfree, (part - 1) & 1, abort_flag, status, 51);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        if (lane == 0) {
-          const int tiles = s.n > half ? 2 : 1;
-          mbar_arrive_expect_tx(bar_q, tiles * tile_rows * 128 * (D / 64));
-          for (int t = 0; t < tiles; ++t)
+        // pages of a unit: lane i has the i-th (one of 128 rows, from `row` on, where pages are larger); looked up a unit ahead
+        auto page_of = [&](int unit) {
+          const int at = unit * kSpUnit + lane * size;
+          return unit < s.u1 && lane * size < kSpUnit && at < shared ? s.table[at / bs] : 0;
+        };
+        int page = page_of(s.u0);
+        if (!values) {
+          if (part > 0) ok = mbar_wait(bar_qfree, (part - 1) & 1, abort_flag, status, 51);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          if (lane == 0) {
+            const int n = s.n > half ? 2 : 1;
+            mbar_arrive_expect_tx(bar_q, n * tile_rows * 128 * (D / 64));
+            for (int t = 0; t < n; ++t)
 #pragma unroll
-            for (int hf = 0; hf < D / 64; ++hf)
-              tma_load_4d(sQ + t * L::kTileBytes + hf * L::kHalf, &maps.q, hf * 64, head0, s.b + t * half, 0, bar_q);
-        }
-        for (int unit = s.u0; unit < s.u1 && ok; ++unit, ++it) {
-          const int st = it % kStages, use = it / kStages, first = unit * kSpUnit, valid = min(kSpUnit, shared - first);
-          // pages of the unit: lane i has the i-th (one of 128 rows, from `row` on, where pages are larger)
-          const int bs = p.block_size, size = min(bs, kSpUnit), pages = (valid + size - 1) / size;
-          int blk = 0, row = 0;
-          if (lane < pages) {
-            const int page = (first + lane * size) / bs;
-            row = first + lane * size - page * bs;
-            blk = table[page];
-            if (blk < 0 || blk >= p.num_blocks) {              // corrupt tables read block 0 instead of faulting
-              RB_BOUNDS_HIT(104);
-              blk = 0;
-            }
+              for (int hf = 0; hf < D / 64; ++hf)
+                tma_load_4d(sQ + t * L::kTileBytes + hf * L::kHalf, &maps.q, hf * 64, head0, s.b + t * half, 0, bar_q);
           }
-          const uint32_t bytes = pages * size * 128 * (D / 64);
-          auto load = [&](const CUtensorMap* m, uint32_t tile, uint32_t bar) {
-            if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
-            __syncwarp();
-            if (lane < pages) {
+        }
+        for (int unit = s.u0; unit < s.u1; ++unit, ++it) {
+          const int st = it % kStages, first = unit * kSpUnit, valid = min(kSpUnit, shared - first), pages = (valid + size - 1) / size;
+          int blk = page;
+          if (lane < pages && (blk < 0 || blk >= p.num_blocks)) {      // corrupt tables read block 0 instead of faulting
+            RB_BOUNDS_HIT(104);
+            blk = 0;
+          }
+          page = page_of(unit + 1);
+          const int row = first % bs * (bs > kSpUnit);
+          const uint32_t tile = tiles + st * L::kTileBytes;
+          const bool tail = values && valid < kSpUnit;
+          const uint32_t bar = tail ? bar_tail : full + 8 * st;
+          ok = mbar_wait(empty + 8 * st, (it / kStages & 1) ^ 1, abort_flag, status, 52 + values);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          if (lane == 0) mbar_arrive_expect_tx(bar, pages * size * 128 * (D / 64));
+          __syncwarp();
+          if (lane < pages) {
 #pragma unroll
-              for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(tile + hf * L::kHalf + lane * size * 128, m, hf * 64, s.vh, row, blk, bar);
-            }
-          };
-          if (!mbar_wait(bar_kempty + 8 * st, (use & 1) ^ 1, abort_flag, status, 52)) ok = false;
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          load(&maps.k, sK + st * L::kTileBytes, bar_kfull + 8 * st);
-          if (!mbar_wait(bar_vempty + 8 * st, (use & 1) ^ 1, abort_flag, status, 53)) ok = false;
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          const uint32_t v_tile = sV + st * L::kTileBytes;
-          if (valid == kSpUnit) {
-            load(&maps.v, v_tile, bar_vfull + 8 * st);
-          } else {
+            for (int hf = 0; hf < D / 64; ++hf) tma_load_4d(tile + hf * L::kHalf + lane * size * 128, map, hf * 64, s.vh, row, blk, bar);
+          }
+          if (tail) {
             // the copies land, then the rows behind the last token become zero, then the tile is full
-            load(&maps.v, v_tile, bar_tail);
-            if (!mbar_wait(bar_tail, tails & 1, abort_flag, status, 54)) ok = false;
+            ok = mbar_wait(bar_tail, tails & 1, abort_flag, status, 54);
             ++tails;
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-            uint8_t* tile = smem + L::kV + st * L::kTileBytes;
+            uint8_t* rows = smem + L::kV + st * L::kTileBytes + valid * 128;
             for (int i = lane; i < (kSpUnit - valid) * 8; i += 32)
 #pragma unroll
-              for (int hf = 0; hf < D / 64; ++hf) *reinterpret_cast<uint4*>(tile + hf * L::kHalf + valid * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+              for (int hf = 0; hf < D / 64; ++hf) *reinterpret_cast<uint4*>(rows + hf * L::kHalf + i * 16) = make_uint4(0u, 0u, 0u, 0u);
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_vfull + 8 * st);
+            if (lane == 0) mbar_arrive(full + 8 * st);
           }
         }
       }
@@ -186,11 +186,12 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
         constexpr uint32_t idesc_pv = umma_idesc_bf16(128, D, 0, 1) & ~drop; // A = P (TMEM), B = V, rows along the sum
         bool ok = true;
         int it = 0, part = 0, done[2] = {0, 0};
-        auto issue_qk = [&](int i, int t) -> bool {
+        // S_t = Q_tile K_i^T
+        auto issue_qk = [&](int i, int t, int tile) -> bool {
           const int st = i % kStages;
           if (!mbar_wait(bar_kfull + 8 * st, (i / kStages) & 1, abort_flag, status, 55)) return false;
           tc_fence_after();
-          const uint64_t q = dQ + t * (L::kTileBytes / 16), k = dK + st * (L::kTileBytes / 16);
+          const uint64_t q = dQ + tile * (L::kTileBytes / 16), k = dK + st * (L::kTileBytes / 16);
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks) {
             const uint64_t off = (ks >> 2) * (L::kHalf / 16) + (ks & 3) * 2;
@@ -199,33 +200,57 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
           umma_commit(bar_sfull + 8 * t);
           return true;
         };
+        // O_t (+)= P_t V_i, once P_t is there
+        auto issue_pv = [&](int i, int t, bool add) -> bool {
+          if (!mbar_wait(bar_pfull + 8 * t, done[t] & 1, abort_flag, status, 58)) return false;
+          ++done[t];
+          tc_fence_after();
+          const uint32_t tmem_p = tmem_base + t * 128, tmem_o = tmem_base + 256 + t * 128;
+          const uint64_t v = dV + (i % kStages) * (L::kTileBytes / 16);
+#pragma unroll
+          for (int ks = 0; ks < kSpUnit / 16; ++ks)
+            umma_bf16_ts(tmem_o, tmem_p + ks * 8, v + ks * (2048 / 16), idesc_pv, (add || ks != 0) ? 1u : 0u);
+          umma_commit(bar_oready + 8 * t);
+          return true;
+        };
         for (int u = u_begin; u < u_end && ok; ++part) {
           const SpPart s = sp_next(p, list, totals, u, u_end);
-          const int n = s.u1 - s.u0, tiles = s.n > half ? 2 : 1;
+          const int n = s.u1 - s.u0;
           ok = mbar_wait(bar_q, part & 1, abort_flag, status, 56);
-          for (int t = 0; t < tiles && ok; ++t) ok = issue_qk(it, t);
-          if (!ok) break;
-          umma_commit(bar_kempty + 8 * (it % kStages));
-          if (n == 1) umma_commit(bar_qfree);
-          for (int j = 0; j < n && ok; ++j) {
-            const int i = it + j, st = i % kStages;
-            if (!mbar_wait(bar_vfull + 8 * st, (i / kStages) & 1, abort_flag, status, 57)) { ok = false; break; }
-            for (int t = 0; t < tiles; ++t) {
-              if (!mbar_wait(bar_pfull + 8 * t, done[t] & 1, abort_flag, status, 58)) { ok = false; break; }
-              ++done[t];
-              tc_fence_after();
-              const uint32_t tmem_p = tmem_base + t * 128, tmem_o = tmem_base + 256 + t * 128;
-              const uint64_t v = dV + st * (L::kTileBytes / 16);
-#pragma unroll
-              for (int ks = 0; ks < kSpUnit / 16; ++ks)
-                umma_bf16_ts(tmem_o, tmem_p + ks * 8, v + ks * (2048 / 16), idesc_pv, (j > 0 || ks != 0) ? 1u : 0u);
-              umma_commit(bar_oready + 8 * t);
-              if (j + 1 < n && !issue_qk(i + 1, t)) { ok = false; break; }   // overwrites S_t / P_t: ordered behind PV(j, t)
-            }
+          if (s.n > half) {                                      // two tiles of rows
+            for (int t = 0; t < 2 && ok; ++t) ok = issue_qk(it, t, t);
             if (!ok) break;
-            umma_commit(bar_vempty + 8 * st);
-            if (j + 1 < n) umma_commit(bar_kempty + 8 * ((i + 1) % kStages));
-            if (j + 2 == n) umma_commit(bar_qfree);              // the last products that read the queries have been issued
+            umma_commit(bar_kempty + 8 * (it % kStages));
+            if (n == 1) umma_commit(bar_qfree);
+            for (int j = 0; j < n && ok; ++j) {
+              const int i = it + j, st = i % kStages;
+              if (!mbar_wait(bar_vfull + 8 * st, (i / kStages) & 1, abort_flag, status, 57)) { ok = false; break; }
+              for (int t = 0; t < 2; ++t) {
+                if (!issue_pv(i, t, j > 0)) { ok = false; break; }
+                if (j + 1 < n && !issue_qk(i + 1, t, t)) { ok = false; break; }   // overwrites S_t / P_t: ordered behind PV(j, t)
+              }
+              if (!ok) break;
+              umma_commit(bar_vempty + 8 * st);
+              if (j + 1 < n) umma_commit(bar_kempty + 8 * ((i + 1) % kStages));
+              if (j + 2 == n) umma_commit(bar_qfree);            // the last products that read the queries have been issued
+            }
+          } else {                                               // one: units in turn with the S and O of A and of B
+            for (int j = 0; j < 2 && j < n && ok; ++j) {
+              ok = issue_qk(it + j, j, 0);
+              if (!ok) break;
+              umma_commit(bar_kempty + 8 * ((it + j) % kStages));
+              if (j + 1 == n) umma_commit(bar_qfree);
+            }
+            for (int j = 0; j < n && ok; ++j) {
+              const int i = it + j, st = i % kStages;
+              if (!mbar_wait(bar_vfull + 8 * st, (i / kStages) & 1, abort_flag, status, 57) || !issue_pv(i, j & 1, j > 1)) { ok = false; break; }
+              umma_commit(bar_vempty + 8 * st);
+              if (j + 2 < n) {
+                if (!issue_qk(i + 2, j & 1, 0)) { ok = false; break; }
+                umma_commit(bar_kempty + 8 * ((i + 2) % kStages));
+                if (j + 3 == n) umma_commit(bar_qfree);
+              }
+            }
           }
           it += n;
         }
@@ -243,10 +268,10 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
     int done = 0;
     for (int u = u_begin; u < u_end && ok;) {
       const SpPart s = sp_next(p, list, totals, u, u_end);
-      if (t == 1 && s.n <= half) continue;                     // no rows for tile B
-      const int shared = shared_of[s.g];
+      const bool twin = s.n <= half;                           // one tile of rows: A has the part's even units, B the odd ones
+      const int shared = shared_of[s.g], step = twin ? 2 : 1, j0 = s.u0 + (twin ? t : 0);
       float m_run = -INFINITY, l_run = 0.f;
-      for (int j = s.u0; j < s.u1; ++j, ++done) {
+      for (int j = j0; j < s.u1; j += step, ++done) {
         if (!mbar_wait(bar_sfull + 8 * t, done & 1, abort_flag, status, 59)) { ok = false; break; }
         tc_fence_after();
         uint32_t r[128];
@@ -275,7 +300,7 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
           m_run = mx;
           l_run *= alpha;
         }
-        if (j > s.u0 && __any_sync(0xffffffffu, grow)) {
+        if (j > j0 && __any_sync(0xffffffffu, grow)) {
           // O has the sum over the units in front once their last product is done; the next one cannot start before P below
           if (!mbar_wait(bar_oready + 8 * t, (done - 1) & 1, abort_flag, status, 60)) { ok = false; break; }
           tc_fence_after();
@@ -312,12 +337,14 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
       }
       if (!ok) break;
       // ---- the part's sums
-      if (!mbar_wait(bar_oready + 8 * t, (done - 1) & 1, abort_flag, status, 61)) break;
+      const bool some = j0 < s.u1;
+      if (some && !mbar_wait(bar_oready + 8 * t, (done - 1) & 1, abort_flag, status, 61)) break;
       tc_fence_after();
-      const int seq = t * half + row / list.per, h = row % list.per;
+      const int seq = (twin ? 0 : t * half) + row / list.per, h = row % list.per;
       const bool real = row < tile_rows && seq < s.n && h < group - (s.vh % list.parts) * list.per;
-      const long long to = sp_row(list, s.vh, s.e, blockIdx.x, s.u0 == 0) + seq * list.per + h;
+      const long long to = sp_row(list, s.vh, s.e, blockIdx.x, s.u0 == 0) + seq * list.per + h + (twin && t ? list.rows : 0);
       if (real) list.ml[to] = make_float2(m_run * sl2, l_run);
+      if (!some) continue;                                     // a part of one unit: B has none
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -395,12 +422,14 @@ bool shared_tc_takes(int batch, int heads, int kv_heads, int block_size, int mos
 rb::SpList shared_tc_list(int batch, int heads, int kv_heads) {
   rb::SpList l;
   memset(&l, 0, sizeof(l));
-  l.entries = batch;
+  l.entries = l.own = batch;
   l.per = heads / kv_heads;
   l.parts = 1;
   l.virtual_heads = kv_heads;
   l.seqs = rb::kStTile / l.per * 2;
   l.ctas = device_sm_count();
+  l.half = l.seqs / 2;
+  l.rows = sp_list_rows(l);
   return l;
 }
 int shared_tc(const rb::SpParams& p, int type, int head_dim, cudaStream_t stream) {

@@ -23,14 +23,14 @@ _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 # The argument blocks of csrc/kernels/beam.h, move_rows.h and shared_prefix.h, packed
 _SELECT = struct.Struct("@7Pq6i")                # logits, scores, ended, out scores, rows, tokens, scratch; pitch; groups, beams, vocab, count, type, end token
 _MOVE = struct.Struct("@P4q2i")                  # base; outer, row and segment stride, segment bytes; outer, segments
-_SHARED = struct.Struct("@10P3q9if")             # q, out, caches, tables, lengths, shared, starts, group of, scratch; pitches, blocks; sizes; scale
+_SHARED = struct.Struct("@10P3q9if")             # q, out, caches, tables, lengths, shared, group of, span of, scratch; pitches, blocks; sizes; scale
 
 N.optional_sig("rb_beam_select", [C.c_char_p, N.c_void_p])
 N.optional_sig("rb_beam_select_scratch_bytes", [N.c_int] * 5, N.c_ll)
 N.optional_sig("rb_move_blocks", [C.c_char_p, N.c_int, N.c_void_p, N.c_void_p, N.c_int, N.c_int, N.c_void_p])
 N.optional_sig("rb_move_reorder", [C.c_char_p, N.c_int, N.c_void_p, N.c_int, N.c_int, N.c_void_p])
 N.optional_sig("rb_shared_prefix", [C.c_char_p, N.c_void_p])
-N.optional_sig("rb_shared_prefix_scratch_bytes", [N.c_int] * 6, N.c_ll)
+N.optional_sig("rb_shared_prefix_scratch_bytes", [N.c_int] * 7, N.c_ll)
 N._LAUNCHES["rb_beam_select"] = 2
 N._LAUNCHES["rb_shared_prefix"] = 3                 # at most: groups of few rows take two
 
@@ -249,8 +249,9 @@ class PrefixGroups:
         starts = [0]
         for n in self.sizes:
             starts.append(starts[-1] + n)
-        both = torch.tensor(starts + [g for g, n in enumerate(self.sizes) for _ in range(n)], dtype=torch.int32).to(device)
-        self.starts, self.group_of = both[:len(starts)], both[len(starts):]
+        span_of = [x for g, n in enumerate(self.sizes) for x in (starts[g], starts[g + 1]) * n]
+        both = torch.tensor(span_of + [g for g, n in enumerate(self.sizes) for _ in range(n)], dtype=torch.int32).to(device)
+        self.span_of, self.group_of = both[:2 * self.batch], both[2 * self.batch:]
 
     def __len__(self) -> int:
         return len(self.sizes)
@@ -293,7 +294,7 @@ def paged_attention_shared(q, k_cache, v_cache, groups: PrefixGroups, shared_len
     if out is not None and (out.dtype is not q.dtype or out.shape != q.shape):
         raise TypeError("paged_attention_shared: out has the shape and type of q")
     dev = q.get_device()
-    _here("paged_attention_shared", dev, k_cache, v_cache, groups.starts, shared_lens, block_tables, context_lens, out)
+    _here("paged_attention_shared", dev, k_cache, v_cache, groups.group_of, shared_lens, block_tables, context_lens, out)
     scale = 1.0 / math.sqrt(d) if scale is None else scale
     if dev < 0:
         r = _shared_cpu(q, k_cache, v_cache, groups, shared_lens, block_tables, context_lens, scale)
@@ -310,10 +311,10 @@ def paged_attention_shared(q, k_cache, v_cache, groups: PrefixGroups, shared_len
     res = out
     if out is None or out.stride(1) != 1 or out.stride(0) & 7 or out.data_ptr() & 15:
         res = torch.empty((batch, width), dtype=q.dtype, device=q.device)
-    scratch = torch.empty(_shared_bytes(batch, heads, hk, d, bs, groups.most), dtype=torch.uint8, device=q.device)
+    scratch = torch.empty(_shared_bytes(batch, len(groups), heads, hk, d, bs, groups.most), dtype=torch.uint8, device=q.device)
     N.check(N.kernels().rb_shared_prefix(
         _SHARED.pack(q.data_ptr(), res.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), shared_lens.data_ptr(),
-                     groups.starts.data_ptr(), groups.group_of.data_ptr(), scratch.data_ptr(), q.stride(0), res.stride(0), nb,
+                     groups.group_of.data_ptr(), groups.span_of.data_ptr(), scratch.data_ptr(), q.stride(0), res.stride(0), nb,
                      batch, len(groups), block_tables.shape[1], bs, heads, hk, d, kind, groups.most, scale), N.stream_ptr()), "rb_shared_prefix")
     return res if out is None or res is out else out.copy_(res)
 
