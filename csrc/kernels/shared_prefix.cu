@@ -34,83 +34,101 @@ __device__ __forceinline__ void sp_mma<__half>(float (&c)[4], const uint32_t (&a
 }
 template <int D, int MT>
 struct SpSmem {
-  static constexpr int kRow = D + 8;             // padded rows (elements): ldmatrix rows hit distinct banks
-  static constexpr int kTile = 32 * kRow;        // a warp's tile of K or V
+  static constexpr int kTile = 32 * D;           // a warp's tile of K or V (elements)
   static constexpr int kQ = kSpWarps * 2 * kTile * 2;                    // byte offsets
-  static constexpr int kMl = kQ + 16 * MT * kRow * 2;
-  static constexpr int kTotals = kMl + kSpWarps * 16 * MT * 8;
+  static constexpr int kMl = kQ + 16 * MT * D * 2;
+  static constexpr int kHeld = kMl + kSpWarps * 16 * MT * 8;
 };
+// Byte offset of 16-byte piece c of row r in a tile of D columns: pieces of eight neighbouring rows, which ldmatrix takes at a time, lie in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t sp_piece(int r, int c) { return (r * (D / 8) + (c ^ (r & 7))) * 16; }
 
+// The copies go on from one part to the next: the next unit's keys, whichever part they are of, are asked for as soon as this unit's scores are formed, its values behind this unit's
+// product.  The warps' sums are joined in the memory of their V tiles (two m-tiles: of K and V, and the next part's keys are asked for behind the join).
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kSpWarps * 32, MT == 1 ? 3 : 2)
 shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
   pdl_wait();
   pdl_launch();
   using L = SpSmem<D, MT>;
-  constexpr int kRow = L::kRow, NT = D / 8, LP = D / 8, kRows = 16 * MT;
-  extern __shared__ __align__(16) uint8_t sp_mem[];
+  constexpr int NT = D / 8, LP = D / 8, kRows = 16 * MT, kQPieces = kRows * LP / (kSpWarps * 32);
+  constexpr bool kAhead = MT == 1;
+  extern __shared__ __align__(128) uint8_t sp_mem[];
   __shared__ int warp_sums[kSpWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
-  T* q_sh = reinterpret_cast<T*>(sp_mem + L::kQ);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
   float2* ml_sh = reinterpret_cast<float2*>(sp_mem + L::kMl);           // [warp][row]: maximum, sum
-  int* totals = reinterpret_cast<int*>(sp_mem + L::kTotals);
-  const uint32_t q_u32 = smem_u32(q_sh), k_u32 = smem_u32(sp_mem) + warp * 2 * L::kTile * 2, v_u32 = k_u32 + L::kTile * 2;
+  const uint32_t q_u32 = smem_u32(sp_mem + L::kQ), k_u32 = smem_u32(sp_mem) + warp * 2 * L::kTile * 2, v_u32 = k_u32 + L::kTile * 2;
+  // fp32 [rows][D] of a warp's sums
+  float* mine = reinterpret_cast<float*>(sp_mem + warp * 2 * L::kTile * 2 + (kAhead ? L::kTile * 2 : 0));
   const SpList& list = p.list;
-  int* shared_of = totals + list.entries + 1;
-  sp_shared(p, shared_of);
-  sp_totals(p, list, shared_of, totals, warp_sums);
-  const int total = totals[list.entries] * list.virtual_heads, group = p.heads / p.kv_heads;
+  const SpHeld held = sp_held(list, reinterpret_cast<int*>(sp_mem + L::kHeld));
+  sp_prepare(p, list, held, warp_sums);
+  const int total = held.totals[list.entries] * list.virtual_heads, group = p.heads / p.kv_heads;
   int u = sp_run(total, list.ctas, blockIdx.x);
   const int u_end = sp_run(total, list.ctas, blockIdx.x + 1);
+  if (u >= u_end) return;
   const T* K = static_cast<const T*>(p.k);
   const T* V = static_cast<const T*>(p.v);
+  const float scale2 = p.scale * kSpLog2e;
 
-  while (u < u_end) {
-    // ---- this part's rows and tokens
-    const SpPart s_ = sp_next(p, list, totals, u, u_end);
-    const int hk = s_.vh / list.parts, head0 = (s_.vh - hk * list.parts) * list.per, per = list.per, real = min(per, group - head0);
-    const int b = s_.b, rows = s_.n * per, shared = shared_of[s_.g], u0 = s_.u0, u1 = s_.u1;
-    const int first = s_.own ? shared : 0, count = s_.own ? sp_length(p, b) - shared : shared;
-    const int* table = s_.table;
-    __syncthreads();                             // the last entry's queries and results have been read
-    for (int i = threadIdx.x; i < kRows * LP; i += blockDim.x) {
-      const int r = i / LP, c = (i - r * LP) * 8;
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      const int s = r / per, h = r - s * per;
-      if (r < rows && h < real)
-        x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (b + s) * p.ld_q + static_cast<long long>(hk * group + head0 + h) * D + c);
-      *reinterpret_cast<uint4*>(q_sh + r * kRow + c) = x;
-    }
-    __syncthreads();
-
-    int slot = 0, n_next = 0;
-    auto locate = [&](int unit) {
-      const int at = unit * kSpUnit + warp * 32;
-      n_next = unit < u1 ? min(32, count - at) : 0;
-      slot = -1;
-      if (lane < n_next) {
-        const int token = first + at + lane, page = token / p.block_size;
-        int blk = table[page];
-        if (blk < 0 || blk >= p.num_blocks) {                          // corrupt tables read block 0 instead of faulting
-          RB_BOUNDS_HIT(104);
-          blk = 0;
-        }
-        slot = blk * p.block_size + (token - page * p.block_size);     // the host bounds num_blocks * block_size below 2^31
-      }
-    };
-    auto request = [&](const T* cache, uint32_t tile) {
-      if (n_next > 0) {
+  SpPart s_ = sp_next(p, list, held, u, u_end);
+  int unit = s_.u0;
+  // ---- rows of queries: loaded into registers, stored when the last part's have been read
+  uint4 q_next[kQPieces];
+  auto load_q = [&](const SpPart& s) {
+    const int hk = s.vh / list.parts, head0 = (s.vh - hk * list.parts) * list.per, real = min(list.per, group - head0), rows = s.n * list.per;
 #pragma unroll
-        for (int i = 0; i < LP; ++i) {
-          const int idx = i * 32 + lane, r = idx / LP, c = (idx - r * LP) * 8;
-          const int s = __shfl_sync(0xffffffffu, slot, r);
-          wm_cp16(tile + (r * kRow + c) * 2, s >= 0 ? cache + (static_cast<long long>(s) * p.kv_heads + hk) * D + c : cache, s >= 0);
-        }
+    for (int i = 0; i < kQPieces; ++i) {
+      const int at = i * kSpWarps * 32 + tid, r = at / LP, c = at - r * LP, seq = r / list.per, h = r - seq * list.per;
+      q_next[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < rows && h < real)
+        q_next[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (s.b + seq) * p.ld_q + static_cast<long long>(hk * group + head0 + h) * D + c * 8);
+    }
+  };
+  auto store_q = [&]() {
+#pragma unroll
+    for (int i = 0; i < kQPieces; ++i) {
+      const int at = i * kSpWarps * 32 + tid, r = at / LP, c = at - r * LP;
+      *reinterpret_cast<uint4*>(sp_mem + L::kQ + sp_piece<D>(r, c)) = q_next[i];
+    }
+  };
+  // ---- keys and values of the located unit
+  int slot = 0, n_next = 0, hk_next = 0;
+  auto locate = [&](const SpPart& s, int of) {
+    const int first = s.own ? s.shared : 0, count = s.own ? sp_length(p, s.b) - s.shared : s.shared, at = of * kSpUnit + warp * 32;
+    hk_next = s.vh / list.parts;
+    n_next = min(32, count - at);
+    slot = -1;
+    if (lane < n_next) {
+      const int token = first + at + lane, page = token / p.block_size;
+      int blk = s.table[page];
+      if (blk < 0 || blk >= p.num_blocks) {                            // corrupt tables read block 0 instead of faulting
+        RB_BOUNDS_HIT(104);
+        blk = 0;
       }
-      wm_cp_commit();
-    };
-    const float scale2 = p.scale * kSpLog2e;
-    float m[MT][2], l[MT][2], acc[MT][NT][4];
+      slot = blk * p.block_size + (token - page * p.block_size);       // the host bounds num_blocks * block_size below 2^31
+    }
+  };
+  auto request = [&](const T* cache, uint32_t tile) {
+    if (n_next > 0) {
+#pragma unroll
+      for (int i = 0; i < LP; ++i) {
+        const int idx = i * 32 + lane, r = idx / LP, c = idx - r * LP;
+        const int s = __shfl_sync(0xffffffffu, slot, r);
+        wm_cp16(tile + sp_piece<D>(r, c), s >= 0 ? cache + (static_cast<long long>(s) * p.kv_heads + hk_next) * D + c * 8 : cache, s >= 0);
+      }
+    }
+    wm_cp_commit();
+  };
+
+  locate(s_, unit);
+  request(K, k_u32);
+  load_q(s_);
+  store_q();
+  request(V, v_u32);
+  __syncthreads();
+  float m[MT][2], l[MT][2], acc[MT][NT][4];
+  auto clear = [&]() {
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
       m[t][0] = m[t][1] = -INFINITY;
@@ -118,161 +136,177 @@ shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) acc[t][n][0] = acc[t][n][1] = acc[t][n][2] = acc[t][n][3] = 0.f;
     }
-    locate(u0);
-    request(K, k_u32);
-    request(V, v_u32);
-    for (int unit = u0; unit < u1; ++unit) {
-      const int n_tok = n_next;
-      wm_cp_wait<1>();                           // this unit's K tile has landed (V may be on its way)
-      __syncwarp();
-      float s[MT][4][4];
+  };
+  clear();
+  for (bool more = true; more;) {
+    const int n_tok = n_next, rows = s_.n * list.per;
+    const bool last = unit + 1 == s_.u1;
+    more = !last || u < u_end;
+    wm_cp_wait<1>();                             // this unit's K tile has landed (V may be on its way)
+    __syncwarp();
+    float s[MT][4][4];
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) s[t][n][0] = s[t][n][1] = s[t][n][2] = s[t][n][3] = 0.f;
-      if (n_tok > 0) {
+      for (int n = 0; n < 4; ++n) s[t][n][0] = s[t][n][1] = s[t][n][2] = s[t][n][3] = 0.f;
+    if (n_tok > 0) {
 #pragma unroll
-        for (int k0 = 0; k0 < D; k0 += 16) {
-          uint32_t bk[2][4];
+      for (int k0 = 0; k0 < D / 8; k0 += 2) {    // pieces of 8 columns
+        uint32_t bk[2][4];
 #pragma unroll
-          for (int np = 0; np < 2; ++np) wm_ldsm_x4(wm_b(k_u32, kRow, np * 16, k0, lane), bk[np]);
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            if (t > 0 && rows <= t * 16) continue;
-            uint32_t a[4];
-            wm_ldsm_x4(wm_a(q_u32, kRow, t * 16, k0, lane), a);
-#pragma unroll
-            for (int np = 0; np < 2; ++np) {
-              sp_mma<T>(s[t][2 * np], a, bk[np][0], bk[np][1]);
-              sp_mma<T>(s[t][2 * np + 1], a, bk[np][2], bk[np][3]);
-            }
-          }
-        }
-      }
-      __syncwarp();                              // every lane has read its K fragments
-      locate(unit + 1);
-      request(K, k_u32);
-      if (n_tok > 0) {
-        uint32_t pf[MT][2][4];
+        for (int np = 0; np < 2; ++np) wm_ldsm_x4(k_u32 + sp_piece<D>(np * 16 + (lane & 7) + ((lane >> 4) << 3), k0 + ((lane >> 3) & 1)), bk[np]);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
           if (t > 0 && rows <= t * 16) continue;
+          uint32_t a[4];
+          wm_ldsm_x4(q_u32 + sp_piece<D>(t * 16 + (lane & 15), k0 + (lane >> 4)), a);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {          // rows gq and gq + 8
-            float mx = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                float& x = s[t][n][2 * i + j];
-                x = n * 8 + 2 * tq + j < n_tok ? x * scale2 : -INFINITY;
-                mx = fmaxf(mx, x);
-              }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mn = fmaxf(m[t][i], mx), from = mn == -INFINITY ? 0.f : mn;       // a row that has seen nothing yet
-            const float al = wm_ex2(m[t][i] - from);
-            float sum = 0.f;
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              const float p0 = wm_ex2(s[t][n][2 * i] - from), p1 = wm_ex2(s[t][n][2 * i + 1] - from);
-              sum += p0 + p1;
-              pf[t][n >> 1][(n & 1) * 2 + i] = sp_pack<T>(p0, p1);
-            }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            l[t][i] = fmaf(l[t][i], al, sum);
-            m[t][i] = mn;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              acc[t][n][2 * i] *= al;
-              acc[t][n][2 * i + 1] *= al;
-            }
+          for (int np = 0; np < 2; ++np) {
+            sp_mma<T>(s[t][2 * np], a, bk[np][0], bk[np][1]);
+            sp_mma<T>(s[t][2 * np + 1], a, bk[np][2], bk[np][3]);
           }
         }
-        wm_cp_wait<1>();                         // this unit's V tile has landed
-        __syncwarp();
+      }
+    }
+    __syncwarp();                                // every lane has read its K fragments
+    // ---- the next unit, of this part or the next
+    const SpPart now = s_;
+    if (!last) {
+      ++unit;
+    } else if (more) {
+      s_ = sp_next(p, list, held, u, u_end);
+      unit = s_.u0;
+    }
+    if (more) locate(s_, unit);
+    else n_next = 0;
+    const bool ahead = kAhead || !last;
+    if (ahead) request(K, k_u32);
+    else wm_cp_commit();
+    if (last && more) load_q(s_);
+    if (n_tok > 0) {
+      uint32_t pf[MT][2][4];
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+      for (int t = 0; t < MT; ++t) {
+        if (t > 0 && rows <= t * 16) continue;
 #pragma unroll
-          for (int n2 = 0; n2 < NT / 2; ++n2) {
-            uint32_t bv[4];
-            wm_ldsm_x4_t(wm_b_t(v_u32, kRow, n2 * 16, ks * 16, lane), bv);
+        for (int i = 0; i < 2; ++i) {            // rows gq and gq + 8
+          float mx = -INFINITY;
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-              if (t > 0 && rows <= t * 16) continue;
-              sp_mma<T>(acc[t][2 * n2], pf[t][ks], bv[0], bv[1]);
-              sp_mma<T>(acc[t][2 * n2 + 1], pf[t][ks], bv[2], bv[3]);
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float& x = s[t][n][2 * i + j];
+              x = n * 8 + 2 * tq + j < n_tok ? x * scale2 : -INFINITY;
+              mx = fmaxf(mx, x);
             }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float mn = fmaxf(m[t][i], mx), from = mn == -INFINITY ? 0.f : mn;       // scores of minus infinity
+          const float al = wm_ex2(m[t][i] - from);
+          float sum = 0.f;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const float p0 = wm_ex2(s[t][n][2 * i] - from), p1 = wm_ex2(s[t][n][2 * i + 1] - from);
+            sum += p0 + p1;
+            pf[t][n >> 1][(n & 1) * 2 + i] = sp_pack<T>(p0, p1);
           }
-        __syncwarp();                            // every lane has read its V fragments
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          l[t][i] = fmaf(l[t][i], al, sum);
+          m[t][i] = mn;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            acc[t][n][2 * i] *= al;
+            acc[t][n][2 * i + 1] *= al;
+          }
+        }
       }
-      request(V, v_u32);
+      wm_cp_wait<1>();                           // this unit's V tile has landed
+      __syncwarp();
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int n2 = 0; n2 < NT / 2; ++n2) {
+          uint32_t bv[4];
+          wm_ldsm_x4_t(v_u32 + sp_piece<D>(ks * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, n2 * 2 + (lane >> 4)), bv);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            if (t > 0 && rows <= t * 16) continue;
+            sp_mma<T>(acc[t][2 * n2], pf[t][ks], bv[0], bv[1]);
+            sp_mma<T>(acc[t][2 * n2 + 1], pf[t][ks], bv[2], bv[3]);
+          }
+        }
+      __syncwarp();                              // every lane has read its V fragments
     }
-
-    // ---- the warps' sums are joined in the memory of their tiles: fp32 [rows][D + 8]
-    wm_cp_wait<0>();
-    __syncwarp();
-    float* mine = reinterpret_cast<float*>(sp_mem + warp * 2 * L::kTile * 2);
+    if (last) {
+      // ---- the part's sums
+      wm_cp_wait<kAhead ? 1 : 0>();              // nothing is on its way into the memory that the sums take
+      __syncwarp();
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      if (t > 0 && rows <= t * 16) continue;
+      for (int t = 0; t < MT; ++t) {
+        if (t > 0 && rows <= t * 16) continue;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = t * 16 + gq + i * 8;
-        if (tq == 0) ml_sh[warp * kRows + r] = make_float2(m[t][i], l[t][i]);
+        for (int i = 0; i < 2; ++i) {
+          const int r = t * 16 + gq + i * 8;
+          if (tq == 0) ml_sh[warp * kRows + r] = make_float2(m[t][i], l[t][i]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(mine + r * kRow + n * 8 + 2 * tq) = make_float2(acc[t][n][2 * i], acc[t][n][2 * i + 1]);
+          for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(mine + r * D + ((n * 8) ^ ((r & 7) * 8)) + 2 * tq) = make_float2(acc[t][n][2 * i], acc[t][n][2 * i + 1]);
+        }
       }
-    }
-    __syncthreads();
-    const long long row0 = sp_row(list, s_.vh, s_.e, blockIdx.x, u0 == 0);
-    for (int i = threadIdx.x; i < rows * (D / 4); i += blockDim.x) {
-      const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
-      float mx = -INFINITY;
+      __syncthreads();
+      const long long row0 = sp_row(list, now.vh, now.e, blockIdx.x, now.u0 == 0);
+      for (int i = tid; i < rows * (D / 4); i += kSpWarps * 32) {
+        const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
+        float mx = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kSpWarps; ++w) mx = fmaxf(mx, ml_sh[w * kRows + r].x);
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      float den = 0.f;
+        for (int w = 0; w < kSpWarps; ++w) mx = fmaxf(mx, ml_sh[w * kRows + r].x);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        float den = 0.f;
 #pragma unroll
-      for (int w = 0; w < kSpWarps; ++w) {
-        const float2 ml = ml_sh[w * kRows + r];
-        const float f = ml.x == -INFINITY ? 0.f : wm_ex2(ml.x - mx);
-        const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sp_mem + w * 2 * L::kTile * 2) + r * kRow + c);
-        sum.x = fmaf(x.x, f, sum.x); sum.y = fmaf(x.y, f, sum.y); sum.z = fmaf(x.z, f, sum.z); sum.w = fmaf(x.w, f, sum.w);
-        den = fmaf(ml.y, f, den);
+        for (int w = 0; w < kSpWarps; ++w) {
+          const float2 ml = ml_sh[w * kRows + r];
+          const float f = ml.x == -INFINITY ? 0.f : wm_ex2(ml.x - mx);
+          const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sp_mem + w * 2 * L::kTile * 2 + (kAhead ? L::kTile * 2 : 0)) + r * D + (c ^ ((r & 7) * 8)));
+          sum.x = fmaf(x.x, f, sum.x); sum.y = fmaf(x.y, f, sum.y); sum.z = fmaf(x.z, f, sum.z); sum.w = fmaf(x.w, f, sum.w);
+          den = fmaf(ml.y, f, den);
+        }
+        *reinterpret_cast<float4*>(list.acc + (row0 + r) * D + c) = sum;
+        if (c == 0) list.ml[row0 + r] = make_float2(mx, den);
       }
-      *reinterpret_cast<float4*>(list.acc + (row0 + r) * D + c) = sum;
-      if (c == 0) list.ml[row0 + r] = make_float2(mx, den);
+      if (!more) return;
+      __syncthreads();                           // sums and queries have been read
+      store_q();
+      if (!kAhead) request(K, k_u32);
+      __syncthreads();
+      clear();
     }
+    request(V, v_u32);
   }
 }
 
-// out[b, head] from the parts of its row.  A CTA has a sequence and a KV head; a row's parts are summed by one warp or, where there are fewer heads than warps, by several, and
-// lanes own D / 32 neighbouring columns.  Grid (batch, KV heads).
+// out[b, head] from the parts of its row.  A CTA has some heads of a sequence and KV head; a row's parts are summed by `share` warps, and
+// lanes own D / 32 neighbouring columns.  Grid (batch, KV heads, parts of a KV head's query heads).
 constexpr int kSpJoinWarps = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(kSpJoinWarps * 32)
-shared_join_kernel(const SpParams p) {
-  pdl_wait();
-  pdl_launch();
+shared_join_kernel(const SpParams p, const int share) {
   constexpr int C = D / 32;
   __shared__ float sum_sh[kSpJoinWarps][D + 2];  // a warp's columns, maximum and sum
   const int b = blockIdx.x, hk = blockIdx.y, group = p.heads / p.kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int2 span = p.span_of[b];
+  const int2 span = p.span_of[b];                // older than the launches in front
   const bool any = sp_length(p, b) > 0;          // a sequence without tokens gets zeros
+  pdl_wait();
+  pdl_launch();
   const int tile = b - (b - span.x) % p.prefix.seqs;
   // parts of an entry that one of two tiles of rows had alone come in twos (see shared_prefix_tc.cu)
   const int twin = p.prefix.half > 0 && min(p.prefix.seqs, span.y - tile) <= p.prefix.half ? 2 : 1;
   // lanes 0, 1: first and last unit over shared tokens, lanes 2, 3: the sequence's own
   const SpList& look = lane & 2 ? p.list : p.prefix;
   const int all = look.totals[look.entries], t0 = look.totals[lane & 2 ? look.own + b : tile], t1 = look.totals[(lane & 2 ? look.own + b : tile) + 1];
-  const int share = group < kSpJoinWarps ? kSpJoinWarps / group : 1;      // warps of a row
-  const int at_once = kSpJoinWarps / share;                             // rows
-  for (int h0 = 0; h0 < group; h0 += at_once) {
-    const int h = h0 + warp / share, which = warp % share;
-    const bool mine = warp / share < at_once && h < group;
+  {
+    const int h = blockIdx.z * (kSpJoinWarps / share) + warp / share, which = warp % share;
+    const bool mine = h < group;
     float mx = -INFINITY, den = 0.f, acc[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = 0.f;
@@ -374,6 +408,7 @@ struct Plan {
   rb::SpList list, prefix;
   size_t smem;
   int tiles;                                     // m-tiles of the split kernel
+  int share;                                     // warps of a row of the join
   bool tc;
 };
 // Shared tokens of groups with more than 16 rows go to the tcgen05 kernel, which takes 256 at a time; the split kernel has one m-tile, or two where rows need them.
@@ -392,13 +427,17 @@ Plan plan_of(int batch, int groups, int heads, int kv_heads, int head_dim, int b
   l.virtual_heads = kv_heads * l.parts;
   l.own = p.tc ? 0 : batch;
   l.entries = l.own + batch;
-  const size_t tiles = head_dim == 64 ? (p.tiles == 1 ? rb::SpSmem<64, 1>::kTotals : rb::SpSmem<64, 2>::kTotals)
-                                      : (p.tiles == 1 ? rb::SpSmem<128, 1>::kTotals : rb::SpSmem<128, 2>::kTotals);
-  p.smem = tiles + (static_cast<size_t>(l.entries) + 1 + groups) * 4;
+  const size_t tiles = head_dim == 64 ? (p.tiles == 1 ? rb::SpSmem<64, 1>::kHeld : rb::SpSmem<64, 2>::kHeld)
+                                      : (p.tiles == 1 ? rb::SpSmem<128, 1>::kHeld : rb::SpSmem<128, 2>::kHeld);
+  p.smem = tiles + rb::sp_held_bytes(l.entries, groups);
   const int resident = static_cast<int>((228 * 1024) / (p.smem + 1024 + 64)), most_resident = p.tiles == 1 ? 3 : 2;
   l.ctas = rbhost::device_sm_count() * (resident < 1 ? 1 : resident < most_resident ? resident : most_resident);
   l.rows = rbhost::sp_list_rows(l);
   p.prefix = p.tc ? rbhost::shared_tc_list(batch, heads, kv_heads) : l;
+  // parts of a row over shared tokens, if these are long: about four for a warp
+  const int tiles_of = (batch + p.prefix.seqs - 1) / p.prefix.seqs, entries = groups > tiles_of ? groups : tiles_of;
+  const long long parts = p.prefix.ctas / (static_cast<long long>(entries) * p.prefix.virtual_heads) * (p.tc ? 2 : 1);
+  p.share = parts >= 24 ? 8 : parts >= 12 ? 4 : parts >= 6 ? 2 : 1;
   return p;
 }
 // Puts a list's arrays at `at` (NULL: only counts) and returns their size.
@@ -412,7 +451,7 @@ long long place(rb::SpList& l, char* at, int head_dim) {
   return totals + ml + rows * head_dim * 4;
 }
 bool sound(int batch, int heads, int kv_heads, int head_dim, int block_size) {
-  return batch >= 0 && batch <= 8192 && kv_heads >= 1 && kv_heads <= 65535 && heads >= kv_heads && heads % kv_heads == 0 && (head_dim == 64 || head_dim == 128) &&
+  return batch >= 0 && batch <= 4096 && kv_heads >= 1 && kv_heads <= 65535 && heads >= kv_heads && heads % kv_heads == 0 && (head_dim == 64 || head_dim == 128) &&
          block_size >= 1;
 }
 
@@ -427,11 +466,18 @@ cudaError_t split(const rb::SpParams& p, const Plan& l, cudaStream_t s) {
   }
   return rbhost::launch_pdl(rb::shared_split_kernel<T, D, MT>, dim3(l.list.ctas), dim3(rb::kSpWarps * 32), l.smem, s, 1, p RB_BOUNDS_ARG);
 }
+// The sequences' own tokens, the shared ones where they have a kernel of their own, and the join.  Neither of the first two reads what the other writes: the second begins as the first
+// one's CTAs leave the SMs.
 template <typename T, int D>
-cudaError_t both(const rb::SpParams& p, const Plan& l, cudaStream_t s) {
-  const cudaError_t e = l.tiles == 1 ? split<T, D, 1>(p, l, s) : split<T, D, 2>(p, l, s);
-  if (e != cudaSuccess) return e;
-  return rbhost::launch_pdl(rb::shared_join_kernel<T, D>, dim3(p.batch, p.kv_heads), dim3(rb::kSpJoinWarps * 32), 0, s, 1, p);
+int launch(const rb::SpParams& p, const Plan& l, int type, cudaStream_t s) {
+  cudaError_t e = l.tiles == 1 ? split<T, D, 1>(p, l, s) : split<T, D, 2>(p, l, s);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (l.tc) {
+    const int code = rbhost::shared_tc(p, type, D, s);
+    if (code) return code;
+  }
+  const int rows = rb::kSpJoinWarps / l.share, group = p.heads / p.kv_heads;
+  return static_cast<int>(rbhost::launch_pdl(rb::shared_join_kernel<T, D>, dim3(p.batch, p.kv_heads, (group + rows - 1) / rows), dim3(rb::kSpJoinWarps * 32), 0, s, 1, p, l.share));
 }
 
 }  // namespace
@@ -476,12 +522,8 @@ RB_API int rb_shared_prefix(const RbSharedPrefixArgs* a, void* stream) {
   p.list = l.list;
   p.prefix = l.prefix;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (l.tc) {
-    const int e = rbhost::shared_tc(p, a->type, a->head_dim, s);
-    if (e) return e;
-  }
-  cudaError_t e;
-  if (a->type == 0) e = a->head_dim == 64 ? both<__nv_bfloat16, 64>(p, l, s) : both<__nv_bfloat16, 128>(p, l, s);
-  else e = a->head_dim == 64 ? both<__half, 64>(p, l, s) : both<__half, 128>(p, l, s);
-  return static_cast<int>(e);
+  int e;
+  if (a->type == 0) e = a->head_dim == 64 ? launch<__nv_bfloat16, 64>(p, l, 0, s) : launch<__nv_bfloat16, 128>(p, l, 0, s);
+  else e = a->head_dim == 64 ? launch<__half, 64>(p, l, 1, s) : launch<__half, 128>(p, l, 1, s);
+  return e;
 }

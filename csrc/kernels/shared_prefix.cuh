@@ -42,36 +42,53 @@ struct SpParams {
 };
 
 __device__ __forceinline__ int sp_length(const SpParams& p, int b) { return min(max(p.lens[b], 0), p.cap); }
-// What each group's sequences read together: no more tokens than the shortest of them has, those without tokens aside, so that all rows of a tile see all of its
-// tokens.  `shared`: [groups] of the CTA's shared memory.
-__device__ __forceinline__ void sp_shared(const SpParams& p, int* shared) {
-  for (int g = threadIdx.x; g < p.groups; g += blockDim.x) shared[g] = INT_MAX;
+// What a CTA's shared memory holds of a list: running totals of the entries' units, and of every entry its tokens and the first sequences of its group and of the next.
+struct SpHeld {
+  int* totals;                                   // [entries + 1]
+  int* tokens;                                   // [entries]; of an own entry: those in front of it, which are shared
+  uint32_t* span;                                // [entries]: two numbers of 16 bits
+};
+__host__ __device__ constexpr size_t sp_held_bytes(int entries, int groups) { return (3 * static_cast<size_t>(entries) + 1 + groups) * 4; }
+__device__ __forceinline__ SpHeld sp_held(const SpList& l, int* at) { return {at, at + l.entries + 1, reinterpret_cast<uint32_t*>(at + 2 * l.entries + 1)}; }
+// Forms them, all threads of a CTA.
+//
+// What a group's sequences read together are no more tokens than the shortest of them has, those without tokens aside, so that all rows of a tile see all of its tokens.  Tiles of rows
+// begin at every `seqs`-th sequence of a group.  The loads of the first sequences of a thread go out together: the chain of latencies is what this costs.
+__device__ __forceinline__ void sp_prepare(const SpParams& p, const SpList& l, const SpHeld& held, int* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int* least = reinterpret_cast<int*>(held.span + l.entries);          // [groups]
+  const int b0 = min(static_cast<int>(threadIdx.x), p.batch - 1), g0 = min(static_cast<int>(threadIdx.x), p.groups - 1);
+  const int length0 = sp_length(p, b0), group0 = p.group_of[b0], said0 = p.shared[g0];
+  const int2 span0 = p.span_of[b0];
+  for (int g = threadIdx.x; g < p.groups; g += blockDim.x) least[g] = INT_MAX;
+  if (threadIdx.x == 0) held.totals[0] = 0;
   __syncthreads();
   for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
-    const int n = sp_length(p, b);
-    if (n > 0) atomicMin(&shared[p.group_of[b]], n);
+    const bool first = b == static_cast<int>(threadIdx.x);
+    const int n = first ? length0 : sp_length(p, b);
+    if (n > 0) atomicMin(&least[first ? group0 : p.group_of[b]], n);
   }
   __syncthreads();
   for (int g = threadIdx.x; g < p.groups; g += blockDim.x) {
-    const int n = shared[g];
-    shared[g] = n == INT_MAX ? 0 : min(n, max(p.shared[g], 0));
+    const int n = least[g];
+    least[g] = n == INT_MAX ? 0 : min(n, max(g == static_cast<int>(threadIdx.x) ? said0 : p.shared[g], 0));
   }
   __syncthreads();
-}
-// Units of entry e: tiles of rows begin at every `seqs`-th sequence of a group.
-__device__ __forceinline__ int sp_units(const SpParams& p, const SpList& l, const int* shared_of, int e) {
-  const int b = e < l.own ? e : e - l.own, shared = shared_of[p.group_of[b]];
-  if (e < l.own) return (b - p.span_of[b].x) % l.seqs == 0 ? (shared + kSpUnit - 1) / kSpUnit : 0;
-  return max(0, sp_length(p, b) - shared + kSpUnit - 1) / kSpUnit;
-}
-// Running totals of the units of all entries, [entries + 1], formed by all threads of a CTA.
-__device__ __forceinline__ void sp_totals(const SpParams& p, const SpList& l, const int* shared_of, int* totals, int* warp_sums) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   int before = 0;
-  if (threadIdx.x == 0) totals[0] = 0;
-  for (int first = 0; first < l.entries; first += blockDim.x) {
-    const int e = first + threadIdx.x;
-    int upto = e < l.entries ? sp_units(p, l, shared_of, e) : 0;
+  for (int e0 = 0; e0 < l.entries; e0 += blockDim.x) {
+    const int e = e0 + threadIdx.x;
+    int upto = 0;
+    if (e < l.entries) {
+      const bool own = e >= l.own;
+      const int b = own ? e - l.own : e;
+      const bool first = b == static_cast<int>(threadIdx.x);
+      const int shared = least[first ? group0 : p.group_of[b]];
+      const int2 span = first ? span0 : p.span_of[b];
+      held.tokens[e] = shared;
+      held.span[e] = static_cast<uint32_t>(span.x) | static_cast<uint32_t>(span.y) << 16;
+      const int count = own ? max(0, (first ? length0 : sp_length(p, b)) - shared) : (b - span.x) % l.seqs == 0 ? shared : 0;
+      upto = (count + kSpUnit - 1) / kSpUnit;
+    }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, upto, o);
@@ -85,12 +102,12 @@ __device__ __forceinline__ void sp_totals(const SpParams& p, const SpList& l, co
       if (w < warp) upto += s;
       all += s;
     }
-    if (e < l.entries) totals[e + 1] = before + upto;
+    if (e < l.entries) held.totals[e + 1] = before + upto;
     before += all;
     __syncthreads();
   }
   if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i <= l.entries; i += blockDim.x) l.totals[i] = totals[i];
+    for (int i = threadIdx.x; i <= l.entries; i += blockDim.x) l.totals[i] = held.totals[i];
 }
 // First unit of CTA c's run, and the CTA that has unit u.
 __device__ __forceinline__ int sp_run(int total, int ctas, int c) {
@@ -104,31 +121,32 @@ __device__ __forceinline__ int sp_cta_of(int total, int ctas, int u) {
 // A part of an entry: units u0 .. u1 - 1 of it, for one virtual KV head.
 struct SpPart {
   int vh, e, u0, u1;
-  int b, g, n;                                   // first sequence, group, sequences of the tile
+  int b, n;                                      // first sequence, sequences of the tile
+  int shared;                                    // tokens that the group shares
   const int* table;
   bool own;
 };
 // The part that a run u .. u_end begins with; u goes behind it.  Every thread that calls it gets the same.
-__device__ __forceinline__ SpPart sp_next(const SpParams& p, const SpList& l, const int* totals, int& u, int u_end) {
+__device__ __forceinline__ SpPart sp_next(const SpParams& p, const SpList& l, const SpHeld& held, int& u, int u_end) {
   SpPart s;
-  const int all = totals[l.entries];
+  const int all = held.totals[l.entries];
   s.vh = u / all;
   const int at = u - s.vh * all;
   int e = 0;
   for (int hi = l.entries; hi - e > 1;) {        // the last entry that begins at or in front of the unit
     const int mid = (e + hi) >> 1;
-    if (totals[mid] <= at) e = mid;
+    if (held.totals[mid] <= at) e = mid;
     else hi = mid;
   }
   s.e = e;
-  s.u0 = at - totals[e];
-  s.u1 = min(totals[e + 1], at + u_end - u) - totals[e];
+  s.u0 = at - held.totals[e];
+  s.u1 = min(held.totals[e + 1], at + u_end - u) - held.totals[e];
   s.own = e >= l.own;
   s.b = s.own ? e - l.own : e;
-  s.g = p.group_of[s.b];
-  const int2 span = p.span_of[s.b];
-  s.n = s.own ? 1 : min(l.seqs, span.y - s.b);
-  s.table = p.tables + static_cast<long long>(s.own ? s.b : span.x) * p.width;
+  s.shared = held.tokens[e];
+  const uint32_t span = held.span[e];
+  s.n = s.own ? 1 : min(l.seqs, static_cast<int>(span >> 16) - s.b);
+  s.table = p.tables + static_cast<long long>(s.own ? s.b : static_cast<int>(span & 0xffffu)) * p.width;
   u += s.u1 - s.u0;
   return s;
 }

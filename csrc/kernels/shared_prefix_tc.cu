@@ -25,12 +25,18 @@ namespace rb {
 constexpr int kStThreads = 384;          // warps 0-7 softmax, 8 and 10 TMA, 9 MMA, 11 only gives its registers away
 constexpr int kStTile = 128;
 constexpr float kStRescale = 8.f;        // log2 units
-constexpr int kStMostBatch = 2048;       // running totals beside 192 KB of tiles
+constexpr int kStMostBatch = 1536;       // their totals, tokens and spans beside 192 KB of tiles
 
 __device__ __forceinline__ void st_ld32(uint32_t taddr, uint32_t* r) { tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r)); }
 __device__ __forceinline__ void st_st32(uint32_t taddr, const uint32_t* r) {
   tmem_st_32x16(taddr, *reinterpret_cast<const uint32_t(*)[16]>(r));
   tmem_st_32x16(taddr + 16, *reinterpret_cast<const uint32_t(*)[16]>(r + 16));
+}
+
+__device__ __forceinline__ float st_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 template <int D>
@@ -54,7 +60,7 @@ struct StMaps {
 template <typename T, int D>
 __global__ void __launch_bounds__(kStThreads, 1)
 shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned int* status RB_BOUNDS_PARAM) {
-  pdl_wait();
+  // No wait for the kernel in front, the sequences' own tokens: it writes nothing that is read here, and what it waited for is done.
   pdl_launch();
   using L = StSmem<D>;
   constexpr int kStages = L::kStages;
@@ -68,15 +74,14 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
   const uint32_t bar_sfull = bar_vempty + 8 * kStages, bar_pfull = bar_sfull + 16, bar_oready = bar_pfull + 16;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + L::kInts);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
-  int* totals = reinterpret_cast<int*>(smem + L::kTotal);
   const SpList& list = p.prefix;
-  int* shared_of = totals + list.entries + 1;
+  const SpHeld held = sp_held(list, reinterpret_cast<int*>(smem + L::kTotal));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr uint32_t kTmemCols = 512;
 
   if (threadIdx.x == 0) {
     mbar_init(bar_q, 1);
-    mbar_init(bar_qfree, 1);
+    mbar_init(bar_qfree, 8);
     mbar_init(bar_tail, 1);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar_kfull + 8 * s, 1);
@@ -95,23 +100,22 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
     tma_prefetch_desc(&maps.k);
     tma_prefetch_desc(&maps.v);
   }
-  sp_shared(p, shared_of);
-  sp_totals(p, list, shared_of, totals, warp_sums);
   if (warp == 9) {
     tmem_alloc(smem_u32(tmem_ptr), kTmemCols);
     tmem_relinquish();
   }
+  sp_prepare(p, list, held, warp_sums);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr;
-  const int total = totals[list.entries] * list.virtual_heads, group = p.heads / p.kv_heads;
+  const int total = held.totals[list.entries] * list.virtual_heads;
   const int u_begin = sp_run(total, list.ctas, blockIdx.x), u_end = sp_run(total, list.ctas, blockIdx.x + 1);
   const int half = list.half;                                  // sequences of one of the two tiles
   const int tile_rows = half * list.per;
 
   if (warp >= 8) {
-    setmaxnreg_dec<56>();
+    setmaxnreg_dec<104>();
     if (warp == 8 || warp == 10) {
       // ---------------------------------------------------------------- TMA producers, all lanes: warp 8 queries and keys, warp 10 values
       const bool values = warp == 10;
@@ -121,8 +125,8 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
       bool ok = true;
       int it = 0, part = 0, tails = 0;
       for (int u = u_begin; u < u_end && ok; ++part) {
-        const SpPart s = sp_next(p, list, totals, u, u_end);
-        const int shared = shared_of[s.g], head0 = s.vh * list.per;
+        const SpPart s = sp_next(p, list, held, u, u_end);
+        const int shared = s.shared, head0 = s.vh * list.per;
         // pages of a unit: lane i has the i-th (one of 128 rows, from `row` on, where pages are larger); looked up a unit ahead
         auto page_of = [&](int unit) {
           const int at = unit * kSpUnit + lane * size;
@@ -214,14 +218,13 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
           return true;
         };
         for (int u = u_begin; u < u_end && ok; ++part) {
-          const SpPart s = sp_next(p, list, totals, u, u_end);
+          const SpPart s = sp_next(p, list, held, u, u_end);
           const int n = s.u1 - s.u0;
           ok = mbar_wait(bar_q, part & 1, abort_flag, status, 56);
           if (s.n > half) {                                      // two tiles of rows
             for (int t = 0; t < 2 && ok; ++t) ok = issue_qk(it, t, t);
             if (!ok) break;
             umma_commit(bar_kempty + 8 * (it % kStages));
-            if (n == 1) umma_commit(bar_qfree);
             for (int j = 0; j < n && ok; ++j) {
               const int i = it + j, st = i % kStages;
               if (!mbar_wait(bar_vfull + 8 * st, (i / kStages) & 1, abort_flag, status, 57)) { ok = false; break; }
@@ -232,14 +235,12 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
               if (!ok) break;
               umma_commit(bar_vempty + 8 * st);
               if (j + 1 < n) umma_commit(bar_kempty + 8 * ((i + 1) % kStages));
-              if (j + 2 == n) umma_commit(bar_qfree);            // the last products that read the queries have been issued
             }
           } else {                                               // one: units in turn with the S and O of A and of B
             for (int j = 0; j < 2 && j < n && ok; ++j) {
               ok = issue_qk(it + j, j, 0);
               if (!ok) break;
               umma_commit(bar_kempty + 8 * ((it + j) % kStages));
-              if (j + 1 == n) umma_commit(bar_qfree);
             }
             for (int j = 0; j < n && ok; ++j) {
               const int i = it + j, st = i % kStages;
@@ -248,7 +249,6 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
               if (j + 2 < n) {
                 if (!issue_qk(i + 2, j & 1, 0)) { ok = false; break; }
                 umma_commit(bar_kempty + 8 * ((i + 2) % kStages));
-                if (j + 3 == n) umma_commit(bar_qfree);
               }
             }
           }
@@ -257,109 +257,141 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
       }
     }
   } else {
-    setmaxnreg_inc<224>();
+    setmaxnreg_inc<200>();
     // ------------------------------------------------------------------ softmax, one row per thread
     const int t = warp >> 2, wq = warp & 3;
-    const int row = wq * 32 + lane;                            // of the tile
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
     const uint32_t tmem_s = tmem_base + t * 128 + lane_off, tmem_o = tmem_base + 256 + t * 128 + lane_off;
     const float sl2 = p.scale * kSpLog2e;
     bool ok = true;
     int done = 0;
+    uint8_t* stage = smem + L::kQ + t * L::kTileBytes + wq * (L::kTileBytes / 4);       // this warp's quarter of a tile of queries, when they are done with
     for (int u = u_begin; u < u_end && ok;) {
-      const SpPart s = sp_next(p, list, totals, u, u_end);
+      const SpPart s = sp_next(p, list, held, u, u_end);
       const bool twin = s.n <= half;                           // one tile of rows: A has the part's even units, B the odd ones
-      const int shared = shared_of[s.g], step = twin ? 2 : 1, j0 = s.u0 + (twin ? t : 0);
+      const int shared = s.shared, step = twin ? 2 : 1, j0 = s.u0 + (twin ? t : 0);
+      const int tile_seqs = twin ? s.n : t == 0 ? half : s.n - half;
+      const bool busy = wq * 32 < tile_seqs * list.per;        // this warp has rows
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = j0; j < s.u1; j += step, ++done) {
         if (!mbar_wait(bar_sfull + 8 * t, done & 1, abort_flag, status, 59)) { ok = false; break; }
         tc_fence_after();
-        uint32_t r[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) st_ld32(tmem_s + c * 32, r + c * 32);
-        tmem_ld_wait();
-        const int valid = shared - j * kSpUnit;
-        if (valid < kSpUnit) {
-#pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i >= valid) r[i] = 0xff800000u;                // -inf
-        }
-        float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 128; i += 4) {
-          mx0 = fmaxf(mx0, __uint_as_float(r[i]));
-          mx1 = fmaxf(mx1, __uint_as_float(r[i + 1]));
-          mx2 = fmaxf(mx2, __uint_as_float(r[i + 2]));
-          mx3 = fmaxf(mx3, __uint_as_float(r[i + 3]));
-        }
-        const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
-        const bool grow = mx > m_run && ((mx - m_run) * sl2 > kStRescale || m_run == -INFINITY);
-        float alpha = 1.f;
-        if (grow) {
-          alpha = m_run == -INFINITY ? 0.f : wm_ex2((m_run - mx) * sl2);
-          m_run = mx;
-          l_run *= alpha;
-        }
-        if (j > j0 && __any_sync(0xffffffffu, grow)) {
-          // O has the sum over the units in front once their last product is done; the next one cannot start before P below
-          if (!mbar_wait(bar_oready + 8 * t, (done - 1) & 1, abort_flag, status, 60)) { ok = false; break; }
-          tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            st_ld32(tmem_o + c * 32, o);
+        if (busy) {
+          const int valid = shared - j * kSpUnit;
+          // 64 scores of the row, those behind the last token -infinity
+          auto scores = [&](int c, uint32_t (&r)[64]) {
+            st_ld32(tmem_s + c * 64, r);
+            st_ld32(tmem_s + c * 64 + 32, r + 32);
             tmem_ld_wait();
+            if (valid < kSpUnit) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            st_st32(tmem_o + c * 32, o);
+              for (int i = 0; i < 64; ++i)
+                if (c * 64 + i >= valid) r[i] = 0xff800000u;
+            }
+          };
+          float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t r[64];
+            scores(c, r);
+#pragma unroll
+            for (int i = 0; i < 64; i += 8) {
+              mx0 = st_max3(mx0, __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+              mx1 = st_max3(mx1, __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+              mx2 = st_max3(mx2, __uint_as_float(r[i + 4]), __uint_as_float(r[i + 5]));
+              mx3 = st_max3(mx3, __uint_as_float(r[i + 6]), __uint_as_float(r[i + 7]));
+            }
           }
+          const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+          const bool grow = mx > m_run && ((mx - m_run) * sl2 > kStRescale || m_run == -INFINITY);
+          float alpha = 1.f;
+          if (grow) {
+            alpha = m_run == -INFINITY ? 0.f : wm_ex2((m_run - mx) * sl2);
+            m_run = mx;
+            l_run *= alpha;
+          }
+          if (j > j0 && __any_sync(0xffffffffu, grow)) {
+            // O has the sum over the units in front once their last product is done; the next one cannot start before P is there
+            if (!mbar_wait(bar_oready + 8 * t, (done - 1) & 1, abort_flag, status, 60)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              st_ld32(tmem_o + c * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              st_st32(tmem_o + c * 32, o);
+            }
+          }
+          const float msc = (m_run == -INFINITY ? 0.f : m_run) * sl2;
+          float rs0 = 0.f, rs1 = 0.f, rs2 = 0.f, rs3 = 0.f;
+          // P takes the columns of scores that have been read.  64 at a time, not all: the loops' code is met for the first time in every launch, and unrolled over a row of 128 that took
+          // 6500 cycles, twice a unit's time
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t r[64];
+            scores(c, r);
+            uint32_t packed[32];
+#pragma unroll
+            for (int i = 0; i < 64; i += 4) {
+              const float p0 = wm_ex2(fmaf(__uint_as_float(r[i]), sl2, -msc)), p1 = wm_ex2(fmaf(__uint_as_float(r[i + 1]), sl2, -msc));
+              const float p2 = wm_ex2(fmaf(__uint_as_float(r[i + 2]), sl2, -msc)), p3 = wm_ex2(fmaf(__uint_as_float(r[i + 3]), sl2, -msc));
+              rs0 += p0;
+              rs1 += p1;
+              rs2 += p2;
+              rs3 += p3;
+              packed[i / 2] = sp_pack<T>(p0, p1);
+              packed[i / 2 + 1] = sp_pack<T>(p2, p3);
+            }
+            st_st32(tmem_s + c * 32, packed);
+          }
+          l_run += (rs0 + rs1) + (rs2 + rs3);
           tmem_st_wait();
         }
-        const float msc = (m_run == -INFINITY ? 0.f : m_run) * sl2;
-        float rs0 = 0.f, rs1 = 0.f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t packed[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float p0 = wm_ex2(fmaf(__uint_as_float(r[c * 32 + 2 * i]), sl2, -msc)), p1 = wm_ex2(fmaf(__uint_as_float(r[c * 32 + 2 * i + 1]), sl2, -msc));
-            rs0 += p0;
-            rs1 += p1;
-            packed[i] = sp_pack<T>(p0, p1);
-          }
-          tmem_st_32x16(tmem_s + c * 16, packed);              // every score is in registers
-        }
-        l_run += rs0 + rs1;
-        tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_pfull + 8 * t);
       }
       if (!ok) break;
-      // ---- the part's sums
+      // ---- the part's sums, 32 columns at a time through shared memory: rows of 512 bytes by threads of their own would be 32 sectors a store
       const bool some = j0 < s.u1;
       if (some && !mbar_wait(bar_oready + 8 * t, (done - 1) & 1, abort_flag, status, 61)) break;
       tc_fence_after();
-      const int seq = (twin ? 0 : t * half) + row / list.per, h = row % list.per;
-      const bool real = row < tile_rows && seq < s.n && h < group - (s.vh % list.parts) * list.per;
-      const long long to = sp_row(list, s.vh, s.e, blockIdx.x, s.u0 == 0) + seq * list.per + h + (twin && t ? list.rows : 0);
-      if (real) list.ml[to] = make_float2(m_run * sl2, l_run);
-      if (!some) continue;                                     // a part of one unit: B has none
+      if (busy) {
+        const long long to = sp_row(list, s.vh, s.e, blockIdx.x, s.u0 == 0) + (twin ? 0 : t * tile_rows) + wq * 32 + (twin && t ? list.rows : 0);
+        const int rows = min(32, tile_seqs * list.per - wq * 32);
+        if (lane < rows) list.ml[to + lane] = make_float2(m_run * sl2, l_run);
+        if (some) {                                            // a part of one unit: B has none
+          constexpr int kCols = 32, kPieces = kCols / 4;       // of 16 bytes
+#pragma unroll 1
+          for (int c = 0; c < D / kCols; ++c) {
+            // piece i of row `lane` to place i ^ lane: no two of eight rows meet in a bank
+            uint32_t o[kCols];
+            st_ld32(tmem_o + c * kCols, o);
+            tmem_ld_wait();
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        st_ld32(tmem_o + c * 32, o);
-        tmem_ld_wait();
-        if (real) {
-          uint4* out = reinterpret_cast<uint4*>(list.acc + to * D + c * 32);
+            for (int i = 0; i < kPieces; ++i)
+              *reinterpret_cast<uint4*>(stage + (lane * kPieces + ((i ^ lane) & (kPieces - 1))) * 16) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) out[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            for (int i = 0; i < kPieces; ++i) {
+              const int r = i * (32 / kPieces) + lane / kPieces, k = lane % kPieces;
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + (r * kPieces + ((k ^ r) & (kPieces - 1))) * 16);
+              if (r < rows) *reinterpret_cast<uint4*>(list.acc + (to + r) * D + c * kCols + k * 4) = v;
+            }
+            __syncwarp();
+          }
         }
       }
+      fence_proxy_async_smem();                                // the next queries come by TMA
       tc_fence_before();                                       // the next part's first product overwrites O behind the next arrival
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_qfree);
     }
   }
 
+  pdl_wait();                                                  // this launch ends behind the one in front, so that the join, which waits for this one, finds both done
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {
@@ -396,16 +428,16 @@ int launch(const rb::SpParams& p, cudaStream_t stream) {
   m = rbhost::get_tmap_4d(p.v, 2, dims, str, box, 1, &err);
   if (!m) return err ? err : -7;
   maps.v = *m;
-  constexpr int kMostSmem = rb::StSmem<D>::kTotal + (2 * rb::kStMostBatch + 1) * 4 + 1024;
+  constexpr size_t kMostSmem = rb::StSmem<D>::kTotal + rb::sp_held_bytes(rb::kStMostBatch, rb::kStMostBatch) + 1024;
   static_assert(kMostSmem + 1024 <= 227 * 1024, "shared memory");
   static bool configured[64] = {false};
   const int dev = rbhost::device_slot();
   if (!configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(rb::shared_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
+    const cudaError_t e = cudaFuncSetAttribute(rb::shared_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostSmem));
     if (e != cudaSuccess) return static_cast<int>(e);
     configured[dev] = true;
   }
-  const size_t smem = rb::StSmem<D>::kTotal + (2 * static_cast<size_t>(p.batch) + 1) * 4 + 1024;
+  const size_t smem = rb::StSmem<D>::kTotal + rb::sp_held_bytes(p.batch, p.groups) + 1024;
   return static_cast<int>(rbhost::launch_pdl(rb::shared_tc_kernel<T, D>, dim3(l.ctas), dim3(rb::kStThreads), smem, stream, 1, maps, p,
                                              rbhost::status_ptr() RB_BOUNDS_ARG));
 }

@@ -17,7 +17,7 @@ import torch
 from .. import _native as N
 
 C = N.C
-MOST_COUNT, MOST_BEAMS, MOST_GROUP, MOST_SEQUENCES = 128, 256, 256, 8192
+MOST_COUNT, MOST_BEAMS, MOST_GROUP, MOST_SEQUENCES = 128, 256, 256, 4096
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 # The argument blocks of csrc/kernels/beam.h, move_rows.h and shared_prefix.h, packed
@@ -277,7 +277,7 @@ def paged_attention_shared(q, k_cache, v_cache, groups: PrefixGroups, shared_len
     each sequence's own.  Where the shortest sequence of a group has fewer tokens (those without any aside) only that many count as shared.  A sequence without tokens
     gets zeros.  Returns [batch, heads * head_dim].
 
-    On a GPU: bf16 or fp16, heads of 64 or 128, up to 8192 sequences.  A sequence's result depends, within rounding, on the batch it is in; the same call gives the
+    On a GPU: bf16 or fp16, heads of 64 or 128, up to 4096 sequences.  A sequence's result depends, within rounding, on the batch it is in; the same call gives the
     same bits."""
     if q.dim() != 2 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or not q.dtype is k_cache.dtype is v_cache.dtype or \
             not k_cache.is_contiguous() or not v_cache.is_contiguous():
