@@ -22,10 +22,10 @@
 
 namespace rb {
 
-constexpr int kStThreads = 384;          // warps 0-7 softmax, 8 and 10 TMA, 9 MMA, 11 only gives its registers away
+constexpr int kStThreads = 384;          // warps 0-7 softmax, 8, 10 and 11 TMA, 9 MMA
 constexpr int kStTile = 128;
 constexpr float kStRescale = 8.f;        // log2 units
-constexpr int kStMostBatch = 1536;       // their totals, tokens and spans beside 192 KB of tiles
+constexpr int kStMostBatch = 1024;       // their totals, tokens and spans beside 192 KB of tiles
 
 __device__ __forceinline__ void st_ld32(uint32_t taddr, uint32_t* r) { tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r)); }
 __device__ __forceinline__ void st_st32(uint32_t taddr, const uint32_t* r) {
@@ -49,8 +49,9 @@ struct StSmem {
   static constexpr int kV = kK + kStages * kTileBytes;
   static constexpr int kBar = kV + kStages * kTileBytes;
   static constexpr int kNumBars = 3 + 4 * kStages + 6;           // q, q free, tail; full and empty per K and V stage; s_full[2], p_full[2], o_ready[2]
-  static constexpr int kInts = kBar + kNumBars * 8;              // TMEM address, abort flag, then running totals and shared tokens
-  static constexpr int kTotal = kInts + 16;
+  static constexpr int kInts = kBar + kNumBars * 8;              // TMEM address, abort flag
+  static constexpr int kStage = (kInts + 16 + 127) / 128 * 128;  // 2 KB for each softmax warp: 16 columns of its rows' sums
+  static constexpr int kTotal = kStage + 8 * 2048;               // then what is held of the list
 };
 
 struct StMaps {
@@ -81,7 +82,7 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
 
   if (threadIdx.x == 0) {
     mbar_init(bar_q, 1);
-    mbar_init(bar_qfree, 8);
+    mbar_init(bar_qfree, 1);
     mbar_init(bar_tail, 1);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar_kfull + 8 * s, 1);
@@ -117,34 +118,22 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
   if (warp >= 8) {
     setmaxnreg_dec<104>();
     if (warp == 8 || warp == 10) {
-      // ---------------------------------------------------------------- TMA producers, all lanes: warp 8 queries and keys, warp 10 values
+      // ---------------------------------------------------------------- TMA producers, all lanes: warp 8 keys, warp 10 values
       const bool values = warp == 10;
       const CUtensorMap* map = values ? &maps.v : &maps.k;
       const uint32_t tiles = values ? sV : sK, full = values ? bar_vfull : bar_kfull, empty = values ? bar_vempty : bar_kempty;
       const int bs = p.block_size, size = min(bs, kSpUnit);    // rows of a copy
       bool ok = true;
-      int it = 0, part = 0, tails = 0;
-      for (int u = u_begin; u < u_end && ok; ++part) {
+      int it = 0, tails = 0;
+      for (int u = u_begin; u < u_end && ok;) {
         const SpPart s = sp_next(p, list, held, u, u_end);
-        const int shared = s.shared, head0 = s.vh * list.per;
+        const int shared = s.shared;
         // pages of a unit: lane i has the i-th (one of 128 rows, from `row` on, where pages are larger); looked up a unit ahead
         auto page_of = [&](int unit) {
           const int at = unit * kSpUnit + lane * size;
           return unit < s.u1 && lane * size < kSpUnit && at < shared ? s.table[at / bs] : 0;
         };
         int page = page_of(s.u0);
-        if (!values) {
-          if (part > 0) ok = mbar_wait(bar_qfree, (part - 1) & 1, abort_flag, status, 51);
-          if (!__all_sync(0xffffffffu, ok)) break;
-          if (lane == 0) {
-            const int n = s.n > half ? 2 : 1;
-            mbar_arrive_expect_tx(bar_q, n * tile_rows * 128 * (D / 64));
-            for (int t = 0; t < n; ++t)
-#pragma unroll
-              for (int hf = 0; hf < D / 64; ++hf)
-                tma_load_4d(sQ + t * L::kTileBytes + hf * L::kHalf, &maps.q, hf * 64, head0, s.b + t * half, 0, bar_q);
-          }
-        }
         for (int unit = s.u0; unit < s.u1; ++unit, ++it) {
           const int st = it % kStages, first = unit * kSpUnit, valid = min(kSpUnit, shared - first), pages = (valid + size - 1) / size;
           int blk = page;
@@ -178,6 +167,22 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
             __syncwarp();
             if (lane == 0) mbar_arrive(full + 8 * st);
           }
+        }
+      }
+    } else if (warp == 11) {
+      // ---------------------------------------------------------------- queries of a part, behind the last product of the part in front
+      bool ok = true;
+      int part = 0;
+      for (int u = u_begin; u < u_end && ok; ++part) {
+        const SpPart s = sp_next(p, list, held, u, u_end);
+        if (part > 0) ok = mbar_wait(bar_qfree, (part - 1) & 1, abort_flag, status, 51);
+        if (ok && lane == 0) {
+          const int n = s.n > half ? 2 : 1;
+          mbar_arrive_expect_tx(bar_q, n * tile_rows * 128 * (D / 64));
+          for (int t = 0; t < n; ++t)
+#pragma unroll
+            for (int hf = 0; hf < D / 64; ++hf)
+              tma_load_4d(sQ + t * L::kTileBytes + hf * L::kHalf, &maps.q, hf * 64, s.vh * list.per, s.b + t * half, 0, bar_q);
         }
       }
     } else if (warp == 9) {
@@ -225,6 +230,7 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
             for (int t = 0; t < 2 && ok; ++t) ok = issue_qk(it, t, t);
             if (!ok) break;
             umma_commit(bar_kempty + 8 * (it % kStages));
+            if (n == 1) umma_commit(bar_qfree);
             for (int j = 0; j < n && ok; ++j) {
               const int i = it + j, st = i % kStages;
               if (!mbar_wait(bar_vfull + 8 * st, (i / kStages) & 1, abort_flag, status, 57)) { ok = false; break; }
@@ -235,12 +241,14 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
               if (!ok) break;
               umma_commit(bar_vempty + 8 * st);
               if (j + 1 < n) umma_commit(bar_kempty + 8 * ((i + 1) % kStages));
+              if (j + 2 == n) umma_commit(bar_qfree);            // the last products that read the queries have been issued
             }
           } else {                                               // one: units in turn with the S and O of A and of B
             for (int j = 0; j < 2 && j < n && ok; ++j) {
               ok = issue_qk(it + j, j, 0);
               if (!ok) break;
               umma_commit(bar_kempty + 8 * ((it + j) % kStages));
+              if (j + 1 == n) umma_commit(bar_qfree);
             }
             for (int j = 0; j < n && ok; ++j) {
               const int i = it + j, st = i % kStages;
@@ -249,6 +257,7 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
               if (j + 2 < n) {
                 if (!issue_qk(i + 2, j & 1, 0)) { ok = false; break; }
                 umma_commit(bar_kempty + 8 * ((i + 2) % kStages));
+                if (j + 3 == n) umma_commit(bar_qfree);
               }
             }
           }
@@ -265,7 +274,7 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
     const float sl2 = p.scale * kSpLog2e;
     bool ok = true;
     int done = 0;
-    uint8_t* stage = smem + L::kQ + t * L::kTileBytes + wq * (L::kTileBytes / 4);       // this warp's quarter of a tile of queries, when they are done with
+    uint8_t* stage = smem + L::kStage + warp * 2048;
     for (int u = u_begin; u < u_end && ok;) {
       const SpPart s = sp_next(p, list, held, u, u_end);
       const bool twin = s.n <= half;                           // one tile of rows: A has the part's even units, B the odd ones
@@ -354,7 +363,7 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
         if (lane == 0) mbar_arrive(bar_pfull + 8 * t);
       }
       if (!ok) break;
-      // ---- the part's sums, 32 columns at a time through shared memory: rows of 512 bytes by threads of their own would be 32 sectors a store
+      // ---- the part's sums, 16 columns at a time through shared memory: rows of 512 bytes by threads of their own would be 32 sectors a store
       const bool some = j0 < s.u1;
       if (some && !mbar_wait(bar_oready + 8 * t, (done - 1) & 1, abort_flag, status, 61)) break;
       tc_fence_after();
@@ -363,31 +372,26 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
         const int rows = min(32, tile_seqs * list.per - wq * 32);
         if (lane < rows) list.ml[to + lane] = make_float2(m_run * sl2, l_run);
         if (some) {                                            // a part of one unit: B has none
-          constexpr int kCols = 32, kPieces = kCols / 4;       // of 16 bytes
 #pragma unroll 1
-          for (int c = 0; c < D / kCols; ++c) {
-            // piece i of row `lane` to place i ^ lane: no two of eight rows meet in a bank
-            uint32_t o[kCols];
-            st_ld32(tmem_o + c * kCols, o);
+          for (int c = 0; c < D / 16; ++c) {
+            // piece i (16 bytes) of row `lane` to place i ^ lane / 2 of 4: no two of eight rows meet in a bank
+            uint32_t o[16];
+            tmem_ld_32x16(tmem_o + c * 16, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i)
-              *reinterpret_cast<uint4*>(stage + (lane * kPieces + ((i ^ lane) & (kPieces - 1))) * 16) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(stage + (lane * 4 + ((i ^ lane >> 1) & 3)) * 16) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
             __syncwarp();
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-              const int r = i * (32 / kPieces) + lane / kPieces, k = lane % kPieces;
-              const uint4 v = *reinterpret_cast<const uint4*>(stage + (r * kPieces + ((k ^ r) & (kPieces - 1))) * 16);
-              if (r < rows) *reinterpret_cast<uint4*>(list.acc + (to + r) * D + c * kCols + k * 4) = v;
+            for (int i = 0; i < 4; ++i) {
+              const int r = i * 8 + (lane >> 2), k = lane & 3;
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + (r * 4 + ((k ^ r >> 1) & 3)) * 16);
+              if (r < rows) *reinterpret_cast<uint4*>(list.acc + (to + r) * D + c * 16 + k * 4) = v;
             }
             __syncwarp();
           }
         }
       }
-      fence_proxy_async_smem();                                // the next queries come by TMA
       tc_fence_before();                                       // the next part's first product overwrites O behind the next arrival
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_qfree);
     }
   }
 
