@@ -1,5 +1,6 @@
 // Paged-KV block allocator: a free list of fixed-size blocks and one block table per sequence, and for models with
 // recurrent layers a free list of state slots of which every sequence holds one from its first reservation to its end.
+// A block may be in several tables (rb_ba_fork): it counts its owners and is free again when the last one lets go of it.
 // Semantics follow the reference's PagedCache (crates/nn/src/kv_cache.rs:382-432) with its defect removed: a
 // second reservation for a sequence extends the table instead of overwriting it (kv_cache.rs:420-423).
 #include <mutex>
@@ -11,11 +12,25 @@
 struct RbBlockAllocator {
   int num_blocks, block_size;
   std::vector<int32_t> free_list;                                // stack; lowest ids are handed out first
+  std::vector<int32_t> owners;                                   // tables that each block is in
+  int shared = 0;                                                // blocks with more than one
   std::unordered_map<int64_t, std::vector<int32_t>> tables;
   bool slotted = false;                                          // sequences also hold a state slot
   std::vector<int32_t> free_slots;
   std::unordered_map<int64_t, int32_t> slots;
   mutable std::mutex mu;
+
+  int32_t take() {
+    const int32_t b = free_list.back();
+    free_list.pop_back();
+    owners[b] = 1;
+    return b;
+  }
+  void give(int32_t b) {
+    const int left = --owners[b];
+    if (left == 1) --shared;
+    if (left == 0) free_list.push_back(b);
+  }
 };
 
 extern "C" {
@@ -26,6 +41,7 @@ RbBlockAllocator* rb_ba_create(int num_blocks, int block_size) {
   a->num_blocks = num_blocks;
   a->block_size = block_size;
   a->free_list.reserve(num_blocks);
+  a->owners.assign(num_blocks, 0);
   for (int i = num_blocks - 1; i >= 0; --i) a->free_list.push_back(i);
   return a;
 }
@@ -81,10 +97,7 @@ int rb_ba_reserve(RbBlockAllocator* a, int64_t seq_id, int num_tokens) {
     return 0;
   }
   auto& tab = a->tables[seq_id];
-  for (int i = 0; i < need; ++i) {
-    tab.push_back(a->free_list.back());
-    a->free_list.pop_back();
-  }
+  for (int i = 0; i < need; ++i) tab.push_back(a->take());
   return need;
 }
 
@@ -93,7 +106,7 @@ int rb_ba_free(RbBlockAllocator* a, int64_t seq_id) {
   auto it = a->tables.find(seq_id);
   if (it == a->tables.end()) return 0;
   const int n = (int)it->second.size();
-  for (auto rit = it->second.rbegin(); rit != it->second.rend(); ++rit) a->free_list.push_back(*rit);
+  for (auto rit = it->second.rbegin(); rit != it->second.rend(); ++rit) a->give(*rit);
   a->tables.erase(it);
   auto st = a->slots.find(seq_id);
   if (st != a->slots.end()) {
@@ -111,10 +124,93 @@ int rb_ba_trim(RbBlockAllocator* a, int64_t seq_id, int num_tokens) {
   if (it == a->tables.end() || num_tokens < 0) return -1;
   int n = 0;
   for (const size_t keep = blocks_for(a, num_tokens); it->second.size() > keep; ++n) {
-    a->free_list.push_back(it->second.back());
+    a->give(it->second.back());
     it->second.pop_back();
   }
   return n;
+}
+
+// Makes `child` a sequence that shares the parent's first num_tokens tokens: full blocks are in both tables, and for a block that these tokens end in the child takes one of its own.
+// Returns 1 when the caller has to copy block *src to *dst, 0 when there is nothing to copy, -1 when the parent is unknown or has no blocks for so many tokens, or the child is there
+// already, -2 when there is no free block or state slot (nothing changed).
+int rb_ba_fork(RbBlockAllocator* a, int64_t parent, int64_t child, int num_tokens, int32_t* src, int32_t* dst) try {
+  std::lock_guard<std::mutex> l(a->mu);
+  auto it = a->tables.find(parent);
+  if (it == a->tables.end() || num_tokens < 0 || blocks_for(a, num_tokens) > (int)it->second.size() || a->tables.count(child)) return -1;
+  const int full = num_tokens / a->block_size;
+  const bool partial = num_tokens % a->block_size != 0;
+  if ((partial && a->free_list.empty()) || (a->slotted && a->free_slots.empty())) return -2;
+  std::vector<int32_t> tab(it->second.begin(), it->second.begin() + full);
+  const int32_t last = partial ? it->second[full] : -1;
+  tab.reserve(full + 1);
+  auto& at = a->tables[child];                                   // may move the parent's entry: not used from here on
+  if (a->slotted) {
+    a->slots[child] = a->free_slots.back();
+    a->free_slots.pop_back();
+  }
+  for (int32_t b : tab)
+    if (++a->owners[b] == 2) ++a->shared;
+  if (partial) {
+    *src = last;
+    *dst = a->take();
+    tab.push_back(*dst);
+  }
+  at.swap(tab);
+  return partial ? 1 : 0;
+} catch (...) {
+  return -2;
+}
+
+int rb_ba_num_shared(const RbBlockAllocator* a) { std::lock_guard<std::mutex> l(a->mu); return a->shared; }
+
+// Gives the sequence blocks of its own in place of shared ones among those of tokens first .. first + n - 1, which are about to be written.  Returns how many pairs of blocks
+// (src, dst, room for `max`) the caller has to copy, -1 for an unknown sequence or tokens without blocks, -2 without enough free blocks or room (nothing changed).
+int rb_ba_own(RbBlockAllocator* a, int64_t seq_id, int64_t first, int64_t n, int32_t* src, int32_t* dst, int max) {
+  std::lock_guard<std::mutex> l(a->mu);
+  auto it = a->tables.find(seq_id);
+  if (it == a->tables.end() || first < 0 || n < 0 || first + n > (int64_t)it->second.size() * a->block_size) return -1;
+  if (n == 0) return 0;
+  const int64_t b0 = first / a->block_size, b1 = (first + n - 1) / a->block_size;
+  int need = 0;
+  for (int64_t i = b0; i <= b1; ++i) need += a->owners[it->second[i]] > 1 ? 1 : 0;
+  if (need > (int)a->free_list.size() || need > max) return -2;
+  int k = 0;
+  for (int64_t i = b0; i <= b1; ++i) {
+    int32_t& b = it->second[i];
+    if (a->owners[b] < 2) continue;
+    src[k] = b;
+    dst[k] = a->take();
+    a->give(b);
+    b = dst[k++];
+  }
+  return k;
+}
+
+// Moves what is in use to the lowest blocks: tables, owners and the free list change at once, and the caller copies the blocks src[i] to dst[i] (room for num_blocks each).
+// Returns the number of pairs, -1 without memory.
+int rb_ba_compact(RbBlockAllocator* a, int32_t* src, int32_t* dst) try {
+  std::lock_guard<std::mutex> l(a->mu);
+  const int used = a->num_blocks - (int)a->free_list.size();
+  std::vector<int32_t> to(a->num_blocks, -1), rest;
+  rest.reserve(a->num_blocks);
+  int n = 0, low = 0;
+  for (int b = used; b < a->num_blocks; ++b) {
+    if (!a->owners[b]) continue;
+    while (a->owners[low]) ++low;
+    src[n] = b;
+    dst[n++] = low;
+    to[b] = low;
+    a->owners[low] = a->owners[b];
+    a->owners[b] = 0;
+  }
+  for (int b = a->num_blocks - 1; b >= used; --b) rest.push_back(b);
+  for (auto& t : a->tables)
+    for (int32_t& b : t.second)
+      if (to[b] >= 0) b = to[b];
+  a->free_list.swap(rest);
+  return n;
+} catch (...) {
+  return -1;
 }
 
 int rb_ba_table_len(const RbBlockAllocator* a, int64_t seq_id) {

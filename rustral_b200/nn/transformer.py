@@ -238,8 +238,11 @@ class TransformerEncoderDecoder(Module, Trainable, Saveable):
         memory = self.encoder.forward(src, ctx)
         return self.decoder.forward(tgt, ctx, memory)
 
-    def generate(self, src, ctx: ForwardCtx, bos: int, eos: int, max_len: int = 32) -> list:
+    def generate(self, src, ctx: ForwardCtx, bos: int, eos: int, max_len: int = 32, beams: int = 1) -> list:
+        """Tokens from `bos` on, greedy, or with `beams` the best of a beam search (by the mean of the tokens' logarithmic probabilities)."""
         memory = self.encoder.forward(src, ctx)
+        if beams > 1:
+            return self._search(memory, ctx, bos, eos, max_len, beams)
         out = [bos]
         for _ in range(max_len):
             tok = self.decoder.generate_token(out, ctx, memory)
@@ -247,3 +250,25 @@ class TransformerEncoderDecoder(Module, Trainable, Saveable):
             if tok == eos:
                 break
         return out
+
+    def _search(self, memory, ctx: ForwardCtx, bos: int, eos: int, max_len: int, beams: int) -> list:
+        """All on the device: ended beams stay in the batch and go on with `eos` at no cost."""
+        dev = memory.device
+        ids = torch.full((beams, 1), bos, dtype=torch.int64, device=dev)
+        scores = torch.full((1, beams), float("-inf"), device=dev)
+        scores[0, 0] = 0.0
+        ended = torch.zeros((1, beams), dtype=torch.bool, device=dev)
+        lens = torch.zeros(beams, dtype=torch.int64, device=dev)
+        memory = memory[:1].expand(beams, -1, -1).contiguous()
+        for _ in range(max_len):
+            logits = self.decoder.forward(ids, ctx, memory)[:, -1].float()
+            scores, rows, tokens = ops.beam_select(logits, scores, beams, ended, eos)
+            state = [ids, lens.view(-1, 1), ended.view(-1, 1)]
+            ops.reorder_rows_(state, rows.view(-1))               # what the chosen beams inherit
+            lens += ~ended.view(-1)
+            ended |= tokens == eos
+            ids = torch.cat([ids, tokens.view(-1, 1)], 1)
+            if bool(ended.all()):
+                break
+        at = int((scores.view(-1) / lens).argmax())
+        return ids[at, :1 + int(lens[at])].tolist()

@@ -270,6 +270,14 @@ def shared_supported(q, k_cache, v_cache) -> bool:
         k_cache.shape[3] in (64, 128) and k_cache.is_contiguous() and v_cache.is_contiguous() and q.shape[0] <= MOST_SEQUENCES
 
 
+def shared_pays(groups: PrefixGroups, shared_lens, row_bytes: int) -> bool:
+    """Whether reading the shared tokens once saves more than the further launches cost.  `row_bytes`: of a token's keys and values."""
+    return row_bytes * sum((n - 1) * p for n, p in zip(groups.sizes, shared_lens)) >= SHARED_PAYS
+
+
+SHARED_PAYS = 32 << 20
+
+
 def paged_attention_shared(q, k_cache, v_cache, groups: PrefixGroups, shared_lens, block_tables, context_lens, scale=None, out=None):
     """Decode attention for sequences that share their first tokens.  q [batch, heads * head_dim] (row-strided views allowed); caches
     [blocks, block_size, kv_heads, head_dim]; block_tables int32 [batch, width], context_lens int32 [batch] as for decode attention; shared_lens int32

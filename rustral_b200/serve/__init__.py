@@ -3,6 +3,7 @@ from .kv_cache import CacheQuantization, CacheConfig, CacheMemoryStats, KVCache,
 from .scheduler import RequestPriority, RequestState, Request, SchedulingPolicy, Batch, Scheduler, PyScheduler, SchedulerStats
 from .sampler import Sampler
 from .model_runner import ModelRunner
+from .beam import BeamSearch, Hypothesis
 from .engine import ServingEngine, ServingMetrics, run_poisson_workload
 
 __all__ = [n for n in dir() if not n.startswith("_")]

@@ -8,6 +8,7 @@ from dataclasses import dataclass
 
 import torch
 
+from .beam import BeamSearch, Hypothesis
 from .model_runner import ModelRunner
 from .sampler import Sampler
 from .scheduler import RequestPriority, RequestState, Scheduler, SchedulingPolicy
@@ -138,6 +139,11 @@ class ServingEngine:
         if not keep_record:
             self.release(rid)
         return tokens
+
+    def beam_search(self, prompt, max_tokens: int, beams: int = 4, length_penalty: float = 1.0) -> list[Hypothesis]:
+        """The best `beams` continuations of one prompt, best first (serve.beam.BeamSearch with the engine's end-of-sequence id).  The search runs to its end before the engine steps
+        again; running requests keep their blocks, so it is refused where the free ones would not do."""
+        return BeamSearch(self.runner, beams, self.eos_id, length_penalty).generate([list(prompt)], max_tokens)[0]
 
     def abort(self, rid: int) -> bool:
         """Cancels one unfinished request: its KV blocks are freed and its prefill progress and callback are dropped.

@@ -158,8 +158,12 @@ class EngineLoop:
         self._thread.start()
 
     def _admit(self, item) -> None:
-        prompt, max_tokens, box, ev = item
+        prompt, max_tokens, box, ev, search = item
         try:
+            if search is not None:                   # a whole search: the others wait for it
+                box.append((True, self.engine.beam_search(prompt, max_tokens, **search)))
+                ev.set()
+                return
             self._waiting[self.engine.submit(prompt, max_tokens)] = (box, ev)
         except Exception as e:   # noqa: BLE001 - delivered to the waiting handler
             box.append((False, e))
@@ -204,9 +208,10 @@ class EngineLoop:
                     continue
                 self._deliver()
 
-    def generate(self, prompt, max_tokens: int, timeout: float | None = 600.0) -> list:
+    def generate(self, prompt, max_tokens: int, timeout: float | None = 600.0, search: dict | None = None) -> list:
+        """The request's tokens, or with `search` (arguments of ServingEngine.beam_search) its hypotheses."""
         box, ev = [], threading.Event()
-        self._inbox.put((list(prompt), int(max_tokens), box, ev), timeout=timeout)
+        self._inbox.put((list(prompt), int(max_tokens), box, ev, search), timeout=timeout)
         if not ev.wait(timeout):
             raise TimeoutError("generation timed out")
         ok, val = box[0]
@@ -220,7 +225,7 @@ class EngineLoop:
 
 
 def engine_generate_fn(engine, loop: "EngineLoop | None" = None):
-    """Handler body of /v1/generate.  With `loop` the request joins the shared engine loop; without it the calling
+    """Handler body of /v1/generate.  "beams" (and "length_penalty") ask for a beam search, whose continuations come back beside the best one's tokens.  With `loop` the request joins the shared engine loop; without it the calling
     thread runs the engine to completion (single-request use)."""
     def fn(body):
         prompt = body.get("prompt")
@@ -231,6 +236,10 @@ def engine_generate_fn(engine, loop: "EngineLoop | None" = None):
             raise BadRequest("token id out of range")
         max_tokens = int(body.get("max_tokens", 16))
         try:
+            if "beams" in body:
+                search = dict(beams=int(body["beams"]), length_penalty=float(body.get("length_penalty", 1.0)))
+                found = loop.generate(prompt, max_tokens, search=search) if loop is not None else engine.beam_search(prompt, max_tokens, **search)
+                return {"tokens": found[0].tokens if found else [], "beams": [{"tokens": h.tokens, "score": h.score} for h in found]}
             if loop is not None:
                 return {"tokens": loop.generate(prompt, max_tokens)}
             return {"tokens": engine.generate(prompt, max_tokens)}

@@ -14,6 +14,7 @@ import torch
 
 from .. import _native as N
 from ..core.errors import InvalidArgument
+from ..ops.beams import copy_blocks_, reorder_rows_
 from ..ops.paged_e4m3 import PagesE4M3, kv_evict_e4m3
 
 
@@ -127,6 +128,14 @@ class KVCache:
     def reset(self) -> None:
         self.len = 0
 
+    def _filled(self) -> list:
+        return [self.k[:, :, :self.len], self.v[:, :, :self.len]]
+
+    def reorder(self, index: torch.Tensor) -> None:
+        """Batch entries in a new order, in place: entry i becomes what entry index[i] (int64 on the cache's device) was, as the beams of a search
+        take over their parents' entries.  Only what is filled moves."""
+        reorder_rows_(self._filled(), index)
+
     def memory_stats(self) -> CacheMemoryStats:
         alloc = 2 * self.k.numel() * self.k.element_size()
         used = int(alloc * self.len / max(1, self.config.max_seq_len))
@@ -188,6 +197,9 @@ class PagedCache:
     Layers with recurrent state add one tensor [num_slots, ...] per state name (`state[layer][name]`); a sequence holds the
     same slot in all of them from its first `allocate` to `free`.  A slot is not cleared when it changes hands: the layers
     take a sequence's state as zero at position 0, whatever the slot holds.
+
+    Sequences may share blocks (`fork`): a block belongs to every table that it is in and is free when the last of them lets go of it.  A sequence that is about
+    to write into a block that others have too takes one of its own first (`own`, which the runner calls), so that no sequence sees another's tokens.
 
     `quantization` FP8 (not with `layers`): keys and values are e4m3 codes with a power of two for each page and head, one
     `ops.PagesE4M3` per layer in `pages` (`k` and `v` stay None); with `attention_weights` they keep the attention weight of every
@@ -267,6 +279,79 @@ class PagedCache:
             self.thinned.discard(seq_id)
         return n
 
+    # ---- blocks of several sequences -------------------------------------------------------------------------------
+    def _block_tensors(self) -> tuple:
+        """(tensors that have a place for every block, the dimension that it is along)."""
+        if self.pages is not None:
+            return [t for p in self.pages for t in (p.k, p.v, p.k_exp, p.v_exp, p.weight) if t is not None], 0
+        if self.k is None:
+            return [], 0
+        if isinstance(self.k, list):
+            return [t for k, v, (ok, ov) in zip(self.k, self.v, self._own) for t, o in ((k, ok), (v, ov)) if o and t is not None], 0
+        return [self.k, self.v], 1
+
+    def copy_blocks(self, src: list, dst: list) -> None:
+        """Blocks src[i] to blocks dst[i], in all layers with one launch (see ops.copy_blocks_)."""
+        tensors, dim = self._block_tensors()
+        copy_blocks_(tensors, src, dst, dim)
+
+    @property
+    def shared_blocks(self) -> int:
+        """Blocks that are in more than one table."""
+        return self._lib.rb_ba_num_shared(self._h)
+
+    def fork(self, parents: list, children: list, num_tokens: list) -> bool:
+        """New sequences children[i] that begin with the first num_tokens[i] cached tokens of sequences parents[i].  Full blocks are shared, a block that these tokens end in is
+        copied, and so is the recurrent state (which is the parent's now, whatever num_tokens).  A parent may have several children.  False (nothing changed) when out of blocks or
+        slots."""
+        if not len(parents) == len(children) == len(num_tokens) or len(set(children)) != len(children):
+            raise InvalidArgument("PagedCache.fork: a parent and a number of tokens for every child, and no child twice")
+        for p, c, n in zip(parents, children, num_tokens):
+            have = self._lib.rb_ba_table_len(self._h, p)
+            if have < 0 or n < 0 or n > have * self.block_size:
+                raise InvalidArgument(f"PagedCache.fork: no sequence {p} with blocks for {n} tokens")
+            if self._lib.rb_ba_table_len(self._h, c) >= 0 or c in parents:
+                raise InvalidArgument(f"PagedCache.fork: sequence {c} is there already")
+        if sum(n % self.block_size != 0 for n in num_tokens) > self.free_blocks or (self.num_slots and len(children) > self.free_slots):
+            return False
+        src, dst, of, to = [], [], C.c_int32(), C.c_int32()
+        for p, c, n in zip(parents, children, num_tokens):
+            code = self._lib.rb_ba_fork(self._h, p, c, n, C.addressof(of), C.addressof(to))
+            if code < 0:
+                raise RuntimeError(f"PagedCache.fork: the allocator refused sequence {c} ({code})")
+            if code:
+                src.append(of.value)
+                dst.append(to.value)
+            if p in self.thinned:
+                self.thinned.add(c)
+        self.copy_blocks(src, dst)
+        if self.num_slots:
+            copy_blocks_([t for d in self.state for t in d.values()], [self.state_slot(p) for p in parents], [self.state_slot(c) for c in children])
+        return True
+
+    def own(self, seq_id: int, first: int, n: int) -> None:
+        """Blocks of its own, with the same content, in place of shared ones among those of the sequence's tokens first .. first + n - 1, which are about to be written."""
+        if n < 1 or not self.shared_blocks:
+            return
+        room = (first + n - 1) // self.block_size - first // self.block_size + 1
+        src, dst = (C.c_int32 * room)(), (C.c_int32 * room)()
+        k = self._lib.rb_ba_own(self._h, seq_id, first, n, C.addressof(src), C.addressof(dst), room)
+        if k == -1:
+            raise IndexError(f"positions {first} to {first + n - 1} of sequence {seq_id} have no blocks")
+        if k < 0:
+            raise RuntimeError(f"no free blocks for sequence {seq_id}, which writes into blocks that others share")
+        self.copy_blocks(src[:k], dst[:k])
+
+    def compact(self) -> int:
+        """Moves what is in use to the first blocks, num_blocks - free_blocks of them, and returns how many blocks moved.  Sequences keep their ids and tokens; block numbers that a program
+        has read before (`block_table`, `slot`) are no longer theirs."""
+        src, dst = (C.c_int32 * self.num_blocks)(), (C.c_int32 * self.num_blocks)()
+        k = self._lib.rb_ba_compact(self._h, C.addressof(src), C.addressof(dst))
+        if k < 0:
+            raise MemoryError("PagedCache.compact")
+        self.copy_blocks(src[:k], dst[:k])
+        return k
+
     def evict(self, seq_ids: list, lens: list, keep: int, recent: int = 0, keep_first: int = 0) -> list:
         """Brings sequences of `lens` cached tokens down to `keep` (see ops.kv_evict_e4m3), every layer by its own tokens' attention weights,
         and gives back the blocks behind their tokens, those that hold none yet among them.  Returns the new lengths; the sequences' positions do not
@@ -283,6 +368,8 @@ class PagedCache:
                 raise InvalidArgument(f"PagedCache.evict: sequence {s} has no blocks for {n} tokens")
         if not seq_ids:
             return []
+        for s, n in zip(seq_ids, lens):
+            self.own(s, 0, n)
         host = torch.empty((len(seq_ids), max(len(t) for t in tables)), dtype=torch.int32)
         self.fill_tables(seq_ids, host)
         device = self.pages[0].k.device
@@ -355,6 +442,10 @@ class BatchedCache:
     @property
     def len(self) -> int:
         return self.layers[0].len
+
+    def reorder(self, index: torch.Tensor) -> None:
+        """`KVCache.reorder` of all layers at once."""
+        reorder_rows_([t for l in self.layers for t in l._filled()], index)
 
     def reset(self) -> None:
         for l in self.layers:

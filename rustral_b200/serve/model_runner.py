@@ -19,6 +19,7 @@ import torch
 from .. import ops
 from ..models.registry import architecture, build_weights
 from ..ops import attention as attn_ops
+from ..ops import beams as beam_ops
 from ..ops import latent as latent_ops
 from ..ops import paged as paged_ops
 from ..ops import paged_e4m3 as e4m3_ops
@@ -40,9 +41,11 @@ class StepBatch:
     `segments`: the same sequences for layers with recurrent state (None: the model has none).  `arrived`: given for a step of decoded
     sequences only whose tables and lengths were complete before it began (see ops.paged.attention_step); positions and slots (None) then
     follow from them where a layer asks.  `cached`: cache slots of all positions of the portions that do not begin at 0 (index -> int64 tensor
-    on the device), where they came with the step's other inputs.  `moved`: the decoded rows' positions are not their lengths less one."""
+    on the device), where they came with the step's other inputs.  `moved`: the decoded rows' positions are not their lengths less one.  `shared`: (ops.PrefixGroups, int32 lengths) of
+    the decoded rows, whose sequences share their first tokens."""
 
-    def __init__(self, ids, pos, slots, spans, rd, tables, bt, ctx, block_size, segments=None, arrived=None, cached=None, moved=False):
+    def __init__(self, ids, pos, slots, spans, rd, tables, bt, ctx, block_size, segments=None, arrived=None, cached=None, moved=False, shared=None):
+        self.shared = shared
         self.moved, self._packed, self._groups = moved, None, None
         self.ids, self._pos, self._slots, self.arrived = ids, pos, slots, arrived      # int64 device tensors, one entry per row
         self.spans = spans                                        # (first row, end row, first position) per portion
@@ -273,7 +276,9 @@ class ModelRunner:
                                           head_gate=None if head_gate is None else head_gate[r0:r1])
         if parts:
             attn_ops.prompt_attention_many(parts, scale)
-        if sb.rd < T:
+        if sb.rd < T and sb.shared is not None and rule is None and gate is None and head_gate is None and dk == dv and beam_ops.shared_supported(q, kc, vc):
+            beam_ops.paged_attention_shared(q[sb.rd:], kc, vc, *sb.shared, sb.bt, sb.ctx, scale, out=a[sb.rd:])
+        elif sb.rd < T:
             paged_ops.paged_attention_decode(q[sb.rd:], kc, vc, sb.bt, sb.ctx, scale, out=a[sb.rd:], rule=rule,
                                              gate=None if gate is None else gate[sb.rd:],
                                              head_gate=None if head_gate is None else head_gate[sb.rd:])
@@ -399,6 +404,11 @@ class ModelRunner:
             want.append([r1 - 1] if c[3] is True else [r0 + i for i in c[3]] if c[3] else [])
         rows = [r for w in want for r in w] + list(range(rd, T))
         every_row = rows == list(range(T))
+        if self.cache.shared_blocks:
+            for s_, tokens, start, _ in chunks:
+                self.cache.own(s_, start, len(tokens))
+            for s_, n in zip(dec_ids, dec_len):
+                self.cache.own(s_, n - 1, 1)
         # All inputs of the step in one page-locked block and one copy: a copy from other memory waits until the stream has come to it, and
         # the host then forms the step's launches while the GPU has nothing to do.  token ids, positions, slots; rows of the logits; slots of
         # the cached positions of later portions (their positions, not copied, at the end); block tables and lengths
@@ -486,22 +496,33 @@ class ModelRunner:
         """Zeros that the steps of one stream share (see ops.paged.attention_step)."""
         return torch.zeros(batch * self.n_kv_head, dtype=torch.int32, device=self.device)
 
-    def _decode_body(self, ids, ctx, bt, segments=None, arrived=None, pos=None):
+    def _decode_body(self, ids, ctx, bt, segments=None, arrived=None, pos=None, shared=None):
         """The device-side part of a decode step on static tensors (captured into a CUDA graph per batch size)."""
-        return self._run(StepBatch(ids, pos, None, [], 0, [], bt, ctx, self.block_size, segments, arrived, moved=pos is not None), None)
+        return self._run(StepBatch(ids, pos, None, [], 0, [], bt, ctx, self.block_size, segments, arrived, moved=pos is not None, shared=shared), None)
 
     @torch.no_grad()
-    def decode(self, seq_ids: list, last_tokens: list, context_lens: list, positions: list | None = None) -> torch.Tensor:
+    def decode(self, seq_ids: list, last_tokens: list, context_lens: list, positions: list | None = None, groups=None,
+               shared_lens: list | None = None) -> torch.Tensor:
         """One new token per sequence.  context_lens[i] counts the tokens in the cache AFTER this token is appended.  `positions`: the tokens'
-        positions, where tokens have left the cache (a cache in e4m3; otherwise they are the lengths less one).
+        positions, where tokens have left the cache (a cache in e4m3; otherwise they are the lengths less one).  `groups` (ops.PrefixGroups of these sequences) and
+        `shared_lens`: the first shared_lens[i] cached tokens of group i's sequences are the same (see PagedCache.fork); where that saves enough (ops.beams.shared_pays) they are
+        read once for the whole group.  Caches in e4m3 and layers with rules of their own read every sequence's.
         Returns logits [batch, vocab_padded] (with CUDA graphs: valid until the next decode call)."""
         dev = self.device
         if positions is not None or self.cache.thinned:
             if positions is not None and len(positions) != len(seq_ids):
                 raise ValueError(f"{len(positions)} positions for {len(seq_ids)} sequences")
             self._check_positions(seq_ids, None if positions is None else dict(zip(seq_ids, positions)), [1] * len(seq_ids))
+        if groups is not None:
+            if groups.batch != len(seq_ids) or shared_lens is None or len(shared_lens) != len(groups):
+                raise ValueError(f"groups of {groups.batch} sequences with a shared length each are needed for {len(seq_ids)} sequences")
+            if self.cache.pages is not None or (dev.type == "cuda" and not beam_ops.shared_pays(groups, shared_lens, self._shared_row)):
+                groups = None
+        if self.cache.shared_blocks:
+            for s, n in zip(seq_ids, context_lens):
+                self.cache.own(s, n - 1, 1)
         if self.use_graphs and dev.type == "cuda":
-            return self._decode_graphed(seq_ids, last_tokens, context_lens, positions)
+            return self._decode_graphed(seq_ids, last_tokens, context_lens, positions, groups, shared_lens)
         ids = torch.tensor(last_tokens, dtype=torch.int64, device=dev)
         ctx = torch.tensor(context_lens, dtype=torch.int32, device=dev)
         max_blocks = max(len(self.cache.block_table(s)) for s in seq_ids)
@@ -509,9 +530,10 @@ class ModelRunner:
         self.cache.fill_tables(seq_ids, bt)
         bt = bt.to(dev)
         seg = Segments.of(self._decode_segments(seq_ids, context_lens), dev) if self.recurrent else None
-        one = self._attends_in_one_launch(context_lens, max_blocks)
+        one = groups is None and self._attends_in_one_launch(context_lens, max_blocks)
         pos = None if positions is None else torch.tensor(positions, dtype=torch.int64, device=dev)
-        return self._decode_body(ids, ctx, bt, seg, self._step_counters(len(seq_ids)) if one else None, pos)
+        shared = None if groups is None else (groups, torch.tensor(shared_lens, dtype=torch.int32, device=dev))
+        return self._decode_body(ids, ctx, bt, seg, self._step_counters(len(seq_ids)) if one else None, pos, shared)
 
     def _table_width(self, context_lens) -> int:
         """Block-table columns of a graphed decode step: the model's whole context when that is at most 1024 blocks, else
@@ -522,36 +544,47 @@ class ModelRunner:
         need = (max(context_lens) + self.block_size - 1) // self.block_size
         return min(full, max(64, 1 << (need - 1).bit_length()))
 
-    @staticmethod
-    def _step_views(buf: torch.Tensor, B: int, width: int, moved: bool = False) -> dict:
-        at = 16 * B if moved else 8 * B
-        return {"ids": buf[:8 * B].view(torch.int64), "pos": buf[8 * B:16 * B].view(torch.int64) if moved else None,
-                "ctx": buf[at:at + 4 * B].view(torch.int32), "bt": buf[at + 4 * B:].view(torch.int32).view(B, width)}
+    @property
+    def _shared_row(self) -> int:
+        """Bytes of a cached token's keys and values in a layer that has most of them."""
+        k = self.cache.k
+        return 0 if k is None else max(t.shape[-1] * t.shape[-2] * t.element_size() * 2 for t in (k if isinstance(k, list) else [k]) if t is not None)
 
-    def _decode_graphed(self, seq_ids, last_tokens, context_lens, positions=None) -> torch.Tensor:
+    @staticmethod
+    def _step_views(buf: torch.Tensor, B: int, width: int, moved: bool = False, groups: int = 0) -> dict:
+        at, end = 16 * B if moved else 8 * B, buf.numel() - 4 * groups
+        return {"ids": buf[:8 * B].view(torch.int64), "pos": buf[8 * B:16 * B].view(torch.int64) if moved else None,
+                "ctx": buf[at:at + 4 * B].view(torch.int32), "bt": buf[at + 4 * B:end].view(torch.int32).view(B, width), "shared": buf[end:].view(torch.int32)}
+
+    def _decode_graphed(self, seq_ids, last_tokens, context_lens, positions=None, groups=None, shared_lens=None) -> torch.Tensor:
         """Replays one captured CUDA graph per batch size, table width and form of the attention: the 10 to 20 launches per layer of a decode step are
         launch-bound from Python, the graph submits them in one call.  Inputs live in a static device buffer that
         one copy refreshes before each replay."""
         B = len(seq_ids)
         dev = self.device
         width = self._table_width(context_lens)
-        one, moved = self._attends_in_one_launch(context_lens, width), positions is not None
-        g = self._graphs.get((B, width, one, moved))
+        one, moved = groups is None and self._attends_in_one_launch(context_lens, width), positions is not None
+        key = (B, width, one, moved, None if groups is None else groups.sizes)
+        g = self._graphs.get(key)
         if g is None:
-            # ids and, where they are given, positions (int64), context lengths and block tables (int32) behind one another: one copy refreshes all
-            buf = torch.zeros((20 if moved else 12) * B + 4 * B * width, dtype=torch.uint8, device=dev)
-            g = {"buf": buf, "seg": None, "graph": None, "out": None, "arrived": self._step_counters(B) if one else None,
-                 **self._step_views(buf, B, width, moved)}
+            # ids and, where they are given, positions (int64), context lengths, block tables and shared lengths (int32) behind one another: one copy refreshes all
+            n_groups = 0 if groups is None else len(groups)
+            buf = torch.zeros((20 if moved else 12) * B + 4 * B * width + 4 * n_groups, dtype=torch.uint8, device=dev)
+            g = {"buf": buf, "seg": None, "graph": None, "out": None, "arrived": self._step_counters(B) if one else None, "n_groups": n_groups,
+                 **self._step_views(buf, B, width, moved, n_groups)}
+            g["groups"] = None if groups is None else (groups, g["shared"])
             if self.recurrent:
                 g["seg"] = Segments(torch.zeros((B, 4), dtype=torch.int32, device=dev), None)
-            self._graphs[(B, width, one, moved)] = g
+            self._graphs[key] = g
         memory, copied = self._memory.take(g["buf"].numel())
         host = memory[:g["buf"].numel()]
-        view = self._step_views(host, B, width, moved)
+        view = self._step_views(host, B, width, moved, g["n_groups"])
         view["ids"].numpy()[:] = last_tokens
         if moved:
             view["pos"].numpy()[:] = positions
         view["ctx"].numpy()[:] = context_lens
+        if groups is not None:
+            view["shared"].numpy()[:] = shared_lens
         self.cache.fill_tables(seq_ids, view["bt"])
         g["buf"].copy_(host, non_blocking=True)
         self._memory.give(memory, copied)
@@ -559,7 +592,7 @@ class ModelRunner:
             g["seg"].table.copy_(torch.tensor(self._decode_segments(seq_ids, context_lens), dtype=torch.int32), non_blocking=True)
         if g["graph"] is None:
             # first use of this batch size: one eager run (lazy kernel configuration, tensor-map cache), then capture
-            out = self._decode_body(g["ids"], g["ctx"], g["bt"], g["seg"], g["arrived"], g["pos"])
+            out = self._decode_body(g["ids"], g["ctx"], g["bt"], g["seg"], g["arrived"], g["pos"], g["groups"])
             torch.cuda.current_stream().synchronize()
             graph = torch.cuda.CUDAGraph()
             # A collection in the middle of a capture could destroy an earlier runner's graphs, which ends the capture with an error
@@ -567,7 +600,7 @@ class ModelRunner:
             gc.disable()
             try:
                 with torch.cuda.graph(graph):
-                    g["out"] = self._decode_body(g["ids"], g["ctx"], g["bt"], g["seg"], g["arrived"], g["pos"])
+                    g["out"] = self._decode_body(g["ids"], g["ctx"], g["bt"], g["seg"], g["arrived"], g["pos"], g["groups"])
             finally:
                 if collecting:
                     gc.enable()
