@@ -275,7 +275,10 @@ def shared_pays(groups: PrefixGroups, shared_lens, row_bytes: int) -> bool:
     return row_bytes * sum((n - 1) * p for n, p in zip(groups.sizes, shared_lens)) >= SHARED_PAYS
 
 
-SHARED_PAYS = 32 << 20
+# Bytes that are not read again.  One B200, attention of a layer, us, every sequence's own reading / one for the group: 4 beams over 300 tokens (12 KV heads of 64; 3 MB) 7.6 / 11.3,
+# 4 over 1000 (8 KV heads of 128; 12 MB) 11.1 / 14.9, 8 over 1000 (29 MB) 12.5 / 20.6, 4 over 4000 (49 MB) 21.4 / 17.6, 16 over 1000 (61 MB) 21.3 / 22.4, 2 over 16000
+# (66 MB) 43.9 / 23.1, 8 over 4000 (115 MB) 38.1 / 25.5, 32 over 2000 (254 MB) 60.0 / 26.4.
+SHARED_PAYS = 48 << 20
 
 
 def paged_attention_shared(q, k_cache, v_cache, groups: PrefixGroups, shared_lens, block_tables, context_lens, scale=None, out=None):
