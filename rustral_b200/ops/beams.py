@@ -59,15 +59,17 @@ def beam_select(logits, scores, count: int, ended=None, end_token: int = 0):
     then the lowest token.  Sums are compared in 64 bits and rounded once.  Minus infinity is a token that is not allowed (or a beam that is not there), and NaN
     counts as that; plus infinity counts as the largest fp32 number.  Fewer continuations than `count`: the remaining places have minus infinity and the group's first
     (row, token) pairs that are not among the continuations.  On a GPU: up to 256 beams and a count of up to 128."""
-    if logits.dim() != 2 or scores.dim() != 2 or logits.dtype not in _TYPES or scores.dtype is not torch.float32 or not scores.is_contiguous():
+    # (Every look at a tensor counts in a small call: attributes are read once.)
+    shape, each, kind = logits.shape, scores.shape, _TYPES.get(logits.dtype)
+    if len(shape) != 2 or len(each) != 2 or kind is None or scores.dtype is not torch.float32 or not scores.is_contiguous():
         raise TypeError("beam_select: logits [groups * beams, vocab] in bf16, fp16 or fp32 and contiguous fp32 scores [groups, beams] are required")
-    (rows, vocab), (groups, beams) = logits.shape, scores.shape
+    (rows, vocab), (groups, beams) = shape, each
     if rows != groups * beams or beams < 1 or vocab < 1:
         raise ValueError(f"beam_select: {rows} rows of {vocab} logits for {groups} groups of {beams} beams")
     if not 1 <= count <= beams * vocab:
         raise ValueError(f"beam_select: {count} of {beams} x {vocab} continuations")
     if ended is not None:
-        if ended.dtype is not torch.bool or ended.shape != scores.shape or not ended.is_contiguous():
+        if ended.dtype is not torch.bool or ended.shape != each or not ended.is_contiguous():
             raise TypeError("beam_select: ended is a contiguous bool tensor of the scores' shape")
         if not 0 <= end_token < vocab:
             raise ValueError(f"beam_select: no token {end_token} in a vocabulary of {vocab}")
@@ -77,17 +79,17 @@ def beam_select(logits, scores, count: int, ended=None, end_token: int = 0):
         return _select_cpu(logits, scores, count, ended, end_token)
     if beams > MOST_BEAMS or count > MOST_COUNT or vocab > 1 << 26:
         raise ValueError(f"beam_select: up to {MOST_BEAMS} beams, a count of up to {MOST_COUNT} and 2^26 tokens are served")
-    if logits.stride(1) != 1 or logits.stride(0) < vocab:
-        logits = logits.contiguous()
-    out_scores = torch.empty((groups, count), dtype=torch.float32, device=logits.device)
-    out = torch.empty((2, groups, count), dtype=torch.int64, device=logits.device)
-    kind = _TYPES[logits.dtype]
-    scratch = torch.empty(_select_bytes(groups, beams, vocab, count, kind), dtype=torch.uint8, device=logits.device)
-    at = out.data_ptr()
+    pitch, step = logits.stride()
+    if step != 1 or pitch < vocab:
+        logits, pitch = logits.contiguous(), vocab
+    out_scores = scores.new_empty((groups, count))
+    out_rows = scores.new_empty((groups, count), dtype=torch.int64)
+    out_tokens = torch.empty_like(out_rows)
+    scratch = scores.new_empty(_select_bytes(groups, beams, vocab, count, kind), dtype=torch.uint8)
     N.check(N.kernels().rb_beam_select(
-        _SELECT.pack(logits.data_ptr(), scores.data_ptr(), 0 if ended is None else ended.data_ptr(), out_scores.data_ptr(), at, at + 8 * groups * count,
-                     scratch.data_ptr(), logits.stride(0), groups, beams, vocab, count, kind, end_token), N.stream_ptr()), "rb_beam_select")
-    return out_scores, out[0], out[1]
+        _SELECT.pack(logits.data_ptr(), scores.data_ptr(), 0 if ended is None else ended.data_ptr(), out_scores.data_ptr(), out_rows.data_ptr(), out_tokens.data_ptr(),
+                     scratch.data_ptr(), pitch, groups, beams, vocab, count, kind, end_token), N.stream_ptr()), "rb_beam_select")
+    return out_scores, out_rows, out_tokens
 
 
 def _clean(x):
@@ -148,19 +150,19 @@ def _row(what: str, t, dim: int) -> tuple:
 
 def _rows(what: str, tensors, dim: int) -> tuple:
     """(device, rows, packed descriptions, how many) of the tensors of a call; those without elements are left out."""
-    dev, rows, packed, seen = None, None, [], set()
+    dev = rows = None
+    packed, seen = [], set()
     for t in tensors:
-        d, at = t.get_device(), t.data_ptr()
+        d = t.get_device()
+        n, *lies = _row(what, t, dim)
         if dev is None:
-            dev = d
+            dev, rows = d, n
         elif dev != d:
             raise ValueError(f"{what}: tensors on different devices")
-        n, *lies = _row(what, t, dim)
-        if rows is None:
-            rows = n
         elif rows != n:
             raise ValueError(f"{what}: tensors of {rows} and of {n} rows")
-        if t.numel():
+        if n and lies[3] and lies[4]:
+            at = t.data_ptr()
             if at in seen:
                 raise ValueError(f"{what}: tensors that share memory")
             seen.add(at)
@@ -252,6 +254,7 @@ class PrefixGroups:
         span_of = [x for g, n in enumerate(self.sizes) for x in (starts[g], starts[g + 1]) * n]
         both = torch.tensor(span_of + [g for g, n in enumerate(self.sizes) for _ in range(n)], dtype=torch.int32).to(device)
         self.span_of, self.group_of = both[:2 * self.batch], both[2 * self.batch:]
+        self.at = (self.group_of.data_ptr(), self.span_of.data_ptr())
 
     def __len__(self) -> int:
         return len(self.sizes)
@@ -278,7 +281,7 @@ def shared_pays(groups: PrefixGroups, shared_lens, row_bytes: int) -> bool:
 # Bytes that are not read again.  One B200, attention of a layer, us, every sequence's own reading / one for the group: 4 beams over 300 tokens (12 KV heads of 64; 3 MB) 7.6 / 11.3,
 # 4 over 1000 (8 KV heads of 128; 12 MB) 11.1 / 14.9, 8 over 1000 (29 MB) 12.5 / 20.6, 4 over 4000 (49 MB) 21.4 / 17.6, 16 over 1000 (61 MB) 21.3 / 22.4, 2 over 16000
 # (66 MB) 43.9 / 23.1, 8 over 4000 (115 MB) 38.1 / 25.5, 32 over 2000 (254 MB) 60.0 / 26.4.
-SHARED_PAYS = 48 << 20
+SHARED_PAYS = 48_000_000
 
 
 def paged_attention_shared(q, k_cache, v_cache, groups: PrefixGroups, shared_lens, block_tables, context_lens, scale=None, out=None):
@@ -290,19 +293,20 @@ def paged_attention_shared(q, k_cache, v_cache, groups: PrefixGroups, shared_len
 
     On a GPU: bf16 or fp16, heads of 64 or 128, up to 4096 sequences.  A sequence's result depends, within rounding, on the batch it is in; the same call gives the
     same bits."""
-    if q.dim() != 2 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or not q.dtype is k_cache.dtype is v_cache.dtype or \
-            not k_cache.is_contiguous() or not v_cache.is_contiguous():
+    qs, ks, dtype = q.shape, k_cache.shape, q.dtype
+    if len(qs) != 2 or len(ks) != 4 or ks != v_cache.shape or not dtype is k_cache.dtype is v_cache.dtype or not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise TypeError("paged_attention_shared: q [batch, heads * head_dim] and contiguous caches [blocks, block_size, kv_heads, head_dim] of its type are required")
-    nb, bs, hk, d = k_cache.shape
-    batch, width = q.shape
-    heads = width // d
+    nb, bs, hk, d = ks
+    batch, width = qs
+    heads, n_groups = width // d, len(groups.sizes)
     if batch != groups.batch or width != heads * d or heads % hk or heads == 0:
-        raise ValueError(f"paged_attention_shared: q of {tuple(q.shape)} for {groups.batch} sequences and {hk} KV heads of {d}")
-    if not (block_tables.dtype is context_lens.dtype is shared_lens.dtype is torch.int32 and block_tables.dim() == 2 and block_tables.is_contiguous() and
+        raise ValueError(f"paged_attention_shared: q of {tuple(qs)} for {groups.batch} sequences and {hk} KV heads of {d}")
+    table = block_tables.shape
+    if not (block_tables.dtype is context_lens.dtype is shared_lens.dtype is torch.int32 and len(table) == 2 and block_tables.is_contiguous() and
             context_lens.is_contiguous() and shared_lens.is_contiguous()) or \
-            not (block_tables.shape[0] == batch and context_lens.shape == (batch,) and shared_lens.shape == (len(groups),)):
+            not (table[0] == batch and context_lens.shape == (batch,) and shared_lens.shape == (n_groups,)):
         raise TypeError("paged_attention_shared: contiguous int32 tables and lengths of every sequence and shared lengths of every group are required")
-    if out is not None and (out.dtype is not q.dtype or out.shape != q.shape):
+    if out is not None and (out.dtype is not dtype or out.shape != qs):
         raise TypeError("paged_attention_shared: out has the shape and type of q")
     dev = q.get_device()
     _here("paged_attention_shared", dev, k_cache, v_cache, groups.group_of, shared_lens, block_tables, context_lens, out)
@@ -310,23 +314,24 @@ def paged_attention_shared(q, k_cache, v_cache, groups: PrefixGroups, shared_len
     if dev < 0:
         r = _shared_cpu(q, k_cache, v_cache, groups, shared_lens, block_tables, context_lens, scale)
         return r if out is None else out.copy_(r)
-    kind = _TYPES[q.dtype]
+    kind = _TYPES.get(dtype, 3)
     if kind > 1 or d not in (64, 128) or batch > MOST_SEQUENCES:
-        raise ValueError(f"paged_attention_shared: bf16 or fp16, heads of 64 or 128 and up to {MOST_SEQUENCES} sequences are served, not {q.dtype}, {d} and {batch}")
-    if batch == 0 or block_tables.shape[1] == 0 or nb == 0 or bs == 0:
+        raise ValueError(f"paged_attention_shared: bf16 or fp16, heads of 64 or 128 and up to {MOST_SEQUENCES} sequences are served, not {dtype}, {d} and {batch}")
+    if batch == 0 or table[1] == 0 or nb == 0 or bs == 0:
         return torch.zeros_like(q) if out is None else out.zero_()
-    if nb * bs > 2 ** 31 - 1 or block_tables.shape[1] * bs > 1 << 30:
+    if nb * bs > 2 ** 31 - 1 or table[1] * bs > 1 << 30:
         raise ValueError("paged_attention_shared: caches of fewer than 2^31 tokens and tables of up to 2^30 are served")
-    if q.stride(1) != 1 or q.stride(0) & 7 or q.data_ptr() & 15:
+    at, (pitch, step) = q.data_ptr(), q.stride()
+    if step != 1 or pitch & 7 or at & 15:
         q = q.clone(memory_format=torch.contiguous_format)
+        at, pitch = q.data_ptr(), width
     res = out
     if out is None or out.stride(1) != 1 or out.stride(0) & 7 or out.data_ptr() & 15:
-        res = torch.empty((batch, width), dtype=q.dtype, device=q.device)
-    scratch = torch.empty(_shared_bytes(batch, len(groups), heads, hk, d, bs, groups.most), dtype=torch.uint8, device=q.device)
+        res = q.new_empty((batch, width))
+    scratch = q.new_empty(_shared_bytes(batch, n_groups, heads, hk, d, bs, groups.most), dtype=torch.uint8)
     N.check(N.kernels().rb_shared_prefix(
-        _SHARED.pack(q.data_ptr(), res.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), shared_lens.data_ptr(),
-                     groups.group_of.data_ptr(), groups.span_of.data_ptr(), scratch.data_ptr(), q.stride(0), res.stride(0), nb,
-                     batch, len(groups), block_tables.shape[1], bs, heads, hk, d, kind, groups.most, scale), N.stream_ptr()), "rb_shared_prefix")
+        _SHARED.pack(at, res.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), shared_lens.data_ptr(), groups.at[0], groups.at[1],
+                     scratch.data_ptr(), pitch, res.stride(0), nb, batch, n_groups, table[1], bs, heads, hk, d, kind, groups.most, scale), N.stream_ptr()), "rb_shared_prefix")
     return res if out is None or res is out else out.copy_(res)
 
 
