@@ -43,8 +43,21 @@ struct SpSmem {
 template <int D>
 __device__ __forceinline__ uint32_t sp_piece(int r, int c) { return (r * (D / 8) + (c ^ (r & 7))) * 16; }
 
+// A unit of a run: where it is in the list of its virtual KV head.
+struct SpUnit {
+  int vh, at, e;
+};
+__device__ __forceinline__ void sp_advance(const SpList& l, const SpHeld& held, SpUnit& c) {
+  if (++c.at == held.totals[l.entries]) {
+    c.at = c.e = 0;
+    ++c.vh;
+  }
+  while (held.totals[c.e + 1] <= c.at) ++c.e;
+}
+
 // The copies go on from one part to the next: the next unit's keys, whichever part they are of, are asked for as soon as this unit's scores are formed, its values behind this unit's
-// product.  The warps' sums are joined in the memory of their V tiles (two m-tiles: of K and V, and the next part's keys are asked for behind the join).
+// product, and its places in the cache are looked up a unit earlier (looked up when they were needed they took 4300 of a unit's 7000 cycles).  The warps' sums are joined in the memory of
+// their V tiles (two m-tiles: of K and V, and the next part's keys are asked for behind the join).
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kSpWarps * 32, MT == 1 ? 3 : 2)
 shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
@@ -63,70 +76,93 @@ shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
   const SpList& list = p.list;
   const SpHeld held = sp_held(list, reinterpret_cast<int*>(sp_mem + L::kHeld));
   sp_prepare(p, list, held, warp_sums);
-  const int total = held.totals[list.entries] * list.virtual_heads, group = p.heads / p.kv_heads;
-  int u = sp_run(total, list.ctas, blockIdx.x);
-  const int u_end = sp_run(total, list.ctas, blockIdx.x + 1);
-  if (u >= u_end) return;
+  const int all = held.totals[list.entries], total = all * list.virtual_heads, group = p.heads / p.kv_heads;
+  const int u_begin = sp_run(total, list.ctas, blockIdx.x);
+  int left = sp_run(total, list.ctas, blockIdx.x + 1) - u_begin;        // units of the run from this one on
+  if (left <= 0) return;
   const T* K = static_cast<const T*>(p.k);
   const T* V = static_cast<const T*>(p.v);
   const float scale2 = p.scale * kSpLog2e;
 
-  SpPart s_ = sp_next(p, list, held, u, u_end);
-  int unit = s_.u0;
+  SpUnit c0;                                     // this unit
+  c0.vh = u_begin / all;
+  c0.at = u_begin - c0.vh * all;
+  c0.e = 0;
+  for (int hi = list.entries; hi - c0.e > 1;) {  // the last entry that begins at or in front of it
+    const int mid = (c0.e + hi) >> 1;
+    if (held.totals[mid] <= c0.at) c0.e = mid;
+    else hi = mid;
+  }
+  auto rows_of = [&](int e) {
+    if (e >= list.own) return list.per;
+    return min(list.seqs, static_cast<int>(held.span[e] >> 16) - e) * list.per;
+  };
   // ---- rows of queries: loaded into registers, stored when the last part's have been read
   uint4 q_next[kQPieces];
-  auto load_q = [&](const SpPart& s) {
-    const int hk = s.vh / list.parts, head0 = (s.vh - hk * list.parts) * list.per, real = min(list.per, group - head0), rows = s.n * list.per;
+  auto load_q = [&](const SpUnit& c) {
+    const int hk = c.vh / list.parts, head0 = (c.vh - hk * list.parts) * list.per, real = min(list.per, group - head0), rows = rows_of(c.e);
+    const int b = c.e >= list.own ? c.e - list.own : c.e;
 #pragma unroll
     for (int i = 0; i < kQPieces; ++i) {
-      const int at = i * kSpWarps * 32 + tid, r = at / LP, c = at - r * LP, seq = r / list.per, h = r - seq * list.per;
+      const int at = i * kSpWarps * 32 + tid, r = at / LP, piece = at - r * LP, seq = r / list.per, h = r - seq * list.per;
       q_next[i] = make_uint4(0u, 0u, 0u, 0u);
       if (r < rows && h < real)
-        q_next[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (s.b + seq) * p.ld_q + static_cast<long long>(hk * group + head0 + h) * D + c * 8);
+        q_next[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (b + seq) * p.ld_q + static_cast<long long>(hk * group + head0 + h) * D + piece * 8);
     }
   };
   auto store_q = [&]() {
 #pragma unroll
     for (int i = 0; i < kQPieces; ++i) {
-      const int at = i * kSpWarps * 32 + tid, r = at / LP, c = at - r * LP;
-      *reinterpret_cast<uint4*>(sp_mem + L::kQ + sp_piece<D>(r, c)) = q_next[i];
+      const int at = i * kSpWarps * 32 + tid, r = at / LP, piece = at - r * LP;
+      *reinterpret_cast<uint4*>(sp_mem + L::kQ + sp_piece<D>(r, piece)) = q_next[i];
     }
   };
-  // ---- keys and values of the located unit
-  int slot = 0, n_next = 0, hk_next = 0;
-  auto locate = [&](const SpPart& s, int of) {
-    const int first = s.own ? s.shared : 0, count = s.own ? sp_length(p, s.b) - s.shared : s.shared, at = of * kSpUnit + warp * 32;
-    hk_next = s.vh / list.parts;
-    n_next = min(32, count - at);
-    slot = -1;
-    if (lane < n_next) {
-      const int token = first + at + lane, page = token / p.block_size;
-      int blk = s.table[page];
+  // ---- places of a unit's keys and values: looked up, then asked for
+  struct Places {
+    int blk, off, n, hk;                         // of the lane's token: block and place in it; the warp's tokens (0 and less: none)
+  };
+  auto look_up = [&](const SpUnit& c) {
+    Places w;
+    const bool own = c.e >= list.own;
+    const int shared = held.shared[c.e], at = (c.at - held.totals[c.e]) * kSpUnit + warp * 32;
+    w.n = min(32, held.count[c.e] - at);
+    w.hk = c.vh / list.parts;
+    w.blk = w.off = 0;
+    if (lane < w.n) {
+      const int token = (own ? shared : 0) + at + lane, page = token / p.block_size;
+      w.off = token - page * p.block_size;
+      w.blk = p.tables[static_cast<long long>(own ? c.e - list.own : static_cast<int>(held.span[c.e] & 0xffffu)) * p.width + page];
+    }
+    return w;
+  };
+  auto request = [&](const T* cache, uint32_t tile, const Places& w) {
+    if (w.n > 0) {
+      int blk = w.blk;
       if (blk < 0 || blk >= p.num_blocks) {                            // corrupt tables read block 0 instead of faulting
         RB_BOUNDS_HIT(104);
         blk = 0;
       }
-      slot = blk * p.block_size + (token - page * p.block_size);       // the host bounds num_blocks * block_size below 2^31
-    }
-  };
-  auto request = [&](const T* cache, uint32_t tile) {
-    if (n_next > 0) {
+      const int slot = blk * p.block_size + w.off;                     // the host bounds num_blocks * block_size below 2^31
 #pragma unroll
       for (int i = 0; i < LP; ++i) {
-        const int idx = i * 32 + lane, r = idx / LP, c = idx - r * LP;
+        const int idx = i * 32 + lane, r = idx / LP, piece = idx - r * LP;
         const int s = __shfl_sync(0xffffffffu, slot, r);
-        wm_cp16(tile + sp_piece<D>(r, c), s >= 0 ? cache + (static_cast<long long>(s) * p.kv_heads + hk_next) * D + c * 8 : cache, s >= 0);
+        wm_cp16(tile + sp_piece<D>(r, piece), r < w.n ? cache + (static_cast<long long>(s) * p.kv_heads + w.hk) * D + piece * 8 : cache, r < w.n);
       }
     }
     wm_cp_commit();
   };
 
-  locate(s_, unit);
-  request(K, k_u32);
-  load_q(s_);
+  Places w0 = look_up(c0);
+  SpUnit c1 = c0;                                // the next unit, if there is one
+  if (left > 1) sp_advance(list, held, c1);
+  Places w1 = look_up(c1);
+  load_q(c0);
+  request(K, k_u32, w0);
+  request(V, v_u32, w0);
   store_q();
-  request(V, v_u32);
   __syncthreads();
+  bool begins = c0.at == held.totals[c0.e];      // this part begins its entry
   float m[MT][2], l[MT][2], acc[MT][NT][4];
   auto clear = [&]() {
 #pragma unroll
@@ -138,10 +174,9 @@ shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
     }
   };
   clear();
-  for (bool more = true; more;) {
-    const int n_tok = n_next, rows = s_.n * list.per;
-    const bool last = unit + 1 == s_.u1;
-    more = !last || u < u_end;
+  for (;; --left) {
+    const int n_tok = w0.n, rows = rows_of(c0.e);
+    const bool more = left > 1, last = !more || c1.e != c0.e || c1.vh != c0.vh;
     wm_cp_wait<1>();                             // this unit's K tile has landed (V may be on its way)
     __syncwarp();
     float s[MT][4][4];
@@ -169,20 +204,14 @@ shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
       }
     }
     __syncwarp();                                // every lane has read its K fragments
-    // ---- the next unit, of this part or the next
-    const SpPart now = s_;
-    if (!last) {
-      ++unit;
-    } else if (more) {
-      s_ = sp_next(p, list, held, u, u_end);
-      unit = s_.u0;
-    }
-    if (more) locate(s_, unit);
-    else n_next = 0;
-    const bool ahead = kAhead || !last;
-    if (ahead) request(K, k_u32);
+    // ---- the next unit's keys, and a look at the one behind it
+    if (!more) w1.n = 0;
+    if (kAhead || !last) request(K, k_u32, w1);
     else wm_cp_commit();
-    if (last && more) load_q(s_);
+    if (last && more) load_q(c1);
+    SpUnit c2 = c1;
+    if (left > 2) sp_advance(list, held, c2);
+    const Places w2 = look_up(c2);
     if (n_tok > 0) {
       uint32_t pf[MT][2][4];
 #pragma unroll
@@ -254,7 +283,7 @@ shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
         }
       }
       __syncthreads();
-      const long long row0 = sp_row(list, now.vh, now.e, blockIdx.x, now.u0 == 0);
+      const long long row0 = sp_row(list, c0.vh, c0.e, blockIdx.x, begins);
       for (int i = tid; i < rows * (D / 4); i += kSpWarps * 32) {
         const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
         float mx = -INFINITY;
@@ -276,11 +305,16 @@ shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
       if (!more) return;
       __syncthreads();                           // sums and queries have been read
       store_q();
-      if (!kAhead) request(K, k_u32);
+      if (!kAhead) request(K, k_u32, w1);
       __syncthreads();
       clear();
+      begins = true;                             // what follows in a run begins at its entry's first unit
     }
-    request(V, v_u32);
+    request(V, v_u32, w1);
+    c0 = c1;
+    w0 = w1;
+    c1 = c2;
+    w1 = w2;
   }
 }
 

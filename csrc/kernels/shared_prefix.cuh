@@ -42,14 +42,19 @@ struct SpParams {
 };
 
 __device__ __forceinline__ int sp_length(const SpParams& p, int b) { return min(max(p.lens[b], 0), p.cap); }
-// What a CTA's shared memory holds of a list: running totals of the entries' units, and of every entry its tokens and the first sequences of its group and of the next.
+// What a CTA's shared memory holds of a list: running totals of the entries' units, and of every entry its tokens, the tokens that its group shares and the first sequences of its group
+// and of the next.
 struct SpHeld {
   int* totals;                                   // [entries + 1]
-  int* tokens;                                   // [entries]; of an own entry: those in front of it, which are shared
+  int* count;                                    // [entries]
+  int* shared;                                   // [entries]
   uint32_t* span;                                // [entries]: two numbers of 16 bits
 };
-__host__ __device__ constexpr size_t sp_held_bytes(int entries, int groups) { return (3 * static_cast<size_t>(entries) + 1 + groups) * 4; }
-__device__ __forceinline__ SpHeld sp_held(const SpList& l, int* at) { return {at, at + l.entries + 1, reinterpret_cast<uint32_t*>(at + 2 * l.entries + 1)}; }
+__host__ __device__ constexpr size_t sp_held_bytes(int entries, int groups) { return (4 * static_cast<size_t>(entries) + 1 + groups) * 4; }
+__device__ __forceinline__ SpHeld sp_held(const SpList& l, int* at) {
+  const int n = l.entries;
+  return {at, at + n + 1, at + 2 * n + 1, reinterpret_cast<uint32_t*>(at + 3 * n + 1)};
+}
 // Forms them, all threads of a CTA.
 //
 // What a group's sequences read together are no more tokens than the shortest of them has, those without tokens aside, so that all rows of a tile see all of its tokens.  Tiles of rows
@@ -84,9 +89,10 @@ __device__ __forceinline__ void sp_prepare(const SpParams& p, const SpList& l, c
       const bool first = b == static_cast<int>(threadIdx.x);
       const int shared = least[first ? group0 : p.group_of[b]];
       const int2 span = first ? span0 : p.span_of[b];
-      held.tokens[e] = shared;
+      held.shared[e] = shared;
       held.span[e] = static_cast<uint32_t>(span.x) | static_cast<uint32_t>(span.y) << 16;
       const int count = own ? max(0, (first ? length0 : sp_length(p, b)) - shared) : (b - span.x) % l.seqs == 0 ? shared : 0;
+      held.count[e] = count;
       upto = (count + kSpUnit - 1) / kSpUnit;
     }
 #pragma unroll
@@ -143,7 +149,7 @@ __device__ __forceinline__ SpPart sp_next(const SpParams& p, const SpList& l, co
   s.u1 = min(held.totals[e + 1], at + u_end - u) - held.totals[e];
   s.own = e >= l.own;
   s.b = s.own ? e - l.own : e;
-  s.shared = held.tokens[e];
+  s.shared = held.shared[e];
   const uint32_t span = held.span[e];
   s.n = s.own ? 1 : min(l.seqs, static_cast<int>(span >> 16) - s.b);
   s.table = p.tables + static_cast<long long>(s.own ? s.b : static_cast<int>(span & 0xffffu)) * p.width;

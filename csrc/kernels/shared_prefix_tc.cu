@@ -25,7 +25,7 @@ namespace rb {
 constexpr int kStThreads = 384;          // warps 0-7 softmax, 8, 10 and 11 TMA, 9 MMA
 constexpr int kStTile = 128;
 constexpr float kStRescale = 8.f;        // log2 units
-constexpr int kStMostBatch = 1024;       // their totals, tokens and spans beside 192 KB of tiles
+constexpr int kStMostBatch = 768;        // their totals, tokens and spans beside 192 KB of tiles
 
 __device__ __forceinline__ void st_ld32(uint32_t taddr, uint32_t* r) { tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r)); }
 __device__ __forceinline__ void st_st32(uint32_t taddr, const uint32_t* r) {

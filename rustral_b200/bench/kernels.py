@@ -5,6 +5,8 @@
     python -m rustral_b200.bench.kernels attention --batch 32 --seq 1024 --heads 12 --head-dim 64 [--impl tc2|tc|mma] [--backward]
     python -m rustral_b200.bench.kernels norm --rows 32768 --n 768
     python -m rustral_b200.bench.kernels adam --numel 124000000
+    python -m rustral_b200.bench.kernels shared --groups 4 --sequences 8 --shared 4000 --own 100 [--every]
+    python -m rustral_b200.bench.kernels beams --groups 64 --beams 4 --vocab 128256 --count 8
     python -m rustral_b200.bench.kernels launch-overhead [--calls 5000]
 
 Timing: CUDA events around each call on the current stream, `--warmup` untimed calls first, a 256 MiB buffer is
@@ -192,6 +194,45 @@ def bench_paged(a):
                    "kv_cache": a.kv_cache, "weights": a.weights, "kv_cache_bytes": int(kv_bytes)})
 
 
+def bench_shared(a):
+    """Decode attention of `groups` groups of `sequences` sequences that share their first `shared` tokens and have `own` more each (ops.paged_attention_shared); `every`: the same
+    batch through decode attention that reads every sequence's tokens."""
+    import math
+    from .. import ops
+    from ..ops import paged
+    B, H, Hk, D, bs = a.groups * a.sequences, a.heads, a.kv_heads, a.head_dim, a.block_size
+    full, tail = a.shared // bs, (a.shared % bs + a.own + bs - 1) // bs
+    nb = a.groups * full + B * tail + 1
+    g = torch.Generator().manual_seed(0)
+    pages = torch.randperm(nb - 1, generator=g).to(torch.int32) + 1
+    bt = torch.empty((B, full + tail), dtype=torch.int32)
+    bt[:, :full] = pages[:a.groups * full].view(a.groups, full).repeat_interleave(a.sequences, 0)
+    bt[:, full:] = pages[a.groups * full:].view(B, tail)
+    kc, vc = (torch.randn((nb, bs, Hk, D), device="cuda").bfloat16() for _ in range(2))
+    bt, q = bt.cuda(), torch.randn(B, H * D, device="cuda").bfloat16()
+    ctx = torch.full((B,), a.shared + a.own, dtype=torch.int32, device="cuda")
+    shared = torch.full((a.groups,), a.shared, dtype=torch.int32, device="cuda")
+    plan, out, scale = ops.PrefixGroups([a.sequences] * a.groups, "cuda"), torch.empty_like(q), 1.0 / math.sqrt(D)
+    if a.every:
+        fn = lambda: paged.paged_attention_decode(q, kc, vc, bt, ctx, scale, out=out)
+    else:
+        fn = lambda: ops.paged_attention_shared(q, kc, vc, plan, shared, bt, ctx, scale, out=out)
+    ms = timed(fn, a.warmup, a.iters)
+    once = 4.0 * Hk * D * (a.groups * a.shared + B * a.own)
+    return report("shared_decode_attention", ms, 4.0 * B * H * D * (a.shared + a.own), once,
+                  {"groups": a.groups, "sequences": a.sequences, "shared": a.shared, "own": a.own, "heads": H, "kv_heads": Hk, "head_dim": D, "block_size": bs, "every": a.every})
+
+
+def bench_beams(a):
+    """Selection of `count` continuations for each of `groups` groups of beams (ops.beam_select)."""
+    from .. import ops
+    x = torch.empty((a.groups * a.beams, (a.vocab + 127) // 128 * 128), device="cuda").normal_(0.0, 2.5).to(getattr(torch, a.dtype))[:, :a.vocab]
+    scores = -20.0 - torch.rand((a.groups, a.beams), device="cuda")
+    ms = timed(lambda: ops.beam_select(x, scores, a.count), a.warmup, a.iters)
+    return report("beam_select", ms, 0, float(a.groups * a.beams * a.vocab * x.element_size()),
+                  {"groups": a.groups, "beams": a.beams, "vocab": a.vocab, "count": a.count, "dtype": a.dtype})
+
+
 def bench_launch_overhead(a):
     import time
 
@@ -274,10 +315,18 @@ def main(argv=None):
     pg.add_argument("--block-size", type=int, default=16)
     pg.add_argument("--kv-cache", default="bf16", choices=["bf16", "e4m3"])
     pg.add_argument("--weights", action="store_true", help="sum every cached token's attention weight (e4m3)")
+    sh = sub.add_parser("shared")
+    for name, default in (("groups", 4), ("sequences", 8), ("shared", 4000), ("own", 100), ("heads", 32), ("kv-heads", 8), ("head-dim", 128), ("block-size", 16)):
+        sh.add_argument("--" + name, type=int, default=default)
+    sh.add_argument("--every", action="store_true", help="read every sequence's tokens instead")
+    be = sub.add_parser("beams")
+    for name, default in (("groups", 64), ("beams", 4), ("vocab", 128256), ("count", 8)):
+        be.add_argument("--" + name, type=int, default=default)
+    be.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float16", "float32"])
     lo = sub.add_parser("launch-overhead")
     lo.add_argument("--calls", type=int, default=5000)
     a = ap.parse_args(argv)
-    return {"launch-overhead": bench_launch_overhead, "paged": bench_paged, "gemm": bench_gemm, "gemm-fp8": bench_gemm_fp8, "attention": bench_attention, "norm": bench_norm, "adam": bench_adam}[a.op](a)
+    return {"launch-overhead": bench_launch_overhead, "paged": bench_paged, "shared": bench_shared, "beams": bench_beams, "gemm": bench_gemm, "gemm-fp8": bench_gemm_fp8, "attention": bench_attention, "norm": bench_norm, "adam": bench_adam}[a.op](a)
 
 
 if __name__ == "__main__":
