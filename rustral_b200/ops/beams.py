@@ -58,7 +58,8 @@ def beam_select(logits, scores, count: int, ended=None, end_token: int = 0):
     Returns (scores fp32, rows int64, tokens int64), each [groups, count] in descending order of the scores; rows index `logits`.  Equal scores go to the lowest row,
     then the lowest token.  Sums are compared in 64 bits and rounded once.  Minus infinity is a token that is not allowed (or a beam that is not there), and NaN
     counts as that; plus infinity counts as the largest fp32 number.  Fewer continuations than `count`: the remaining places have minus infinity and the group's first
-    (row, token) pairs that are not among the continuations.  On a GPU: up to 256 beams and a count of up to 128."""
+    (row, token) pairs that are not among the continuations.  A row's logits are compared as they are: of two so close that their 64-bit sums are equal either
+    may come first.  A sum is as exact as its row's sum of exponentials, which is formed in 32 bits.  On a GPU: up to 256 beams and a count of up to 128."""
     # (Every look at a tensor counts in a small call: attributes are read once.)
     shape, each, kind = logits.shape, scores.shape, _TYPES.get(logits.dtype)
     if len(shape) != 2 or len(each) != 2 or kind is None or scores.dtype is not torch.float32 or not scores.is_contiguous():
@@ -145,13 +146,24 @@ def _row(what: str, t, dim: int) -> tuple:
         raise ValueError(f"{what}: the rows of a tensor of shape {tuple(shape)} and strides {tuple(stride)} are not pieces at equal distances")
     n, far = outer[0] if outer else (1, 0)
     segs, apart = inner[0] if inner else (1, 0)
+    end = piece
+    for length, apart_ in sorted([(n, far), (rows, stride[dim] if rows > 1 else 0), (segs, apart)], key=lambda x: x[1]):
+        if length > 1 and apart_ < end:
+            raise ValueError(f"{what}: the rows of a tensor of shape {tuple(shape)} and strides {tuple(stride)} share memory")
+        end += max(length - 1, 0) * apart_
     return rows, far * size, (stride[dim] if rows > 1 else 0) * size, apart * size, piece * size, n, segs
 
 
-def _rows(what: str, tensors, dim: int) -> tuple:
+def _listed(what: str, tensors) -> tuple:
+    if isinstance(tensors, torch.Tensor):
+        raise TypeError(f"{what}: a list of tensors is required")
+    return tuple(tensors)
+
+
+def _rows(what: str, tensors, dim: int, index=None) -> tuple:
     """(device, rows, packed descriptions, how many) of the tensors of a call; those without elements are left out."""
     dev = rows = None
-    packed, seen = [], set()
+    packed, seen = [], set() if index is None else {index.data_ptr()}
     for t in tensors:
         d = t.get_device()
         n, *lies = _row(what, t, dim)
@@ -176,6 +188,7 @@ def copy_blocks_(tensors, src, dst, dim: int = 0) -> None:
     """Copies blocks in place: t[dst[i]] <- t[src[i]] along dimension `dim` of every tensor (one number of blocks for all of them; other sizes, types and strides may
     differ).  src and dst are numbers on the host (lists or the like); the call refuses blocks that are not there, a destination twice, and a destination that is a source
     too, before it copies anything.  The tensors share no memory.  A CUDA graph keeps the numbers that it was captured with."""
+    tensors = _listed("copy_blocks_", tensors)
     try:
         src, dst = array("i", src), array("i", dst)
     except (TypeError, OverflowError) as e:
@@ -212,8 +225,9 @@ def reorder_rows_(tensors, index, dim: int = 0, group: int | None = None) -> Non
     """Rows in a new order, in place: t[i] <- what t[index[i]] was, along dimension `dim` of every tensor (one number of rows for all; other sizes, types and strides
     may differ).  index: int64 [rows] on the tensors' device, any map.  `group`: rows come in groups of that many, as the beams of several prompts do, and indices stay
     in their row's group (None: all rows are one); an index that does not leaves its row as it is.  On a GPU a group has up to 256 rows.  The tensors share no
-    memory."""
-    dev, rows, packed, count = _rows("reorder_rows_", tensors, dim)
+    memory, with the index neither."""
+    tensors = _listed("reorder_rows_", tensors)
+    dev, rows, packed, count = _rows("reorder_rows_", tensors, dim, index)
     if rows is None:
         return
     if index.dtype is not torch.int64 or index.dim() != 1 or not index.is_contiguous():

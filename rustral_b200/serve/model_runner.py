@@ -550,6 +550,8 @@ class ModelRunner:
         k = self.cache.k
         return 0 if k is None else max(t.shape[-1] * t.shape[-2] * t.element_size() * 2 for t in (k if isinstance(k, list) else [k]) if t is not None)
 
+    MOST_SHAPED = 32                                              # captured steps for batches in groups of certain sizes; the oldest makes room
+
     @staticmethod
     def _step_views(buf: torch.Tensor, B: int, width: int, moved: bool = False, groups: int = 0) -> dict:
         at, end = 16 * B if moved else 8 * B, buf.numel() - 4 * groups
@@ -567,6 +569,10 @@ class ModelRunner:
         key = (B, width, one, moved, None if groups is None else groups.sizes)
         g = self._graphs.get(key)
         if g is None:
+            shaped = [k for k in self._graphs if k[4] is not None]
+            if groups is not None and len(shaped) >= self.MOST_SHAPED:
+                torch.cuda.current_stream().synchronize()         # it may be running
+                del self._graphs[shaped[0]]
             # ids and, where they are given, positions (int64), context lengths, block tables and shared lengths (int32) behind one another: one copy refreshes all
             n_groups = 0 if groups is None else len(groups)
             buf = torch.zeros((20 if moved else 12) * B + 4 * B * width + 4 * n_groups, dtype=torch.uint8, device=dev)

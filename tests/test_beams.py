@@ -306,6 +306,28 @@ def test_reorder_rows_refuses(device):
     ops.reorder_rows_([torch.zeros(6, 0, device=device)], i)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_moves_refuse_memory_that_is_there_twice(device):
+    """One tensor in place of a list, rows that overlap, an index among the tensors; tensors may come from a generator."""
+    base, i = torch.arange(36.0, device=device), torch.tensor([1, 0, 2, 3, 4, 5], device=device)
+    rows = base[:30].view(6, 5)
+    for t in (base.as_strided((6, 8), (4, 1)), base.as_strided((2, 6, 3), (4, 4, 1)), base.as_strided((6, 2, 3), (4, 2, 1))):
+        with pytest.raises(ValueError):
+            ops.reorder_rows_([t], i, dim=1 if t.shape[0] == 2 else 0)
+        with pytest.raises(ValueError):
+            ops.copy_blocks_([t], [0], [1], dim=1 if t.shape[0] == 2 else 0)
+    with pytest.raises(ValueError):
+        ops.reorder_rows_([rows, i], i)
+    with pytest.raises(TypeError):
+        ops.reorder_rows_(base[:36].view(6, 6), i)
+    with pytest.raises(TypeError):
+        ops.copy_blocks_(base[:36].view(6, 6), [0], [1])
+    assert torch.equal(base.cpu(), torch.arange(36.0)) and i.tolist() == [1, 0, 2, 3, 4, 5]
+    ops.reorder_rows_((t for t in [rows]), i)
+    ops.copy_blocks_((t for t in [rows.t()]), [2], [4], dim=1)
+    assert rows[:, 0].tolist() == [5, 0, 10, 15, 10, 25]
+
+
 @pytest.mark.gpu
 def test_reorder_rows_refuses_what_the_kernel_does_not_serve():
     with pytest.raises(ValueError):
@@ -385,6 +407,8 @@ ATTENDED = [
     ([3], [700], [1, 100, 10], 16, 1, 40, 64, torch.bfloat16),        # more heads of a group than a tile has rows
     ([10], [260], [1] * 10, 16, 1, 71, 64, torch.bfloat16),
     ([300], [130], [2] * 300, 16, 1, 1, 64, torch.bfloat16),
+    ([1] * 4090 + [3, 3], [1] * 4090 + [140, 20], [1 + i % 3 for i in range(4096)], 16, 1, 2, 64, torch.bfloat16),    # as many sequences as there may be
+    ([2000, 2096], [40, 3], [1 + i % 3 for i in range(4096)], 16, 1, 1, 128, torch.float16),
 ]
 
 
