@@ -12,20 +12,28 @@
 // Tokens behind a group's shared ones lie in the same pages, or in none: the last unit's scores are masked, and the rows of its V tile behind the last
 // token are set to zero, since a weight of zero times what they hold need not be zero.
 //
+// The sequences' own tokens are read in the same launch by CTAs of their own, three runs of four warps each (shared_prefix_split.cuh): one part of the GPU is bound by products and
+// exponentials while the other waits for memory.  One after the other they took 145 us where it is 133 now (256 sequences with 4 rows each for 8 KV heads of 128, 16384 shared and 16 to 512 own
+// tokens), 73.5 and 71.7 for 12 groups of 8, 54.6 and 50.8 for one document of 32771 tokens and 16 sequences.  Every CTA finds from the lengths how many CTAs each kind gets.
+//
 // Bound by the softmax's exponentials and the products where there are 256 rows, by the keys' and values' bytes where there are few.
 #define RB_INLINE_WAITS                 // registers are reallocated between warp groups
 #include <string.h>
 
 #include <type_traits>
 
-#include "shared_prefix.cuh"
+#include "shared_prefix_split.cuh"
 
 namespace rb {
 
 constexpr int kStThreads = 384;          // warps 0-7 softmax, 8, 10 and 11 TMA, 9 MMA
 constexpr int kStTile = 128;
 constexpr float kStRescale = 8.f;        // log2 units
-constexpr int kStMostBatch = 768;        // their totals, tokens and spans beside 192 KB of tiles
+constexpr int kStMostBatch = 704;        // their totals, tokens and spans beside 192 KB of tiles
+constexpr int kStRuns = 3;               // of a CTA that has sequences' own tokens
+// What a unit of 128 tokens takes a CTA, relative to one another: with two tiles of rows, with one, and of a sequence's own.  The first case above takes 133 us with 5 : 3 : 2, 146 with
+// 6 : 3 : 2 and 143 with 4 : 3 : 2; the second 71.7, or 73.7 with 5 : 2 : 2 and 79 with 5 : 4 : 2.
+constexpr int kStTwo = 5, kStOne = 3, kStOwn = 2;
 
 __device__ __forceinline__ void st_ld32(uint32_t taddr, uint32_t* r) { tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r)); }
 __device__ __forceinline__ void st_st32(uint32_t taddr, const uint32_t* r) {
@@ -47,27 +55,27 @@ struct StSmem {
   static constexpr int kQ = 0;                                   // two tiles
   static constexpr int kK = kQ + 2 * kTileBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
-  static constexpr int kBar = kV + kStages * kTileBytes;
+  static constexpr int kStage = kV + kStages * kTileBytes;       // 2 KB for each softmax warp: 16 columns of its rows' sums
+  static constexpr int kBar = kStage + 8 * 2048;
   static constexpr int kNumBars = 3 + 4 * kStages + 6;           // q, q free, tail; full and empty per K and V stage; s_full[2], p_full[2], o_ready[2]
   static constexpr int kInts = kBar + kNumBars * 8;              // TMEM address, abort flag
-  static constexpr int kStage = (kInts + 16 + 127) / 128 * 128;  // 2 KB for each softmax warp: 16 columns of its rows' sums
-  static constexpr int kTotal = kStage + 8 * 2048;               // then what is held of the list
+  static constexpr int kTotal = (kInts + 8 + 15) / 16 * 16;      // then what is held of the lists
 };
 
 struct StMaps {
-  CUtensorMap q, k, v;
+  CUtensorMap q, k, v, own_k, own_v;
 };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kStThreads, 1)
 shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned int* status RB_BOUNDS_PARAM) {
-  // No wait for the kernel in front, the sequences' own tokens: it writes nothing that is read here, and what it waited for is done.
-  pdl_launch();
   using L = StSmem<D>;
   constexpr int kStages = L::kStages;
   extern __shared__ __align__(1024) uint8_t st_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(st_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int warp_sums[kStThreads / 32];
+  __shared__ unsigned long long work;
+  __shared__ uint64_t own_bars[2 * kStThreads / 32];
   const uint32_t sbase = smem_u32(smem), sQ = sbase + L::kQ, sK = sbase + L::kK, sV = sbase + L::kV;
   const uint32_t b0 = sbase + L::kBar;
   const uint32_t bar_q = b0, bar_qfree = b0 + 8, bar_tail = b0 + 16;
@@ -76,7 +84,10 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + L::kInts);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
   const SpList& list = p.prefix;
-  const SpHeld held = sp_held(list, reinterpret_cast<int*>(smem + L::kTotal));
+  int* const own_totals = reinterpret_cast<int*>(smem + L::kTotal);
+  int* const totals = own_totals + p.batch + 1;
+  const SpHeld own = {own_totals, totals + p.batch + 1, totals + 2 * p.batch + 1, reinterpret_cast<uint32_t*>(totals + 3 * p.batch + 1), totals + 4 * p.batch + 1};
+  const SpHeld held = {totals, nullptr, own.shared, own.span, nullptr};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr uint32_t kTmemCols = 512;
 
@@ -95,27 +106,47 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
       mbar_init(bar_pfull + 8 * t, 4);
       mbar_init(bar_oready + 8 * t, 1);
     }
+    for (int i = 0; i < 2 * kStThreads / 32; ++i) mbar_init(smem_u32(own_bars + i), 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&maps.q);
     tma_prefetch_desc(&maps.k);
     tma_prefetch_desc(&maps.v);
+    tma_prefetch_desc(&maps.own_k);
+    tma_prefetch_desc(&maps.own_v);
   }
   if (warp == 9) {
     tmem_alloc(smem_u32(tmem_ptr), kTmemCols);
     tmem_relinquish();
   }
-  sp_prepare(p, list, held, warp_sums);
+  pdl_wait();
+  pdl_launch();
+  sp_prepare(p, own, warp_sums, totals, &work, kStOne, kStTwo);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr;
   const int total = held.totals[list.entries] * list.virtual_heads;
-  const int u_begin = sp_run(total, list.ctas, blockIdx.x), u_end = sp_run(total, list.ctas, blockIdx.x + 1);
+  // ---- the last CTAs, as many as their units' share of the work, have the sequences' own tokens
+  const int ctas = gridDim.x;
+  const unsigned long long w_own = static_cast<unsigned long long>(own_totals[p.batch]) * p.list.virtual_heads * kStOwn, w_all = w_own + work * list.virtual_heads;
+  int n_own = w_all == 0 ? 0 : static_cast<int>((ctas * w_own + w_all / 2) / w_all);
+  if (w_own > 0 && n_own == 0) n_own = 1;
+  if (w_own < w_all && n_own == ctas) n_own = ctas - 1;
+  const int n_shared = ctas - n_own;
+  if (blockIdx.x == 0) {
+    sp_keep_totals(list, totals, n_shared);
+    sp_keep_totals(p.list, own_totals, n_own * kStRuns);
+  }
+  const int u_begin = n_shared ? sp_run(total, n_shared, blockIdx.x) : 0, u_end = n_shared ? sp_run(total, n_shared, blockIdx.x + 1) : 0;
   const int half = list.half;                                  // sequences of one of the two tiles
   const int tile_rows = half * list.per;
 
-  if (warp >= 8) {
+  if (static_cast<int>(blockIdx.x) >= n_shared) {
+    const int run = warp / kSpWarps;
+    const SpTma tma = {&maps.own_k, &maps.own_v, smem_u32(own_bars) + run * kSpWarps * 16, abort_flag, status};
+    sp_split<T, D, 1, true>(p, p.list, own, smem + run * SpSmem<D, 1>::kRun, (blockIdx.x - n_shared) * kStRuns + run, n_own * kStRuns, threadIdx.x % (kSpWarps * 32), 1 + run, tma RB_BOUNDS_PASS);
+  } else if (warp >= 8) {
     setmaxnreg_dec<104>();
     if (warp == 8 || warp == 10) {
       // ---------------------------------------------------------------- TMA producers, all lanes: warp 8 keys, warp 10 values
@@ -395,7 +426,6 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
     }
   }
 
-  pdl_wait();                                                  // this launch ends behind the one in front, so that the join, which waits for this one, finds both done
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {
@@ -432,8 +462,19 @@ int launch(const rb::SpParams& p, cudaStream_t stream) {
   m = rbhost::get_tmap_4d(p.v, 2, dims, str, box, 1, &err);
   if (!m) return err ? err : -7;
   maps.v = *m;
-  constexpr size_t kMostSmem = rb::StSmem<D>::kTotal + rb::sp_held_bytes(rb::kStMostBatch, rb::kStMostBatch) + 1024;
-  static_assert(kMostSmem + 1024 <= 227 * 1024, "shared memory");
+  // of the sequences' own tokens: 64 columns, tokens of all pages, the halves of a head, heads
+  const int grain = 1 << p.list.log_grain;
+  const uint64_t own_dims[4] = {64, (uint64_t)p.num_blocks * p.block_size, D / 64, (uint64_t)p.kv_heads}, own_str[3] = {token, 128, (uint64_t)D * 2};
+  const uint32_t own_box[4] = {64, (uint32_t)grain, D / 64, 1};
+  m = rbhost::get_tmap_4d(p.k, 2, own_dims, own_str, own_box, 1, &err);
+  if (!m) return err ? err : -7;
+  maps.own_k = *m;
+  m = rbhost::get_tmap_4d(p.v, 2, own_dims, own_str, own_box, 1, &err);
+  if (!m) return err ? err : -7;
+  maps.own_v = *m;
+  auto smem_of = [](int batch, int groups) { return rb::StSmem<D>::kTotal + (5 * static_cast<size_t>(batch) + 2 + groups) * 4 + 1024; };
+  constexpr size_t kMostSmem = rb::StSmem<D>::kTotal + (6 * static_cast<size_t>(rb::kStMostBatch) + 2) * 4 + 1024;
+  static_assert(kMostSmem + 1024 <= 227 * 1024 && rb::kStRuns * rb::SpSmem<D, 1>::kRun <= rb::StSmem<D>::kBar && rb::kStRuns * rb::kSpWarps * 32 == rb::kStThreads, "shared memory");
   static bool configured[64] = {false};
   const int dev = rbhost::device_slot();
   if (!configured[dev]) {
@@ -441,7 +482,7 @@ int launch(const rb::SpParams& p, cudaStream_t stream) {
     if (e != cudaSuccess) return static_cast<int>(e);
     configured[dev] = true;
   }
-  const size_t smem = rb::StSmem<D>::kTotal + rb::sp_held_bytes(p.batch, p.groups) + 1024;
+  const size_t smem = smem_of(p.batch, p.groups);
   return static_cast<int>(rbhost::launch_pdl(rb::shared_tc_kernel<T, D>, dim3(l.ctas), dim3(rb::kStThreads), smem, stream, 1, maps, p,
                                              rbhost::status_ptr() RB_BOUNDS_ARG));
 }
@@ -450,7 +491,7 @@ int launch(const rb::SpParams& p, cudaStream_t stream) {
 
 namespace rbhost {
 
-// Pages that a unit of 128 tokens has a whole number of, or that have a whole number of units; every sequence's rows of a KV head in one tile.
+// Pages that a unit of 128 tokens (and a warp's 32 of a sequence's own) has a whole number of, or that have a whole number of units; every sequence's rows of a KV head in one tile.
 bool shared_tc_takes(int batch, int heads, int kv_heads, int block_size, int most) {
   return batch <= rb::kStMostBatch && heads / kv_heads <= rb::kStTile && most >= 1 &&
          (block_size % rb::kSpUnit == 0 || (block_size >= 8 && rb::kSpUnit % block_size == 0)) && block_size < (1 << 20);
@@ -468,6 +509,7 @@ rb::SpList shared_tc_list(int batch, int heads, int kv_heads) {
   l.rows = sp_list_rows(l);
   return l;
 }
+int shared_tc_runs() { return device_sm_count() * rb::kStRuns; }
 int shared_tc(const rb::SpParams& p, int type, int head_dim, cudaStream_t stream) {
   if (type == 0) return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, stream) : launch<__nv_bfloat16, 128>(p, stream);
   return head_dim == 64 ? launch<__half, 64>(p, stream) : launch<__half, 128>(p, stream);

@@ -32,7 +32,7 @@ N.optional_sig("rb_move_reorder", [C.c_char_p, N.c_int, N.c_void_p, N.c_int, N.c
 N.optional_sig("rb_shared_prefix", [C.c_char_p, N.c_void_p])
 N.optional_sig("rb_shared_prefix_scratch_bytes", [N.c_int] * 7, N.c_ll)
 N._LAUNCHES["rb_beam_select"] = 2
-N._LAUNCHES["rb_shared_prefix"] = 3                 # at most: groups of few rows take two
+N._LAUNCHES["rb_shared_prefix"] = 2
 
 
 def _here(what: str, dev: int, *tensors) -> None:
@@ -293,8 +293,8 @@ def shared_pays(groups: PrefixGroups, shared_lens, row_bytes: int) -> bool:
 
 
 # Bytes that are not read again.  One B200, attention of a layer, us, every sequence's own reading / one for the group: 4 beams over 300 tokens (12 KV heads of 64; 3 MB) 7.6 / 11.3,
-# 4 over 1000 (8 KV heads of 128; 12 MB) 11.1 / 14.9, 8 over 1000 (29 MB) 12.5 / 20.6, 4 over 4000 (49 MB) 21.4 / 17.6, 16 over 1000 (61 MB) 21.3 / 22.4, 2 over 16000
-# (66 MB) 43.9 / 23.1, 8 over 4000 (115 MB) 38.1 / 25.5, 32 over 2000 (254 MB) 60.0 / 26.4.
+# 4 over 1000 (8 KV heads of 128; 12 MB) 7.5 / 15.2, 8 over 1000 (29 MB) 12.4 / 18.9, 4 over 4000 (49 MB) 21.4 / 17.9, 4 times 4 over 1000 (49 MB) 20.2 / 17.7, 16 over 1000
+# (61 MB) 21.5 / 19.9, 2 over 16000 (66 MB) 43.7 / 22.3, 8 over 4000 (115 MB) 38.1 / 21.1, 32 over 2000 (254 MB) 59.8 / 22.5.
 SHARED_PAYS = 48_000_000
 
 
