@@ -38,8 +38,9 @@ shared_split_kernel(const SpParams p RB_BOUNDS_PARAM) {
 constexpr int kSpJoinWarps = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(kSpJoinWarps * 32)
-shared_join_kernel(const SpParams p, const int share) {
+shared_join_kernel(const SpParams p, const int log_share) {
   constexpr int C = D / 32;
+  const int share = 1 << log_share;
   __shared__ float sum_sh[kSpJoinWarps][D + 2];  // a warp's columns, maximum and sum
   const int b = blockIdx.x, hk = blockIdx.y, group = p.heads / p.kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -54,21 +55,21 @@ shared_join_kernel(const SpParams p, const int share) {
   const SpList& look = lane & 2 ? p.list : p.prefix;
   const int all = look.totals[look.entries], runs = look.totals[look.entries + 1], t0 = look.totals[lane & 2 ? look.own + b : tile], t1 = look.totals[(lane & 2 ? look.own + b : tile) + 1];
   {
-    const int h = blockIdx.z * (kSpJoinWarps / share) + warp / share, which = warp % share;
+    const int h = (blockIdx.z * (blockDim.x >> 5) + warp) >> log_share, which = warp & (share - 1);
     const bool mine = h < group;
     float mx = -INFINITY, den = 0.f, acc[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = 0.f;
     if (mine && any) {
       // parts over shared tokens, then the sequence's own: how many CTAs, the first, and the rows where its part and those of CTA 0 are
-      const int k_look = h / look.per, u = (hk * look.parts + k_look) * all + (lane & 1 ? t1 - 1 : t0);
+      const int k_look = look.parts == 1 ? 0 : h / look.per, u = (hk * look.parts + k_look) * all + (lane & 1 ? t1 - 1 : t0);
       const int cta = t1 > t0 ? sp_cta_of(all * look.virtual_heads, runs, u) : lane & 1 ? -1 : 0;
       int n[2], c0[2];
       long long row[2], later[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const SpList& l = i == 0 ? p.prefix : p.list;
-        const int e = i == 0 ? tile : l.own + b, k = h / l.per, vh = hk * l.parts + k, r = (i == 0 ? b - tile : 0) * l.per + h - k * l.per;
+        const int e = i == 0 ? tile : l.own + b, k = l.parts == 1 ? 0 : h / l.per, vh = hk * l.parts + k, r = (i == 0 ? b - tile : 0) * l.per + h - k * l.per;
         c0[i] = __shfl_sync(0xffffffffu, cta, 2 * i);
         n[i] = __shfl_sync(0xffffffffu, cta, 2 * i + 1) - c0[i] + 1;
         row[i] = sp_row(l, vh, e, 0, true) + r;
@@ -95,7 +96,7 @@ shared_join_kernel(const SpParams p, const int share) {
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[c] *= again;
         mx = top;
-        const int m = min(32, (parts - s0 + share - 1) / share);
+        const int m = min(32, (parts - s0 + share - 1) >> log_share);
 #pragma unroll 8
         for (int k = 0; k < m; ++k) {
           const float fk = __shfl_sync(0xffffffffu, f, k);
@@ -157,11 +158,11 @@ struct Plan {
   rb::SpList list, prefix;
   size_t smem;
   int tiles;                                     // m-tiles of the split kernel
-  int share;                                     // warps of a row of the join
+  int log_share;                                 // 2^log_share warps of a row of the join
   bool tc;
 };
-// Groups with more than 16 rows go to the tcgen05 kernel, which takes 256 at a time (64 sequences with 4 rows each over 8000 shared tokens: 64 us, with tiles of 32 rows on mma.sync over 200),
-// where pages, batch and scale allow; else this file's has one m-tile, or two where rows need them.
+// Groups with more than 16 rows go to the tcgen05 kernel, which takes 256 at a time where pages, batch and scale allow
+// (256 sequences with 4 rows each for 8 KV heads over 16384 shared tokens took 456 us with tiles of 32 rows on mma.sync, 133 now); else this file's has one m-tile, or two where rows need them.
 Plan plan_of(int batch, int groups, int heads, int kv_heads, int head_dim, int block_size, int most, bool positive) {
   Plan p;
   memset(&p, 0, sizeof(p));
@@ -185,10 +186,10 @@ Plan plan_of(int batch, int groups, int heads, int kv_heads, int head_dim, int b
   l.ctas = p.tc ? rbhost::shared_tc_runs() : rbhost::device_sm_count() * (resident < 1 ? 1 : resident < most_resident ? resident : most_resident);
   l.rows = rbhost::sp_list_rows(l);
   p.prefix = p.tc ? rbhost::shared_tc_list(batch, heads, kv_heads) : l;
-  // parts of a row over shared tokens, if these are long: about four for a warp
+  // parts of a row over shared tokens, if these are long: up to about five for a warp, which looks every row's up first
   const int tiles_of = (batch + p.prefix.seqs - 1) / p.prefix.seqs, entries = groups > tiles_of ? groups : tiles_of;
-  const long long parts = p.prefix.ctas / (static_cast<long long>(entries) * p.prefix.virtual_heads) * (p.tc ? 2 : 1);
-  p.share = parts >= 24 ? 8 : parts >= 12 ? 4 : parts >= 6 ? 2 : 1;
+  const long long parts = p.prefix.ctas / (static_cast<long long>(entries) * p.prefix.virtual_heads) * (p.prefix.half > 0 && most <= p.prefix.half ? 2 : 1);
+  p.log_share = parts >= 24 ? 3 : parts >= 12 ? 2 : parts >= 6 ? 1 : 0;
   return p;
 }
 // Puts a list's arrays at `at` (NULL: only counts) and returns their size.
@@ -222,8 +223,8 @@ template <typename T, int D>
 int launch(const rb::SpParams& p, const Plan& l, int type, cudaStream_t s) {
   const int code = l.tc ? rbhost::shared_tc(p, type, D, s) : static_cast<int>(l.tiles == 1 ? split<T, D, 1>(p, l, s) : split<T, D, 2>(p, l, s));
   if (code) return code;
-  const int rows = rb::kSpJoinWarps / l.share, group = p.heads / p.kv_heads;
-  return static_cast<int>(rbhost::launch_pdl(rb::shared_join_kernel<T, D>, dim3(p.batch, p.kv_heads, (group + rows - 1) / rows), dim3(rb::kSpJoinWarps * 32), 0, s, 1, p, l.share));
+  const int group = p.heads / p.kv_heads, warps = (group << l.log_share) < rb::kSpJoinWarps ? group << l.log_share : rb::kSpJoinWarps, rows = warps >> l.log_share;
+  return static_cast<int>(rbhost::launch_pdl(rb::shared_join_kernel<T, D>, dim3(p.batch, p.kv_heads, (group + rows - 1) / rows), dim3(warps * 32), 0, s, 1, p, l.log_share));
 }
 
 }  // namespace
