@@ -57,7 +57,7 @@ struct StSmem {
   static constexpr int kV = kK + kStages * kTileBytes;
   static constexpr int kStage = kV + kStages * kTileBytes;       // 2 KB for each softmax warp: 16 columns of its rows' sums
   static constexpr int kBar = kStage + 8 * 2048;
-  static constexpr int kNumBars = 3 + 4 * kStages + 6;           // q, q free, tail; full and empty per K and V stage; s_full[2], p_full[2], o_ready[2]
+  static constexpr int kNumBars = 3 + 4 * kStages + 8;           // q, q free, tail; full and empty per K and V stage; s_full[2], o_ready[2], p_full[2][2]
   static constexpr int kInts = kBar + kNumBars * 8;              // TMEM address, abort flag
   static constexpr int kTotal = (kInts + 8 + 15) / 16 * 16;      // then what is held of the lists
 };
@@ -80,7 +80,7 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
   const uint32_t b0 = sbase + L::kBar;
   const uint32_t bar_q = b0, bar_qfree = b0 + 8, bar_tail = b0 + 16;
   const uint32_t bar_kfull = b0 + 24, bar_kempty = bar_kfull + 8 * kStages, bar_vfull = bar_kempty + 8 * kStages, bar_vempty = bar_vfull + 8 * kStages;
-  const uint32_t bar_sfull = bar_vempty + 8 * kStages, bar_pfull = bar_sfull + 16, bar_oready = bar_pfull + 16;
+  const uint32_t bar_sfull = bar_vempty + 8 * kStages, bar_oready = bar_sfull + 16, bar_pfull = bar_oready + 16;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + L::kInts);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
   const SpList& list = p.prefix;
@@ -103,7 +103,8 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(bar_sfull + 8 * t, 1);
-      mbar_init(bar_pfull + 8 * t, 4);
+      mbar_init(bar_pfull + 16 * t, 4);
+      mbar_init(bar_pfull + 16 * t + 8, 4);
       mbar_init(bar_oready + 8 * t, 1);
     }
     for (int i = 0; i < 2 * kStThreads / 32; ++i) mbar_init(smem_u32(own_bars + i), 1);
@@ -240,16 +241,19 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
           umma_commit(bar_sfull + 8 * t);
           return true;
         };
-        // O_t (+)= P_t V_i, once P_t is there
+        // O_t (+)= P_t V_i, each half of the unit's tokens once P_t has it
         auto issue_pv = [&](int i, int t, bool add) -> bool {
-          if (!mbar_wait(bar_pfull + 8 * t, done[t] & 1, abort_flag, status, 58)) return false;
-          ++done[t];
-          tc_fence_after();
           const uint32_t tmem_p = tmem_base + t * 128, tmem_o = tmem_base + 256 + t * 128;
           const uint64_t v = dV + (i % kStages) * (L::kTileBytes / 16);
 #pragma unroll
-          for (int ks = 0; ks < kSpUnit / 16; ++ks)
+          for (int ks = 0; ks < kSpUnit / 16; ++ks) {
+            if (ks % (kSpUnit / 32) == 0) {
+              if (!mbar_wait(bar_pfull + 16 * t + (ks ? 8 : 0), done[t] & 1, abort_flag, status, 58)) return false;
+              tc_fence_after();
+            }
             umma_bf16_ts(tmem_o, tmem_p + ks * 8, v + ks * (2048 / 16), idesc_pv, (add || ks != 0) ? 1u : 0u);
+          }
+          ++done[t];
           umma_commit(bar_oready + 8 * t);
           return true;
         };
@@ -385,13 +389,16 @@ shared_tc_kernel(const __grid_constant__ StMaps maps, const SpParams p, unsigned
               packed[i / 2 + 1] = sp_pack<T>(p2, p3);
             }
             st_st32(tmem_s + c * 32, packed);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_pfull + 16 * t + 8 * c);          // the products of the first half run beside the second's exponentials
           }
           l_run += (rs0 + rs1) + (rs2 + rs3);
-          tmem_st_wait();
+        } else if (lane == 0) {
+          mbar_arrive(bar_pfull + 16 * t);
+          mbar_arrive(bar_pfull + 16 * t + 8);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_pfull + 8 * t);
       }
       if (!ok) break;
       // ---- the part's sums, 16 columns at a time through shared memory: rows of 512 bytes by threads of their own would be 32 sectors a store
