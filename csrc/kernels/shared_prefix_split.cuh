@@ -53,7 +53,7 @@ __device__ __forceinline__ void sp_advance(const SpList& l, const SpHeld& held, 
 }
 
 // The copies go on from one part to the next: the next unit's keys, whichever part they are of, are asked for as soon as this unit's scores are formed, its values behind this unit's
-// product, and its places in the cache are looked up a unit earlier (looked up when they were needed they took 4300 of a unit's 7000 cycles).  Bound by the chain of these steps, 5000 cycles
+// product, and its places in the cache are looked up a unit earlier (looked up when they were needed they took 4300 of a unit's 7000 cycles).  Bound by the chain of these steps, 4500 cycles
 // for a unit with three runs on an SM, of which waits for memory are a tenth.  The warps' sums are joined in the memory of
 // their V tiles (two m-tiles: of K and V, and the next part's keys are asked for behind the join).
 //
@@ -101,8 +101,11 @@ __device__ __forceinline__ void sp_split(const SpParams& p, const SpList& list, 
   }
   c0.hk = c0.vh / list.parts;
   c0.upto = held.totals[c0.e + 1];
+  // runs whose keys and values come by TMA have entries of sequences' own tokens only
+  auto is_own = [&](int e) { return TMA || e >= list.own; };
+  auto first_of = [&](int e) { return TMA ? e : e >= list.own ? e - list.own : e; };
   auto rows_of = [&](int e) {
-    if (e >= list.own) return list.per;
+    if (is_own(e)) return list.per;
     return min(list.seqs, static_cast<int>(held.span[e] >> 16) - e) * list.per;
   };
   // ---- rows of queries: loaded into registers, stored when the last part's have been read
@@ -116,7 +119,7 @@ __device__ __forceinline__ void sp_split(const SpParams& p, const SpList& list, 
   }
   auto load_q = [&](const SpUnit& c) {
     const int head0 = (c.vh - c.hk * list.parts) * list.per, real = min(list.per, group - head0);
-    const int b = c.e >= list.own ? c.e - list.own : c.e, seqs = c.e >= list.own ? 1 : min(list.seqs, static_cast<int>(held.span[c.e] >> 16) - c.e);
+    const int b = first_of(c.e), seqs = is_own(c.e) ? 1 : min(list.seqs, static_cast<int>(held.span[c.e] >> 16) - c.e);
 #pragma unroll
     for (int i = 0; i < kQPieces; ++i) {
       const int piece = (i * kSpWarps * 32 + tid) % LP;
@@ -135,25 +138,28 @@ __device__ __forceinline__ void sp_split(const SpParams& p, const SpList& list, 
   auto page_of = [&](int token) { return p.log_block >= 0 ? token >> p.log_block : token / p.block_size; };
   // ---- places of a unit's keys and values: looked up, then asked for
   struct Places {
-    int blk, off, n, hk;                         // of the lane's token or page: block and place in it; the warp's tokens (0 and less: none)
+    int blk, off, n, hk, lead;                   // of the lane's token or page: block and place in it; the warp's tokens (0 and less: none), the first `lead` of them others'
   };
   auto look_up = [&](const SpUnit& c) {
     Places w;
-    const bool own = c.e >= list.own;
+    const bool own = is_own(c.e);
     const int shared = held.shared[c.e], at = (c.at - held.totals[c.e]) * kSpUnit + warp * 32;
     w.n = min(32, held.count[c.e] - at);
     w.hk = c.hk;
     w.blk = w.off = 0;
+    w.lead = 0;
+    const int* table = p.tables + static_cast<long long>(own ? first_of(c.e) : static_cast<int>(held.span[c.e] & 0xffffu)) * p.width;
     if (TMA) {                                   // of the lane's page
+      if (at == 0) w.lead = shared & (size - 1); // the first tokens of an entry may be others'
       if (lane * size < w.n) {
-        const int token = (own ? shared & -size : 0) + at + lane * size, page = page_of(token);
+        const int token = (shared & -size) + at + lane * size, page = page_of(token);
         w.off = token - page * p.block_size;
-        w.blk = p.tables[static_cast<long long>(own ? c.e - list.own : static_cast<int>(held.span[c.e] & 0xffffu)) * p.width + page];
+        w.blk = table[page];
       }
     } else if (lane < w.n) {
       const int token = (own ? shared : 0) + at + lane, page = page_of(token);
       w.off = token - page * p.block_size;
-      w.blk = p.tables[static_cast<long long>(own ? c.e - list.own : static_cast<int>(held.span[c.e] & 0xffffu)) * p.width + page];
+      w.blk = table[page];
     }
     return w;
   };
@@ -217,8 +223,7 @@ __device__ __forceinline__ void sp_split(const SpParams& p, const SpList& list, 
   uint32_t phase = 0;                            // of this warp's two barriers
   for (;; --left) {
     const int n_tok = w0.n, rows = rows_of(c0.e);
-    // the first tokens of an entry may be others'
-    const int lead = TMA && warp == 0 && c0.e >= list.own && c0.at == held.totals[c0.e] ? held.shared[c0.e] & (size - 1) : 0;
+    const int lead = TMA ? w0.lead : 0;
     const bool more = left > 1, last = !more || c1.e != c0.e || c1.vh != c0.vh;
     if (!TMA) wm_cp_wait<1>();                   // this unit's K tile has landed (V may be on its way)
     else if (n_tok > 0) mbar_wait(tma.bars + warp * 16, phase, tma.abort_flag, tma.status, 62);
@@ -290,9 +295,7 @@ __device__ __forceinline__ void sp_split(const SpParams& p, const SpList& list, 
             sum += p0 + p1;
             pf[t][n >> 1][(n & 1) * 2 + i] = sp_pack<T>(p0, p1);
           }
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          l[t][i] = fmaf(l[t][i], al, sum);
+          l[t][i] = fmaf(l[t][i], al, sum);      // of this lane's tokens
           m[t][i] = mn;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
@@ -343,6 +346,8 @@ __device__ __forceinline__ void sp_split(const SpParams& p, const SpList& list, 
         for (int i = 0; i < 2; ++i) {
           if (TMA && i == 1 && rows <= 8) continue;
           const int r = t * 16 + gq + i * 8;
+          l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], 1);
+          l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], 2);
           if (tq == 0) ml_sh[warp * kRows + r] = make_float2(m[t][i], l[t][i]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(mine + r * D + ((n * 8) ^ ((r & 7) * 8)) + 2 * tq) = make_float2(acc[t][n][2 * i], acc[t][n][2 * i + 1]);

@@ -13,8 +13,8 @@
 // token are set to zero, since a weight of zero times what they hold need not be zero.
 //
 // The sequences' own tokens are read in the same launch by CTAs of their own, three runs of four warps each (shared_prefix_split.cuh): one part of the GPU is bound by products and
-// exponentials while the other waits for memory.  One after the other they took 145 us where it is 133 now (256 sequences with 4 rows each for 8 KV heads of 128, 16384 shared and 16 to 512 own
-// tokens), 73.5 and 71.7 for 12 groups of 8, 54.6 and 50.8 for one document of 32771 tokens and 16 sequences.  Every CTA finds from the lengths how many CTAs each kind gets.
+// exponentials while the other waits for memory.  One after the other they took 145 us, beside one another 133, 122 with all later steps (256 sequences with 4 rows each for 8 KV heads of 128, 16384 shared and 16 to 512 own
+// tokens); 73.5, 71.7 and 72 for 12 groups of 8; 54.6, 50.8 and 49 for one document of 32771 tokens and 16 sequences.  Every CTA finds from the lengths how many CTAs each kind gets.
 //
 // Bound by the softmax's exponentials and the products where there are 256 rows, by the keys' and values' bytes where there are few.
 #define RB_INLINE_WAITS                 // registers are reallocated between warp groups
@@ -31,8 +31,8 @@ constexpr int kStTile = 128;
 constexpr float kStRescale = 8.f;        // log2 units
 constexpr int kStMostBatch = 704;        // their totals, tokens and spans beside 192 KB of tiles
 constexpr int kStRuns = 3;               // of a CTA that has sequences' own tokens
-// What a unit of 128 tokens takes a CTA, relative to one another: with two tiles of rows, with one, and of a sequence's own.  The first case above takes 133 us with 5 : 3 : 2, 146 with
-// 6 : 3 : 2 and 143 with 4 : 3 : 2; the second 71.7, or 73.7 with 5 : 2 : 2 and 79 with 5 : 4 : 2.
+// What a unit of 128 tokens takes a CTA, relative to one another: with two tiles of rows, with one, and of a sequence's own.  When they were set the first case above took 133 us
+// with 5 : 3 : 2, 146 with 6 : 3 : 2 and 143 with 4 : 3 : 2; the second 71.7, or 73.7 with 5 : 2 : 2 and 79 with 5 : 4 : 2.
 constexpr int kStTwo = 5, kStOne = 3, kStOwn = 2;
 
 __device__ __forceinline__ void st_ld32(uint32_t taddr, uint32_t* r) { tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r)); }
