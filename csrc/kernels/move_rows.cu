@@ -8,6 +8,9 @@
 // In place, a row may be wanted by several others and be overwritten itself.  A thread owns one column, 16 bytes of every row of a group: it loads all of
 // the column before it stores any of it, so that no other thread and no second buffer takes part, whatever the index says.  Rows that stay are
 // neither read for themselves nor written.
+//
+// One B200: 256 blocks of 32 KB in the keys and values of 8 layers, 42.9 us, 6.26 TB/s of reads and writes (a plain copy: 6.57); 16 beams in groups of 4, keys and values of 4 layers
+// of 12 heads over 1000 tokens, 47.4 us, 5.45 TB/s.  Small calls are their launch, 2.4 to 3.2 us.
 #include "move_rows.h"
 
 #include <string.h>

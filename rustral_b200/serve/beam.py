@@ -145,7 +145,7 @@ class BeamSearch:
                         self._finish(g, g.beams[parent][1] + [token], best[i][j], True)
                 else:
                     chosen.append((parent, token, best[i][j]))
-            self._judge(g, chosen, length)
+            self._settle(g, chosen, length)
             chosen += [(chosen[0][0] if chosen else 0, 0, float("-inf"))] * (K - len(chosen))          # beams that are not there
             kept = {p for p, _, _ in chosen}
             dropped += [s for p, (s, _, _) in enumerate(g.beams) if p not in kept]
@@ -169,7 +169,7 @@ class BeamSearch:
             for s, (_, _, at, g) in zip(new, forks):
                 g.beams[at] = (s, *g.beams[at][1:])
 
-    def _judge(self, g: _Group, chosen: list, length: int) -> None:
+    def _settle(self, g: _Group, chosen: list, length: int) -> None:
         """Whether the search over a prompt is over: no beam is left, or `beams` finished continuations rank above the best beam."""
         if not chosen:
             g.over = True
