@@ -28,15 +28,16 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// Every size has a word of its own: of two that shared one, larger tensors (more than 2^20 cached tokens) got maps of smaller ones at the same address.
 struct Key {
-  uint64_t v[8];
+  uint64_t v[13];
   bool operator==(const Key& o) const { return memcmp(v, o.v, sizeof(v)) == 0; }
 };
 struct KeyHash {
   size_t operator()(const Key& k) const {
     uint64_t h = 1469598103934665603ull;
-    for (int i = 0; i < 8; ++i) {
-      h ^= k.v[i];
+    for (const uint64_t w : k.v) {
+      h ^= w;
       h *= 1099511628211ull;
     }
     return static_cast<size_t>(h);
@@ -50,7 +51,7 @@ const CUtensorMap* get_tmap_2d(const void* base, int elem_bytes, uint64_t inner,
                                uint32_t box_inner, uint32_t box_outer, int swizzle128, int* err) {
   int dev = 0;
   cudaGetDevice(&dev);
-  Key k;
+  Key k = {};
   k.v[0] = reinterpret_cast<uint64_t>(base);
   k.v[1] = inner; k.v[2] = outer; k.v[3] = ld;
   k.v[4] = (static_cast<uint64_t>(box_inner) << 32) | box_outer;
@@ -97,16 +98,15 @@ const CUtensorMap* get_tmap_4d(const void* base, int elem_bytes, const uint64_t 
                                const uint32_t box[4], int swizzle128, int* err) {
   int dev = 0;
   cudaGetDevice(&dev);
-  Key k;
+  Key k = {};
   k.v[0] = reinterpret_cast<uint64_t>(base);
-  k.v[1] = dims[0] | (dims[1] << 20) | (dims[2] << 40);
-  k.v[2] = dims[3] | (static_cast<uint64_t>(box[0]) << 32) | (static_cast<uint64_t>(box[2]) << 44);
-  k.v[3] = strides_bytes[0];
-  k.v[4] = strides_bytes[1];
-  k.v[5] = strides_bytes[2];
-  k.v[6] = static_cast<uint64_t>(elem_bytes) | (static_cast<uint64_t>(swizzle128) << 8) | (4ull << 16) |
-           (static_cast<uint64_t>(box[1]) << 24) | (static_cast<uint64_t>(box[3]) << 40);
-  k.v[7] = static_cast<uint64_t>(dev);
+  for (int i = 0; i < 4; ++i) k.v[1 + i] = dims[i];
+  for (int i = 0; i < 3; ++i) k.v[5 + i] = strides_bytes[i];
+  k.v[8] = static_cast<uint64_t>(box[0]) << 32 | box[1];
+  k.v[9] = static_cast<uint64_t>(box[2]) << 32 | box[3];
+  k.v[10] = static_cast<uint64_t>(elem_bytes);
+  k.v[11] = static_cast<uint64_t>(swizzle128) << 32 | 4;
+  k.v[12] = static_cast<uint64_t>(dev);
   std::lock_guard<std::mutex> lock(g_mu);
   auto it = g_cache.find(k);
   if (it != g_cache.end()) return it->second;
