@@ -3,6 +3,7 @@
 // A block may be in several tables (rb_ba_fork): it counts its owners and is free again when the last one lets go of it.
 // Semantics follow the reference's PagedCache (crates/nn/src/kv_cache.rs:382-432) with its defect removed: a
 // second reservation for a sequence extends the table instead of overwriting it (kv_cache.rs:420-423).
+#include <algorithm>
 #include <mutex>
 #include <unordered_map>
 #include <vector>
@@ -163,27 +164,43 @@ int rb_ba_fork(RbBlockAllocator* a, int64_t parent, int64_t child, int num_token
 
 int rb_ba_num_shared(const RbBlockAllocator* a) { std::lock_guard<std::mutex> l(a->mu); return a->shared; }
 
-// Gives the sequence blocks of its own in place of shared ones among those of tokens first .. first + n - 1, which are about to be written.  Returns how many pairs of blocks
-// (src, dst, room for `max`) the caller has to copy, -1 for an unknown sequence or tokens without blocks, -2 without enough free blocks or room (nothing changed).
-int rb_ba_own(RbBlockAllocator* a, int64_t seq_id, int64_t first, int64_t n, int32_t* src, int32_t* dst, int max) {
+// Gives sequences blocks of their own in place of shared ones among those of tokens first[i] .. first[i] + count[i] - 1 of sequence ids[i], which are about to be written.  Returns how many
+// pairs of blocks (src, dst, room for `max`) the caller has to copy, -1 for an unknown sequence or tokens without blocks, -2 without enough free blocks, room or memory (nothing changed
+// in either case).  Of sequences that share a block with each other alone, the last one keeps it.
+int rb_ba_own(RbBlockAllocator* a, const int64_t* ids, const int64_t* first, const int64_t* count, int n, int32_t* src, int32_t* dst, int max) try {
   std::lock_guard<std::mutex> l(a->mu);
-  auto it = a->tables.find(seq_id);
-  if (it == a->tables.end() || first < 0 || n < 0 || first + n > (int64_t)it->second.size() * a->block_size) return -1;
-  if (n == 0) return 0;
-  const int64_t b0 = first / a->block_size, b1 = (first + n - 1) / a->block_size;
-  int need = 0;
-  for (int64_t i = b0; i <= b1; ++i) need += a->owners[it->second[i]] > 1 ? 1 : 0;
-  if (need > (int)a->free_list.size() || need > max) return -2;
+  for (int i = 0; i < n; ++i) {
+    auto it = a->tables.find(ids[i]);
+    if (it == a->tables.end() || first[i] < 0 || count[i] < 0 || first[i] + count[i] > (int64_t)it->second.size() * a->block_size) return -1;
+  }
+  std::vector<int32_t*> changed;
+  changed.reserve(std::min<size_t>(max < 0 ? 0 : max, a->free_list.size()));
   int k = 0;
-  for (int64_t i = b0; i <= b1; ++i) {
-    int32_t& b = it->second[i];
-    if (a->owners[b] < 2) continue;
-    src[k] = b;
-    dst[k] = a->take();
-    a->give(b);
-    b = dst[k++];
+  for (int i = 0; i < n; ++i) {
+    if (count[i] == 0) continue;
+    std::vector<int32_t>& tab = a->tables.find(ids[i])->second;
+    for (int64_t j = first[i] / a->block_size; j <= (first[i] + count[i] - 1) / a->block_size; ++j) {
+      int32_t& b = tab[j];
+      if (a->owners[b] < 2) continue;
+      if (k == max || a->free_list.empty()) {
+        while (k-- > 0) {                                        // everything as it was, the order of the free list too
+          a->owners[dst[k]] = 0;
+          a->free_list.push_back(dst[k]);
+          if (++a->owners[src[k]] == 2) ++a->shared;
+          *changed[k] = src[k];
+        }
+        return -2;
+      }
+      src[k] = b;
+      dst[k] = a->take();
+      a->give(b);
+      b = dst[k++];
+      changed.push_back(&b);
+    }
   }
   return k;
+} catch (...) {
+  return -2;
 }
 
 // Moves what is in use to the lowest blocks: tables, owners and the free list change at once, and the caller copies the blocks src[i] to dst[i] (room for num_blocks each).

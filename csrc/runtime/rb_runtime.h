@@ -27,7 +27,7 @@ int rb_ba_num_sequences(const RbBlockAllocator* a);
 // Blocks in several tables: see block_allocator.cpp.
 int rb_ba_fork(RbBlockAllocator* a, int64_t parent, int64_t child, int num_tokens, int32_t* src, int32_t* dst);
 int rb_ba_num_shared(const RbBlockAllocator* a);                                         // blocks with more than one owner
-int rb_ba_own(RbBlockAllocator* a, int64_t seq_id, int64_t first, int64_t n, int32_t* src, int32_t* dst, int max);
+int rb_ba_own(RbBlockAllocator* a, const int64_t* ids, const int64_t* first, const int64_t* count, int n, int32_t* src, int32_t* dst, int max);
 int rb_ba_compact(RbBlockAllocator* a, int32_t* src, int32_t* dst);
 // State slots of models with recurrent layers: once set, a sequence's first reservation takes a free slot (and fails without
 // one) and rb_ba_free gives it back.

@@ -44,7 +44,7 @@ def declare_runtime(lib) -> None:
     _sig(lib, "rb_ba_slot", [P, LL, I], LL)
     _sig(lib, "rb_ba_fork", [P, LL, LL, I, P, P], I)
     _sig(lib, "rb_ba_num_shared", [P], I)
-    _sig(lib, "rb_ba_own", [P, LL, LL, LL, P, P, I], I)
+    _sig(lib, "rb_ba_own", [P, P, P, P, I, P, P, I], I)
     _sig(lib, "rb_ba_compact", [P, P, P], I)
     _sig(lib, "rb_ba_set_state_slots", [P, I], I)
     _sig(lib, "rb_ba_state_slot", [P, LL], I)

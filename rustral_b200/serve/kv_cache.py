@@ -331,16 +331,25 @@ class PagedCache:
 
     def own(self, seq_id: int, first: int, n: int) -> None:
         """Blocks of its own, with the same content, in place of shared ones among those of the sequence's tokens first .. first + n - 1, which are about to be written."""
-        if n < 1 or not self.shared_blocks:
+        self.own_all([seq_id], [first], [n])
+
+    def own_all(self, seq_ids: list, first: list, n: list) -> None:
+        """`own` for several sequences, tokens first[i] .. first[i] + n[i] - 1 of each: all of them, or an error that leaves every table as it was."""
+        wanted = [(s, f, c) for s, f, c in zip(seq_ids, first, n) if c > 0]
+        if not wanted or not self.shared_blocks:
             return
-        room = (first + n - 1) // self.block_size - first // self.block_size + 1
-        src, dst = (C.c_int32 * room)(), (C.c_int32 * room)()
-        k = self._lib.rb_ba_own(self._h, seq_id, first, n, C.addressof(src), C.addressof(dst), room)
+        bs = self.block_size
+        room = min(sum((f + c - 1) // bs - f // bs + 1 for _, f, c in wanted), self.free_blocks)
+        numbers = (C.c_int64 * (3 * len(wanted)))(*(x for column in zip(*wanted) for x in column))
+        pairs = (C.c_int32 * (2 * room))()
+        at, to = C.addressof(numbers), C.addressof(pairs)
+        k = self._lib.rb_ba_own(self._h, at, at + 8 * len(wanted), at + 16 * len(wanted), len(wanted), to, to + 4 * room, room)
         if k == -1:
-            raise IndexError(f"positions {first} to {first + n - 1} of sequence {seq_id} have no blocks")
+            raise IndexError("tokens that are about to be written have no blocks: (sequence, first, number) " + ", ".join(str(w) for w in wanted))
         if k < 0:
-            raise RuntimeError(f"no free blocks for sequence {seq_id}, which writes into blocks that others share")
-        self.copy_blocks(src[:k], dst[:k])
+            raise RuntimeError("no free blocks for sequences that write into blocks that others share")
+        if k:
+            self.copy_blocks(pairs[:k], pairs[room:room + k])
 
     def compact(self) -> int:
         """Moves what is in use to the first blocks, num_blocks - free_blocks of them, and returns how many blocks moved.  Sequences keep their ids and tokens; block numbers that a program
@@ -366,10 +375,12 @@ class PagedCache:
                 raise InvalidArgument(f"PagedCache.evict: no sequence {s}")
             if n < 0 or n > len(t) * self.block_size:
                 raise InvalidArgument(f"PagedCache.evict: sequence {s} has no blocks for {n} tokens")
+        if keep < 1 or recent < 0 or keep_first < 0 or recent + keep_first > keep:
+            raise ValueError("PagedCache.evict: keep must be at least 1 and at least recent + keep_first")
         if not seq_ids:
             return []
-        for s, n in zip(seq_ids, lens):
-            self.own(s, 0, n)
+        # tokens move to the first `keep` places; sequences that lose none stay as they are, with the blocks that they share
+        self.own_all(seq_ids, [0] * len(lens), [keep if n > keep else 0 for n in lens])
         host = torch.empty((len(seq_ids), max(len(t) for t in tables)), dtype=torch.int32)
         self.fill_tables(seq_ids, host)
         device = self.pages[0].k.device

@@ -1,10 +1,12 @@
 """Several continuations of one prompt where caches are large, tensors lie together, weights are kept and calls are refused (ops.beams, serve.PagedCache, serve.BeamSearch)."""
 import math
+import random
 
 import pytest
 import torch
 
 from rustral_b200 import ops
+from rustral_b200.serve import CacheQuantization, PagedCache
 from test_beams import attend64, bound
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -33,3 +35,80 @@ def test_attention_shared_in_a_larger_cache_at_the_same_address(dim, more, cuda_
         place[pages] = torch.arange(len(pages))
         want, most = attend64(q, *held, place[t.long()], lens, 1.0 / math.sqrt(dim))
         assert ((got.cpu().double() - want).abs() <= bound(want, most, torch.bfloat16)).all()
+
+
+# ---- shared blocks -----------------------------------------------------------------------------------------------------------------------------
+def weighed(blocks, device="cpu", bs=16):
+    return PagedCache(blocks, bs, 2, 2, 64, device=device, quantization=CacheQuantization.FP8, attention_weights=True)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_evict_leaves_what_loses_no_tokens(device):
+    """Only sequences that lose tokens get blocks of their own, and those only for the tokens that are kept; without room for all of them nothing changes."""
+    c = weighed(5, device)
+    c.allocate(1, 48)
+    for p in c.pages:
+        p.weight.copy_(torch.arange(p.weight.numel()).view(p.weight.shape))
+        p.k.view(torch.uint8).random_(0, 127), p.v.view(torch.uint8).random_(0, 127)
+    assert c.fork([1, 1], [2, 3], [48, 32])
+    tables = [c.block_table(s) for s in (1, 2, 3)]
+    state = [[t.clone() for t in (p.k.view(torch.uint8), p.v.view(torch.uint8), p.weight)] for p in c.pages]
+
+    def unchanged():
+        assert [c.block_table(s) for s in (1, 2, 3)] == tables and c.free_blocks == 2 and c.shared_blocks == 3 and not c.thinned
+        assert all(torch.equal(a, b) for p, was in zip(c.pages, state) for a, b in zip((p.k.view(torch.uint8), p.v.view(torch.uint8), p.weight), was))
+    assert c.evict([1, 2, 3], [48, 48, 32], 48) == [48, 48, 32]
+    unchanged()
+    for bad in (dict(keep=0), dict(keep=16, recent=9, keep_first=8), dict(keep=16, recent=-1)):
+        with pytest.raises(ValueError):
+            c.evict([1], [48], **bad)
+        unchanged()
+    with pytest.raises(RuntimeError):
+        c.evict([1, 3], [48, 32], 31)                              # the first would get two blocks, the other ones two
+    unchanged()
+    assert c.evict([1, 3], [48, 32], 32, recent=32) == [32, 32]    # the second stays; the last 32 tokens of the first
+    assert c.block_table(3) == tables[2] and c.block_table(2) == tables[1] and not set(c.block_table(1)) & set(tables[1]) and c.thinned == {1}
+    for p, (k, v, w) in zip(c.pages, state):
+        for new, old in zip(c.block_table(1), tables[0][1:]):
+            assert torch.equal(p.weight[new], w[old])
+        for b in tables[1]:
+            assert torch.equal(p.weight[b], w[b]) and torch.equal(p.k.view(torch.uint8)[b], k[b]) and torch.equal(p.v.view(torch.uint8)[b], v[b])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("seed", range(3))
+def test_blocks_of_their_own_for_several_sequences_or_none(device, seed):
+    rng = random.Random(seed)
+    c = PagedCache(20, 4, num_layers=1, num_kv_heads=1, head_dim=8, dtype=torch.float32, device=device)
+    c.allocate(0, 40)
+    c.k.copy_(torch.arange(20.0).view(1, 20, 1, 1, 1).expand_as(c.k))
+    first = [float(c.k[0, b, 0, 0, 0]) for b in c.block_table(0)]
+    assert c.fork([0] * 4, [1, 2, 3, 4], [rng.randrange(4, 40, 4) for _ in range(4)])
+    refused = 0
+    for _ in range(40):
+        some = rng.sample(range(5), rng.randint(1, 4))
+        spans = []
+        for s in some:
+            room = 4 * len(c.block_table(s))
+            lo = rng.randrange(room)
+            spans.append((lo, rng.randint(0, min(room - lo, 9))))
+        before, free, shared = [c.block_table(s) for s in range(5)], c.free_blocks, c.shared_blocks
+        try:
+            c.own_all(some, [lo for lo, _ in spans], [n for _, n in spans])
+        except RuntimeError:
+            refused += 1
+            assert [c.block_table(s) for s in range(5)] == before and (c.free_blocks, c.shared_blocks) == (free, shared)
+            s = rng.randint(1, 4)                                  # room for the next ones
+            c.free(s)
+            assert c.fork([0], [s], [rng.randrange(4, 40, 4)])
+            continue
+        tables = [c.block_table(s) for s in range(5)]
+        for s, (lo, n) in zip(some, spans):
+            for i in range(lo // 4, (lo + n - 1) // 4 + 1 if n else 0):
+                assert sum(tables[s][i] in t for t in tables) == 1
+        assert all([float(c.k[0, b, 0, 0, 0]) for b in t] == first[:len(t)] for t in tables)
+        assert c.num_blocks - c.free_blocks == len(set().union(*map(set, tables)))
+    assert refused
+    with pytest.raises(IndexError):
+        c.own_all([0, 1, 77], [0, 0, 0], [1, 1, 1])
+    c.own_all([77], [0], [0])
