@@ -54,8 +54,10 @@ class BeamSearch:
         return ids
 
     def blocks_needed(self, prompt_lens: list, max_tokens: int) -> int:
-        """Blocks of the cache that a search over these prompts can take at most."""
+        """Blocks of the cache that a search over these prompts can take at most: a prompt's full blocks once and the others for every beam (where attention weights are summed: all)."""
         c = self.runner.cache
+        if self.runner.kv_weights:
+            return sum(self.beams * c.blocks_needed(n + max_tokens) for n in prompt_lens)
         return sum(n // c.block_size + self.beams * (c.blocks_needed(n + max_tokens) - n // c.block_size) for n in prompt_lens)
 
     @torch.no_grad()

@@ -302,8 +302,9 @@ class PagedCache:
 
     def fork(self, parents: list, children: list, num_tokens: list) -> bool:
         """New sequences children[i] that begin with the first num_tokens[i] cached tokens of sequences parents[i].  Full blocks are shared, a block that these tokens end in is
-        copied, and so is the recurrent state (which is the parent's now, whatever num_tokens).  A parent may have several children.  False (nothing changed) when out of blocks or
-        slots."""
+        copied, and so is the recurrent state (which is the parent's now, whatever num_tokens).  A parent may have several children.  Where attention weights are kept, children begin
+        with the parent's; a runner that sums them gives a decoded sequence blocks of its own for all of its tokens, so that such sequences share blocks until their first step.  False
+        (nothing changed) when out of blocks or slots."""
         if not len(parents) == len(children) == len(num_tokens) or len(set(children)) != len(children):
             raise InvalidArgument("PagedCache.fork: a parent and a number of tokens for every child, and no child twice")
         for p, c, n in zip(parents, children, num_tokens):

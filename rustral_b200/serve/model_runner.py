@@ -371,6 +371,14 @@ class ModelRunner:
             if p is not None and (p < 0 or (self.cfg.arch == "gpt2" and p + n > self.cfg.seq_len)):
                 raise ValueError(f"sequence {s}: no position {p if p < 0 else p + n - 1}")
 
+    def _own_blocks(self, chunks: list, dec_ids: list, dec_len: list) -> None:
+        """Blocks of their own for what the sequences of a step write: their new tokens, and where attention weights are summed the weights of all that a decoded row sees
+        (sequences that share a page would add to the same sums, in no order)."""
+        if self.cache.shared_blocks:
+            ones = [1] * len(dec_ids) if not self.kv_weights else dec_len
+            self.cache.own_all([c[0] for c in chunks] + list(dec_ids), [c[2] for c in chunks] + [n - m for n, m in zip(dec_len, ones)],
+                               [len(c[1]) for c in chunks] + list(ones))
+
     @torch.no_grad()
     def step_mixed(self, chunks: list, dec_ids: list, dec_tok: list, dec_len: list, positions: dict | None = None):
         """One model pass over several prompt chunks and the decode batch.
@@ -404,11 +412,7 @@ class ModelRunner:
             want.append([r1 - 1] if c[3] is True else [r0 + i for i in c[3]] if c[3] else [])
         rows = [r for w in want for r in w] + list(range(rd, T))
         every_row = rows == list(range(T))
-        if self.cache.shared_blocks:
-            for s_, tokens, start, _ in chunks:
-                self.cache.own(s_, start, len(tokens))
-            for s_, n in zip(dec_ids, dec_len):
-                self.cache.own(s_, n - 1, 1)
+        self._own_blocks(chunks, dec_ids, dec_len)
         # All inputs of the step in one page-locked block and one copy: a copy from other memory waits until the stream has come to it, and
         # the host then forms the step's launches while the GPU has nothing to do.  token ids, positions, slots; rows of the logits; slots of
         # the cached positions of later portions (their positions, not copied, at the end); block tables and lengths
@@ -518,9 +522,7 @@ class ModelRunner:
                 raise ValueError(f"groups of {groups.batch} sequences with a shared length each are needed for {len(seq_ids)} sequences")
             if self.cache.pages is not None or (dev.type == "cuda" and not beam_ops.shared_pays(groups, shared_lens, self._shared_row)):
                 groups = None
-        if self.cache.shared_blocks:
-            for s, n in zip(seq_ids, context_lens):
-                self.cache.own(s, n - 1, 1)
+        self._own_blocks([], seq_ids, context_lens)
         if self.use_graphs and dev.type == "cuda":
             return self._decode_graphed(seq_ids, last_tokens, context_lens, positions, groups, shared_lens)
         ids = torch.tensor(last_tokens, dtype=torch.int64, device=dev)

@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from rustral_b200 import ops
-from rustral_b200.serve import CacheQuantization, PagedCache
+from rustral_b200.models.config import preset
+from rustral_b200.serve import BeamSearch, CacheQuantization, ModelRunner, PagedCache
 from test_beams import attend64, bound
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -112,3 +113,58 @@ def test_blocks_of_their_own_for_several_sequences_or_none(device, seed):
     with pytest.raises(IndexError):
         c.own_all([0, 1, 77], [0, 0, 0], [1, 1, 1])
     c.own_all([77], [0], [0])
+
+
+# ---- attention weights of forked sequences -----------------------------------------------------------------------------------------------------
+def weighing_runner(device, blocks=64):
+    kw = dict(n_head=8, n_kv_head=2, d_model=512) if device == "cuda" else {}
+    return ModelRunner(preset("llama-test", **kw), device=device, num_blocks=blocks, block_size=16, seed=2, kv_quantization=CacheQuantization.FP8, kv_weights=True)
+
+
+def sums(r, seq, n):
+    """The weights of a sequence's first n tokens, [layers, KV heads, n]."""
+    table = r.cache.block_table(seq)
+    return torch.stack([torch.cat(list(p.weight[table].transpose(0, 1).flatten(1)[:, :n]), 0) for p in r.cache.pages]).cpu()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("mixed", [False, True])
+def test_forked_sequences_sum_weights_of_their_own(device, mixed):
+    """Parent and children decoded together sum what sequences that never shared a block sum: the same operations on the same numbers, bit for bit."""
+    prompt, more, last = list(range(3, 40)), list(range(60, 66)), [7, 300, 11, 500]
+    got = []
+    for forked in (False, True):
+        r = weighing_runner(device)
+        r.cache.allocate(1, 38)
+        r.prefill(1, prompt)
+        r.decode([1], [9], [38])
+        if forked:
+            assert r.cache.fork([1] * 3, [2, 3, 4], [38] * 3) and r.cache.shared_blocks == 2
+        else:
+            for s in (2, 3, 4):
+                r.cache.allocate(s, 38)
+                r.prefill(s, prompt)
+                r.decode([s], [9], [38])
+        for s in (1, 2, 3):
+            r.cache.allocate(s, 48)
+        for step in range(2):
+            n = [39 + step] * 3
+            if mixed:
+                r.cache.allocate(9, 8)
+                r.step_mixed([(9, more, 0, True)], [1, 2, 3], last[:3], n)
+            else:
+                r.decode([1, 2, 3], last[:3], n)
+        got.append([sums(r, s, 40 if s < 4 else 38) for s in (1, 2, 3, 4)])
+        assert r.cache.shared_blocks == 0 and r.cache.evict([1, 4], [40, 38], 20, recent=4) == [20, 20]
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+def test_beam_search_where_weights_are_kept():
+    r = weighing_runner("cpu", blocks=3 * 4)
+    plain = ModelRunner(preset("llama-test"), device="cpu", num_blocks=64, block_size=16, seed=2, kv_quantization=CacheQuantization.FP8)
+    prompt = list(range(20, 53))
+    with pytest.raises(ValueError, match="blocks"):
+        BeamSearch(r, 4).generate([prompt], 20)
+    found = BeamSearch(r, 3).generate([prompt], 20)[0]            # every block that there is
+    assert [h.tokens for h in found] == [h.tokens for h in BeamSearch(plain, 3).generate([prompt], 20)[0]] and r.cache.free_blocks == 12
