@@ -46,7 +46,7 @@ def _here(what: str, dev: int, *tensors) -> None:
 
 # ---- selection ---------------------------------------------------------------------------------------------------------------------------
 @functools.lru_cache(4096)
-def _select_bytes(*sizes) -> int:
+def _select_bytes(dev, *sizes) -> int:                               # (work is cut by the number of SMs of the device, which is the current one)
     return N.kernels().rb_beam_select_scratch_bytes(*sizes)
 
 
@@ -86,7 +86,7 @@ def beam_select(logits, scores, count: int, ended=None, end_token: int = 0):
     out_scores = scores.new_empty((groups, count))
     out_rows = scores.new_empty((groups, count), dtype=torch.int64)
     out_tokens = torch.empty_like(out_rows)
-    scratch = scores.new_empty(_select_bytes(groups, beams, vocab, count, kind), dtype=torch.uint8)
+    scratch = scores.new_empty(_select_bytes(dev, groups, beams, vocab, count, kind), dtype=torch.uint8)
     N.check(N.kernels().rb_beam_select(
         _SELECT.pack(logits.data_ptr(), scores.data_ptr(), 0 if ended is None else ended.data_ptr(), out_scores.data_ptr(), out_rows.data_ptr(), out_tokens.data_ptr(),
                      scratch.data_ptr(), pitch, groups, beams, vocab, count, kind, end_token), N.stream_ptr()), "rb_beam_select")
@@ -275,7 +275,7 @@ class PrefixGroups:
 
 
 @functools.lru_cache(4096)
-def _shared_bytes(*sizes) -> int:
+def _shared_bytes(dev, *sizes) -> int:                               # (as for _select_bytes)
     return N.kernels().rb_shared_prefix_scratch_bytes(*sizes)
 
 
@@ -342,7 +342,7 @@ def paged_attention_shared(q, k_cache, v_cache, groups: PrefixGroups, shared_len
     res = out
     if out is None or out.stride(1) != 1 or out.stride(0) & 7 or out.data_ptr() & 15:
         res = q.new_empty((batch, width))
-    scratch = q.new_empty(_shared_bytes(batch, n_groups, heads, hk, d, bs, groups.most), dtype=torch.uint8)
+    scratch = q.new_empty(_shared_bytes(dev, batch, n_groups, heads, hk, d, bs, groups.most), dtype=torch.uint8)
     N.check(N.kernels().rb_shared_prefix(
         _SHARED.pack(at, res.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), shared_lens.data_ptr(), groups.at[0], groups.at[1],
                      scratch.data_ptr(), pitch, res.stride(0), nb, batch, n_groups, table[1], bs, heads, hk, d, kind, groups.most, scale), N.stream_ptr()), "rb_shared_prefix")

@@ -107,7 +107,7 @@ def _ptr(t) -> int:
 
 
 @functools.lru_cache(4096)
-def _scratch_floats(*sizes) -> int:
+def _scratch_floats(dev, *sizes) -> int:                             # (work is cut by the number of SMs of the device, which is the current one)
     return N.kernels().rb_e4m3_decode_scratch_floats(*sizes)
 
 
@@ -294,7 +294,7 @@ def paged_attention_decode_e4m3(q, pages: PagesE4M3, block_tables, context_lens,
         q, ld_q = q.contiguous(), row
     if width == 0:
         return out.zero_()
-    floats = _scratch_floats(B, heads, G, D, width, bs, accumulate)
+    floats = _scratch_floats(pages.k.get_device(), B, heads, G, D, width, bs, accumulate)
     scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     a = _DECODE.pack(*_native(pages, shape), q.data_ptr(), out.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), _ptr(scratch),
                      ld_q, out.stride(0), B, width, heads, _TYPES[kind], accumulate, scale)

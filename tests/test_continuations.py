@@ -168,3 +168,30 @@ def test_beam_search_where_weights_are_kept():
         BeamSearch(r, 4).generate([prompt], 20)
     found = BeamSearch(r, 3).generate([prompt], 20)[0]            # every block that there is
     assert [h.tokens for h in found] == [h.tokens for h in BeamSearch(plain, 3).generate([prompt], 20)[0]] and r.cache.free_blocks == 12
+
+
+# ---- scratch -----------------------------------------------------------------------------------------------------------------------------------
+def test_scratch_is_sized_for_the_device_of_the_call(monkeypatch):
+    """Two devices with different numbers of SMs, in turn: how work is cut, and so the scratch, goes by them."""
+    from rustral_b200 import _native as N
+    from rustral_b200.ops import beams, paged_e4m3
+    now = []
+
+    class Kernels:
+        def rb_beam_select_scratch_bytes(self, groups, beams, vocab, count, kind):
+            return 1000 * now[-1] + groups
+
+        def rb_shared_prefix_scratch_bytes(self, batch, groups, heads, kv_heads, dim, bs, most):
+            return 2000 * now[-1] + batch
+
+        def rb_e4m3_decode_scratch_floats(self, batch, heads, kv_heads, dim, width, bs, accumulate):
+            return 3000 * now[-1] + batch
+    monkeypatch.setattr(N, "kernels", Kernels)
+    sizes = {0: 148, 1: 160}
+    for dev in (0, 1, 0, 1):
+        now.append(sizes[dev])
+        assert beams._select_bytes(dev, 7, 4, 1009, 8, 0) == 1000 * sizes[dev] + 7
+        assert beams._shared_bytes(dev, 9, 2, 4, 2, 64, 16, 5) == 2000 * sizes[dev] + 9
+        assert paged_e4m3._scratch_floats(dev, 11, 4, 2, 64, 33, 16, True) == 3000 * sizes[dev] + 11
+    for cached in (beams._select_bytes, beams._shared_bytes, paged_e4m3._scratch_floats):
+        cached.cache_clear()                                       # nothing of this stays
