@@ -295,6 +295,15 @@ class PagedCache:
         tensors, dim = self._block_tensors()
         copy_blocks_(tensors, src, dst, dim)
 
+    def _on_current_device(self) -> None:
+        """Raises what a copy of blocks would, before a table changes."""
+        held = [self.pages[0].k] if self.pages is not None else self.k if isinstance(self.k, list) else [self.k]
+        t = next((t for t in held if t is not None), None)
+        if t is None:
+            t = next((t for d in self.state for t in d.values()), None)
+        if t is not None and t.get_device() >= 0 and t.get_device() != torch._C._cuda_getDevice():
+            raise ValueError("PagedCache: the cache is not on the current device")
+
     @property
     def shared_blocks(self) -> int:
         """Blocks that are in more than one table."""
@@ -313,6 +322,7 @@ class PagedCache:
                 raise InvalidArgument(f"PagedCache.fork: no sequence {p} with blocks for {n} tokens")
             if self._lib.rb_ba_table_len(self._h, c) >= 0 or c in parents:
                 raise InvalidArgument(f"PagedCache.fork: sequence {c} is there already")
+        self._on_current_device()
         if sum(n % self.block_size != 0 for n in num_tokens) > self.free_blocks or (self.num_slots and len(children) > self.free_slots):
             return False
         src, dst, of, to = [], [], C.c_int32(), C.c_int32()
@@ -339,6 +349,7 @@ class PagedCache:
         wanted = [(s, f, c) for s, f, c in zip(seq_ids, first, n) if c > 0]
         if not wanted or not self.shared_blocks:
             return
+        self._on_current_device()
         bs = self.block_size
         room = min(sum((f + c - 1) // bs - f // bs + 1 for _, f, c in wanted), self.free_blocks)
         numbers = (C.c_int64 * (3 * len(wanted)))(*(x for column in zip(*wanted) for x in column))
@@ -355,6 +366,7 @@ class PagedCache:
     def compact(self) -> int:
         """Moves what is in use to the first blocks, num_blocks - free_blocks of them, and returns how many blocks moved.  Sequences keep their ids and tokens; block numbers that a program
         has read before (`block_table`, `slot`) are no longer theirs."""
+        self._on_current_device()
         src, dst = (C.c_int32 * self.num_blocks)(), (C.c_int32 * self.num_blocks)()
         k = self._lib.rb_ba_compact(self._h, C.addressof(src), C.addressof(dst))
         if k < 0:

@@ -7,7 +7,7 @@ import torch
 
 from rustral_b200 import ops
 from rustral_b200.models.config import preset
-from rustral_b200.serve import BeamSearch, CacheQuantization, ModelRunner, PagedCache
+from rustral_b200.serve import BeamSearch, CacheLayer, CacheQuantization, ModelRunner, PagedCache
 from test_beams import attend64, bound
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -113,6 +113,38 @@ def test_blocks_of_their_own_for_several_sequences_or_none(device, seed):
     with pytest.raises(IndexError):
         c.own_all([0, 1, 77], [0, 0, 0], [1, 1, 1])
     c.own_all([77], [0], [0])
+
+
+class Elsewhere:
+    """A tensor as one on the second of two devices looks to the host."""
+
+    def __init__(self, t):
+        self.t = t
+
+    def get_device(self):
+        return 1
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+@pytest.mark.parametrize("layers", [None, [CacheLayer(1, 8, 8)], [CacheLayer(state=(("z", (7,), None),))]])
+def test_a_cache_on_another_device_is_refused_before_tables_change(layers, monkeypatch):
+    c = PagedCache(6, 4, num_kv_heads=1, head_dim=8, dtype=torch.float32, layers=layers)
+    c.allocate(1, 8), c.allocate(2, 6)
+    assert c.fork([2], [3], [4])
+    c.free(1)
+    if layers is None:
+        c.k, c.v = Elsewhere(c.k), Elsewhere(c.v)
+    else:
+        c.k, c.v = ([Elsewhere(t) for t in ts] for ts in (c.k, c.v)) if layers[0].kv_heads else (c.k, c.v)
+        c.state = [{n: Elsewhere(t) for n, t in d.items()} for d in c.state]
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0)
+    tables, free = [c.block_table(s) for s in (2, 3)], c.free_blocks
+    for call in (lambda: c.fork([2], [4], [6]), lambda: c.own(3, 0, 4), lambda: c.own_all([2, 3], [0, 0], [6, 4]), c.compact):
+        with pytest.raises(ValueError, match="device"):
+            call()
+        assert [c.block_table(s) for s in (2, 3)] == tables and c.block_table(4) == [] and (c.free_blocks, c.shared_blocks) == (free, 1)
 
 
 # ---- attention weights of forked sequences -----------------------------------------------------------------------------------------------------
