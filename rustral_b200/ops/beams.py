@@ -189,6 +189,8 @@ def copy_blocks_(tensors, src, dst, dim: int = 0) -> None:
     differ).  src and dst are numbers on the host (lists or the like); the call refuses blocks that are not there, a destination twice, and a destination that is a source
     too, before it copies anything.  The tensors share no memory.  A CUDA graph keeps the numbers that it was captured with."""
     tensors = _listed("copy_blocks_", tensors)
+    if isinstance(src, (bytes, bytearray)) or isinstance(dst, (bytes, bytearray)):          # their bytes would be taken for those of the numbers
+        raise ValueError("copy_blocks_: src and dst are lists of block numbers")
     try:
         src, dst = array("i", src), array("i", dst)
     except (TypeError, OverflowError) as e:

@@ -202,6 +202,19 @@ def test_beam_search_where_weights_are_kept():
     assert [h.tokens for h in found] == [h.tokens for h in BeamSearch(plain, 3).generate([prompt], 20)[0]] and r.cache.free_blocks == 12
 
 
+# ---- moves -----------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("device", DEVICES)
+def test_blocks_are_numbers_not_bytes(device):
+    t = torch.arange(8.0, device=device).view(4, 2)
+    for bad in (bytes, bytearray):
+        for src, dst in ((bad(4), [1]), ([0], bad(b"\1\0\0\0")), (bad(4), bad(b"\1\0\0\0"))):
+            with pytest.raises(ValueError):
+                ops.copy_blocks_([t], src, dst)
+    assert t.flatten().tolist() == list(range(8))
+    ops.copy_blocks_([t], torch.tensor([0]), (1,))
+    assert t[1].tolist() == [0, 1]
+
+
 # ---- scratch -----------------------------------------------------------------------------------------------------------------------------------
 def test_scratch_is_sized_for_the_device_of_the_call(monkeypatch):
     """Two devices with different numbers of SMs, in turn: how work is cut, and so the scratch, goes by them."""
