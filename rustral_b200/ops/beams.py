@@ -115,14 +115,16 @@ def _select_cpu(logits, scores, count, ended, end_token):
 
 # ---- moves -----------------------------------------------------------------------------------------------------------------------------------
 def _row(what: str, t, dim: int) -> tuple:
-    """(rows, and how they lie in memory: outer stride, row stride, segment stride, segment bytes, outer, segments) of the rows of `t` along `dim`."""
+    """(rows, and how they lie in memory: outer stride, row stride, segment stride, segment bytes, outer, segments) of the rows of `t` along `dim`, the bytes from the
+    first to the last, and the same in runs (bytes of one, then (number, distance) from the widest distance down)."""
     shape, size = t.shape, t.element_size()
     if not 0 <= dim < len(shape):
         raise ValueError(f"{what}: a tensor of shape {tuple(shape)} has no rows along dimension {dim}")
     rows = shape[dim]
     if t.is_contiguous():
         row = math.prod(shape[dim + 1:]) * size
-        return rows, rows * row, row, 0, row, math.prod(shape[:dim]), 1
+        n = math.prod(shape[:dim])
+        return rows, (rows * row, row, 0, row, n, 1), n * rows * row, (n * rows * row, ())
     stride = t.stride()
 
     def merged(dims):
@@ -146,12 +148,67 @@ def _row(what: str, t, dim: int) -> tuple:
         raise ValueError(f"{what}: the rows of a tensor of shape {tuple(shape)} and strides {tuple(stride)} are not pieces at equal distances")
     n, far = outer[0] if outer else (1, 0)
     segs, apart = inner[0] if inner else (1, 0)
-    end = piece
+    end, runs = piece, []
     for length, apart_ in sorted([(n, far), (rows, stride[dim] if rows > 1 else 0), (segs, apart)], key=lambda x: x[1]):
+        if length > 1:
+            runs.insert(0, (length, apart_ * size))
         if length > 1 and apart_ < end:
             raise ValueError(f"{what}: the rows of a tensor of shape {tuple(shape)} and strides {tuple(stride)} share memory")
         end += max(length - 1, 0) * apart_
-    return rows, far * size, (stride[dim] if rows > 1 else 0) * size, apart * size, piece * size, n, segs
+    return rows, (far * size, (stride[dim] if rows > 1 else 0) * size, apart * size, piece * size, n, segs), end * size, (piece * size, tuple(runs))
+
+
+def _meet(gap: int, run: int, many: tuple, run2: int, many2: tuple, looks: list) -> bool:
+    """Whether two tensors share a byte, the second `gap` bytes behind the first: runs of `run` bytes, in turn repeated as `many` (number, distance) says from the widest down.
+    Only repetitions whose extents meet are looked at; more than `looks` of them count as meeting."""
+    far, far2 = (r + sum((n - 1) * s for n, s in m) for r, m in ((run, many), (run2, many2)))
+    if gap >= far or -gap >= far2:
+        return False
+    if not many and not many2:
+        return True
+    looks[0] -= 1
+    if looks[0] < 0:
+        return True
+    if many and many2 and many[0][1] == many2[0][1]:              # both go on at one distance: by the difference of the two numbers
+        (n, s), (n2, _) = many[0], many2[0]
+        near, near2 = far - (n - 1) * s, far2 - (n2 - 1) * s
+        return any(_meet(gap + k * s, run, many[1:], run2, many2[1:], looks) for k in range(max(1 - n, -((near2 + gap - 1) // s)), min(n2 - 1, (near - gap - 1) // s) + 1))
+    if not many or (many2 and many2[0][1] > many[0][1]):
+        return _meet(-gap, run2, many2, run, many, looks)
+    n, s = many[0]
+    near = far - (n - 1) * s
+    return any(_meet(gap - i * s, run, many[1:], run2, many2, looks) for i in range(max(0, -((near - gap - 1) // s)), min(n - 1, (gap + far2 - 1) // s) + 1))
+
+
+def _apart(what: str, spans: list) -> None:
+    """Refuses tensors that share memory.  spans: (first address, behind the last, runs) of each."""
+    spans.sort()
+    behind = 0
+    for at, end, _ in spans:
+        if at < behind:
+            break
+        behind = end
+    else:
+        return
+    together, behind = [], 0                                      # those whose extents meet
+    for span in spans:
+        if span[0] >= behind:
+            together.append([])
+        together[-1].append(span)
+        behind = max(behind, span[1])
+    for some in together:
+        wide = {many[0][1] if many else 0 for _, _, (_, many) in some}
+        if len(wide) == 1 and 0 not in wide:                      # parts of one tensor's rows, as a rule: their places within a row do not meet
+            s = wide.pop()
+            places = sorted((at % s, at % s + end - at - (many[0][0] - 1) * s) for at, end, (_, many) in some)
+            if all(a[1] <= b[0] for a, b in zip(places, places[1:])) and places[-1][1] <= places[0][0] + s:
+                continue
+        for i, (at, end, (run, many)) in enumerate(some):
+            for at2, _, (run2, many2) in some[i + 1:]:
+                if at2 >= end:
+                    break
+                if _meet(at2 - at, run, many, run2, many2, [4096]):
+                    raise ValueError(f"{what}: tensors that share memory")
 
 
 def _listed(what: str, tensors) -> tuple:
@@ -163,10 +220,10 @@ def _listed(what: str, tensors) -> tuple:
 def _rows(what: str, tensors, dim: int, index=None) -> tuple:
     """(device, rows, packed descriptions, how many) of the tensors of a call; those without elements are left out."""
     dev = rows = None
-    packed, seen = [], set() if index is None else {index.data_ptr()}
+    packed, spans = [], []
     for t in tensors:
         d = t.get_device()
-        n, *lies = _row(what, t, dim)
+        n, lies, extent, runs = _row(what, t, dim)
         if dev is None:
             dev, rows = d, n
         elif dev != d:
@@ -175,10 +232,12 @@ def _rows(what: str, tensors, dim: int, index=None) -> tuple:
             raise ValueError(f"{what}: tensors of {rows} and of {n} rows")
         if n and lies[3] and lies[4]:
             at = t.data_ptr()
-            if at in seen:
-                raise ValueError(f"{what}: tensors that share memory")
-            seen.add(at)
+            spans.append((at, at + extent, runs))
             packed.append(_MOVE.pack(at, *lies))
+    if index is not None:
+        at, size = index.data_ptr(), index.numel() * index.element_size()
+        spans.append((at, at + size, (size, ())))
+    _apart(what, spans)
     if dev is not None and dev >= 0 and dev != torch._C._cuda_getDevice():
         raise ValueError(f"{what}: the tensors are not on the current device")
     return dev, rows, b"".join(packed), len(packed)
@@ -187,7 +246,7 @@ def _rows(what: str, tensors, dim: int, index=None) -> tuple:
 def copy_blocks_(tensors, src, dst, dim: int = 0) -> None:
     """Copies blocks in place: t[dst[i]] <- t[src[i]] along dimension `dim` of every tensor (one number of blocks for all of them; other sizes, types and strides may
     differ).  src and dst are numbers on the host (lists or the like); the call refuses blocks that are not there, a destination twice, and a destination that is a source
-    too, before it copies anything.  The tensors share no memory.  A CUDA graph keeps the numbers that it was captured with."""
+    too, and tensors that share memory, before it copies anything.  A CUDA graph keeps the numbers that it was captured with."""
     tensors = _listed("copy_blocks_", tensors)
     if isinstance(src, (bytes, bytearray)) or isinstance(dst, (bytes, bytearray)):          # their bytes would be taken for those of the numbers
         raise ValueError("copy_blocks_: src and dst are lists of block numbers")
@@ -226,8 +285,8 @@ def _bits(t):
 def reorder_rows_(tensors, index, dim: int = 0, group: int | None = None) -> None:
     """Rows in a new order, in place: t[i] <- what t[index[i]] was, along dimension `dim` of every tensor (one number of rows for all; other sizes, types and strides
     may differ).  index: int64 [rows] on the tensors' device, any map.  `group`: rows come in groups of that many, as the beams of several prompts do, and indices stay
-    in their row's group (None: all rows are one); an index that does not leaves its row as it is.  On a GPU a group has up to 256 rows.  The tensors share no
-    memory, with the index neither."""
+    in their row's group (None: all rows are one); an index that does not leaves its row as it is.  On a GPU a group has up to 256 rows.  Tensors that share
+    memory, with the index too, are refused."""
     tensors = _listed("reorder_rows_", tensors)
     dev, rows, packed, count = _rows("reorder_rows_", tensors, dim, index)
     if rows is None:

@@ -215,6 +215,78 @@ def test_blocks_are_numbers_not_bytes(device):
     assert t[1].tolist() == [0, 1]
 
 
+def bytes_of(t, base):
+    """The addresses of a tensor's bytes, relative to `base`'s first."""
+    at = torch.arange(t.element_size())
+    for n, s in zip(t.shape, t.stride()):
+        at = (at[:, None] + torch.arange(n) * s * t.element_size()).flatten()
+    return (at + t.data_ptr() - base.data_ptr()).tolist()
+
+
+def cut(base, rng, rows):
+    """A view of `rows` rows (dimension 1) somewhere in a flat tensor, its rows pieces at equal distances."""
+    pitch = rng.choice((24, 24, 40, 48, 60))
+    piece, segs = rng.randint(1, 6), rng.randint(1, 3)
+    apart = rng.randint(piece, 12)
+    outer = rng.randint(1, 2)
+    first = rng.randrange(200)
+    return base.as_strided((outer, rows, segs, piece), (rows * pitch + rng.choice((0, 7)), pitch, apart, 1), first)
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_moves_refuse_tensors_that_share_memory_and_no_others(seed):
+    """Views of one tensor at random places, against the set of their bytes."""
+    rng, base = random.Random(seed), torch.arange(2000, dtype=torch.int32)
+    rows, met, index = 4, [0, 0], torch.tensor([1, 0, 3, 3])
+    for _ in range(250):
+        ts = [cut(base, rng, rows) for _ in range(rng.choice((2, 2, 3)))]
+        every = [b for t in ts for b in bytes_of(t, base)]
+        together = len(set(every)) < len(every)                   # two tensors, or two rows of one
+        met[together] += 1
+        was, want = base.clone(), base.clone()
+        if together:
+            with pytest.raises(ValueError):
+                ops.reorder_rows_(ts, index, dim=1)
+            with pytest.raises(ValueError):
+                ops.copy_blocks_(ts, [1], [0], dim=1)
+        else:
+            for t in ts:
+                v = want.as_strided(t.shape, t.stride(), t.storage_offset())
+                v.copy_(v[:, index].clone())
+            ops.reorder_rows_(ts, index, dim=1)
+        assert torch.equal(base, want)
+        base.copy_(was)
+    assert min(met) > 20
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_moves_of_parts_of_one_tensor(device):
+    """Overlapping parts are refused, keys and values of all layers in one tensor of blocks are not; an index in memory of theirs is."""
+    x = torch.arange(48.0, device=device).view(6, 8)
+    was, i = x.clone(), torch.tensor([1, 0, 3, 2], device=device)
+    for a, b in ((x[:4], x[2:]), (x[:4, :5], x[1:5, 4:]), (x[:4], x[1:5, 3:4]), (x[:4, ::4], x[:4, 4:])):
+        with pytest.raises(ValueError):
+            ops.reorder_rows_([a, b], i)
+        with pytest.raises(ValueError):
+            ops.copy_blocks_([a, b], [0], [3])
+    longs = torch.arange(20, device=device).view(4, 5)
+    with pytest.raises(ValueError):
+        ops.reorder_rows_([longs[:2]], longs.view(-1)[7:9])
+    with pytest.raises(ValueError):
+        ops.reorder_rows_([longs], longs[1, :4])
+    assert torch.equal(x, was) and longs.flatten().tolist() == list(range(20))
+    inside = torch.tensor([[7, 7, 1, 0], [8, 8, 9, 9]], device=device)               # the index between its rows' columns
+    ops.reorder_rows_([inside[:, :2]], inside[0, 2:])
+    assert inside.tolist() == [[8, 8, 1, 0], [7, 7, 9, 9]]
+    ops.reorder_rows_([x[:4, :4], x[:4, 4:]], i)
+    assert torch.equal(x, was[[1, 0, 3, 2, 4, 5]])
+    packed = torch.randn(5, 8, 2, 3, device=device)                # [blocks, layers, keys and values, ...]
+    want = packed.clone()
+    want[4] = want[1]
+    ops.copy_blocks_([packed[:, l, j] for l in range(8) for j in range(2)], [1], [4])
+    assert torch.equal(packed, want)
+
+
 # ---- scratch -----------------------------------------------------------------------------------------------------------------------------------
 def test_scratch_is_sized_for_the_device_of_the_call(monkeypatch):
     """Two devices with different numbers of SMs, in turn: how work is cut, and so the scratch, goes by them."""
