@@ -222,6 +222,8 @@ def _rows(what: str, tensors, dim: int, index=None) -> tuple:
     dev = rows = None
     packed, spans = [], []
     for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled() and (t.is_leaf or t._base is not None and t._base.is_leaf):
+            raise ValueError(f"{what}: a leaf that requires a gradient is not written in place")
         d = t.get_device()
         n, lies, extent, runs = _row(what, t, dim)
         if dev is None:
@@ -246,7 +248,7 @@ def _rows(what: str, tensors, dim: int, index=None) -> tuple:
 def copy_blocks_(tensors, src, dst, dim: int = 0) -> None:
     """Copies blocks in place: t[dst[i]] <- t[src[i]] along dimension `dim` of every tensor (one number of blocks for all of them; other sizes, types and strides may
     differ).  src and dst are numbers on the host (lists or the like); the call refuses blocks that are not there, a destination twice, and a destination that is a source
-    too, and tensors that share memory, before it copies anything.  A CUDA graph keeps the numbers that it was captured with."""
+    too, tensors that share memory, and (where gradients are recorded) leaves that require one, before it copies anything.  No gradient follows the rows.  A CUDA graph keeps the numbers that it was captured with."""
     tensors = _listed("copy_blocks_", tensors)
     if isinstance(src, (bytes, bytearray)) or isinstance(dst, (bytes, bytearray)):          # their bytes would be taken for those of the numbers
         raise ValueError("copy_blocks_: src and dst are lists of block numbers")
@@ -286,7 +288,7 @@ def reorder_rows_(tensors, index, dim: int = 0, group: int | None = None) -> Non
     """Rows in a new order, in place: t[i] <- what t[index[i]] was, along dimension `dim` of every tensor (one number of rows for all; other sizes, types and strides
     may differ).  index: int64 [rows] on the tensors' device, any map.  `group`: rows come in groups of that many, as the beams of several prompts do, and indices stay
     in their row's group (None: all rows are one); an index that does not leaves its row as it is.  On a GPU a group has up to 256 rows.  Tensors that share
-    memory, with the index too, are refused."""
+    memory, with the index too, are refused, and so are leaves that require a gradient where gradients are recorded; no gradient follows the rows."""
     tensors = _listed("reorder_rows_", tensors)
     dev, rows, packed, count = _rows("reorder_rows_", tensors, dim, index)
     if rows is None:

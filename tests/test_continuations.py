@@ -287,6 +287,26 @@ def test_moves_of_parts_of_one_tensor(device):
     assert torch.equal(packed, want)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_moves_refuse_leaves_that_require_a_gradient(device):
+    w, i = torch.nn.Parameter(torch.arange(12.0, device=device).view(4, 3)), torch.tensor([3, 2, 1, 0], device=device)
+    other = torch.zeros(4, 2, device=device)
+    for t in (w, w[:, 1:], w.view(4, 3, 1)):
+        with pytest.raises(ValueError):
+            ops.reorder_rows_([other, t], i)
+        with pytest.raises(ValueError):
+            ops.copy_blocks_([other, t], [0], [1])
+    assert w.flatten().tolist() == list(range(12))
+    with torch.no_grad():
+        ops.reorder_rows_([w], i)
+        ops.copy_blocks_([w[:, 1:]], [0], [1])
+    assert w.tolist() == [[9, 10, 11], [6, 10, 11], [3, 4, 5], [0, 1, 2]]
+    cache = torch.zeros(4, 3, device=device)                       # a dense cache that was filled where gradients are recorded
+    cache[:2] = w[:2] * 2
+    ops.reorder_rows_([cache], i)
+    assert cache.tolist() == [[0, 0, 0], [0, 0, 0], [12, 20, 22], [18, 20, 22]]
+
+
 # ---- scratch -----------------------------------------------------------------------------------------------------------------------------------
 def test_scratch_is_sized_for_the_device_of_the_call(monkeypatch):
     """Two devices with different numbers of SMs, in turn: how work is cut, and so the scratch, goes by them."""
