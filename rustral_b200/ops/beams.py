@@ -385,6 +385,8 @@ def paged_attention_shared(q, k_cache, v_cache, groups: PrefixGroups, shared_len
         raise TypeError("paged_attention_shared: contiguous int32 tables and lengths of every sequence and shared lengths of every group are required")
     if out is not None and (out.dtype is not dtype or out.shape != qs):
         raise TypeError("paged_attention_shared: out has the shape and type of q")
+    if out is not None and batch > 1 and out.stride(1) in (0, 1) and out.stride(0) < width:
+        raise ValueError("paged_attention_shared: the rows of out share memory")
     dev = q.get_device()
     _here("paged_attention_shared", dev, k_cache, v_cache, groups.group_of, shared_lens, block_tables, context_lens, out)
     scale = 1.0 / math.sqrt(d) if scale is None else scale
@@ -399,7 +401,7 @@ def paged_attention_shared(q, k_cache, v_cache, groups: PrefixGroups, shared_len
     if nb * bs > 2 ** 31 - 1 or table[1] * bs > 1 << 30:
         raise ValueError("paged_attention_shared: caches of fewer than 2^31 tokens and tables of up to 2^30 are served")
     at, (pitch, step) = q.data_ptr(), q.stride()
-    if step != 1 or pitch & 7 or at & 15:
+    if step != 1 or pitch < width or pitch & 7 or at & 15:           # (rows that overlap, as of an expanded one, are nothing that a tensor map describes)
         q = q.clone(memory_format=torch.contiguous_format)
         at, pitch = q.data_ptr(), width
     res = out

@@ -8,7 +8,7 @@ import torch
 from rustral_b200 import ops
 from rustral_b200.models.config import preset
 from rustral_b200.serve import BeamSearch, CacheLayer, CacheQuantization, ModelRunner, PagedCache
-from test_beams import attend64, bound
+from test_beams import attend64, bound, forked
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 I32 = torch.int32
@@ -36,6 +36,30 @@ def test_attention_shared_in_a_larger_cache_at_the_same_address(dim, more, cuda_
         place[pages] = torch.arange(len(pages))
         want, most = attend64(q, *held, place[t.long()], lens, 1.0 / math.sqrt(dim))
         assert ((got.cpu().double() - want).abs() <= bound(want, most, torch.bfloat16)).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [4, 40])
+def test_attention_shared_of_one_row_for_all_and_into_rows_apart(device, n):
+    """A query that is one row for every sequence; results into rows of a wider tensor, columns of a transposed one, and none whose rows share memory."""
+    sizes, shared, lens, dim = [n], [33], [34 + i % 9 for i in range(n)], 64
+    k, v, t = forked(sizes, shared, lens, 16, 2, dim, torch.bfloat16, n, hole=0.0)
+    q = torch.randn(1, 4 * dim, generator=torch.Generator().manual_seed(n)).bfloat16()
+    want, most = attend64(q.expand(n, -1), k, v, t, lens, 1.0 / math.sqrt(dim))
+    tensors = (k.to(device), v.to(device), ops.PrefixGroups(sizes, device), *(torch.tensor(x, dtype=I32, device=device) for x in (shared, t.tolist(), lens)))
+    limit = bound(want, most, torch.bfloat16)
+    whole = torch.zeros(n, 4 * dim + 8, dtype=torch.bfloat16, device=device)
+    columns = torch.zeros(4 * dim, n, dtype=torch.bfloat16, device=device)
+    apart = torch.zeros(n, 8 * dim, dtype=torch.bfloat16, device=device)
+    for out in (None, whole[:, 8:], whole[:, 5:-3], columns.t(), apart[:, ::2]):
+        got = ops.paged_attention_shared(q.to(device).expand(n, -1), *tensors, out=out)
+        assert ((got.cpu().double() - want).abs() <= limit).all() and (out is None or got is out)
+    assert not apart[:, 1::2].any()
+    flat = torch.zeros(n * 4 * dim, dtype=torch.bfloat16, device=device)
+    for out in (flat[:4 * dim].expand(n, -1), flat.as_strided((n, 4 * dim), (8, 1)), flat[:n].view(n, 1).expand(n, 4 * dim)):
+        with pytest.raises(ValueError):
+            ops.paged_attention_shared(q.to(device).expand(n, -1), *tensors, out=out)
+    assert not flat.any()
 
 
 # ---- shared blocks -----------------------------------------------------------------------------------------------------------------------------
