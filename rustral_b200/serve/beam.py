@@ -8,12 +8,15 @@ The reference decodes greedily, one sequence at a time (crates/nn/src/transforme
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 
 import torch
 
 from .. import ops
 from .model_runner import ModelRunner
+
+MOST_PENALTY = 600.0                                              # length ** length_penalty is a power of e between -600 and 600: a 64-bit number, like a sum over it
 
 
 @dataclass
@@ -44,7 +47,9 @@ class BeamSearch:
     def __init__(self, runner: ModelRunner, beams: int = 4, eos_id: int | None = None, length_penalty: float = 1.0, first_seq: int = 1 << 40):
         if not 1 <= beams <= ops.beams.MOST_COUNT // 2:
             raise ValueError(f"BeamSearch: 1 to {ops.beams.MOST_COUNT // 2} beams")
-        self.runner, self.beams, self.eos_id, self.length_penalty = runner, beams, eos_id, length_penalty
+        if not math.isfinite(length_penalty):
+            raise ValueError(f"BeamSearch: a length penalty of {length_penalty}")
+        self.runner, self.beams, self.eos_id, self.length_penalty = runner, beams, eos_id, float(length_penalty)
         self.vocab = runner.cfg.vocab_size
         self._next = first_seq
 
@@ -66,6 +71,8 @@ class BeamSearch:
         cache, cfg = self.runner.cache, self.runner.cfg
         if max_tokens < 1 or not all(len(p) for p in prompts):
             raise ValueError("BeamSearch: prompts of a token at least and max_tokens of at least 1")
+        if abs(self.length_penalty) * math.log(max_tokens) > MOST_PENALTY:
+            raise ValueError(f"BeamSearch: a length penalty of {self.length_penalty} for up to {max_tokens} tokens")
         for p in prompts:
             if len(p) + max_tokens > cfg.seq_len:
                 raise ValueError(f"prompt + max_tokens exceeds the model's context of {cfg.seq_len}")

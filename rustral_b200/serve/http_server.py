@@ -237,7 +237,10 @@ def engine_generate_fn(engine, loop: "EngineLoop | None" = None):
         max_tokens = int(body.get("max_tokens", 16))
         try:
             if "beams" in body:
-                search = dict(beams=int(body["beams"]), length_penalty=float(body.get("length_penalty", 1.0)))
+                try:
+                    search = dict(beams=int(body["beams"]), length_penalty=float(body.get("length_penalty", 1.0)))
+                except (TypeError, OverflowError):
+                    raise BadRequest("beams and length_penalty must be numbers") from None
                 found = loop.generate(prompt, max_tokens, search=search) if loop is not None else engine.beam_search(prompt, max_tokens, **search)
                 return {"tokens": found[0].tokens if found else [], "beams": [{"tokens": h.tokens, "score": h.score} for h in found]}
             if loop is not None:

@@ -356,3 +356,27 @@ def test_scratch_is_sized_for_the_device_of_the_call(monkeypatch):
         assert paged_e4m3._scratch_floats(dev, 11, 4, 2, 64, 33, 16, True) == 3000 * sizes[dev] + 11
     for cached in (beams._select_bytes, beams._shared_bytes, paged_e4m3._scratch_floats):
         cached.cache_clear()                                       # nothing of this stays
+
+
+# ---- the search ------------------------------------------------------------------------------------------------------------------------------------
+def test_length_penalties_that_are_no_powers_are_refused_first(monkeypatch):
+    """Before a prompt is computed; a server answers that the request is bad."""
+    from rustral_b200.serve import ServingEngine
+    from rustral_b200.serve.http_server import BadRequest, engine_generate_fn
+    r = ModelRunner(preset("gpt2-test"), device="cpu", num_blocks=32, block_size=4, seed=2)
+    want = {}
+    for alpha in (-30.0, -1, 0, 1, 60.0):
+        found = BeamSearch(r, 3, length_penalty=alpha).generate([[5, 6, 7]], 6)[0]
+        assert all(h.ranked == h.score / 6.0 ** alpha for h in found)
+        want[alpha] = [h.tokens for h in found]
+    assert len({str(w) for w in want.values()}) == 1               # all are six tokens long
+    monkeypatch.setattr(ModelRunner, "step_mixed", lambda *a, **k: 1 / 0)
+    for alpha in (math.nan, math.inf, -math.inf, 1e6, -1e6, 10 ** 6):
+        with pytest.raises(ValueError):
+            BeamSearch(r, 2, length_penalty=alpha).generate([[5, 6]], 5)
+    fn = engine_generate_fn(ServingEngine(r))
+    bad = [{"length_penalty": x} for x in (math.nan, 1e6, -1e6, "long", None, [1.0], 10 ** 400)] + [{"beams": x} for x in (None, [2], "two", math.inf, math.nan)]
+    for body in bad:
+        with pytest.raises(BadRequest):
+            fn({"prompt": [1, 2], "max_tokens": 5, "beams": 2, **body})
+    assert r.cache.free_blocks == 32
