@@ -1,6 +1,10 @@
 """Several continuations of one prompt where caches are large, tensors lie together, weights are kept and calls are refused (ops.beams, serve.PagedCache, serve.BeamSearch)."""
+import json
 import math
+import os
 import random
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -8,10 +12,47 @@ import torch
 from rustral_b200 import ops
 from rustral_b200.models.config import preset
 from rustral_b200.serve import BeamSearch, CacheLayer, CacheQuantization, ModelRunner, PagedCache
-from test_beams import attend64, bound, forked
+from test_beam_search import scores_are_their_tokens, sharp
+from test_beams import attend64, bound, choose, forked, same_choice
+from test_serving_e4m3 import Ranks
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 I32 = torch.int32
+
+
+@pytest.fixture
+def watched(request):
+    """On a GPU: fails the test where a wait of a kernel ran out."""
+    if request.node.callspec.params["device"] != "cpu":
+        request.getfixturevalue("cuda_status")
+
+
+# ---- selection -----------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 900), (torch.bfloat16, 1000), (torch.float32, 20000), (torch.bfloat16, 20001)])
+def test_beam_select_of_more_equal_candidates_than_a_list_holds(device, dtype, vocab, watched):
+    """Equal rows with 100 equal best tokens each: of 1600 equal candidates the first rows' first tokens, an ended beam's and dead beams' places between them."""
+    x = torch.linspace(-2.0, 1.0, vocab)[torch.randperm(vocab, generator=torch.Generator().manual_seed(vocab))]
+    x[torch.randperm(vocab, generator=torch.Generator().manual_seed(1))[:100]] = 3.0
+    x = x.to(dtype).expand(16, vocab).contiguous()
+    scores, ended = torch.full((1, 16), -2.5), torch.zeros(1, 16, dtype=torch.bool)
+    for count in (128, 101, 7):
+        same_choice(ops.beam_select(x.to(device), scores.to(device), count), choose(x, scores, count))
+    scores[0, 1], scores[0, 3], ended[0, 2], ended[0, 5] = -math.inf, math.nan, True, True
+    for count in (128, 120):
+        same_choice(ops.beam_select(x.to(device), scores.to(device), count, ended.to(device), 11), choose(x, scores, count, ended, 11))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_beam_select_of_many_rows_waits_for_its_copies(dtype, cuda_status):
+    """Rows that come by bulk copies, twice over them where there are infinities."""
+    x = torch.empty(600, 50008, device="cuda").normal_(0.0, 2.5, generator=torch.Generator(device="cuda").manual_seed(1)).to(dtype)
+    x[7, 123] = math.inf
+    x[300:304] = math.nan
+    scores = -torch.rand(150, 4, device="cuda")
+    got, want = ops.beam_select(x, scores, 8), ops.beam_select(x.cpu(), scores.cpu(), 8)
+    assert torch.equal(got[1].cpu(), want[1]) and torch.equal(got[2].cpu(), want[2])
 
 
 # ---- attention over a shared prefix ------------------------------------------------------------------------------------------------------------
@@ -60,6 +101,66 @@ def test_attention_shared_of_one_row_for_all_and_into_rows_apart(device, n):
         with pytest.raises(ValueError):
             ops.paged_attention_shared(q.to(device).expand(n, -1), *tensors, out=out)
     assert not flat.any()
+
+
+MORE = [
+    # group sizes, shared tokens, own tokens of every sequence, block size, KV heads, heads of each, head size, type, scale (None: as a rule)
+    ([30], [203], [1 + i for i in range(30)], 8, 2, 4, 64, torch.bfloat16, None),
+    ([7, 25], [64, 517], [3 * i for i in range(32)], 8, 1, 4, 128, torch.float16, None),
+    ([20], [500], [1 + 17 * i for i in range(20)], 384, 1, 4, 128, torch.bfloat16, None),
+    ([20, 3], [385, 900], [100] * 23, 384, 2, 2, 64, torch.float16, None),
+    ([20], [300], [1 + i for i in range(20)], 16, 2, 4, 64, torch.bfloat16, 0.0),
+    ([20], [300], [1 + i for i in range(20)], 16, 2, 4, 128, torch.bfloat16, -0.1),
+    ([3], [300], [1, 40, 200], 16, 2, 4, 64, torch.float16, 0.0),
+    ([3], [300], [1, 40, 200], 16, 2, 4, 128, torch.bfloat16, -0.1),
+    ([704], [200], [2] * 704, 16, 1, 1, 64, torch.bfloat16, None),
+    ([705], [200], [2] * 705, 16, 1, 1, 64, torch.bfloat16, None),
+]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("case", range(len(MORE)))
+def test_attention_shared_of_other_pages_and_scales(device, case, watched):
+    sizes, shared, mine, bs, kv, per, dim, dtype, scale = MORE[case]
+    owner = [i for i, n in enumerate(sizes) for _ in range(n)]
+    lens = [shared[g] + n for g, n in zip(owner, mine)]
+    k, v, t = forked(sizes, shared, lens, bs, kv, dim, dtype, 50 + case)
+    q = (torch.randn(len(lens), kv * per * dim, generator=torch.Generator().manual_seed(case)) * 2).to(dtype)
+    want, most = attend64(q, k, v, t, lens, 1.0 / math.sqrt(dim) if scale is None else scale)
+    got = ops.paged_attention_shared(*(x.to(device) for x in (q, k, v)), ops.PrefixGroups(sizes, device),
+                                     *(x.to(device) for x in (torch.tensor(shared, dtype=I32), t, torch.tensor(lens, dtype=I32))), scale=scale)
+    assert ((got.cpu().double() - want).abs() <= bound(want, most, dtype)).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n,bs,dim", [(4, 16, 64), (24, 16, 64), (24, 8, 128), (24, 128, 64), (24, 256, 128)])
+def test_attention_shared_of_tables_that_name_no_block(device, n, bs, dim, watched):
+    """Entries below zero and behind the last block count as block 0, of shared tokens and of a sequence's own."""
+    shared, lens = 3 * bs, [3 * bs + 1 + (7 * i) % (2 * bs) for i in range(n)]
+    k, v, t = forked([n], [shared], lens, bs, 1, dim, torch.bfloat16, n + bs, width=5, hole=0.5)
+    blocks, bad = k.shape[0], torch.tensor([-1, -1 << 31, k.shape[0], (1 << 31) - 1], dtype=I32)
+    t[0, 1], t[1, 3], t[2, 3:5], t[3, 3] = bad[0], bad[1], bad[2:4], bad[3]
+    clean = torch.where((t >= 0) & (t < blocks), t, 0)
+    clean[:, :3] = clean[0, :3]                                    # the first one's table is the group's
+    q = torch.randn(n, 4 * dim, generator=torch.Generator().manual_seed(n)).bfloat16()
+    want, most = attend64(q, k, v, clean, lens, 1.0 / math.sqrt(dim))
+    got = ops.paged_attention_shared(*(x.to(device) for x in (q, k, v)), ops.PrefixGroups([n], device),
+                                     *(x.to(device) for x in (torch.tensor([shared], dtype=I32), t, torch.tensor(lens, dtype=I32))))
+    assert ((got.cpu().double() - want).abs() <= bound(want, most, torch.bfloat16)).all()
+
+
+@pytest.mark.gpu
+def test_checking_build_reports_tables_that_name_no_block():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, RUSTRAL_BOUNDS="1", PYTHONPATH=root + os.pathsep + os.environ.get("PYTHONPATH", ""))
+    res = subprocess.run([sys.executable, os.path.join(root, "tests", "bounds_continuations_worker.py")], env=env, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, res.stdout[-2000:] + res.stderr[-2000:]
+    out = json.loads(res.stdout.strip().splitlines()[-1])
+    for name in ("few", "many"):
+        assert out.pop(name + "_ok") == [[0, 0, True]]
+        for kind in ("shared", "own"):
+            assert out.pop(f"{name}_{kind}") == [[8, 104, True]] * 4
+    assert not out
 
 
 # ---- shared blocks -----------------------------------------------------------------------------------------------------------------------------
@@ -380,3 +481,20 @@ def test_length_penalties_that_are_no_powers_are_refused_first(monkeypatch):
         with pytest.raises(BadRequest):
             fn({"prompt": [1, 2], "max_tokens": 5, "beams": 2, **body})
     assert r.cache.free_blocks == 32
+
+
+def test_two_ranks_search_alike():
+    """Two tensor-parallel ranks find the same continuations, and their scores are what the whole model gives these tokens."""
+    from concurrent.futures import ThreadPoolExecutor
+    from rustral_b200.serve.weights import InferenceWeights
+    cfg = preset("llama-test", seq_len=512, n_layer=2, d_model=256, n_head=4, ffn_dim=256, n_kv_head=2)
+    whole = sharp(ModelRunner(cfg, device="cpu", num_blocks=64, seed=3), 4)
+    ranks = Ranks(2)
+    shards = [ModelRunner(cfg, params=InferenceWeights.shard_of(whole.params, cfg, i, 2), device="cpu", num_blocks=64, tp=ranks.of(i)) for i in range(2)]
+    prompts = [[5, 300, 17, 44, 9], list(range(100, 140))]
+    with ThreadPoolExecutor(2) as pool:
+        got = list(pool.map(lambda r: BeamSearch(r, 3, eos_id=7).generate(prompts, 6), shards))
+    assert got[0] == got[1] and all(r.cache.free_blocks == 64 for r in shards)
+    for p, found in zip(prompts, got[0]):
+        assert len(found) == 3
+        scores_are_their_tokens(whole, p, found, 1e-3)
