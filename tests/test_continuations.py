@@ -55,6 +55,70 @@ def test_beam_select_of_many_rows_waits_for_its_copies(dtype, cuda_status):
     assert torch.equal(got[1].cpu(), want[1]) and torch.equal(got[2].cpu(), want[2])
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_beam_select_of_groups_without_a_live_beam(device, watched):
+    x = torch.randn(9, 50, generator=torch.Generator().manual_seed(3))
+    scores, ended = torch.full((3, 3), -math.inf), torch.zeros(3, 3, dtype=torch.bool)
+    scores[1], scores[2, 1] = torch.tensor([math.nan, -math.inf, -math.inf]), -4.0
+    ended[2, 1] = ended[0, 0] = True
+    for count in (1, 5, 120):
+        same_choice(ops.beam_select(x.to(device), scores.to(device), count, ended.to(device), 49), choose(x, scores, count, ended, 49))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,vocab,skip", [(torch.bfloat16, 9_000_001, 1), (torch.float32, 1 << 26, 0), (torch.float16, 5_000_000, 0)])
+def test_beam_select_of_long_rows(dtype, vocab, skip, cuda_status):
+    """One row in thousands of pieces.  Its sum of exponentials is checked by the definition on the host; see there for what a score may be off."""
+    x = torch.empty(1, vocab + 8, device="cuda").normal_(0.0, 2.5, generator=torch.Generator(device="cuda").manual_seed(1)).to(dtype)[:, skip:vocab + skip]
+    scores = torch.tensor([[-3.0]])
+    got = ops.beam_select(x, scores.cuda(), 128)
+    row = x[0].cpu().double()
+    row -= torch.logsumexp(row, 0) + 3.0
+    best = torch.topk(row, 1000)
+    order = sorted(zip((-best.values).tolist(), best.indices.tolist()))
+    last = order[127][0]                                           # all that are as good as the last one, in the order of their tokens
+    order = sorted([p for p in order if p[0] < last] + [(last, i) for i in (row == -last).nonzero()[:, 0].tolist()])[:128]
+    assert got[2].tolist() == [[i for _, i in order]] and got[1].tolist() == [[0] * 128]
+    want = -torch.tensor([p for p, _ in order], dtype=torch.float64)
+    assert ((got[0][0].cpu().double() - want).abs() <= 2.0 ** -17 + want.abs() * 2.0 ** -24).all()
+
+
+@pytest.mark.gpu
+def test_a_step_of_beams_captured_and_replayed(cuda_status):
+    """Selection and what the selected inherit in one graph, on a stream of its own, twice with other logits, beside the same on another stream."""
+    beams, vocab = 6, 3001
+    g = torch.Generator().manual_seed(9)
+    draws = [torch.randn(2 * beams, vocab, generator=g).bfloat16() for _ in range(3)]
+    held = torch.randn(2 * beams, 40, generator=g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    done = []
+    for stream in streams:
+        with torch.cuda.stream(stream):
+            x, s, h, c = draws[0].cuda(), torch.zeros(2, beams, device="cuda"), held.cuda(), torch.arange(30.0, device="cuda").view(10, 3)
+            best = ops.beam_select(x, s, beams)                    # kernels are set up before the capture
+            ops.reorder_rows_([h.clone()], best[1].view(-1), group=beams)
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                best = ops.beam_select(x, s, beams)
+                ops.reorder_rows_([h], best[1].view(-1), group=beams)
+                ops.copy_blocks_([c], [1, 2], [5, 7])
+            done.append((graph, x, h, c, best))
+    torch.cuda.synchronize()
+    for d in draws[1:]:
+        for stream, (graph, x, h, c, _) in zip(streams, done):
+            with torch.cuda.stream(stream):
+                x.copy_(d.cuda())
+                c[1] += 1
+                graph.replay()
+        torch.cuda.synchronize()
+        want = ops.beam_select(d, torch.zeros(2, beams), beams)
+        held = held[want[1].view(-1)]
+        for _, _, h, c, best in done:
+            assert torch.equal(best[1].cpu(), want[1]) and torch.equal(best[2].cpu(), want[2]) and torch.equal(h.cpu(), held)
+            assert torch.equal(c[5], c[1]) and torch.equal(c[7], c[2])
+
+
 # ---- attention over a shared prefix ------------------------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim,more", [(64, 1 << 20), (128, 1 << 21)])
@@ -161,6 +225,24 @@ def test_checking_build_reports_tables_that_name_no_block():
         for kind in ("shared", "own"):
             assert out.pop(f"{name}_{kind}") == [[8, 104, True]] * 4
     assert not out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 20])
+def test_attention_shared_past_four_gigabytes(n, cuda_status):
+    """Pages behind 2^31 numbers of a cache, shared ones and a sequence's own."""
+    bs, kv, per, dim, blocks = 16, 8, 4, 128, 140000
+    lens = [40 + i for i in range(n)]
+    small = forked([n], [32], lens, bs, kv, dim, torch.bfloat16, n, hole=0.0)
+    k, v = (torch.zeros(blocks, bs, kv, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    pages = blocks - 1 - torch.arange(small[0].shape[0])
+    k[pages.cuda()], v[pages.cuda()] = small[0].cuda(), small[1].cuda()
+    t = pages[small[2].clamp(max=len(pages) - 1).long()].to(I32)
+    q = torch.randn(n, kv * per * dim, generator=torch.Generator().manual_seed(n)).bfloat16()
+    want, most = attend64(q, small[0], small[1], small[2], lens, 1.0 / math.sqrt(dim))
+    got = ops.paged_attention_shared(q.cuda(), k, v, ops.PrefixGroups([n], "cuda"), torch.tensor([32], dtype=I32, device="cuda"), t.cuda(),
+                                     torch.tensor(lens, dtype=I32, device="cuda"))
+    assert ((got.cpu().double() - want).abs() <= bound(want, most, torch.bfloat16)).all()
 
 
 # ---- shared blocks -----------------------------------------------------------------------------------------------------------------------------
@@ -430,6 +512,19 @@ def test_moves_refuse_leaves_that_require_a_gradient(device):
     cache[:2] = w[:2] * 2
     ops.reorder_rows_([cache], i)
     assert cache.tolist() == [[0, 0, 0], [0, 0, 0], [12, 20, 22], [18, 20, 22]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 20])
+def test_reorder_rows_past_four_gigabytes(rows):
+    """Distances of rows and of copies that do not fit 32 bits."""
+    size = (1 << 32) // rows + 4096
+    t = torch.zeros(2, rows, size // 16 * 16, dtype=torch.uint8, device="cuda")
+    t[:, :, -5000::7] = torch.arange(1, 2 * rows + 1, dtype=torch.uint8, device="cuda").view(2, rows, 1)
+    index = torch.arange(rows, device="cuda").flip(0)
+    ops.reorder_rows_([t], index, dim=1)
+    want = torch.arange(1, 2 * rows + 1, dtype=torch.uint8, device="cuda").view(2, rows, 1).flip(1)
+    assert bool((t[:, :, -5000::7] == want).all()) and not t[:, :, -4999::7].any() and not t[:, :, :4096].any()
 
 
 # ---- scratch -----------------------------------------------------------------------------------------------------------------------------------
