@@ -182,16 +182,8 @@ def _meet(gap: int, run: int, many: tuple, run2: int, many2: tuple, looks: list)
 
 def _apart(what: str, spans: list) -> None:
     """Refuses tensors that share memory.  spans: (first address, behind the last, runs) of each."""
-    spans.sort()
-    behind = 0
-    for at, end, _ in spans:
-        if at < behind:
-            break
-        behind = end
-    else:
-        return
     together, behind = [], 0                                      # those whose extents meet
-    for span in spans:
+    for span in sorted(spans):
         if span[0] >= behind:
             together.append([])
         together[-1].append(span)
@@ -220,7 +212,7 @@ def _listed(what: str, tensors) -> tuple:
 def _rows(what: str, tensors, dim: int, index=None) -> tuple:
     """(device, rows, packed descriptions, how many) of the tensors of a call; those without elements are left out."""
     dev = rows = None
-    packed, spans = [], []
+    packed, spans, behind, ascending = [], [], 0, True            # (tensors made one after the other lie so, as a rule)
     for t in tensors:
         if t.requires_grad and torch.is_grad_enabled() and (t.is_leaf or t._base is not None and t._base.is_leaf):
             raise ValueError(f"{what}: a leaf that requires a gradient is not written in place")
@@ -234,12 +226,17 @@ def _rows(what: str, tensors, dim: int, index=None) -> tuple:
             raise ValueError(f"{what}: tensors of {rows} and of {n} rows")
         if n and lies[3] and lies[4]:
             at = t.data_ptr()
-            spans.append((at, at + extent, runs))
+            end = at + extent
+            ascending &= at >= behind
+            behind = end
+            spans.append((at, end, runs))
             packed.append(_MOVE.pack(at, *lies))
     if index is not None:
         at, size = index.data_ptr(), index.numel() * index.element_size()
+        ascending &= at >= behind or (bool(spans) and at + size <= spans[0][0])
         spans.append((at, at + size, (size, ())))
-    _apart(what, spans)
+    if not ascending:
+        _apart(what, spans)
     if dev is not None and dev >= 0 and dev != torch._C._cuda_getDevice():
         raise ValueError(f"{what}: the tensors are not on the current device")
     return dev, rows, b"".join(packed), len(packed)
