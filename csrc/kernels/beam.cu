@@ -236,8 +236,9 @@ __device__ __forceinline__ void bs_bulk(uint32_t dst, const void* src, uint32_t 
 // chunk of E under the chunk's largest number: the n best numbers lie in the n chunks whose largest are the best (of equal ones the first), and which of a chunk's they are is
 // looked up once, at the end.  So the pass over the logits is a maximum and an exponential per number, a barrier for four tiles and few chunks noted.
 //
-// 64 groups of 4 rows of 128256 numbers of 16 bits: 29 us with the group's launch, near the memory's rate between the CTAs' starts (first tile, its bound) and ends (lists), which all
-// have at the same times.  When they were tried, against 32: three stages of the ring 39, twice the pieces 35, lists of numbers in place of chunks 46.
+// 64 groups of 4 rows of 128256 numbers of 16 bits (65.7 MB): 29 us with the group's launch where the logits are in the L2, 36 with it flushed.  This kernel's part is 25 us and reads at
+// 2.6 TB/s: 512 CTAs start (first tile, its bound) and end (lists) at the same times, with nothing in flight, and two stages are few in between.  When they were tried, against 32: three
+// stages of the ring 39, twice the pieces 35, lists of numbers in place of chunks 46.
 // BULK: tiles come through the ring; else a piece is one tile, or rows do not begin on 16 bytes.
 template <typename T, int E, bool BULK>
 __global__ void __launch_bounds__(kBsThreads, 4)

@@ -162,7 +162,7 @@ struct Plan {
   bool tc;
 };
 // Groups with more than 16 rows go to the tcgen05 kernel, which takes 256 at a time where pages, batch and scale allow
-// (256 sequences with 4 rows each for 8 KV heads over 16384 shared tokens took 456 us with tiles of 32 rows on mma.sync, 122 now); else this file's has one m-tile, or two where rows need them.
+// (256 sequences with 4 rows each for 8 KV heads over 16384 shared tokens took 456 us with tiles of 32 rows on mma.sync, 124 now); else this file's has one m-tile, or two where rows need them.
 Plan plan_of(int batch, int groups, int heads, int kv_heads, int head_dim, int block_size, int most, bool positive) {
   Plan p;
   memset(&p, 0, sizeof(p));

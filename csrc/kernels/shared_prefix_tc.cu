@@ -13,7 +13,8 @@
 // token are set to zero, since a weight of zero times what they hold need not be zero.
 //
 // The sequences' own tokens are read in the same launch by CTAs of their own, three runs of four warps each (shared_prefix_split.cuh): one part of the GPU is bound by products and
-// exponentials while the other waits for memory.  One after the other they took 145 us, beside one another 133, 122 with all later steps (256 sequences with 4 rows each for 8 KV heads of 128, 16384 shared and 16 to 512 own
+// exponentials while the other waits for memory.  From a captured graph, one after the other they took 145 us, beside one another 133, 122 to 124 with all later steps, as calls among
+// others, where the clock is lower, 137 (256 sequences with 4 rows each for 8 KV heads of 128, 16384 shared and 16 to 512 own
 // tokens); 73.5, 71.7 and 72 for 12 groups of 8; 54.6, 50.8 and 49 for one document of 32771 tokens and 16 sequences.  Every CTA finds from the lengths how many CTAs each kind gets.
 //
 // Bound by the softmax's exponentials and the products where there are 256 rows, by the keys' and values' bytes where there are few.
@@ -29,10 +30,13 @@ namespace rb {
 constexpr int kStThreads = 384;          // warps 0-7 softmax, 8, 10 and 11 TMA, 9 MMA
 constexpr int kStTile = 128;
 constexpr float kStRescale = 8.f;        // log2 units
-constexpr int kStMostBatch = 704;        // their totals, tokens and spans beside 192 KB of tiles
+// Sequences whose totals, tokens and spans fit beside 192 KB of tiles.  One more and a batch has tiles of 32 rows on mma.sync: one group over 4000 shared and 100 own tokens, 32 heads
+// (8 KV) of 128, 704 sequences 137 us, 705 478.
+constexpr int kStMostBatch = 704;
 constexpr int kStRuns = 3;               // of a CTA that has sequences' own tokens
 // What a unit of 128 tokens takes a CTA, relative to one another: with two tiles of rows, with one, and of a sequence's own.  When they were set the first case above took 133 us
-// with 5 : 3 : 2, 146 with 6 : 3 : 2 and 143 with 4 : 3 : 2; the second 71.7, or 73.7 with 5 : 2 : 2 and 79 with 5 : 4 : 2.
+// with 5 : 3 : 2, 146 with 6 : 3 : 2 and 143 with 4 : 3 : 2; the second 71.7, or 73.7 with 5 : 2 : 2 and 79 with 5 : 4 : 2.  Both are bf16, 8 KV heads of 128 and pages of 16: other
+// shapes get the same shares, unmeasured.
 constexpr int kStTwo = 5, kStOne = 3, kStOwn = 2;
 
 __device__ __forceinline__ void st_ld32(uint32_t taddr, uint32_t* r) { tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r)); }
