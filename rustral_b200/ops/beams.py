@@ -182,8 +182,16 @@ def _meet(gap: int, run: int, many: tuple, run2: int, many2: tuple, looks: list)
 
 def _apart(what: str, spans: list) -> None:
     """Refuses tensors that share memory.  spans: (first address, behind the last, runs) of each."""
+    spans.sort()
+    behind = 0
+    for at, end, _ in spans:
+        if at < behind:
+            break
+        behind = end
+    else:
+        return
     together, behind = [], 0                                      # those whose extents meet
-    for span in sorted(spans):
+    for span in spans:
         if span[0] >= behind:
             together.append([])
         together[-1].append(span)
