@@ -1,6 +1,7 @@
 // Host-side services shared by all kernels of this library: the per-device status buffer, the
 // tensor-map cache and device queries.
 #include <mutex>
+#include <new>
 #include <string.h>
 #include <unordered_map>
 #include <vector>
@@ -44,7 +45,26 @@ struct KeyHash {
   }
 };
 std::mutex g_mu;
-std::unordered_map<Key, CUtensorMap*, KeyHash> g_cache;
+std::unordered_map<Key, CUtensorMap*, KeyHash> g_cache, g_set_aside;
+constexpr size_t kMostMaps = 65536;
+
+// Puts a map into the cache, which is bounded: a full one is set aside, and its maps are given up when the next one is full.  A caller may still hold maps of it: a product's second
+// operand may be the one that fills the cache, and another thread may copy a map that it was given.
+const CUtensorMap* keep(const Key& k, CUtensorMap* m, int* err) {
+  try {
+    if (g_cache.size() >= kMostMaps) {
+      for (auto& kv : g_set_aside) delete kv.second;
+      g_set_aside.clear();
+      g_set_aside.swap(g_cache);
+    }
+    g_cache.emplace(k, m);
+    return m;
+  } catch (...) {
+    delete m;
+    if (err) *err = -11;
+    return nullptr;
+  }
+}
 }  // namespace
 
 const CUtensorMap* get_tmap_2d(const void* base, int elem_bytes, uint64_t inner, uint64_t outer, uint64_t ld,
@@ -69,11 +89,8 @@ const CUtensorMap* get_tmap_2d(const void* base, int elem_bytes, uint64_t inner,
   }
   EncodeTiledFn fn = encode_fn();
   if (!fn) { if (err) *err = -10; return nullptr; }
-  if (g_cache.size() > 65536) {   // bound the cache; maps are cheap to rebuild
-    for (auto& kv : g_cache) delete kv.second;
-    g_cache.clear();
-  }
-  CUtensorMap* m = new CUtensorMap;
+  CUtensorMap* m = new (std::nothrow) CUtensorMap;
+  if (!m) { if (err) *err = -11; return nullptr; }
   cuuint64_t gdim[2] = {inner, outer};
   cuuint64_t gstride[1] = {ld * static_cast<uint64_t>(elem_bytes)};
   cuuint32_t box[2] = {box_inner, box_outer};
@@ -88,8 +105,7 @@ const CUtensorMap* get_tmap_2d(const void* base, int elem_bytes, uint64_t inner,
     if (err) *err = -100 - static_cast<int>(r);
     return nullptr;
   }
-  g_cache.emplace(k, m);
-  return m;
+  return keep(k, m, err);
 }
 
 // 4-D variant for [batch, seq, head, dim] views: dims / strides are given innermost first, strides in BYTES for
@@ -119,7 +135,8 @@ const CUtensorMap* get_tmap_4d(const void* base, int elem_bytes, const uint64_t 
   }
   EncodeTiledFn fn = encode_fn();
   if (!fn) { if (err) *err = -10; return nullptr; }
-  CUtensorMap* m = new CUtensorMap;
+  CUtensorMap* m = new (std::nothrow) CUtensorMap;
+  if (!m) { if (err) *err = -11; return nullptr; }
   cuuint64_t gdim[4] = {dims[0], dims[1], dims[2], dims[3]};
   cuuint64_t gstride[3] = {strides_bytes[0], strides_bytes[1], strides_bytes[2]};
   cuuint32_t bx[4] = {box[0], box[1], box[2], box[3]};
@@ -133,8 +150,7 @@ const CUtensorMap* get_tmap_4d(const void* base, int elem_bytes, const uint64_t 
     if (err) *err = -100 - static_cast<int>(r);
     return nullptr;
   }
-  g_cache.emplace(k, m);
-  return m;
+  return keep(k, m, err);
 }
 
 int device_sm_count() {

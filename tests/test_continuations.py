@@ -245,6 +245,24 @@ def test_attention_shared_past_four_gigabytes(n, cuda_status):
     assert ((got.cpu().double() - want).abs() <= bound(want, most, torch.bfloat16)).all()
 
 
+@pytest.mark.gpu
+def test_attention_shared_while_the_cache_of_tensor_maps_turns_over(cuda_status):
+    """More queries at addresses of their own than there is room for maps: each has the result of a copy of it at one address, bit for bit."""
+    n, dim, calls = 20, 64, 2 * 65536 + 2000
+    k, v, t = (x.cuda() for x in forked([n], [33], [40] * n, 16, 1, dim, torch.bfloat16, 5, hole=0.0))
+    plan, shared, lens = ops.PrefixGroups([n], "cuda"), torch.tensor([33], dtype=I32, device="cuda"), torch.full((n,), 40, dtype=I32, device="cuda")
+    base = torch.randn(n * dim + 8 * calls, generator=torch.Generator().manual_seed(6)).bfloat16().cuda()
+    out, again, copy = (torch.empty(n, dim, dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for i in range(calls):
+        q = base[8 * i:8 * i + n * dim].view(n, dim)
+        ops.paged_attention_shared(q, k, v, plan, shared, t, lens, out=out)
+        if i % 300 == 0 or i % 65536 < 20 or i % 65536 > 65480:
+            ops.paged_attention_shared(copy.copy_(q), k, v, plan, shared, t, lens, out=again)
+            differ += (out != again).sum()
+    assert int(differ) == 0
+
+
 # ---- shared blocks -----------------------------------------------------------------------------------------------------------------------------
 def weighed(blocks, device="cpu", bs=16):
     return PagedCache(blocks, bs, 2, 2, 64, device=device, quantization=CacheQuantization.FP8, attention_weights=True)
